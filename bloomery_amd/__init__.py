@@ -26,6 +26,7 @@ PATH_AUTO, PATH_PER_SLOT, PATH_GROUPED, PATH_GEMM = 0, 1, 2, 3
 ACT_SILU_MUL, ACT_SWIGLU_CLAMP, ACT_SWIGLU_OAI, ACT_SITU, ACT_SWIGLU_GCLAMP = 0, 1, 2, 3, 4
 SITE_F32_PRODUCT = 21
 HOST_SLOT = 0xFFFFFFFF
+F32, F16, BF16 = 0, 1, 30
 
 OK, ESHAPE, EDRIVER, ETYPE, EARG, EFAULT = 0, -1, -2, -3, -4, -5
 
@@ -98,6 +99,17 @@ SYMBOLS = {
     "bm_card_quantize": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp]),
     "bm_card_gemv": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp]),
     "bm_card_gemv_sel": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp]),
+    "bm_expert_sort_work": (_i64, [_i, _i]),
+    "bm_expert_sort": (_i, [_vp, _vp, _i, _i, _i, _vp, _i, _i64, _i, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "bm_expert_sort_grad": (_i, [_vp, _vp, _i, _i64, _vp, _i, _i, _i, _vp, _i64]),
+    "bm_expert_combine": (_i, [_vp, _vp, _i, _i64, _vp, _vp, _vp, _i64, _i, _i, _i, _vp, _i64]),
+    "bm_expert_combine_grad": (_i, [_vp, _vp, _i, _i64, _vp, _i64, _vp, _vp, _i, _i, _i, _vp, _i64, _vp]),
+    "bm_i8_row_bytes": (_i64, [_i]),
+    "bm_i8_quantize": (_i, [_vp, _vp, _i, _i64, _i, _i, _vp, _vp, _vp]),
+    "bm_i8_swiglu_quantize": (_i, [_vp, _vp, _vp, _i, _i64, _i, _i, _vp, _vp, _vp, _vp]),
+    "bm_i8_gemm": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _i, _i64]),
+    "bm_i8_gemm_x": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i, _i64, _i, _vp, _vp, _vp, _i, _i64]),
+    "bm_i8_gemm_experts": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _i, _i64]),
     "bm_gguf_open": (_i, [C.c_char_p, C.POINTER(_vp)]),
     "bm_gguf_open_split": (_i, [C.c_char_p, C.POINTER(_vp)]),
     "bm_gguf_close": (None, [_vp]),
@@ -158,6 +170,16 @@ def row_bytes(wtype, k):
 
 def col_bytes(wtype, k):
     return int(load_library().bm_col_bytes(wtype, k))
+
+
+def i8_row_bytes(k):
+    """Bytes of a row of 8-bit codes: k rounded up to 16."""
+    return int(load_library().bm_i8_row_bytes(k))
+
+
+def expert_sort_work(n_slots, n_experts):
+    """Words of scratch that enqueue_expert_sort takes."""
+    return int(load_library().bm_expert_sort_work(n_slots, n_experts))
 
 
 class DeviceBuffer:
@@ -370,6 +392,10 @@ def _ptr(x):
     return x  # a raw device address (e.g. torch.Tensor.data_ptr())
 
 
+def _line(ld, width):
+    return width if ld is None else ld
+
+
 class GateAct(C.Structure):
     """bm_gate_act: a gate . up launch's own rule and its limit (SiTU: the gate's beta)."""
     _fields_ = [("rule", C.c_int), ("limit", C.c_float)]
@@ -562,6 +588,53 @@ class Gpu:
     def enqueue_card_gemv_sel(self, w, codes, d8, s8, sel, n_slots, rows_per_expert, y):
         self._check(self.lib.bm_card_gemv_sel(self.ctx, w.handle, _ptr(codes), _ptr(d8), _ptr(s8), _ptr(sel), n_slots,
                                               rows_per_expert, _ptr(y)))
+
+    # -- experts in other forms: rows of F32, F16 or BF16 elements (lines in elements; None: rows back to back) sorted by expert and back
+    def enqueue_expert_sort(self, sel, n_tokens, top_k, n_experts, x, dtype, width, order, start, place, rows, work=None, ld_x=None,
+                            ld_rows=None):
+        """Tables of the picks and the tokens' rows at their slots' places (bm_expert_sort); x and rows None: the tables alone."""
+        self._check(self.lib.bm_expert_sort(self.ctx, _ptr(sel), n_tokens, top_k, n_experts, _ptr(x), dtype, _line(ld_x, width), width,
+                                            _ptr(order), _ptr(start), _ptr(place), _ptr(rows), _line(ld_rows, width), _ptr(work)))
+
+    def enqueue_expert_sort_grad(self, d_rows, dtype, place, n_tokens, top_k, width, dx, ld_rows=None, ld_dx=None):
+        self._check(self.lib.bm_expert_sort_grad(self.ctx, _ptr(d_rows), dtype, _line(ld_rows, width), _ptr(place), n_tokens, top_k, width,
+                                                 _ptr(dx), _line(ld_dx, width)))
+
+    def enqueue_expert_combine(self, rows, dtype, place, wts, resid, n_tokens, top_k, width, y, ld_rows=None, ld_resid=None, ld_y=None):
+        """The sorted rows back at their tokens: the slots' weighted sum onto the residual (None: no add)."""
+        self._check(self.lib.bm_expert_combine(self.ctx, _ptr(rows), dtype, _line(ld_rows, width), _ptr(place), _ptr(wts), _ptr(resid),
+                                               _line(ld_resid, width), n_tokens, top_k, width, _ptr(y), _line(ld_y, width)))
+
+    def enqueue_expert_combine_grad(self, dy, dtype, rows, place, wts, n_tokens, top_k, width, d_rows, d_wts, ld_dy=None, ld_rows=None,
+                                    ld_d_rows=None):
+        self._check(self.lib.bm_expert_combine_grad(self.ctx, _ptr(dy), dtype, _line(ld_dy, width), _ptr(rows), _line(ld_rows, width), _ptr(place),
+                                                    _ptr(wts), n_tokens, top_k, width, _ptr(d_rows), _line(ld_d_rows, width), _ptr(d_wts)))
+
+    # -- products in 8-bit integers: codes of i8_row_bytes(k) bytes a row and an f32 scale a row, on both sides
+    def enqueue_i8_quantize(self, x, dtype, m, k, codes, scales, ld_x=None, live=None):
+        """live: a device word; rows at or past its value keep what they held."""
+        self._check(self.lib.bm_i8_quantize(self.ctx, _ptr(x), dtype, _line(ld_x, k), m, k, _ptr(live), _ptr(codes), _ptr(scales)))
+
+    def enqueue_i8_swiglu_quantize(self, g, u, dtype, m, k, codes, scales, ld=None, live=None, rule=None):
+        self._check(self.lib.bm_i8_swiglu_quantize(self.ctx, _ptr(g), _ptr(u), dtype, _line(ld, k), m, k, _rule(rule), _ptr(live), _ptr(codes),
+                                                   _ptr(scales)))
+
+    def enqueue_i8_gemm(self, w, w_scales, rows, k, codes, scales, m, y, y_type, ld_y=None):
+        self._check(self.lib.bm_i8_gemm(self.ctx, _ptr(w), _ptr(w_scales), rows, k, _ptr(codes), _ptr(scales), m, _ptr(y), y_type,
+                                        _line(ld_y, rows)))
+
+    def enqueue_i8_gemm_x(self, w, w_scales, rows, k, x, x_type, m, codes, scales, y, y_type, ld_x=None, ld_y=None):
+        """enqueue_i8_quantize of the m rows of x and enqueue_i8_gemm in one call (the same bits)."""
+        self._check(self.lib.bm_i8_gemm_x(self.ctx, _ptr(w), _ptr(w_scales), rows, k, _ptr(x), x_type, _line(ld_x, k), m, _ptr(codes),
+                                          _ptr(scales), _ptr(y), y_type, _line(ld_y, rows)))
+
+    def enqueue_i8_gemm_experts(self, w, w_scales, n_experts, rows_per_expert, k, codes, scales, order, start, n_slots, top_k, y, y_type,
+                                ld_y=None, n_cols=None):
+        """top_k > 0: every slot of a token reads the token's column; 0: entry j reads column j."""
+        if n_cols is None:
+            n_cols = n_slots // top_k if top_k > 0 else n_slots
+        self._check(self.lib.bm_i8_gemm_experts(self.ctx, _ptr(w), _ptr(w_scales), n_experts, rows_per_expert, k, _ptr(codes), _ptr(scales),
+                                                n_cols, _ptr(order), _ptr(start), n_slots, top_k, _ptr(y), y_type, _line(ld_y, rows_per_expert)))
 
     # -- grouped decode: the slot table by expert and the tile launchers
     def tile_cap(self, n_slots, n_experts):

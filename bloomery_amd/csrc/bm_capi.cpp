@@ -77,7 +77,7 @@ static size_t dev_col_bytes(int wtype, int k) { return (size_t)bmk::act_col_byte
 
 extern "C" {
 
-int bm_version(void) { return 101; }
+int bm_version(void) { return 102; }
 
 int64_t bm_row_bytes(int wtype, int k) {
     if (!known_type(wtype)) return BM_ETYPE;
@@ -1405,6 +1405,230 @@ int bm_card_gemv_sel(bm_ctx *ctx, const bm_weights *w, const int8_t *codes_dev, 
     if (rc) return rc;
     return driver(ctx, what, bmk::card_gemv_sel(launch_of(ctx), w->wtype, w->dev, n_experts, w->k, codes_dev, d8_dev, s8_dev, sel_dev,
                                                 n_slots, rows_per_expert, y_dev));
+}
+
+// ------------------------------------------------------------------------------- rows by expert and 8-bit products
+
+// These entries look at their numbers before their context, so that what they refuse can be seen without a device.
+
+// The context's device for the launches of a call, whatever device the calling thread is on.
+struct DeviceScope {
+    int was = -1;
+    explicit DeviceScope(int device) {
+        if (hipGetDevice(&was) != hipSuccess || was == device || hipSetDevice(device) != hipSuccess) was = -1;
+    }
+    ~DeviceScope() {
+        if (was >= 0) (void)hipSetDevice(was);
+    }
+};
+
+static bool elem_type(int t) { return t == BM_F32 || t == BM_F16 || t == BM_BF16; }
+static int check_elem(bm_ctx *ctx, const char *what, int type) {
+    if (!elem_type(type)) return fail(ctx, BM_ETYPE, "%s: element type %d is not one of 0 f32, 1 f16, 30 bf16", what, type);
+    return BM_OK;
+}
+// A matrix of n rows of `width` elements, `ld` apart.
+static int check_rows(bm_ctx *ctx, const char *what, const char *name, const void *p, int type, int width, int64_t ld) {
+    const int eb = type == BM_F32 ? 4 : 2;
+    if (!p) return fail(ctx, BM_EARG, "%s: %s is NULL", what, name);
+    if (((uintptr_t)p & (eb - 1)) != 0) return fail(ctx, BM_ESHAPE, "%s: %s %p is not aligned to its %d-byte elements", what, name, p, eb);
+    if (ld < width || ld > (int64_t)1 << 40) return fail(ctx, BM_ESHAPE, "%s: %s rows of %d elements lie %lld apart", what, name, width, (long long)ld);
+    return BM_OK;
+}
+static int check_words(bm_ctx *ctx, const char *what, const char *name, const void *p) {
+    if (!p) return fail(ctx, BM_EARG, "%s: %s is NULL", what, name);
+    if (((uintptr_t)p & 3) != 0) return fail(ctx, BM_ESHAPE, "%s: %s %p is not 4-byte aligned", what, name, p);
+    return BM_OK;
+}
+static int check_tokens(bm_ctx *ctx, const char *what, int n_tokens, int top_k) {
+    if (n_tokens < 1 || top_k < 1 || top_k > bmk::kMaxCombineSlots || (int64_t)n_tokens * top_k > bmk::kTileMaxSlots)
+        return fail(ctx, BM_ESHAPE, "%s: %d tokens of %d slots (1 .. %d a token, at most %d in all)", what, n_tokens, top_k, bmk::kMaxCombineSlots,
+                    bmk::kTileMaxSlots);
+    return BM_OK;
+}
+static int check_width(bm_ctx *ctx, const char *what, int width) {
+    if (width < 1 || width > 1 << 24) return fail(ctx, BM_ESHAPE, "%s: rows of %d elements (1 .. 2^24)", what, width);
+    return BM_OK;
+}
+#define BM_TRY(call)                                                                                                                       \
+    do {                                                                                                                                   \
+        const int rc_ = (call);                                                                                                            \
+        if (rc_) return rc_;                                                                                                               \
+    } while (0)
+
+int64_t bm_expert_sort_work(int n_slots, int n_experts) {
+    if (n_slots < 1 || n_slots > bmk::kTileMaxSlots || n_experts < 1 || n_experts > bmk::kBucketExperts) return BM_ESHAPE;
+    return (int64_t)bmk::expert_sort_work(n_slots, n_experts);
+}
+
+int bm_expert_sort(bm_ctx *ctx, const uint32_t *sel_dev, int n_tokens, int top_k, int n_experts, const void *x_dev, int type, int64_t ld_x,
+                   int width, uint32_t *order_dev, uint32_t *start_dev, uint32_t *place_dev, void *rows_dev, int64_t ld_rows, uint32_t *work_dev) {
+    const char *what = "bm_expert_sort";
+    BM_TRY(check_tokens(ctx, what, n_tokens, top_k));
+    if (n_experts < 1 || n_experts > bmk::kBucketExperts) return fail(ctx, BM_ESHAPE, "%s: %d experts (1 .. %d)", what, n_experts, bmk::kBucketExperts);
+    BM_TRY(check_words(ctx, what, "sel_dev", sel_dev));
+    BM_TRY(check_words(ctx, what, "order_dev", order_dev));
+    BM_TRY(check_words(ctx, what, "start_dev", start_dev));
+    BM_TRY(check_words(ctx, what, "place_dev", place_dev));
+    if (bmk::expert_sort_work(n_tokens * top_k, n_experts) > 0) BM_TRY(check_words(ctx, what, "work_dev", work_dev));
+    if (x_dev || rows_dev) {
+        BM_TRY(check_elem(ctx, what, type));
+        BM_TRY(check_width(ctx, what, width));
+        BM_TRY(check_rows(ctx, what, "x_dev", x_dev, type, width, ld_x));
+        BM_TRY(check_rows(ctx, what, "rows_dev", rows_dev, type, width, ld_rows));
+    }
+    if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
+    DeviceScope on(ctx->device);
+    return driver(ctx, what, bmk::expert_sort(launch_of(ctx), sel_dev, n_tokens, top_k, n_experts, x_dev, type, ld_x, width, order_dev, start_dev,
+                                              place_dev, rows_dev, ld_rows, work_dev));
+}
+
+static int expert_sum(bm_ctx *ctx, const char *what, const char *from, const void *rows_dev, int type, int64_t ld_rows, const uint32_t *place_dev,
+                      const float *w_dev, const void *resid_dev, int64_t ld_resid, int n_tokens, int top_k, int width, const char *to, void *y_dev,
+                      int64_t ld_y) {
+    BM_TRY(check_tokens(ctx, what, n_tokens, top_k));
+    BM_TRY(check_elem(ctx, what, type));
+    BM_TRY(check_width(ctx, what, width));
+    BM_TRY(check_rows(ctx, what, from, rows_dev, type, width, ld_rows));
+    BM_TRY(check_words(ctx, what, "place_dev", place_dev));
+    if (resid_dev) BM_TRY(check_rows(ctx, what, "resid_dev", resid_dev, type, width, ld_resid));
+    BM_TRY(check_rows(ctx, what, to, y_dev, type, width, ld_y));
+    if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
+    DeviceScope on(ctx->device);
+    return driver(ctx, what, bmk::expert_combine(launch_of(ctx), rows_dev, type, ld_rows, place_dev, w_dev, resid_dev, ld_resid, n_tokens, top_k,
+                                                 width, y_dev, ld_y));
+}
+
+int bm_expert_sort_grad(bm_ctx *ctx, const void *d_rows_dev, int type, int64_t ld_rows, const uint32_t *place_dev, int n_tokens, int top_k,
+                        int width, void *dx_dev, int64_t ld_dx) {
+    return expert_sum(ctx, "bm_expert_sort_grad", "d_rows_dev", d_rows_dev, type, ld_rows, place_dev, nullptr, nullptr, 0, n_tokens, top_k, width,
+                      "dx_dev", dx_dev, ld_dx);
+}
+
+int bm_expert_combine(bm_ctx *ctx, const void *rows_dev, int type, int64_t ld_rows, const uint32_t *place_dev, const float *w_dev,
+                      const void *resid_dev, int64_t ld_resid, int n_tokens, int top_k, int width, void *y_dev, int64_t ld_y) {
+    BM_TRY(check_words(ctx, "bm_expert_combine", "w_dev", w_dev));
+    return expert_sum(ctx, "bm_expert_combine", "rows_dev", rows_dev, type, ld_rows, place_dev, w_dev, resid_dev, ld_resid, n_tokens, top_k, width,
+                      "y_dev", y_dev, ld_y);
+}
+
+int bm_expert_combine_grad(bm_ctx *ctx, const void *dy_dev, int type, int64_t ld_dy, const void *rows_dev, int64_t ld_rows,
+                           const uint32_t *place_dev, const float *w_dev, int n_tokens, int top_k, int width, void *d_rows_dev, int64_t ld_d_rows,
+                           float *d_w_dev) {
+    const char *what = "bm_expert_combine_grad";
+    BM_TRY(check_tokens(ctx, what, n_tokens, top_k));
+    BM_TRY(check_elem(ctx, what, type));
+    BM_TRY(check_width(ctx, what, width));
+    BM_TRY(check_rows(ctx, what, "dy_dev", dy_dev, type, width, ld_dy));
+    BM_TRY(check_rows(ctx, what, "rows_dev", rows_dev, type, width, ld_rows));
+    BM_TRY(check_words(ctx, what, "place_dev", place_dev));
+    BM_TRY(check_words(ctx, what, "w_dev", w_dev));
+    BM_TRY(check_rows(ctx, what, "d_rows_dev", d_rows_dev, type, width, ld_d_rows));
+    BM_TRY(check_words(ctx, what, "d_w_dev", d_w_dev));
+    if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
+    DeviceScope on(ctx->device);
+    return driver(ctx, what, bmk::expert_combine_grad(launch_of(ctx), dy_dev, type, ld_dy, rows_dev, ld_rows, place_dev, w_dev, n_tokens, top_k,
+                                                      width, d_rows_dev, ld_d_rows, d_w_dev));
+}
+
+int64_t bm_i8_row_bytes(int k) { return k < 1 || k > bmk::kI8MaxK ? (int64_t)BM_ESHAPE : (int64_t)bmk::i8_row_bytes(k); }
+
+constexpr int kI8MaxRows = 1 << 22;
+
+static int check_codes(bm_ctx *ctx, const char *what, const char *name, const void *codes, const char *scales_name, const void *scales) {
+    if (!codes) return fail(ctx, BM_EARG, "%s: %s is NULL", what, name);
+    if (((uintptr_t)codes & 15) != 0) return fail(ctx, BM_ESHAPE, "%s: %s %p must be 16-byte aligned", what, name, codes);
+    return check_words(ctx, what, scales_name, scales);
+}
+static int check_i8(bm_ctx *ctx, const char *what, int m, int k) {
+    if (m < 1 || m > kI8MaxRows) return fail(ctx, BM_ESHAPE, "%s: m = %d rows (1 .. %d)", what, m, kI8MaxRows);
+    if (k < 1 || k > bmk::kI8MaxK) return fail(ctx, BM_ESHAPE, "%s: rows of k = %d values (1 .. %d)", what, k, bmk::kI8MaxK);
+    return BM_OK;
+}
+
+static int i8_quant(bm_ctx *ctx, const char *what, const void *x_dev, const void *u_dev, bool glu, int type, int64_t ld, int m, int k,
+                    const bm_gate_act *rule, const uint32_t *live_dev, int8_t *codes_dev, float *scales_dev) {
+    BM_TRY(check_i8(ctx, what, m, k));
+    BM_TRY(check_elem(ctx, what, type));
+    BM_TRY(check_rows(ctx, what, glu ? "g_dev" : "x_dev", x_dev, type, k, ld));
+    if (glu) BM_TRY(check_rows(ctx, what, "u_dev", u_dev, type, k, ld));
+    if (((uintptr_t)live_dev & 3) != 0) return fail(ctx, BM_ESHAPE, "%s: live_dev %p is not 4-byte aligned", what, (const void *)live_dev);
+    BM_TRY(check_codes(ctx, what, "codes_dev", codes_dev, "scales_dev", scales_dev));
+    bmk::GateRule checked = {0u, 0.0f};
+    if (rule) BM_TRY(rule_checked(ctx, what, rule->rule, rule->limit, &checked));
+    if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
+    bmk::Launch L = launch_of(ctx);
+    if (rule) L.rule = checked;
+    DeviceScope on(ctx->device);
+    return driver(ctx, what, bmk::i8_quantize(L, x_dev, u_dev, type, ld, m, k, live_dev, codes_dev, scales_dev));
+}
+
+int bm_i8_quantize(bm_ctx *ctx, const void *x_dev, int type, int64_t ld_x, int m, int k, const uint32_t *live_dev, int8_t *codes_dev,
+                   float *scales_dev) {
+    return i8_quant(ctx, "bm_i8_quantize", x_dev, nullptr, false, type, ld_x, m, k, nullptr, live_dev, codes_dev, scales_dev);
+}
+
+int bm_i8_swiglu_quantize(bm_ctx *ctx, const void *g_dev, const void *u_dev, int type, int64_t ld, int m, int k, const bm_gate_act *rule,
+                          const uint32_t *live_dev, int8_t *codes_dev, float *scales_dev) {
+    return i8_quant(ctx, "bm_i8_swiglu_quantize", g_dev, u_dev, true, type, ld, m, k, rule, live_dev, codes_dev, scales_dev);
+}
+
+static int check_i8_weights(bm_ctx *ctx, const char *what, const int8_t *w_dev, const float *w_scales_dev, int rows, int k) {
+    if (rows < 1 || rows > kI8MaxRows) return fail(ctx, BM_ESHAPE, "%s: rows = %d of a matrix (1 .. %d)", what, rows, kI8MaxRows);
+    if (k < 1 || k > bmk::kI8MaxK) return fail(ctx, BM_ESHAPE, "%s: rows of k = %d values (1 .. %d)", what, k, bmk::kI8MaxK);
+    return check_codes(ctx, what, "w_dev", w_dev, "w_scales_dev", w_scales_dev);
+}
+
+int bm_i8_gemm(bm_ctx *ctx, const int8_t *w_dev, const float *w_scales_dev, int rows, int k, const int8_t *codes_dev, const float *scales_dev,
+               int m, void *y_dev, int y_type, int64_t ld_y) {
+    const char *what = "bm_i8_gemm";
+    BM_TRY(check_i8_weights(ctx, what, w_dev, w_scales_dev, rows, k));
+    BM_TRY(check_i8(ctx, what, m, k));
+    BM_TRY(check_codes(ctx, what, "codes_dev", codes_dev, "scales_dev", scales_dev));
+    BM_TRY(check_elem(ctx, what, y_type));
+    BM_TRY(check_rows(ctx, what, "y_dev", y_dev, y_type, rows, ld_y));
+    if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
+    DeviceScope on(ctx->device);
+    return driver(ctx, what, bmk::i8_gemm(launch_of(ctx), w_dev, w_scales_dev, 1, rows, k, codes_dev, scales_dev, m, nullptr, nullptr, 0, 0, y_dev,
+                                          y_type, ld_y));
+}
+
+int bm_i8_gemm_x(bm_ctx *ctx, const int8_t *w_dev, const float *w_scales_dev, int rows, int k, const void *x_dev, int x_type, int64_t ld_x, int m,
+                 int8_t *codes_dev, float *scales_dev, void *y_dev, int y_type, int64_t ld_y) {
+    const char *what = "bm_i8_gemm_x";
+    BM_TRY(check_i8_weights(ctx, what, w_dev, w_scales_dev, rows, k));
+    BM_TRY(check_i8(ctx, what, m, k));
+    BM_TRY(check_elem(ctx, what, x_type));
+    BM_TRY(check_rows(ctx, what, "x_dev", x_dev, x_type, k, ld_x));
+    BM_TRY(check_codes(ctx, what, "codes_dev", codes_dev, "scales_dev", scales_dev));
+    BM_TRY(check_elem(ctx, what, y_type));
+    BM_TRY(check_rows(ctx, what, "y_dev", y_dev, y_type, rows, ld_y));
+    if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
+    DeviceScope on(ctx->device);
+    const bmk::Launch L = launch_of(ctx);
+    BM_TRY(driver(ctx, what, bmk::i8_quantize(L, x_dev, nullptr, x_type, ld_x, m, k, nullptr, codes_dev, scales_dev)));
+    return driver(ctx, what, bmk::i8_gemm(L, w_dev, w_scales_dev, 1, rows, k, codes_dev, scales_dev, m, nullptr, nullptr, 0, 0, y_dev, y_type, ld_y));
+}
+
+int bm_i8_gemm_experts(bm_ctx *ctx, const int8_t *w_dev, const float *w_scales_dev, int n_experts, int rows_per_expert, int k,
+                       const int8_t *codes_dev, const float *scales_dev, int n_cols, const uint32_t *order_dev, const uint32_t *start_dev,
+                       int n_slots, int top_k, void *y_dev, int y_type, int64_t ld_y) {
+    const char *what = "bm_i8_gemm_experts";
+    BM_TRY(check_i8_weights(ctx, what, w_dev, w_scales_dev, rows_per_expert, k));
+    if (n_experts < 1 || n_experts > bmk::kBucketExperts) return fail(ctx, BM_ESHAPE, "%s: %d experts (1 .. %d)", what, n_experts, bmk::kBucketExperts);
+    if (n_slots < 1 || n_slots > bmk::kTileMaxSlots) return fail(ctx, BM_ESHAPE, "%s: %d slots (1 .. %d)", what, n_slots, bmk::kTileMaxSlots);
+    if (n_cols < 1 || n_cols > kI8MaxRows) return fail(ctx, BM_ESHAPE, "%s: %d columns (1 .. %d)", what, n_cols, kI8MaxRows);
+    if (top_k < 0) return fail(ctx, BM_ESHAPE, "%s: top_k = %d", what, top_k);
+    if (top_k == 0 && n_cols < n_slots) return fail(ctx, BM_ESHAPE, "%s: a column a slot, and %d columns for %d slots", what, n_cols, n_slots);
+    BM_TRY(check_codes(ctx, what, "codes_dev", codes_dev, "scales_dev", scales_dev));
+    if (top_k > 0) BM_TRY(check_words(ctx, what, "order_dev", order_dev));
+    BM_TRY(check_words(ctx, what, "start_dev", start_dev));
+    BM_TRY(check_elem(ctx, what, y_type));
+    BM_TRY(check_rows(ctx, what, "y_dev", y_dev, y_type, rows_per_expert, ld_y));
+    if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
+    DeviceScope on(ctx->device);
+    return driver(ctx, what, bmk::i8_gemm(launch_of(ctx), w_dev, w_scales_dev, n_experts, rows_per_expert, k, codes_dev, scales_dev, n_cols,
+                                          top_k > 0 ? order_dev : nullptr, start_dev, n_slots, top_k, y_dev, y_type, ld_y));
 }
 
 // ------------------------------------------------------------------------------------ graphs and events

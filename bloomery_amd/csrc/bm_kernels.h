@@ -196,6 +196,34 @@ hipError_t card_gemv(const Launch &L, int wtype, const uint8_t *w, long rows, in
 hipError_t card_gemv_sel(const Launch &L, int wtype, const uint8_t *w, int n_experts, int k, const int8_t *codes, const float *d8,
                          const int32_t *s8, const uint32_t *sel, int n_slots, int rows_per_expert, float *y);
 
+// ------------------------------------------------------- rows sorted by expert and back (bm_rows.hip)
+
+// et: an element type, ggml's numbers (0 f32, 1 f16, 30 bf16); lines in elements. At most kTileMaxSlots slots, kBucketExperts experts and
+// kMaxCombineSlots slots a token.
+// Slots that one launch sorts without `work`.
+constexpr uint32_t kSortFew = 2048;
+size_t expert_sort_work(int n_slots, int n_experts); // words
+// x and rows NULL: the tables alone
+hipError_t expert_sort(const Launch &L, const uint32_t *sel, int n_tokens, int top_k, int n_experts, const void *x, int et, int64_t ldx,
+                       int width, uint32_t *order, uint32_t *start, uint32_t *place, void *rows, int64_t ld_rows, uint32_t *work);
+// w NULL: ones (the gradient of the sort); resid NULL: none
+hipError_t expert_combine(const Launch &L, const void *rows, int et, int64_t ld_rows, const uint32_t *place, const float *w, const void *resid,
+                          int64_t ld_resid, int n_tokens, int top_k, int width, void *y, int64_t ld_y);
+hipError_t expert_combine_grad(const Launch &L, const void *dy, int et, int64_t ld_dy, const void *rows, int64_t ld_rows, const uint32_t *place,
+                               const float *w, int n_tokens, int top_k, int width, void *d_rows, int64_t ld_d_rows, float *d_w);
+
+// --------------------------------------------------------------------- products in 8-bit integers (bm_i8.hip)
+
+// The most values a row may hold: 127 * 128 * 131072 < 2^31.
+constexpr int kI8MaxK = 131072;
+inline int i8_row_bytes(int k) { return (k + 15) & ~15; }
+// u (optional): the rows are the launch's gate rule of x and u. live (optional): a device word, rows from there on keep what they hold.
+hipError_t i8_quantize(const Launch &L, const void *x, const void *u, int et, int64_t ld, int m, int k, const uint32_t *live, int8_t *codes,
+                       float *scales);
+// start NULL: one matrix against n_cols columns. Else entry j of expert e's run reads column order[j] / top_k, or j where top_k is 0.
+hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_experts, int rows, int k, const int8_t *q, const float *qs, int n_cols,
+                   const uint32_t *order, const uint32_t *start, int n_slots, int top_k, void *y, int et, int64_t ld);
+
 } // namespace bmk
 
 #endif // BM_KERNELS_H

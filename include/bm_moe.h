@@ -472,6 +472,77 @@ int bm_card_gemv(bm_ctx *ctx, const bm_weights *w, const int8_t *codes_dev, cons
 int bm_card_gemv_sel(bm_ctx *ctx, const bm_weights *w, const int8_t *codes_dev, const float *d8_dev, const int32_t *s8_dev,
                      const uint32_t *sel_dev, int n_slots, int rows_per_expert, float *y_dev);
 
+/* ------------------------------------------------------- experts in other forms: rows by expert and back */
+
+/* Element types of rows, numbered as ggml numbers them. */
+#define BM_F32 0
+#define BM_F16 1
+#define BM_BF16 30
+
+/* The entries of this section and the next take rows of f32, f16 or bf16 elements: row r begins ld elements behind row r - 1 (ld at
+ * least the row's width), pointers are aligned to the element, and nothing more is asked of either. Sums and products are
+ * formed in f32 and rounded once to the rows' type, to nearest even. Buffers of one call must not overlap. They have no
+ * counterpart in the reference, whose experts are GGUF blocks throughout: they serve experts that a program computes (or trains)
+ * by products of its own, with the picks and weights of bm_route_softmax / bm_norm_route. 1 .. 64 slots a token, at most 2^22
+ * slots and 1024 experts. */
+
+/* Tokens sorted by expert. sel_dev[n_tokens * top_k]: slot s belongs to token s / top_k. order_dev and start_dev become bm_buckets'
+ * tables, place_dev[s] the place of slot s in order (order's inverse; 0xffffffff for a slot that no run lists), and row place[s]
+ * of rows_dev token s / top_k's row of x_dev. An id at or past n_experts joins no run and, unless it is BM_HOST_SLOT, raises
+ * BM_SITE_EXPERT_ID. Entries of order_dev and rows of rows_dev behind the last listed one keep what they held. x_dev and rows_dev
+ * both NULL: the tables alone (type, width and the lines are not looked at). rows_dev: n_tokens * top_k rows.
+ * work_dev: bm_expert_sort_work(n_tokens * top_k, n_experts) words of scratch that holds nothing between calls (NULL where that is 0: a
+ * sort of up to 2048 slots is one launch, a longer one three). At most ceil(n_slots / 512) * n_experts words. */
+int64_t bm_expert_sort_work(int n_slots, int n_experts);
+int bm_expert_sort(bm_ctx *ctx, const uint32_t *sel_dev, int n_tokens, int top_k, int n_experts, const void *x_dev, int type, int64_t ld_x,
+                   int width, uint32_t *order_dev, uint32_t *start_dev, uint32_t *place_dev, void *rows_dev, int64_t ld_rows, uint32_t *work_dev);
+/* Its gradient: dx[t] = sum of d_rows[place[s]] over token t's listed slots, ascending. A token with none gets zeros. */
+int bm_expert_sort_grad(bm_ctx *ctx, const void *d_rows_dev, int type, int64_t ld_rows, const uint32_t *place_dev, int n_tokens, int top_k,
+                        int width, void *dx_dev, int64_t ld_dx);
+/* And back: y[t] = (acc = 0; for token t's listed slots s ascending: acc = fma(w[s], rows[place[s]], acc)) + resid[t], bm_combine_tokens'
+ * sum over sorted rows. A slot that is not listed adds nothing, whatever its weight. resid_dev may be NULL (no add). A place at
+ * or past n_tokens * top_k other than 0xffffffff raises BM_SITE_EXPERT_ID and adds nothing, here and in the gradients. */
+int bm_expert_combine(bm_ctx *ctx, const void *rows_dev, int type, int64_t ld_rows, const uint32_t *place_dev, const float *w_dev,
+                      const void *resid_dev, int64_t ld_resid, int n_tokens, int top_k, int width, void *y_dev, int64_t ld_y);
+/* Its gradients: d_rows[place[s]] = w[s] * dy[t] and d_w[s] = <dy[t], rows[place[s]]> (f32, each dot summed in one order whatever the
+ * launch; 0 for a slot that is not listed); resid's gradient is dy. Rows of d_rows_dev that no slot is placed at keep what they held. */
+int bm_expert_combine_grad(bm_ctx *ctx, const void *dy_dev, int type, int64_t ld_dy, const void *rows_dev, int64_t ld_rows,
+                           const uint32_t *place_dev, const float *w_dev, int n_tokens, int top_k, int width, void *d_rows_dev, int64_t ld_d_rows,
+                           float *d_w_dev);
+
+/* ----------------------------------------------------------------------------- products in 8-bit integers */
+
+/* Rows as 8-bit integers with a scale each - a token's activations, or a matrix's output channels: s = the f32 rounding of max |x| / 127,
+ * a code the real quotient x / s rounded to the nearest whole number, halves to even, held to +-127 (exactly: no code depends on how
+ * a quotient is rounded on the way). A row whose s is 0 has zero codes. A row of codes is bm_i8_row_bytes(k) = k rounded up to 16
+ * bytes, back to back, zeros behind the k-th; codes are 16-byte aligned. k is 1 .. 131072, so that a row's sum of products of a code
+ * and any byte fits 32 bits. A row holding a value that is not finite raises BM_SITE_QUANT_COLUMN and gets a NaN scale and zero codes. */
+int64_t bm_i8_row_bytes(int k);
+/* m rows (1 .. 2^22) of k elements. live_dev (optional): a device word; rows at or past its value keep what they held (of sorted rows:
+ * start_dev + n_experts). */
+int bm_i8_quantize(bm_ctx *ctx, const void *x_dev, int type, int64_t ld_x, int m, int k, const uint32_t *live_dev, int8_t *codes_dev,
+                   float *scales_dev);
+/* The same of the gate rule's values of two inputs (bm_swiglu_quant in this form; rule NULL: the context's), g_dev and u_dev rows both ld
+ * apart; the values are f32 on the way. */
+int bm_i8_swiglu_quantize(bm_ctx *ctx, const void *g_dev, const void *u_dev, int type, int64_t ld, int m, int k, const bm_gate_act *rule,
+                          const uint32_t *live_dev, int8_t *codes_dev, float *scales_dev);
+/* y[t * ld_y + r] = (f32(sum over k of codes[t] . w[r]) * scales[t]) * w_scales[r] for t < m, r < rows (1 .. 2^22 each): the sum in
+ * int32, exact, so the value does not depend on how the work is split. w_dev: rows of bm_i8_row_bytes(k) bytes; what they hold behind
+ * the k-th is not looked at (the codes' zeros meet it). */
+int bm_i8_gemm(bm_ctx *ctx, const int8_t *w_dev, const float *w_scales_dev, int rows, int k, const int8_t *codes_dev, const float *scales_dev,
+               int m, void *y_dev, int y_type, int64_t ld_y);
+/* bm_i8_quantize of x_dev's m rows and bm_i8_gemm in one call: the same bits in y_dev, codes_dev and scales_dev (caller-held, m rows). */
+int bm_i8_gemm_x(bm_ctx *ctx, const int8_t *w_dev, const float *w_scales_dev, int rows, int k, const void *x_dev, int x_type, int64_t ld_x, int m,
+                 int8_t *codes_dev, float *scales_dev, void *y_dev, int y_type, int64_t ld_y);
+/* The product over experts' runs (bm_buckets' or bm_expert_sort's tables of n_slots slots): entry j of start[e] .. start[e + 1] writes
+ * y[j * ld_y + r] = bm_i8_gemm's value of expert e's row r and column c(j); c(j) = order[j] / top_k, every slot of a token reading the
+ * token's column (bm_gemm's top_k), or j itself where top_k is 0 (order_dev is not read then and may be NULL). w_dev: n_experts x
+ * rows_per_expert rows. Rows of y_dev that no entry writes keep what they held. A run outside 0 .. n_slots raises
+ * BM_SITE_EXPERT_ID and is skipped; an entry whose slot or column (n_cols of them) does not exist raises it and gets NaN. */
+int bm_i8_gemm_experts(bm_ctx *ctx, const int8_t *w_dev, const float *w_scales_dev, int n_experts, int rows_per_expert, int k,
+                       const int8_t *codes_dev, const float *scales_dev, int n_cols, const uint32_t *order_dev, const uint32_t *start_dev,
+                       int n_slots, int top_k, void *y_dev, int y_type, int64_t ld_y);
+
 /* ------------------------------------------------------------------------------------------- model files */
 
 /* A GGUF file's header and a read-only mapping of it: the part of the reference's reader (crates/gguf/src/lib.rs:
