@@ -232,7 +232,6 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
         for (int r = 0; r < R; r++)
 #pragma unroll
             for (int c = 0; c < C; c++) acc[r][c] = v4i{0, 0, 0, 0};
-#pragma unroll 2
         for (u32 s = wave; s < steps; s += NW) {
             const u32 at = 64 * s + 16 * (lane >> 4);
             const bool in = at < a.kp; // a piece past the row: any of the row's bytes against zeros
@@ -277,13 +276,209 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
     }
 }
 
+// Many columns a matrix: BT columns x BR rows a workgroup, 128 bytes of k a step through LDS, where the loads put them themselves (16 bytes a
+// lane, no register in between): while the waves multiply one step the next is on its way into the other buffer, one barrier a step. A wave holds
+// (BT / WT) x (BR / WR) sums in v_mfma_i32_32x32x32_i8's form.
+// A step's rows are 128-byte lines of eight 16-byte pieces; piece c of line r lies at place c ^ swizzle(r), which the lane that asks for it
+// arranges, so that the pieces that the matrix instructions take of 32 lines at once come from all the banks.
+typedef int v16i __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(1))) void i8_gptr;
+typedef __attribute__((address_space(3))) void i8_lptr;
+
+__device__ const uint4 kI8Zeros = {0, 0, 0, 0};
+
+template <int BT, int BR, int WT, int WR>
+struct I8Tile {
+    static constexpr int kWaves = WT * WR, kThreads = 64 * kWaves, kLines = BT + BR, kStage = kLines * 128;
+    static constexpr int kRounds = kLines / 8 / kWaves; // loads a wave and step, eight lines each
+    static constexpr int TT = BT / WT / 32, TR = BR / WR / 32;
+    static_assert(kLines % (8 * kWaves) == 0 && BT % (32 * WT) == 0 && BR % (32 * WR) == 0, "whole waves");
+};
+
+__device__ __forceinline__ u32 i8_swizzle(u32 line) { return (line >> 1) & 7; }
+
+// The tile of workgroup b: an expert's run cut into tiles of BT entries, numbered through the experts in order. False: there is none.
+template <int BT>
+__device__ __forceinline__ bool i8_find_tile(const I8Args &a, u32 tile, u32 &expert, u32 &t0) {
+    const u32 lane = threadIdx.x & 63;
+    u32 before = 0;
+    for (u32 e0 = 0; e0 < a.n_experts; e0 += 64) {
+        const u32 e = e0 + lane;
+        u32 c = 0;
+        if (e < a.n_experts) {
+            const u32 j0 = a.start[e], j1 = a.start[e + 1];
+            if (j0 <= j1 && j1 <= a.n_slots) c = (j1 - j0 + BT - 1) / BT;
+            else if (tile == 0 && threadIdx.x < 64) bm_raise(a.fault, a.layer, kSiteExpertId);
+        }
+        u32 upto = c;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const u32 o = (u32)__shfl_up((int)upto, d, 64);
+            if (lane >= (u32)d) upto += o;
+        }
+        const unsigned long long mine = __ballot(c != 0 && before + upto - c <= tile && tile < before + upto);
+        if (mine) {
+            const int l = __builtin_ctzll(mine);
+            expert = e0 + (u32)l;
+            t0 = (tile - before - (u32)__shfl((int)(upto - c), l, 64)) * BT;
+            return true;
+        }
+        before += (u32)__shfl((int)upto, 63, 64);
+    }
+    return false;
+}
+
+// What a wave asked for has landed, and every wave is done with the buffer that is written next. (The wait as a builtin: the compiler counts
+// it, where behind one in asm it would wait for the loads that follow too.)
+__device__ __forceinline__ void i8_turn() {
+    __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070); // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __asm__ volatile("" ::: "memory");
+}
+
+// A wave's loads of a step: pieces past the end of the rows come from zeros.
+template <class G>
+__device__ __forceinline__ void i8_ask(const int8_t *(&src)[G::kRounds], uint8_t *buf, u32 wave, bool last, const bool (&past)[2]) {
+#pragma unroll
+    for (int r = 0; r < G::kRounds; r++) {
+        const int8_t *p = last && past[r & 1] ? reinterpret_cast<const int8_t *>(&kI8Zeros) : src[r];
+        __builtin_amdgcn_global_load_lds((i8_gptr *)p, (i8_lptr *)(buf + (wave * G::kRounds + r) * 1024), 16, 0, 0);
+        src[r] += 128;
+    }
+}
+
+// The next step is asked for and the present one multiplied. That the two buffers are apart is said by restrict: else the compiler waits for
+// the loads into one in front of every read of the other.
+template <class G>
+__device__ __forceinline__ void i8_step(const int8_t *(&src)[G::kRounds], const uint8_t *__restrict__ buf, uint8_t *__restrict__ next, u32 wave,
+                                        bool more, bool last, const bool (&past)[2], u32 wr, u32 wt, const u32 (&at)[4], v16i (&acc)[G::TR][G::TT]) {
+    if (more) i8_ask<G>(src, next, wave, last, past);
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        v4i A[G::TR], B[G::TT];
+#pragma unroll
+        for (int i = 0; i < G::TR; i++) A[i] = *reinterpret_cast<const v4i *>(buf + (wr + 32 * i) * 128 + at[c]);
+#pragma unroll
+        for (int j = 0; j < G::TT; j++) B[j] = *reinterpret_cast<const v4i *>(buf + (wt + 32 * j) * 128 + at[c]);
+#pragma unroll
+        for (int i = 0; i < G::TR; i++)
+#pragma unroll
+            for (int j = 0; j < G::TT; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(A[i], B[j], acc[i][j], 0, 0, 0);
+    }
+}
+
+// A wave's sums as values: column l % 32, rows 8 (x / 4) + 4 (l / 32) + x % 4 of a 32 x 32 tile.
+template <int ET, class G>
+__device__ __forceinline__ void i8_tile_out(const I8Args &a, const I8Run &run, u32 e0, u32 row0, const v16i (&acc)[G::TR][G::TT]) {
+    const u32 lane = threadIdx.x & 63;
+    row0 += 4 * (lane >> 5);
+#pragma unroll
+    for (int j = 0; j < G::TT; j++) {
+        const u32 e = e0 + 32 * j + (lane & 31);
+        if (e >= run.j1) continue;
+        bool bad;
+        const u32 col = i8_column(a, e, bad);
+        if (bad) bm_raise(a.fault, a.layer, kSiteExpertId);
+        const float sc = bad ? bm_bits_f32(0x7fc00000u) : a.qs[col];
+#pragma unroll
+        for (int i = 0; i < G::TR; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const u32 row = row0 + 32 * i + 8 * q;
+                if (row >= a.rows) continue;
+                float s[4], v[4];
+                elem_load_some<kElemF32, 4>(run.ws, row, a.rows - row, s);
+#pragma unroll
+                for (int x = 0; x < 4; x++) v[x] = __fmul_rn(__fmul_rn((float)acc[i][j][4 * q + x], sc), s[x]);
+                elem_store_some<ET, 4>(a.y, (size_t)e * a.ld + row, a.rows - row, v);
+            }
+    }
+}
+
+template <int BT, int BR, int WT, int WR>
+__global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_i8_tile(I8Args a, u32 n_row_tiles) {
+    using G = I8Tile<BT, BR, WT, WR>;
+    __shared__ __align__(16) uint8_t even[G::kStage];
+    __shared__ __align__(16) uint8_t odd[G::kStage];
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = (u32)__builtin_amdgcn_readfirstlane(tid >> 6);
+    u32 expert = 0, t0;
+    if (a.start) {
+        if (!i8_find_tile<BT>(a, blockIdx.x / n_row_tiles, expert, t0)) return;
+    } else {
+        t0 = (blockIdx.x / n_row_tiles) * BT;
+    }
+    const u32 r0 = (blockIdx.x % n_row_tiles) * BR;
+    I8Run run;
+    if (!i8_run(a, expert, run)) return;
+    t0 += run.j0;
+    const u32 steps = (a.kp + 127) / 128;
+
+    const int8_t *src[G::kRounds];
+    bool past[2];
+#pragma unroll
+    for (int r = 0; r < G::kRounds; r++) {
+        const u32 line = (wave * G::kRounds + r) * 8 + (lane >> 3), piece = (lane & 7) ^ i8_swizzle(line);
+        if (line < BT) {
+            const u32 j = t0 + line;
+            bool bad;
+            src[r] = a.q + (size_t)i8_column(a, j < run.j1 ? j : run.j1 - 1, bad) * a.kp + 16 * piece;
+        } else {
+            const u32 row = r0 + line - BT;
+            src[r] = run.w + (size_t)(row < a.rows ? row : a.rows - 1) * a.kp + 16 * piece;
+        }
+        // (the place of a piece differs between even and odd rounds only)
+        if (r < 2) past[r] = (steps - 1) * 128 + 16 * piece >= a.kp;
+    }
+    static_assert(G::kRounds >= 2 && G::kRounds % 2 == 0, "even and odd rounds");
+    v16i acc[G::TR][G::TT];
+#pragma unroll
+    for (int i = 0; i < G::TR; i++)
+#pragma unroll
+        for (int j = 0; j < G::TT; j++)
+#pragma unroll
+            for (int x = 0; x < 16; x++) acc[i][j][x] = 0;
+    const u32 wt = (wave % WT) * (BT / WT), wr = BT + (wave / WT) * (BR / WR); // this wave's first lines
+    u32 at[4];
+#pragma unroll
+    for (u32 c = 0; c < 4; c++) at[c] = (lane & 31) * 128 + 16 * ((2 * c + (lane >> 5)) ^ i8_swizzle(lane & 31));
+    i8_ask<G>(src, even, wave, steps == 1, past);
+    for (u32 s = 0;;) {
+        i8_turn();
+        i8_step<G>(src, even, odd, wave, s + 1 < steps, s + 2 == steps, past, wr, wt, at, acc);
+        if (++s == steps) break;
+        i8_turn();
+        i8_step<G>(src, odd, even, wave, s + 1 < steps, s + 2 == steps, past, wr, wt, at, acc);
+        if (++s == steps) break;
+    }
+    if (a.et == kElemF32) i8_tile_out<kElemF32, G>(a, run, t0 + wt, r0 + (wr - BT), acc);
+    else if (a.et == kElemF16) i8_tile_out<kElemF16, G>(a, run, t0 + wt, r0 + (wr - BT), acc);
+    else i8_tile_out<kElemBF16, G>(a, run, t0 + wt, r0 + (wr - BT), acc);
+}
+
+template <int BT, int BR, int WT, int WR>
+static void tile_launch(const Launch &L, const I8Args &a, u32 entries) {
+    const u32 row_tiles = (a.rows + BR - 1) / BR;
+    u32 tiles = (entries + BT - 1) / BT;
+    if (a.start) tiles = entries / BT + (a.n_experts < entries ? a.n_experts : entries); // at most a ragged tile an expert
+    hipLaunchKernelGGL((k_i8_tile<BT, BR, WT, WR>), dim3(tiles * row_tiles), dim3(64 * WT * WR), 0, L.stream, a, row_tiles);
+}
+
+template <int C>
+static void few_launch(const Launch &L, const I8Args &a, u32 entries) {
+    const u32 z = a.start ? 1u : (entries + 16 * C - 1) / (16 * C);
+    hipLaunchKernelGGL((k_i8_few<1, C, 8>), dim3((a.rows + 15) / 16, a.start ? a.n_experts : 1u, z < 65535u ? z : 65535u), dim3(512), 0, L.stream, a);
+}
+
 hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_experts, int rows, int k, const int8_t *q, const float *qs, int n_cols,
                    const uint32_t *order, const uint32_t *start, int n_slots, int top_k, void *y, int et, int64_t ld) {
     const I8Args a = {w, ws, (u32)rows, (u32)i8_row_bytes(k), q, qs, (u32)n_cols, order, start, (u32)n_slots, (u32)top_k, (u32)n_cols, (u32)n_experts,
                       y, (size_t)ld, et, L.fault, L.layer};
-    const u32 entries = start ? (u32)n_slots : (u32)n_cols;
-    const u32 z = start ? 1u : (entries + 31) / 32;
-    hipLaunchKernelGGL((k_i8_few<1, 2, 8>), dim3(((u32)rows + 15) / 16, start ? (u32)n_experts : 1u, z < 65535u ? z : 65535u), dim3(512), 0, L.stream, a);
+    const u32 entries = start ? (u32)n_slots : (u32)n_cols, each = entries / (u32)n_experts;
+    if (each >= 512 && rows >= 512) tile_launch<256, 256, 4, 2>(L, a, entries);
+    else if (each >= 24 && rows >= 64) tile_launch<128, 128, 2, 2>(L, a, entries);
+    else if (each > 16 || start) few_launch<2>(L, a, entries);
+    else few_launch<1>(L, a, entries);
     return hipGetLastError();
 }
 
