@@ -285,14 +285,12 @@ typedef int v16i __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(1))) void i8_gptr;
 typedef __attribute__((address_space(3))) void i8_lptr;
 
-__device__ const uint4 kI8Zeros = {0, 0, 0, 0};
-
 template <int BT, int BR, int WT, int WR>
 struct I8Tile {
-    static constexpr int kWaves = WT * WR, kThreads = 64 * kWaves, kLines = BT + BR, kStage = kLines * 128;
-    static constexpr int kRounds = kLines / 8 / kWaves; // loads a wave and step, eight lines each
+    static constexpr int kColumns = BT, kRows = BR, kWaves = WT * WR, kThreads = 64 * kWaves, kStage = (BT + BR) * 128;
+    static constexpr int RT = BT / 8 / kWaves, RR = BR / 8 / kWaves; // a wave's loads a step, eight lines each, of columns and of rows
     static constexpr int TT = BT / WT / 32, TR = BR / WR / 32;
-    static_assert(kLines % (8 * kWaves) == 0 && BT % (32 * WT) == 0 && BR % (32 * WR) == 0, "whole waves");
+    static_assert(BT % (16 * kWaves) == 0 && BR % (16 * kWaves) == 0 && BT % (32 * WT) == 0 && BR % (32 * WR) == 0, "whole waves, even rounds");
 };
 
 __device__ __forceinline__ u32 i8_swizzle(u32 line) { return (line >> 1) & 7; }
@@ -319,8 +317,8 @@ __device__ __forceinline__ bool i8_find_tile(const I8Args &a, u32 tile, u32 &exp
         const unsigned long long mine = __ballot(c != 0 && before + upto - c <= tile && tile < before + upto);
         if (mine) {
             const int l = __builtin_ctzll(mine);
-            expert = e0 + (u32)l;
-            t0 = (tile - before - (u32)__shfl((int)(upto - c), l, 64)) * BT;
+            expert = (u32)__builtin_amdgcn_readfirstlane((int)(e0 + (u32)l));
+            t0 = (u32)__builtin_amdgcn_readfirstlane((int)((tile - before - (u32)__shfl((int)(upto - c), l, 64)) * BT));
             return true;
         }
         before += (u32)__shfl((int)upto, 63, 64);
@@ -337,35 +335,91 @@ __device__ __forceinline__ void i8_turn() {
     __asm__ volatile("" ::: "memory");
 }
 
-// A wave's loads of a step: pieces past the end of the rows come from zeros.
+// Where a lane's loads begin: offsets of its lines' pieces from the tile's first column and row, and how far each goes back in the last step
+// where the rows end before the piece does (to the line's first piece, which is there; the columns' are zeroed in LDS).
 template <class G>
-__device__ __forceinline__ void i8_ask(const int8_t *(&src)[G::kRounds], uint8_t *buf, u32 wave, bool last, const bool (&past)[2]) {
+struct I8Src {
+    const int8_t *q, *w; // this step's
+    u32 col[G::RT], row[G::RR], back[2];
+};
+template <class G>
+__device__ __forceinline__ void i8_ask(I8Src<G> &s, uint8_t *buf, u32 wave, bool last) {
 #pragma unroll
-    for (int r = 0; r < G::kRounds; r++) {
-        const int8_t *p = last && past[r & 1] ? reinterpret_cast<const int8_t *>(&kI8Zeros) : src[r];
-        __builtin_amdgcn_global_load_lds((i8_gptr *)p, (i8_lptr *)(buf + (wave * G::kRounds + r) * 1024), 16, 0, 0);
-        src[r] += 128;
+    for (int r = 0; r < G::RT; r++)
+        __builtin_amdgcn_global_load_lds((i8_gptr *)(s.q + (s.col[r] - (last ? s.back[r & 1] : 0u))), (i8_lptr *)(buf + (wave * G::RT + r) * 1024), 16, 0, 0);
+#pragma unroll
+    for (int r = 0; r < G::RR; r++)
+        __builtin_amdgcn_global_load_lds((i8_gptr *)(s.w + (s.row[r] - (last ? s.back[r & 1] : 0u))),
+                                         (i8_lptr *)(buf + G::kColumns * 128 + (wave * G::RR + r) * 1024), 16, 0, 0);
+    s.q += 128;
+    s.w += 128;
+}
+// The columns' pieces from `have` on, in a step that has landed.
+template <class G>
+__device__ __forceinline__ void i8_zero_past(uint8_t *buf, u32 have) {
+    for (u32 i = threadIdx.x; i < G::kColumns * 8; i += G::kThreads)
+        if (((i & 7) ^ i8_swizzle(i >> 3)) >= have) *reinterpret_cast<uint4 *>(buf + 16 * i) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+}
+
+// What the matrix instructions take of 32 bytes of k (c of a step's four).
+template <class G>
+struct I8Frag {
+    v4i a[G::TR], b[G::TT];
+};
+// Where a lane's reads begin, for each 32 bytes of a step: of rows and of columns. The upper buffer's carry their buffer's place with them (and
+// are read at `up` in front of it), so that a read's address is one register and a constant that its instruction can hold.
+struct I8At {
+    u32 a[4], b[4];
+};
+template <class G, bool UP>
+__device__ __forceinline__ void i8_read(I8Frag<G> &f, const uint8_t *__restrict__ buf, const I8At &at, int c) {
+    constexpr u32 up = UP ? (u32)G::kStage : 0u;
+#pragma unroll
+    for (int i = 0; i < G::TR; i++) f.a[i] = *reinterpret_cast<const v4i *>(buf + (int)(at.a[c] - up + i * 4096));
+#pragma unroll
+    for (int j = 0; j < G::TT; j++) f.b[j] = *reinterpret_cast<const v4i *>(buf + (int)(at.b[c] - up + j * 4096));
+}
+template <class G>
+__device__ __forceinline__ void i8_multiply(const I8Frag<G> &f, v16i (&acc)[G::TR][G::TT]) {
+#pragma unroll
+    for (int i = 0; i < G::TR; i++)
+#pragma unroll
+        for (int j = 0; j < G::TT; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.a[i], f.b[j], acc[i][j], 0, 0, 0);
+}
+// The reads of the next 32 bytes between the products of these: one for every MFMAS / READS of them.
+template <class G>
+__device__ __forceinline__ void i8_weave() {
+#pragma unroll
+    for (int i = 0; i < G::TR + G::TT; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                                  // an LDS read
+        __builtin_amdgcn_sched_group_barrier(0x008, G::TR * G::TT / (G::TR + G::TT), 0); // products
     }
 }
 
-// The next step is asked for and the present one multiplied. That the two buffers are apart is said by restrict: else the compiler waits for
-// the loads into one in front of every read of the other.
-template <class G>
-__device__ __forceinline__ void i8_step(const int8_t *(&src)[G::kRounds], const uint8_t *__restrict__ buf, uint8_t *__restrict__ next, u32 wave,
-                                        bool more, bool last, const bool (&past)[2], u32 wr, u32 wt, const u32 (&at)[4], v16i (&acc)[G::TR][G::TT]) {
-    if (more) i8_ask<G>(src, next, wave, last, past);
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-        v4i A[G::TR], B[G::TT];
-#pragma unroll
-        for (int i = 0; i < G::TR; i++) A[i] = *reinterpret_cast<const v4i *>(buf + (wr + 32 * i) * 128 + at[c]);
-#pragma unroll
-        for (int j = 0; j < G::TT; j++) B[j] = *reinterpret_cast<const v4i *>(buf + (wt + 32 * j) * 128 + at[c]);
-#pragma unroll
-        for (int i = 0; i < G::TR; i++)
-#pragma unroll
-            for (int j = 0; j < G::TT; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(A[i], B[j], acc[i][j], 0, 0, 0);
+// A step: its 128 bytes of k from buf, whose first 32 are in f already; leaves the next step's first 32 there. That the two buffers are apart is
+// said by restrict: else the compiler waits for the loads into one in front of every read of the other. The turn comes before the last
+// products, so that the next step's reads and the loads of the one behind it go out under them.
+template <class G, bool UP>
+__device__ __forceinline__ void i8_step(I8Src<G> &src, uint8_t *__restrict__ buf, uint8_t *__restrict__ next, u32 wave, u32 left, u32 tail,
+                                        const I8At (&at)[2], I8Frag<G> &f, v16i (&acc)[G::TR][G::TT]) {
+    I8Frag<G> g;
+    i8_read<G, UP>(g, buf, at[UP], 1);
+    i8_multiply<G>(f, acc);
+    i8_weave<G>();
+    i8_read<G, UP>(f, buf, at[UP], 2);
+    i8_multiply<G>(g, acc);
+    i8_weave<G>();
+    i8_read<G, UP>(g, buf, at[UP], 3);
+    i8_multiply<G>(f, acc);
+    i8_weave<G>();
+    if (left > 0) {
+        i8_turn();
+        if (left > 1) i8_ask<G>(src, buf, wave, left == 2);
+        else if (tail < 8) i8_zero_past<G>(next, tail);
+        i8_read<G, !UP>(f, next, at[!UP], 0);
     }
+    i8_multiply<G>(g, acc);
 }
 
 // A wave's sums as values: column l % 32, rows 8 (x / 4) + 4 (l / 32) + x % 4 of a 32 x 32 tile.
@@ -396,10 +450,10 @@ __device__ __forceinline__ void i8_tile_out(const I8Args &a, const I8Run &run, u
     }
 }
 
-template <int BT, int BR, int WT, int WR>
-__global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_i8_tile(I8Args a, u32 n_row_tiles) {
+template <int BT, int BR, int WT, int WR, int EU>
+__global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU, EU))) void k_i8_tile(I8Args a, u32 n_row_tiles) {
     using G = I8Tile<BT, BR, WT, WR>;
-    __shared__ __align__(16) uint8_t even[G::kStage];
+    __shared__ __align__(1024) uint8_t even[G::kStage]; // the lower one: the larger alignment comes first
     __shared__ __align__(16) uint8_t odd[G::kStage];
     const u32 tid = threadIdx.x, lane = tid & 63, wave = (u32)__builtin_amdgcn_readfirstlane(tid >> 6);
     u32 expert = 0, t0;
@@ -411,26 +465,30 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(2,
     const u32 r0 = (blockIdx.x % n_row_tiles) * BR;
     I8Run run;
     if (!i8_run(a, expert, run)) return;
-    t0 += run.j0;
-    const u32 steps = (a.kp + 127) / 128;
+    t0 = (u32)__builtin_amdgcn_readfirstlane((int)(t0 + run.j0));
+    const u32 steps = (a.kp + 127) / 128, tail = (a.kp - (steps - 1) * 128) / 16; // pieces of the last step
 
-    const int8_t *src[G::kRounds];
-    bool past[2];
+    // columns and rows past the last are the last ones again, and not stored
+    I8Src<G> src;
+    src.q = a.order ? a.q : a.q + (size_t)t0 * a.kp;
+    src.w = run.w + (size_t)r0 * a.kp;
 #pragma unroll
-    for (int r = 0; r < G::kRounds; r++) {
-        const u32 line = (wave * G::kRounds + r) * 8 + (lane >> 3), piece = (lane & 7) ^ i8_swizzle(line);
-        if (line < BT) {
-            const u32 j = t0 + line;
-            bool bad;
-            src[r] = a.q + (size_t)i8_column(a, j < run.j1 ? j : run.j1 - 1, bad) * a.kp + 16 * piece;
-        } else {
-            const u32 row = r0 + line - BT;
-            src[r] = run.w + (size_t)(row < a.rows ? row : a.rows - 1) * a.kp + 16 * piece;
-        }
-        // (the place of a piece differs between even and odd rounds only)
-        if (r < 2) past[r] = (steps - 1) * 128 + 16 * piece >= a.kp;
+    for (int r = 0; r < G::RT; r++) {
+        const u32 line = (wave * G::RT + r) * 8 + (lane >> 3), j = min(t0 + line, run.j1 - 1);
+        bool bad;
+        src.col[r] = (a.order ? i8_column(a, j, bad) : j - t0) * a.kp + 16 * ((lane & 7) ^ i8_swizzle(line));
     }
-    static_assert(G::kRounds >= 2 && G::kRounds % 2 == 0, "even and odd rounds");
+#pragma unroll
+    for (int r = 0; r < G::RR; r++) {
+        const u32 line = (wave * G::RR + r) * 8 + (lane >> 3);
+        src.row[r] = (min(r0 + line, a.rows - 1) - r0) * a.kp + 16 * ((lane & 7) ^ i8_swizzle(line));
+    }
+#pragma unroll
+    for (int r = 0; r < 2; r++) { // (a lane's piece differs between even and odd rounds only)
+        const u32 piece = (lane & 7) ^ i8_swizzle(8 * r + (lane >> 3));
+        src.back[r] = piece >= tail ? 16 * piece : 0;
+    }
+
     v16i acc[G::TR][G::TT];
 #pragma unroll
     for (int i = 0; i < G::TR; i++)
@@ -439,29 +497,40 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
             for (int x = 0; x < 16; x++) acc[i][j][x] = 0;
     const u32 wt = (wave % WT) * (BT / WT), wr = BT + (wave / WT) * (BR / WR); // this wave's first lines
-    u32 at[4];
+    I8At at[2];
 #pragma unroll
-    for (u32 c = 0; c < 4; c++) at[c] = (lane & 31) * 128 + 16 * ((2 * c + (lane >> 5)) ^ i8_swizzle(lane & 31));
-    i8_ask<G>(src, even, wave, steps == 1, past);
-    for (u32 s = 0;;) {
-        i8_turn();
-        i8_step<G>(src, even, odd, wave, s + 1 < steps, s + 2 == steps, past, wr, wt, at, acc);
-        if (++s == steps) break;
-        i8_turn();
-        i8_step<G>(src, odd, even, wave, s + 1 < steps, s + 2 == steps, past, wr, wt, at, acc);
-        if (++s == steps) break;
+    for (u32 c = 0; c < 4; c++) {
+        const u32 piece = (lane & 31) * 128 + 16 * ((2 * c + (lane >> 5)) ^ i8_swizzle(lane & 31));
+#pragma unroll
+        for (u32 up = 0; up < 2; up++) {
+            at[up].a[c] = piece + wr * 128 + up * G::kStage;
+            at[up].b[c] = piece + wt * 128 + up * G::kStage;
+            __asm__("" : "+v"(at[up].a[c]), "+v"(at[up].b[c])); // one register each from here on, whatever constants meet them
+        }
+    }
+    i8_ask<G>(src, even, wave, steps == 1);
+    if (steps > 1) i8_ask<G>(src, odd, wave, steps == 2);
+    i8_turn();
+    if (steps == 1 && tail < 8) i8_zero_past<G>(even, tail);
+    I8Frag<G> f;
+    i8_read<G, false>(f, even, at[0], 0);
+    for (u32 left = steps - 1;;) {
+        i8_step<G, false>(src, even, odd, wave, left, tail, at, f, acc);
+        if (left-- == 0) break;
+        i8_step<G, true>(src, odd, even, wave, left, tail, at, f, acc);
+        if (left-- == 0) break;
     }
     if (a.et == kElemF32) i8_tile_out<kElemF32, G>(a, run, t0 + wt, r0 + (wr - BT), acc);
     else if (a.et == kElemF16) i8_tile_out<kElemF16, G>(a, run, t0 + wt, r0 + (wr - BT), acc);
     else i8_tile_out<kElemBF16, G>(a, run, t0 + wt, r0 + (wr - BT), acc);
 }
 
-template <int BT, int BR, int WT, int WR>
+template <int BT, int BR, int WT, int WR, int EU>
 static void tile_launch(const Launch &L, const I8Args &a, u32 entries) {
     const u32 row_tiles = (a.rows + BR - 1) / BR;
     u32 tiles = (entries + BT - 1) / BT;
     if (a.start) tiles = entries / BT + (a.n_experts < entries ? a.n_experts : entries); // at most a ragged tile an expert
-    hipLaunchKernelGGL((k_i8_tile<BT, BR, WT, WR>), dim3(tiles * row_tiles), dim3(64 * WT * WR), 0, L.stream, a, row_tiles);
+    hipLaunchKernelGGL((k_i8_tile<BT, BR, WT, WR, EU>), dim3(tiles * row_tiles), dim3(64 * WT * WR), 0, L.stream, a, row_tiles);
 }
 
 template <int C>
@@ -475,8 +544,8 @@ hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_expe
     const I8Args a = {w, ws, (u32)rows, (u32)i8_row_bytes(k), q, qs, (u32)n_cols, order, start, (u32)n_slots, (u32)top_k, (u32)n_cols, (u32)n_experts,
                       y, (size_t)ld, et, L.fault, L.layer};
     const u32 entries = start ? (u32)n_slots : (u32)n_cols, each = entries / (u32)n_experts;
-    if (each >= 512 && rows >= 512) tile_launch<256, 256, 4, 2>(L, a, entries);
-    else if (each >= 24 && rows >= 64) tile_launch<128, 128, 2, 2>(L, a, entries);
+    if (each >= 512 && rows >= 512) tile_launch<256, 256, 4, 2, 2>(L, a, entries);
+    else if (each >= 24 && rows >= 64) tile_launch<128, 128, 2, 2, 2>(L, a, entries);
     else if (each > 16 || start) few_launch<2>(L, a, entries);
     else few_launch<1>(L, a, entries);
     return hipGetLastError();
