@@ -422,31 +422,51 @@ __device__ __forceinline__ void i8_step(I8Src<G> &src, uint8_t *__restrict__ buf
     i8_multiply<G>(g, acc);
 }
 
-// A wave's sums as values: column l % 32, rows 8 (x / 4) + 4 (l / 32) + x % 4 of a 32 x 32 tile.
+// A wave's sums as values. The matrix instruction leaves column l % 32, rows 8 (x / 4) + 4 (l / 32) + x % 4 of a 32 x 32 tile in lane l; the sums
+// go through LDS (32 columns at a time, a wave's own part of it, four rows a piece, pieces turned by the column for the banks), so that a
+// lane stores sixteen bytes of a row of y and a row's lanes are neighbours. (Straight from the registers, eight bytes a lane and 32 rows of y an
+// instruction, a tile's end took 27 us; 8192 x 8192 outputs 1.2 TB/s.)
 template <int ET, class G>
-__device__ __forceinline__ void i8_tile_out(const I8Args &a, const I8Run &run, u32 e0, u32 row0, const v16i (&acc)[G::TR][G::TT]) {
-    const u32 lane = threadIdx.x & 63;
-    row0 += 4 * (lane >> 5);
+__device__ __forceinline__ void i8_tile_out(const I8Args &a, const I8Run &run, uint8_t *lds, u32 e0, u32 row0, const v16i (&acc)[G::TR][G::TT]) {
+    constexpr int kLine = G::TR * 8;                                                 // pieces of a column here
+    constexpr int kValues = ET == kElemF32 ? 4 : 8, kLanes = G::TR * 32 / kValues; // a lane's values, and a column's lanes
+    static_assert(G::TT <= 2, "a lane a column");
+    const u32 lane = threadIdx.x & 63, mine = row0 + kValues * (lane % kLanes);
+    float col_scale = 0.0f, row_scale[kValues];
+    if (lane < G::TT * 32 && e0 + lane < run.j1) {
+        bool bad;
+        const u32 col = i8_column(a, e0 + lane, bad);
+        if (bad) bm_raise(a.fault, a.layer, kSiteExpertId);
+        col_scale = bad ? bm_bits_f32(0x7fc00000u) : a.qs[col];
+    }
+    if (mine < a.rows) elem_load_some<kElemF32, kValues>(run.ws, mine, a.rows - mine, row_scale);
 #pragma unroll
     for (int j = 0; j < G::TT; j++) {
-        const u32 e = e0 + 32 * j + (lane & 31);
-        if (e >= run.j1) continue;
-        bool bad;
-        const u32 col = i8_column(a, e, bad);
-        if (bad) bm_raise(a.fault, a.layer, kSiteExpertId);
-        const float sc = bad ? bm_bits_f32(0x7fc00000u) : a.qs[col];
+        const u32 t = lane & 31;
 #pragma unroll
         for (int i = 0; i < G::TR; i++)
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                const u32 row = row0 + 32 * i + 8 * q;
-                if (row >= a.rows) continue;
-                float s[4], v[4];
-                elem_load_some<kElemF32, 4>(run.ws, row, a.rows - row, s);
-#pragma unroll
-                for (int x = 0; x < 4; x++) v[x] = __fmul_rn(__fmul_rn((float)acc[i][j][4 * q + x], sc), s[x]);
-                elem_store_some<ET, 4>(a.y, (size_t)e * a.ld + row, a.rows - row, v);
+                const u32 piece = 8 * i + 2 * q + (lane >> 5);
+                *reinterpret_cast<v4i *>(lds + 16 * (t * kLine + (piece ^ (t & (kLine - 1))))) =
+                    v4i{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
             }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int n = 0; n < 32 * kLanes / 64; n++) {
+            const u32 c = n * (64 / kLanes) + lane / kLanes, e = e0 + 32 * j + c;
+            const float s = __shfl(col_scale, 32 * j + c, 64);
+            float v[kValues];
+#pragma unroll
+            for (int p = 0; p < kValues / 4; p++) {
+                const u32 piece = (lane % kLanes) * (kValues / 4) + p;
+                const v4i sum = *reinterpret_cast<const v4i *>(lds + 16 * (c * kLine + (piece ^ (c & (kLine - 1)))));
+#pragma unroll
+                for (int x = 0; x < 4; x++) v[4 * p + x] = __fmul_rn(__fmul_rn((float)sum[x], s), row_scale[4 * p + x]);
+            }
+            if (e < run.j1 && mine < a.rows) elem_store_some<ET, kValues>(a.y, (size_t)e * a.ld + mine, a.rows - mine, v);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
@@ -520,9 +540,13 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
         i8_step<G, true>(src, odd, even, wave, left, tail, at, f, acc);
         if (left-- == 0) break;
     }
-    if (a.et == kElemF32) i8_tile_out<kElemF32, G>(a, run, t0 + wt, r0 + (wr - BT), acc);
-    else if (a.et == kElemF16) i8_tile_out<kElemF16, G>(a, run, t0 + wt, r0 + (wr - BT), acc);
-    else i8_tile_out<kElemBF16, G>(a, run, t0 + wt, r0 + (wr - BT), acc);
+    __syncthreads(); // the buffers are the sums' from here
+    static_assert(G::kWaves * G::TR * 4096 <= 2 * G::kStage && G::kStage % (G::TR * 4096) == 0, "a wave's part lies in one buffer");
+    constexpr u32 kEven = G::kStage / (G::TR * 4096);
+    uint8_t *part = wave < kEven ? even + wave * (G::TR * 4096) : odd + (wave - kEven) * (G::TR * 4096);
+    if (a.et == kElemF32) i8_tile_out<kElemF32, G>(a, run, part, t0 + wt, r0 + (wr - BT), acc);
+    else if (a.et == kElemF16) i8_tile_out<kElemF16, G>(a, run, part, t0 + wt, r0 + (wr - BT), acc);
+    else i8_tile_out<kElemBF16, G>(a, run, part, t0 + wt, r0 + (wr - BT), acc);
 }
 
 template <int BT, int BR, int WT, int WR, int EU>
