@@ -206,7 +206,7 @@ __device__ __forceinline__ void i8_store4(const I8Args &a, u32 j, u32 r, const f
 // Few columns a matrix: 16 R rows a workgroup against 16 C columns, its NW waves dealing the row's 64-byte steps among them. Weights go
 // from memory to registers in the form v_mfma_i32_16x16x64_i8 takes them (lane l: row l % 16, bytes 16 (l / 16) .. + 15 of the step), each once;
 // the columns come from the cache. The waves' sums meet in LDS as integers.
-template <int R, int C, int NW>
+template <int R, int C, int NW, int U>
 __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
     __shared__ v4i part[NW][R * C][64];
     const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = threadIdx.x;
@@ -232,22 +232,39 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
         for (int r = 0; r < R; r++)
 #pragma unroll
             for (int c = 0; c < C; c++) acc[r][c] = v4i{0, 0, 0, 0};
-        for (u32 s = wave; s < steps; s += NW) {
-            const u32 at = 64 * s + 16 * (lane >> 4);
-            const bool in = at < a.kp; // a piece past the row: any of the row's bytes against zeros
-            const u32 off = in ? at : 0;
-            v4i A[R], B[C];
+        // U steps asked for at a time, the next U while these are multiplied
+        v4i A[2][U][R], B[2][U][C];
+        auto ask = [&](u32 s, v4i (&fa)[U][R], v4i (&fb)[U][C]) {
 #pragma unroll
-            for (int r = 0; r < R; r++) A[r] = *reinterpret_cast<const v4i *>(wp[r] + off);
+            for (int u = 0; u < U; u++) {
+                const u32 at = 64 * (s + u * NW) + 16 * (lane >> 4), off = at < a.kp ? at : 0; // past the row: its first bytes, against zeros
 #pragma unroll
-            for (int c = 0; c < C; c++) {
-                B[c] = *reinterpret_cast<const v4i *>(qp[c] + off);
-                if (!in) B[c] = v4i{0, 0, 0, 0};
+                for (int r = 0; r < R; r++) fa[u][r] = *reinterpret_cast<const v4i *>(wp[r] + off);
+#pragma unroll
+                for (int c = 0; c < C; c++) fb[u][c] = *reinterpret_cast<const v4i *>(qp[c] + off);
             }
+        };
+        auto multiply = [&](u32 s, v4i (&fa)[U][R], v4i (&fb)[U][C]) {
 #pragma unroll
-            for (int r = 0; r < R; r++)
+            for (int u = 0; u < U; u++) {
+                const bool in = 64 * (s + u * NW) + 16 * (lane >> 4) < a.kp;
 #pragma unroll
-                for (int c = 0; c < C; c++) acc[r][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[r], B[c], acc[r][c], 0, 0, 0);
+                for (int c = 0; c < C; c++) {
+                    const v4i b = in ? fb[u][c] : v4i{0, 0, 0, 0};
+#pragma unroll
+                    for (int r = 0; r < R; r++) acc[r][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[u][r], b, acc[r][c], 0, 0, 0);
+                }
+            }
+        };
+        u32 s = wave;
+        ask(s, A[0], B[0]);
+        for (;;) {
+            if (s + U * NW < steps) ask(s + U * NW, A[1], B[1]);
+            multiply(s, A[0], B[0]);
+            if ((s += U * NW) >= steps) break;
+            if (s + U * NW < steps) ask(s + U * NW, A[0], B[0]);
+            multiply(s, A[1], B[1]);
+            if ((s += U * NW) >= steps) break;
         }
 #pragma unroll
         for (int r = 0; r < R; r++)
@@ -276,21 +293,24 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
     }
 }
 
-// Many columns a matrix: BT columns x BR rows a workgroup, 128 bytes of k a step through LDS, where the loads put them themselves (16 bytes a
-// lane, no register in between): while the waves multiply one step the next is on its way into the other buffer, one barrier a step. A wave holds
-// (BT / WT) x (BR / WR) sums in v_mfma_i32_32x32x32_i8's form.
+// Many columns a matrix: BT columns x BR rows a workgroup, 128 bytes of k a step through a ring of S LDS buffers, where the loads put them
+// themselves (16 bytes a lane, no register in between): while the waves multiply one step the next S - 1 are on their way, one barrier a step. A
+// wave holds (BT / WT) x (BR / WR) sums in v_mfma_i32_16x16x64_i8's form.
 // A step's rows are 128-byte lines of eight 16-byte pieces; piece c of line r lies at place c ^ swizzle(r), which the lane that asks for it
-// arranges, so that the pieces that the matrix instructions take of 32 lines at once come from all the banks.
-typedef int v16i __attribute__((ext_vector_type(16)));
+// arranges, so that the pieces that the matrix instructions take of 16 lines at once come from all the banks.
 typedef __attribute__((address_space(1))) void i8_gptr;
 typedef __attribute__((address_space(3))) void i8_lptr;
 
-template <int BT, int BR, int WT, int WR>
+template <int BT, int BR, int WT, int WR, int S>
 struct I8Tile {
-    static constexpr int kColumns = BT, kRows = BR, kWaves = WT * WR, kThreads = 64 * kWaves, kStage = (BT + BR) * 128;
-    static constexpr int RT = BT / 8 / kWaves, RR = BR / 8 / kWaves; // a wave's loads a step, eight lines each, of columns and of rows
-    static constexpr int TT = BT / WT / 32, TR = BR / WR / 32;
-    static_assert(BT % (16 * kWaves) == 0 && BR % (16 * kWaves) == 0 && BT % (32 * WT) == 0 && BR % (32 * WR) == 0, "whole waves, even rounds");
+    static constexpr int kColumns = BT, kRows = BR, kRing = S, kWaves = WT * WR, kThreads = 64 * kWaves, kStage = (BT + BR) * 128;
+    // a wave's loads a step, eight lines each, of columns and of rows (the last waves may repeat some of rows)
+    static constexpr int RT = BT / 8 / kWaves, RR = (BR / 8 + kWaves - 1) / kWaves;
+    static constexpr int TT = BT / WT / 16, TR = BR / WR / 16, H0 = (TR + 1) / 2, H1 = TR / 2; // a wave's tiles of 16, its rows in two halves
+    static_assert(BT % (8 * kWaves) == 0 && BT % (16 * WT) == 0 && BR % (16 * WR) == 0 && TR > 1, "whole waves");
+    static_assert(S == 2 || (S == 4 && BR % (8 * kWaves) == 0), "where steps overlap, their loads are counted: as many for every wave");
+    // buffers from this one on lie past what a read's constant reaches
+    static constexpr int kUp = S * kStage <= 65536 ? S : S / 2;
 };
 
 __device__ __forceinline__ u32 i8_swizzle(u32 line) { return (line >> 1) & 7; }
@@ -326,11 +346,14 @@ __device__ __forceinline__ bool i8_find_tile(const I8Args &a, u32 tile, u32 &exp
     return false;
 }
 
-// What a wave asked for has landed, and every wave is done with the buffer that is written next. (The wait as a builtin: the compiler counts
-// it, where behind one in asm it would wait for the loads that follow too.)
+// All but the last AHEAD steps that a wave asked for have landed, and every wave is done with the buffer that is written next. (The wait as a
+// builtin: the compiler counts it, where behind one in asm it would wait for the loads that follow too.)
+template <class G, int AHEAD>
 __device__ __forceinline__ void i8_turn() {
+    constexpr int n = AHEAD * (G::RT + G::RR);
+    static_assert(n < 64, "vmcnt");
     __asm__ volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070); // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt(0x0070 | (n & 15) | (n >> 4) << 14); // vmcnt(n) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     __asm__ volatile("" ::: "memory");
 }
@@ -342,15 +365,25 @@ struct I8Src {
     const int8_t *q, *w; // this step's
     u32 col[G::RT], row[G::RR], back[2];
 };
+// The eight rows of a wave's r-th load: where there are not as many for every wave, the last ones are asked for again.
+template <class G>
+__device__ __forceinline__ u32 i8_row_group(u32 wave, int r) {
+    const u32 group = wave * G::RR + r;
+    return G::kRows % (8 * G::kWaves) == 0 ? group : min(group, (u32)G::kRows / 8 - 1);
+}
 template <class G>
 __device__ __forceinline__ void i8_ask(I8Src<G> &s, uint8_t *buf, u32 wave, bool last) {
 #pragma unroll
-    for (int r = 0; r < G::RT; r++)
-        __builtin_amdgcn_global_load_lds((i8_gptr *)(s.q + (s.col[r] - (last ? s.back[r & 1] : 0u))), (i8_lptr *)(buf + (wave * G::RT + r) * 1024), 16, 0, 0);
+    for (int r = 0; r < G::RT; r++) {
+        const u32 group = wave * G::RT + r;
+        __builtin_amdgcn_global_load_lds((i8_gptr *)(s.q + (s.col[r] - (last ? s.back[group & 1] : 0u))), (i8_lptr *)(buf + group * 1024), 16, 0, 0);
+    }
 #pragma unroll
-    for (int r = 0; r < G::RR; r++)
-        __builtin_amdgcn_global_load_lds((i8_gptr *)(s.w + (s.row[r] - (last ? s.back[r & 1] : 0u))),
-                                         (i8_lptr *)(buf + G::kColumns * 128 + (wave * G::RR + r) * 1024), 16, 0, 0);
+    for (int r = 0; r < G::RR; r++) {
+        const u32 group = i8_row_group<G>(wave, r);
+        __builtin_amdgcn_global_load_lds((i8_gptr *)(s.w + (s.row[r] - (last ? (group & 1 ? s.back[1] : s.back[0]) : 0u))),
+                                         (i8_lptr *)(buf + G::kColumns * 128 + group * 1024), 16, 0, 0);
+    }
     s.q += 128;
     s.w += 128;
 }
@@ -362,119 +395,138 @@ __device__ __forceinline__ void i8_zero_past(uint8_t *buf, u32 have) {
     __syncthreads();
 }
 
-// What the matrix instructions take of 32 bytes of k (c of a step's four).
-template <class G>
-struct I8Frag {
-    v4i a[G::TR], b[G::TT];
-};
-// Where a lane's reads begin, for each 32 bytes of a step: of rows and of columns. The upper buffer's carry their buffer's place with them (and
-// are read at `up` in front of it), so that a read's address is one register and a constant that its instruction can hold.
+// Where a lane's reads begin, for each 64 bytes of a step: of rows and of columns. The upper buffers' carry the first one's place with them
+// (and are read that far in front), so that a read's address is one register and a constant that its instruction can hold.
 struct I8At {
-    u32 a[4], b[4];
+    u32 a[2], b[2];
 };
-template <class G, bool UP>
-__device__ __forceinline__ void i8_read(I8Frag<G> &f, const uint8_t *__restrict__ buf, const I8At &at, int c) {
-    constexpr u32 up = UP ? (u32)G::kStage : 0u;
+// What the matrix instructions take of 64 bytes of k of N tiles, from the FIRST on.
+template <class G, int B, int N>
+__device__ __forceinline__ void i8_read(v4i (&f)[N], const uint8_t *__restrict__ buf, u32 at, int first) {
+    constexpr u32 up = B >= G::kUp ? (u32)G::kUp * G::kStage : 0u;
 #pragma unroll
-    for (int i = 0; i < G::TR; i++) f.a[i] = *reinterpret_cast<const v4i *>(buf + (int)(at.a[c] - up + i * 4096));
-#pragma unroll
-    for (int j = 0; j < G::TT; j++) f.b[j] = *reinterpret_cast<const v4i *>(buf + (int)(at.b[c] - up + j * 4096));
+    for (int i = 0; i < N; i++) f[i] = *reinterpret_cast<const v4i *>(buf + (int)(at - up + (first + i) * 2048));
 }
-template <class G>
-__device__ __forceinline__ void i8_multiply(const I8Frag<G> &f, v16i (&acc)[G::TR][G::TT]) {
+template <int N, int TT>
+__device__ __forceinline__ void i8_multiply(const v4i (&a)[N], const v4i (&b)[TT], v4i (*acc)[TT]) {
 #pragma unroll
-    for (int i = 0; i < G::TR; i++)
+    for (int i = 0; i < N; i++)
 #pragma unroll
-        for (int j = 0; j < G::TT; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.a[i], f.b[j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < TT; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i], b[j], acc[i][j], 0, 0, 0);
 }
-// The reads of the next 32 bytes between the products of these: one for every MFMAS / READS of them.
-template <class G>
+// READS of what comes next between MFMAS products of what is there.
+template <int READS, int MFMAS>
 __device__ __forceinline__ void i8_weave() {
 #pragma unroll
-    for (int i = 0; i < G::TR + G::TT; i++) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                                  // an LDS read
-        __builtin_amdgcn_sched_group_barrier(0x008, G::TR * G::TT / (G::TR + G::TT), 0); // products
+    for (int i = 0; i < READS; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);              // an LDS read
+        __builtin_amdgcn_sched_group_barrier(0x008, MFMAS / READS ? MFMAS / READS : 1, 0); // products
     }
 }
 
-// A step: its 128 bytes of k from buf, whose first 32 are in f already; leaves the next step's first 32 there. That the two buffers are apart is
+// A step: its 128 bytes of k from buf in four parts - 64 bytes against half of the wave's rows each -, whose first part's pieces are in a0 and b0
+// already; leaves the next step's there. A part's pieces are read under the products of the part before. That the two buffers are apart is
 // said by restrict: else the compiler waits for the loads into one in front of every read of the other. The turn comes before the last
-// products, so that the next step's reads and the loads of the one behind it go out under them.
-template <class G, bool UP>
+// part, so that the next step's reads and the loads of the one behind it go out under its products.
+// FULL: more steps are left behind this one than the ring holds, so that nothing is asked of where the rows end. B: buf's number.
+template <class G, int B, bool FULL>
 __device__ __forceinline__ void i8_step(I8Src<G> &src, uint8_t *__restrict__ buf, uint8_t *__restrict__ next, u32 wave, u32 left, u32 tail,
-                                        const I8At (&at)[2], I8Frag<G> &f, v16i (&acc)[G::TR][G::TT]) {
-    I8Frag<G> g;
-    i8_read<G, UP>(g, buf, at[UP], 1);
-    i8_multiply<G>(f, acc);
-    i8_weave<G>();
-    i8_read<G, UP>(f, buf, at[UP], 2);
-    i8_multiply<G>(g, acc);
-    i8_weave<G>();
-    i8_read<G, UP>(g, buf, at[UP], 3);
-    i8_multiply<G>(f, acc);
-    i8_weave<G>();
-    if (left > 0) {
-        i8_turn();
-        if (left > 1) i8_ask<G>(src, buf, wave, left == 2);
-        else if (tail < 8) i8_zero_past<G>(next, tail);
-        i8_read<G, !UP>(f, next, at[!UP], 0);
+                                        const I8At (&at)[2], v4i (&a0)[G::H0], v4i (&b0)[G::TT], v4i (&acc)[G::TR][G::TT]) {
+    constexpr int kUp = B >= G::kUp, kNext = (B + 1) % G::kRing, kNextUp = kNext >= G::kUp;
+    v4i a1[G::H1], b1[G::TT];
+    i8_read<G, B>(a1, buf, at[kUp].a[0], G::H0);
+    i8_multiply(a0, b0, acc);
+    i8_weave<G::H1, G::H0 * G::TT>();
+    i8_read<G, B>(a0, buf, at[kUp].a[1], 0);
+    i8_read<G, B>(b1, buf, at[kUp].b[1], 0);
+    i8_multiply(a1, b0, acc + G::H0);
+    i8_weave<G::H0 + G::TT, G::H1 * G::TT>();
+    i8_read<G, B>(a1, buf, at[kUp].a[1], G::H0);
+    i8_multiply(a0, b1, acc);
+    i8_weave<G::H1, G::H0 * G::TT>();
+    if constexpr (FULL) {
+        i8_turn<G, G::kRing - 2>();
+        i8_ask<G>(src, buf, wave, false);
+    } else if (left > 0) {
+        if (G::kRing == 2 || left == 1) i8_turn<G, 0>();
+        else if (left == 2) i8_turn<G, G::kRing == 2 ? 0 : 1>();
+        else i8_turn<G, G::kRing - 2>();
+        if (left >= (u32)G::kRing) i8_ask<G>(src, buf, wave, left == (u32)G::kRing);
+        else if (left == 1 && tail < 8) i8_zero_past<G>(next, tail);
     }
-    i8_multiply<G>(g, acc);
+    if (FULL || left > 0) {
+        i8_read<G, kNext>(a0, next, at[kNextUp].a[0], 0);
+        i8_read<G, kNext>(b0, next, at[kNextUp].b[0], 0);
+    }
+    i8_multiply(a1, b1, acc + G::H0);
+    if constexpr (FULL) i8_weave<G::H0 + G::TT, G::H1 * G::TT>();
 }
 
-// A wave's sums as values. The matrix instruction leaves column l % 32, rows 8 (x / 4) + 4 (l / 32) + x % 4 of a 32 x 32 tile in lane l; the sums
-// go through LDS (32 columns at a time, a wave's own part of it, four rows a piece, pieces turned by the column for the banks), so that a
-// lane stores sixteen bytes of a row of y and a row's lanes are neighbours. (Straight from the registers, eight bytes a lane and 32 rows of y an
+// Where piece p of column c lies in a line of LINE pieces: turned by the column within the pieces' largest power of two.
+template <int LINE>
+__device__ __forceinline__ u32 i8_turned(u32 p, u32 c) {
+    constexpr u32 kPow = LINE & -LINE;
+    return p ^ (c & (kPow - 1));
+}
+
+// A wave's sums as values. The matrix instruction leaves column l % 16, rows 4 (l / 16) .. + 3 of a 16 x 16 tile in lane l; the sums go through LDS
+// (32 columns at a time, a wave's own part of it, four rows a piece, pieces turned by the column for the banks), so that a lane stores
+// sixteen bytes of a row of y and a row's lanes are neighbours. (Straight from the registers, eight bytes a lane and 32 rows of y an
 // instruction, a tile's end took 27 us; 8192 x 8192 outputs 1.2 TB/s.)
 template <int ET, class G>
-__device__ __forceinline__ void i8_tile_out(const I8Args &a, const I8Run &run, uint8_t *lds, u32 e0, u32 row0, const v16i (&acc)[G::TR][G::TT]) {
-    constexpr int kLine = G::TR * 8;                                                 // pieces of a column here
-    constexpr int kValues = ET == kElemF32 ? 4 : 8, kLanes = G::TR * 32 / kValues; // a lane's values, and a column's lanes
-    static_assert(G::TT <= 2, "a lane a column");
-    const u32 lane = threadIdx.x & 63, mine = row0 + kValues * (lane % kLanes);
-    float col_scale = 0.0f, row_scale[kValues];
-    if (lane < G::TT * 32 && e0 + lane < run.j1) {
+__device__ __forceinline__ void i8_tile_out(const I8Args &a, const I8Run &run, uint8_t *lds, u32 e0, u32 row0, const v4i (&acc)[G::TR][G::TT]) {
+    constexpr int kLine = G::TR * 4, kPiecesOut = ET == kElemF32 ? 1 : 2, kValues = 4 * kPiecesOut; // a column's pieces; a lane's pieces and values a store
+    constexpr int kBusy = kLine / kPiecesOut, kLanes = kBusy <= 8 ? 8 : kBusy <= 16 ? 16 : 32;        // a column's lanes: a power of two, the last ones idle
+    static_assert(kLine % kPiecesOut == 0 && kBusy <= kLanes, "whole lanes");
+    static_assert(G::TT % 2 == 0 && G::TT <= 4, "a lane a column, 32 at a time");
+    const u32 lane = threadIdx.x & 63;
+    float col_scale = 0.0f;
+    if (lane < G::TT * 16 && e0 + lane < run.j1) {
         bool bad;
         const u32 col = i8_column(a, e0 + lane, bad);
         if (bad) bm_raise(a.fault, a.layer, kSiteExpertId);
         col_scale = bad ? bm_bits_f32(0x7fc00000u) : a.qs[col];
     }
-    if (mine < a.rows) elem_load_some<kElemF32, kValues>(run.ws, mine, a.rows - mine, row_scale);
+    const u32 first = lane % kLanes * kPiecesOut, row = row0 + 4 * first; // this lane's pieces of every column, and its rows
+    const bool mine = lane % kLanes < (u32)kBusy && row < a.rows;
+    float r[kValues];
+    if (mine) elem_load_some<kElemF32, kValues>(run.ws, row, a.rows - row, r);
 #pragma unroll
-    for (int j = 0; j < G::TT; j++) {
-        const u32 t = lane & 31;
+    for (int j = 0; j < G::TT; j += 2) {
 #pragma unroll
-        for (int i = 0; i < G::TR; i++)
+        for (int jj = 0; jj < 2; jj++) {
+            const u32 t = 16 * jj + (lane & 15);
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const u32 piece = 8 * i + 2 * q + (lane >> 5);
-                *reinterpret_cast<v4i *>(lds + 16 * (t * kLine + (piece ^ (t & (kLine - 1))))) =
-                    v4i{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-            }
+            for (int i = 0; i < G::TR; i++)
+                *reinterpret_cast<v4i *>(lds + 16 * (t * kLine + i8_turned<kLine>(4 * i + (lane >> 4), t))) = acc[i][j + jj];
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int n = 0; n < 32 * kLanes / 64; n++) {
-            const u32 c = n * (64 / kLanes) + lane / kLanes, e = e0 + 32 * j + c;
-            const float s = __shfl(col_scale, 32 * j + c, 64);
+            const u32 c = n * (64 / kLanes) + lane / kLanes, e = e0 + 16 * j + c;
+            const float s = __shfl(col_scale, 16 * j + c, 64);
+            if (!mine || e >= run.j1) continue;
             float v[kValues];
 #pragma unroll
-            for (int p = 0; p < kValues / 4; p++) {
-                const u32 piece = (lane % kLanes) * (kValues / 4) + p;
-                const v4i sum = *reinterpret_cast<const v4i *>(lds + 16 * (c * kLine + (piece ^ (c & (kLine - 1)))));
+            for (int p = 0; p < kPiecesOut; p++) {
+                const v4i sum = *reinterpret_cast<const v4i *>(lds + 16 * (c * kLine + i8_turned<kLine>(first + p, c)));
 #pragma unroll
-                for (int x = 0; x < 4; x++) v[4 * p + x] = __fmul_rn(__fmul_rn((float)sum[x], s), row_scale[4 * p + x]);
+                for (int x = 0; x < 4; x++) v[4 * p + x] = __fmul_rn(__fmul_rn((float)sum[x], s), r[4 * p + x]);
             }
-            if (e < run.j1 && mine < a.rows) elem_store_some<ET, kValues>(a.y, (size_t)e * a.ld + mine, a.rows - mine, v);
+            elem_store_some<ET, kValues>(a.y, (size_t)e * a.ld + row, a.rows - row, v);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
-template <int BT, int BR, int WT, int WR, int EU>
-__global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU, EU))) void k_i8_tile(I8Args a, u32 n_row_tiles) {
-    using G = I8Tile<BT, BR, WT, WR>;
-    __shared__ __align__(1024) uint8_t even[G::kStage]; // the lower one: the larger alignment comes first
-    __shared__ __align__(16) uint8_t odd[G::kStage];
+template <int BT, int BR, int WT, int WR, int S, int EU>
+__global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU))) void k_i8_tile(I8Args a, u32 n_row_tiles) {
+    using G = I8Tile<BT, BR, WT, WR, S>;
+    // in this order: the larger alignment comes first
+    __shared__ __align__(4096) uint8_t ring0[G::kStage];
+    __shared__ __align__(2048) uint8_t ring1[G::kStage];
+    __shared__ __align__(1024) uint8_t ring2[S > 2 ? G::kStage : 16];
+    __shared__ __align__(512) uint8_t ring3[S > 2 ? G::kStage : 16];
     const u32 tid = threadIdx.x, lane = tid & 63, wave = (u32)__builtin_amdgcn_readfirstlane(tid >> 6);
     u32 expert = 0, t0;
     if (a.start) {
@@ -500,78 +552,145 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     }
 #pragma unroll
     for (int r = 0; r < G::RR; r++) {
-        const u32 line = (wave * G::RR + r) * 8 + (lane >> 3);
+        const u32 line = i8_row_group<G>(wave, r) * 8 + (lane >> 3);
         src.row[r] = (min(r0 + line, a.rows - 1) - r0) * a.kp + 16 * ((lane & 7) ^ i8_swizzle(line));
     }
 #pragma unroll
-    for (int r = 0; r < 2; r++) { // (a lane's piece differs between even and odd rounds only)
+    for (int r = 0; r < 2; r++) { // (a lane's piece differs between even and odd groups of eight lines only)
         const u32 piece = (lane & 7) ^ i8_swizzle(8 * r + (lane >> 3));
         src.back[r] = piece >= tail ? 16 * piece : 0;
     }
 
-    v16i acc[G::TR][G::TT];
+    v4i acc[G::TR][G::TT];
 #pragma unroll
     for (int i = 0; i < G::TR; i++)
 #pragma unroll
-        for (int j = 0; j < G::TT; j++)
-#pragma unroll
-            for (int x = 0; x < 16; x++) acc[i][j][x] = 0;
+        for (int j = 0; j < G::TT; j++) acc[i][j] = v4i{0, 0, 0, 0};
     const u32 wt = (wave % WT) * (BT / WT), wr = BT + (wave / WT) * (BR / WR); // this wave's first lines
     I8At at[2];
 #pragma unroll
-    for (u32 c = 0; c < 4; c++) {
-        const u32 piece = (lane & 31) * 128 + 16 * ((2 * c + (lane >> 5)) ^ i8_swizzle(lane & 31));
+    for (u32 c = 0; c < 2; c++) {
+        const u32 piece = (lane & 15) * 128 + 16 * ((4 * c + (lane >> 4)) ^ i8_swizzle(lane & 15));
 #pragma unroll
         for (u32 up = 0; up < 2; up++) {
-            at[up].a[c] = piece + wr * 128 + up * G::kStage;
-            at[up].b[c] = piece + wt * 128 + up * G::kStage;
+            at[up].a[c] = piece + wr * 128 + up * G::kUp * G::kStage;
+            at[up].b[c] = piece + wt * 128 + up * G::kUp * G::kStage;
             __asm__("" : "+v"(at[up].a[c]), "+v"(at[up].b[c])); // one register each from here on, whatever constants meet them
         }
     }
-    i8_ask<G>(src, even, wave, steps == 1);
-    if (steps > 1) i8_ask<G>(src, odd, wave, steps == 2);
-    i8_turn();
-    if (steps == 1 && tail < 8) i8_zero_past<G>(even, tail);
-    I8Frag<G> f;
-    i8_read<G, false>(f, even, at[0], 0);
-    for (u32 left = steps - 1;;) {
-        i8_step<G, false>(src, even, odd, wave, left, tail, at, f, acc);
-        if (left-- == 0) break;
-        i8_step<G, true>(src, odd, even, wave, left, tail, at, f, acc);
-        if (left-- == 0) break;
+    i8_ask<G>(src, ring0, wave, steps == 1);
+    if (steps > 1) i8_ask<G>(src, ring1, wave, steps == 2);
+    if (S > 2 && steps > 2) i8_ask<G>(src, ring2, wave, steps == 3);
+    if (S > 2 && steps > 3) i8_ask<G>(src, ring3, wave, steps == 4);
+    if (steps >= (u32)S) i8_turn<G, S - 1>();
+    else i8_turn<G, 0>();
+    if (steps == 1 && tail < 8) i8_zero_past<G>(ring0, tail);
+    v4i a0[G::H0], b0[G::TT];
+    i8_read<G, 0>(a0, ring0, at[0].a[0], 0);
+    i8_read<G, 0>(b0, ring0, at[0].b[0], 0);
+    u32 left = steps - 1;
+    if constexpr (S == 2) {
+        for (; left >= 4; left -= 2) {
+            i8_step<G, 0, true>(src, ring0, ring1, wave, 0, 0, at, a0, b0, acc);
+            i8_step<G, 1, true>(src, ring1, ring0, wave, 0, 0, at, a0, b0, acc);
+        }
+        for (;;) {
+            i8_step<G, 0, false>(src, ring0, ring1, wave, left, tail, at, a0, b0, acc);
+            if (left-- == 0) break;
+            i8_step<G, 1, false>(src, ring1, ring0, wave, left, tail, at, a0, b0, acc);
+            if (left-- == 0) break;
+        }
+    } else {
+        for (; left >= 8; left -= 4) {
+            i8_step<G, 0, true>(src, ring0, ring1, wave, 0, 0, at, a0, b0, acc);
+            i8_step<G, 1, true>(src, ring1, ring2, wave, 0, 0, at, a0, b0, acc);
+            i8_step<G, 2, true>(src, ring2, ring3, wave, 0, 0, at, a0, b0, acc);
+            i8_step<G, 3, true>(src, ring3, ring0, wave, 0, 0, at, a0, b0, acc);
+        }
+        for (;;) {
+            i8_step<G, 0, false>(src, ring0, ring1, wave, left, tail, at, a0, b0, acc);
+            if (left-- == 0) break;
+            i8_step<G, 1, false>(src, ring1, ring2, wave, left, tail, at, a0, b0, acc);
+            if (left-- == 0) break;
+            i8_step<G, 2, false>(src, ring2, ring3, wave, left, tail, at, a0, b0, acc);
+            if (left-- == 0) break;
+            i8_step<G, 3, false>(src, ring3, ring0, wave, left, tail, at, a0, b0, acc);
+            if (left-- == 0) break;
+        }
     }
     __syncthreads(); // the buffers are the sums' from here
-    static_assert(G::kWaves * G::TR * 4096 <= 2 * G::kStage && G::kStage % (G::TR * 4096) == 0, "a wave's part lies in one buffer");
-    constexpr u32 kEven = G::kStage / (G::TR * 4096);
-    uint8_t *part = wave < kEven ? even + wave * (G::TR * 4096) : odd + (wave - kEven) * (G::TR * 4096);
+    constexpr u32 kPart = G::TR * 2048, kEven = G::kStage / kPart; // a wave's part, and how many lie in the first buffer
+    static_assert(G::kWaves <= 2 * kEven, "every part lies in one buffer");
+    uint8_t *part = wave < kEven ? ring0 + wave * kPart : ring1 + (wave - kEven) * kPart;
     if (a.et == kElemF32) i8_tile_out<kElemF32, G>(a, run, part, t0 + wt, r0 + (wr - BT), acc);
     else if (a.et == kElemF16) i8_tile_out<kElemF16, G>(a, run, part, t0 + wt, r0 + (wr - BT), acc);
     else i8_tile_out<kElemBF16, G>(a, run, part, t0 + wt, r0 + (wr - BT), acc);
 }
 
-template <int BT, int BR, int WT, int WR, int EU>
+template <int BT, int BR, int WT, int WR, int S, int EU>
 static void tile_launch(const Launch &L, const I8Args &a, u32 entries) {
     const u32 row_tiles = (a.rows + BR - 1) / BR;
     u32 tiles = (entries + BT - 1) / BT;
     if (a.start) tiles = entries / BT + (a.n_experts < entries ? a.n_experts : entries); // at most a ragged tile an expert
-    hipLaunchKernelGGL((k_i8_tile<BT, BR, WT, WR, EU>), dim3(tiles * row_tiles), dim3(64 * WT * WR), 0, L.stream, a, row_tiles);
+    hipLaunchKernelGGL((k_i8_tile<BT, BR, WT, WR, S, EU>), dim3(tiles * row_tiles), dim3(64 * WT * WR), 0, L.stream, a, row_tiles);
 }
 
-template <int C>
+template <int R, int C, int NW, int U>
 static void few_launch(const Launch &L, const I8Args &a, u32 entries) {
     const u32 z = a.start ? 1u : (entries + 16 * C - 1) / (16 * C);
-    hipLaunchKernelGGL((k_i8_few<1, C, 8>), dim3((a.rows + 15) / 16, a.start ? a.n_experts : 1u, z < 65535u ? z : 65535u), dim3(512), 0, L.stream, a);
+    hipLaunchKernelGGL((k_i8_few<R, C, NW, U>), dim3((a.rows + 16 * R - 1) / (16 * R), a.start ? a.n_experts : 1u, z < 65535u ? z : 65535u), dim3(64 * NW), 0,
+                       L.stream, a);
 }
 
+// Which form: all give the same bits. us on MI355X, bf16 out, weights of three sets in turn, the chosen form's first.
+//   One matrix. Large tiles are the better the more of them there are, and whole rounds of 256 compute units count: a round of 256 x 256 tiles takes
+//   64 units of time, of 256 x 224 57, of two 128 x 128 a unit 39. (4096 x 7168 x 7168: 512 tiles of 224 rows are two rounds, 179, 448 of 256 take
+//   the same two, 198, 128 x 128 223; 4096 cubed 58, 90, 66; 8192 cubed 453, 507, 538; 4096 x 2048 x 7168, the 128 x 128 first, 59, 80, 69.)
+//   Below some hundred large tiles the smaller ones fill the card: 1024 x 7168 x 2048 in 128 x 128 21.5 (64 x 128: 26.4); 2048 cubed in 64 x 128 14.7
+//   (128 x 128: 16.9); 256 x 7168 x 2048 in 64 x 64 9.9 (64 x 128: 12.3); 128 x 2048 x 7168 in 32 x 64 15.1 (64 x 64: 15.8), the last two with
+//   four steps in flight, as few workgroups need. Up to 32 columns, and where even those tiles are few, every workgroup's waves share a row's k: 24 x 7168 x 2048 6.5
+//   (32 x 64: 7.5), 64 x 2048 x 7168 12.0 (15.0); 16 x 7168 x 2048 5.8 (7.3), 1 x 2048 x 7168 6.6 (14.8). There two tiles of 16 rows a workgroup of four waves
+//   from 320 tiles on (24 columns: 6.5 against 7.8), else one of eight waves (1 x 2048 x 7168: 6.6 against 9.9).
+//   Experts, by slots an expert: 2048 tokens, top 8 of 128 (128 slots each), 768 x 2048 rows in 128 x 128 81 (64 x 128: 88, 256 x 256: 85); 512 tokens in 64 x 128 50
+//   (128 x 128: 54); 64 tokens in 32 x 64 33 (64 x 128: 34, waves sharing k 41); one token's eight slots by waves sharing k 7.9 (32 x 64: 9.1);
+//   4096 tokens, top 8 of 32, 7168 x 2048 rows in 256 x 256 573 (256 x 224: 594, 128 x 128: 630).
 hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_experts, int rows, int k, const int8_t *q, const float *qs, int n_cols,
                    const uint32_t *order, const uint32_t *start, int n_slots, int top_k, void *y, int et, int64_t ld) {
     const I8Args a = {w, ws, (u32)rows, (u32)i8_row_bytes(k), q, qs, (u32)n_cols, order, start, (u32)n_slots, (u32)top_k, (u32)n_cols, (u32)n_experts,
                       y, (size_t)ld, et, L.fault, L.layer};
-    const u32 entries = start ? (u32)n_slots : (u32)n_cols, each = entries / (u32)n_experts;
-    if (each >= 512 && rows >= 512) tile_launch<256, 256, 4, 2, 2>(L, a, entries);
-    else if (each >= 24 && rows >= 64) tile_launch<128, 128, 2, 2, 2>(L, a, entries);
-    else if (each > 16 || start) few_launch<2>(L, a, entries);
-    else few_launch<1>(L, a, entries);
+    const u32 n = start ? (u32)n_slots : (u32)n_cols;
+    const auto up = [](u32 x, u32 y) { return (x + y - 1) / y; };
+    const auto tiles = [&](u32 bt, u32 br) { return (uint64_t)up(n, bt) * up(a.rows, br); };
+    // the tiles' offsets of gathered columns are 32 bits
+    const bool reach = !order || (uint64_t)n_cols * a.kp <= 0xffffffffu;
+    if (start && reach && n > 16) {
+        const u32 each = n / (u32)n_experts;
+        if (each >= 512) tile_launch<256, 256, 4, 2, 2, 2>(L, a, n);
+        else if (each >= 96) tile_launch<128, 128, 2, 2, 2, 2>(L, a, n);
+        else if (each >= 12) tile_launch<64, 128, 1, 4, 2, 2>(L, a, n);
+        else tile_launch<32, 64, 1, 2, 2, 2>(L, a, n);
+        return hipGetLastError();
+    }
+    if (!start && n > 32 && tiles(32, 64) >= 96) {
+        if (tiles(256, 256) >= 96) {
+            const uint64_t by256 = 64 * ((tiles(256, 256) + 255) / 256), by224 = 57 * ((tiles(256, 224) + 255) / 256), by128 = 39 * ((tiles(128, 128) + 511) / 512);
+            if (by256 <= by224 && by256 <= by128) tile_launch<256, 256, 4, 2, 2, 2>(L, a, n);
+            else if (by224 <= by128) tile_launch<256, 224, 4, 2, 2, 2>(L, a, n);
+            else tile_launch<128, 128, 2, 2, 2, 2>(L, a, n);
+        } else if (tiles(128, 128) >= 320) tile_launch<128, 128, 2, 2, 2, 2>(L, a, n);
+        else if (tiles(64, 128) >= 256) tile_launch<64, 128, 1, 4, 2, 2>(L, a, n);
+        else if (tiles(64, 64) >= 192) tile_launch<64, 64, 2, 2, 4, 2>(L, a, n);
+        else tile_launch<32, 64, 1, 2, 4, 2>(L, a, n);
+        return hipGetLastError();
+    }
+    const bool wide = (start ? (uint64_t)(n < (u32)n_experts ? n : (u32)n_experts) : 1) * up(a.rows, 16) >= 320;
+    if (n <= 16 || start) {
+        if (wide) few_launch<2, 1, 4, 4>(L, a, n);
+        else few_launch<1, 1, 8, 2>(L, a, n);
+    } else {
+        if (wide && n <= 32) few_launch<2, 2, 4, 4>(L, a, n);
+        else few_launch<1, 2, 8, 2>(L, a, n);
+    }
     return hipGetLastError();
 }
 
