@@ -30,21 +30,40 @@ struct SortArgs {
     u32 *fault, layer;
 };
 
-// A token's row to the places of its slots in LDS (kUnlisted: not stored). EB: bytes of an element.
-template <int EB>
-__device__ __forceinline__ void move_row(const SortArgs &a, u32 token, const u32 *places) {
+// A token's row to the places of its slots in LDS (kUnlisted: not stored). EB: bytes of an element. The row's first pieces are asked for before
+// the places are known (row_ahead): the two latencies run side by side.
+constexpr u32 kRowAhead = 2;
+struct RowAhead {
+    uint4 v[kRowAhead];
+};
+__device__ __forceinline__ RowAhead row_ahead(const SortArgs &a, u32 token) {
+    RowAhead r;
     const uint8_t *from = a.x + (size_t)token * a.x_line;
-    for (u32 at = 16 * threadIdx.x; at < a.row_bytes; at += 16 * kRowThreads) {
-        if (at + 16 <= a.row_bytes) {
-            const uint4 v = bm_ld16u(from + at);
-            for (u32 k = 0; k < a.top_k; k++)
-                if (places[k] != kUnlisted) __builtin_memcpy(a.rows + (size_t)places[k] * a.rows_line + at, &v, 16);
-        } else {
-            for (u32 b = at; b < a.row_bytes; b += EB)
-                for (u32 k = 0; k < a.top_k; k++)
-                    if (places[k] != kUnlisted) __builtin_memcpy(a.rows + (size_t)places[k] * a.rows_line + b, from + b, EB);
-        }
+#pragma unroll
+    for (u32 i = 0; i < kRowAhead; i++) {
+        const u32 at = 16 * (threadIdx.x + i * kRowThreads);
+        if (at + 16 <= a.row_bytes) r.v[i] = bm_ld16u(from + at);
     }
+    return r;
+}
+template <int EB>
+__device__ __forceinline__ void move_row(const SortArgs &a, u32 token, const u32 *places, const RowAhead &ahead) {
+    const uint8_t *from = a.x + (size_t)token * a.x_line;
+    const auto piece = [&](u32 at, uint4 v) {
+        for (u32 k = 0; k < a.top_k; k++)
+            if (places[k] != kUnlisted) __builtin_memcpy(a.rows + (size_t)places[k] * a.rows_line + at, &v, 16);
+    };
+#pragma unroll
+    for (u32 i = 0; i < kRowAhead; i++) {
+        const u32 at = 16 * (threadIdx.x + i * kRowThreads);
+        if (at + 16 <= a.row_bytes) piece(at, ahead.v[i]);
+    }
+    for (u32 at = 16 * (threadIdx.x + kRowAhead * kRowThreads); at + 16 <= a.row_bytes; at += 16 * kRowThreads) piece(at, bm_ld16u(from + at));
+    // what is left of a row that is no whole number of pieces, an element a thread
+    const u32 b = (a.row_bytes & ~15u) + EB * threadIdx.x;
+    if (b < a.row_bytes)
+        for (u32 k = 0; k < a.top_k; k++)
+            if (places[k] != kUnlisted) __builtin_memcpy(a.rows + (size_t)places[k] * a.rows_line + b, from + b, EB);
 }
 
 // The whole sort in one launch: a workgroup a token finds its slots' places by counting what stands in front of them among all
@@ -84,6 +103,8 @@ __global__ __launch_bounds__(kRowThreads) void k_sort_few(SortArgs a) {
         return;
     }
     const u32 token = blockIdx.x, s0 = token * a.top_k;
+    RowAhead ahead;
+    if (a.x) ahead = row_ahead(a, token);
     for (u32 k = tid; k < a.top_k; k += kRowThreads) places[k] = 0;
     __syncthreads();
     for (u32 k0 = 0; k0 < a.top_k; k0 += 8) {
@@ -113,15 +134,16 @@ __global__ __launch_bounds__(kRowThreads) void k_sort_few(SortArgs a) {
     }
     if (!a.x) return;
     __syncthreads();
-    move_row<EB>(a, token, places);
+    move_row<EB>(a, token, places, ahead);
 }
 
 // ---- many slots, in three launches over chunks of slots, a wave each.
-// 1. A chunk's counts an expert into work[chunk * n_experts ..], and every slot's rank among its chunk's slots of its expert into
-//    place (the slots of a wave that share an expert find each other bit by bit of the id).
+// 1. A chunk's counts an expert into work[expert * chunks + chunk], and every slot's rank among its chunk's slots of its expert into
+//    place (the slots of a wave that share an expert find each other bit by bit of the id). Eight ids a lane are asked for at once.
+constexpr u32 kSortAhead = 8;
 __host__ __device__ inline u32 sort_chunk_len(u32 n) {
     const u32 per = (n + 255) / 256; // at most 256 chunks
-    return per < 512 ? 512 : (per + 63) & ~63u;
+    return per < 64 * kSortAhead ? 64 * kSortAhead : (per + 63) & ~63u;
 }
 
 __global__ __launch_bounds__(64) void k_sort_count(SortArgs a, u32 n, u32 per) {
@@ -130,64 +152,87 @@ __global__ __launch_bounds__(64) void k_sort_count(SortArgs a, u32 n, u32 per) {
     for (u32 e = lane; e < a.n_experts; e += 64) count[e] = 0;
     __syncthreads();
     const int bits = 32 - __builtin_clz(a.n_experts | 1u);
-    for (u32 b = lo; b < hi; b += 64) {
-        const u32 s = b + lane, id = s < hi ? a.sel[s] : kUnlisted;
-        const bool listed = id < a.n_experts;
-        if (!listed && id != kUnlisted) bm_raise(a.fault, a.layer, kSiteExpertId);
-        unsigned long long same = __ballot(listed);
-        for (int k = 0; k < bits; k++) {
-            const unsigned long long set = __ballot((id >> k) & 1u);
-            same &= ((id >> k) & 1u) ? set : ~set;
+    for (u32 b = lo; b < hi; b += 64 * kSortAhead) {
+        u32 ids[kSortAhead];
+#pragma unroll
+        for (u32 i = 0; i < kSortAhead; i++) ids[i] = b + 64 * i + lane < hi ? a.sel[b + 64 * i + lane] : kUnlisted;
+#pragma unroll
+        for (u32 i = 0; i < kSortAhead; i++) {
+            const u32 s = b + 64 * i + lane, id = ids[i];
+            const bool listed = id < a.n_experts;
+            if (!listed && id != kUnlisted) bm_raise(a.fault, a.layer, kSiteExpertId);
+            unsigned long long same = __ballot(listed);
+            for (int k = 0; k < bits; k++) {
+                const unsigned long long set = __ballot((id >> k) & 1u);
+                same &= ((id >> k) & 1u) ? set : ~set;
+            }
+            const u32 below = (u32)__builtin_popcountll(same & ((1ull << lane) - 1ull));
+            const u32 had = listed ? count[id] : 0; // every lane of the wave reads before the first of a group adds
+            if (listed && below == 0) count[id] = had + (u32)__builtin_popcountll(same);
+            if (s < hi) a.place[s] = listed ? had + below : kUnlisted;
+            __syncthreads();
         }
-        const u32 below = (u32)__builtin_popcountll(same & ((1ull << lane) - 1ull));
-        const u32 had = listed ? count[id] : 0; // every lane of the wave reads before the first of a group adds
-        if (listed && below == 0) count[id] = had + (u32)__builtin_popcountll(same);
-        if (s < hi) a.place[s] = listed ? had + below : kUnlisted;
-        __syncthreads();
     }
-    for (u32 e = lane; e < a.n_experts; e += 64) a.work[(size_t)blockIdx.x * a.n_experts + e] = count[e];
+    for (u32 e = lane; e < a.n_experts; e += 64) a.work[(size_t)e * gridDim.x + blockIdx.x] = count[e];
 }
 
-// 2. The counts' running sums over chunks inside an expert, behind the experts' own: work becomes the place of a chunk's first slot.
+// 2. An expert's counts become their running sums over the chunks, a wave an expert; the experts' own running sums are the runs' bounds.
 __global__ __launch_bounds__(1024) void k_sort_scan(SortArgs a, u32 chunks) {
-    __shared__ u32 scan[17];
-    const u32 e = threadIdx.x;
-    u32 sum = 0;
-    if (e < a.n_experts)
-        for (u32 c = 0; c < chunks; c++) sum += a.work[(size_t)c * a.n_experts + e];
-    u32 total;
-    u32 at = block_scan_1024(sum, scan, &total);
-    if (e < a.n_experts) {
-        a.start[e] = at;
-        for (u32 c = 0; c < chunks; c++) {
-            const u32 v = a.work[(size_t)c * a.n_experts + e];
-            a.work[(size_t)c * a.n_experts + e] = at;
-            at += v;
+    __shared__ u32 scan[17], count[kBucketExperts];
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (u32 e0 = wave; e0 < a.n_experts; e0 += 16 * 8) { // eight experts of a wave's at a time, asked for together
+        u32 had[8];
+#pragma unroll
+        for (u32 i = 0; i < 8; i++) had[i] = 0;
+        for (u32 c0 = 0; c0 < chunks; c0 += 64) {
+            const u32 c = c0 + lane;
+            u32 v[8];
+#pragma unroll
+            for (u32 i = 0; i < 8; i++) v[i] = e0 + 16 * i < a.n_experts && c < chunks ? a.work[(size_t)(e0 + 16 * i) * chunks + c] : 0;
+#pragma unroll
+            for (u32 i = 0; i < 8; i++) {
+                u32 upto = v[i];
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const u32 o = (u32)__shfl_up((int)upto, d, 64);
+                    if (lane >= (u32)d) upto += o;
+                }
+                if (e0 + 16 * i < a.n_experts && c < chunks) a.work[(size_t)(e0 + 16 * i) * chunks + c] = had[i] + upto - v[i];
+                had[i] += (u32)__shfl((int)upto, 63, 64);
+            }
         }
+#pragma unroll
+        for (u32 i = 0; i < 8; i++)
+            if (lane == 0 && e0 + 16 * i < a.n_experts) count[e0 + 16 * i] = had[i];
     }
-    if (e == 0) a.start[a.n_experts] = total;
+    __syncthreads();
+    u32 total;
+    const u32 at = block_scan_1024(tid < a.n_experts ? count[tid] : 0, scan, &total);
+    if (tid < a.n_experts) a.start[tid] = at;
+    if (tid == 0) a.start[a.n_experts] = total;
 }
 
 // 3. Places and order of a token's slots, and its row to them.
-__device__ __forceinline__ u32 sort_settle(const SortArgs &a, u32 s, u32 per) {
-    const u32 id = a.sel[s];
+__device__ __forceinline__ u32 sort_settle(const SortArgs &a, u32 s, u32 per, u32 chunks) {
+    const u32 id = a.sel[s], rank = a.place[s];
     if (id >= a.n_experts) return kUnlisted; // place holds kUnlisted already
-    const u32 p = a.work[(size_t)(s / per) * a.n_experts + id] + a.place[s];
+    const u32 p = a.start[id] + a.work[(size_t)id * chunks + s / per] + rank;
     a.place[s] = p;
     a.order[p] = s;
     return p;
 }
 template <int EB>
-__global__ __launch_bounds__(kRowThreads) void k_sort_move(SortArgs a, u32 per) {
+__global__ __launch_bounds__(kRowThreads) void k_sort_move(SortArgs a, u32 per, u32 chunks) {
     __shared__ u32 places[kMaxCombineSlots];
     const u32 token = blockIdx.x;
-    if (threadIdx.x < a.top_k) places[threadIdx.x] = sort_settle(a, token * a.top_k + threadIdx.x, per);
+    const RowAhead ahead = row_ahead(a, token);
+    if (threadIdx.x < a.top_k) places[threadIdx.x] = sort_settle(a, token * a.top_k + threadIdx.x, per, chunks);
     __syncthreads();
-    move_row<EB>(a, token, places);
+    move_row<EB>(a, token, places, ahead);
 }
-__global__ __launch_bounds__(kRowThreads) void k_sort_places(SortArgs a, u32 n, u32 per) {
+__global__ __launch_bounds__(kRowThreads) void k_sort_places(SortArgs a, u32 n, u32 per, u32 chunks) {
     const u32 s = blockIdx.x * kRowThreads + threadIdx.x;
-    if (s < n) sort_settle(a, s, per);
+    if (s < n) sort_settle(a, s, per, chunks);
 }
 
 size_t expert_sort_work(int n_slots, int n_experts) {
@@ -210,9 +255,9 @@ hipError_t expert_sort(const Launch &L, const uint32_t *sel, int n_tokens, int t
     const u32 per = sort_chunk_len(n), chunks = (n + per - 1) / per;
     hipLaunchKernelGGL(k_sort_count, dim3(chunks), dim3(64), 0, L.stream, a, n, per);
     hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, L.stream, a, chunks);
-    if (!x) hipLaunchKernelGGL(k_sort_places, dim3((n + kRowThreads - 1) / kRowThreads), dim3(kRowThreads), 0, L.stream, a, n, per);
-    else if (eb == 4) hipLaunchKernelGGL(k_sort_move<4>, dim3((unsigned)n_tokens), dim3(kRowThreads), 0, L.stream, a, per);
-    else hipLaunchKernelGGL(k_sort_move<2>, dim3((unsigned)n_tokens), dim3(kRowThreads), 0, L.stream, a, per);
+    if (!x) hipLaunchKernelGGL(k_sort_places, dim3((n + kRowThreads - 1) / kRowThreads), dim3(kRowThreads), 0, L.stream, a, n, per, chunks);
+    else if (eb == 4) hipLaunchKernelGGL(k_sort_move<4>, dim3((unsigned)n_tokens), dim3(kRowThreads), 0, L.stream, a, per, chunks);
+    else hipLaunchKernelGGL(k_sort_move<2>, dim3((unsigned)n_tokens), dim3(kRowThreads), 0, L.stream, a, per, chunks);
     return hipGetLastError();
 }
 
@@ -238,44 +283,88 @@ __device__ __forceinline__ u32 checked_place(u32 p, u32 n_slots, u32 *fault, u32
     return kUnlisted;
 }
 
-// y[t] = (acc = 0; slots ascending: acc = fma(w, row, acc)) + resid[t], in f32 and rounded once: bm_combine_tokens' order. A thread holds
-// eight values of a token (1 << log threads a token, several tokens a workgroup where rows are short); its slots' places, weights
-// and rows are asked for eight slots at a time, so that a row's latency is paid once for all of them.
-template <int ET>
-__global__ __launch_bounds__(kRowThreads) void k_expert_combine(CombineArgs a, u32 log) {
-    const u32 t = blockIdx.x * (kRowThreads >> log) + (threadIdx.x >> log);
-    if (t >= a.n_tokens) return;
-    for (u32 c = 8 * (threadIdx.x & ((1u << log) - 1u)); c < a.width; c += 8u << log) {
-        const u32 have = a.width - c;
-        float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, r[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (a.resid) elem_load_some<ET, 8>(a.resid, (size_t)t * a.ld_resid + c, have, r);
-        for (u32 k0 = 0; k0 < a.top_k; k0 += 8) {
-            u32 p[8];
-            float w[8], v[8][8];
+// A batch of eight slots' places and weights. A slot that is not listed (or past the token's last) is read through the place of one that is, or the
+// first row, and what comes is not used: its request is answered by the cache, and no branch parts the eight.
+struct Slots8 {
+    u32 p[8];
+    float w[8];
+    bool on[8];
+};
+__device__ __forceinline__ Slots8 slots8(const u32 *place, const float *w, size_t s0, u32 have, u32 n_slots, u32 *fault, u32 layer) {
+    Slots8 r;
 #pragma unroll
-            for (u32 k = 0; k < 8; k++) {
-                const u32 s = t * a.top_k + (k0 + k < a.top_k ? k0 + k : k0);
-                p[k] = k0 + k < a.top_k ? a.place[s] : kUnlisted;
-                w[k] = a.w ? a.w[s] : 1.0f;
-            }
-#pragma unroll
-            for (u32 k = 0; k < 8; k++) {
-                p[k] = checked_place(p[k], a.n_slots, a.fault, a.layer);
-                if (p[k] != kUnlisted) elem_load_some<ET, 8>(a.rows, (size_t)p[k] * a.ld_rows + c, have, v[k]);
-                else
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[k][j] = 0.0f;
-            }
-#pragma unroll
-            for (u32 k = 0; k < 8; k++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) acc[j] = p[k] != kUnlisted ? fmaf(w[k], v[k][j], acc[j]) : acc[j];
-        }
-        if (a.resid)
-#pragma unroll
-            for (int j = 0; j < 8; j++) acc[j] = __fadd_rn(acc[j], r[j]);
-        elem_store_some<ET, 8>(a.y, (size_t)t * a.ld_y + c, have, acc);
+    for (u32 k = 0; k < 8; k++) {
+        const size_t s = s0 + (k < have ? k : 0);
+        r.p[k] = k < have ? place[s] : kUnlisted;
+        r.w[k] = w ? w[s] : 1.0f;
     }
+    u32 some = 0;
+#pragma unroll
+    for (u32 k = 0; k < 8; k++) {
+        r.p[k] = checked_place(r.p[k], n_slots, fault, layer);
+        r.on[k] = r.p[k] != kUnlisted;
+        some = r.on[k] ? r.p[k] : some;
+    }
+#pragma unroll
+    for (u32 k = 0; k < 8; k++) r.p[k] = r.on[k] ? r.p[k] : some;
+    return r;
+}
+
+// y[t] = (acc = 0; slots ascending: acc = fma(w, row, acc)) + resid[t], in f32 and rounded once: bm_combine_tokens' order. A thread holds a
+// 16-byte piece of a token (1 << log threads a token, several tokens a workgroup where rows are short); its slots' rows are asked for eight
+// at a time, so that a row's latency is paid once for all of them. What is left of a row that is no whole number of pieces goes an element a thread.
+template <int ET>
+__device__ __forceinline__ void combine_piece(const CombineArgs &a, const Slots8 &s, u32 c, float (&acc)[kElemPiece<ET>]) {
+    uint4 v[8];
+#pragma unroll
+    for (u32 k = 0; k < 8; k++) v[k] = elem_piece<ET>(a.rows, (size_t)s.p[k] * a.ld_rows + c);
+#pragma unroll
+    for (u32 k = 0; k < 8; k++) {
+        float f[kElemPiece<ET>];
+        elem_unpack<ET>(v[k], f);
+#pragma unroll
+        for (int j = 0; j < kElemPiece<ET>; j++) acc[j] = s.on[k] ? fmaf(s.w[k], f[j], acc[j]) : acc[j];
+    }
+}
+template <int ET, bool EIGHT> // EIGHT: at most eight slots a token, whose places a thread keeps
+__global__ __launch_bounds__(kRowThreads) void k_expert_combine(CombineArgs a, u32 log) {
+    constexpr int V = kElemPiece<ET>;
+    const u32 t = blockIdx.x * (kRowThreads >> log) + (threadIdx.x >> log), mine = threadIdx.x & ((1u << log) - 1u);
+    if (t >= a.n_tokens) return;
+    const size_t s0 = (size_t)t * a.top_k;
+    Slots8 s;
+    if constexpr (EIGHT) s = slots8(a.place, a.w, s0, a.top_k, a.n_slots, a.fault, a.layer);
+    for (u32 c = V * mine; c + V <= a.width; c += V << log) {
+        float acc[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) acc[j] = 0.0f;
+        uint4 r;
+        if (a.resid) r = elem_piece<ET>(a.resid, (size_t)t * a.ld_resid + c);
+        if constexpr (EIGHT) {
+            combine_piece<ET>(a, s, c, acc);
+        } else {
+            for (u32 k0 = 0; k0 < a.top_k; k0 += 8) {
+                s = slots8(a.place, a.w, s0 + k0, a.top_k - k0, a.n_slots, a.fault, a.layer);
+                combine_piece<ET>(a, s, c, acc);
+            }
+        }
+        if (a.resid) {
+            float f[V];
+            elem_unpack<ET>(r, f);
+#pragma unroll
+            for (int j = 0; j < V; j++) acc[j] = __fadd_rn(acc[j], f[j]);
+        }
+        elem_piece_store<ET>(a.y, (size_t)t * a.ld_y + c, elem_pack<ET>(acc));
+    }
+    const u32 c = a.width / V * V + mine; // (1 << log is V at least)
+    if (c >= a.width) return;
+    float acc = 0.0f;
+    for (u32 k = 0; k < a.top_k; k++) {
+        const u32 p = checked_place(a.place[s0 + k], a.n_slots, a.fault, a.layer);
+        if (p != kUnlisted) acc = fmaf(a.w ? a.w[s0 + k] : 1.0f, elem_load1<ET>(a.rows, (size_t)p * a.ld_rows + c), acc);
+    }
+    if (a.resid) acc = __fadd_rn(acc, elem_load1<ET>(a.resid, (size_t)t * a.ld_resid + c));
+    elem_store1<ET>(a.y, (size_t)t * a.ld_y + c, acc);
 }
 
 struct CombineGradArgs {
@@ -297,40 +386,44 @@ struct CombineGradArgs {
 // four waves.
 template <int ET>
 __global__ __launch_bounds__(kRowThreads) void k_expert_combine_grad(CombineGradArgs a) {
+    constexpr int V = kElemPiece<ET>;
     __shared__ float part[4][8];
     const u32 t = blockIdx.x, tid = threadIdx.x;
     for (u32 k0 = 0; k0 < a.top_k; k0 += 8) {
-        u32 p[8];
-        float w[8], dot[8];
+        const Slots8 s = slots8(a.place, a.w, (size_t)t * a.top_k + k0, a.top_k - k0, a.n_slots, a.fault, a.layer);
+        float dot[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        for (u32 c = V * tid; c + V <= a.width; c += V * kRowThreads) {
+            uint4 v[8];
+            const uint4 gp = elem_piece<ET>(a.dy, (size_t)t * a.ld_dy + c);
 #pragma unroll
-        for (u32 k = 0; k < 8; k++) {
-            const u32 s = t * a.top_k + (k0 + k < a.top_k ? k0 + k : k0);
-            p[k] = k0 + k < a.top_k ? checked_place(a.place[s], a.n_slots, a.fault, a.layer) : kUnlisted;
-            w[k] = a.w[s];
-            dot[k] = 0.0f;
+            for (u32 k = 0; k < 8; k++) v[k] = elem_piece<ET>(a.rows, (size_t)s.p[k] * a.ld_rows + c);
+            float g[V];
+            elem_unpack<ET>(gp, g);
+#pragma unroll
+            for (u32 k = 0; k < 8; k++) {
+                float f[V], d[V];
+                elem_unpack<ET>(v[k], f);
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    dot[k] = fmaf(g[j], f[j], dot[k]);
+                    d[j] = __fmul_rn(s.w[k], g[j]);
+                }
+                if (s.on[k]) elem_piece_store<ET>(a.d_rows, (size_t)s.p[k] * a.ld_d_rows + c, elem_pack<ET>(d));
+            }
         }
-        for (u32 c = 8 * tid; c < a.width; c += 8 * kRowThreads) {
-            const u32 have = a.width - c;
-            float g[8], v[8][8];
-            elem_load_some<ET, 8>(a.dy, (size_t)t * a.ld_dy + c, have, g);
+        const u32 c = a.width / V * V + tid;
+        if (c < a.width) {
+            const float g = elem_load1<ET>(a.dy, (size_t)t * a.ld_dy + c);
 #pragma unroll
             for (u32 k = 0; k < 8; k++)
-                if (p[k] != kUnlisted) elem_load_some<ET, 8>(a.rows, (size_t)p[k] * a.ld_rows + c, have, v[k]);
-#pragma unroll
-            for (u32 k = 0; k < 8; k++)
-                if (p[k] != kUnlisted) {
-                    float d[8];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        dot[k] = fmaf(g[j], v[k][j], dot[k]);
-                        d[j] = __fmul_rn(w[k], g[j]);
-                    }
-                    elem_store_some<ET, 8>(a.d_rows, (size_t)p[k] * a.ld_d_rows + c, have, d);
+                if (s.on[k]) {
+                    dot[k] = fmaf(g, elem_load1<ET>(a.rows, (size_t)s.p[k] * a.ld_rows + c), dot[k]);
+                    elem_store1<ET>(a.d_rows, (size_t)s.p[k] * a.ld_d_rows + c, __fmul_rn(s.w[k], g));
                 }
         }
 #pragma unroll
         for (u32 k = 0; k < 8; k++) {
-            const float sum = wave_sum(dot[k]);
+            const float sum = wave_sum(s.on[k] ? dot[k] : 0.0f);
             if ((tid & 63) == 0) part[tid >> 6][k] = sum;
         }
         __syncthreads();
@@ -342,11 +435,13 @@ __global__ __launch_bounds__(kRowThreads) void k_expert_combine_grad(CombineGrad
 
 template <int ET>
 static void combine_launch(const Launch &L, const CombineArgs &a) {
-    const u32 pieces = (a.width + 7) / 8;
+    const u32 pieces = a.width / kElemPiece<ET>;
     u32 log = 3;
     while (log < 8 && (1u << log) < pieces) log++;
     const u32 tokens = kRowThreads >> log;
-    hipLaunchKernelGGL(k_expert_combine<ET>, dim3((a.n_tokens + tokens - 1) / tokens), dim3(kRowThreads), 0, L.stream, a, log);
+    const dim3 grid((a.n_tokens + tokens - 1) / tokens), block(kRowThreads);
+    if (a.top_k <= 8) hipLaunchKernelGGL((k_expert_combine<ET, true>), grid, block, 0, L.stream, a, log);
+    else hipLaunchKernelGGL((k_expert_combine<ET, false>), grid, block, 0, L.stream, a, log);
 }
 
 hipError_t expert_combine(const Launch &L, const void *rows, int et, int64_t ld_rows, const uint32_t *place, const float *w, const void *resid,
