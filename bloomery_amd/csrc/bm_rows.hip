@@ -139,46 +139,64 @@ __global__ __launch_bounds__(kRowThreads) void k_sort_few(SortArgs a) {
 
 // ---- many slots, in three launches over chunks of slots, a wave each.
 // 1. A chunk's counts an expert into work[expert * chunks + chunk], and every slot's rank among its chunk's slots of its expert into
-//    place (the slots of a wave that share an expert find each other bit by bit of the id). Eight ids a lane are asked for at once.
-constexpr u32 kSortAhead = 8;
+//    place. Eight waves share a chunk, an eighth each with counts of its own: the slots of a wave that share an expert find each other bit
+//    by bit of the id, and an expert's counts are summed over the waves in front. (One wave a chunk of 512 took 6.2 us where this takes 4.)
+constexpr u32 kSortWaves = 8;
 __host__ __device__ inline u32 sort_chunk_len(u32 n) {
-    const u32 per = (n + 255) / 256; // at most 256 chunks
-    return per < 64 * kSortAhead ? 64 * kSortAhead : (per + 63) & ~63u;
+    const u32 per = (n + 255) / 256, least = 64 * kSortWaves; // at most 256 chunks
+    return (per + least - 1) / least * least;
 }
 
-__global__ __launch_bounds__(64) void k_sort_count(SortArgs a, u32 n, u32 per) {
-    __shared__ u32 count[kBucketExperts];
-    const u32 lane = threadIdx.x, lo = blockIdx.x * per, hi = lo + per < n ? lo + per : n;
-    for (u32 e = lane; e < a.n_experts; e += 64) count[e] = 0;
+__global__ __launch_bounds__(64 * kSortWaves) void k_sort_count(SortArgs a, u32 n, u32 per) {
+    __shared__ u32 count[kSortWaves * kBucketExperts];
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, share = per / kSortWaves;
+    const u32 lo = blockIdx.x * per + wave * share, hi = min(lo + share, n);
+    u32 id = lo + lane < hi ? a.sel[lo + lane] : kUnlisted; // the first 64 slots' ids come while the counts are cleared
+    for (u32 i = tid; i < kSortWaves * a.n_experts; i += 64 * kSortWaves) count[i] = 0;
     __syncthreads();
+    u32 *mine = count + wave * a.n_experts;
     const int bits = 32 - __builtin_clz(a.n_experts | 1u);
-    for (u32 b = lo; b < hi; b += 64 * kSortAhead) {
-        u32 ids[kSortAhead];
-#pragma unroll
-        for (u32 i = 0; i < kSortAhead; i++) ids[i] = b + 64 * i + lane < hi ? a.sel[b + 64 * i + lane] : kUnlisted;
-#pragma unroll
-        for (u32 i = 0; i < kSortAhead; i++) {
-            const u32 s = b + 64 * i + lane, id = ids[i];
-            const bool listed = id < a.n_experts;
-            if (!listed && id != kUnlisted) bm_raise(a.fault, a.layer, kSiteExpertId);
-            unsigned long long same = __ballot(listed);
-            for (int k = 0; k < bits; k++) {
-                const unsigned long long set = __ballot((id >> k) & 1u);
-                same &= ((id >> k) & 1u) ? set : ~set;
-            }
-            const u32 below = (u32)__builtin_popcountll(same & ((1ull << lane) - 1ull));
-            const u32 had = listed ? count[id] : 0; // every lane of the wave reads before the first of a group adds
-            if (listed && below == 0) count[id] = had + (u32)__builtin_popcountll(same);
-            if (s < hi) a.place[s] = listed ? had + below : kUnlisted;
-            __syncthreads();
+    u32 first = 0; // the rank of the only slot a lane has where a wave has 64 at most
+    for (u32 b = lo; b < hi; b += 64) {
+        const u32 s = b + lane;
+        if (b != lo) id = s < hi ? a.sel[s] : kUnlisted;
+        const bool listed = id < a.n_experts;
+        if (!listed && id != kUnlisted) bm_raise(a.fault, a.layer, kSiteExpertId);
+        unsigned long long same = __ballot(listed);
+        for (int k = 0; k < bits; k++) {
+            const unsigned long long set = __ballot((id >> k) & 1u);
+            same &= ((id >> k) & 1u) ? set : ~set;
         }
+        const u32 below = (u32)__builtin_popcountll(same & ((1ull << lane) - 1ull));
+        const u32 had = listed ? mine[id] : 0; // every lane of the wave reads before the first of a group adds
+        if (listed && below == 0) mine[id] = had + (u32)__builtin_popcountll(same);
+        first = had + below;
+        if (share > 64 && s < hi) a.place[s] = first;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    for (u32 e = lane; e < a.n_experts; e += 64) a.work[(size_t)e * gridDim.x + blockIdx.x] = count[e];
+    __syncthreads();
+    for (u32 e = tid; e < a.n_experts; e += 64 * kSortWaves) { // counts -> what the waves in front hold
+        u32 sum = 0;
+#pragma unroll
+        for (u32 w = 0; w < kSortWaves; w++) {
+            const u32 c = count[w * a.n_experts + e];
+            count[w * a.n_experts + e] = sum;
+            sum += c;
+        }
+        a.work[(size_t)e * gridDim.x + blockIdx.x] = sum;
+    }
+    __syncthreads();
+    for (u32 b = lo; b < hi; b += 64) {
+        const u32 s = b + lane;
+        if (s >= hi) break;
+        if (share > 64) id = a.sel[s], first = a.place[s];
+        a.place[s] = id < a.n_experts ? mine[id] + first : kUnlisted;
+    }
 }
 
 // 2. An expert's counts become their running sums over the chunks, a wave an expert; the experts' own running sums are the runs' bounds.
 __global__ __launch_bounds__(1024) void k_sort_scan(SortArgs a, u32 chunks) {
-    __shared__ u32 scan[17], count[kBucketExperts];
+    __shared__ u32 scan[16], count[kBucketExperts];
     const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (u32 e0 = wave; e0 < a.n_experts; e0 += 16 * 8) { // eight experts of a wave's at a time, asked for together
         u32 had[8];
@@ -206,10 +224,20 @@ __global__ __launch_bounds__(1024) void k_sort_scan(SortArgs a, u32 chunks) {
             if (lane == 0 && e0 + 16 * i < a.n_experts) count[e0 + 16 * i] = had[i];
     }
     __syncthreads();
-    u32 total;
-    const u32 at = block_scan_1024(tid < a.n_experts ? count[tid] : 0, scan, &total);
-    if (tid < a.n_experts) a.start[tid] = at;
-    if (tid == 0) a.start[a.n_experts] = total;
+    const u32 c = tid < a.n_experts ? count[tid] : 0;
+    u32 upto = c;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const u32 o = (u32)__shfl_up((int)upto, d, 64);
+        if (lane >= (u32)d) upto += o;
+    }
+    if (lane == 63) scan[wave] = upto;
+    __syncthreads();
+    u32 before = 0;
+#pragma unroll
+    for (u32 w = 0; w < 16; w++) before += w < wave ? scan[w] : 0;
+    if (tid < a.n_experts) a.start[tid] = before + upto - c;
+    if (tid + 1 == a.n_experts) a.start[a.n_experts] = before + upto;
 }
 
 // 3. Places and order of a token's slots, and its row to them.
@@ -253,7 +281,7 @@ hipError_t expert_sort(const Launch &L, const uint32_t *sel, int n_tokens, int t
         return hipGetLastError();
     }
     const u32 per = sort_chunk_len(n), chunks = (n + per - 1) / per;
-    hipLaunchKernelGGL(k_sort_count, dim3(chunks), dim3(64), 0, L.stream, a, n, per);
+    hipLaunchKernelGGL(k_sort_count, dim3(chunks), dim3(64 * kSortWaves), 0, L.stream, a, n, per);
     hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, L.stream, a, chunks);
     if (!x) hipLaunchKernelGGL(k_sort_places, dim3((n + kRowThreads - 1) / kRowThreads), dim3(kRowThreads), 0, L.stream, a, n, per, chunks);
     else if (eb == 4) hipLaunchKernelGGL(k_sort_move<4>, dim3((unsigned)n_tokens), dim3(kRowThreads), 0, L.stream, a, per, chunks);
