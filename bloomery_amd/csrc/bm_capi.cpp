@@ -1605,9 +1605,8 @@ int bm_i8_gemm_x(bm_ctx *ctx, const int8_t *w_dev, const float *w_scales_dev, in
     BM_TRY(check_rows(ctx, what, "y_dev", y_dev, y_type, rows, ld_y));
     if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
     DeviceScope on(ctx->device);
-    const bmk::Launch L = launch_of(ctx);
-    BM_TRY(driver(ctx, what, bmk::i8_quantize(L, x_dev, nullptr, x_type, ld_x, m, k, nullptr, codes_dev, scales_dev)));
-    return driver(ctx, what, bmk::i8_gemm(L, w_dev, w_scales_dev, 1, rows, k, codes_dev, scales_dev, m, nullptr, nullptr, 0, 0, y_dev, y_type, ld_y));
+    return driver(ctx, what, bmk::i8_gemm_x(launch_of(ctx), w_dev, w_scales_dev, rows, k, x_dev, x_type, ld_x, m, codes_dev, scales_dev, y_dev,
+                                            y_type, ld_y));
 }
 
 int bm_i8_gemm_experts(bm_ctx *ctx, const int8_t *w_dev, const float *w_scales_dev, int n_experts, int rows_per_expert, int k,

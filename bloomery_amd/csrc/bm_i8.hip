@@ -27,6 +27,28 @@ __device__ __forceinline__ int i8_code(float v, float s, float inv) {
     return (int)fminf(fmaxf(n, -127.0f), 127.0f);
 }
 
+// A row's scale from the bits of its largest magnitude (positive floats order as their bits; infinities and NaN lie on top).
+struct I8Scale {
+    float s, up, su, inv; // small scales, whose reciprocal could overflow, go up by 2^100 with their values (exactly)
+    bool bad, zero;
+};
+__device__ __forceinline__ I8Scale i8_scale(u32 most) {
+    I8Scale r;
+    r.bad = most >= 0x7f800000u;
+    r.s = r.bad ? bm_bits_f32(0x7fc00000u) : __fdiv_rn(bm_bits_f32(most), 127.0f);
+    r.up = r.s < 0x1p-64f ? 0x1p100f : 1.0f;
+    r.su = r.s * r.up;
+    r.inv = __fdiv_rn(1.0f, r.su);
+    r.zero = r.bad || r.s == 0.0f;
+    return r;
+}
+__device__ __forceinline__ uint2 i8_codes(const float (&v)[8], const I8Scale &s) {
+    u32 word[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; j++) word[j / 4] |= ((u32)(s.zero ? 0 : i8_code(v[j] * s.up, s.su, s.inv)) & 0xffu) << (8 * (j % 4));
+    return make_uint2(word[0], word[1]);
+}
+
 struct QuantArgs {
     const void *x, *u; // u: the second input of a gate rule
     size_t ld;
@@ -99,25 +121,17 @@ __global__ __launch_bounds__(256) void k_i8_quantize(QuantArgs a) {
         __syncthreads();
         most = max(max(top[0], top[1]), max(top[2], top[3]));
     }
-    // positive floats order as their bits; infinities and NaN lie on top
-    const bool bad = most >= 0x7f800000u;
-    const float s = bad ? bm_bits_f32(0x7fc00000u) : __fdiv_rn(bm_bits_f32(most), 127.0f);
+    const I8Scale sc = i8_scale(most);
     if (lane == 0) {
-        a.scales[row] = s;
-        if (bad) bm_raise(a.fault, a.layer, kSiteQuantColumn);
+        a.scales[row] = sc.s;
+        if (sc.bad) bm_raise(a.fault, a.layer, kSiteQuantColumn);
     }
-    // small scales, whose reciprocal could overflow, go up by 2^100 with their values (exactly)
-    const float up = s < 0x1p-64f ? 0x1p100f : 1.0f, su = s * up, inv = __fdiv_rn(1.0f, su);
-    const bool zero = bad || most == 0 || s == 0.0f;
     int8_t *out = a.codes + (size_t)row * a.kp;
 #pragma unroll
     for (int i = 0; i < (CH ? CH : 1); i++)
         for (u32 c = lane + (u32)i * T; c < pieces; c += CH ? pieces : T) {
             if constexpr (CH == 0) quant_values<ET, GLU>(a, row, 8 * c, v[0], odd);
-            u32 word[2] = {0, 0};
-#pragma unroll
-            for (int j = 0; j < 8; j++) word[j / 4] |= ((u32)(zero ? 0 : i8_code(v[i][j] * up, su, inv)) & 0xffu) << (8 * (j % 4));
-            *reinterpret_cast<uint2 *>(out + 8 * c) = make_uint2(word[0], word[1]);
+            *reinterpret_cast<uint2 *>(out + 8 * c) = i8_codes(v[i], sc);
         }
 }
 
@@ -290,6 +304,118 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
             }
         }
         __syncthreads();
+    }
+}
+
+// A few rows from their floating values: k_i8_few's product with the quantizer in front of it in every workgroup, while the first weights are on
+// their way. M (a power of two, at least the rows): the waves are dealt to the rows, 4 pieces of eight values a thread at most. The codes
+// go to LDS; the first workgroup leaves them and the scales in memory too.
+// Ahead of the two launches while a thread has few values to quantize (us, one launch / two, bf16): 768 x 2048, one row 4.9 / 7.5, four 5.6 / 8.0, eight 7.3 /
+// 8.3; 7168 x 2048, one 5.6 / 8.1, four 7.0 / 8.2, eight 9.3 / 8.2; 7168 x 7168, one 11.9 / 17.1, two 14.5 / 17.2; 8192 x 1024, eight 5.8 / 7.9.
+// So: up to four rows of what four pieces a thread hold, eight rows of half that.
+constexpr int kFewX = 8, kFewXWaves = 8; // rows at most
+constexpr u32 few_x_values(u32 M) { return 64 * kFewXWaves * (M < 8 ? 32 : 16) / M; } // values a row may have
+template <int ET, int M, int R, int U>
+__global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArgs qa) {
+    constexpr int NW = kFewXWaves, T = 64 * NW / M; // threads a row
+    extern __shared__ __align__(16) uint8_t few_lds[];
+    int8_t *codes = reinterpret_cast<int8_t *>(few_lds); // M rows of kp
+    __shared__ v4i part[NW][R][64];
+    __shared__ u32 top[NW];
+    __shared__ float scale[M];
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, steps = (a.kp + 63) / 64, r0 = blockIdx.x * (16 * R);
+    const int8_t *wp[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) wp[r] = a.w + (size_t)min(r0 + 16 * r + (lane & 15), a.rows - 1) * a.kp;
+    v4i A[2][U][R];
+    const auto ask = [&](u32 s, v4i (&f)[U][R]) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const u32 at = 64 * (s + u * NW) + 16 * (lane >> 4), off = at < a.kp ? at : 0; // past the row: its first bytes, against zeros
+#pragma unroll
+            for (int r = 0; r < R; r++) f[u][r] = *reinterpret_cast<const v4i *>(wp[r] + off);
+        }
+    };
+    // the rows' values, then the first weights
+    const u32 row = tid / T, mine = tid % T, pieces = a.kp / 8;
+    float v[4][8];
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const u32 c = mine + i * T;
+        if (row < qa.m && c < pieces) quant_values<ET, false>(qa, row, 8 * c, v[i], odd);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[i][j] = 0.0f;
+    }
+    ask(wave, A[0]);
+    u32 most = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) most = max(most, bm_f32_bits(v[i][j]) & 0x7fffffffu);
+    most = bm_max32(most);
+    most = max(most, (u32)__shfl_xor((int)most, 32, 64));
+    if constexpr (M < NW) {
+        if (lane == 0) top[wave] = most;
+        __syncthreads();
+        most = 0;
+#pragma unroll
+        for (int w = 0; w < NW / M; w++) most = max(most, top[row * (NW / M) + w]);
+    }
+    const I8Scale sc = i8_scale(most);
+    if (mine == 0) {
+        scale[row] = sc.s;
+        if (blockIdx.x == 0 && row < qa.m) {
+            qa.scales[row] = sc.s;
+            if (sc.bad) bm_raise(a.fault, a.layer, kSiteQuantColumn);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const u32 c = mine + i * T;
+        if (c >= pieces) break;
+        const uint2 word = i8_codes(v[i], sc);
+        *reinterpret_cast<uint2 *>(codes + row * a.kp + 8 * c) = word;
+        if (blockIdx.x == 0 && row < qa.m) *reinterpret_cast<uint2 *>(qa.codes + (size_t)row * a.kp + 8 * c) = word;
+    }
+    __syncthreads();
+
+    v4i acc[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) acc[r] = v4i{0, 0, 0, 0};
+    const u32 col = lane & 15;
+    const auto multiply = [&](u32 s, const v4i (&f)[U][R]) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const u32 at = 64 * (s + u * NW) + 16 * (lane >> 4);
+            v4i b = v4i{0, 0, 0, 0};
+            if (col < (u32)M && at < a.kp) b = *reinterpret_cast<const v4i *>(codes + col * a.kp + at);
+#pragma unroll
+            for (int r = 0; r < R; r++) acc[r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[u][r], b, acc[r], 0, 0, 0);
+        }
+    };
+    for (u32 s = wave;;) {
+        if (s + U * NW < steps) ask(s + U * NW, A[1]);
+        multiply(s, A[0]);
+        if ((s += U * NW) >= steps) break;
+        if (s + U * NW < steps) ask(s + U * NW, A[0]);
+        multiply(s, A[1]);
+        if ((s += U * NW) >= steps) break;
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) part[wave][r][lane] = acc[r];
+    __syncthreads();
+    for (u32 i = tid; i < R * 64; i += 64 * NW) {
+        const u32 l = i % 64, j = l & 15, out = r0 + 16 * (i / 64) + 4 * (l >> 4);
+        if (j >= a.m || out >= a.rows) continue;
+        v4i sum = part[0][i / 64][l];
+#pragma unroll
+        for (int w = 1; w < NW; w++) sum += part[w][i / 64][l];
+        float y[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) y[x] = __fmul_rn(__fmul_rn((float)sum[x], scale[j]), a.ws[min(out + x, a.rows - 1)]);
+        i8_store4(a, j, out, y);
     }
 }
 
@@ -640,6 +766,38 @@ static void few_launch(const Launch &L, const I8Args &a, u32 entries) {
     const u32 z = a.start ? 1u : (entries + 16 * C - 1) / (16 * C);
     hipLaunchKernelGGL((k_i8_few<R, C, NW, U>), dim3((a.rows + 16 * R - 1) / (16 * R), a.start ? a.n_experts : 1u, z < 65535u ? z : 65535u), dim3(64 * NW), 0,
                        L.stream, a);
+}
+
+template <int ET, int M, int R>
+static void few_x_launch(const Launch &L, const I8Args &a, const QuantArgs &q) {
+    hipLaunchKernelGGL((k_i8_few_x<ET, M, R, 2>), dim3((a.rows + 16 * R - 1) / (16 * R)), dim3(64 * kFewXWaves), M * a.kp, L.stream, a, q);
+}
+template <int ET, int M>
+static void few_x_by_rows(const Launch &L, const I8Args &a, const QuantArgs &q) {
+    if ((a.rows + 15) / 16 >= 320) few_x_launch<ET, M, 2>(L, a, q);
+    else few_x_launch<ET, M, 1>(L, a, q);
+}
+template <int ET>
+static void few_x_by_columns(const Launch &L, const I8Args &a, const QuantArgs &q) {
+    if (a.m == 1) few_x_by_rows<ET, 1>(L, a, q);
+    else if (a.m == 2) few_x_by_rows<ET, 2>(L, a, q);
+    else if (a.m <= 4) few_x_by_rows<ET, 4>(L, a, q);
+    else few_x_by_rows<ET, 8>(L, a, q);
+}
+
+hipError_t i8_gemm_x(const Launch &L, const int8_t *w, const float *ws, int rows, int k, const void *x, int x_et, int64_t ld_x, int m, int8_t *codes,
+                     float *scales, void *y, int et, int64_t ld) {
+    const u32 kp = (u32)i8_row_bytes(k), M = m <= 1 ? 1 : m <= 2 ? 2 : m <= 4 ? 4 : 8;
+    if (m <= kFewX && kp <= few_x_values(M)) {
+        const I8Args a = {w, ws, (u32)rows, kp, codes, scales, (u32)m, nullptr, nullptr, 0, 0, (u32)m, 1, y, (size_t)ld, et, L.fault, L.layer};
+        const QuantArgs q = {x, nullptr, (size_t)ld_x, (u32)m, (u32)k, kp, nullptr, codes, scales, L.rule, L.fault, L.layer};
+        if (x_et == kElemF32) few_x_by_columns<kElemF32>(L, a, q);
+        else if (x_et == kElemF16) few_x_by_columns<kElemF16>(L, a, q);
+        else few_x_by_columns<kElemBF16>(L, a, q);
+        return hipGetLastError();
+    }
+    const hipError_t e = i8_quantize(L, x, nullptr, x_et, ld_x, m, k, nullptr, codes, scales);
+    return e != hipSuccess ? e : i8_gemm(L, w, ws, 1, rows, k, codes, scales, m, nullptr, nullptr, 0, 0, y, et, ld);
 }
 
 // Which form: all give the same bits. us on MI355X, bf16 out, weights of three sets in turn, the chosen form's first.

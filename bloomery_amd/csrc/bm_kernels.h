@@ -201,7 +201,7 @@ hipError_t card_gemv_sel(const Launch &L, int wtype, const uint8_t *w, int n_exp
 // et: an element type, ggml's numbers (0 f32, 1 f16, 30 bf16); lines in elements. At most kTileMaxSlots slots, kBucketExperts experts and
 // kMaxCombineSlots slots a token.
 // Slots that one launch sorts without `work`.
-constexpr uint32_t kSortFew = 2048;
+constexpr uint32_t kSortFew = 4096;
 size_t expert_sort_work(int n_slots, int n_experts); // words
 // x and rows NULL: the tables alone
 hipError_t expert_sort(const Launch &L, const uint32_t *sel, int n_tokens, int top_k, int n_experts, const void *x, int et, int64_t ldx,
@@ -223,6 +223,9 @@ hipError_t i8_quantize(const Launch &L, const void *x, const void *u, int et, in
 // start NULL: one matrix against n_cols columns. Else entry j of expert e's run reads column order[j] / top_k, or j where top_k is 0.
 hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_experts, int rows, int k, const int8_t *q, const float *qs, int n_cols,
                    const uint32_t *order, const uint32_t *start, int n_slots, int top_k, void *y, int et, int64_t ld);
+// i8_quantize and i8_gemm of one matrix; a few rows in one launch.
+hipError_t i8_gemm_x(const Launch &L, const int8_t *w, const float *ws, int rows, int k, const void *x, int x_et, int64_t ld_x, int m, int8_t *codes,
+                     float *scales, void *y, int et, int64_t ld);
 
 } // namespace bmk
 

@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kRowThreads) void k_sort_few(SortArgs a) {
 }
 
 // ---- many slots, in three launches over chunks of slots, a wave each.
-// 1. A chunk's counts an expert into work[expert * chunks + chunk], and every slot's rank among its chunk's slots of its expert into
+// 1. A chunk's counts an expert into work[chunk * n_experts + expert], and every slot's rank among its chunk's slots of its expert into
 //    place. Eight waves share a chunk, an eighth each with counts of its own: the slots of a wave that share an expert find each other bit
 //    by bit of the id, and an expert's counts are summed over the waves in front. (One wave a chunk of 512 took 6.2 us where this takes 4.)
 constexpr u32 kSortWaves = 8;
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void k_sort_count(SortArgs a, u32 
             count[w * a.n_experts + e] = sum;
             sum += c;
         }
-        a.work[(size_t)e * gridDim.x + blockIdx.x] = sum;
+        a.work[(size_t)blockIdx.x * a.n_experts + e] = sum;
     }
     __syncthreads();
     for (u32 b = lo; b < hi; b += 64) {
@@ -194,37 +194,32 @@ __global__ __launch_bounds__(64 * kSortWaves) void k_sort_count(SortArgs a, u32 
     }
 }
 
-// 2. An expert's counts become their running sums over the chunks, a wave an expert; the experts' own running sums are the runs' bounds.
-__global__ __launch_bounds__(1024) void k_sort_scan(SortArgs a, u32 chunks) {
-    __shared__ u32 scan[16], count[kBucketExperts];
+// 2. The counts become the places of the chunks' first slots: running sums over an expert's chunks behind the runs' bounds. A thread has an expert
+//    and a run of the chunks (at most 32 threads an expert), whose counts it asks for sixteen at a time; it reads them twice, the second time
+//    from the cache.
+__global__ __launch_bounds__(1024) void k_sort_scan(SortArgs a, u32 chunks, u32 log_experts) {
+    __shared__ u32 part[1024], scan[16];
     const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (u32 e0 = wave; e0 < a.n_experts; e0 += 16 * 8) { // eight experts of a wave's at a time, asked for together
-        u32 had[8];
+    const u32 e = tid & ((1u << log_experts) - 1u), group = tid >> log_experts, groups = min(1024u >> log_experts, 32u);
+    const u32 share = (chunks + groups - 1) / groups, lo = min(group * share, chunks), hi = e < a.n_experts ? min(lo + share, chunks) : lo;
+    u32 sum = 0;
+    for (u32 c0 = lo; c0 < hi; c0 += 16) {
+        u32 v[16];
 #pragma unroll
-        for (u32 i = 0; i < 8; i++) had[i] = 0;
-        for (u32 c0 = 0; c0 < chunks; c0 += 64) {
-            const u32 c = c0 + lane;
-            u32 v[8];
+        for (u32 i = 0; i < 16; i++) v[i] = c0 + i < hi ? a.work[(size_t)(c0 + i) * a.n_experts + e] : 0;
 #pragma unroll
-            for (u32 i = 0; i < 8; i++) v[i] = e0 + 16 * i < a.n_experts && c < chunks ? a.work[(size_t)(e0 + 16 * i) * chunks + c] : 0;
-#pragma unroll
-            for (u32 i = 0; i < 8; i++) {
-                u32 upto = v[i];
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) {
-                    const u32 o = (u32)__shfl_up((int)upto, d, 64);
-                    if (lane >= (u32)d) upto += o;
-                }
-                if (e0 + 16 * i < a.n_experts && c < chunks) a.work[(size_t)(e0 + 16 * i) * chunks + c] = had[i] + upto - v[i];
-                had[i] += (u32)__shfl((int)upto, 63, 64);
-            }
-        }
-#pragma unroll
-        for (u32 i = 0; i < 8; i++)
-            if (lane == 0 && e0 + 16 * i < a.n_experts) count[e0 + 16 * i] = had[i];
+        for (u32 i = 0; i < 16; i++) sum += v[i];
     }
+    part[tid] = sum;
     __syncthreads();
-    const u32 c = tid < a.n_experts ? count[tid] : 0;
+    u32 before = 0, count = 0; // of this expert: in the groups in front, in all
+    for (u32 g = 0; g < groups; g++) {
+        const u32 v = part[(g << log_experts) + e];
+        before += g < group ? v : 0;
+        count += v;
+    }
+    // the bounds: the running sum over the experts, in the first group's threads
+    const u32 c = group == 0 ? count : 0;
     u32 upto = c;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -232,35 +227,50 @@ __global__ __launch_bounds__(1024) void k_sort_scan(SortArgs a, u32 chunks) {
         if (lane >= (u32)d) upto += o;
     }
     if (lane == 63) scan[wave] = upto;
-    __syncthreads();
-    u32 before = 0;
+    __syncthreads(); // (every thread has read its part)
+    u32 at = upto - c;
 #pragma unroll
-    for (u32 w = 0; w < 16; w++) before += w < wave ? scan[w] : 0;
-    if (tid < a.n_experts) a.start[tid] = before + upto - c;
-    if (tid + 1 == a.n_experts) a.start[a.n_experts] = before + upto;
+    for (u32 w = 0; w < 16; w++) at += w < wave ? scan[w] : 0;
+    if (group == 0) part[e] = at;
+    __syncthreads();
+    if (group == 0 && e < a.n_experts) {
+        a.start[e] = at;
+        if (e + 1 == a.n_experts) a.start[a.n_experts] = at + count;
+    }
+    at = part[e] + before;
+    for (u32 c0 = lo; c0 < hi; c0 += 16) {
+        u32 v[16];
+#pragma unroll
+        for (u32 i = 0; i < 16; i++) v[i] = c0 + i < hi ? a.work[(size_t)(c0 + i) * a.n_experts + e] : 0;
+#pragma unroll
+        for (u32 i = 0; i < 16; i++) {
+            if (c0 + i < hi) a.work[(size_t)(c0 + i) * a.n_experts + e] = at;
+            at += v[i];
+        }
+    }
 }
 
 // 3. Places and order of a token's slots, and its row to them.
-__device__ __forceinline__ u32 sort_settle(const SortArgs &a, u32 s, u32 per, u32 chunks) {
+__device__ __forceinline__ u32 sort_settle(const SortArgs &a, u32 s, u32 per) {
     const u32 id = a.sel[s], rank = a.place[s];
     if (id >= a.n_experts) return kUnlisted; // place holds kUnlisted already
-    const u32 p = a.start[id] + a.work[(size_t)id * chunks + s / per] + rank;
+    const u32 p = a.work[(size_t)(s / per) * a.n_experts + id] + rank;
     a.place[s] = p;
     a.order[p] = s;
     return p;
 }
 template <int EB>
-__global__ __launch_bounds__(kRowThreads) void k_sort_move(SortArgs a, u32 per, u32 chunks) {
+__global__ __launch_bounds__(kRowThreads) void k_sort_move(SortArgs a, u32 per) {
     __shared__ u32 places[kMaxCombineSlots];
     const u32 token = blockIdx.x;
     const RowAhead ahead = row_ahead(a, token);
-    if (threadIdx.x < a.top_k) places[threadIdx.x] = sort_settle(a, token * a.top_k + threadIdx.x, per, chunks);
+    if (threadIdx.x < a.top_k) places[threadIdx.x] = sort_settle(a, token * a.top_k + threadIdx.x, per);
     __syncthreads();
     move_row<EB>(a, token, places, ahead);
 }
-__global__ __launch_bounds__(kRowThreads) void k_sort_places(SortArgs a, u32 n, u32 per, u32 chunks) {
+__global__ __launch_bounds__(kRowThreads) void k_sort_places(SortArgs a, u32 n, u32 per) {
     const u32 s = blockIdx.x * kRowThreads + threadIdx.x;
-    if (s < n) sort_settle(a, s, per, chunks);
+    if (s < n) sort_settle(a, s, per);
 }
 
 size_t expert_sort_work(int n_slots, int n_experts) {
@@ -282,10 +292,12 @@ hipError_t expert_sort(const Launch &L, const uint32_t *sel, int n_tokens, int t
     }
     const u32 per = sort_chunk_len(n), chunks = (n + per - 1) / per;
     hipLaunchKernelGGL(k_sort_count, dim3(chunks), dim3(64 * kSortWaves), 0, L.stream, a, n, per);
-    hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, L.stream, a, chunks);
-    if (!x) hipLaunchKernelGGL(k_sort_places, dim3((n + kRowThreads - 1) / kRowThreads), dim3(kRowThreads), 0, L.stream, a, n, per, chunks);
-    else if (eb == 4) hipLaunchKernelGGL(k_sort_move<4>, dim3((unsigned)n_tokens), dim3(kRowThreads), 0, L.stream, a, per, chunks);
-    else hipLaunchKernelGGL(k_sort_move<2>, dim3((unsigned)n_tokens), dim3(kRowThreads), 0, L.stream, a, per, chunks);
+    u32 log_experts = 0;
+    while ((1u << log_experts) < a.n_experts) log_experts++;
+    hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, L.stream, a, chunks, log_experts);
+    if (!x) hipLaunchKernelGGL(k_sort_places, dim3((n + kRowThreads - 1) / kRowThreads), dim3(kRowThreads), 0, L.stream, a, n, per);
+    else if (eb == 4) hipLaunchKernelGGL(k_sort_move<4>, dim3((unsigned)n_tokens), dim3(kRowThreads), 0, L.stream, a, per);
+    else hipLaunchKernelGGL(k_sort_move<2>, dim3((unsigned)n_tokens), dim3(kRowThreads), 0, L.stream, a, per);
     return hipGetLastError();
 }
 

@@ -492,7 +492,7 @@ int bm_card_gemv_sel(bm_ctx *ctx, const bm_weights *w, const int8_t *codes_dev, 
  * BM_SITE_EXPERT_ID. Entries of order_dev and rows of rows_dev behind the last listed one keep what they held. x_dev and rows_dev
  * both NULL: the tables alone (type, width and the lines are not looked at). rows_dev: n_tokens * top_k rows.
  * work_dev: bm_expert_sort_work(n_tokens * top_k, n_experts) words of scratch that holds nothing between calls (NULL where that is 0: a
- * sort of up to 2048 slots is one launch, a longer one three). At most ceil(n_slots / 512) * n_experts words. */
+ * sort of up to 4096 slots is one launch, a longer one three). At most ceil(n_slots / 512) * n_experts words. */
 int64_t bm_expert_sort_work(int n_slots, int n_experts);
 int bm_expert_sort(bm_ctx *ctx, const uint32_t *sel_dev, int n_tokens, int top_k, int n_experts, const void *x_dev, int type, int64_t ld_x,
                    int width, uint32_t *order_dev, uint32_t *start_dev, uint32_t *place_dev, void *rows_dev, int64_t ld_rows, uint32_t *work_dev);

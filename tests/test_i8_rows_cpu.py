@@ -84,15 +84,15 @@ def test_tokens_slots_and_experts(name):
 
 
 def test_sort_scratch_and_the_tables_alone():
-    assert bm.expert_sort_work(2048, 1024) == 0 and bm.expert_sort_work(1, 1) == 0
+    assert bm.expert_sort_work(4096, 1024) == 0 and bm.expert_sort_work(1, 1) == 0
     assert bm.expert_sort_work(0, 4) == bm.ESHAPE and bm.expert_sort_work(4, 1025) == bm.ESHAPE and bm.expert_sort_work((1 << 22) + 1, 4) == bm.ESHAPE
-    for n in (2049, 5000, 65536, 100000, 1 << 22):
+    for n in (4097, 5000, 65536, 100000, 1 << 22):
         for experts in (1, 7, 128, 1024):
             assert 0 < bm.expert_sort_work(n, experts) <= -(-n // 512) * experts
     none = dict(x=None, rows=None, type=99, width=-1, ld_x=-5, ld_rows=0)  # not looked at
     assert call("bm_expert_sort", **none)[1].endswith("ctx is NULL")
     assert call("bm_expert_sort", x=None)[0] == bm.EARG and call("bm_expert_sort", rows=None)[0] == bm.EARG  # one without the other
-    assert call("bm_expert_sort", n_tokens=256, work=None)[1].endswith("ctx is NULL")  # 2048 slots need none
+    assert call("bm_expert_sort", n_tokens=512, work=None)[1].endswith("ctx is NULL")  # 4096 slots need none
 
 
 @pytest.mark.parametrize("name", [n for n in GOOD if n.startswith("bm_i8")])
