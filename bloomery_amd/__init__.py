@@ -195,6 +195,10 @@ class DeviceBuffer:
     def nbytes(self):
         return self.count * self.dtype.itemsize
 
+    @property
+    def _as_parameter_(self):  # an entry that takes an address takes the buffer (None once it is freed)
+        return self.ptr
+
     def upload(self, host):
         host = np.ascontiguousarray(host, self.dtype).reshape(-1)
         assert host.size <= self.count
@@ -390,10 +394,6 @@ def _ptr(x):
     if isinstance(x, DeviceBuffer):
         return x.ptr
     return x  # a raw device address (e.g. torch.Tensor.data_ptr())
-
-
-def _line(ld, width):
-    return width if ld is None else ld
 
 
 class GateAct(C.Structure):
@@ -593,48 +593,48 @@ class Gpu:
     def enqueue_expert_sort(self, sel, n_tokens, top_k, n_experts, x, dtype, width, order, start, place, rows, work=None, ld_x=None,
                             ld_rows=None):
         """Tables of the picks and the tokens' rows at their slots' places (bm_expert_sort); x and rows None: the tables alone."""
-        self._check(self.lib.bm_expert_sort(self.ctx, _ptr(sel), n_tokens, top_k, n_experts, _ptr(x), dtype, _line(ld_x, width), width,
-                                            _ptr(order), _ptr(start), _ptr(place), _ptr(rows), _line(ld_rows, width), _ptr(work)))
+        self._check(self.lib.bm_expert_sort(self.ctx, sel, n_tokens, top_k, n_experts, x, dtype, width if ld_x is None else ld_x, width,
+                                            order, start, place, rows, width if ld_rows is None else ld_rows, work))
 
     def enqueue_expert_sort_grad(self, d_rows, dtype, place, n_tokens, top_k, width, dx, ld_rows=None, ld_dx=None):
-        self._check(self.lib.bm_expert_sort_grad(self.ctx, _ptr(d_rows), dtype, _line(ld_rows, width), _ptr(place), n_tokens, top_k, width,
-                                                 _ptr(dx), _line(ld_dx, width)))
+        self._check(self.lib.bm_expert_sort_grad(self.ctx, d_rows, dtype, width if ld_rows is None else ld_rows, place, n_tokens, top_k, width,
+                                                 dx, width if ld_dx is None else ld_dx))
 
     def enqueue_expert_combine(self, rows, dtype, place, wts, resid, n_tokens, top_k, width, y, ld_rows=None, ld_resid=None, ld_y=None):
         """The sorted rows back at their tokens: the slots' weighted sum onto the residual (None: no add)."""
-        self._check(self.lib.bm_expert_combine(self.ctx, _ptr(rows), dtype, _line(ld_rows, width), _ptr(place), _ptr(wts), _ptr(resid),
-                                               _line(ld_resid, width), n_tokens, top_k, width, _ptr(y), _line(ld_y, width)))
+        self._check(self.lib.bm_expert_combine(self.ctx, rows, dtype, width if ld_rows is None else ld_rows, place, wts, resid,
+                                               width if ld_resid is None else ld_resid, n_tokens, top_k, width, y, width if ld_y is None else ld_y))
 
     def enqueue_expert_combine_grad(self, dy, dtype, rows, place, wts, n_tokens, top_k, width, d_rows, d_wts, ld_dy=None, ld_rows=None,
                                     ld_d_rows=None):
-        self._check(self.lib.bm_expert_combine_grad(self.ctx, _ptr(dy), dtype, _line(ld_dy, width), _ptr(rows), _line(ld_rows, width), _ptr(place),
-                                                    _ptr(wts), n_tokens, top_k, width, _ptr(d_rows), _line(ld_d_rows, width), _ptr(d_wts)))
+        self._check(self.lib.bm_expert_combine_grad(self.ctx, dy, dtype, width if ld_dy is None else ld_dy, rows, width if ld_rows is None else ld_rows, place,
+                                                    wts, n_tokens, top_k, width, d_rows, width if ld_d_rows is None else ld_d_rows, d_wts))
 
     # -- products in 8-bit integers: codes of i8_row_bytes(k) bytes a row and an f32 scale a row, on both sides
     def enqueue_i8_quantize(self, x, dtype, m, k, codes, scales, ld_x=None, live=None):
         """live: a device word; rows at or past its value keep what they held."""
-        self._check(self.lib.bm_i8_quantize(self.ctx, _ptr(x), dtype, _line(ld_x, k), m, k, _ptr(live), _ptr(codes), _ptr(scales)))
+        self._check(self.lib.bm_i8_quantize(self.ctx, x, dtype, k if ld_x is None else ld_x, m, k, live, codes, scales))
 
     def enqueue_i8_swiglu_quantize(self, g, u, dtype, m, k, codes, scales, ld=None, live=None, rule=None):
-        self._check(self.lib.bm_i8_swiglu_quantize(self.ctx, _ptr(g), _ptr(u), dtype, _line(ld, k), m, k, _rule(rule), _ptr(live), _ptr(codes),
-                                                   _ptr(scales)))
+        self._check(self.lib.bm_i8_swiglu_quantize(self.ctx, g, u, dtype, k if ld is None else ld, m, k, _rule(rule) if rule is not None else None, live, codes,
+                                                   scales))
 
     def enqueue_i8_gemm(self, w, w_scales, rows, k, codes, scales, m, y, y_type, ld_y=None):
-        self._check(self.lib.bm_i8_gemm(self.ctx, _ptr(w), _ptr(w_scales), rows, k, _ptr(codes), _ptr(scales), m, _ptr(y), y_type,
-                                        _line(ld_y, rows)))
+        self._check(self.lib.bm_i8_gemm(self.ctx, w, w_scales, rows, k, codes, scales, m, y, y_type,
+                                        rows if ld_y is None else ld_y))
 
     def enqueue_i8_gemm_x(self, w, w_scales, rows, k, x, x_type, m, codes, scales, y, y_type, ld_x=None, ld_y=None):
         """enqueue_i8_quantize of the m rows of x and enqueue_i8_gemm in one call (the same bits)."""
-        self._check(self.lib.bm_i8_gemm_x(self.ctx, _ptr(w), _ptr(w_scales), rows, k, _ptr(x), x_type, _line(ld_x, k), m, _ptr(codes),
-                                          _ptr(scales), _ptr(y), y_type, _line(ld_y, rows)))
+        self._check(self.lib.bm_i8_gemm_x(self.ctx, w, w_scales, rows, k, x, x_type, k if ld_x is None else ld_x, m, codes,
+                                          scales, y, y_type, rows if ld_y is None else ld_y))
 
     def enqueue_i8_gemm_experts(self, w, w_scales, n_experts, rows_per_expert, k, codes, scales, order, start, n_slots, top_k, y, y_type,
                                 ld_y=None, n_cols=None):
         """top_k > 0: every slot of a token reads the token's column; 0: entry j reads column j."""
         if n_cols is None:
             n_cols = n_slots // top_k if top_k > 0 else n_slots
-        self._check(self.lib.bm_i8_gemm_experts(self.ctx, _ptr(w), _ptr(w_scales), n_experts, rows_per_expert, k, _ptr(codes), _ptr(scales),
-                                                n_cols, _ptr(order), _ptr(start), n_slots, top_k, _ptr(y), y_type, _line(ld_y, rows_per_expert)))
+        self._check(self.lib.bm_i8_gemm_experts(self.ctx, w, w_scales, n_experts, rows_per_expert, k, codes, scales,
+                                                n_cols, order, start, n_slots, top_k, y, y_type, rows_per_expert if ld_y is None else ld_y))
 
     # -- grouped decode: the slot table by expert and the tile launchers
     def tile_cap(self, n_slots, n_experts):

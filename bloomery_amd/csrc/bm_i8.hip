@@ -258,6 +258,19 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
             bool bad;
             qp[c] = a.q + (size_t)i8_column(a, j < run.j1 ? j : run.j1 - 1, bad) * a.kp;
         }
+        // a thread's outputs at the end - four rows (4 (l / 16) ..) of one column (l % 16) of tile tid / 64 - and their scales, asked for now
+        static_assert(R * C <= NW, "one piece a thread");
+        const u32 tile = tid / 64, j = t0 + 16 * (tile % C) + (lane & 15), row = r0 + 16 * (tile / C) + 4 * (lane >> 4);
+        const bool out = tile < R * C && j < run.j1 && row < a.rows;
+        float scale = 0.0f, row_scale[4];
+        if (out) {
+            bool bad;
+            const u32 col = i8_column(a, j, bad);
+            if (bad) bm_raise(a.fault, a.layer, kSiteExpertId);
+            scale = bad ? bm_bits_f32(0x7fc00000u) : a.qs[col];
+#pragma unroll
+            for (int x = 0; x < 4; x++) row_scale[x] = run.ws[min(row + x, a.rows - 1)];
+        }
         v4i acc[R][C];
 #pragma unroll
         for (int r = 0; r < R; r++)
@@ -302,23 +315,14 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
 #pragma unroll
             for (int c = 0; c < C; c++) part[wave][r * C + c][lane] = acc[r][c];
         __syncthreads();
-        // four rows (4 (l / 16) ..) of one column (l % 16) a lane of a tile
-        for (u32 i = tid; i < R * C * 64; i += 64 * NW) {
-            const u32 tile = i / 64, l = i % 64;
-            v4i sum = part[0][tile][l];
+        if (out) {
+            v4i sum = part[0][tile][lane];
 #pragma unroll
-            for (int w = 1; w < NW; w++) sum += part[w][tile][l];
-            const u32 j = t0 + 16 * (tile % C) + (l & 15), row = r0 + 16 * (tile / C) + 4 * (l >> 4);
-            if (j < run.j1 && row < a.rows) {
-                bool bad;
-                const u32 col = i8_column(a, j, bad);
-                if (bad) bm_raise(a.fault, a.layer, kSiteExpertId);
-                const float s = bad ? bm_bits_f32(0x7fc00000u) : a.qs[col];
-                float v[4];
+            for (int w = 1; w < NW; w++) sum += part[w][tile][lane];
+            float v[4];
 #pragma unroll
-                for (int x = 0; x < 4; x++) v[x] = __fmul_rn(__fmul_rn((float)sum[x], s), run.ws[row + x < a.rows ? row + x : row]);
-                i8_store4(a, j, row, v);
-            }
+            for (int x = 0; x < 4; x++) v[x] = __fmul_rn(__fmul_rn((float)sum[x], scale), row_scale[x]);
+            i8_store4(a, j, row, v);
         }
         __syncthreads();
     }
@@ -353,6 +357,14 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
             for (int r = 0; r < R; r++) f[u][r] = *reinterpret_cast<const v4i *>(wp[r] + off);
         }
     };
+    // a thread's outputs at the end, and the scales of their rows
+    static_assert(R <= NW, "one piece a thread");
+    const u32 j = lane & 15, out = r0 + 16 * wave + 4 * (lane >> 4);
+    const bool mine_out = wave < R && j < a.m && out < a.rows;
+    float row_scale[4];
+    if (mine_out)
+#pragma unroll
+        for (int x = 0; x < 4; x++) row_scale[x] = a.ws[min(out + x, a.rows - 1)];
     // the rows' values, then the first weights
     const u32 row = tid / T, mine = tid % T, pieces = a.kp / 8;
     float v[4][8];
@@ -423,17 +435,14 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
 #pragma unroll
     for (int r = 0; r < R; r++) part[wave][r][lane] = acc[r];
     __syncthreads();
-    for (u32 i = tid; i < R * 64; i += 64 * NW) {
-        const u32 l = i % 64, j = l & 15, out = r0 + 16 * (i / 64) + 4 * (l >> 4);
-        if (j >= a.m || out >= a.rows) continue;
-        v4i sum = part[0][i / 64][l];
+    if (!mine_out) return;
+    v4i sum = part[0][wave][lane];
 #pragma unroll
-        for (int w = 1; w < NW; w++) sum += part[w][i / 64][l];
-        float y[4];
+    for (int w = 1; w < NW; w++) sum += part[w][wave][lane];
+    float y[4];
 #pragma unroll
-        for (int x = 0; x < 4; x++) y[x] = __fmul_rn(__fmul_rn((float)sum[x], scale[j]), a.ws[min(out + x, a.rows - 1)]);
-        i8_store4(a, j, out, y);
-    }
+    for (int x = 0; x < 4; x++) y[x] = __fmul_rn(__fmul_rn((float)sum[x], scale[j]), row_scale[x]);
+    i8_store4(a, j, out, y);
 }
 
 // Many columns a matrix: BT columns x BR rows a workgroup, 128 bytes of k a step through a ring of S LDS buffers, where the loads put them
@@ -458,33 +467,42 @@ struct I8Tile {
 
 __device__ __forceinline__ u32 i8_swizzle(u32 line) { return (line >> 1) & 7; }
 
-// The tile of workgroup b: an expert's run cut into tiles of BT entries, numbered through the experts in order. False: there is none.
+// A tile of the experts: their runs cut into tiles of BT entries, numbered through the experts in order. False: there is none of that number. The bounds
+// of 256 experts are asked for at once; a run that is none raises ExpertId (once a launch and wave of the first tile) and has no tiles.
 template <int BT>
 __device__ __forceinline__ bool i8_find_tile(const I8Args &a, u32 tile, u32 &expert, u32 &t0) {
     const u32 lane = threadIdx.x & 63;
     u32 before = 0;
-    for (u32 e0 = 0; e0 < a.n_experts; e0 += 64) {
-        const u32 e = e0 + lane;
-        u32 c = 0;
-        if (e < a.n_experts) {
-            const u32 j0 = a.start[e], j1 = a.start[e + 1];
-            if (j0 <= j1 && j1 <= a.n_slots) c = (j1 - j0 + BT - 1) / BT;
-            else if (tile == 0 && threadIdx.x < 64) bm_raise(a.fault, a.layer, kSiteExpertId);
-        }
-        u32 upto = c;
+    for (u32 e0 = 0; e0 < a.n_experts; e0 += 256) {
+        u32 j0[4], j1[4];
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const u32 o = (u32)__shfl_up((int)upto, d, 64);
-            if (lane >= (u32)d) upto += o;
+        for (u32 i = 0; i < 4; i++) {
+            const u32 e = min(e0 + 64 * i + lane, a.n_experts - 1);
+            j0[i] = a.start[e];
+            j1[i] = a.start[e + 1];
         }
-        const unsigned long long mine = __ballot(c != 0 && before + upto - c <= tile && tile < before + upto);
-        if (mine) {
-            const int l = __builtin_ctzll(mine);
-            expert = (u32)__builtin_amdgcn_readfirstlane((int)(e0 + (u32)l));
-            t0 = (u32)__builtin_amdgcn_readfirstlane((int)((tile - before - (u32)__shfl((int)(upto - c), l, 64)) * BT));
-            return true;
+#pragma unroll
+        for (u32 i = 0; i < 4; i++) {
+            const u32 e = e0 + 64 * i + lane;
+            if (e0 + 64 * i >= a.n_experts) break;
+            const bool run = j0[i] <= j1[i] && j1[i] <= a.n_slots;
+            if (e < a.n_experts && !run && tile == 0) bm_raise(a.fault, a.layer, kSiteExpertId);
+            const u32 c = e < a.n_experts && run ? (j1[i] - j0[i] + BT - 1) / BT : 0;
+            u32 upto = c;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const u32 o = (u32)__shfl_up((int)upto, d, 64);
+                if (lane >= (u32)d) upto += o;
+            }
+            const unsigned long long mine = __ballot(c != 0 && before + upto - c <= tile && tile < before + upto);
+            if (mine) {
+                const int l = __builtin_ctzll(mine);
+                expert = (u32)__builtin_amdgcn_readfirstlane((int)(e0 + 64 * i + (u32)l));
+                t0 = (u32)__builtin_amdgcn_readfirstlane((int)((tile - before - (u32)__shfl((int)(upto - c), l, 64)) * BT));
+                return true;
+            }
+            before += (u32)__shfl((int)upto, 63, 64);
         }
-        before += (u32)__shfl((int)upto, 63, 64);
     }
     return false;
 }
@@ -663,7 +681,7 @@ __device__ __forceinline__ void i8_tile_out(const I8Args &a, const I8Run &run, u
 }
 
 template <int BT, int BR, int WT, int WR, int S, int EU>
-__global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU))) void k_i8_tile(I8Args a, u32 n_row_tiles) {
+__global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU))) void k_i8_tile(I8Args a, u32 n_row_tiles, u32 group) {
     using G = I8Tile<BT, BR, WT, WR, S>;
     // in this order: the larger alignment comes first
     __shared__ __align__(4096) uint8_t ring0[G::kStage];
@@ -671,13 +689,21 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     __shared__ __align__(1024) uint8_t ring2[S > 2 ? G::kStage : 16];
     __shared__ __align__(512) uint8_t ring3[S > 2 ? G::kStage : 16];
     const u32 tid = threadIdx.x, lane = tid & 63, wave = (u32)__builtin_amdgcn_readfirstlane(tid >> 6);
-    u32 expert = 0, t0;
-    if (a.start) {
-        if (!i8_find_tile<BT>(a, blockIdx.x / n_row_tiles, expert, t0)) return;
+    // Workgroups go to the chip's eight dies in turn (b to die b % 8, each with its own L2). Neighbouring workgroups share a tile's columns across
+    // the dies, and a die's workgroups four of the rows' tiles and eight of the columns'. An expert with fewer tiles of rows than dies
+    // would so have its rows on every die: there (`group`) a group of its tiles of columns stays on one die, all rows of it.
+    u32 expert = 0, t0, row_tile, tile;
+    if (group) {
+        const u32 i = blockIdx.x >> 3, per = group * n_row_tiles;
+        row_tile = i % per / group;
+        tile = (i / per * 8 + (blockIdx.x & 7)) * group + i % group;
     } else {
-        t0 = (blockIdx.x / n_row_tiles) * BT;
+        row_tile = blockIdx.x % n_row_tiles;
+        tile = blockIdx.x / n_row_tiles;
     }
-    const u32 r0 = (blockIdx.x % n_row_tiles) * BR;
+    if (!a.start) t0 = tile * BT;
+    else if (!i8_find_tile<BT>(a, tile, expert, t0)) return;
+    const u32 r0 = row_tile * BR;
     I8Run run;
     if (!i8_run(a, expert, run)) return;
     t0 = (u32)__builtin_amdgcn_readfirstlane((int)(t0 + run.j0));
@@ -770,19 +796,27 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     else i8_tile_out<kElemBF16, G>(a, run, part, t0 + wt, r0 + (wr - BT), acc);
 }
 
+// Whether a launch along one dimension has fewer threads than its limit, 2^32.
+static bool i8_launchable(uint64_t groups, u32 threads) { return groups * threads <= 0xffffffffu; }
+
 template <int BT, int BR, int WT, int WR, int S, int EU>
-static void tile_launch(const Launch &L, const I8Args &a, u32 entries) {
+static hipError_t tile_launch(const Launch &L, const I8Args &a, u32 entries) {
     const u32 row_tiles = (a.rows + BR - 1) / BR;
     u32 tiles = (entries + BT - 1) / BT;
     if (a.start) tiles = entries / BT + (a.n_experts < entries ? a.n_experts : entries); // at most a ragged tile an expert
-    hipLaunchKernelGGL((k_i8_tile<BT, BR, WT, WR, S, EU>), dim3(tiles * row_tiles), dim3(64 * WT * WR), 0, L.stream, a, row_tiles);
+    const u32 group = a.start && row_tiles < 8 ? 2 : 0;
+    if (group) tiles = (tiles + 8 * group - 1) / (8 * group) * (8 * group);
+    if (!i8_launchable((uint64_t)tiles * row_tiles, 64 * WT * WR)) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((k_i8_tile<BT, BR, WT, WR, S, EU>), dim3(tiles * row_tiles), dim3(64 * WT * WR), 0, L.stream, a, row_tiles, group);
+    return hipGetLastError();
 }
 
 template <int R, int C, int NW, int U>
-static void few_launch(const Launch &L, const I8Args &a, u32 entries) {
+static hipError_t few_launch(const Launch &L, const I8Args &a, u32 entries) {
     const u32 z = a.start ? 1u : (entries + 16 * C - 1) / (16 * C);
     hipLaunchKernelGGL((k_i8_few<R, C, NW, U>), dim3((a.rows + 16 * R - 1) / (16 * R), a.start ? a.n_experts : 1u, z < 65535u ? z : 65535u), dim3(64 * NW), 0,
                        L.stream, a);
+    return hipGetLastError();
 }
 
 template <int ET, int M, int R>
@@ -826,9 +860,12 @@ hipError_t i8_gemm_x(const Launch &L, const int8_t *w, const float *ws, int rows
 //   four steps in flight, as few workgroups need. Up to 32 columns, and where even those tiles are few, every workgroup's waves share a row's k: 24 x 7168 x 2048 6.5
 //   (32 x 64: 7.5), 64 x 2048 x 7168 12.0 (15.0); 16 x 7168 x 2048 5.8 (7.3), 1 x 2048 x 7168 6.6 (14.8). There two tiles of 16 rows a workgroup of four waves
 //   from 320 tiles on (24 columns: 6.5 against 7.8), else one of eight waves (1 x 2048 x 7168: 6.6 against 9.9).
-//   Experts, by slots an expert: 2048 tokens, top 8 of 128 (128 slots each), 768 x 2048 rows in 128 x 128 81 (64 x 128: 88, 256 x 256: 85); 512 tokens in 64 x 128 50
-//   (128 x 128: 54); 64 tokens in 32 x 64 33 (64 x 128: 34, waves sharing k 41); one token's eight slots by waves sharing k 7.9 (32 x 64: 9.1);
-//   4096 tokens, top 8 of 32, 7168 x 2048 rows in 256 x 256 573 (256 x 224: 594, 128 x 128: 630).
+//   Experts, by slots an expert: 4096 tokens, top 8 of 32 (1024 slots each), 7168 x 2048 rows in 256 x 256 595 (128 x 128: 658, 64 x 256: 714); 2048 tokens, top 8 of 128, 768 x 2048
+//   in 64 x 256 72 (256 x 256: 79, 128 x 128: 78, 64 x 128: 76), 2048 x 768 87 (103, 91, 91); 512 tokens 46 (64 x 128: 51), one round of tiles; 1024 tokens in 64 x 128 58
+//   (64 x 256: 63), 333 tokens, top 8 of 64, 7168 x 2048 189 (193; own columns, f16, 156 and 166); 128 tokens
+//   (8 slots each) in 32 x 64 37 (64 x 256: 39), 16 tokens 20 (24; waves sharing k 25); one token's eight slots by waves sharing k 7.9 (32 x 64: 9.1). A die's group of two
+//   tiles of columns (k_i8_tile) in these: 2048 tokens 72, without 88; where a run's rows are eight tiles or more it loses (333 tokens, 7168 rows in
+//   64 x 128, 189 without, 204 with).
 hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_experts, int rows, int k, const int8_t *q, const float *qs, int n_cols,
                    const uint32_t *order, const uint32_t *start, int n_slots, int top_k, void *y, int et, int64_t ld) {
     const I8Args a = {w, ws, (u32)rows, (u32)i8_row_bytes(k), q, qs, (u32)n_cols, order, start, (u32)n_slots, (u32)top_k, (u32)n_cols, (u32)n_experts,
@@ -840,33 +877,26 @@ hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_expe
     const bool reach = !order || (uint64_t)n_cols * a.kp <= 0xffffffffu;
     if (start && reach && n > 16) {
         const u32 each = n / (u32)n_experts;
-        if (each >= 512) tile_launch<256, 256, 4, 2, 2, 2>(L, a, n);
-        else if (each >= 96) tile_launch<128, 128, 2, 2, 2, 2>(L, a, n);
-        else if (each >= 12) tile_launch<64, 128, 1, 4, 2, 2>(L, a, n);
-        else tile_launch<32, 64, 1, 2, 2, 2>(L, a, n);
-        return hipGetLastError();
+        if (each >= 512) return tile_launch<256, 256, 4, 2, 2, 2>(L, a, n);
+        // 64 x 256 where its tiles (half a tile more an expert) are one round of two a compute unit, or the runs long
+        if (each >= 96 || (each >= 12 && (uint64_t)(n / 64 + (u32)n_experts / 2) * up(a.rows, 256) <= 512)) return tile_launch<64, 256, 1, 4, 2, 2>(L, a, n);
+        if (each >= 12) return tile_launch<64, 128, 1, 4, 2, 2>(L, a, n);
+        return tile_launch<32, 64, 1, 2, 2, 2>(L, a, n);
     }
     if (!start && n > 32 && tiles(32, 64) >= 96) {
         if (tiles(256, 256) >= 96) {
             const uint64_t by256 = 64 * ((tiles(256, 256) + 255) / 256), by224 = 57 * ((tiles(256, 224) + 255) / 256), by128 = 39 * ((tiles(128, 128) + 511) / 512);
-            if (by256 <= by224 && by256 <= by128) tile_launch<256, 256, 4, 2, 2, 2>(L, a, n);
-            else if (by224 <= by128) tile_launch<256, 224, 4, 2, 2, 2>(L, a, n);
-            else tile_launch<128, 128, 2, 2, 2, 2>(L, a, n);
-        } else if (tiles(128, 128) >= 320) tile_launch<128, 128, 2, 2, 2, 2>(L, a, n);
-        else if (tiles(64, 128) >= 256) tile_launch<64, 128, 1, 4, 2, 2>(L, a, n);
-        else if (tiles(64, 64) >= 192) tile_launch<64, 64, 2, 2, 4, 2>(L, a, n);
-        else tile_launch<32, 64, 1, 2, 4, 2>(L, a, n);
-        return hipGetLastError();
+            if (by256 <= by224 && by256 <= by128) return tile_launch<256, 256, 4, 2, 2, 2>(L, a, n);
+            return by224 <= by128 ? tile_launch<256, 224, 4, 2, 2, 2>(L, a, n) : tile_launch<128, 128, 2, 2, 2, 2>(L, a, n);
+        }
+        if (tiles(128, 128) >= 320) return tile_launch<128, 128, 2, 2, 2, 2>(L, a, n);
+        if (tiles(64, 128) >= 256) return tile_launch<64, 128, 1, 4, 2, 2>(L, a, n);
+        if (tiles(64, 64) >= 192) return tile_launch<64, 64, 2, 2, 4, 2>(L, a, n);
+        return tile_launch<32, 64, 1, 2, 4, 2>(L, a, n);
     }
     const bool wide = (start ? (uint64_t)(n < (u32)n_experts ? n : (u32)n_experts) : 1) * up(a.rows, 16) >= 320;
-    if (n <= 16 || start) {
-        if (wide) few_launch<2, 1, 4, 4>(L, a, n);
-        else few_launch<1, 1, 8, 2>(L, a, n);
-    } else {
-        if (wide && n <= 32) few_launch<2, 2, 4, 4>(L, a, n);
-        else few_launch<1, 2, 8, 2>(L, a, n);
-    }
-    return hipGetLastError();
+    if (n <= 16 || start) return wide ? few_launch<2, 1, 4, 4>(L, a, n) : few_launch<1, 1, 8, 2>(L, a, n);
+    return wide && n <= 32 ? few_launch<2, 2, 4, 4>(L, a, n) : few_launch<1, 2, 8, 2>(L, a, n);
 }
 
 } // namespace bmk
