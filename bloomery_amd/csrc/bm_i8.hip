@@ -234,7 +234,7 @@ __device__ __forceinline__ void i8_store4(const I8Args &a, u32 j, u32 r, const f
     else elem_store_some<kElemBF16, 4>(a.y, at, have, v);
 }
 
-// Few columns a matrix: 16 R rows a workgroup against 16 C columns, its NW waves dealing the row's 64-byte steps among them. Weights go
+// Few columns a matrix: 16 R rows a workgroup against 16 C columns, its NW waves dealing the row's 128-byte lines among them. Weights go
 // from memory to registers in the form v_mfma_i32_16x16x64_i8 takes them (lane l: row l % 16, bytes 16 (l / 16) .. + 15 of the step), each once;
 // the columns come from the cache. The waves' sums meet in LDS as integers.
 template <int R, int C, int NW, int U>
@@ -243,7 +243,7 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
     const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = threadIdx.x;
     I8Run run;
     if (!i8_run(a, blockIdx.y, run)) return;
-    const u32 r0 = blockIdx.x * (16 * R), steps = (a.kp + 63) / 64;
+    const u32 r0 = blockIdx.x * (16 * R), lines = (a.kp + 127) / 128;
     const int8_t *wp[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -276,12 +276,14 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
         for (int r = 0; r < R; r++)
 #pragma unroll
             for (int c = 0; c < C; c++) acc[r][c] = v4i{0, 0, 0, 0};
-        // U steps asked for at a time, the next U while these are multiplied
+        // U halves of lines asked for at a time (a line's two by one wave, one after the other: the second comes from the vector cache), the next U
+        // while these are multiplied
+        static_assert(U % 2 == 0, "whole lines");
         v4i A[2][U][R], B[2][U][C];
         auto ask = [&](u32 s, v4i (&fa)[U][R], v4i (&fb)[U][C]) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const u32 at = 64 * (s + u * NW) + 16 * (lane >> 4), off = at < a.kp ? at : 0; // past the row: its first bytes, against zeros
+                const u32 at = 128 * (s + u / 2 * NW) + 64 * (u % 2) + 16 * (lane >> 4), off = at < a.kp ? at : 0; // past the row: its first bytes, against zeros
 #pragma unroll
                 for (int r = 0; r < R; r++) fa[u][r] = *reinterpret_cast<const v4i *>(wp[r] + off);
 #pragma unroll
@@ -291,7 +293,7 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
         auto multiply = [&](u32 s, v4i (&fa)[U][R], v4i (&fb)[U][C]) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const bool in = 64 * (s + u * NW) + 16 * (lane >> 4) < a.kp;
+                const bool in = 128 * (s + u / 2 * NW) + 64 * (u % 2) + 16 * (lane >> 4) < a.kp;
 #pragma unroll
                 for (int c = 0; c < C; c++) {
                     const v4i b = in ? fb[u][c] : v4i{0, 0, 0, 0};
@@ -303,12 +305,12 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
         u32 s = wave;
         ask(s, A[0], B[0]);
         for (;;) {
-            if (s + U * NW < steps) ask(s + U * NW, A[1], B[1]);
+            if (s + U / 2 * NW < lines) ask(s + U / 2 * NW, A[1], B[1]);
             multiply(s, A[0], B[0]);
-            if ((s += U * NW) >= steps) break;
-            if (s + U * NW < steps) ask(s + U * NW, A[0], B[0]);
+            if ((s += U / 2 * NW) >= lines) break;
+            if (s + U / 2 * NW < lines) ask(s + U / 2 * NW, A[0], B[0]);
             multiply(s, A[1], B[1]);
-            if ((s += U * NW) >= steps) break;
+            if ((s += U / 2 * NW) >= lines) break;
         }
 #pragma unroll
         for (int r = 0; r < R; r++)
@@ -344,7 +346,7 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
     __shared__ v4i part[NW][R][64];
     __shared__ u32 top[NW];
     __shared__ float scale[M];
-    const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, steps = (a.kp + 63) / 64, r0 = blockIdx.x * (16 * R);
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lines = (a.kp + 127) / 128, r0 = blockIdx.x * (16 * R);
     const int8_t *wp[R];
 #pragma unroll
     for (int r = 0; r < R; r++) wp[r] = a.w + (size_t)min(r0 + 16 * r + (lane & 15), a.rows - 1) * a.kp;
@@ -352,7 +354,7 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
     const auto ask = [&](u32 s, v4i (&f)[U][R]) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const u32 at = 64 * (s + u * NW) + 16 * (lane >> 4), off = at < a.kp ? at : 0; // past the row: its first bytes, against zeros
+            const u32 at = 128 * (s + u / 2 * NW) + 64 * (u % 2) + 16 * (lane >> 4), off = at < a.kp ? at : 0; // past the row: its first bytes, against zeros
 #pragma unroll
             for (int r = 0; r < R; r++) f[u][r] = *reinterpret_cast<const v4i *>(wp[r] + off);
         }
@@ -417,7 +419,7 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
     const auto multiply = [&](u32 s, const v4i (&f)[U][R]) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const u32 at = 64 * (s + u * NW) + 16 * (lane >> 4);
+            const u32 at = 128 * (s + u / 2 * NW) + 64 * (u % 2) + 16 * (lane >> 4);
             v4i b = v4i{0, 0, 0, 0};
             if (col < (u32)M && at < a.kp) b = *reinterpret_cast<const v4i *>(codes + col * a.kp + at);
 #pragma unroll
@@ -425,12 +427,12 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
         }
     };
     for (u32 s = wave;;) {
-        if (s + U * NW < steps) ask(s + U * NW, A[1]);
+        if (s + U / 2 * NW < lines) ask(s + U / 2 * NW, A[1]);
         multiply(s, A[0]);
-        if ((s += U * NW) >= steps) break;
-        if (s + U * NW < steps) ask(s + U * NW, A[0]);
+        if ((s += U / 2 * NW) >= lines) break;
+        if (s + U / 2 * NW < lines) ask(s + U / 2 * NW, A[0]);
         multiply(s, A[1]);
-        if ((s += U * NW) >= steps) break;
+        if ((s += U / 2 * NW) >= lines) break;
     }
 #pragma unroll
     for (int r = 0; r < R; r++) part[wave][r][lane] = acc[r];
@@ -453,8 +455,9 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
 typedef __attribute__((address_space(1))) void i8_gptr;
 typedef __attribute__((address_space(3))) void i8_lptr;
 
-template <int BT, int BR, int WT, int WR, int S>
+template <int BT, int BR, int WT, int WR, int S, bool WHOLE>
 struct I8Tile {
+    static constexpr bool kWhole = WHOLE;
     static constexpr int kColumns = BT, kRows = BR, kRing = S, kWaves = WT * WR, kThreads = 64 * kWaves, kStage = (BT + BR) * 128;
     // a wave's loads a step, eight lines each, of columns and of rows (the last waves may repeat some of rows)
     static constexpr int RT = BT / 8 / kWaves, RR = (BR / 8 + kWaves - 1) / kWaves;
@@ -623,6 +626,38 @@ __device__ __forceinline__ void i8_step(I8Src<G> &src, uint8_t *__restrict__ buf
     if constexpr (FULL) i8_weave<G::H0 + G::TT, G::H1 * G::TT>();
 }
 
+// The same with a whole step's pieces in registers, f for the present step and g for the next: where a part has few products, a step would be four
+// waits for LDS (some 580 cycles a step of 32 x 64 sums) and is one so.
+template <class G>
+struct I8Whole {
+    v4i a[2][G::TR], b[2][G::TT];
+};
+template <class G, int B>
+__device__ __forceinline__ void i8_read_whole(I8Whole<G> &f, const uint8_t *__restrict__ buf, const I8At (&at)[2]) {
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        i8_read<G, B>(f.a[c], buf, at[B >= G::kUp].a[c], 0);
+        i8_read<G, B>(f.b[c], buf, at[B >= G::kUp].b[c], 0);
+    }
+}
+template <class G, int B, bool FULL>
+__device__ __forceinline__ void i8_step_whole(I8Src<G> &src, uint8_t *__restrict__ buf, uint8_t *__restrict__ next, u32 wave, u32 left, u32 tail,
+                                              const I8At (&at)[2], const I8Whole<G> &f, I8Whole<G> &g, v4i (&acc)[G::TR][G::TT]) {
+    if constexpr (FULL) {
+        i8_turn<G, G::kRing - 2>();
+        i8_ask<G>(src, buf, wave, false);
+    } else if (left > 0) {
+        if (G::kRing == 2 || left == 1) i8_turn<G, 0>();
+        else if (left == 2) i8_turn<G, G::kRing == 2 ? 0 : 1>();
+        else i8_turn<G, G::kRing - 2>();
+        if (left >= (u32)G::kRing) i8_ask<G>(src, buf, wave, left == (u32)G::kRing);
+        else if (left == 1 && tail < 8) i8_zero_past<G>(next, tail);
+    }
+    if (FULL || left > 0) i8_read_whole<G, (B + 1) % G::kRing>(g, next, at);
+#pragma unroll
+    for (int c = 0; c < 2; c++) i8_multiply(f.a[c], f.b[c], acc);
+}
+
 // Where piece p of column c lies in a line of LINE pieces: turned by the column within the pieces' largest power of two.
 template <int LINE>
 __device__ __forceinline__ u32 i8_turned(u32 p, u32 c) {
@@ -680,9 +715,9 @@ __device__ __forceinline__ void i8_tile_out(const I8Args &a, const I8Run &run, u
     }
 }
 
-template <int BT, int BR, int WT, int WR, int S, int EU>
+template <int BT, int BR, int WT, int WR, int S, bool WHOLE, int EU>
 __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU))) void k_i8_tile(I8Args a, u32 n_row_tiles, u32 group) {
-    using G = I8Tile<BT, BR, WT, WR, S>;
+    using G = I8Tile<BT, BR, WT, WR, S, WHOLE>;
     // in this order: the larger alignment comes first
     __shared__ __align__(4096) uint8_t ring0[G::kStage];
     __shared__ __align__(2048) uint8_t ring1[G::kStage];
@@ -754,11 +789,45 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     if (steps >= (u32)S) i8_turn<G, S - 1>();
     else i8_turn<G, 0>();
     if (steps == 1 && tail < 8) i8_zero_past<G>(ring0, tail);
-    v4i a0[G::H0], b0[G::TT];
-    i8_read<G, 0>(a0, ring0, at[0].a[0], 0);
-    i8_read<G, 0>(b0, ring0, at[0].b[0], 0);
     u32 left = steps - 1;
-    if constexpr (S == 2) {
+    if constexpr (WHOLE) {
+        // (rings of an even number of buffers: the two sets of registers change places with every step)
+        I8Whole<G> f, g;
+        i8_read_whole<G, 0>(f, ring0, at);
+        if constexpr (S == 2) {
+            for (; left >= 4; left -= 2) {
+                i8_step_whole<G, 0, true>(src, ring0, ring1, wave, 0, 0, at, f, g, acc);
+                i8_step_whole<G, 1, true>(src, ring1, ring0, wave, 0, 0, at, g, f, acc);
+            }
+            for (;;) {
+                i8_step_whole<G, 0, false>(src, ring0, ring1, wave, left, tail, at, f, g, acc);
+                if (left-- == 0) break;
+                i8_step_whole<G, 1, false>(src, ring1, ring0, wave, left, tail, at, g, f, acc);
+                if (left-- == 0) break;
+            }
+        } else {
+            for (; left >= 8; left -= 4) {
+                i8_step_whole<G, 0, true>(src, ring0, ring1, wave, 0, 0, at, f, g, acc);
+                i8_step_whole<G, 1, true>(src, ring1, ring2, wave, 0, 0, at, g, f, acc);
+                i8_step_whole<G, 2, true>(src, ring2, ring3, wave, 0, 0, at, f, g, acc);
+                i8_step_whole<G, 3, true>(src, ring3, ring0, wave, 0, 0, at, g, f, acc);
+            }
+            for (;;) {
+                i8_step_whole<G, 0, false>(src, ring0, ring1, wave, left, tail, at, f, g, acc);
+                if (left-- == 0) break;
+                i8_step_whole<G, 1, false>(src, ring1, ring2, wave, left, tail, at, g, f, acc);
+                if (left-- == 0) break;
+                i8_step_whole<G, 2, false>(src, ring2, ring3, wave, left, tail, at, f, g, acc);
+                if (left-- == 0) break;
+                i8_step_whole<G, 3, false>(src, ring3, ring0, wave, left, tail, at, g, f, acc);
+                if (left-- == 0) break;
+            }
+        }
+    } else {
+        static_assert(WHOLE || S == 2, "parts of a step in a ring of two");
+        v4i a0[G::H0], b0[G::TT];
+        i8_read<G, 0>(a0, ring0, at[0].a[0], 0);
+        i8_read<G, 0>(b0, ring0, at[0].b[0], 0);
         for (; left >= 4; left -= 2) {
             i8_step<G, 0, true>(src, ring0, ring1, wave, 0, 0, at, a0, b0, acc);
             i8_step<G, 1, true>(src, ring1, ring0, wave, 0, 0, at, a0, b0, acc);
@@ -767,23 +836,6 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
             i8_step<G, 0, false>(src, ring0, ring1, wave, left, tail, at, a0, b0, acc);
             if (left-- == 0) break;
             i8_step<G, 1, false>(src, ring1, ring0, wave, left, tail, at, a0, b0, acc);
-            if (left-- == 0) break;
-        }
-    } else {
-        for (; left >= 8; left -= 4) {
-            i8_step<G, 0, true>(src, ring0, ring1, wave, 0, 0, at, a0, b0, acc);
-            i8_step<G, 1, true>(src, ring1, ring2, wave, 0, 0, at, a0, b0, acc);
-            i8_step<G, 2, true>(src, ring2, ring3, wave, 0, 0, at, a0, b0, acc);
-            i8_step<G, 3, true>(src, ring3, ring0, wave, 0, 0, at, a0, b0, acc);
-        }
-        for (;;) {
-            i8_step<G, 0, false>(src, ring0, ring1, wave, left, tail, at, a0, b0, acc);
-            if (left-- == 0) break;
-            i8_step<G, 1, false>(src, ring1, ring2, wave, left, tail, at, a0, b0, acc);
-            if (left-- == 0) break;
-            i8_step<G, 2, false>(src, ring2, ring3, wave, left, tail, at, a0, b0, acc);
-            if (left-- == 0) break;
-            i8_step<G, 3, false>(src, ring3, ring0, wave, left, tail, at, a0, b0, acc);
             if (left-- == 0) break;
         }
     }
@@ -799,7 +851,7 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
 // Whether a launch along one dimension has fewer threads than its limit, 2^32.
 static bool i8_launchable(uint64_t groups, u32 threads) { return groups * threads <= 0xffffffffu; }
 
-template <int BT, int BR, int WT, int WR, int S, int EU>
+template <int BT, int BR, int WT, int WR, int S, bool WHOLE, int EU>
 static hipError_t tile_launch(const Launch &L, const I8Args &a, u32 entries) {
     const u32 row_tiles = (a.rows + BR - 1) / BR;
     u32 tiles = (entries + BT - 1) / BT;
@@ -807,7 +859,7 @@ static hipError_t tile_launch(const Launch &L, const I8Args &a, u32 entries) {
     const u32 group = a.start && row_tiles < 8 ? 2 : 0;
     if (group) tiles = (tiles + 8 * group - 1) / (8 * group) * (8 * group);
     if (!i8_launchable((uint64_t)tiles * row_tiles, 64 * WT * WR)) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((k_i8_tile<BT, BR, WT, WR, S, EU>), dim3(tiles * row_tiles), dim3(64 * WT * WR), 0, L.stream, a, row_tiles, group);
+    hipLaunchKernelGGL((k_i8_tile<BT, BR, WT, WR, S, WHOLE, EU>), dim3(tiles * row_tiles), dim3(64 * WT * WR), 0, L.stream, a, row_tiles, group);
     return hipGetLastError();
 }
 
@@ -877,22 +929,22 @@ hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_expe
     const bool reach = !order || (uint64_t)n_cols * a.kp <= 0xffffffffu;
     if (start && reach && n > 16) {
         const u32 each = n / (u32)n_experts;
-        if (each >= 512) return tile_launch<256, 256, 4, 2, 2, 2>(L, a, n);
+        if (each >= 512) return tile_launch<256, 256, 4, 2, 2, false, 2>(L, a, n);
         // 64 x 256 where its tiles (half a tile more an expert) are one round of two a compute unit, or the runs long
-        if (each >= 96 || (each >= 12 && (uint64_t)(n / 64 + (u32)n_experts / 2) * up(a.rows, 256) <= 512)) return tile_launch<64, 256, 1, 4, 2, 2>(L, a, n);
-        if (each >= 12) return tile_launch<64, 128, 1, 4, 2, 2>(L, a, n);
-        return tile_launch<32, 64, 1, 2, 2, 2>(L, a, n);
+        if (each >= 96 || (each >= 12 && (uint64_t)(n / 64 + (u32)n_experts / 2) * up(a.rows, 256) <= 512)) return tile_launch<64, 256, 1, 4, 2, false, 2>(L, a, n);
+        if (each >= 12) return tile_launch<64, 128, 1, 4, 2, false, 2>(L, a, n);
+        return tile_launch<32, 64, 1, 2, 2, false, 2>(L, a, n);
     }
     if (!start && n > 32 && tiles(32, 64) >= 96) {
         if (tiles(256, 256) >= 96) {
             const uint64_t by256 = 64 * ((tiles(256, 256) + 255) / 256), by224 = 57 * ((tiles(256, 224) + 255) / 256), by128 = 39 * ((tiles(128, 128) + 511) / 512);
-            if (by256 <= by224 && by256 <= by128) return tile_launch<256, 256, 4, 2, 2, 2>(L, a, n);
-            return by224 <= by128 ? tile_launch<256, 224, 4, 2, 2, 2>(L, a, n) : tile_launch<128, 128, 2, 2, 2, 2>(L, a, n);
+            if (by256 <= by224 && by256 <= by128) return tile_launch<256, 256, 4, 2, 2, false, 2>(L, a, n);
+            return by224 <= by128 ? tile_launch<256, 224, 4, 2, 2, false, 2>(L, a, n) : tile_launch<128, 128, 2, 2, 2, false, 2>(L, a, n);
         }
-        if (tiles(128, 128) >= 320) return tile_launch<128, 128, 2, 2, 2, 2>(L, a, n);
-        if (tiles(64, 128) >= 256) return tile_launch<64, 128, 1, 4, 2, 2>(L, a, n);
-        if (tiles(64, 64) >= 192) return tile_launch<64, 64, 2, 2, 4, 2>(L, a, n);
-        return tile_launch<32, 64, 1, 2, 4, 2>(L, a, n);
+        if (tiles(128, 128) >= 320) return tile_launch<128, 128, 2, 2, 2, false, 2>(L, a, n);
+        if (tiles(64, 128) >= 256) return tile_launch<64, 128, 1, 4, 2, false, 2>(L, a, n);
+        if (tiles(64, 64) >= 192) return tile_launch<64, 64, 2, 2, 4, true, 2>(L, a, n);
+        return tile_launch<32, 64, 1, 2, 4, true, 2>(L, a, n);
     }
     const bool wide = (start ? (uint64_t)(n < (u32)n_experts ? n : (u32)n_experts) : 1) * up(a.rows, 16) >= 320;
     if (n <= 16 || start) return wide ? few_launch<2, 1, 4, 4>(L, a, n) : few_launch<1, 1, 8, 2>(L, a, n);
