@@ -234,33 +234,121 @@ __device__ __forceinline__ void i8_store4(const I8Args &a, u32 j, u32 r, const f
     else elem_store_some<kElemBF16, 4>(a.y, at, have, v);
 }
 
-// Few columns a matrix: 16 R rows a workgroup against 16 C columns, its NW waves dealing the row's 128-byte lines among them. Weights go
-// from memory to registers in the form v_mfma_i32_16x16x64_i8 takes them (lane l: row l % 16, bytes 16 (l / 16) .. + 15 of the step), each once;
-// the columns come from the cache. The waves' sums meet in LDS as integers.
-template <int R, int C, int NW, int U>
+// ---- lines through LDS. 128-byte lines of k, eight 16-byte pieces each, come from memory straight into LDS (16 bytes a lane, no register in between),
+// eight lanes a line: asked for in the matrix instructions' own form, sixteen rows side by side in neighbouring lanes, a line would take the
+// vector cache four times as long. Piece c of line r lies at place c ^ swizzle(r), which the lane that asks for it arranges, so that the
+// pieces that the matrix instructions take of 16 lines at once come from all the banks.
+typedef __attribute__((address_space(1))) void i8_gptr;
+typedef __attribute__((address_space(3))) void i8_lptr;
+
+__device__ __forceinline__ u32 i8_swizzle(u32 line) { return (line >> 1) & 7; }
+
+// N groups of eight lines of a wave's own, a stage of its ring. Line l of rows that end before the piece does is read at its first
+// piece, which is there; whoever multiplies puts zeros in the columns' place.
+template <int N>
+struct I8Lines {
+    static constexpr int kStage = N * 1024;
+    const int8_t *from[N]; // this lane's row of each group
+    u32 piece[2];          // and its piece, of even and odd groups
+    __device__ __forceinline__ void begin(u32 lane) {
+#pragma unroll
+        for (u32 g = 0; g < 2; g++) piece[g] = 16 * ((lane & 7) ^ i8_swizzle(8 * g + (lane >> 3)));
+    }
+    __device__ __forceinline__ void ask(uint8_t *stage, u32 line, u32 kp) const {
+        u32 at[2];
+#pragma unroll
+        for (int g = 0; g < 2; g++) at[g] = 128 * line + (128 * line + piece[g] < kp ? piece[g] : 0u);
+#pragma unroll
+        for (int g = 0; g < N; g++) __builtin_amdgcn_global_load_lds((i8_gptr *)(from[g] + at[g & 1]), (i8_lptr *)(stage + g * 1024), 16, 0, 0);
+    }
+};
+// What the matrix instructions take of line group t (sixteen lines) of a stage: half c of the lines.
+__device__ __forceinline__ v4i i8_of_line(const uint8_t *stage, u32 lane, int t, int c) {
+    return *reinterpret_cast<const v4i *>(stage + t * 2048 + (lane & 15) * 128 + 16 * ((4 * c + (lane >> 4)) ^ i8_swizzle(lane & 15)));
+}
+// All but the last n of a wave's loads have landed, and its reads are done.
+template <int n>
+__device__ __forceinline__ void i8_landed() {
+    static_assert(n < 64, "vmcnt");
+    __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (n & 15) | (n >> 4) << 14); // vmcnt(n) lgkmcnt(0)
+    __asm__ volatile("" ::: "memory");
+}
+
+// The workgroup's writes to LDS are there for all of it; loads on their way into LDS are not waited for.
+__device__ __forceinline__ void i8_meet() {
+    __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f); // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __asm__ volatile("" ::: "memory");
+}
+
+// Few columns a matrix: 16 R rows a workgroup against 16 C columns, its NW waves dealing the row's lines among them, each through a ring of four
+// stages of its own, two on their way while one is multiplied and the fourth is asked for. The waves' sums meet in LDS as integers.
+template <int R, int C, int NW>
 __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
-    __shared__ v4i part[NW][R * C][64];
-    const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = threadIdx.x;
+    typedef I8Lines<2 * (R + C)> L;
+    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[NW * L::kStage], ring3[NW * L::kStage];
+    static_assert(R * C * 1024 <= L::kStage && R * C <= NW, "a wave's sums lie in its stage, one piece a thread");
+    const u32 lane = threadIdx.x & 63, tid = threadIdx.x, wave = (u32)__builtin_amdgcn_readfirstlane(tid >> 6);
     I8Run run;
     if (!i8_run(a, blockIdx.y, run)) return;
-    const u32 r0 = blockIdx.x * (16 * R), lines = (a.kp + 127) / 128;
-    const int8_t *wp[R];
+    const u32 r0 = blockIdx.x * (16 * R), lines = (a.kp + 127) / 128, mine = wave * L::kStage;
+    L src;
+    src.begin(lane);
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        const u32 row = r0 + 16 * r + (lane & 15);
-        wp[r] = run.w + (size_t)(row < a.rows ? row : a.rows - 1) * a.kp; // rows past the last are not stored
-    }
+    for (u32 g = 0; g < 2 * R; g++) src.from[g] = run.w + (size_t)min(r0 + 8 * g + (lane >> 3), a.rows - 1) * a.kp; // rows past the last are not stored
     for (u32 t0 = run.j0 + blockIdx.z * (16 * C); t0 < run.j1; t0 += gridDim.z * (16 * C)) {
-        const int8_t *qp[C];
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            const u32 j = t0 + 16 * c + (lane & 15);
+        for (u32 g = 0; g < 2 * C; g++) {
             bool bad;
-            qp[c] = a.q + (size_t)i8_column(a, j < run.j1 ? j : run.j1 - 1, bad) * a.kp;
+            src.from[2 * R + g] = a.q + (size_t)i8_column(a, min(t0 + 8 * g + (lane >> 3), run.j1 - 1), bad) * a.kp;
         }
-        // a thread's outputs at the end - four rows (4 (l / 16) ..) of one column (l % 16) of tile tid / 64 - and their scales, asked for now
-        static_assert(R * C <= NW, "one piece a thread");
-        const u32 tile = tid / 64, j = t0 + 16 * (tile % C) + (lane & 15), row = r0 + 16 * (tile / C) + 4 * (lane >> 4);
+        if (wave < lines) src.ask(ring0 + mine, wave, a.kp);
+        if (wave + NW < lines) src.ask(ring1 + mine, wave + NW, a.kp);
+        if (wave + 2 * NW < lines) src.ask(ring2 + mine, wave + 2 * NW, a.kp);
+        v4i acc[R][C];
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int c = 0; c < C; c++) acc[r][c] = v4i{0, 0, 0, 0};
+        const auto step = [&](const uint8_t *stage, uint8_t *free, u32 l) {
+            constexpr int n = 2 * (R + C);
+            if (l + 2 * NW < lines) i8_landed<2 * n>();
+            else if (l + NW < lines) i8_landed<n>();
+            else i8_landed<0>();
+            v4i A[2][R], B[2][C];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int r = 0; r < R; r++) A[h][r] = i8_of_line(stage + mine, lane, r, h);
+#pragma unroll
+                for (int c = 0; c < C; c++) B[h][c] = i8_of_line(stage + mine, lane, R + c, h);
+            }
+            if (l + 3 * NW < lines) src.ask(free + mine, l + 3 * NW, a.kp);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const bool in = 128 * l + 64 * h + 16 * (lane >> 4) < a.kp;
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    const v4i b = in ? B[h][c] : v4i{0, 0, 0, 0};
+#pragma unroll
+                    for (int r = 0; r < R; r++) acc[r][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[h][r], b, acc[r][c], 0, 0, 0);
+                }
+            }
+        };
+        for (u32 l = wave; l < lines;) {
+            step(ring0, ring3, l);
+            if ((l += NW) >= lines) break;
+            step(ring1, ring0, l);
+            if ((l += NW) >= lines) break;
+            step(ring2, ring1, l);
+            if ((l += NW) >= lines) break;
+            step(ring3, ring2, l);
+            l += NW;
+        }
+        // a thread's outputs: four rows (4 (l / 16) ..) of one column (l % 16) of tile tid / 64
+        const u32 tile = wave, j = t0 + 16 * (tile % C) + (lane & 15), row = r0 + 16 * (tile / C) + 4 * (lane >> 4);
         const bool out = tile < R * C && j < run.j1 && row < a.rows;
         float scale = 0.0f, row_scale[4];
         if (out) {
@@ -271,56 +359,16 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
 #pragma unroll
             for (int x = 0; x < 4; x++) row_scale[x] = run.ws[min(row + x, a.rows - 1)];
         }
-        v4i acc[R][C];
+        i8_landed<0>();
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int c = 0; c < C; c++) acc[r][c] = v4i{0, 0, 0, 0};
-        // U halves of lines asked for at a time (a line's two by one wave, one after the other: the second comes from the vector cache), the next U
-        // while these are multiplied
-        static_assert(U % 2 == 0, "whole lines");
-        v4i A[2][U][R], B[2][U][C];
-        auto ask = [&](u32 s, v4i (&fa)[U][R], v4i (&fb)[U][C]) {
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const u32 at = 128 * (s + u / 2 * NW) + 64 * (u % 2) + 16 * (lane >> 4), off = at < a.kp ? at : 0; // past the row: its first bytes, against zeros
-#pragma unroll
-                for (int r = 0; r < R; r++) fa[u][r] = *reinterpret_cast<const v4i *>(wp[r] + off);
-#pragma unroll
-                for (int c = 0; c < C; c++) fb[u][c] = *reinterpret_cast<const v4i *>(qp[c] + off);
-            }
-        };
-        auto multiply = [&](u32 s, v4i (&fa)[U][R], v4i (&fb)[U][C]) {
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const bool in = 128 * (s + u / 2 * NW) + 64 * (u % 2) + 16 * (lane >> 4) < a.kp;
-#pragma unroll
-                for (int c = 0; c < C; c++) {
-                    const v4i b = in ? fb[u][c] : v4i{0, 0, 0, 0};
-#pragma unroll
-                    for (int r = 0; r < R; r++) acc[r][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[u][r], b, acc[r][c], 0, 0, 0);
-                }
-            }
-        };
-        u32 s = wave;
-        ask(s, A[0], B[0]);
-        for (;;) {
-            if (s + U / 2 * NW < lines) ask(s + U / 2 * NW, A[1], B[1]);
-            multiply(s, A[0], B[0]);
-            if ((s += U / 2 * NW) >= lines) break;
-            if (s + U / 2 * NW < lines) ask(s + U / 2 * NW, A[0], B[0]);
-            multiply(s, A[1], B[1]);
-            if ((s += U / 2 * NW) >= lines) break;
-        }
-#pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int c = 0; c < C; c++) part[wave][r * C + c][lane] = acc[r][c];
+            for (int c = 0; c < C; c++) *reinterpret_cast<v4i *>(ring0 + mine + (r * C + c) * 1024 + 16 * lane) = acc[r][c];
         __syncthreads();
         if (out) {
-            v4i sum = part[0][tile][lane];
+            v4i sum = v4i{0, 0, 0, 0};
 #pragma unroll
-            for (int w = 1; w < NW; w++) sum += part[w][tile][lane];
+            for (int w = 0; w < NW; w++) sum += *reinterpret_cast<const v4i *>(ring0 + w * L::kStage + tile * 1024 + 16 * lane);
             float v[4];
 #pragma unroll
             for (int x = 0; x < 4; x++) v[x] = __fmul_rn(__fmul_rn((float)sum[x], scale), row_scale[x]);
@@ -338,48 +386,37 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
 // So: up to four rows of what four pieces a thread hold, eight rows of half that.
 constexpr int kFewX = 8, kFewXWaves = 8; // rows at most
 constexpr u32 few_x_values(u32 M) { return 64 * kFewXWaves * (M < 8 ? 32 : 16) / M; } // values a row may have
-template <int ET, int M, int R, int U>
+template <int ET, int M, int R>
 __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArgs qa) {
     constexpr int NW = kFewXWaves, T = 64 * NW / M; // threads a row
+    typedef I8Lines<2 * R> L;
     extern __shared__ __align__(16) uint8_t few_lds[];
     int8_t *codes = reinterpret_cast<int8_t *>(few_lds); // M rows of kp
-    __shared__ v4i part[NW][R][64];
+    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[NW * L::kStage], ring3[NW * L::kStage];
+    static_assert(R * 1024 <= L::kStage && R <= NW, "a wave's sums lie in its stage, one piece a thread");
     __shared__ u32 top[NW];
     __shared__ float scale[M];
-    const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lines = (a.kp + 127) / 128, r0 = blockIdx.x * (16 * R);
-    const int8_t *wp[R];
-#pragma unroll
-    for (int r = 0; r < R; r++) wp[r] = a.w + (size_t)min(r0 + 16 * r + (lane & 15), a.rows - 1) * a.kp;
-    v4i A[2][U][R];
-    const auto ask = [&](u32 s, v4i (&f)[U][R]) {
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const u32 at = 128 * (s + u / 2 * NW) + 64 * (u % 2) + 16 * (lane >> 4), off = at < a.kp ? at : 0; // past the row: its first bytes, against zeros
-#pragma unroll
-            for (int r = 0; r < R; r++) f[u][r] = *reinterpret_cast<const v4i *>(wp[r] + off);
-        }
-    };
-    // a thread's outputs at the end, and the scales of their rows
-    static_assert(R <= NW, "one piece a thread");
-    const u32 j = lane & 15, out = r0 + 16 * wave + 4 * (lane >> 4);
-    const bool mine_out = wave < R && j < a.m && out < a.rows;
-    float row_scale[4];
-    if (mine_out)
-#pragma unroll
-        for (int x = 0; x < 4; x++) row_scale[x] = a.ws[min(out + x, a.rows - 1)];
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = (u32)__builtin_amdgcn_readfirstlane(tid >> 6);
+    const u32 lines = (a.kp + 127) / 128, r0 = blockIdx.x * (16 * R), mine = wave * L::kStage;
     // the rows' values, then the first weights
-    const u32 row = tid / T, mine = tid % T, pieces = a.kp / 8;
+    const u32 row = tid / T, first = tid % T, pieces = a.kp / 8;
     float v[4][8];
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const u32 c = mine + i * T;
+        const u32 c = first + i * T;
         if (row < qa.m && c < pieces) quant_values<ET, false>(qa, row, 8 * c, v[i], odd);
         else
 #pragma unroll
             for (int j = 0; j < 8; j++) v[i][j] = 0.0f;
     }
-    ask(wave, A[0]);
+    L src;
+    src.begin(lane);
+#pragma unroll
+    for (u32 g = 0; g < 2 * R; g++) src.from[g] = a.w + (size_t)min(r0 + 8 * g + (lane >> 3), a.rows - 1) * a.kp; // rows past the last are not stored
+    if (wave < lines) src.ask(ring0 + mine, wave, a.kp);
+    if (wave + NW < lines) src.ask(ring1 + mine, wave + NW, a.kp);
+    if (wave + 2 * NW < lines) src.ask(ring2 + mine, wave + 2 * NW, a.kp);
     u32 most = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -389,13 +426,13 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
     most = max(most, (u32)__shfl_xor((int)most, 32, 64));
     if constexpr (M < NW) {
         if (lane == 0) top[wave] = most;
-        __syncthreads();
+        i8_meet();
         most = 0;
 #pragma unroll
         for (int w = 0; w < NW / M; w++) most = max(most, top[row * (NW / M) + w]);
     }
     const I8Scale sc = i8_scale(most);
-    if (mine == 0) {
+    if (first == 0) {
         scale[row] = sc.s;
         if (blockIdx.x == 0 && row < qa.m) {
             qa.scales[row] = sc.s;
@@ -404,47 +441,67 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const u32 c = mine + i * T;
+        const u32 c = first + i * T;
         if (c >= pieces) break;
         const uint2 word = i8_codes(v[i], sc);
         *reinterpret_cast<uint2 *>(codes + row * a.kp + 8 * c) = word;
         if (blockIdx.x == 0 && row < qa.m) *reinterpret_cast<uint2 *>(qa.codes + (size_t)row * a.kp + 8 * c) = word;
     }
-    __syncthreads();
+    i8_meet();
 
     v4i acc[R];
 #pragma unroll
     for (int r = 0; r < R; r++) acc[r] = v4i{0, 0, 0, 0};
     const u32 col = lane & 15;
-    const auto multiply = [&](u32 s, const v4i (&f)[U][R]) {
+    const auto step = [&](const uint8_t *stage, uint8_t *free, u32 l) {
+        constexpr int n = 2 * R;
+        if (l + 2 * NW < lines) i8_landed<2 * n>();
+        else if (l + NW < lines) i8_landed<n>();
+        else i8_landed<0>();
+        v4i A[2][R], B[2];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const u32 at = 128 * (s + u / 2 * NW) + 64 * (u % 2) + 16 * (lane >> 4);
-            v4i b = v4i{0, 0, 0, 0};
-            if (col < (u32)M && at < a.kp) b = *reinterpret_cast<const v4i *>(codes + col * a.kp + at);
+        for (int h = 0; h < 2; h++) {
+            const u32 at = 128 * l + 64 * h + 16 * (lane >> 4);
+            B[h] = v4i{0, 0, 0, 0};
+            if (col < (u32)M && at < a.kp) B[h] = *reinterpret_cast<const v4i *>(codes + col * a.kp + at);
 #pragma unroll
-            for (int r = 0; r < R; r++) acc[r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[u][r], b, acc[r], 0, 0, 0);
+            for (int r = 0; r < R; r++) A[h][r] = i8_of_line(stage + mine, lane, r, h);
         }
-    };
-    for (u32 s = wave;;) {
-        if (s + U / 2 * NW < lines) ask(s + U / 2 * NW, A[1]);
-        multiply(s, A[0]);
-        if ((s += U / 2 * NW) >= lines) break;
-        if (s + U / 2 * NW < lines) ask(s + U / 2 * NW, A[0]);
-        multiply(s, A[1]);
-        if ((s += U / 2 * NW) >= lines) break;
-    }
+        if (l + 3 * NW < lines) src.ask(free + mine, l + 3 * NW, a.kp);
 #pragma unroll
-    for (int r = 0; r < R; r++) part[wave][r][lane] = acc[r];
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int r = 0; r < R; r++) acc[r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[h][r], B[h], acc[r], 0, 0, 0);
+    };
+    for (u32 l = wave; l < lines;) {
+        step(ring0, ring3, l);
+        if ((l += NW) >= lines) break;
+        step(ring1, ring0, l);
+        if ((l += NW) >= lines) break;
+        step(ring2, ring1, l);
+        if ((l += NW) >= lines) break;
+        step(ring3, ring2, l);
+        l += NW;
+    }
+    // a thread's outputs: four rows (4 (l / 16) ..) of one column (l % 16) of tile tid / 64
+    const u32 out = r0 + 16 * wave + 4 * (lane >> 4);
+    const bool mine_out = wave < R && col < a.m && out < a.rows;
+    float row_scale[4];
+    if (mine_out)
+#pragma unroll
+        for (int x = 0; x < 4; x++) row_scale[x] = a.ws[min(out + x, a.rows - 1)];
+    i8_landed<0>();
+#pragma unroll
+    for (int r = 0; r < R; r++) *reinterpret_cast<v4i *>(ring0 + mine + r * 1024 + 16 * lane) = acc[r];
     __syncthreads();
     if (!mine_out) return;
-    v4i sum = part[0][wave][lane];
+    v4i sum = v4i{0, 0, 0, 0};
 #pragma unroll
-    for (int w = 1; w < NW; w++) sum += part[w][wave][lane];
+    for (int w = 0; w < NW; w++) sum += *reinterpret_cast<const v4i *>(ring0 + w * L::kStage + wave * 1024 + 16 * lane);
     float y[4];
 #pragma unroll
-    for (int x = 0; x < 4; x++) y[x] = __fmul_rn(__fmul_rn((float)sum[x], scale[j]), row_scale[x]);
-    i8_store4(a, j, out, y);
+    for (int x = 0; x < 4; x++) y[x] = __fmul_rn(__fmul_rn((float)sum[x], scale[col]), row_scale[x]);
+    i8_store4(a, col, out, y);
 }
 
 // Many columns a matrix: BT columns x BR rows a workgroup, 128 bytes of k a step through a ring of S LDS buffers, where the loads put them
@@ -452,9 +509,6 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
 // wave holds (BT / WT) x (BR / WR) sums in v_mfma_i32_16x16x64_i8's form.
 // A step's rows are 128-byte lines of eight 16-byte pieces; piece c of line r lies at place c ^ swizzle(r), which the lane that asks for it
 // arranges, so that the pieces that the matrix instructions take of 16 lines at once come from all the banks.
-typedef __attribute__((address_space(1))) void i8_gptr;
-typedef __attribute__((address_space(3))) void i8_lptr;
-
 template <int BT, int BR, int WT, int WR, int S, bool WHOLE>
 struct I8Tile {
     static constexpr bool kWhole = WHOLE;
@@ -467,8 +521,6 @@ struct I8Tile {
     // buffers from this one on lie past what a read's constant reaches
     static constexpr int kUp = S * kStage <= 65536 ? S : S / 2;
 };
-
-__device__ __forceinline__ u32 i8_swizzle(u32 line) { return (line >> 1) & 7; }
 
 // A tile of the experts: their runs cut into tiles of BT entries, numbered through the experts in order. False: there is none of that number. The bounds
 // of 256 experts are asked for at once; a run that is none raises ExpertId (once a launch and wave of the first tile) and has no tiles.
@@ -863,17 +915,17 @@ static hipError_t tile_launch(const Launch &L, const I8Args &a, u32 entries) {
     return hipGetLastError();
 }
 
-template <int R, int C, int NW, int U>
+template <int R, int C, int NW>
 static hipError_t few_launch(const Launch &L, const I8Args &a, u32 entries) {
     const u32 z = a.start ? 1u : (entries + 16 * C - 1) / (16 * C);
-    hipLaunchKernelGGL((k_i8_few<R, C, NW, U>), dim3((a.rows + 16 * R - 1) / (16 * R), a.start ? a.n_experts : 1u, z < 65535u ? z : 65535u), dim3(64 * NW), 0,
+    hipLaunchKernelGGL((k_i8_few<R, C, NW>), dim3((a.rows + 16 * R - 1) / (16 * R), a.start ? a.n_experts : 1u, z < 65535u ? z : 65535u), dim3(64 * NW), 0,
                        L.stream, a);
     return hipGetLastError();
 }
 
 template <int ET, int M, int R>
 static void few_x_launch(const Launch &L, const I8Args &a, const QuantArgs &q) {
-    hipLaunchKernelGGL((k_i8_few_x<ET, M, R, 2>), dim3((a.rows + 16 * R - 1) / (16 * R)), dim3(64 * kFewXWaves), M * a.kp, L.stream, a, q);
+    hipLaunchKernelGGL((k_i8_few_x<ET, M, R>), dim3((a.rows + 16 * R - 1) / (16 * R)), dim3(64 * kFewXWaves), M * a.kp, L.stream, a, q);
 }
 template <int ET, int M>
 static void few_x_by_rows(const Launch &L, const I8Args &a, const QuantArgs &q) {
@@ -907,11 +959,12 @@ hipError_t i8_gemm_x(const Launch &L, const int8_t *w, const float *ws, int rows
 //   One matrix. Large tiles are the better the more of them there are, and whole rounds of 256 compute units count: a round of 256 x 256 tiles takes
 //   64 units of time, of 256 x 224 57, of two 128 x 128 a unit 39. (4096 x 7168 x 7168: 512 tiles of 224 rows are two rounds, 179, 448 of 256 take
 //   the same two, 198, 128 x 128 223; 4096 cubed 58, 90, 66; 8192 cubed 453, 507, 538; 4096 x 2048 x 7168, the 128 x 128 first, 59, 80, 69.)
-//   Below some hundred large tiles the smaller ones fill the card: 1024 x 7168 x 2048 in 128 x 128 21.5 (64 x 128: 26.4); 2048 cubed in 64 x 128 14.7
-//   (128 x 128: 16.9); 256 x 7168 x 2048 in 64 x 64 9.9 (64 x 128: 12.3); 128 x 2048 x 7168 in 32 x 64 15.1 (64 x 64: 15.8), the last two with
-//   four steps in flight, as few workgroups need. Up to 32 columns, and where even those tiles are few, every workgroup's waves share a row's k: 24 x 7168 x 2048 6.5
-//   (32 x 64: 7.5), 64 x 2048 x 7168 12.0 (15.0); 16 x 7168 x 2048 5.8 (7.3), 1 x 2048 x 7168 6.6 (14.8). There two tiles of 16 rows a workgroup of four waves
-//   from 320 tiles on (24 columns: 6.5 against 7.8), else one of eight waves (1 x 2048 x 7168: 6.6 against 9.9).
+//   Below some hundred large tiles the smaller ones fill the card: 1024 x 7168 x 2048 in 128 x 128 21.6 (64 x 128: 27.8); 2048 cubed in 64 x 128 15.4
+//   (128 x 128: 16.1); 256 x 7168 x 2048 in 64 x 64 10.4 (64 x 128: 12.9); 256 x 2048 x 7168 in 32 x 64 13.5 (64 x 64: 14.4), the last two with four steps in
+//   flight, as few workgroups need.
+//   Where tiles of at most 32 x 32 are no more than the compute units, a workgroup's waves share a row's k (k_i8_few), in the smallest tile that is one
+//   round: 34 x 544 x 8064 in 16 x 16 5.6 (16 x 32: 7.0, 32 x 64 whole rows 13), 64 x 2048 x 7168 in 16 x 32 6.5 (32 x 32: 7.9; 12.8), 128 x 2048 x 7168 in 32 x 32 8.1 (16 x 32:
+//   11.2; 12.9), 24 x 7168 x 2048 5.1 (7.1), one row of 2048 x 7168 4.9, of 7168 x 7168 9.6; two rounds lose, 64 x 7168 x 2048 8.2 (32 x 64: 7.5).
 //   Experts, by slots an expert: 4096 tokens, top 8 of 32 (1024 slots each), 7168 x 2048 rows in 256 x 256 595 (128 x 128: 658, 64 x 256: 714); 2048 tokens, top 8 of 128, 768 x 2048
 //   in 64 x 256 72 (256 x 256: 79, 128 x 128: 78, 64 x 128: 76), 2048 x 768 87 (103, 91, 91); 512 tokens 46 (64 x 128: 51), one round of tiles; 1024 tokens in 64 x 128 58
 //   (64 x 256: 63), 333 tokens, top 8 of 64, 7168 x 2048 189 (193; own columns, f16, 156 and 166); 128 tokens
@@ -927,28 +980,28 @@ hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_expe
     const auto tiles = [&](u32 bt, u32 br) { return (uint64_t)up(n, bt) * up(a.rows, br); };
     // the tiles' offsets of gathered columns are 32 bits
     const bool reach = !order || (uint64_t)n_cols * a.kp <= 0xffffffffu;
-    if (start && reach && n > 16) {
+    if (start) {
+        if (n <= 32 || !reach) return few_launch<2, 1, 3>(L, a, n);
         const u32 each = n / (u32)n_experts;
         if (each >= 512) return tile_launch<256, 256, 4, 2, 2, false, 2>(L, a, n);
         // 64 x 256 where its tiles (half a tile more an expert) are one round of two a compute unit, or the runs long
-        if (each >= 96 || (each >= 12 && (uint64_t)(n / 64 + (u32)n_experts / 2) * up(a.rows, 256) <= 512)) return tile_launch<64, 256, 1, 4, 2, false, 2>(L, a, n);
+        if (each >= 96 || (each >= 12 && (uint64_t)(n / 64 + (u32)n_experts / 2) * up(a.rows, 256) <= 512)) return tile_launch<64, 256, 1, 4, 2, true, 2>(L, a, n);
         if (each >= 12) return tile_launch<64, 128, 1, 4, 2, false, 2>(L, a, n);
-        return tile_launch<32, 64, 1, 2, 2, false, 2>(L, a, n);
+        return tile_launch<32, 64, 1, 2, 2, true, 2>(L, a, n);
     }
-    if (!start && n > 32 && tiles(32, 64) >= 96) {
-        if (tiles(256, 256) >= 96) {
-            const uint64_t by256 = 64 * ((tiles(256, 256) + 255) / 256), by224 = 57 * ((tiles(256, 224) + 255) / 256), by128 = 39 * ((tiles(128, 128) + 511) / 512);
-            if (by256 <= by224 && by256 <= by128) return tile_launch<256, 256, 4, 2, 2, false, 2>(L, a, n);
-            return by224 <= by128 ? tile_launch<256, 224, 4, 2, 2, false, 2>(L, a, n) : tile_launch<128, 128, 2, 2, 2, false, 2>(L, a, n);
-        }
-        if (tiles(128, 128) >= 320) return tile_launch<128, 128, 2, 2, 2, false, 2>(L, a, n);
-        if (tiles(64, 128) >= 256) return tile_launch<64, 128, 1, 4, 2, false, 2>(L, a, n);
-        if (tiles(64, 64) >= 192) return tile_launch<64, 64, 2, 2, 4, true, 2>(L, a, n);
-        return tile_launch<32, 64, 1, 2, 4, true, 2>(L, a, n);
+    if (tiles(16, 16) <= 256) return few_launch<1, 1, 8>(L, a, n);
+    if (tiles(16, 32) <= 256) return few_launch<2, 1, 4>(L, a, n);
+    if (n <= 16) return few_launch<2, 1, 3>(L, a, n);
+    if (n <= 32 || tiles(32, 32) <= 256) return few_launch<2, 2, 4>(L, a, n);
+    if (tiles(256, 256) >= 96) {
+        const uint64_t by256 = 64 * ((tiles(256, 256) + 255) / 256), by224 = 57 * ((tiles(256, 224) + 255) / 256), by128 = 39 * ((tiles(128, 128) + 511) / 512);
+        if (by256 <= by224 && by256 <= by128) return tile_launch<256, 256, 4, 2, 2, false, 2>(L, a, n);
+        return by224 <= by128 ? tile_launch<256, 224, 4, 2, 2, false, 2>(L, a, n) : tile_launch<128, 128, 2, 2, 2, true, 2>(L, a, n);
     }
-    const bool wide = (start ? (uint64_t)(n < (u32)n_experts ? n : (u32)n_experts) : 1) * up(a.rows, 16) >= 320;
-    if (n <= 16 || start) return wide ? few_launch<2, 1, 4, 4>(L, a, n) : few_launch<1, 1, 8, 2>(L, a, n);
-    return wide && n <= 32 ? few_launch<2, 2, 4, 4>(L, a, n) : few_launch<1, 2, 8, 2>(L, a, n);
+    if (tiles(128, 128) >= 320) return tile_launch<128, 128, 2, 2, 2, true, 2>(L, a, n);
+    if (tiles(64, 128) >= 256) return tile_launch<64, 128, 1, 4, 2, true, 2>(L, a, n);
+    if (tiles(64, 64) >= 192) return tile_launch<64, 64, 2, 2, 4, true, 2>(L, a, n);
+    return tile_launch<32, 64, 1, 2, 4, true, 2>(L, a, n);
 }
 
 } // namespace bmk
