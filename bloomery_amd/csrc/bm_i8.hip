@@ -98,26 +98,83 @@ __device__ __forceinline__ void quant_values(const QuantArgs &a, u32 row, u32 c,
     }
 }
 
+// A thread's CH pieces of a row, from piece `first` on, T apart: whole pieces are all asked for before the first is looked at (a thread past the last asks
+// for that one and takes zeros), the ragged one that a row may end with by itself.
+template <int ET, bool GLU, int T, int CH>
+struct QuantPieces {
+    static constexpr int V = kElemPiece<ET>, P = 8 / V;
+    uint4 x[CH][P], u[GLU ? CH : 1][P];
+    __device__ __forceinline__ void ask(const QuantArgs &a, u32 row, u32 first) {
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            const size_t at = (size_t)row * a.ld + 8 * min(first + i * T, a.k / 8 - 1);
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+                x[i][p] = elem_piece<ET>(a.x, at + p * V);
+                if constexpr (GLU) u[i][p] = elem_piece<ET>(a.u, at + p * V);
+            }
+        }
+    }
+    __device__ __forceinline__ void values(const QuantArgs &a, u32 row, u32 first, float (&v)[CH][8], bool &odd) const {
+        const u32 whole = a.k / 8;
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            const bool in = first + i * T < whole;
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+                float e[V];
+                elem_unpack<ET>(x[i][p], e);
+                if constexpr (GLU) {
+                    float f[V];
+                    elem_unpack<ET>(u[i][p], f);
+                    if (a.rule.act == 0u) { // a piece's values together, no branch between them
+#pragma unroll
+                        for (int j = 0; j < V; j++) e[j] = bm_swiglu(e[j], f[j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < V; j++) {
+                            bool o = false;
+                            e[j] = bm_gate_rule(a.rule.act, a.rule.limit, in ? e[j] : 0.0f, in ? f[j] : 0.0f, o);
+                            odd |= o;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < V; j++) v[i][p * V + j] = in ? e[j] : 0.0f;
+            }
+        }
+        if ((a.k & 7) && whole % T == first && whole / T < CH) {
+            float tail[8];
+            quant_values<ET, GLU>(a, row, 8 * whole, tail, odd);
+#pragma unroll
+            for (int i = 0; i < CH; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[i][j] = (u32)i == whole / T ? tail[j] : v[i][j];
+        }
+    }
+};
+
 // T threads a row (a wave, or the workgroup), CH pieces of eight values a thread held in registers between the maximum and the codes; CH = 0: a
 // row of any length, read twice (the second time from the cache).
 template <int ET, bool GLU, int T, int CH>
-__global__ __launch_bounds__(256) void k_i8_quantize(QuantArgs a) {
-    __shared__ u32 top[4];
-    const u32 lane = threadIdx.x % T, row = blockIdx.x * (256 / T) + threadIdx.x / T;
+__global__ __launch_bounds__(T < 256 ? 256 : T) void k_i8_quantize(QuantArgs a) {
+    constexpr int kThreads = T < 256 ? 256 : T;
+    __shared__ u32 top[T / 64];
+    const u32 lane = threadIdx.x % T, row = blockIdx.x * (kThreads / T) + threadIdx.x / T;
     const u32 m = a.live ? min(a.m, *a.live) : a.m;
-    if (row >= m) return; // whole waves (T = 64) or the workgroup (T = 256)
+    if (row >= m) return; // whole waves (T = 64) or the workgroup
     float v[CH ? CH : 1][8];
     u32 most = 0;
     bool odd = false;
     const u32 pieces = a.kp / 8;
     if constexpr (CH > 0) {
+        QuantPieces<ET, GLU, T, CH> in;
+        if (a.k >= 8) {
+            in.ask(a, row, lane);
+            in.values(a, row, lane, v, odd);
+        } else {
 #pragma unroll
-        for (int i = 0; i < CH; i++) {
-            const u32 c = lane + i * T;
-            if (c < pieces) quant_values<ET, GLU>(a, row, 8 * c, v[i], odd);
-            else
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[i][j] = 0.0f;
+            for (int i = 0; i < CH; i++) quant_values<ET, GLU>(a, row, 8 * (lane + i * T), v[i], odd);
         }
 #pragma unroll
         for (int i = 0; i < CH; i++)
@@ -133,10 +190,11 @@ __global__ __launch_bounds__(256) void k_i8_quantize(QuantArgs a) {
     if (GLU && odd) bm_raise(a.fault, a.layer, kSiteF32Product);
     most = bm_max32(most);
     most = max(most, (u32)__shfl_xor((int)most, 32, 64));
-    if constexpr (T == 256) {
+    if constexpr (T > 64) {
         if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = most;
         __syncthreads();
-        most = max(max(top[0], top[1]), max(top[2], top[3]));
+#pragma unroll
+        for (int w = 0; w < T / 64; w++) most = max(most, top[w]);
     }
     const I8Scale sc = i8_scale(most);
     if (lane == 0) {
@@ -152,15 +210,24 @@ __global__ __launch_bounds__(256) void k_i8_quantize(QuantArgs a) {
         }
 }
 
+template <int ET, bool GLU, int T, int CH>
+static void quant_start(const Launch &L, const QuantArgs &a) {
+    constexpr u32 threads = T < 256 ? 256 : T, rows = threads / T;
+    hipLaunchKernelGGL((k_i8_quantize<ET, GLU, T, CH>), dim3((a.m + rows - 1) / rows), dim3(threads), 0, L.stream, a);
+}
+// us on MI355X, bf16, alone and behind the gate rule. While the rows are not eight a compute unit a row's length is dealt to more threads, a piece each: 24 x
+// 7168 4.0 and 4.2 (256 threads of four pieces: 5.5, 6.3), 1500 x 7168 10.2 and 15.2 (10.8, 16.7), 1024 x 4096 4.9 and 6.8 (5.4, 7.6); behind that more pieces a thread
+// ask for more at once: 4096 x 7168 18.2 and 32.6 (1024 threads: 22.0, 34.7); 18.2 us are 4.8 TB/s, what a copy reaches. Short rows take a wave each, 16384 x 768 11.5
+// and 19.0 (a workgroup: 16.2, 30.6).
 template <int ET, bool GLU>
 static void quant_launch(const Launch &L, const QuantArgs &a) {
-    const dim3 block(256), wave_a_row((a.m + 3) / 4), group_a_row(a.m);
-    if (a.kp <= 512) hipLaunchKernelGGL((k_i8_quantize<ET, GLU, 64, 1>), wave_a_row, block, 0, L.stream, a);
-    else if (a.kp <= 1024) hipLaunchKernelGGL((k_i8_quantize<ET, GLU, 64, 2>), wave_a_row, block, 0, L.stream, a);
-    else if (a.kp <= 2048) hipLaunchKernelGGL((k_i8_quantize<ET, GLU, 256, 1>), group_a_row, block, 0, L.stream, a);
-    else if (a.kp <= 4096) hipLaunchKernelGGL((k_i8_quantize<ET, GLU, 256, 2>), group_a_row, block, 0, L.stream, a);
-    else if (a.kp <= 8192) hipLaunchKernelGGL((k_i8_quantize<ET, GLU, 256, 4>), group_a_row, block, 0, L.stream, a);
-    else hipLaunchKernelGGL((k_i8_quantize<ET, GLU, 256, 0>), group_a_row, block, 0, L.stream, a);
+    const bool few = a.m <= 2048;
+    if (a.kp <= 512) quant_start<ET, GLU, 64, 1>(L, a);
+    else if (a.kp <= 1024) quant_start<ET, GLU, 64, 2>(L, a);
+    else if (a.kp <= 2048) quant_start<ET, GLU, 256, 1>(L, a);
+    else if (a.kp <= 4096) few ? quant_start<ET, GLU, 512, 1>(L, a) : quant_start<ET, GLU, 256, 2>(L, a);
+    else if (a.kp <= 8192) few ? quant_start<ET, GLU, 1024, 1>(L, a) : quant_start<ET, GLU, 256, 4>(L, a);
+    else quant_start<ET, GLU, 1024, 0>(L, a);
 }
 
 hipError_t i8_quantize(const Launch &L, const void *x, const void *u, int et, int64_t ld, int m, int k, const uint32_t *live, int8_t *codes,
@@ -223,6 +290,19 @@ __device__ __forceinline__ u32 i8_column(const I8Args &a, u32 j, bool &bad) {
     if (s < a.n_slots && c < a.n_cols) return c;
     bad = true;
     return 0;
+}
+
+// The columns of N entries, their slots asked for at once.
+template <int N>
+__device__ __forceinline__ void i8_columns(const I8Args &a, u32 (&j)[N]) {
+    u32 s[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) s[i] = a.order[j[i]];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const u32 c = a.top_k ? s[i] / a.top_k : j[i];
+        j[i] = s[i] < a.n_slots && c < a.n_cols ? c : 0u;
+    }
 }
 
 // Four neighbouring values of an output row from r on, those below `rows`.
@@ -299,11 +379,12 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
 #pragma unroll
     for (u32 g = 0; g < 2 * R; g++) src.from[g] = run.w + (size_t)min(r0 + 8 * g + (lane >> 3), a.rows - 1) * a.kp; // rows past the last are not stored
     for (u32 t0 = run.j0 + blockIdx.z * (16 * C); t0 < run.j1; t0 += gridDim.z * (16 * C)) {
+        u32 col[2 * C];
 #pragma unroll
-        for (u32 g = 0; g < 2 * C; g++) {
-            bool bad;
-            src.from[2 * R + g] = a.q + (size_t)i8_column(a, min(t0 + 8 * g + (lane >> 3), run.j1 - 1), bad) * a.kp;
-        }
+        for (u32 g = 0; g < 2 * C; g++) col[g] = min(t0 + 8 * g + (lane >> 3), run.j1 - 1);
+        if (a.order) i8_columns<2 * C>(a, col);
+#pragma unroll
+        for (u32 g = 0; g < 2 * C; g++) src.from[2 * R + g] = a.q + (size_t)col[g] * a.kp;
         if (wave < lines) src.ask(ring0 + mine, wave, a.kp);
         if (wave + NW < lines) src.ask(ring1 + mine, wave + NW, a.kp);
         if (wave + 2 * NW < lines) src.ask(ring2 + mine, wave + 2 * NW, a.kp);
@@ -381,17 +462,18 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
 // A few rows from their floating values: k_i8_few's product with the quantizer in front of it in every workgroup, while the first weights are on
 // their way. M (a power of two, at least the rows): the waves are dealt to the rows, 4 pieces of eight values a thread at most. The codes
 // go to LDS; the first workgroup leaves them and the scales in memory too.
-// Ahead of the two launches while a thread has few values to quantize (us, one launch / two, bf16): 768 x 2048, one row 4.9 / 7.5, four 5.6 / 8.0, eight 7.3 /
-// 8.3; 7168 x 2048, one 5.6 / 8.1, four 7.0 / 8.2, eight 9.3 / 8.2; 7168 x 7168, one 11.9 / 17.1, two 14.5 / 17.2; 8192 x 1024, eight 5.8 / 7.9.
-// So: up to four rows of what four pieces a thread hold, eight rows of half that.
+// The values are asked for first, then three lines of weights, which stay on their way while the values become codes.
+// Ahead of the two launches wherever a thread's four pieces hold the rows (us, one launch / two, bf16): 768 x 2048, one row 5.1 / 7.4, four 6.0 / 7.7, eight 6.8 /
+// 7.6; 7168 x 2048, one 6.0 / 7.7, four 6.9 / 7.8, eight 7.5 / 7.9; 7168 x 7168, one 10.8 / 12.5, two 12.0 / 12.8; 8192 x 1024, eight 5.9 / 7.7. Tiles of 32 rows
+// where those of 16 are more than the compute units (80 KB of LDS, one a unit): 5000 x 2048, one row 5.8 (16 rows: 8.3).
 constexpr int kFewX = 8, kFewXWaves = 8; // rows at most
-constexpr u32 few_x_values(u32 M) { return 64 * kFewXWaves * (M < 8 ? 32 : 16) / M; } // values a row may have
+constexpr u32 few_x_values(u32 M) { return 64 * kFewXWaves * 8 * 4 / M; } // values a row may have
 template <int ET, int M, int R>
 __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArgs qa) {
-    constexpr int NW = kFewXWaves, T = 64 * NW / M; // threads a row
+    constexpr int NW = kFewXWaves, T = 64 * NW / M, kPieces = 4; // threads a row, pieces a thread
     typedef I8Lines<2 * R> L;
-    extern __shared__ __align__(16) uint8_t few_lds[];
-    int8_t *codes = reinterpret_cast<int8_t *>(few_lds); // M rows of kp
+    // M rows of kp. An array of its own, which no load on its way into LDS reaches: a write to it waits for none
+    __shared__ __align__(16) int8_t codes[M * few_x_values(M)];
     __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[NW * L::kStage], ring3[NW * L::kStage];
     static_assert(R * 1024 <= L::kStage && R <= NW, "a wave's sums lie in its stage, one piece a thread");
     __shared__ u32 top[NW];
@@ -400,26 +482,25 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
     const u32 lines = (a.kp + 127) / 128, r0 = blockIdx.x * (16 * R), mine = wave * L::kStage;
     // the rows' values, then the first weights
     const u32 row = tid / T, first = tid % T, pieces = a.kp / 8;
-    float v[4][8];
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const u32 c = first + i * T;
-        if (row < qa.m && c < pieces) quant_values<ET, false>(qa, row, 8 * c, v[i], odd);
-        else
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[i][j] = 0.0f;
-    }
+    QuantPieces<ET, false, T, kPieces> in;
+    in.ask(qa, min(row, qa.m - 1), first); // rows past the last are the last once more, and not multiplied
     L src;
     src.begin(lane);
 #pragma unroll
     for (u32 g = 0; g < 2 * R; g++) src.from[g] = a.w + (size_t)min(r0 + 8 * g + (lane >> 3), a.rows - 1) * a.kp; // rows past the last are not stored
-    if (wave < lines) src.ask(ring0 + mine, wave, a.kp);
-    if (wave + NW < lines) src.ask(ring1 + mine, wave + NW, a.kp);
-    if (wave + 2 * NW < lines) src.ask(ring2 + mine, wave + 2 * NW, a.kp);
+    // three lines whether or not there are as many (then the last once more): the wait for the values leaves a known number of loads on their way
+    src.ask(ring0 + mine, min(wave, lines - 1), a.kp);
+    src.ask(ring1 + mine, min(wave + NW, lines - 1), a.kp);
+    src.ask(ring2 + mine, min(wave + 2 * NW, lines - 1), a.kp);
+    __builtin_amdgcn_sched_barrier(0);
+    i8_landed<6 * R>();
+    __builtin_amdgcn_sched_barrier(0);
+    float v[kPieces][8];
+    bool odd = false;
+    in.values(qa, min(row, qa.m - 1), first, v, odd);
     u32 most = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < kPieces; i++)
 #pragma unroll
         for (int j = 0; j < 8; j++) most = max(most, bm_f32_bits(v[i][j]) & 0x7fffffffu);
     most = bm_max32(most);
@@ -440,7 +521,7 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < kPieces; i++) {
         const u32 c = first + i * T;
         if (c >= pieces) break;
         const uint2 word = i8_codes(v[i], sc);
@@ -462,8 +543,9 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const u32 at = 128 * l + 64 * h + 16 * (lane >> 4);
-            B[h] = v4i{0, 0, 0, 0};
-            if (col < (u32)M && at < a.kp) B[h] = *reinterpret_cast<const v4i *>(codes + col * a.kp + at);
+            const bool in = col < (u32)M && at < a.kp;
+            const v4i b = *reinterpret_cast<const v4i *>(codes + (in ? col * a.kp + at : 0u));
+            B[h] = in ? b : v4i{0, 0, 0, 0};
 #pragma unroll
             for (int r = 0; r < R; r++) A[h][r] = i8_of_line(stage + mine, lane, r, h);
         }
@@ -800,12 +882,12 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     I8Src<G> src;
     src.q = a.order ? a.q : a.q + (size_t)t0 * a.kp;
     src.w = run.w + (size_t)r0 * a.kp;
+    u32 col[G::RT];
 #pragma unroll
-    for (int r = 0; r < G::RT; r++) {
-        const u32 line = (wave * G::RT + r) * 8 + (lane >> 3), j = min(t0 + line, run.j1 - 1);
-        bool bad;
-        src.col[r] = (a.order ? i8_column(a, j, bad) : j - t0) * a.kp + 16 * ((lane & 7) ^ i8_swizzle(line));
-    }
+    for (int r = 0; r < G::RT; r++) col[r] = min(t0 + (wave * G::RT + r) * 8 + (lane >> 3), run.j1 - 1);
+    if (a.order) i8_columns<G::RT>(a, col);
+#pragma unroll
+    for (int r = 0; r < G::RT; r++) src.col[r] = (a.order ? col[r] : col[r] - t0) * a.kp + 16 * ((lane & 7) ^ i8_swizzle((wave * G::RT + r) * 8 + (lane >> 3)));
 #pragma unroll
     for (int r = 0; r < G::RR; r++) {
         const u32 line = i8_row_group<G>(wave, r) * 8 + (lane >> 3);
@@ -925,11 +1007,11 @@ static hipError_t few_launch(const Launch &L, const I8Args &a, u32 entries) {
 
 template <int ET, int M, int R>
 static void few_x_launch(const Launch &L, const I8Args &a, const QuantArgs &q) {
-    hipLaunchKernelGGL((k_i8_few_x<ET, M, R>), dim3((a.rows + 16 * R - 1) / (16 * R)), dim3(64 * kFewXWaves), M * a.kp, L.stream, a, q);
+    hipLaunchKernelGGL((k_i8_few_x<ET, M, R>), dim3((a.rows + 16 * R - 1) / (16 * R)), dim3(64 * kFewXWaves), 0, L.stream, a, q);
 }
 template <int ET, int M>
 static void few_x_by_rows(const Launch &L, const I8Args &a, const QuantArgs &q) {
-    if ((a.rows + 15) / 16 >= 320) few_x_launch<ET, M, 2>(L, a, q);
+    if ((a.rows + 15) / 16 > 256) few_x_launch<ET, M, 2>(L, a, q);
     else few_x_launch<ET, M, 1>(L, a, q);
 }
 template <int ET>
@@ -943,7 +1025,7 @@ static void few_x_by_columns(const Launch &L, const I8Args &a, const QuantArgs &
 hipError_t i8_gemm_x(const Launch &L, const int8_t *w, const float *ws, int rows, int k, const void *x, int x_et, int64_t ld_x, int m, int8_t *codes,
                      float *scales, void *y, int et, int64_t ld) {
     const u32 kp = (u32)i8_row_bytes(k), M = m <= 1 ? 1 : m <= 2 ? 2 : m <= 4 ? 4 : 8;
-    if (m <= kFewX && kp <= few_x_values(M)) {
+    if (m <= kFewX && k >= 8 && kp <= few_x_values(M)) {
         const I8Args a = {w, ws, (u32)rows, kp, codes, scales, (u32)m, nullptr, nullptr, 0, 0, (u32)m, 1, y, (size_t)ld, et, L.fault, L.layer};
         const QuantArgs q = {x, nullptr, (size_t)ld_x, (u32)m, (u32)k, kp, nullptr, codes, scales, L.rule, L.fault, L.layer};
         if (x_et == kElemF32) few_x_by_columns<kElemF32>(L, a, q);
