@@ -1,0 +1,185 @@
+"""GPU tests of every form that the products in 8-bit integers and their quantizer take, at sizes that lead to it: all forms of a product give the
+same bits, so they are held to the rule's value, or to one another. The integer sums of the references are formed in f64, which
+holds them exactly."""
+import numpy as np
+import pytest
+import torch
+
+import bloomery_amd as bm
+from common import normal_f32
+from rows_common import NAMES, NUMPY, TORCH, bits, codes_of, padded, rounded, tables
+from test_gpu_i8 import Held, clean, gpu, held, junk_padded, picks, quantize, some_matrix  # noqa: F401 (fixtures)
+
+pytestmark = pytest.mark.gpu
+PTR = torch.Tensor.data_ptr
+
+
+def value(q, s, w, ws):
+    """The product's f32 value, from exact sums."""
+    sums = (q.astype(np.float64) @ w.astype(np.float64).T).astype(np.float32)
+    return (sums * s[:, None]).astype(np.float32) * ws[None, :]
+
+
+# by the count of tiles: waves sharing k (tiles of 16 x 16, 16 x 32, 32 x 32), then tiles of 32 x 64, 64 x 64 (two rings), 64 x 128, 128 x 128, 256 x
+# 256, 256 x 224; k of three lines and a piece, of half a line, of many lines and an odd number of values
+SIZES = ((7, 4000, 272), (16, 8200, 272), (1, 9001, 1030), (20, 8300, 100), (90, 1200, 272), (250, 1000, 2056), (40, 9000, 272), (700, 1100, 272), (700, 1100, 40), (650, 1300, 1111),
+         (1600, 1400, 272), (1500, 1500, 144), (2050, 1600, 272), (2300, 2300, 272), (2301, 2299, 130), (4000, 4000, 272), (4001, 3999, 30), (4000, 3500, 272), (3990, 3490, 650))
+
+
+@pytest.mark.parametrize("m,rows,k", SIZES)
+def test_product_in_every_form(gpu, held, m, rows, k):
+    rng = np.random.default_rng(m + rows + k)
+    w, ws = some_matrix(rng, rows, k)
+    q = rng.integers(-127, 128, (m, k), dtype=np.int16).astype(np.int8)
+    s = rng.random(m).astype(np.float32)
+    dtype = (bm.F32, bm.F16, bm.BF16)[k % 3]
+    y = held.out(NUMPY[dtype], m * rows)
+    gpu.enqueue_i8_gemm(held.up(junk_padded(w, k, rng)), held.up(ws), rows, k, held.up(padded(q, k)), held.up(s), m, y, dtype)
+    got, want = y.download().reshape(m, rows), bits(value(q, s, w, ws), dtype)
+    assert np.array_equal(got, want), f"{np.count_nonzero(got != want)} of {got.size} values differ"
+    clean(gpu)
+
+
+# slots an expert: long runs (256 x 256), of some hundred (64 x 256), many tiles of short ones (64 x 128), shorter still (32 x 64), behind more than one
+# reading of 256 bounds
+@pytest.mark.parametrize("m,n,top_k,rows,k", ((1100, 2, 1, 300, 272), (900, 3, 2, 513, 40), (200, 64, 4, 2900, 48), (330, 90, 4, 3100, 144), (20, 300, 4, 70, 272), (200, 1000, 2, 40, 16),
+                                              (999, 512, 8, 100, 48), (12, 1024, 3, 257, 272)))
+@pytest.mark.parametrize("own", (False, True), ids=("shared", "own"))
+def test_experts_product_in_every_form(gpu, held, own, m, n, top_k, rows, k):
+    rng = np.random.default_rng(m + n + rows)
+    ids = picks(rng, m, n, top_k)
+    order, start, _ = tables(ids, n)
+    n_slots, listed = m * top_k, int(start[-1])
+    full = np.full(n_slots, 0x12345678, np.uint32)
+    full[:listed] = order
+    w, ws = some_matrix(rng, n * rows, k)
+    cols = n_slots if own else m
+    q = rng.integers(-127, 128, (cols, k), dtype=np.int16).astype(np.int8)
+    s = rng.random(cols).astype(np.float32)
+    y = held.out(np.float32, n_slots * rows)
+    gpu.enqueue_i8_gemm_experts(held.up(junk_padded(w, k, rng)), held.up(ws), n, rows, k, held.up(padded(q, k)), held.up(s), None if own else held.up(full), held.up(start),
+                                n_slots, 0 if own else top_k, y, bm.F32)
+    got = y.download().reshape(n_slots, rows)
+    col = np.arange(listed) if own else order // top_k
+    for e in range(n):
+        a, b = int(start[e]), int(start[e + 1])
+        if b > a:
+            want = value(q[col[a:b]], s[col[a:b]], w[e * rows:(e + 1) * rows], ws[e * rows:(e + 1) * rows])
+            assert np.array_equal(got[a:b], want), f"expert {e}"
+    assert (got[listed:].view(np.uint8) == 0xEE).all()
+    clean(gpu)
+
+
+@pytest.mark.parametrize("dtype", (bm.F32, bm.F16, bm.BF16), ids=NAMES.get)
+@pytest.mark.parametrize("rows,k", ((40, 8), (40, 9), (100, 2048), (33, 2050), (20, 4090), (20, 4096), (20, 4101), (17, 8192), (50, 16384), (50, 16385), (4097, 77), (5000, 2048)))
+def test_few_rows_in_one_call_are_the_two_calls(gpu, held, dtype, rows, k):
+    rng = np.random.default_rng(rows + k)
+    w, ws = some_matrix(rng, rows, k)
+    wd, wsd, kp = held.up(junk_padded(w, k, rng)), held.up(ws), bm.i8_row_bytes(k)
+    x = rounded(normal_f32(rng, (9, k)), dtype)
+    codes, scales = codes_of(x)
+    for m in range(1, 10):
+        c1, s1 = quantize(gpu, held, x[:m], dtype, k)
+        y1, y2 = held.out(NUMPY[dtype], m * rows), held.out(NUMPY[dtype], (m + 1) * rows, 0x77)
+        c2, s2 = held.out(np.int8, (m + 1) * kp, 0x33), held.out(np.float32, m + 1, 0x44)
+        gpu.enqueue_i8_gemm(wd, wsd, rows, k, c1, s1, m, y1, dtype)
+        gpu.enqueue_i8_gemm_x(wd, wsd, rows, k, held.up(bits(x[:m], dtype)), dtype, m, c2, s2, y2, dtype)
+        assert np.array_equal(c1.download().reshape(m, kp), padded(codes[:m], k)) and np.array_equal(s1.download(), scales[:m])
+        assert np.array_equal(y1.download(), y2.download()[:m * rows]), m
+        assert np.array_equal(c1.download(), c2.download()[:m * kp]) and np.array_equal(s1.download(), s2.download()[:m])
+        # the row behind the last is left as it was
+        assert (y2.download()[m * rows:].view(np.uint8) == 0x77).all() and (c2.download()[m * kp:] == 0x33).all()
+        assert (s2.download()[m:].view(np.uint8) == 0x44).all()
+    clean(gpu)
+
+
+@pytest.mark.parametrize("dtype", (bm.F32, bm.F16, bm.BF16), ids=NAMES.get)
+@pytest.mark.parametrize("m,k", ((3, 3), (2100, 5), (30, 1020), (30, 2050), (2100, 2050), (2060, 4096), (30, 4099), (2100, 4099), (30, 8191), (2060, 8192), (5, 8193), (3, 40000)))
+def test_quantizer_in_every_form(gpu, held, dtype, m, k):
+    rng = np.random.default_rng(m + k)
+    x = rounded(normal_f32(rng, (m, k)), dtype)
+    q, s = codes_of(x)
+    codes, scales = quantize(gpu, held, x, dtype, k, ld=k + 1)
+    assert np.array_equal(scales.download(), s)
+    assert np.array_equal(codes.download().reshape(m, -1), padded(q, k))
+    # the gate rule's values: rows by themselves (a form for few of them) and all together
+    g, u = x, rounded(normal_f32(rng, (m, k)), dtype)
+    gd, ud, kp = held.up(bits(g, dtype)), held.up(bits(u, dtype)), bm.i8_row_bytes(k)
+    c1, s1, c2, s2 = held.out(np.int8, m * kp), held.out(np.float32, m), held.out(np.int8, 2 * kp), held.out(np.float32, 2)
+    gpu.enqueue_i8_swiglu_quantize(gd, ud, dtype, m, k, c1, s1)
+    gpu.enqueue_i8_swiglu_quantize(held.up(bits(g[-2:], dtype)), held.up(bits(u[-2:], dtype)), dtype, 2, k, c2, s2)
+    assert np.array_equal(c1.download()[-2 * kp:], c2.download()) and np.array_equal(s1.download()[-2:], s2.download())
+    silu = g[-2:] / (1 + np.exp(-g[-2:])) * u[-2:]
+    # a code's value is within half a step of the scale, and two f32 roundings and an exponential's few ulps of the gate's
+    step = s2.download().astype(np.float64)[:, None]
+    assert (np.abs(c2.download().reshape(2, kp)[:, :k] * step - silu) <= step * (0.5 + 127 * 2.0 ** -20)).all()
+    clean(gpu)
+
+
+def test_offsets_past_32_bits(gpu):
+    """A matrix of 4.3 GB as rows, as columns, as gathered columns and as an expert's rows: its last rows against sums on the host."""
+    k, n = 131072, 32800
+    torch.manual_seed(3)
+    big = torch.randint(-127, 128, (n, k), dtype=torch.int8, device="cuda")
+    few = torch.randint(-127, 128, (40, k), dtype=torch.int8, device="cuda")
+    big_s, few_s = torch.rand(n, device="cuda"), torch.rand(40, device="cuda")
+    at = torch.tensor([0, 5, 16383, 16384, n - 33, n - 2, n - 1])
+    sums = (big[at.cuda()].cpu().double() @ few.cpu().double().t()).float()
+    b, f = big_s.cpu()[at][:, None], few_s.cpu()[None]
+    as_rows, as_columns = (sums * f) * b, (sums * b) * f
+    for m in (1, 40):
+        y = torch.zeros(m, n, device="cuda")
+        torch.cuda.synchronize()
+        gpu.enqueue_i8_gemm(PTR(big), PTR(big_s), n, k, PTR(few), PTR(few_s), m, PTR(y), bm.F32)
+        gpu.sync()
+        assert torch.equal(y.cpu()[:, at], as_rows[:, :m].t()), m
+    y = torch.zeros(n, 40, device="cuda")
+    torch.cuda.synchronize()
+    gpu.enqueue_i8_gemm(PTR(few), PTR(few_s), 40, k, PTR(big), PTR(big_s), n, PTR(y), bm.F32)
+    gpu.sync()
+    assert torch.equal(y.cpu()[at], as_columns)
+    # the columns behind an order, of one expert's 40 slots: offsets of gathered columns past 32 bits
+    order = torch.cat((at, torch.arange(33))).int().cuda()
+    start, y = torch.tensor([0, 40], dtype=torch.int32, device="cuda"), torch.zeros(40, 40, device="cuda")
+    torch.cuda.synchronize()
+    slots = n  # every column's slot exists; one expert's run lists forty of them
+    table = torch.zeros(slots, dtype=torch.int32, device="cuda")
+    table[:40] = order
+    y = torch.zeros(slots, 40, device="cuda")
+    torch.cuda.synchronize()
+    gpu.enqueue_i8_gemm_experts(PTR(few), PTR(few_s), 1, 40, k, PTR(big), PTR(big_s), PTR(table), PTR(start), slots, 1, PTR(y), bm.F32, n_cols=n)
+    gpu.sync()
+    assert torch.equal(y.cpu()[:7], as_columns) and not y[40:].any()
+    # two experts of 16400 rows, the second's past 32 bits
+    y = torch.zeros(40, n // 2, device="cuda")
+    start = torch.tensor([0, 20, 40], dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    gpu.enqueue_i8_gemm_experts(PTR(big), PTR(big_s), 2, n // 2, k, PTR(few), PTR(few_s), None, PTR(start), 40, 0, PTR(y), bm.F32)
+    gpu.sync()
+    inside = at[4:] - n // 2
+    assert torch.equal(y.cpu()[20:, inside], as_rows[4:, 20:].t())
+    clean(gpu)
+
+
+def test_two_contexts_at_once(gpu):
+    """Two contexts, each on a stream of its own with the buffers of its own call, and the same weights: neither waits for nor disturbs the other."""
+    rng = np.random.default_rng(21)
+    rows, k, m = 700, 1000, 300
+    w, ws = some_matrix(rng, rows, k)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    contexts = [bm.Gpu(0, stream=s.cuda_stream) for s in streams]
+    try:
+        wt, wst = torch.from_numpy(junk_padded(w, k, rng)).cuda(), torch.from_numpy(ws).cuda()
+        xs = [torch.from_numpy(normal_f32(rng, (m, k))).cuda() for _ in range(2)]
+        outs = [(torch.zeros(m, bm.i8_row_bytes(k), dtype=torch.int8, device="cuda"), torch.zeros(m, device="cuda"), torch.zeros(m, rows, device="cuda")) for _ in range(2)]
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for c, x, (codes, scales, y) in zip(contexts, xs, outs):
+                c.enqueue_i8_gemm_x(PTR(wt), PTR(wst), rows, k, PTR(x), bm.F32, m, PTR(codes), PTR(scales), PTR(y), bm.F32)
+        torch.cuda.synchronize()
+        for x, (_, _, y) in zip(xs, outs):
+            q, s = codes_of(x.cpu().numpy())
+            assert np.array_equal(y.cpu().numpy(), value(q, s, w, ws))
+    finally:
+        for c in contexts:
+            c.close()
