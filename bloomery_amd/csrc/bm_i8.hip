@@ -1048,12 +1048,14 @@ hipError_t i8_gemm_x(const Launch &L, const int8_t *w, const float *ws, int rows
 //   Where tiles of at most 32 x 32 are no more than the compute units, a workgroup's waves share a row's k (k_i8_few), in the smallest tile that is one
 //   round: 34 x 544 x 8064 in 16 x 16 5.6 (16 x 32: 7.0, 32 x 64 whole rows 13), 64 x 2048 x 7168 in 16 x 32 6.5 (32 x 32: 7.9; 12.8), 128 x 2048 x 7168 in 32 x 32 8.1 (16 x 32:
 //   11.2; 12.9), 24 x 7168 x 2048 5.1 (7.1), one row of 2048 x 7168 4.9, of 7168 x 7168 9.6; two rounds lose, 64 x 7168 x 2048 8.2 (32 x 64: 7.5).
-//   Experts, by slots an expert: 4096 tokens, top 8 of 32 (1024 slots each), 7168 x 2048 rows in 256 x 256 595 (128 x 128: 658, 64 x 256: 714); 2048 tokens, top 8 of 128, 768 x 2048
-//   in 64 x 256 72 (256 x 256: 79, 128 x 128: 78, 64 x 128: 76), 2048 x 768 87 (103, 91, 91); 512 tokens 46 (64 x 128: 51), one round of tiles; 1024 tokens in 64 x 128 58
-//   (64 x 256: 63), 333 tokens, top 8 of 64, 7168 x 2048 189 (193; own columns, f16, 156 and 166); 128 tokens
-//   (8 slots each) in 32 x 64 37 (64 x 256: 39), 16 tokens 20 (24; waves sharing k 25); one token's eight slots by waves sharing k 7.9 (32 x 64: 9.1). A die's group of two
-//   tiles of columns (k_i8_tile) in these: 2048 tokens 72, without 88; where a run's rows are eight tiles or more it loses (333 tokens, 7168 rows in
-//   64 x 128, 189 without, 204 with).
+//   Experts, by slots an expert. From 352 on 256 x 256: 375 slots, 64 experts, 1024 x 2048 88.9 (128 x 128: 94.9), 1024 slots, 32 experts, 7168 x 2048 589 (638, 64 x
+//   256: 699); from 144 on 128 x 128: 250 slots, 64 experts, 1024 x 2048 70.9 (256 x 256: 75.8, 64 x 256: 80.4), 150 slots, 7168 x 2048 295 (341, 317), 256 slots, 128 experts, 768 x 2048
+//   102 (113, 115); then 64 x 256: 128 slots, 768 x 2048 73.1 (128 x 128: 77.5, 64 x 128: 79), 2048 x 768 85 (89, 89); 32 slots 45.2 (64 x 128: 52), one round of tiles; more of them in 64 x 128: 64
+//   slots 59.5 (64 x 256: 63.5), 42 slots, 64 experts, 7168 x 2048 190.5 (193); 8 slots an expert in 32 x 64 37.5 (64 x 256: 39.8), one slot 20 (24; waves sharing k 25); one token's
+//   eight slots by waves sharing k 6.6 (32 x 64: 9.1).
+//   A die's group of two tiles of columns (k_i8_tile) in these: 128 slots, 768 x 2048 72, without 88 (its weights are then fetched 1.8 times: 369 MB at 5.5 TB/s); 256 slots 102, without
+//   117. Where a run's rows are eight tiles or more it loses (64 experts, 7168 x 2048 190.8 without, 201 with); dies with whole ranges of the experts lose there too (202) and gain
+//   little here (69).
 hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_experts, int rows, int k, const int8_t *q, const float *qs, int n_cols,
                    const uint32_t *order, const uint32_t *start, int n_slots, int top_k, void *y, int et, int64_t ld) {
     const I8Args a = {w, ws, (u32)rows, (u32)i8_row_bytes(k), q, qs, (u32)n_cols, order, start, (u32)n_slots, (u32)top_k, (u32)n_cols, (u32)n_experts,
@@ -1066,7 +1068,8 @@ hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_expe
     if (start) {
         if (n <= 32 || !reach) return few_launch<2, 1, 3>(L, a, n);
         const u32 each = n / (u32)n_experts;
-        if (each >= 512) return tile_launch<256, 256, 4, 2, 2, false, 2>(L, a, n);
+        if (each >= 352) return tile_launch<256, 256, 4, 2, 2, false, 2>(L, a, n);
+        if (each >= 144) return tile_launch<128, 128, 2, 2, 2, true, 2>(L, a, n);
         // 64 x 256 where its tiles (half a tile more an expert) are one round of two a compute unit, or the runs long
         if (each >= 96 || (each >= 12 && (uint64_t)(n / 64 + (u32)n_experts / 2) * up(a.rows, 256) <= 512)) return tile_launch<64, 256, 1, 4, 2, true, 2>(L, a, n);
         if (each >= 12) return tile_launch<64, 128, 1, 4, 2, true, 2>(L, a, n);
