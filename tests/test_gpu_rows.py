@@ -47,7 +47,8 @@ def check_sort(got, ids, n, x, dtype, width):
                                                  (17, 1024, 3, 33, (0, 1)), (9, 64, 64, 129, (3, 0)), (300, 4, 2, 100, (0, 0)), (256, 16, 8, 40, (0, 0)),
                                                  (257, 16, 8, 40, (1, 1)), (1000, 128, 8, 24, (0, 0)), (2500, 1, 1, 9, (0, 3)), (700, 1024, 4, 17, (0, 0)),
                                                  (50, 100, 64, 5, (0, 0)), (512, 16, 8, 8, (0, 0)), (513, 16, 8, 9, (0, 1)), (5000, 1, 1, 3, (0, 0)),
-                                                 (1500, 1024, 4, 8, (0, 0)), (2100, 130, 8, 16, (0, 0)), (150, 600, 40, 4, (0, 0)), (20000, 7, 7, 2, (0, 0))))
+                                                 (1500, 1024, 4, 8, (0, 0)), (2100, 130, 8, 16, (0, 0)), (150, 600, 40, 4, (0, 0)), (20000, 7, 7, 2, (0, 0)),
+                                                 (7, 5, 1, 4100, (0, 1)), (4095, 64, 1, 20, (0, 0)), (1001, 9, 2, 300, (2, 0)), (9, 9, 2, 5003, (0, 0)), (1365, 20, 3, 12, (0, 0)), (6, 7, 5, 2100, (0, 0))))
 def test_sort_is_the_stable_one(gpu, held, dtype, m, n, top_k, width, pad):
     rng = np.random.default_rng(m + n + width)
     ids = picks(rng, m, n, top_k)
