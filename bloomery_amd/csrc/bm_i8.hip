@@ -590,8 +590,8 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
 // Many columns a matrix: BT columns x BR rows a workgroup, 128 bytes of k a step through a ring of S LDS buffers, where the loads put them
 // themselves (16 bytes a lane, no register in between): while the waves multiply one step the next S - 1 are on their way, one barrier a step. A
 // wave holds (BT / WT) x (BR / WR) sums in v_mfma_i32_16x16x64_i8's form.
-// Large products are bound by the clock that power leaves the matrix cores: 4096 x 7168 x 7168 in 176 to 187 us, 2.2 to 2.4 POP/s (matrix cores busy 61 % of the
-// time at what a bare loop of these instructions reaches on such data, 3.3 POP/s; LDS 27 %, no bank conflicts; the library's product of the same size takes 180).
+// Large products are bound by the matrix cores and the clock that power leaves them: 4096 x 7168 x 7168 in 176 to 187 us, 2.2 to 2.4 POP/s, matrix cores busy 61 %
+// of the cycles, LDS 27 %, no bank conflicts (a bare loop of these instructions on such data reaches 3.3 POP/s; the library's product of the same size takes 180 us).
 // Small ones by the latency of a step's loads (777 x 2000 x 1996: matrix cores 12 %), experts' by their weights from memory.
 template <int BT, int BR, int WT, int WR, int S, bool WHOLE>
 struct I8Tile {

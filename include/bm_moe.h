@@ -501,7 +501,8 @@ int bm_expert_sort_grad(bm_ctx *ctx, const void *d_rows_dev, int type, int64_t l
                         int width, void *dx_dev, int64_t ld_dx);
 /* And back: y[t] = (acc = 0; for token t's listed slots s ascending: acc = fma(w[s], rows[place[s]], acc)) + resid[t], bm_combine_tokens'
  * sum over sorted rows. A slot that is not listed adds nothing, whatever its weight. resid_dev may be NULL (no add). A place at
- * or past n_tokens * top_k other than 0xffffffff raises BM_SITE_EXPERT_ID and adds nothing, here and in the gradients. */
+ * or past n_tokens * top_k other than 0xffffffff raises BM_SITE_EXPERT_ID and adds nothing, here and in the gradients. (rows_dev, and
+ * d_rows_dev above, hold n_tokens * top_k rows; the first may be read, and not used, where a token has no listed slot.) */
 int bm_expert_combine(bm_ctx *ctx, const void *rows_dev, int type, int64_t ld_rows, const uint32_t *place_dev, const float *w_dev,
                       const void *resid_dev, int64_t ld_resid, int n_tokens, int top_k, int width, void *y_dev, int64_t ld_y);
 /* Its gradients: d_rows[place[s]] = w[s] * dy[t] and d_w[s] = <dy[t], rows[place[s]]> (f32, each dot summed in one order whatever the
