@@ -210,18 +210,24 @@ __global__ __launch_bounds__(64 * kSortWaves) void k_sort_count(SortArgs a, u32 
 }
 
 // 2. The counts become the places of the chunks' first slots (4 us for 64 chunks of 128 experts, latency: one workgroup, two passes): running sums over an expert's chunks behind the runs' bounds. A thread has an expert
-//    and a run of the chunks (at most 32 threads an expert), whose counts it asks for sixteen at a time; it reads them twice, the second time
-//    from the cache.
+//    and a run of the chunks (at most 32 threads an expert), whose counts it asks for sixteen at a time; it keeps the first sixteen, and reads what
+//    is behind them twice, the second time from the cache.
 __global__ __launch_bounds__(1024) void k_sort_scan(SortArgs a, u32 chunks, u32 log_experts) {
     __shared__ u32 part[1024], scan[16];
     const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const u32 e = tid & ((1u << log_experts) - 1u), group = tid >> log_experts, groups = min(1024u >> log_experts, 32u);
     const u32 share = (chunks + groups - 1) / groups, lo = min(group * share, chunks), hi = e < a.n_experts ? min(lo + share, chunks) : lo;
-    u32 sum = 0;
-    for (u32 c0 = lo; c0 < hi; c0 += 16) {
-        u32 v[16];
+    u32 sum = 0, first[16];
+    const auto counts = [&](u32 c0, u32 (&v)[16]) {
 #pragma unroll
         for (u32 i = 0; i < 16; i++) v[i] = c0 + i < hi ? a.work[(size_t)(c0 + i) * a.n_experts + e] : 0;
+    };
+    counts(lo, first);
+#pragma unroll
+    for (u32 i = 0; i < 16; i++) sum += first[i];
+    for (u32 c0 = lo + 16; c0 < hi; c0 += 16) {
+        u32 v[16];
+        counts(c0, v);
 #pragma unroll
         for (u32 i = 0; i < 16; i++) sum += v[i];
     }
@@ -253,15 +259,18 @@ __global__ __launch_bounds__(1024) void k_sort_scan(SortArgs a, u32 chunks, u32 
         if (e + 1 == a.n_experts) a.start[a.n_experts] = at + count;
     }
     at = part[e] + before;
-    for (u32 c0 = lo; c0 < hi; c0 += 16) {
-        u32 v[16];
-#pragma unroll
-        for (u32 i = 0; i < 16; i++) v[i] = c0 + i < hi ? a.work[(size_t)(c0 + i) * a.n_experts + e] : 0;
+    const auto settle = [&](u32 c0, const u32 (&v)[16]) {
 #pragma unroll
         for (u32 i = 0; i < 16; i++) {
             if (c0 + i < hi) a.work[(size_t)(c0 + i) * a.n_experts + e] = at;
             at += v[i];
         }
+    };
+    settle(lo, first);
+    for (u32 c0 = lo + 16; c0 < hi; c0 += 16) {
+        u32 v[16];
+        counts(c0, v);
+        settle(c0, v);
     }
 }
 

@@ -70,6 +70,46 @@ def test_experts_product_in_every_form(gpu, held, own, m, n, top_k, rows, k):
     clean(gpu)
 
 
+@pytest.mark.parametrize("rows", (40, 300))
+@pytest.mark.parametrize("own", (False, True), ids=("shared", "own"))
+def test_tables_that_are_none_in_tiles(gpu, held, own, rows):
+    """Runs outside the slots are skipped and raise, runs of nothing write nothing, an entry whose slot does not exist is NaN: of more slots than a
+    wave's columns."""
+    rng = np.random.default_rng(31 + rows)
+    n, n_slots, top_k, k = 5, 150, 2, 272
+    w, ws = some_matrix(rng, n * rows, k)
+    cols = n_slots if own else n_slots // top_k
+    q = rng.integers(-127, 128, (cols, k), dtype=np.int16).astype(np.int8)
+    s = rng.random(cols).astype(np.float32)
+    order = rng.permutation(n_slots).astype(np.uint32)
+    wd, wsd, qd, sd = held.up(junk_padded(w, k, rng)), held.up(ws), held.up(padded(q, k)), held.up(s)
+    gpu.fault_clear()
+    for start, runs in (((0, 0, 0, 0, 0, 0), {}), ((7, 7, 7, 7, 7, 7), {}), ((0, 40, 30, 0xFFFFFFF0, 70, 150), {0: (0, 40), 4: (70, 150)}),
+                        ((0, 70, 70, 71, 149, 151), {0: (0, 70), 2: (70, 71), 3: (71, 149)}), ((151, 152, 0xFFFFFFFF, 3, 3, 90), {4: (3, 90)})):
+        y = held.out(np.float32, n_slots * rows)
+        gpu.enqueue_i8_gemm_experts(wd, wsd, n, rows, k, qd, sd, None if own else held.up(order), held.up(np.array(start, np.uint32)), n_slots, 0 if own else top_k, y, bm.F32,
+                                    n_cols=cols)
+        got, done = y.download().reshape(n_slots, rows), np.zeros(n_slots, bool)
+        for e, (a, b) in runs.items():
+            col = np.arange(a, b) if own else order[a:b] // top_k
+            assert np.array_equal(got[a:b], value(q[col], s[col], w[e * rows:(e + 1) * rows], ws[e * rows:(e + 1) * rows])), e
+            done[a:b] = True
+        assert (got[~done].view(np.uint32) == 0xEEEEEEEE).all()
+        raised = gpu.fault()[0] & 0xFF == bm.SITE_EXPERT_ID
+        assert raised == any(a > b or b > n_slots for a, b in zip(start, start[1:]))
+        gpu.fault_clear()
+    if own:
+        return
+    bad = order.copy()
+    bad[[0, 9, 149]] = [n_slots, 0xFFFFFFFF, 0x80000000]
+    y = held.out(np.float32, n_slots * rows)
+    gpu.enqueue_i8_gemm_experts(wd, wsd, n, rows, k, qd, sd, held.up(bad), held.up(np.array((0, 40, 90, 91, 91, 150), np.uint32)), n_slots, top_k, y, bm.F32)
+    got = y.download().reshape(n_slots, rows)
+    assert np.isnan(got[[0, 9, 149]]).all() and np.isfinite(np.delete(got, [0, 9, 149], 0)).all()
+    assert gpu.fault()[0] & 0xFF == bm.SITE_EXPERT_ID
+    gpu.fault_clear()
+
+
 @pytest.mark.parametrize("dtype", (bm.F32, bm.F16, bm.BF16), ids=NAMES.get)
 @pytest.mark.parametrize("rows,k", ((40, 8), (40, 9), (100, 2048), (33, 2050), (20, 4090), (20, 4096), (20, 4101), (17, 8192), (50, 16384), (50, 16385), (4097, 77), (5000, 2048)))
 def test_few_rows_in_one_call_are_the_two_calls(gpu, held, dtype, rows, k):
