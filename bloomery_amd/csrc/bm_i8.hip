@@ -10,6 +10,8 @@
 // so every split of k gives the same bits.
 #include "bm_elem.hpp"
 
+#include <algorithm>
+
 namespace bmk {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
@@ -1055,6 +1057,10 @@ hipError_t i8_gemm_x(const Launch &L, const int8_t *w, const float *ws, int rows
 //   102 (113, 115); then 64 x 256: 128 slots, 768 x 2048 73.1 (128 x 128: 77.5, 64 x 128: 79), 2048 x 768 85 (89, 89); 32 slots 45.2 (64 x 128: 52), one round of tiles; more of them in 64 x 128: 64
 //   slots 59.5 (64 x 256: 63.5), 42 slots, 64 experts, 7168 x 2048 190.5 (193); 8 slots an expert in 32 x 64 37.5 (64 x 256: 39.8), one slot 20 (24; waves sharing k 25); one token's
 //   eight slots by waves sharing k 6.6 (32 x 64: 9.1).
+//   While 64 x 64 tiles are few, so that a compute unit has one to four: short runs in 32 x 64 with four steps in flight, 20 tokens, top 4 of 52, 288 x 6224 13.9 (two steps 24.5, 64 x
+//   64 25.7), 152 tokens, top 5 of 54, 688 x 3376 35.5 (64 x 256: 48.4), 100 tokens, top 2 of 16, 1024 x 4096 15.8 (18.3, 27.4); longer ones in 64 x 64, with four steps up to one a
+//   unit, 100 tokens, top 8 of 16, 768 x 2048 10.7 (two steps 12.4, 64 x 256 17.4), with two steps behind that, 400 tokens, top 2 of 8, 2048 x 2048 13.6 (four 16.1, 64 x 256 17.8), 600
+//   tokens, 1000 x 1000 9.7 (10.1, 13.8); least of all by waves sharing k, 40 tokens, top 4 of 32, 96 x 4000 7.0 (32 x 64: 10.2).
 //   A die's group of two tiles of columns (k_i8_tile) in these: 128 slots, 768 x 2048 72, without 88 (its weights are then fetched 1.8 times: 369 MB at 5.5 TB/s); 256 slots 102, without
 //   117. Where a run's rows are eight tiles or more it loses (64 experts, 7168 x 2048 190.8 without, 201 with); dies with whole ranges of the experts lose there too (202) and gain
 //   little here (69).
@@ -1069,7 +1075,13 @@ hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_expe
     const bool reach = !order || (uint64_t)n_cols * a.kp <= 0xffffffffu;
     if (start) {
         if (n <= 32 || !reach) return few_launch<2, 1, 3>(L, a, n);
-        const u32 each = n / (u32)n_experts;
+        const u32 each = n / (u32)n_experts, runs = n < (u32)n_experts ? n : (u32)n_experts;
+        // 64 x 64 tiles: every run has one, and half a one more than its slots fill
+        const uint64_t small = (uint64_t)std::max(runs, n / 64 + runs / 2) * up(a.rows, 64);
+        if (each <= 16 && small <= 64) return few_launch<2, 2, 4>(L, a, n);
+        if (each < 24 && small <= 600) return tile_launch<32, 64, 1, 2, 4, true, 2>(L, a, n);
+        if (each >= 24 && small <= 256) return tile_launch<64, 64, 2, 2, 4, true, 2>(L, a, n);
+        if (each >= 24 && small <= 1024) return tile_launch<64, 64, 2, 2, 2, true, 2>(L, a, n);
         if (each >= 352) return tile_launch<256, 256, 4, 2, 2, false, 2>(L, a, n);
         if (each >= 144) return tile_launch<128, 128, 2, 2, 2, true, 2>(L, a, n);
         // 64 x 256 where its tiles (half a tile more an expert) are one round of two a compute unit, or the runs long
