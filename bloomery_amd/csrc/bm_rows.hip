@@ -347,30 +347,32 @@ __device__ __forceinline__ u32 checked_place(u32 p, u32 n_slots, u32 *fault, u32
     return kUnlisted;
 }
 
-// A batch of eight slots' places and weights. A slot that is not listed (or past the token's last) is read through the place of one that is, or the
-// first row, and what comes is not used: its request is answered by the cache, and no branch parts the eight.
-struct Slots8 {
-    u32 p[8];
-    float w[8];
-    bool on[8];
+// A batch of K slots' places and weights. A slot that is not listed (or past the token's last) is read through the place of one that is, or the
+// first row, and what comes is not used: its request is answered by the cache, and no branch parts the batch.
+template <int K>
+struct Slots {
+    u32 p[K];
+    float w[K];
+    bool on[K];
 };
-__device__ __forceinline__ Slots8 slots8(const u32 *place, const float *w, size_t s0, u32 have, u32 n_slots, u32 *fault, u32 layer) {
-    Slots8 r;
+template <int K>
+__device__ __forceinline__ Slots<K> slots_of(const u32 *place, const float *w, size_t s0, u32 have, u32 n_slots, u32 *fault, u32 layer) {
+    Slots<K> r;
 #pragma unroll
-    for (u32 k = 0; k < 8; k++) {
+    for (u32 k = 0; k < K; k++) {
         const size_t s = s0 + (k < have ? k : 0);
         r.p[k] = k < have ? place[s] : kUnlisted;
         r.w[k] = w ? w[s] : 1.0f;
     }
     u32 some = 0;
 #pragma unroll
-    for (u32 k = 0; k < 8; k++) {
+    for (u32 k = 0; k < K; k++) {
         r.p[k] = checked_place(r.p[k], n_slots, fault, layer);
         r.on[k] = r.p[k] != kUnlisted;
         some = r.on[k] ? r.p[k] : some;
     }
 #pragma unroll
-    for (u32 k = 0; k < 8; k++) r.p[k] = r.on[k] ? r.p[k] : some;
+    for (u32 k = 0; k < K; k++) r.p[k] = r.on[k] ? r.p[k] : some;
     return r;
 }
 
@@ -378,39 +380,39 @@ __device__ __forceinline__ Slots8 slots8(const u32 *place, const float *w, size_
 // 16-byte piece of a token (1 << log threads a token, several tokens a workgroup where rows are short); its slots' rows are asked for eight
 // at a time, so that a row's latency is paid once for all of them. What is left of a row that is no whole number of pieces goes an element a thread.
 // Memory: 1500 tokens of 7168 f16 from eight rows each, 194 MB, in 41.5 us, 4.7 TB/s; 16 tokens 4.9 us, the launch.
-template <int ET>
-__device__ __forceinline__ void combine_piece(const CombineArgs &a, const Slots8 &s, u32 c, float (&acc)[kElemPiece<ET>]) {
-    uint4 v[8];
+template <int ET, int K>
+__device__ __forceinline__ void combine_piece(const CombineArgs &a, const Slots<K> &s, u32 c, float (&acc)[kElemPiece<ET>]) {
+    uint4 v[K];
 #pragma unroll
-    for (u32 k = 0; k < 8; k++) v[k] = elem_piece<ET>(a.rows, (size_t)s.p[k] * a.ld_rows + c);
+    for (u32 k = 0; k < K; k++) v[k] = elem_piece<ET>(a.rows, (size_t)s.p[k] * a.ld_rows + c);
 #pragma unroll
-    for (u32 k = 0; k < 8; k++) {
+    for (u32 k = 0; k < K; k++) {
         float f[kElemPiece<ET>];
         elem_unpack<ET>(v[k], f);
 #pragma unroll
         for (int j = 0; j < kElemPiece<ET>; j++) acc[j] = s.on[k] ? fmaf(s.w[k], f[j], acc[j]) : acc[j];
     }
 }
-template <int ET, bool EIGHT> // EIGHT: at most eight slots a token, whose places a thread keeps
+template <int ET, int K, bool ALL> // ALL: at most K slots a token, whose places a thread keeps
 __global__ __launch_bounds__(kRowThreads) void k_expert_combine(CombineArgs a, u32 log) {
     constexpr int V = kElemPiece<ET>;
     const u32 t = blockIdx.x * (kRowThreads >> log) + (threadIdx.x >> log), mine = threadIdx.x & ((1u << log) - 1u);
     if (t >= a.n_tokens) return;
     const size_t s0 = (size_t)t * a.top_k;
-    Slots8 s;
-    if constexpr (EIGHT) s = slots8(a.place, a.w, s0, a.top_k, a.n_slots, a.fault, a.layer);
+    Slots<K> s;
+    if constexpr (ALL) s = slots_of<K>(a.place, a.w, s0, a.top_k, a.n_slots, a.fault, a.layer);
     for (u32 c = V * mine; c + V <= a.width; c += V << log) {
         float acc[V];
 #pragma unroll
         for (int j = 0; j < V; j++) acc[j] = 0.0f;
         uint4 r;
         if (a.resid) r = elem_piece<ET>(a.resid, (size_t)t * a.ld_resid + c);
-        if constexpr (EIGHT) {
-            combine_piece<ET>(a, s, c, acc);
+        if constexpr (ALL) {
+            combine_piece<ET, K>(a, s, c, acc);
         } else {
-            for (u32 k0 = 0; k0 < a.top_k; k0 += 8) {
-                s = slots8(a.place, a.w, s0 + k0, a.top_k - k0, a.n_slots, a.fault, a.layer);
-                combine_piece<ET>(a, s, c, acc);
+            for (u32 k0 = 0; k0 < a.top_k; k0 += K) {
+                s = slots_of<K>(a.place, a.w, s0 + k0, a.top_k - k0, a.n_slots, a.fault, a.layer);
+                combine_piece<ET, K>(a, s, c, acc);
             }
         }
         if (a.resid) {
@@ -446,26 +448,27 @@ struct CombineGradArgs {
     u32 *fault, layer;
 };
 
-// d_rows[place[s]] = w[s] dy[t], d_w[s] = <dy[t], rows[place[s]]>: a workgroup a token, eight slots at a time, so that a piece of dy is
-// read once for eight rows that are asked for together. Every dot is summed in one order: a thread's pieces, the wave, the
+// d_rows[place[s]] = w[s] dy[t], d_w[s] = <dy[t], rows[place[s]]>: T threads a token (the workgroup, or a wave where rows are short), K slots at a time, so
+// that a piece of dy is read once for K rows that are asked for together. Every dot is summed in one order: a thread's pieces, the wave, the
 // four waves. Memory, as much read as written: 4096 tokens of 2048 bf16, 285 MB, in 62 us, 4.6 TB/s.
-template <int ET>
+template <int ET, int K, int T>
 __global__ __launch_bounds__(kRowThreads) void k_expert_combine_grad(CombineGradArgs a) {
     constexpr int V = kElemPiece<ET>;
-    __shared__ float part[4][8];
-    const u32 t = blockIdx.x, tid = threadIdx.x;
-    for (u32 k0 = 0; k0 < a.top_k; k0 += 8) {
-        const Slots8 s = slots8(a.place, a.w, (size_t)t * a.top_k + k0, a.top_k - k0, a.n_slots, a.fault, a.layer);
-        float dot[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        for (u32 c = V * tid; c + V <= a.width; c += V * kRowThreads) {
-            uint4 v[8];
+    __shared__ float part[4][K];
+    const u32 t = blockIdx.x * (kRowThreads / T) + threadIdx.x / T, tid = threadIdx.x % T;
+    if (t >= a.n_tokens) return; // whole waves (T = 64), or nobody
+    for (u32 k0 = 0; k0 < a.top_k; k0 += K) {
+        const Slots<K> s = slots_of<K>(a.place, a.w, (size_t)t * a.top_k + k0, a.top_k - k0, a.n_slots, a.fault, a.layer);
+        float dot[K] = {};
+        for (u32 c = V * tid; c + V <= a.width; c += V * T) {
+            uint4 v[K];
             const uint4 gp = elem_piece<ET>(a.dy, (size_t)t * a.ld_dy + c);
 #pragma unroll
-            for (u32 k = 0; k < 8; k++) v[k] = elem_piece<ET>(a.rows, (size_t)s.p[k] * a.ld_rows + c);
+            for (u32 k = 0; k < K; k++) v[k] = elem_piece<ET>(a.rows, (size_t)s.p[k] * a.ld_rows + c);
             float g[V];
             elem_unpack<ET>(gp, g);
 #pragma unroll
-            for (u32 k = 0; k < 8; k++) {
+            for (u32 k = 0; k < K; k++) {
                 float f[V], d[V];
                 elem_unpack<ET>(v[k], f);
 #pragma unroll
@@ -480,21 +483,27 @@ __global__ __launch_bounds__(kRowThreads) void k_expert_combine_grad(CombineGrad
         if (c < a.width) {
             const float g = elem_load1<ET>(a.dy, (size_t)t * a.ld_dy + c);
 #pragma unroll
-            for (u32 k = 0; k < 8; k++)
+            for (u32 k = 0; k < K; k++)
                 if (s.on[k]) {
                     dot[k] = fmaf(g, elem_load1<ET>(a.rows, (size_t)s.p[k] * a.ld_rows + c), dot[k]);
                     elem_store1<ET>(a.d_rows, (size_t)s.p[k] * a.ld_d_rows + c, __fmul_rn(s.w[k], g));
                 }
         }
 #pragma unroll
-        for (u32 k = 0; k < 8; k++) {
+        for (u32 k = 0; k < K; k++) {
             const float sum = wave_sum(s.on[k] ? dot[k] : 0.0f);
-            if ((tid & 63) == 0) part[tid >> 6][k] = sum;
+            if constexpr (T == 64) {
+                if (tid == 0 && k0 + k < a.top_k) a.d_w[(size_t)t * a.top_k + k0 + k] = sum;
+            } else if ((tid & 63) == 0) {
+                part[tid >> 6][k] = sum;
+            }
         }
-        __syncthreads();
-        if (tid < 8 && k0 + tid < a.top_k)
-            a.d_w[(size_t)t * a.top_k + k0 + tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
-        __syncthreads();
+        if constexpr (T > 64) {
+            __syncthreads();
+            if (tid < K && k0 + tid < a.top_k)
+                a.d_w[(size_t)t * a.top_k + k0 + tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+            __syncthreads();
+        }
     }
 }
 
@@ -505,8 +514,25 @@ static void combine_launch(const Launch &L, const CombineArgs &a) {
     while (log < 8 && (1u << log) < pieces) log++;
     const u32 tokens = kRowThreads >> log;
     const dim3 grid((a.n_tokens + tokens - 1) / tokens), block(kRowThreads);
-    if (a.top_k <= 8) hipLaunchKernelGGL((k_expert_combine<ET, true>), grid, block, 0, L.stream, a, log);
-    else hipLaunchKernelGGL((k_expert_combine<ET, false>), grid, block, 0, L.stream, a, log);
+    if (a.top_k == 1) hipLaunchKernelGGL((k_expert_combine<ET, 1, true>), grid, block, 0, L.stream, a, log);
+    else if (a.top_k == 2) hipLaunchKernelGGL((k_expert_combine<ET, 2, true>), grid, block, 0, L.stream, a, log);
+    else if (a.top_k <= 4) hipLaunchKernelGGL((k_expert_combine<ET, 4, true>), grid, block, 0, L.stream, a, log);
+    else if (a.top_k <= 8) hipLaunchKernelGGL((k_expert_combine<ET, 8, true>), grid, block, 0, L.stream, a, log);
+    else hipLaunchKernelGGL((k_expert_combine<ET, 8, false>), grid, block, 0, L.stream, a, log);
+}
+
+template <int ET, int K>
+static void grad_start(const Launch &L, const CombineGradArgs &a) {
+    const dim3 block(kRowThreads);
+    if (a.width <= 128 * kElemPiece<ET>) hipLaunchKernelGGL((k_expert_combine_grad<ET, K, 64>), dim3((a.n_tokens + 3) / 4), block, 0, L.stream, a);
+    else hipLaunchKernelGGL((k_expert_combine_grad<ET, K, 256>), dim3(a.n_tokens), block, 0, L.stream, a);
+}
+template <int ET>
+static void grad_launch(const Launch &L, const CombineGradArgs &a) {
+    if (a.top_k == 1) grad_start<ET, 1>(L, a);
+    else if (a.top_k == 2) grad_start<ET, 2>(L, a);
+    else if (a.top_k <= 4) grad_start<ET, 4>(L, a);
+    else grad_start<ET, 8>(L, a);
 }
 
 hipError_t expert_combine(const Launch &L, const void *rows, int et, int64_t ld_rows, const uint32_t *place, const float *w, const void *resid,
@@ -523,10 +549,9 @@ hipError_t expert_combine_grad(const Launch &L, const void *dy, int et, int64_t 
                                const float *w, int n_tokens, int top_k, int width, void *d_rows, int64_t ld_d_rows, float *d_w) {
     const CombineGradArgs a = {dy, (size_t)ld_dy, rows, (size_t)ld_rows, place, w, d_rows, (size_t)ld_d_rows, d_w, (u32)n_tokens, (u32)top_k,
                                (u32)width, (u32)n_tokens * (u32)top_k, L.fault, L.layer};
-    const dim3 grid((unsigned)n_tokens), block(kRowThreads);
-    if (et == kElemF32) hipLaunchKernelGGL(k_expert_combine_grad<kElemF32>, grid, block, 0, L.stream, a);
-    else if (et == kElemF16) hipLaunchKernelGGL(k_expert_combine_grad<kElemF16>, grid, block, 0, L.stream, a);
-    else hipLaunchKernelGGL(k_expert_combine_grad<kElemBF16>, grid, block, 0, L.stream, a);
+    if (et == kElemF32) grad_launch<kElemF32>(L, a);
+    else if (et == kElemF16) grad_launch<kElemF16>(L, a);
+    else grad_launch<kElemBF16>(L, a);
     return hipGetLastError();
 }
 

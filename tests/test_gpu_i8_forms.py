@@ -40,10 +40,11 @@ def test_product_in_every_form(gpu, held, m, rows, k):
     clean(gpu)
 
 
-# slots an expert: long runs (256 x 256), of some hundred (64 x 256), many tiles of short ones (64 x 128), shorter still (32 x 64), behind more than one
-# reading of 256 bounds
+# by slots an expert and the count of tiles: 256 x 256, 128 x 128, 64 x 256, 64 x 128, 32 x 64 (two rings), 64 x 64 (two rings), waves sharing k; behind
+# more than one reading of 256 bounds
 @pytest.mark.parametrize("m,n,top_k,rows,k", ((1100, 2, 1, 300, 272), (900, 3, 2, 513, 40), (200, 64, 4, 2900, 48), (330, 90, 4, 3100, 144), (20, 300, 4, 70, 272), (200, 1000, 2, 40, 16),
-                                              (999, 512, 8, 100, 48), (12, 1024, 3, 257, 272)))
+                                              (999, 512, 8, 100, 48), (12, 1024, 3, 257, 272), (3000, 8, 1, 2000, 48), (1500, 8, 1, 3010, 144), (900, 8, 1, 4500, 48), (64, 128, 2, 700, 272), (50, 30, 4, 600, 272), (300, 9, 1, 333, 400),
+                                              (700, 10, 1, 1500, 100), (40, 32, 4, 96, 400)))
 @pytest.mark.parametrize("own", (False, True), ids=("shared", "own"))
 def test_experts_product_in_every_form(gpu, held, own, m, n, top_k, rows, k):
     rng = np.random.default_rng(m + n + rows)

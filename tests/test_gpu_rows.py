@@ -122,7 +122,8 @@ class Rows:
 
 
 BATCHES = ((1, 4, 1, 1, 0), (1, 8, 8, 2048, 0), (2, 16, 3, 7, 2), (5, 9, 9, 100, 0), (16, 128, 8, 2048, 0), (33, 64, 17, 513, 1), (3, 100, 64, 72, 0),
-           (200, 8, 2, 24, 0), (40, 32, 8, 4100, 4), (77, 16, 4, 64, 0))
+           (200, 8, 2, 24, 0), (40, 32, 8, 4100, 4), (77, 16, 4, 64, 0), (303, 9, 1, 425, 0), (50, 9, 1, 2100, 1), (50, 9, 2, 1024, 0),
+           (50, 9, 2, 1030, 0), (21, 9, 4, 130, 3), (60, 12, 3, 2600, 0), (30, 12, 6, 500, 0))
 
 
 def near(got, exact, terms, n_roundings, dtype):
