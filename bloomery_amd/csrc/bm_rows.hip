@@ -521,6 +521,9 @@ static void combine_launch(const Launch &L, const CombineArgs &a) {
     else hipLaunchKernelGGL((k_expert_combine<ET, 8, false>), grid, block, 0, L.stream, a, log);
 }
 
+// us, bf16. A batch as small as the token's slots, which eight at a time would ask for again: 4096 tokens of one slot, 2048 wide, gradients 9.8 (by eights 20.3), sum 6.1 (12.7); of
+// four 24.6 and 14.4 (29.5, 17.3). A wave a token up to 128 pieces: 4096 tokens of eight slots, 1024 wide, 25.1 (a workgroup a token 29.3), 8192 tokens, 512 wide, 25.7
+// (41.0), of two slots 8.1 (32.8); 1400 wide by workgroups 31.
 template <int ET, int K>
 static void grad_start(const Launch &L, const CombineGradArgs &a) {
     const dim3 block(kRowThreads);
