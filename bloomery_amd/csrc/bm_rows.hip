@@ -37,18 +37,19 @@ struct RowAhead {
     uint4 v[N];
 };
 template <u32 N>
-__device__ __forceinline__ RowAhead<N> row_ahead(const SortArgs &a, u32 token) {
+__device__ __forceinline__ RowAhead<N> row_ahead(const SortArgs &a, u32 token, u32 thread, u32 threads) {
     RowAhead<N> r;
     const uint8_t *from = a.x + (size_t)token * a.x_line;
 #pragma unroll
     for (u32 i = 0; i < N; i++) {
-        const u32 at = 16 * (threadIdx.x + i * kRowThreads);
+        const u32 at = 16 * (thread + i * threads);
         if (at + 16 <= a.row_bytes) r.v[i] = bm_ld16u(from + at);
     }
     return r;
 }
+// (eight threads at least)
 template <int EB, u32 N>
-__device__ __forceinline__ void move_row(const SortArgs &a, u32 token, const u32 *places, const RowAhead<N> &ahead) {
+__device__ __forceinline__ void move_row(const SortArgs &a, u32 token, const u32 *places, const RowAhead<N> &ahead, u32 thread, u32 threads) {
     const uint8_t *from = a.x + (size_t)token * a.x_line;
     const auto piece = [&](u32 at, uint4 v) {
         for (u32 k = 0; k < a.top_k; k++)
@@ -56,12 +57,12 @@ __device__ __forceinline__ void move_row(const SortArgs &a, u32 token, const u32
     };
 #pragma unroll
     for (u32 i = 0; i < N; i++) {
-        const u32 at = 16 * (threadIdx.x + i * kRowThreads);
+        const u32 at = 16 * (thread + i * threads);
         if (at + 16 <= a.row_bytes) piece(at, ahead.v[i]);
     }
-    for (u32 at = 16 * (threadIdx.x + N * kRowThreads); at + 16 <= a.row_bytes; at += 16 * kRowThreads) piece(at, bm_ld16u(from + at));
+    for (u32 at = 16 * (thread + N * threads); at + 16 <= a.row_bytes; at += 16 * threads) piece(at, bm_ld16u(from + at));
     // what is left of a row that is no whole number of pieces, an element a thread
-    const u32 b = (a.row_bytes & ~15u) + EB * threadIdx.x;
+    const u32 b = (a.row_bytes & ~15u) + EB * thread;
     if (b < a.row_bytes)
         for (u32 k = 0; k < a.top_k; k++)
             if (places[k] != kUnlisted) __builtin_memcpy(a.rows + (size_t)places[k] * a.rows_line + b, from + b, EB);
@@ -109,7 +110,7 @@ __global__ __launch_bounds__(kRowThreads) void k_sort_few(SortArgs a) {
     RowAhead<T == 1 ? 2 : 1> ahead[T];
     if (a.x)
 #pragma unroll
-        for (u32 t = 0; t < T; t++) ahead[t] = row_ahead<T == 1 ? 2 : 1>(a, min(token + t, a.n_tokens - 1));
+        for (u32 t = 0; t < T; t++) ahead[t] = row_ahead<T == 1 ? 2 : 1>(a, min(token + t, a.n_tokens - 1), tid, kRowThreads);
     for (u32 k = tid; k < have; k += kRowThreads) places[k] = 0;
     __syncthreads();
     for (u32 k0 = 0; k0 < have; k0 += 8) {
@@ -141,7 +142,7 @@ __global__ __launch_bounds__(kRowThreads) void k_sort_few(SortArgs a) {
     __syncthreads();
 #pragma unroll
     for (u32 t = 0; t < T; t++)
-        if (token + t < a.n_tokens) move_row<EB>(a, token + t, places + t * a.top_k, ahead[t]);
+        if (token + t < a.n_tokens) move_row<EB>(a, token + t, places + t * a.top_k, ahead[t], tid, kRowThreads);
 }
 template <int EB>
 static void few_launch(const Launch &L, const SortArgs &a) {
@@ -283,14 +284,16 @@ __device__ __forceinline__ u32 sort_settle(const SortArgs &a, u32 s, u32 per) {
     a.order[p] = s;
     return p;
 }
+//    1 << log threads a token, several tokens a workgroup where rows are short (the whole sort, three launches, of 4810 tokens, eight slots, 128 wide, 13.4 us; a workgroup a token 15.6).
 template <int EB>
-__global__ __launch_bounds__(kRowThreads) void k_sort_move(SortArgs a, u32 per) {
-    __shared__ u32 places[kMaxCombineSlots];
-    const u32 token = blockIdx.x;
-    const RowAhead<2> ahead = row_ahead<2>(a, token);
-    if (threadIdx.x < a.top_k) places[threadIdx.x] = sort_settle(a, token * a.top_k + threadIdx.x, per);
+__global__ __launch_bounds__(kRowThreads) void k_sort_move(SortArgs a, u32 per, u32 log) {
+    __shared__ u32 places[kRowThreads / 8 * kMaxCombineSlots];
+    const u32 tid = threadIdx.x, mine = tid >> log, thread = tid & ((1u << log) - 1u), tokens = kRowThreads >> log;
+    const u32 token0 = blockIdx.x * tokens, token = min(token0 + mine, a.n_tokens - 1), have = min(tokens, a.n_tokens - token0) * a.top_k;
+    const RowAhead<2> ahead = row_ahead<2>(a, token, thread, 1u << log);
+    for (u32 i = tid; i < have; i += kRowThreads) places[i] = sort_settle(a, token0 * a.top_k + i, per);
     __syncthreads();
-    move_row<EB>(a, token, places, ahead);
+    if (token0 + mine < a.n_tokens) move_row<EB>(a, token, places + mine * a.top_k, ahead, thread, 1u << log);
 }
 __global__ __launch_bounds__(kRowThreads) void k_sort_places(SortArgs a, u32 n, u32 per) {
     const u32 s = blockIdx.x * kRowThreads + threadIdx.x;
@@ -320,8 +323,14 @@ hipError_t expert_sort(const Launch &L, const uint32_t *sel, int n_tokens, int t
     while ((1u << log_experts) < a.n_experts) log_experts++;
     hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, L.stream, a, chunks, log_experts);
     if (!x) hipLaunchKernelGGL(k_sort_places, dim3((n + kRowThreads - 1) / kRowThreads), dim3(kRowThreads), 0, L.stream, a, n, per);
-    else if (eb == 4) hipLaunchKernelGGL(k_sort_move<4>, dim3((unsigned)n_tokens), dim3(kRowThreads), 0, L.stream, a, per);
-    else hipLaunchKernelGGL(k_sort_move<2>, dim3((unsigned)n_tokens), dim3(kRowThreads), 0, L.stream, a, per);
+    else {
+        u32 log = 3;
+        while (log < 8 && (16u << log) < a.row_bytes) log++;
+        const u32 tokens = kRowThreads >> log;
+        const dim3 grid((a.n_tokens + tokens - 1) / tokens);
+        if (eb == 4) hipLaunchKernelGGL(k_sort_move<4>, grid, dim3(kRowThreads), 0, L.stream, a, per, log);
+        else hipLaunchKernelGGL(k_sort_move<2>, grid, dim3(kRowThreads), 0, L.stream, a, per, log);
+    }
     return hipGetLastError();
 }
 
