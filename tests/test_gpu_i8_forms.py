@@ -224,3 +224,43 @@ def test_two_contexts_at_once(gpu):
     finally:
         for c in contexts:
             c.close()
+
+
+@pytest.mark.parametrize("m", (1, 6, 40, 700))
+def test_a_product_captured_and_replayed(gpu, held, m):
+    """Two products behind one another as one graph, replayed over other rows with eager work between the replays."""
+    rng = np.random.default_rng(41 + m)
+    hidden, rows, dtype = 512, 1100, bm.BF16
+    w1, ws1 = some_matrix(rng, rows, hidden)
+    w2, ws2 = some_matrix(rng, hidden, rows)
+    d1, s1, d2, s2 = held.up(w1), held.up(ws1), held.up(junk_padded(w2, rows, rng)), held.up(ws2)
+    x, y, z = held.out(np.uint16, m * hidden), held.out(np.uint16, m * rows), held.out(np.uint16, m * hidden)
+    codes, scales = held.out(np.int8, m * bm.i8_row_bytes(rows)), held.out(np.float32, m)
+
+    def enqueue():
+        gpu.enqueue_i8_gemm_x(d1, s1, rows, hidden, x, dtype, m, codes, scales, y, dtype)
+        gpu.enqueue_i8_gemm_x(d2, s2, hidden, rows, y, dtype, m, codes, scales, z, dtype)
+
+    x.upload(bits(normal_f32(rng, (m, hidden)), dtype))
+    gpu.capture_begin()
+    enqueue()
+    graph = gpu.capture_end()
+    try:
+        for _ in range(3):
+            xf = rounded(normal_f32(rng, (m, hidden)), dtype)
+            x.upload(bits(xf, dtype))
+            for b in (y, z, codes, scales):
+                b.fill_bytes(0xEE)
+            gpu.graph_launch(graph)
+            replayed = [b.download() for b in (y, z, codes, scales)]
+            q, s = codes_of(xf)
+            assert np.array_equal(replayed[0].reshape(m, rows), bits(value(q, s, w1, ws1), dtype))
+            for b in (y, z, codes, scales):
+                b.fill_bytes(0x11)
+            enqueue()
+            gpu.sync()
+            for a, b in zip(replayed, (y, z, codes, scales)):
+                assert np.array_equal(a.view(np.uint8), b.download().view(np.uint8))
+    finally:
+        gpu.graph_destroy(graph)
+    clean(gpu)
