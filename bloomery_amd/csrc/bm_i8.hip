@@ -1047,8 +1047,9 @@ hipError_t i8_gemm_x(const Launch &L, const int8_t *w, const float *ws, int rows
 //   the same two, 198, 128 x 128 223; 4096 cubed 58, 90, 66; 8192 cubed 453, 507, 538; 4096 x 2048 x 7168, the 128 x 128 first, 59, 80, 69.)
 //   Below some hundred large tiles the smaller ones fill the card. 64 x 64 with four steps in flight while they are one round of two a unit: 1024 x 2048 x 7168 25.2
 //   (64 x 128: 36.1, 128 x 128: 37.8), 256 x 7168 x 2048 10.0 (12.9, 14.5); with two steps, five a unit, up to three: 1280 x 2048 x 2048 12.8 (64 x 128: 14.8), 1536 rows 12.7 (14.2), but
-//   2048 16.8 (15.6). Then 64 x 128 for little more than a round of two, 700 x 7168 x 2048 18.5 (128 x 128: 19.5), and 128 x 128: 1024 x 7168 x 2048 21.0 (64 x 128: 27.3). Fewer
-//   than three 64 x 64 for four units are 32 x 64's: 256 x 2048 x 7168 13.2 (14.3).
+//   2048 16.8 (15.6). Then 64 x 128 for little more than a round of two, 700 x 7168 x 2048 18.5 (128 x 128: 19.5), and 128 x 128: 1024 x 7168 x 2048 21.0 (64 x 128: 27.3). 32 x 64
+//   while they are one round: 256 x 2048 x 7168 13.2 (64 x 64: 14.3); two rounds lose, 1280 x 512 x 4096 13.1 (11.0). Short rows need no four steps: 640 x 1024 x 512 in 64 x 64 with two
+//   steps 4.4 (four: 4.8), 400 x 1500 x 1024 5.9 (6.5).
 //   Where tiles of at most 32 x 32 are no more than the compute units, a workgroup's waves share a row's k (k_i8_few), in the smallest tile that is one
 //   round: 34 x 544 x 8064 in 16 x 16 5.6 (16 x 32: 7.0, 32 x 64 whole rows 13), 64 x 2048 x 7168 in 16 x 32 6.5 (32 x 32: 7.9; 12.8), 128 x 2048 x 7168 in 32 x 32 8.1 (16 x 32:
 //   11.2; 12.9), 24 x 7168 x 2048 5.1 (7.1), one row of 2048 x 7168 4.9, of 7168 x 7168 9.6; two rounds lose, 64 x 7168 x 2048 8.2 (32 x 64: 7.5).
@@ -1093,8 +1094,8 @@ hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_expe
     if (tiles(16, 32) <= 256) return few_launch<2, 1, 4>(L, a, n);
     if (n <= 16) return few_launch<2, 1, 3>(L, a, n);
     if (n <= 32 || tiles(32, 32) <= 256) return few_launch<2, 2, 4>(L, a, n);
-    if (tiles(64, 64) < 192) return tile_launch<32, 64, 1, 2, 4, true, 2>(L, a, n);
-    if (tiles(64, 64) <= 512) return tile_launch<64, 64, 2, 2, 4, true, 2>(L, a, n);
+    if (tiles(32, 64) <= 256) return tile_launch<32, 64, 1, 2, 4, true, 2>(L, a, n);
+    if (tiles(64, 64) <= 512 && a.kp > 1024) return tile_launch<64, 64, 2, 2, 4, true, 2>(L, a, n);
     if (tiles(64, 64) <= 768) return tile_launch<64, 64, 2, 2, 2, true, 2>(L, a, n);
     if (tiles(256, 256) >= 96) {
         const uint64_t by256 = 64 * ((tiles(256, 256) + 255) / 256), by224 = 57 * ((tiles(256, 224) + 255) / 256), by128 = 39 * ((tiles(128, 128) + 511) / 512);

@@ -22,7 +22,7 @@ def value(q, s, w, ws):
 
 # by the count of tiles: waves sharing k (tiles of 16 x 16, 16 x 32, 32 x 32), then tiles of 32 x 64, 64 x 64 (two rings), 64 x 128, 128 x 128, 256 x
 # 256, 256 x 224; k of three lines and a piece, of half a line, of many lines and an odd number of values
-SIZES = ((7, 4000, 272), (16, 8200, 272), (1, 9001, 1030), (20, 8300, 100), (90, 1200, 272), (250, 1000, 2056), (40, 9000, 272), (700, 1100, 272), (700, 1100, 40), (650, 1300, 1111),
+SIZES = ((7, 4000, 272), (16, 8200, 272), (1, 9001, 1030), (20, 8300, 100), (90, 1200, 272), (250, 1000, 2056), (40, 9000, 272), (200, 1600, 272), (250, 2000, 1040), (700, 1100, 272), (700, 1100, 40), (650, 1300, 1111),
          (1600, 1400, 272), (1500, 1500, 144), (2050, 1600, 272), (2300, 2300, 272), (2301, 2299, 130), (4000, 4000, 272), (4001, 3999, 30), (4000, 3500, 272), (3990, 3490, 650))
 
 
