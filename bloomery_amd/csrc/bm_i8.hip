@@ -609,11 +609,13 @@ struct I8Tile {
 };
 
 // A tile of the experts: their runs cut into tiles of BT entries, numbered through the experts in order. False: there is none of that number. The bounds
-// of 256 experts are asked for at once; a run that is none raises ExpertId (once a launch and wave of the first tile) and has no tiles.
+// of 256 experts are asked for at once; a run that is none has no tiles. `check`: every run is looked at, those behind the tile too, and one that
+// is none raises ExpertId (one workgroup of a launch does so).
 template <int BT>
-__device__ __forceinline__ bool i8_find_tile(const I8Args &a, u32 tile, u32 &expert, u32 &t0) {
+__device__ __forceinline__ bool i8_find_tile(const I8Args &a, u32 tile, bool check, u32 &expert, u32 &t0) {
     const u32 lane = threadIdx.x & 63;
     u32 before = 0;
+    bool found = false;
     for (u32 e0 = 0; e0 < a.n_experts; e0 += 256) {
         u32 j0[4], j1[4];
 #pragma unroll
@@ -622,12 +624,18 @@ __device__ __forceinline__ bool i8_find_tile(const I8Args &a, u32 tile, u32 &exp
             j0[i] = a.start[e];
             j1[i] = a.start[e + 1];
         }
+        if (check) {
+            bool none = false;
+#pragma unroll
+            for (u32 i = 0; i < 4; i++) none |= j0[i] > j1[i] || j1[i] > a.n_slots; // (lanes past the last look at the last once more)
+            if (none) bm_raise(a.fault, a.layer, kSiteExpertId);
+            if (found) continue;
+        }
 #pragma unroll
         for (u32 i = 0; i < 4; i++) {
             const u32 e = e0 + 64 * i + lane;
             if (e0 + 64 * i >= a.n_experts) break;
             const bool run = j0[i] <= j1[i] && j1[i] <= a.n_slots;
-            if (e < a.n_experts && !run && tile == 0) bm_raise(a.fault, a.layer, kSiteExpertId);
             const u32 c = e < a.n_experts && run ? (j1[i] - j0[i] + BT - 1) / BT : 0;
             u32 upto = c;
 #pragma unroll
@@ -640,12 +648,14 @@ __device__ __forceinline__ bool i8_find_tile(const I8Args &a, u32 tile, u32 &exp
                 const int l = __builtin_ctzll(mine);
                 expert = (u32)__builtin_amdgcn_readfirstlane((int)(e0 + 64 * i + (u32)l));
                 t0 = (u32)__builtin_amdgcn_readfirstlane((int)((tile - before - (u32)__shfl((int)(upto - c), l, 64)) * BT));
-                return true;
+                if (!check) return true;
+                found = true;
+                break;
             }
             before += (u32)__shfl((int)upto, 63, 64);
         }
     }
-    return false;
+    return found;
 }
 
 // All but the last AHEAD steps that a wave asked for have landed, and every wave is done with the buffer that is written next. (The wait as a
@@ -875,7 +885,7 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
         tile = blockIdx.x / n_row_tiles;
     }
     if (!a.start) t0 = tile * BT;
-    else if (!i8_find_tile<BT>(a, tile, expert, t0)) return;
+    else if (!i8_find_tile<BT>(a, tile, tile == 0 && row_tile == 0, expert, t0)) return;
     const u32 r0 = row_tile * BR;
     I8Run run;
     if (!i8_run(a, expert, run)) return;

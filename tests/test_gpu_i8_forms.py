@@ -264,3 +264,31 @@ def test_a_product_captured_and_replayed(gpu, held, m):
     finally:
         gpu.graph_destroy(graph)
     clean(gpu)
+
+
+@pytest.mark.parametrize("n,bad", ((60, 59), (100, 70), (300, 64), (300, 255), (300, 299), (1024, 900)))
+def test_a_run_that_is_none_far_behind_the_first_raises(gpu, held, n, bad):
+    """Wherever in the table: the runs in front of it and behind it are computed, and the fault is there."""
+    rng = np.random.default_rng(n + bad)
+    n_slots, rows, k = 700, 130, 48
+    w, ws = some_matrix(rng, n * rows, k)
+    q = rng.integers(-127, 128, (n_slots, k), dtype=np.int16).astype(np.int8)
+    s = rng.random(n_slots).astype(np.float32)
+    start = np.linspace(0, n_slots, n + 1).astype(np.uint32)
+    wd, wsd, qd, sd = held.up(w), held.up(ws), held.up(q), held.up(s)
+    for end in (None, n_slots + 1, 0xFFFFFFFF):
+        table = start.copy()
+        if end is not None:
+            table[bad + 1] = end  # the run `bad` passes the slots, and the one behind it runs backwards
+        gpu.fault_clear()
+        y = held.out(np.float32, n_slots * rows)
+        gpu.enqueue_i8_gemm_experts(wd, wsd, n, rows, k, qd, sd, None, held.up(table), n_slots, 0, y, bm.F32)
+        got, done = y.download().reshape(n_slots, rows), np.zeros(n_slots, bool)
+        for e in range(n):
+            a, b = int(table[e]), int(table[e + 1])
+            if a <= b <= n_slots:
+                assert np.array_equal(got[a:b], value(q[a:b], s[a:b], w[e * rows:(e + 1) * rows], ws[e * rows:(e + 1) * rows])), e
+                done[a:b] = True
+        assert (got[~done].view(np.uint32) == 0xEEEEEEEE).all()
+        assert (gpu.fault()[0] & 0xFF == bm.SITE_EXPERT_ID) == (end is not None)
+        gpu.fault_clear()
