@@ -1461,7 +1461,7 @@ int64_t bm_expert_sort_work(int n_slots, int n_experts) {
     return (int64_t)bmk::expert_sort_work(n_slots, n_experts);
 }
 
-int bm_expert_sort(bm_ctx *ctx, const uint32_t *sel_dev, int n_tokens, int top_k, int n_experts, const void *x_dev, int type, int64_t ld_x,
+int bm_expert_sort(bm_ctx *ctx, const uint32_t *sel_dev, int n_tokens, int top_k, int n_experts, const void *x_dev, int elem_type, int64_t ld_x,
                    int width, uint32_t *order_dev, uint32_t *start_dev, uint32_t *place_dev, void *rows_dev, int64_t ld_rows, uint32_t *work_dev) {
     const char *what = "bm_expert_sort";
     BM_TRY(check_tokens(ctx, what, n_tokens, top_k));
@@ -1472,62 +1472,62 @@ int bm_expert_sort(bm_ctx *ctx, const uint32_t *sel_dev, int n_tokens, int top_k
     BM_TRY(check_words(ctx, what, "place_dev", place_dev));
     if (bmk::expert_sort_work(n_tokens * top_k, n_experts) > 0) BM_TRY(check_words(ctx, what, "work_dev", work_dev));
     if (x_dev || rows_dev) {
-        BM_TRY(check_elem(ctx, what, type));
+        BM_TRY(check_elem(ctx, what, elem_type));
         BM_TRY(check_width(ctx, what, width));
-        BM_TRY(check_rows(ctx, what, "x_dev", x_dev, type, width, ld_x));
-        BM_TRY(check_rows(ctx, what, "rows_dev", rows_dev, type, width, ld_rows));
+        BM_TRY(check_rows(ctx, what, "x_dev", x_dev, elem_type, width, ld_x));
+        BM_TRY(check_rows(ctx, what, "rows_dev", rows_dev, elem_type, width, ld_rows));
     }
     if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
     DeviceScope on(ctx->device);
-    return driver(ctx, what, bmk::expert_sort(launch_of(ctx), sel_dev, n_tokens, top_k, n_experts, x_dev, type, ld_x, width, order_dev, start_dev,
+    return driver(ctx, what, bmk::expert_sort(launch_of(ctx), sel_dev, n_tokens, top_k, n_experts, x_dev, elem_type, ld_x, width, order_dev, start_dev,
                                               place_dev, rows_dev, ld_rows, work_dev));
 }
 
-static int expert_sum(bm_ctx *ctx, const char *what, const char *from, const void *rows_dev, int type, int64_t ld_rows, const uint32_t *place_dev,
+static int expert_sum(bm_ctx *ctx, const char *what, const char *from, const void *rows_dev, int elem_type, int64_t ld_rows, const uint32_t *place_dev,
                       const float *w_dev, const void *resid_dev, int64_t ld_resid, int n_tokens, int top_k, int width, const char *to, void *y_dev,
                       int64_t ld_y) {
     BM_TRY(check_tokens(ctx, what, n_tokens, top_k));
-    BM_TRY(check_elem(ctx, what, type));
+    BM_TRY(check_elem(ctx, what, elem_type));
     BM_TRY(check_width(ctx, what, width));
-    BM_TRY(check_rows(ctx, what, from, rows_dev, type, width, ld_rows));
+    BM_TRY(check_rows(ctx, what, from, rows_dev, elem_type, width, ld_rows));
     BM_TRY(check_words(ctx, what, "place_dev", place_dev));
-    if (resid_dev) BM_TRY(check_rows(ctx, what, "resid_dev", resid_dev, type, width, ld_resid));
-    BM_TRY(check_rows(ctx, what, to, y_dev, type, width, ld_y));
+    if (resid_dev) BM_TRY(check_rows(ctx, what, "resid_dev", resid_dev, elem_type, width, ld_resid));
+    BM_TRY(check_rows(ctx, what, to, y_dev, elem_type, width, ld_y));
     if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
     DeviceScope on(ctx->device);
-    return driver(ctx, what, bmk::expert_combine(launch_of(ctx), rows_dev, type, ld_rows, place_dev, w_dev, resid_dev, ld_resid, n_tokens, top_k,
+    return driver(ctx, what, bmk::expert_combine(launch_of(ctx), rows_dev, elem_type, ld_rows, place_dev, w_dev, resid_dev, ld_resid, n_tokens, top_k,
                                                  width, y_dev, ld_y));
 }
 
-int bm_expert_sort_grad(bm_ctx *ctx, const void *d_rows_dev, int type, int64_t ld_rows, const uint32_t *place_dev, int n_tokens, int top_k,
+int bm_expert_sort_grad(bm_ctx *ctx, const void *d_rows_dev, int elem_type, int64_t ld_rows, const uint32_t *place_dev, int n_tokens, int top_k,
                         int width, void *dx_dev, int64_t ld_dx) {
-    return expert_sum(ctx, "bm_expert_sort_grad", "d_rows_dev", d_rows_dev, type, ld_rows, place_dev, nullptr, nullptr, 0, n_tokens, top_k, width,
+    return expert_sum(ctx, "bm_expert_sort_grad", "d_rows_dev", d_rows_dev, elem_type, ld_rows, place_dev, nullptr, nullptr, 0, n_tokens, top_k, width,
                       "dx_dev", dx_dev, ld_dx);
 }
 
-int bm_expert_combine(bm_ctx *ctx, const void *rows_dev, int type, int64_t ld_rows, const uint32_t *place_dev, const float *w_dev,
+int bm_expert_combine(bm_ctx *ctx, const void *rows_dev, int elem_type, int64_t ld_rows, const uint32_t *place_dev, const float *w_dev,
                       const void *resid_dev, int64_t ld_resid, int n_tokens, int top_k, int width, void *y_dev, int64_t ld_y) {
     BM_TRY(check_words(ctx, "bm_expert_combine", "w_dev", w_dev));
-    return expert_sum(ctx, "bm_expert_combine", "rows_dev", rows_dev, type, ld_rows, place_dev, w_dev, resid_dev, ld_resid, n_tokens, top_k, width,
+    return expert_sum(ctx, "bm_expert_combine", "rows_dev", rows_dev, elem_type, ld_rows, place_dev, w_dev, resid_dev, ld_resid, n_tokens, top_k, width,
                       "y_dev", y_dev, ld_y);
 }
 
-int bm_expert_combine_grad(bm_ctx *ctx, const void *dy_dev, int type, int64_t ld_dy, const void *rows_dev, int64_t ld_rows,
+int bm_expert_combine_grad(bm_ctx *ctx, const void *dy_dev, int elem_type, int64_t ld_dy, const void *rows_dev, int64_t ld_rows,
                            const uint32_t *place_dev, const float *w_dev, int n_tokens, int top_k, int width, void *d_rows_dev, int64_t ld_d_rows,
                            float *d_w_dev) {
     const char *what = "bm_expert_combine_grad";
     BM_TRY(check_tokens(ctx, what, n_tokens, top_k));
-    BM_TRY(check_elem(ctx, what, type));
+    BM_TRY(check_elem(ctx, what, elem_type));
     BM_TRY(check_width(ctx, what, width));
-    BM_TRY(check_rows(ctx, what, "dy_dev", dy_dev, type, width, ld_dy));
-    BM_TRY(check_rows(ctx, what, "rows_dev", rows_dev, type, width, ld_rows));
+    BM_TRY(check_rows(ctx, what, "dy_dev", dy_dev, elem_type, width, ld_dy));
+    BM_TRY(check_rows(ctx, what, "rows_dev", rows_dev, elem_type, width, ld_rows));
     BM_TRY(check_words(ctx, what, "place_dev", place_dev));
     BM_TRY(check_words(ctx, what, "w_dev", w_dev));
-    BM_TRY(check_rows(ctx, what, "d_rows_dev", d_rows_dev, type, width, ld_d_rows));
+    BM_TRY(check_rows(ctx, what, "d_rows_dev", d_rows_dev, elem_type, width, ld_d_rows));
     BM_TRY(check_words(ctx, what, "d_w_dev", d_w_dev));
     if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
     DeviceScope on(ctx->device);
-    return driver(ctx, what, bmk::expert_combine_grad(launch_of(ctx), dy_dev, type, ld_dy, rows_dev, ld_rows, place_dev, w_dev, n_tokens, top_k,
+    return driver(ctx, what, bmk::expert_combine_grad(launch_of(ctx), dy_dev, elem_type, ld_dy, rows_dev, ld_rows, place_dev, w_dev, n_tokens, top_k,
                                                       width, d_rows_dev, ld_d_rows, d_w_dev));
 }
 
@@ -1546,12 +1546,12 @@ static int check_i8(bm_ctx *ctx, const char *what, int m, int k) {
     return BM_OK;
 }
 
-static int i8_quant(bm_ctx *ctx, const char *what, const void *x_dev, const void *u_dev, bool glu, int type, int64_t ld, int m, int k,
+static int i8_quant(bm_ctx *ctx, const char *what, const void *x_dev, const void *u_dev, bool glu, int elem_type, int64_t ld, int m, int k,
                     const bm_gate_act *rule, const uint32_t *live_dev, int8_t *codes_dev, float *scales_dev) {
     BM_TRY(check_i8(ctx, what, m, k));
-    BM_TRY(check_elem(ctx, what, type));
-    BM_TRY(check_rows(ctx, what, glu ? "g_dev" : "x_dev", x_dev, type, k, ld));
-    if (glu) BM_TRY(check_rows(ctx, what, "u_dev", u_dev, type, k, ld));
+    BM_TRY(check_elem(ctx, what, elem_type));
+    BM_TRY(check_rows(ctx, what, glu ? "g_dev" : "x_dev", x_dev, elem_type, k, ld));
+    if (glu) BM_TRY(check_rows(ctx, what, "u_dev", u_dev, elem_type, k, ld));
     if (((uintptr_t)live_dev & 3) != 0) return fail(ctx, BM_ESHAPE, "%s: live_dev %p is not 4-byte aligned", what, (const void *)live_dev);
     BM_TRY(check_codes(ctx, what, "codes_dev", codes_dev, "scales_dev", scales_dev));
     bmk::GateRule checked = {0u, 0.0f};
@@ -1560,17 +1560,17 @@ static int i8_quant(bm_ctx *ctx, const char *what, const void *x_dev, const void
     bmk::Launch L = launch_of(ctx);
     if (rule) L.rule = checked;
     DeviceScope on(ctx->device);
-    return driver(ctx, what, bmk::i8_quantize(L, x_dev, u_dev, type, ld, m, k, live_dev, codes_dev, scales_dev));
+    return driver(ctx, what, bmk::i8_quantize(L, x_dev, u_dev, elem_type, ld, m, k, live_dev, codes_dev, scales_dev));
 }
 
-int bm_i8_quantize(bm_ctx *ctx, const void *x_dev, int type, int64_t ld_x, int m, int k, const uint32_t *live_dev, int8_t *codes_dev,
+int bm_i8_quantize(bm_ctx *ctx, const void *x_dev, int elem_type, int64_t ld_x, int m, int k, const uint32_t *live_dev, int8_t *codes_dev,
                    float *scales_dev) {
-    return i8_quant(ctx, "bm_i8_quantize", x_dev, nullptr, false, type, ld_x, m, k, nullptr, live_dev, codes_dev, scales_dev);
+    return i8_quant(ctx, "bm_i8_quantize", x_dev, nullptr, false, elem_type, ld_x, m, k, nullptr, live_dev, codes_dev, scales_dev);
 }
 
-int bm_i8_swiglu_quantize(bm_ctx *ctx, const void *g_dev, const void *u_dev, int type, int64_t ld, int m, int k, const bm_gate_act *rule,
+int bm_i8_swiglu_quantize(bm_ctx *ctx, const void *g_dev, const void *u_dev, int elem_type, int64_t ld, int m, int k, const bm_gate_act *rule,
                           const uint32_t *live_dev, int8_t *codes_dev, float *scales_dev) {
-    return i8_quant(ctx, "bm_i8_swiglu_quantize", g_dev, u_dev, true, type, ld, m, k, rule, live_dev, codes_dev, scales_dev);
+    return i8_quant(ctx, "bm_i8_swiglu_quantize", g_dev, u_dev, true, elem_type, ld, m, k, rule, live_dev, codes_dev, scales_dev);
 }
 
 static int check_i8_weights(bm_ctx *ctx, const char *what, const int8_t *w_dev, const float *w_scales_dev, int rows, int k) {

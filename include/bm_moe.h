@@ -490,24 +490,24 @@ int bm_card_gemv_sel(bm_ctx *ctx, const bm_weights *w, const int8_t *codes_dev, 
  * tables, place_dev[s] the place of slot s in order (order's inverse; 0xffffffff for a slot that no run lists), and row place[s]
  * of rows_dev token s / top_k's row of x_dev. An id at or past n_experts joins no run and, unless it is BM_HOST_SLOT, raises
  * BM_SITE_EXPERT_ID. Entries of order_dev and rows of rows_dev behind the last listed one keep what they held. x_dev and rows_dev
- * both NULL: the tables alone (type, width and the lines are not looked at). rows_dev: n_tokens * top_k rows.
+ * both NULL: the tables alone (elem_type, width and the lines are not looked at). rows_dev: n_tokens * top_k rows.
  * work_dev: bm_expert_sort_work(n_tokens * top_k, n_experts) words of scratch that holds nothing between calls (NULL where that is 0: a
  * sort of up to 4096 slots is one launch, a longer one three). At most ceil(n_slots / 512) * n_experts words. */
 int64_t bm_expert_sort_work(int n_slots, int n_experts);
-int bm_expert_sort(bm_ctx *ctx, const uint32_t *sel_dev, int n_tokens, int top_k, int n_experts, const void *x_dev, int type, int64_t ld_x,
+int bm_expert_sort(bm_ctx *ctx, const uint32_t *sel_dev, int n_tokens, int top_k, int n_experts, const void *x_dev, int elem_type, int64_t ld_x,
                    int width, uint32_t *order_dev, uint32_t *start_dev, uint32_t *place_dev, void *rows_dev, int64_t ld_rows, uint32_t *work_dev);
 /* Its gradient: dx[t] = sum of d_rows[place[s]] over token t's listed slots, ascending. A token with none gets zeros. */
-int bm_expert_sort_grad(bm_ctx *ctx, const void *d_rows_dev, int type, int64_t ld_rows, const uint32_t *place_dev, int n_tokens, int top_k,
+int bm_expert_sort_grad(bm_ctx *ctx, const void *d_rows_dev, int elem_type, int64_t ld_rows, const uint32_t *place_dev, int n_tokens, int top_k,
                         int width, void *dx_dev, int64_t ld_dx);
 /* And back: y[t] = (acc = 0; for token t's listed slots s ascending: acc = fma(w[s], rows[place[s]], acc)) + resid[t], bm_combine_tokens'
  * sum over sorted rows. A slot that is not listed adds nothing, whatever its weight. resid_dev may be NULL (no add). A place at
  * or past n_tokens * top_k other than 0xffffffff raises BM_SITE_EXPERT_ID and adds nothing, here and in the gradients. (rows_dev, and
  * d_rows_dev above, hold n_tokens * top_k rows; the first may be read, and not used, where a token has no listed slot.) */
-int bm_expert_combine(bm_ctx *ctx, const void *rows_dev, int type, int64_t ld_rows, const uint32_t *place_dev, const float *w_dev,
+int bm_expert_combine(bm_ctx *ctx, const void *rows_dev, int elem_type, int64_t ld_rows, const uint32_t *place_dev, const float *w_dev,
                       const void *resid_dev, int64_t ld_resid, int n_tokens, int top_k, int width, void *y_dev, int64_t ld_y);
 /* Its gradients: d_rows[place[s]] = w[s] * dy[t] and d_w[s] = <dy[t], rows[place[s]]> (f32, each dot summed in one order whatever the
  * launch; 0 for a slot that is not listed); resid's gradient is dy. Rows of d_rows_dev that no slot is placed at keep what they held. */
-int bm_expert_combine_grad(bm_ctx *ctx, const void *dy_dev, int type, int64_t ld_dy, const void *rows_dev, int64_t ld_rows,
+int bm_expert_combine_grad(bm_ctx *ctx, const void *dy_dev, int elem_type, int64_t ld_dy, const void *rows_dev, int64_t ld_rows,
                            const uint32_t *place_dev, const float *w_dev, int n_tokens, int top_k, int width, void *d_rows_dev, int64_t ld_d_rows,
                            float *d_w_dev);
 
@@ -521,11 +521,11 @@ int bm_expert_combine_grad(bm_ctx *ctx, const void *dy_dev, int type, int64_t ld
 int64_t bm_i8_row_bytes(int k);
 /* m rows (1 .. 2^22) of k elements. live_dev (optional): a device word; rows at or past its value keep what they held (of sorted rows:
  * start_dev + n_experts). */
-int bm_i8_quantize(bm_ctx *ctx, const void *x_dev, int type, int64_t ld_x, int m, int k, const uint32_t *live_dev, int8_t *codes_dev,
+int bm_i8_quantize(bm_ctx *ctx, const void *x_dev, int elem_type, int64_t ld_x, int m, int k, const uint32_t *live_dev, int8_t *codes_dev,
                    float *scales_dev);
 /* The same of the gate rule's values of two inputs (bm_swiglu_quant in this form; rule NULL: the context's), g_dev and u_dev rows both ld
  * apart; the values are f32 on the way. */
-int bm_i8_swiglu_quantize(bm_ctx *ctx, const void *g_dev, const void *u_dev, int type, int64_t ld, int m, int k, const bm_gate_act *rule,
+int bm_i8_swiglu_quantize(bm_ctx *ctx, const void *g_dev, const void *u_dev, int elem_type, int64_t ld, int m, int k, const bm_gate_act *rule,
                           const uint32_t *live_dev, int8_t *codes_dev, float *scales_dev);
 /* y[t * ld_y + r] = (f32(sum over k of codes[t] . w[r]) * scales[t]) * w_scales[r] for t < m, r < rows (1 .. 2^22 each): the sum in
  * int32, exact, so the value does not depend on how the work is split. w_dev: rows of bm_i8_row_bytes(k) bytes; what they hold behind

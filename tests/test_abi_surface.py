@@ -53,3 +53,28 @@ def test_the_build_recipe_names_every_source_of_the_library():
     assert len(srcs) >= 7
     for s in srcs:
         assert f'"{s}"' in recipe, f"{s} is built by the Makefile and missing from the build.rs shown"
+
+
+# what Rust takes for no plain identifier (strict and reserved words)
+RUST_WORDS = set("""as break const continue crate else enum extern false fn for if impl in let loop match mod move mut pub ref return self Self static
+struct super trait true type unsafe use where while async await dyn abstract become box do final macro override priv typeof unsized virtual
+yield try gen""".split())
+RUST_TYPE = re.compile(r"(\*(const|mut) )*(c_int|c_char|c_void|usize|[iu](8|16|32|64)|f32|f64|bool|bm_\w+)$")
+
+
+def test_the_binding_block_is_rust():
+    """A name that is a word of the language's own, in one declaration, costs the whole block: names of functions, arguments and fields, and
+    the types of arguments and results, in every Rust block of the notes."""
+    blocks = re.findall(r"```rust\n(.*?)```", open(NOTES).read(), flags=re.S)
+    assert blocks
+    block = "\n".join(blocks)
+    for name in re.findall(r"pub (?:const |static |fn |struct )?(r#\w+|\w+)\s*[:({=]", block):
+        assert name not in RUST_WORDS, name
+    functions = re.findall(r"pub fn (bm_\w+)\s*\((.*?)\)\s*(?:->\s*([^;]*?))?\s*;", block, flags=re.S)
+    assert len(functions) > 60
+    for name, params, result in functions:
+        assert not result or RUST_TYPE.match(" ".join(result.split())), (name, result)
+        for p in filter(None, (" ".join(p.split()) for p in params.split(","))):
+            arg, of = (t.strip() for t in p.split(":", 1))
+            assert re.fullmatch(r"(r#)?[a-z_]\w*", arg) and arg not in RUST_WORDS, f"{name}: {arg} is no name of an argument"
+            assert RUST_TYPE.match(of), (name, p)
