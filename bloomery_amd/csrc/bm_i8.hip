@@ -16,6 +16,15 @@ namespace bmk {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 
+// A dimension of a launch has fewer than 2^32 threads. Workgroups that would be more go along a second one, 2^20 a step; i8_group numbers them through
+// (the last step may be ragged: what it has too many finds nothing to do).
+constexpr u32 kGroupsLog = 20;
+static dim3 i8_grid(uint64_t groups, u32 threads) {
+    if (groups * threads <= 0xffffffffu) return dim3((u32)groups);
+    return dim3(1u << kGroupsLog, (u32)((groups + (1u << kGroupsLog) - 1) >> kGroupsLog));
+}
+__device__ __forceinline__ u32 i8_group() { return blockIdx.y << kGroupsLog | blockIdx.x; }
+
 // ------------------------------------------------------------------------------------------------ quantizer
 
 // The code of v under scale s (normal, not small), inv = fl(1 / s). rint(v * inv) is off by one at most, and only where the quotient lies
@@ -162,7 +171,7 @@ template <int ET, bool GLU, int T, int CH>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void k_i8_quantize(QuantArgs a) {
     constexpr int kThreads = T < 256 ? 256 : T;
     __shared__ u32 top[T / 64];
-    const u32 lane = threadIdx.x % T, row = blockIdx.x * (kThreads / T) + threadIdx.x / T;
+    const u32 lane = threadIdx.x % T, row = i8_group() * (kThreads / T) + threadIdx.x / T;
     const u32 m = a.live ? min(a.m, *a.live) : a.m;
     if (row >= m) return; // whole waves (T = 64) or the workgroup
     float v[CH ? CH : 1][8];
@@ -215,7 +224,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_i8_quantize(QuantArgs a) 
 template <int ET, bool GLU, int T, int CH>
 static void quant_start(const Launch &L, const QuantArgs &a) {
     constexpr u32 threads = T < 256 ? 256 : T, rows = threads / T;
-    hipLaunchKernelGGL((k_i8_quantize<ET, GLU, T, CH>), dim3((a.m + rows - 1) / rows), dim3(threads), 0, L.stream, a);
+    hipLaunchKernelGGL((k_i8_quantize<ET, GLU, T, CH>), i8_grid((a.m + rows - 1) / rows, threads), dim3(threads), 0, L.stream, a);
 }
 // us on MI355X, bf16, alone and behind the gate rule. While the rows are not eight a compute unit a row's length is dealt to more threads, a piece each: 24 x
 // 7168 4.0 and 4.2 (256 threads of four pieces: 5.5, 6.3), 1500 x 7168 10.2 and 15.2 (10.8, 16.7), 1024 x 4096 4.9 and 6.8 (5.4, 7.6); behind that more pieces a thread

@@ -292,3 +292,43 @@ def test_a_run_that_is_none_far_behind_the_first_raises(gpu, held, n, bad):
         assert (got[~done].view(np.uint32) == 0xEEEEEEEE).all()
         assert (gpu.fault()[0] & 0xFF == bm.SITE_EXPERT_ID) == (end is not None)
         gpu.fault_clear()
+
+
+def needs_memory(gigabytes):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < gigabytes << 30:
+        pytest.skip(f"{gigabytes} GiB of the card's memory are not free")
+
+
+def test_the_most_rows_of_the_longest_form(gpu):
+    """2^22 rows past 8192 values, a workgroup of 1024 threads each: 2^32 threads. Rows of zeros, some others spread among them."""
+    needs_memory(110)
+    m, k = 1 << 22, 8193
+    kp = bm.i8_row_bytes(k)
+    at = torch.tensor([0, 1, (1 << 20) - 1, 1 << 20, (1 << 21) + 7, 3 << 20, m - 2, m - 1])
+    torch.manual_seed(5)
+    some = torch.randn(at.numel(), k).bfloat16()
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    x[at.cuda()] = some.cuda()
+    codes, scales = torch.empty(m, kp, dtype=torch.int8, device="cuda").fill_(0x55), torch.full((m,), -1.0, device="cuda")
+    q, s = codes_of(some.float().numpy())
+    live = torch.tensor([m - 1], dtype=torch.int32, device="cuda")
+    try:
+        for n, word in ((m - 1, PTR(live)), (m, None)):
+            torch.cuda.synchronize()
+            gpu.enqueue_i8_quantize(PTR(x), bm.BF16, m, k, PTR(codes), PTR(scales), live=word)
+            gpu.sync()
+            if n < m:  # the row behind the last is left as it was
+                assert (codes[n:].cpu() == 0x55).all() and scales[n].item() == -1.0
+            there = at[at < n]
+            assert np.array_equal(codes[there.cuda()].cpu().numpy(), padded(q[:there.numel()], k))
+            want = torch.zeros(n)
+            want[there] = torch.from_numpy(s)[:there.numel()]
+            assert torch.equal(scales[:n].cpu(), want)
+        codes[at.cuda()] = 0
+        for part in codes.view(torch.int64).split(1 << 19):
+            assert not part.any().item()
+        clean(gpu)
+    finally:
+        del x, codes
+        torch.cuda.empty_cache()
