@@ -884,17 +884,20 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     // Workgroups go to the chip's eight dies in turn (b to die b % 8, each with its own L2). Neighbouring workgroups share a tile's columns across
     // the dies, and a die's workgroups four of the rows' tiles and eight of the columns'. An expert with fewer tiles of rows than dies
     // would so have its rows on every die: there (`group`) a group of its tiles of columns stays on one die, all rows of it.
+    const u32 block = i8_group();
     u32 expert = 0, t0, row_tile, tile;
     if (group) {
-        const u32 i = blockIdx.x >> 3, per = group * n_row_tiles;
+        const u32 i = block >> 3, per = group * n_row_tiles;
         row_tile = i % per / group;
-        tile = (i / per * 8 + (blockIdx.x & 7)) * group + i % group;
+        tile = (i / per * 8 + (block & 7)) * group + i % group;
     } else {
-        row_tile = blockIdx.x % n_row_tiles;
-        tile = blockIdx.x / n_row_tiles;
+        row_tile = block % n_row_tiles;
+        tile = block / n_row_tiles;
     }
-    if (!a.start) t0 = tile * BT;
-    else if (!i8_find_tile<BT>(a, tile, tile == 0 && row_tile == 0, expert, t0)) return;
+    if (!a.start) {
+        t0 = tile * BT;
+        if (t0 >= a.m) return;
+    } else if (!i8_find_tile<BT>(a, tile, tile == 0 && row_tile == 0, expert, t0)) return;
     const u32 r0 = row_tile * BR;
     I8Run run;
     if (!i8_run(a, expert, run)) return;
@@ -1005,9 +1008,6 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     else i8_tile_out<kElemBF16, G>(a, run, part, t0 + wt, r0 + (wr - BT), acc);
 }
 
-// Whether a launch along one dimension has fewer threads than its limit, 2^32.
-static bool i8_launchable(uint64_t groups, u32 threads) { return groups * threads <= 0xffffffffu; }
-
 template <int BT, int BR, int WT, int WR, int S, bool WHOLE, int EU>
 static hipError_t tile_launch(const Launch &L, const I8Args &a, u32 entries) {
     const u32 row_tiles = (a.rows + BR - 1) / BR;
@@ -1015,8 +1015,7 @@ static hipError_t tile_launch(const Launch &L, const I8Args &a, u32 entries) {
     if (a.start) tiles = entries / BT + (a.n_experts < entries ? a.n_experts : entries); // at most a ragged tile an expert
     const u32 group = a.start && row_tiles < 8 ? 2 : 0;
     if (group) tiles = (tiles + 8 * group - 1) / (8 * group) * (8 * group);
-    if (!i8_launchable((uint64_t)tiles * row_tiles, 64 * WT * WR)) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((k_i8_tile<BT, BR, WT, WR, S, WHOLE, EU>), dim3(tiles * row_tiles), dim3(64 * WT * WR), 0, L.stream, a, row_tiles, group);
+    hipLaunchKernelGGL((k_i8_tile<BT, BR, WT, WR, S, WHOLE, EU>), i8_grid((uint64_t)tiles * row_tiles, 64 * WT * WR), dim3(64 * WT * WR), 0, L.stream, a, row_tiles, group);
     return hipGetLastError();
 }
 

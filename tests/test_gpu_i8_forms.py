@@ -332,3 +332,31 @@ def test_the_most_rows_of_the_longest_form(gpu):
     finally:
         del x, codes
         torch.cuda.empty_cache()
+
+
+def test_the_most_rows_an_expert(gpu):
+    """Experts of 2^22 rows each: more than 2^32 threads of tiles, counted by the most that the runs may make."""
+    needs_memory(70)
+    n, rows, k = 600, 1 << 22, 16
+    torch.manual_seed(6)
+    w, ws = torch.empty(n * rows, k, dtype=torch.int8, device="cuda"), torch.empty(n * rows, device="cuda")
+    for part, scales in zip(w.split(1 << 28), ws.split(1 << 28)):
+        part.random_(-127, 128)
+        scales.uniform_()
+    q, s = torch.randint(-127, 128, (n, k), dtype=torch.int8, device="cuda"), torch.rand(n, device="cuda")
+    # a slot an expert, but for one with none and its neighbour with two
+    start = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    start[8] = 7
+    y = torch.empty(n, rows, dtype=torch.bfloat16, device="cuda").fill_(float("nan"))
+    try:
+        torch.cuda.synchronize()
+        gpu.enqueue_i8_gemm_experts(PTR(w), PTR(ws), n, rows, k, PTR(q), PTR(s), None, PTR(start), n, 0, PTR(y), bm.BF16)
+        gpu.sync()
+        for e in range(n):
+            a, b = int(start[e]), int(start[e + 1])
+            sums = q[a:b].float() @ w[e * rows:(e + 1) * rows].float().t()  # exact: below 2^24
+            assert torch.equal(y[a:b], (sums * s[a:b, None] * ws[e * rows:(e + 1) * rows]).bfloat16()), e
+        clean(gpu)
+    finally:
+        del w, ws, y, part, scales
+        torch.cuda.empty_cache()
