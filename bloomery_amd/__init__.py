@@ -124,6 +124,7 @@ SYMBOLS = {
     "bm_weights_from_gguf": (_i, [_vp, _vp, C.c_char_p, C.POINTER(_vp), C.POINTER(_i), C.POINTER(_i)]),
     "bm_set_gemm_mode": (_i, [_vp, _i]),
     "bm_set_down_form": (_i, [_vp, _i]),
+    "bm_i8_gemm_form": (_i, [_i, _i, _i, _i, _i, _i]),
     "bm_block_sums": (_i, [_vp, _vp, _i64, _vp, _i, _vp]),
     "bm_capture_begin": (_i, [_vp]),
     "bm_capture_end": (_i, [_vp, C.POINTER(_vp)]),
@@ -175,6 +176,14 @@ def col_bytes(wtype, k):
 def i8_row_bytes(k):
     """Bytes of a row of 8-bit codes: k rounded up to 16."""
     return int(load_library().bm_i8_row_bytes(k))
+
+
+def i8_gemm_form(rows, k, n_cols, n_experts=0, n_slots=0, top_k=0):
+    """(columns, rows, waves, LDS buffers) of a workgroup of the form that enqueue_i8_gemm (n_experts 0) or enqueue_i8_gemm_experts takes."""
+    form = int(load_library().bm_i8_gemm_form(n_experts, rows, k, n_cols, n_slots, top_k))
+    if form < 0:
+        raise GpuError(form, f"bm_i8_gemm_form: {n_experts} experts of {rows} x {k}, {n_cols} columns, {n_slots} slots, top_k {top_k}")
+    return form & 1023, form >> 10 & 1023, form >> 20 & 15, form >> 24 & 15
 
 
 def expert_sort_work(n_slots, n_experts):

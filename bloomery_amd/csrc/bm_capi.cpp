@@ -77,7 +77,7 @@ static size_t dev_col_bytes(int wtype, int k) { return (size_t)bmk::act_col_byte
 
 extern "C" {
 
-int bm_version(void) { return 102; }
+int bm_version(void) { return 103; }
 
 int64_t bm_row_bytes(int wtype, int k) {
     if (!known_type(wtype)) return BM_ETYPE;
@@ -1573,9 +1573,13 @@ int bm_i8_swiglu_quantize(bm_ctx *ctx, const void *g_dev, const void *u_dev, int
     return i8_quant(ctx, "bm_i8_swiglu_quantize", g_dev, u_dev, true, elem_type, ld, m, k, rule, live_dev, codes_dev, scales_dev);
 }
 
-static int check_i8_weights(bm_ctx *ctx, const char *what, const int8_t *w_dev, const float *w_scales_dev, int rows, int k) {
+static int check_i8_matrix(bm_ctx *ctx, const char *what, int rows, int k) {
     if (rows < 1 || rows > kI8MaxRows) return fail(ctx, BM_ESHAPE, "%s: rows = %d of a matrix (1 .. %d)", what, rows, kI8MaxRows);
     if (k < 1 || k > bmk::kI8MaxK) return fail(ctx, BM_ESHAPE, "%s: rows of k = %d values (1 .. %d)", what, k, bmk::kI8MaxK);
+    return BM_OK;
+}
+static int check_i8_weights(bm_ctx *ctx, const char *what, const int8_t *w_dev, const float *w_scales_dev, int rows, int k) {
+    BM_TRY(check_i8_matrix(ctx, what, rows, k));
     return check_codes(ctx, what, "w_dev", w_dev, "w_scales_dev", w_scales_dev);
 }
 
@@ -1609,16 +1613,21 @@ int bm_i8_gemm_x(bm_ctx *ctx, const int8_t *w_dev, const float *w_scales_dev, in
                                             y_type, ld_y));
 }
 
-int bm_i8_gemm_experts(bm_ctx *ctx, const int8_t *w_dev, const float *w_scales_dev, int n_experts, int rows_per_expert, int k,
-                       const int8_t *codes_dev, const float *scales_dev, int n_cols, const uint32_t *order_dev, const uint32_t *start_dev,
-                       int n_slots, int top_k, void *y_dev, int y_type, int64_t ld_y) {
-    const char *what = "bm_i8_gemm_experts";
-    BM_TRY(check_i8_weights(ctx, what, w_dev, w_scales_dev, rows_per_expert, k));
+static int check_i8_runs(bm_ctx *ctx, const char *what, int n_experts, int n_cols, int n_slots, int top_k) {
     if (n_experts < 1 || n_experts > bmk::kBucketExperts) return fail(ctx, BM_ESHAPE, "%s: %d experts (1 .. %d)", what, n_experts, bmk::kBucketExperts);
     if (n_slots < 1 || n_slots > bmk::kTileMaxSlots) return fail(ctx, BM_ESHAPE, "%s: %d slots (1 .. %d)", what, n_slots, bmk::kTileMaxSlots);
     if (n_cols < 1 || n_cols > kI8MaxRows) return fail(ctx, BM_ESHAPE, "%s: %d columns (1 .. %d)", what, n_cols, kI8MaxRows);
     if (top_k < 0) return fail(ctx, BM_ESHAPE, "%s: top_k = %d", what, top_k);
     if (top_k == 0 && n_cols < n_slots) return fail(ctx, BM_ESHAPE, "%s: a column a slot, and %d columns for %d slots", what, n_cols, n_slots);
+    return BM_OK;
+}
+
+int bm_i8_gemm_experts(bm_ctx *ctx, const int8_t *w_dev, const float *w_scales_dev, int n_experts, int rows_per_expert, int k,
+                       const int8_t *codes_dev, const float *scales_dev, int n_cols, const uint32_t *order_dev, const uint32_t *start_dev,
+                       int n_slots, int top_k, void *y_dev, int y_type, int64_t ld_y) {
+    const char *what = "bm_i8_gemm_experts";
+    BM_TRY(check_i8_weights(ctx, what, w_dev, w_scales_dev, rows_per_expert, k));
+    BM_TRY(check_i8_runs(ctx, what, n_experts, n_cols, n_slots, top_k));
     BM_TRY(check_codes(ctx, what, "codes_dev", codes_dev, "scales_dev", scales_dev));
     if (top_k > 0) BM_TRY(check_words(ctx, what, "order_dev", order_dev));
     BM_TRY(check_words(ctx, what, "start_dev", start_dev));
@@ -1628,6 +1637,14 @@ int bm_i8_gemm_experts(bm_ctx *ctx, const int8_t *w_dev, const float *w_scales_d
     DeviceScope on(ctx->device);
     return driver(ctx, what, bmk::i8_gemm(launch_of(ctx), w_dev, w_scales_dev, n_experts, rows_per_expert, k, codes_dev, scales_dev, n_cols,
                                           top_k > 0 ? order_dev : nullptr, start_dev, n_slots, top_k, y_dev, y_type, ld_y));
+}
+
+int bm_i8_gemm_form(int n_experts, int rows, int k, int n_cols, int n_slots, int top_k) {
+    const char *what = "bm_i8_gemm_form";
+    BM_TRY(check_i8_matrix(nullptr, what, rows, k));
+    if (n_experts == 0) BM_TRY(check_i8(nullptr, what, n_cols, k));
+    else BM_TRY(check_i8_runs(nullptr, what, n_experts, n_cols, n_slots, top_k));
+    return bmk::i8_gemm_form(n_experts, rows, k, n_cols, n_slots, top_k);
 }
 
 // ------------------------------------------------------------------------------------ graphs and events

@@ -1059,6 +1059,23 @@ hipError_t i8_gemm_x(const Launch &L, const int8_t *w, const float *ws, int rows
     return e != hipSuccess ? e : i8_gemm(L, w, ws, 1, rows, k, codes, scales, m, nullptr, nullptr, 0, 0, y, et, ld);
 }
 
+// The forms, by what a workgroup has: columns x rows, its waves and its LDS buffers.
+enum I8Form : u32 {
+    kFew16x16,      // k_i8_few: 16 x 16, waves sharing k
+    kFew16x32,      // 16 x 32
+    kFew16x32Three, // the same by three waves
+    kFew32x32,
+    kTile32x64Ring4, // k_i8_tile, steps in a ring of four or two
+    kTile32x64,
+    kTile64x64Ring4,
+    kTile64x64,
+    kTile64x128,
+    kTile64x256,
+    kTile128x128,
+    kTile256x224,
+    kTile256x256,
+};
+
 // Which form: all give the same bits. us on MI355X, bf16 out, weights of three sets in turn, the chosen form's first.
 //   One matrix. Large tiles are the better the more of them there are, and whole rounds of 256 compute units count: a round of 256 x 256 tiles takes
 //   64 units of time, of 256 x 224 57, of two 128 x 128 a unit 39. (4096 x 7168 x 7168: 512 tiles of 224 rows are two rounds, 179, 448 of 256 take
@@ -1083,44 +1100,72 @@ hipError_t i8_gemm_x(const Launch &L, const int8_t *w, const float *ws, int rows
 //   A die's group of two tiles of columns (k_i8_tile) in these: 128 slots, 768 x 2048 72, without 88 (its weights are then fetched 1.8 times: 369 MB at 5.5 TB/s); 256 slots 102, without
 //   117. Where a run's rows are eight tiles or more it loses (64 experts, 7168 x 2048 190.8 without, 201 with); dies with whole ranges of the experts lose there too (202) and gain
 //   little here (69).
+// n_experts 0: one matrix, n its columns; else n slots. reach: the tiles' offsets of gathered columns, 32 bits, hold the columns.
+static I8Form i8_form(u32 n_experts, u32 rows, u32 kp, u32 n, bool reach) {
+    const auto up = [](u32 x, u32 y) { return (x + y - 1) / y; };
+    const auto tiles = [&](u32 bt, u32 br) { return (uint64_t)up(n, bt) * up(rows, br); };
+    if (n_experts) {
+        if (n <= 32 || !reach) return kFew16x32Three;
+        const u32 each = n / n_experts, runs = n < n_experts ? n : n_experts;
+        // 64 x 64 tiles: every run has one, and half a one more than its slots fill
+        const uint64_t small = (uint64_t)std::max(runs, n / 64 + runs / 2) * up(rows, 64);
+        if (each <= 16 && small <= 64) return kFew32x32;
+        if (each < 24 && small <= 600) return kTile32x64Ring4;
+        if (each >= 24 && small <= 256) return kTile64x64Ring4;
+        if (each >= 24 && small <= 1024) return kTile64x64;
+        if (each >= 352) return kTile256x256;
+        if (each >= 144) return kTile128x128;
+        // 64 x 256 where its tiles (half a tile more an expert) are one round of two a compute unit, or the runs long
+        if (each >= 96 || (each >= 12 && (uint64_t)(n / 64 + n_experts / 2) * up(rows, 256) <= 512)) return kTile64x256;
+        return each >= 12 ? kTile64x128 : kTile32x64;
+    }
+    if (tiles(16, 16) <= 256) return kFew16x16;
+    if (tiles(16, 32) <= 256) return kFew16x32;
+    if (n <= 16) return kFew16x32Three;
+    if (n <= 32 || tiles(32, 32) <= 256) return kFew32x32;
+    if (tiles(32, 64) <= 256) return kTile32x64Ring4;
+    if (tiles(64, 64) <= 512 && kp > 1024) return kTile64x64Ring4;
+    if (tiles(64, 64) <= 768) return kTile64x64;
+    if (tiles(256, 256) >= 96) {
+        const uint64_t by256 = 64 * ((tiles(256, 256) + 255) / 256), by224 = 57 * ((tiles(256, 224) + 255) / 256), by128 = 39 * ((tiles(128, 128) + 511) / 512);
+        if (by256 <= by224 && by256 <= by128) return kTile256x256;
+        return by224 <= by128 ? kTile256x224 : kTile128x128;
+    }
+    return tiles(64, 128) <= 640 ? kTile64x128 : kTile128x128;
+}
+static bool i8_reach(bool gathered, int n_cols, u32 kp) { return !gathered || (uint64_t)n_cols * kp <= 0xffffffffu; }
+
+int i8_gemm_form(int n_experts, int rows, int k, int n_cols, int n_slots, int top_k) {
+    static const struct {
+        u32 columns, rows, waves, buffers;
+    } of[] = {{16, 16, 8, 4}, {16, 32, 4, 4}, {16, 32, 3, 4}, {32, 32, 4, 4}, {32, 64, 2, 4}, {32, 64, 2, 2}, {64, 64, 4, 4},
+              {64, 64, 4, 2}, {64, 128, 4, 2}, {64, 256, 4, 2}, {128, 128, 4, 2}, {256, 224, 8, 2}, {256, 256, 8, 2}};
+    const u32 kp = (u32)i8_row_bytes(k);
+    const auto &f = of[i8_form((u32)n_experts, (u32)rows, kp, (u32)(n_experts ? n_slots : n_cols), i8_reach(n_experts && top_k > 0, n_cols, kp))];
+    return (int)(f.columns | f.rows << 10 | f.waves << 20 | f.buffers << 24);
+}
+
 hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_experts, int rows, int k, const int8_t *q, const float *qs, int n_cols,
                    const uint32_t *order, const uint32_t *start, int n_slots, int top_k, void *y, int et, int64_t ld) {
     const I8Args a = {w, ws, (u32)rows, (u32)i8_row_bytes(k), q, qs, (u32)n_cols, order, start, (u32)n_slots, (u32)top_k, (u32)n_cols, (u32)n_experts,
                       y, (size_t)ld, et, L.fault, L.layer};
     const u32 n = start ? (u32)n_slots : (u32)n_cols;
-    const auto up = [](u32 x, u32 y) { return (x + y - 1) / y; };
-    const auto tiles = [&](u32 bt, u32 br) { return (uint64_t)up(n, bt) * up(a.rows, br); };
-    // the tiles' offsets of gathered columns are 32 bits
-    const bool reach = !order || (uint64_t)n_cols * a.kp <= 0xffffffffu;
-    if (start) {
-        if (n <= 32 || !reach) return few_launch<2, 1, 3>(L, a, n);
-        const u32 each = n / (u32)n_experts, runs = n < (u32)n_experts ? n : (u32)n_experts;
-        // 64 x 64 tiles: every run has one, and half a one more than its slots fill
-        const uint64_t small = (uint64_t)std::max(runs, n / 64 + runs / 2) * up(a.rows, 64);
-        if (each <= 16 && small <= 64) return few_launch<2, 2, 4>(L, a, n);
-        if (each < 24 && small <= 600) return tile_launch<32, 64, 1, 2, 4, true, 2>(L, a, n);
-        if (each >= 24 && small <= 256) return tile_launch<64, 64, 2, 2, 4, true, 2>(L, a, n);
-        if (each >= 24 && small <= 1024) return tile_launch<64, 64, 2, 2, 2, true, 2>(L, a, n);
-        if (each >= 352) return tile_launch<256, 256, 4, 2, 2, false, 2>(L, a, n);
-        if (each >= 144) return tile_launch<128, 128, 2, 2, 2, true, 2>(L, a, n);
-        // 64 x 256 where its tiles (half a tile more an expert) are one round of two a compute unit, or the runs long
-        if (each >= 96 || (each >= 12 && (uint64_t)(n / 64 + (u32)n_experts / 2) * up(a.rows, 256) <= 512)) return tile_launch<64, 256, 1, 4, 2, true, 2>(L, a, n);
-        if (each >= 12) return tile_launch<64, 128, 1, 4, 2, true, 2>(L, a, n);
-        return tile_launch<32, 64, 1, 2, 2, true, 2>(L, a, n);
+    switch (i8_form(start ? a.n_experts : 0, a.rows, a.kp, n, i8_reach(order != nullptr, n_cols, a.kp))) {
+    case kFew16x16: return few_launch<1, 1, 8>(L, a, n);
+    case kFew16x32: return few_launch<2, 1, 4>(L, a, n);
+    case kFew16x32Three: return few_launch<2, 1, 3>(L, a, n);
+    case kFew32x32: return few_launch<2, 2, 4>(L, a, n);
+    case kTile32x64Ring4: return tile_launch<32, 64, 1, 2, 4, true, 2>(L, a, n);
+    case kTile32x64: return tile_launch<32, 64, 1, 2, 2, true, 2>(L, a, n);
+    case kTile64x64Ring4: return tile_launch<64, 64, 2, 2, 4, true, 2>(L, a, n);
+    case kTile64x64: return tile_launch<64, 64, 2, 2, 2, true, 2>(L, a, n);
+    case kTile64x128: return tile_launch<64, 128, 1, 4, 2, true, 2>(L, a, n);
+    case kTile64x256: return tile_launch<64, 256, 1, 4, 2, true, 2>(L, a, n);
+    case kTile128x128: return tile_launch<128, 128, 2, 2, 2, true, 2>(L, a, n);
+    case kTile256x224: return tile_launch<256, 224, 4, 2, 2, false, 2>(L, a, n);
+    case kTile256x256: return tile_launch<256, 256, 4, 2, 2, false, 2>(L, a, n);
     }
-    if (tiles(16, 16) <= 256) return few_launch<1, 1, 8>(L, a, n);
-    if (tiles(16, 32) <= 256) return few_launch<2, 1, 4>(L, a, n);
-    if (n <= 16) return few_launch<2, 1, 3>(L, a, n);
-    if (n <= 32 || tiles(32, 32) <= 256) return few_launch<2, 2, 4>(L, a, n);
-    if (tiles(32, 64) <= 256) return tile_launch<32, 64, 1, 2, 4, true, 2>(L, a, n);
-    if (tiles(64, 64) <= 512 && a.kp > 1024) return tile_launch<64, 64, 2, 2, 4, true, 2>(L, a, n);
-    if (tiles(64, 64) <= 768) return tile_launch<64, 64, 2, 2, 2, true, 2>(L, a, n);
-    if (tiles(256, 256) >= 96) {
-        const uint64_t by256 = 64 * ((tiles(256, 256) + 255) / 256), by224 = 57 * ((tiles(256, 224) + 255) / 256), by128 = 39 * ((tiles(128, 128) + 511) / 512);
-        if (by256 <= by224 && by256 <= by128) return tile_launch<256, 256, 4, 2, 2, false, 2>(L, a, n);
-        return by224 <= by128 ? tile_launch<256, 224, 4, 2, 2, false, 2>(L, a, n) : tile_launch<128, 128, 2, 2, 2, true, 2>(L, a, n);
-    }
-    return tiles(64, 128) <= 640 ? tile_launch<64, 128, 1, 4, 2, true, 2>(L, a, n) : tile_launch<128, 128, 2, 2, 2, true, 2>(L, a, n);
+    return hipErrorInvalidValue;
 }
 
 } // namespace bmk

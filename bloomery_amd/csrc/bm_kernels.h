@@ -223,6 +223,8 @@ hipError_t i8_quantize(const Launch &L, const void *x, const void *u, int et, in
 // start NULL: one matrix against n_cols columns. Else entry j of expert e's run reads column order[j] / top_k, or j where top_k is 0.
 hipError_t i8_gemm(const Launch &L, const int8_t *w, const float *ws, int n_experts, int rows, int k, const int8_t *q, const float *qs, int n_cols,
                    const uint32_t *order, const uint32_t *start, int n_slots, int top_k, void *y, int et, int64_t ld);
+// The form that i8_gemm takes (bm_i8_gemm_form's word). n_experts 0: one matrix against n_cols columns.
+int i8_gemm_form(int n_experts, int rows, int k, int n_cols, int n_slots, int top_k);
 // i8_quantize and i8_gemm of one matrix; a few rows in one launch.
 hipError_t i8_gemm_x(const Launch &L, const int8_t *w, const float *ws, int rows, int k, const void *x, int x_et, int64_t ld_x, int m, int8_t *codes,
                      float *scales, void *y, int et, int64_t ld);

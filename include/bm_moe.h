@@ -604,6 +604,11 @@ int bm_weights_from_gguf(bm_ctx *ctx, const bm_gguf *g, const char *name, bm_wei
  * bit identity, crates/qdot/tests/qdot.rs:738,818,2664). */
 int bm_block_sums(bm_ctx *ctx, const bm_weights *w, int64_t row, const bm_act *act, int col, int32_t *out_dev);
 
+/* Which of its forms bm_i8_gemm (n_experts 0: n_cols columns of one matrix; the last two numbers are not looked at) or
+ * bm_i8_gemm_experts takes for these sizes, so that a test knows which kernel a size runs: the columns and rows of a workgroup in bits 0..9
+ * and 10..19, its waves in 20..23, its LDS buffers in 24..27. All forms give the same bits. BM_ESHAPE for numbers that the entry refuses. */
+int bm_i8_gemm_form(int n_experts, int rows, int k, int n_cols, int n_slots, int top_k);
+
 /* ------------------------------------------------------------------------------------ graphs and events */
 
 typedef struct bm_graph bm_graph; /* an instantiated HIP graph of launches captured on the context's stream */
