@@ -7,7 +7,7 @@ import torch
 
 import bloomery_amd as bm
 from common import normal_f32
-from rows_common import NAMES, NUMPY, TORCH, bits, codes_of, padded, rounded, tables
+from rows_common import NAMES, NUMPY, TORCH, bits, codes_of, lines, padded, rounded, tables
 from test_gpu_i8 import Held, clean, gpu, held, junk_padded, picks, quantize, some_matrix  # noqa: F401 (fixtures)
 
 pytestmark = pytest.mark.gpu
@@ -360,3 +360,25 @@ def test_the_most_rows_an_expert(gpu):
     finally:
         del w, ws, y, part, scales
         torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", (bm.F32, bm.F16, bm.BF16), ids=NAMES.get)
+@pytest.mark.parametrize("m,k", ((2100, 5), (300, 500), (301, 770), (30, 2050), (2100, 2050), (100, 1500), (2061, 4096), (2100, 4099), (40, 8191), (2060, 8192), (9, 8193), (5, 40000)))
+def test_the_gate_rules_values_of_every_row(gpu, held, dtype, m, k):
+    """Codes and scales of every row against silu(g) u in 64 bits, in every form: the exponential, the divide and the products are off by 64 x 2^-24
+    at most, a scale by that and its own rounding, a code by half a step and twice that of at most 127."""
+    rng = np.random.default_rng(3 * m + k)
+    scale = np.exp(normal_f32(rng, (m, 1)))  # rows that no other row's scale fits
+    g, u = rounded(normal_f32(rng, (m, k)), dtype), rounded(normal_f32(rng, (m, k)) * scale, dtype)
+    kp, ld = bm.i8_row_bytes(k), k + 1
+    codes, scales = held.out(np.int8, (m + 1) * kp, 0x55), held.out(np.float32, m + 1)
+    gpu.enqueue_i8_swiglu_quantize(held.up(lines(g, dtype, ld, np.nan)), held.up(lines(u, dtype, ld, np.nan)), dtype, m, k, codes, scales, ld=ld)
+    h = g / (1 + np.exp(-g)) * u
+    step = np.abs(h).max(axis=1) / 127
+    got, s = codes.download().reshape(m + 1, kp), scales.download()
+    tol = 64 * 2.0 ** -24
+    assert np.allclose(s[:m], step, rtol=tol + 2.0 ** -23, atol=0)
+    assert (np.abs(got[:m, :k] - h / step[:, None]) <= 0.5 + 127 * (2 * tol + 2.0 ** -22)).all()
+    assert (np.abs(got[:m].astype(int)).max(axis=1) == 127).all() and not got[:m, k:].any()
+    assert (got[m] == 0x55).all() and s[m:].view(np.uint32)[0] == 0xEEEEEEEE
+    clean(gpu)
