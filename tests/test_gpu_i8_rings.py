@@ -85,3 +85,35 @@ def test_experts(gpu, form, size, own, k):
             assert torch.equal(y[a:b], value(q[col[a:b]], s[col[a:b]], w[of], ws[of]).to(TORCH[dtype])), f"expert {e}"
     assert (y[listed:] == 7.0).all()
     clean(gpu)
+
+
+# (form, experts, rows): a table of 32767 slots
+FAR = (((64, 64, 4, 2), 1, 40), ((256, 256, 8, 2), 1, 200), ((128, 128, 4, 2), 128, 100), ((64, 256, 4, 2), 300, 70), ((64, 128, 4, 2), 1000, 70))
+
+
+def test_gathered_columns_far_into_the_tiles_reach(gpu):
+    """Columns of 4.3 GB, the most that 32-bit offsets hold, behind an order, in every form of tiles that such a table takes."""
+    k, cols = 131072, 32767
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(11)
+    q, s = torch.randint(-127, 128, (cols, k), dtype=torch.int8, device="cuda", generator=gen), torch.rand(cols, device="cuda", generator=gen)
+    listed = torch.tensor([cols - 1, 0, 16383, 16384, 16385, 20000, cols - 2] + list(range(cols - 60, cols - 20)), device="cuda")
+    table = torch.full((cols,), 0x12345678, dtype=torch.int32, device="cuda")
+    table[:listed.numel()] = listed.int()
+    for form, n, rows in FAR:
+        assert bm.i8_gemm_form(rows, k, cols, n, cols, 1) == form
+        w, ws = torch.randint(-128, 128, (n * rows, k), dtype=torch.int8, device="cuda", generator=gen), torch.rand(n * rows, device="cuda", generator=gen)
+        start = torch.full((n + 1,), 4, dtype=torch.int32, device="cuda")  # the first and the last expert's runs
+        start[0], start[n] = 0, listed.numel()
+        y = torch.full((cols, rows), 7.0, device="cuda")
+        torch.cuda.synchronize()
+        gpu.enqueue_i8_gemm_experts(PTR(w), PTR(ws), n, rows, k, PTR(q), PTR(s), PTR(table), PTR(start), cols, 1, PTR(y), bm.F32)
+        gpu.sync()
+        for e in {0, n - 1}:
+            at = torch.arange(int(start[e]), int(start[e + 1]), device="cuda")
+            of = slice(e * rows, (e + 1) * rows)
+            assert torch.equal(y[at], value(q[listed[at]], s[listed[at]], w[of], ws[of])), form
+        assert (y[listed.numel():] == 7.0).all()
+        del w
+    clean(gpu)
+    torch.cuda.empty_cache()
