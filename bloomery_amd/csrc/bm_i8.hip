@@ -229,7 +229,8 @@ static void quant_start(const Launch &L, const QuantArgs &a) {
 // us on MI355X, bf16, alone and behind the gate rule. While the rows are not eight a compute unit a row's length is dealt to more threads, a piece each: 24 x
 // 7168 4.0 and 4.2 (256 threads of four pieces: 5.5, 6.3), 1500 x 7168 10.2 and 15.2 (10.8, 16.7), 1024 x 4096 4.9 and 6.8 (5.4, 7.6); behind that more pieces a thread
 // ask for more at once: 4096 x 7168 18.2 and 32.6 (1024 threads: 22.0, 34.7); 18.2 us are 4.8 TB/s, what a copy reaches. Short rows take a wave each, 16384 x 768 11.5
-// and 19.0 (a workgroup: 16.2, 30.6).
+// and 19.0 (a workgroup: 16.2, 30.6). Rows past 8192 values are read twice, a piece in flight a thread, the rule's values formed twice: 4096 x 18432 56.4 and 151 (4.0 and 2.5
+// TB/s), 256 x 18432 6.7 and 12.6, one row 5.2 and 10.6.
 template <int ET, bool GLU>
 static void quant_launch(const Launch &L, const QuantArgs &a) {
     const bool few = a.m <= 2048;
@@ -601,9 +602,12 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
 // Many columns a matrix: BT columns x BR rows a workgroup, 128 bytes of k a step through a ring of S LDS buffers, where the loads put them
 // themselves (16 bytes a lane, no register in between): while the waves multiply one step the next S - 1 are on their way, one barrier a step. A
 // wave holds (BT / WT) x (BR / WR) sums in v_mfma_i32_16x16x64_i8's form.
-// Large products are bound by the matrix cores and the clock that power leaves them: 4096 x 7168 x 7168 in 176 to 187 us, 2.2 to 2.4 POP/s, matrix cores busy 61 %
+// Large products are bound by the matrix cores and the clock that power leaves them: 4096 x 7168 x 7168 in 168 to 177 us, 2.4 to 2.5 POP/s, matrix cores busy 61 %
 // of the cycles, LDS 27 %, no bank conflicts (a bare loop of these instructions on such data reaches 3.3 POP/s; the library's product of the same size takes 180 us).
-// Small ones by the latency of a step's loads (777 x 2000 x 1996: matrix cores 12 %), experts' by their weights from memory.
+// From rest the clock falls behind the first launches and comes back: of 200 in a row the first six take 173 to 180 us, the seventh to the sixtieth 185 to 225, the last
+// hundred 167 to 177. Its form, 256 x 224, keeps one register of 256 in scratch memory, stored in front of the loop and fetched behind it.
+// Small ones are bound by the latency of a step's loads (777 x 2000 x 1996: matrix cores 12 %), or by the way from L2 to LDS, which a smaller tile takes more often: 1024 x
+// 2048 x 7168 in 64 x 64 moves 512 tiles x 56 steps x 16 KB = 470 MB in 25.2 us, 18.7 TB/s. Experts' are bound by their weights from memory.
 template <int BT, int BR, int WT, int WR, int S, bool WHOLE>
 struct I8Tile {
     static constexpr bool kWhole = WHOLE;
@@ -1100,6 +1104,9 @@ enum I8Form : u32 {
 //   A die's group of two tiles of columns (k_i8_tile) in these: 128 slots, 768 x 2048 72, without 88 (its weights are then fetched 1.8 times: 369 MB at 5.5 TB/s); 256 slots 102, without
 //   117. Where a run's rows are eight tiles or more it loses (64 experts, 7168 x 2048 190.8 without, 201 with); dies with whole ranges of the experts lose there too (202) and gain
 //   little here (69).
+//   Experts' gathered columns past 4 GiB, which the tiles' 32-bit offsets do not reach, go by waves sharing k however many there are: 599187 tokens of 7168, top 4 of 256, 2048
+//   rows 409 ms, one token fewer, in 256 x 256, 33 to 38. One token's experts launch every expert's tiles, most with nothing to do: top 8 of 256, 2048 x 7168 31 with the
+//   quantizer, 7168 x 2048 45 (57344 workgroups, 1792 of them with work), of 128, 768 x 2048 9.9.
 // n_experts 0: one matrix, n its columns; else n slots. reach: the tiles' offsets of gathered columns, 32 bits, hold the columns.
 static I8Form i8_form(u32 n_experts, u32 rows, u32 kp, u32 n, bool reach) {
     const auto up = [](u32 x, u32 y) { return (x + y - 1) / y; };
