@@ -8,22 +8,11 @@
 //
 // A row of codes is k rounded up to 16 bytes, zeros behind the last value. The integer sum is exact for k up to 131072 (127 * 128 a product),
 // so every split of k gives the same bits.
-#include "bm_elem.hpp"
+#include "bm_lines.hpp"
 
 #include <algorithm>
 
 namespace bmk {
-
-typedef int v4i __attribute__((ext_vector_type(4)));
-
-// A dimension of a launch has fewer than 2^32 threads. Workgroups that would be more go along a second one, 2^20 a step; i8_group numbers them through
-// (the last step may be ragged: what it has too many finds nothing to do).
-constexpr u32 kGroupsLog = 20;
-static dim3 i8_grid(uint64_t groups, u32 threads) {
-    if (groups * threads <= 0xffffffffu) return dim3((u32)groups);
-    return dim3(1u << kGroupsLog, (u32)((groups + (1u << kGroupsLog) - 1) >> kGroupsLog));
-}
-__device__ __forceinline__ u32 i8_group() { return blockIdx.y << kGroupsLog | blockIdx.x; }
 
 // ------------------------------------------------------------------------------------------------ quantizer
 
@@ -171,7 +160,7 @@ template <int ET, bool GLU, int T, int CH>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void k_i8_quantize(QuantArgs a) {
     constexpr int kThreads = T < 256 ? 256 : T;
     __shared__ u32 top[T / 64];
-    const u32 lane = threadIdx.x % T, row = i8_group() * (kThreads / T) + threadIdx.x / T;
+    const u32 lane = threadIdx.x % T, row = group_index() * (kThreads / T) + threadIdx.x / T;
     const u32 m = a.live ? min(a.m, *a.live) : a.m;
     if (row >= m) return; // whole waves (T = 64) or the workgroup
     float v[CH ? CH : 1][8];
@@ -224,7 +213,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_i8_quantize(QuantArgs a) 
 template <int ET, bool GLU, int T, int CH>
 static void quant_start(const Launch &L, const QuantArgs &a) {
     constexpr u32 threads = T < 256 ? 256 : T, rows = threads / T;
-    hipLaunchKernelGGL((k_i8_quantize<ET, GLU, T, CH>), i8_grid((a.m + rows - 1) / rows, threads), dim3(threads), 0, L.stream, a);
+    hipLaunchKernelGGL((k_i8_quantize<ET, GLU, T, CH>), group_grid((a.m + rows - 1) / rows, threads), dim3(threads), 0, L.stream, a);
 }
 // us on MI355X, bf16, alone and behind the gate rule. While the rows are not eight a compute unit a row's length is dealt to more threads, a piece each: 24 x
 // 7168 4.0 and 4.2 (256 threads of four pieces: 5.5, 6.3), 1500 x 7168 10.2 and 15.2 (10.8, 16.7), 1024 x 4096 4.9 and 6.8 (5.4, 7.6); behind that more pieces a thread
@@ -294,93 +283,12 @@ __device__ __forceinline__ bool i8_run(const I8Args &a, u32 e, I8Run &r) {
     r = I8Run{j0, j1, a.w + (size_t)e * a.rows * a.kp, a.ws + (size_t)e * a.rows};
     return j1 > j0;
 }
-// Entry j's column; one that names no column raises ExpertId and gets column 0 with a NaN scale.
-__device__ __forceinline__ u32 i8_column(const I8Args &a, u32 j, bool &bad) {
-    bad = false;
-    if (!a.order) return j;
-    const u32 s = a.order[j], c = a.top_k ? s / a.top_k : j;
-    if (s < a.n_slots && c < a.n_cols) return c;
-    bad = true;
-    return 0;
-}
-
-// The columns of N entries, their slots asked for at once.
-template <int N>
-__device__ __forceinline__ void i8_columns(const I8Args &a, u32 (&j)[N]) {
-    u32 s[N];
-#pragma unroll
-    for (int i = 0; i < N; i++) s[i] = a.order[j[i]];
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const u32 c = a.top_k ? s[i] / a.top_k : j[i];
-        j[i] = s[i] < a.n_slots && c < a.n_cols ? c : 0u;
-    }
-}
-
-// Four neighbouring values of an output row from r on, those below `rows`.
-__device__ __forceinline__ void i8_store4(const I8Args &a, u32 j, u32 r, const float (&v)[4]) {
-    const size_t at = (size_t)j * a.ld + r;
-    const u32 have = a.rows - r;
-    if (a.et == kElemF32) elem_store_some<kElemF32, 4>(a.y, at, have, v);
-    else if (a.et == kElemF16) elem_store_some<kElemF16, 4>(a.y, at, have, v);
-    else elem_store_some<kElemBF16, 4>(a.y, at, have, v);
-}
-
-// ---- lines through LDS. 128-byte lines of k, eight 16-byte pieces each, come from memory straight into LDS (16 bytes a lane, no register in between),
-// eight lanes a line: asked for in the matrix instructions' own form, sixteen rows side by side in neighbouring lanes, a line would take the
-// vector cache four times as long. Piece c of line r lies at place c ^ swizzle(r), which the lane that asks for it arranges, so that the
-// pieces that the matrix instructions take of 16 lines at once come from all the banks.
-typedef __attribute__((address_space(1))) void i8_gptr;
-typedef __attribute__((address_space(3))) void i8_lptr;
-
-__device__ __forceinline__ u32 i8_swizzle(u32 line) { return (line >> 1) & 7; }
-
-// N groups of eight lines of a wave's own, a stage of its ring. Line l of rows that end before the piece does is read at its first
-// piece, which is there; whoever multiplies puts zeros in the columns' place.
-template <int N>
-struct I8Lines {
-    static constexpr int kStage = N * 1024;
-    const int8_t *from[N]; // this lane's row of each group
-    u32 piece[2];          // and its piece, of even and odd groups
-    __device__ __forceinline__ void begin(u32 lane) {
-#pragma unroll
-        for (u32 g = 0; g < 2; g++) piece[g] = 16 * ((lane & 7) ^ i8_swizzle(8 * g + (lane >> 3)));
-    }
-    __device__ __forceinline__ void ask(uint8_t *stage, u32 line, u32 kp) const {
-        u32 at[2];
-#pragma unroll
-        for (int g = 0; g < 2; g++) at[g] = 128 * line + (128 * line + piece[g] < kp ? piece[g] : 0u);
-#pragma unroll
-        for (int g = 0; g < N; g++) __builtin_amdgcn_global_load_lds((i8_gptr *)(from[g] + at[g & 1]), (i8_lptr *)(stage + g * 1024), 16, 0, 0);
-    }
-};
-// What the matrix instructions take of line group t (sixteen lines) of a stage: half c of the lines.
-__device__ __forceinline__ v4i i8_of_line(const uint8_t *stage, u32 lane, int t, int c) {
-    return *reinterpret_cast<const v4i *>(stage + t * 2048 + (lane & 15) * 128 + 16 * ((4 * c + (lane >> 4)) ^ i8_swizzle(lane & 15)));
-}
-// All but the last n of a wave's loads have landed, and its reads are done.
-template <int n>
-__device__ __forceinline__ void i8_landed() {
-    static_assert(n < 64, "vmcnt");
-    __asm__ volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070 | (n & 15) | (n >> 4) << 14); // vmcnt(n) lgkmcnt(0)
-    __asm__ volatile("" ::: "memory");
-}
-
-// The workgroup's writes to LDS are there for all of it; loads on their way into LDS are not waited for.
-__device__ __forceinline__ void i8_meet() {
-    __asm__ volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xc07f); // lgkmcnt(0)
-    __builtin_amdgcn_s_barrier();
-    __asm__ volatile("" ::: "memory");
-}
-
 // Few columns a matrix, bound by the launch and by a line's way from memory (24 x 7168 x 2048: 14.7 MB of weights in 5.1 us, 2.9 TB/s; 7168 x 7168 and one column: 51 MB
 // in 9.6, 5.3 TB/s): 16 R rows a workgroup against 16 C columns, its NW waves dealing the row's lines among them, each through a ring of four
 // stages of its own, two on their way while one is multiplied and the fourth is asked for. The waves' sums meet in LDS as integers.
 template <int R, int C, int NW>
 __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
-    typedef I8Lines<2 * (R + C)> L;
+    typedef Lines<2 * (R + C)> L;
     __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[NW * L::kStage], ring3[NW * L::kStage];
     static_assert(R * C * 1024 <= L::kStage && R * C <= NW, "a wave's sums lie in its stage, one piece a thread");
     const u32 lane = threadIdx.x & 63, tid = threadIdx.x, wave = (u32)__builtin_amdgcn_readfirstlane(tid >> 6);
@@ -395,7 +303,7 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
         u32 col[2 * C];
 #pragma unroll
         for (u32 g = 0; g < 2 * C; g++) col[g] = min(t0 + 8 * g + (lane >> 3), run.j1 - 1);
-        if (a.order) i8_columns<2 * C>(a, col);
+        if (a.order) run_columns(a, col);
 #pragma unroll
         for (u32 g = 0; g < 2 * C; g++) src.from[2 * R + g] = a.q + (size_t)col[g] * a.kp;
         if (wave < lines) src.ask(ring0 + mine, wave, a.kp);
@@ -408,16 +316,16 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
             for (int c = 0; c < C; c++) acc[r][c] = v4i{0, 0, 0, 0};
         const auto step = [&](const uint8_t *stage, uint8_t *free, u32 l) {
             constexpr int n = 2 * (R + C);
-            if (l + 2 * NW < lines) i8_landed<2 * n>();
-            else if (l + NW < lines) i8_landed<n>();
-            else i8_landed<0>();
+            if (l + 2 * NW < lines) loads_landed<2 * n>();
+            else if (l + NW < lines) loads_landed<n>();
+            else loads_landed<0>();
             v4i A[2][R], B[2][C];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
 #pragma unroll
-                for (int r = 0; r < R; r++) A[h][r] = i8_of_line(stage + mine, lane, r, h);
+                for (int r = 0; r < R; r++) A[h][r] = line_piece(stage + mine, lane, r, h);
 #pragma unroll
-                for (int c = 0; c < C; c++) B[h][c] = i8_of_line(stage + mine, lane, R + c, h);
+                for (int c = 0; c < C; c++) B[h][c] = line_piece(stage + mine, lane, R + c, h);
             }
             if (l + 3 * NW < lines) src.ask(free + mine, l + 3 * NW, a.kp);
 #pragma unroll
@@ -447,13 +355,13 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
         float scale = 0.0f, row_scale[4];
         if (out) {
             bool bad;
-            const u32 col = i8_column(a, j, bad);
+            const u32 col = run_column(a, j, bad);
             if (bad) bm_raise(a.fault, a.layer, kSiteExpertId);
             scale = bad ? bm_bits_f32(0x7fc00000u) : a.qs[col];
 #pragma unroll
             for (int x = 0; x < 4; x++) row_scale[x] = run.ws[min(row + x, a.rows - 1)];
         }
-        i8_landed<0>();
+        loads_landed<0>();
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
@@ -466,7 +374,7 @@ __global__ __launch_bounds__(64 * NW) void k_i8_few(I8Args a) {
             float v[4];
 #pragma unroll
             for (int x = 0; x < 4; x++) v[x] = __fmul_rn(__fmul_rn((float)sum[x], scale), row_scale[x]);
-            i8_store4(a, j, row, v);
+            run_store4(a, j, row, v);
         }
         __syncthreads();
     }
@@ -484,7 +392,7 @@ constexpr u32 few_x_values(u32 M) { return 64 * kFewXWaves * 8 * 4 / M; } // val
 template <int ET, int M, int R>
 __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArgs qa) {
     constexpr int NW = kFewXWaves, T = 64 * NW / M, kPieces = 4; // threads a row, pieces a thread
-    typedef I8Lines<2 * R> L;
+    typedef Lines<2 * R> L;
     // M rows of kp. An array of its own, which no load on its way into LDS reaches: a write to it waits for none
     __shared__ __align__(16) int8_t codes[M * few_x_values(M)];
     __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[NW * L::kStage], ring3[NW * L::kStage];
@@ -506,7 +414,7 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
     src.ask(ring1 + mine, min(wave + NW, lines - 1), a.kp);
     src.ask(ring2 + mine, min(wave + 2 * NW, lines - 1), a.kp);
     __builtin_amdgcn_sched_barrier(0);
-    i8_landed<6 * R>();
+    loads_landed<6 * R>();
     __builtin_amdgcn_sched_barrier(0);
     float v[kPieces][8];
     bool odd = false;
@@ -520,7 +428,7 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
     most = max(most, (u32)__shfl_xor((int)most, 32, 64));
     if constexpr (M < NW) {
         if (lane == 0) top[wave] = most;
-        i8_meet();
+        lds_meet();
         most = 0;
 #pragma unroll
         for (int w = 0; w < NW / M; w++) most = max(most, top[row * (NW / M) + w]);
@@ -541,7 +449,7 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
         *reinterpret_cast<uint2 *>(codes + row * a.kp + 8 * c) = word;
         if (blockIdx.x == 0 && row < qa.m) *reinterpret_cast<uint2 *>(qa.codes + (size_t)row * a.kp + 8 * c) = word;
     }
-    i8_meet();
+    lds_meet();
 
     v4i acc[R];
 #pragma unroll
@@ -549,9 +457,9 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
     const u32 col = lane & 15;
     const auto step = [&](const uint8_t *stage, uint8_t *free, u32 l) {
         constexpr int n = 2 * R;
-        if (l + 2 * NW < lines) i8_landed<2 * n>();
-        else if (l + NW < lines) i8_landed<n>();
-        else i8_landed<0>();
+        if (l + 2 * NW < lines) loads_landed<2 * n>();
+        else if (l + NW < lines) loads_landed<n>();
+        else loads_landed<0>();
         v4i A[2][R], B[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -560,7 +468,7 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
             const v4i b = *reinterpret_cast<const v4i *>(codes + (in ? col * a.kp + at : 0u));
             B[h] = in ? b : v4i{0, 0, 0, 0};
 #pragma unroll
-            for (int r = 0; r < R; r++) A[h][r] = i8_of_line(stage + mine, lane, r, h);
+            for (int r = 0; r < R; r++) A[h][r] = line_piece(stage + mine, lane, r, h);
         }
         if (l + 3 * NW < lines) src.ask(free + mine, l + 3 * NW, a.kp);
 #pragma unroll
@@ -585,7 +493,7 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
     if (mine_out)
 #pragma unroll
         for (int x = 0; x < 4; x++) row_scale[x] = a.ws[min(out + x, a.rows - 1)];
-    i8_landed<0>();
+    loads_landed<0>();
 #pragma unroll
     for (int r = 0; r < R; r++) *reinterpret_cast<v4i *>(ring0 + mine + r * 1024 + 16 * lane) = acc[r];
     __syncthreads();
@@ -596,7 +504,7 @@ __global__ __launch_bounds__(64 * kFewXWaves) void k_i8_few_x(I8Args a, QuantArg
     float y[4];
 #pragma unroll
     for (int x = 0; x < 4; x++) y[x] = __fmul_rn(__fmul_rn((float)sum[x], scale[col]), row_scale[x]);
-    i8_store4(a, col, out, y);
+    run_store4(a, col, out, y);
 }
 
 // Many columns a matrix: BT columns x BR rows a workgroup, 128 bytes of k a step through a ring of S LDS buffers, where the loads put them
@@ -620,56 +528,6 @@ struct I8Tile {
     // buffers from this one on lie past what a read's constant reaches
     static constexpr int kUp = S * kStage <= 65536 ? S : S / 2;
 };
-
-// A tile of the experts: their runs cut into tiles of BT entries, numbered through the experts in order. False: there is none of that number. The bounds
-// of 256 experts are asked for at once; a run that is none has no tiles. `check`: every run is looked at, those behind the tile too, and one that
-// is none raises ExpertId (one workgroup of a launch does so).
-template <int BT>
-__device__ __forceinline__ bool i8_find_tile(const I8Args &a, u32 tile, bool check, u32 &expert, u32 &t0) {
-    const u32 lane = threadIdx.x & 63;
-    u32 before = 0;
-    bool found = false;
-    for (u32 e0 = 0; e0 < a.n_experts; e0 += 256) {
-        u32 j0[4], j1[4];
-#pragma unroll
-        for (u32 i = 0; i < 4; i++) {
-            const u32 e = min(e0 + 64 * i + lane, a.n_experts - 1);
-            j0[i] = a.start[e];
-            j1[i] = a.start[e + 1];
-        }
-        if (check) {
-            bool none = false;
-#pragma unroll
-            for (u32 i = 0; i < 4; i++) none |= j0[i] > j1[i] || j1[i] > a.n_slots; // (lanes past the last look at the last once more)
-            if (none) bm_raise(a.fault, a.layer, kSiteExpertId);
-            if (found) continue;
-        }
-#pragma unroll
-        for (u32 i = 0; i < 4; i++) {
-            const u32 e = e0 + 64 * i + lane;
-            if (e0 + 64 * i >= a.n_experts) break;
-            const bool run = j0[i] <= j1[i] && j1[i] <= a.n_slots;
-            const u32 c = e < a.n_experts && run ? (j1[i] - j0[i] + BT - 1) / BT : 0;
-            u32 upto = c;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const u32 o = (u32)__shfl_up((int)upto, d, 64);
-                if (lane >= (u32)d) upto += o;
-            }
-            const unsigned long long mine = __ballot(c != 0 && before + upto - c <= tile && tile < before + upto);
-            if (mine) {
-                const int l = __builtin_ctzll(mine);
-                expert = (u32)__builtin_amdgcn_readfirstlane((int)(e0 + 64 * i + (u32)l));
-                t0 = (u32)__builtin_amdgcn_readfirstlane((int)((tile - before - (u32)__shfl((int)(upto - c), l, 64)) * BT));
-                if (!check) return true;
-                found = true;
-                break;
-            }
-            before += (u32)__shfl((int)upto, 63, 64);
-        }
-    }
-    return found;
-}
 
 // All but the last AHEAD steps that a wave asked for have landed, and every wave is done with the buffer that is written next. (The wait as a
 // builtin: the compiler counts it, where behind one in asm it would wait for the loads that follow too.)
@@ -701,13 +559,13 @@ __device__ __forceinline__ void i8_ask(I8Src<G> &s, uint8_t *buf, u32 wave, bool
 #pragma unroll
     for (int r = 0; r < G::RT; r++) {
         const u32 group = wave * G::RT + r;
-        __builtin_amdgcn_global_load_lds((i8_gptr *)(s.q + (s.col[r] - (last ? s.back[group & 1] : 0u))), (i8_lptr *)(buf + group * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((lds_from *)(s.q + (s.col[r] - (last ? s.back[group & 1] : 0u))), (lds_to *)(buf + group * 1024), 16, 0, 0);
     }
 #pragma unroll
     for (int r = 0; r < G::RR; r++) {
         const u32 group = i8_row_group<G>(wave, r);
-        __builtin_amdgcn_global_load_lds((i8_gptr *)(s.w + (s.row[r] - (last ? (group & 1 ? s.back[1] : s.back[0]) : 0u))),
-                                         (i8_lptr *)(buf + G::kColumns * 128 + group * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((lds_from *)(s.w + (s.row[r] - (last ? (group & 1 ? s.back[1] : s.back[0]) : 0u))),
+                                         (lds_to *)(buf + G::kColumns * 128 + group * 1024), 16, 0, 0);
     }
     s.q += 128;
     s.w += 128;
@@ -716,7 +574,7 @@ __device__ __forceinline__ void i8_ask(I8Src<G> &s, uint8_t *buf, u32 wave, bool
 template <class G>
 __device__ __forceinline__ void i8_zero_past(uint8_t *buf, u32 have) {
     for (u32 i = threadIdx.x; i < G::kColumns * 8; i += G::kThreads)
-        if (((i & 7) ^ i8_swizzle(i >> 3)) >= have) *reinterpret_cast<uint4 *>(buf + 16 * i) = make_uint4(0, 0, 0, 0);
+        if (((i & 7) ^ line_swizzle(i >> 3)) >= have) *reinterpret_cast<uint4 *>(buf + 16 * i) = make_uint4(0, 0, 0, 0);
     __syncthreads();
 }
 
@@ -840,7 +698,7 @@ __device__ __forceinline__ void i8_tile_out(const I8Args &a, const I8Run &run, u
     float col_scale = 0.0f;
     if (lane < G::TT * 16 && e0 + lane < run.j1) {
         bool bad;
-        const u32 col = i8_column(a, e0 + lane, bad);
+        const u32 col = run_column(a, e0 + lane, bad);
         if (bad) bm_raise(a.fault, a.layer, kSiteExpertId);
         col_scale = bad ? bm_bits_f32(0x7fc00000u) : a.qs[col];
     }
@@ -888,7 +746,7 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     // Workgroups go to the chip's eight dies in turn (b to die b % 8, each with its own L2). Neighbouring workgroups share a tile's columns across
     // the dies, and a die's workgroups four of the rows' tiles and eight of the columns'. An expert with fewer tiles of rows than dies
     // would so have its rows on every die: there (`group`) a group of its tiles of columns stays on one die, all rows of it.
-    const u32 block = i8_group();
+    const u32 block = group_index();
     u32 expert = 0, t0, row_tile, tile;
     if (group) {
         const u32 i = block >> 3, per = group * n_row_tiles;
@@ -901,7 +759,7 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     if (!a.start) {
         t0 = tile * BT;
         if (t0 >= a.m) return;
-    } else if (!i8_find_tile<BT>(a, tile, tile == 0 && row_tile == 0, expert, t0)) return;
+    } else if (!run_tile<BT>(a, tile, tile == 0 && row_tile == 0, expert, t0)) return;
     const u32 r0 = row_tile * BR;
     I8Run run;
     if (!i8_run(a, expert, run)) return;
@@ -915,17 +773,17 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     u32 col[G::RT];
 #pragma unroll
     for (int r = 0; r < G::RT; r++) col[r] = min(t0 + (wave * G::RT + r) * 8 + (lane >> 3), run.j1 - 1);
-    if (a.order) i8_columns<G::RT>(a, col);
+    if (a.order) run_columns(a, col);
 #pragma unroll
-    for (int r = 0; r < G::RT; r++) src.col[r] = (a.order ? col[r] : col[r] - t0) * a.kp + 16 * ((lane & 7) ^ i8_swizzle((wave * G::RT + r) * 8 + (lane >> 3)));
+    for (int r = 0; r < G::RT; r++) src.col[r] = (a.order ? col[r] : col[r] - t0) * a.kp + 16 * ((lane & 7) ^ line_swizzle((wave * G::RT + r) * 8 + (lane >> 3)));
 #pragma unroll
     for (int r = 0; r < G::RR; r++) {
         const u32 line = i8_row_group<G>(wave, r) * 8 + (lane >> 3);
-        src.row[r] = (min(r0 + line, a.rows - 1) - r0) * a.kp + 16 * ((lane & 7) ^ i8_swizzle(line));
+        src.row[r] = (min(r0 + line, a.rows - 1) - r0) * a.kp + 16 * ((lane & 7) ^ line_swizzle(line));
     }
 #pragma unroll
     for (int r = 0; r < 2; r++) { // (a lane's piece differs between even and odd groups of eight lines only)
-        const u32 piece = (lane & 7) ^ i8_swizzle(8 * r + (lane >> 3));
+        const u32 piece = (lane & 7) ^ line_swizzle(8 * r + (lane >> 3));
         src.back[r] = piece >= tail ? 16 * piece : 0;
     }
 
@@ -938,7 +796,7 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     I8At at[2];
 #pragma unroll
     for (u32 c = 0; c < 2; c++) {
-        const u32 piece = (lane & 15) * 128 + 16 * ((4 * c + (lane >> 4)) ^ i8_swizzle(lane & 15));
+        const u32 piece = (lane & 15) * 128 + 16 * ((4 * c + (lane >> 4)) ^ line_swizzle(lane & 15));
 #pragma unroll
         for (u32 up = 0; up < 2; up++) {
             at[up].a[c] = piece + wr * 128 + up * G::kUp * G::kStage;
@@ -1019,7 +877,7 @@ static hipError_t tile_launch(const Launch &L, const I8Args &a, u32 entries) {
     if (a.start) tiles = entries / BT + (a.n_experts < entries ? a.n_experts : entries); // at most a ragged tile an expert
     const u32 group = a.start && row_tiles < 8 ? 2 : 0;
     if (group) tiles = (tiles + 8 * group - 1) / (8 * group) * (8 * group);
-    hipLaunchKernelGGL((k_i8_tile<BT, BR, WT, WR, S, WHOLE, EU>), i8_grid((uint64_t)tiles * row_tiles, 64 * WT * WR), dim3(64 * WT * WR), 0, L.stream, a, row_tiles, group);
+    hipLaunchKernelGGL((k_i8_tile<BT, BR, WT, WR, S, WHOLE, EU>), group_grid((uint64_t)tiles * row_tiles, 64 * WT * WR), dim3(64 * WT * WR), 0, L.stream, a, row_tiles, group);
     return hipGetLastError();
 }
 
