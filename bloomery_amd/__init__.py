@@ -110,6 +110,16 @@ SYMBOLS = {
     "bm_i8_gemm": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _i, _i64]),
     "bm_i8_gemm_x": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i, _i64, _i, _vp, _vp, _vp, _i, _i64]),
     "bm_i8_gemm_experts": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _i, _i64]),
+    "bm_mx4_row_bytes": (_i64, [_i]),
+    "bm_mx4_row_scales": (_i64, [_i]),
+    "bm_mx4_quantize": (_i, [_vp, _vp, _i, _i64, _i, _i, _vp, _vp, _vp]),
+    "bm_mx4_swiglu_quantize": (_i, [_vp, _vp, _vp, _i, _i64, _i, _i, _vp, _vp, _vp, _vp]),
+    "bm_mx4_dequantize": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i, _i64]),
+    "bm_mx4_gemm": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _i, _i64]),
+    "bm_mx4_gemm_x": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i, _i64, _i, _vp, _vp, _vp, _i, _i64]),
+    "bm_mx4_gemm_experts": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _i, _i64]),
+    "bm_mx4_moe_work": (_i64, [_i, _i, _i, _i]),
+    "bm_mx4_moe": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _i64, _i, _vp, _vp, _i, _vp, _i64, _vp, _vp, _i64, _vp]),
     "bm_gguf_open": (_i, [C.c_char_p, C.POINTER(_vp)]),
     "bm_gguf_open_split": (_i, [C.c_char_p, C.POINTER(_vp)]),
     "bm_gguf_close": (None, [_vp]),
@@ -184,6 +194,21 @@ def i8_gemm_form(rows, k, n_cols, n_experts=0, n_slots=0, top_k=0):
     if form < 0:
         raise GpuError(form, f"bm_i8_gemm_form: {n_experts} experts of {rows} x {k}, {n_cols} columns, {n_slots} slots, top_k {top_k}")
     return form & 1023, form >> 10 & 1023, form >> 20 & 15, form >> 24 & 15
+
+
+def mx4_row_bytes(k):
+    """Bytes of a row of 4-bit codes: 16 for each block of 32 values."""
+    return int(load_library().bm_mx4_row_bytes(k))
+
+
+def mx4_row_scales(k):
+    """Bytes of a row of block scales: one for each block of 32 values, rounded up to 16."""
+    return int(load_library().bm_mx4_row_scales(k))
+
+
+def mx4_moe_work(n_tokens, top_k, hidden, ff):
+    """Bytes of scratch that enqueue_mx4_moe takes."""
+    return int(load_library().bm_mx4_moe_work(n_tokens, top_k, hidden, ff))
 
 
 def expert_sort_work(n_slots, n_experts):
@@ -644,6 +669,42 @@ class Gpu:
             n_cols = n_slots // top_k if top_k > 0 else n_slots
         self._check(self.lib.bm_i8_gemm_experts(self.ctx, w, w_scales, n_experts, rows_per_expert, k, codes, scales,
                                                 n_cols, order, start, n_slots, top_k, y, y_type, rows_per_expert if ld_y is None else ld_y))
+
+    # -- microscaled 4-bit floating point: codes of mx4_row_bytes(k) and scales of mx4_row_scales(k) bytes a row, on both sides
+    def enqueue_mx4_quantize(self, x, dtype, m, k, codes, scales, ld_x=None, live=None):
+        """live: a device word; rows at or past its value keep what they held."""
+        self._check(self.lib.bm_mx4_quantize(self.ctx, x, dtype, k if ld_x is None else ld_x, m, k, live, codes, scales))
+
+    def enqueue_mx4_swiglu_quantize(self, g, u, dtype, m, k, codes, scales, ld=None, live=None, rule=None):
+        self._check(self.lib.bm_mx4_swiglu_quantize(self.ctx, g, u, dtype, k if ld is None else ld, m, k, _rule(rule) if rule is not None else None, live,
+                                                    codes, scales))
+
+    def enqueue_mx4_dequantize(self, codes, scales, m, k, y, dtype, ld_y=None):
+        """The values that the codes stand for."""
+        self._check(self.lib.bm_mx4_dequantize(self.ctx, codes, scales, m, k, y, dtype, k if ld_y is None else ld_y))
+
+    def enqueue_mx4_gemm(self, w, w_scales, rows, k, codes, scales, m, y, y_type, ld_y=None):
+        self._check(self.lib.bm_mx4_gemm(self.ctx, w, w_scales, rows, k, codes, scales, m, y, y_type, rows if ld_y is None else ld_y))
+
+    def enqueue_mx4_gemm_x(self, w, w_scales, rows, k, x, x_type, m, codes, scales, y, y_type, ld_x=None, ld_y=None):
+        """enqueue_mx4_quantize of the m rows of x and enqueue_mx4_gemm in one call."""
+        self._check(self.lib.bm_mx4_gemm_x(self.ctx, w, w_scales, rows, k, x, x_type, k if ld_x is None else ld_x, m, codes, scales, y, y_type,
+                                           rows if ld_y is None else ld_y))
+
+    def enqueue_mx4_gemm_experts(self, w, w_scales, n_experts, rows_per_expert, k, codes, scales, order, start, n_slots, top_k, y, y_type,
+                                 ld_y=None, n_cols=None):
+        """top_k > 0: every slot of a token reads the token's column; 0: entry j reads column j."""
+        if n_cols is None:
+            n_cols = n_slots // top_k if top_k > 0 else n_slots
+        self._check(self.lib.bm_mx4_gemm_experts(self.ctx, w, w_scales, n_experts, rows_per_expert, k, codes, scales, n_cols, order, start, n_slots,
+                                                 top_k, y, y_type, rows_per_expert if ld_y is None else ld_y))
+
+    def enqueue_mx4_moe(self, gate, up, down, n_experts, hidden, ff, x, dtype, n_tokens, sel, weights, top_k, resid, y, work, ld_x=None, ld_resid=None,
+                        ld_y=None, rule=None):
+        """gate, up, down: (codes, scales) of the experts' stacks. work: mx4_moe_work(n_tokens, top_k, hidden, ff) bytes."""
+        self._check(self.lib.bm_mx4_moe(self.ctx, *gate, *up, *down, n_experts, hidden, ff, x, dtype, hidden if ld_x is None else ld_x, n_tokens, sel,
+                                        weights, top_k, resid, hidden if ld_resid is None else ld_resid, _rule(rule) if rule is not None else None, y,
+                                        hidden if ld_y is None else ld_y, work))
 
     # -- grouped decode: the slot table by expert and the tile launchers
     def tile_cap(self, n_slots, n_experts):

@@ -1647,6 +1647,157 @@ int bm_i8_gemm_form(int n_experts, int rows, int k, int n_cols, int n_slots, int
     return bmk::i8_gemm_form(n_experts, rows, k, n_cols, n_slots, top_k);
 }
 
+// ------------------------------------------------------------------------- microscaled 4-bit floating point
+
+int64_t bm_mx4_row_bytes(int k) { return k < 1 || k > bmk::kMx4MaxK ? (int64_t)BM_ESHAPE : (int64_t)bmk::mx4_row_bytes(k); }
+int64_t bm_mx4_row_scales(int k) { return k < 1 || k > bmk::kMx4MaxK ? (int64_t)BM_ESHAPE : (int64_t)bmk::mx4_row_scales(k); }
+
+static int check_aligned(bm_ctx *ctx, const char *what, const char *name, const void *p) {
+    if (!p) return fail(ctx, BM_EARG, "%s: %s is NULL", what, name);
+    if (((uintptr_t)p & 15) != 0) return fail(ctx, BM_ESHAPE, "%s: %s %p must be 16-byte aligned", what, name, p);
+    return BM_OK;
+}
+static int check_mx4(bm_ctx *ctx, const char *what, const char *name, const void *codes, const char *scales_name, const void *scales) {
+    BM_TRY(check_aligned(ctx, what, name, codes));
+    return check_aligned(ctx, what, scales_name, scales);
+}
+static int check_mx4_size(bm_ctx *ctx, const char *what, const char *name, int rows, int k) {
+    if (rows < 1 || rows > kI8MaxRows) return fail(ctx, BM_ESHAPE, "%s: %s = %d rows (1 .. %d)", what, name, rows, kI8MaxRows);
+    if (k < 1 || k > bmk::kMx4MaxK) return fail(ctx, BM_ESHAPE, "%s: rows of k = %d values (1 .. %d)", what, k, bmk::kMx4MaxK);
+    return BM_OK;
+}
+
+static int mx4_quant(bm_ctx *ctx, const char *what, const void *x_dev, const void *u_dev, bool glu, int elem_type, int64_t ld, int m, int k,
+                     const bm_gate_act *rule, const uint32_t *live_dev, uint8_t *codes_dev, uint8_t *scales_dev) {
+    BM_TRY(check_mx4_size(ctx, what, "m", m, k));
+    BM_TRY(check_elem(ctx, what, elem_type));
+    BM_TRY(check_rows(ctx, what, glu ? "g_dev" : "x_dev", x_dev, elem_type, k, ld));
+    if (glu) BM_TRY(check_rows(ctx, what, "u_dev", u_dev, elem_type, k, ld));
+    if (((uintptr_t)live_dev & 3) != 0) return fail(ctx, BM_ESHAPE, "%s: live_dev %p is not 4-byte aligned", what, (const void *)live_dev);
+    BM_TRY(check_mx4(ctx, what, "codes_dev", codes_dev, "scales_dev", scales_dev));
+    bmk::GateRule checked = {0u, 0.0f};
+    if (rule) BM_TRY(rule_checked(ctx, what, rule->rule, rule->limit, &checked));
+    if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
+    bmk::Launch L = launch_of(ctx);
+    if (rule) L.rule = checked;
+    DeviceScope on(ctx->device);
+    return driver(ctx, what, bmk::mx4_quantize(L, x_dev, u_dev, elem_type, ld, m, k, live_dev, codes_dev, scales_dev));
+}
+
+int bm_mx4_quantize(bm_ctx *ctx, const void *x_dev, int elem_type, int64_t ld_x, int m, int k, const uint32_t *live_dev, uint8_t *codes_dev,
+                    uint8_t *scales_dev) {
+    return mx4_quant(ctx, "bm_mx4_quantize", x_dev, nullptr, false, elem_type, ld_x, m, k, nullptr, live_dev, codes_dev, scales_dev);
+}
+
+int bm_mx4_swiglu_quantize(bm_ctx *ctx, const void *g_dev, const void *u_dev, int elem_type, int64_t ld, int m, int k, const bm_gate_act *rule,
+                           const uint32_t *live_dev, uint8_t *codes_dev, uint8_t *scales_dev) {
+    return mx4_quant(ctx, "bm_mx4_swiglu_quantize", g_dev, u_dev, true, elem_type, ld, m, k, rule, live_dev, codes_dev, scales_dev);
+}
+
+int bm_mx4_dequantize(bm_ctx *ctx, const uint8_t *codes_dev, const uint8_t *scales_dev, int m, int k, void *y_dev, int elem_type, int64_t ld_y) {
+    const char *what = "bm_mx4_dequantize";
+    BM_TRY(check_mx4_size(ctx, what, "m", m, k));
+    BM_TRY(check_mx4(ctx, what, "codes_dev", codes_dev, "scales_dev", scales_dev));
+    BM_TRY(check_elem(ctx, what, elem_type));
+    BM_TRY(check_rows(ctx, what, "y_dev", y_dev, elem_type, k, ld_y));
+    if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
+    DeviceScope on(ctx->device);
+    return driver(ctx, what, bmk::mx4_dequantize(launch_of(ctx), codes_dev, scales_dev, m, k, y_dev, elem_type, ld_y));
+}
+
+int bm_mx4_gemm(bm_ctx *ctx, const uint8_t *w_dev, const uint8_t *w_scales_dev, int rows, int k, const uint8_t *codes_dev, const uint8_t *scales_dev,
+                int m, void *y_dev, int y_type, int64_t ld_y) {
+    const char *what = "bm_mx4_gemm";
+    BM_TRY(check_mx4_size(ctx, what, "rows", rows, k));
+    BM_TRY(check_mx4(ctx, what, "w_dev", w_dev, "w_scales_dev", w_scales_dev));
+    BM_TRY(check_mx4_size(ctx, what, "m", m, k));
+    BM_TRY(check_mx4(ctx, what, "codes_dev", codes_dev, "scales_dev", scales_dev));
+    BM_TRY(check_elem(ctx, what, y_type));
+    BM_TRY(check_rows(ctx, what, "y_dev", y_dev, y_type, rows, ld_y));
+    if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
+    DeviceScope on(ctx->device);
+    return driver(ctx, what, bmk::mx4_gemm(launch_of(ctx), w_dev, w_scales_dev, 1, rows, k, codes_dev, scales_dev, m, nullptr, nullptr, 0, 0, y_dev,
+                                           y_type, ld_y));
+}
+
+int bm_mx4_gemm_x(bm_ctx *ctx, const uint8_t *w_dev, const uint8_t *w_scales_dev, int rows, int k, const void *x_dev, int x_type, int64_t ld_x, int m,
+                  uint8_t *codes_dev, uint8_t *scales_dev, void *y_dev, int y_type, int64_t ld_y) {
+    const char *what = "bm_mx4_gemm_x";
+    BM_TRY(check_mx4_size(ctx, what, "rows", rows, k));
+    BM_TRY(check_mx4(ctx, what, "w_dev", w_dev, "w_scales_dev", w_scales_dev));
+    BM_TRY(check_mx4_size(ctx, what, "m", m, k));
+    BM_TRY(check_elem(ctx, what, x_type));
+    BM_TRY(check_rows(ctx, what, "x_dev", x_dev, x_type, k, ld_x));
+    BM_TRY(check_mx4(ctx, what, "codes_dev", codes_dev, "scales_dev", scales_dev));
+    BM_TRY(check_elem(ctx, what, y_type));
+    BM_TRY(check_rows(ctx, what, "y_dev", y_dev, y_type, rows, ld_y));
+    if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
+    DeviceScope on(ctx->device);
+    return driver(ctx, what, bmk::mx4_gemm_x(launch_of(ctx), w_dev, w_scales_dev, rows, k, x_dev, x_type, ld_x, m, codes_dev, scales_dev, y_dev, y_type,
+                                             ld_y));
+}
+
+int bm_mx4_gemm_experts(bm_ctx *ctx, const uint8_t *w_dev, const uint8_t *w_scales_dev, int n_experts, int rows_per_expert, int k,
+                        const uint8_t *codes_dev, const uint8_t *scales_dev, int n_cols, const uint32_t *order_dev, const uint32_t *start_dev,
+                        int n_slots, int top_k, void *y_dev, int y_type, int64_t ld_y) {
+    const char *what = "bm_mx4_gemm_experts";
+    BM_TRY(check_mx4_size(ctx, what, "rows", rows_per_expert, k));
+    BM_TRY(check_mx4(ctx, what, "w_dev", w_dev, "w_scales_dev", w_scales_dev));
+    BM_TRY(check_i8_runs(ctx, what, n_experts, n_cols, n_slots, top_k));
+    BM_TRY(check_mx4(ctx, what, "codes_dev", codes_dev, "scales_dev", scales_dev));
+    if (top_k > 0) BM_TRY(check_words(ctx, what, "order_dev", order_dev));
+    BM_TRY(check_words(ctx, what, "start_dev", start_dev));
+    BM_TRY(check_elem(ctx, what, y_type));
+    BM_TRY(check_rows(ctx, what, "y_dev", y_dev, y_type, rows_per_expert, ld_y));
+    if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
+    DeviceScope on(ctx->device);
+    return driver(ctx, what, bmk::mx4_gemm(launch_of(ctx), w_dev, w_scales_dev, n_experts, rows_per_expert, k, codes_dev, scales_dev, n_cols,
+                                           top_k > 0 ? order_dev : nullptr, start_dev, n_slots, top_k, y_dev, y_type, ld_y));
+}
+
+static int check_mx4_moe(bm_ctx *ctx, const char *what, int n_tokens, int top_k, int hidden, int ff) {
+    if (n_tokens < 1 || n_tokens > bmk::kMx4MoeTokens || top_k < 1 || top_k > bmk::kMaxCombineSlots)
+        return fail(ctx, BM_ESHAPE, "%s: %d tokens of %d slots (1 .. %d tokens, 1 .. %d slots a token)", what, n_tokens, top_k, bmk::kMx4MoeTokens,
+                    bmk::kMaxCombineSlots);
+    if (hidden < 1 || hidden > bmk::kMx4MaxK || ff < 1 || ff > bmk::kMx4MaxK)
+        return fail(ctx, BM_ESHAPE, "%s: hidden = %d, ff = %d values (1 .. %d)", what, hidden, ff, bmk::kMx4MaxK);
+    return BM_OK;
+}
+
+int64_t bm_mx4_moe_work(int n_tokens, int top_k, int hidden, int ff) {
+    BM_TRY(check_mx4_moe(nullptr, "bm_mx4_moe_work", n_tokens, top_k, hidden, ff));
+    return (int64_t)bmk::mx4_moe_work(n_tokens, top_k, hidden, ff);
+}
+
+int bm_mx4_moe(bm_ctx *ctx, const uint8_t *wg_dev, const uint8_t *wg_scales_dev, const uint8_t *wu_dev, const uint8_t *wu_scales_dev,
+               const uint8_t *wd_dev, const uint8_t *wd_scales_dev, int n_experts, int hidden, int ff, const void *x_dev, int elem_type, int64_t ld_x,
+               int n_tokens, const uint32_t *sel_dev, const float *w_dev, int top_k, const void *resid_dev, int64_t ld_resid, const bm_gate_act *rule,
+               void *y_dev, int64_t ld_y, void *work_dev) {
+    const char *what = "bm_mx4_moe";
+    BM_TRY(check_mx4_moe(ctx, what, n_tokens, top_k, hidden, ff));
+    if (n_experts < 1 || n_experts > bmk::kBucketExperts) return fail(ctx, BM_ESHAPE, "%s: %d experts (1 .. %d)", what, n_experts, bmk::kBucketExperts);
+    BM_TRY(check_mx4(ctx, what, "wg_dev", wg_dev, "wg_scales_dev", wg_scales_dev));
+    BM_TRY(check_mx4(ctx, what, "wu_dev", wu_dev, "wu_scales_dev", wu_scales_dev));
+    BM_TRY(check_mx4(ctx, what, "wd_dev", wd_dev, "wd_scales_dev", wd_scales_dev));
+    BM_TRY(check_elem(ctx, what, elem_type));
+    BM_TRY(check_rows(ctx, what, "x_dev", x_dev, elem_type, hidden, ld_x));
+    BM_TRY(check_words(ctx, what, "sel_dev", sel_dev));
+    BM_TRY(check_words(ctx, what, "w_dev", w_dev));
+    if (resid_dev) BM_TRY(check_rows(ctx, what, "resid_dev", resid_dev, elem_type, hidden, ld_resid));
+    BM_TRY(check_rows(ctx, what, "y_dev", y_dev, elem_type, hidden, ld_y));
+    if (resid_dev == y_dev && ld_resid != ld_y)
+        return fail(ctx, BM_ESHAPE, "%s: y_dev is resid_dev, and their rows lie %lld and %lld apart", what, (long long)ld_y, (long long)ld_resid);
+    BM_TRY(check_aligned(ctx, what, "work_dev", work_dev));
+    bmk::GateRule checked = {0u, 0.0f};
+    if (rule) BM_TRY(rule_checked(ctx, what, rule->rule, rule->limit, &checked));
+    if (!ctx) return fail(nullptr, BM_EARG, "%s: ctx is NULL", what);
+    bmk::Launch L = launch_of(ctx);
+    if (rule) L.rule = checked;
+    DeviceScope on(ctx->device);
+    return driver(ctx, what, bmk::mx4_moe(L, {wg_dev, wg_scales_dev}, {wu_dev, wu_scales_dev}, {wd_dev, wd_scales_dev}, n_experts, hidden, ff, x_dev,
+                                          elem_type, ld_x, n_tokens, sel_dev, w_dev, top_k, resid_dev, ld_resid, y_dev, ld_y, work_dev));
+}
+
 // ------------------------------------------------------------------------------------ graphs and events
 
 struct bm_graph {

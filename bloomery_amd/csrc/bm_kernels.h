@@ -229,6 +229,31 @@ int i8_gemm_form(int n_experts, int rows, int k, int n_cols, int n_slots, int to
 hipError_t i8_gemm_x(const Launch &L, const int8_t *w, const float *ws, int rows, int k, const void *x, int x_et, int64_t ld_x, int m, int8_t *codes,
                      float *scales, void *y, int et, int64_t ld);
 
+// ------------------------------------------------------ microscaled 4-bit floating point (bm_mx4.hip)
+
+// The most values a row may hold.
+constexpr int kMx4MaxK = 131072;
+inline int mx4_row_bytes(int k) { return (k + 31) / 32 * 16; }
+inline int mx4_row_scales(int k) { return (k + 511) / 512 * 16; }
+// u (optional): the rows are the launch's gate rule of x and u. live (optional): a device word, rows from there on keep what they hold.
+hipError_t mx4_quantize(const Launch &L, const void *x, const void *u, int et, int64_t ld, int m, int k, const uint32_t *live, uint8_t *codes,
+                        uint8_t *scales);
+hipError_t mx4_dequantize(const Launch &L, const uint8_t *codes, const uint8_t *scales, int m, int k, void *y, int et, int64_t ld);
+// start NULL: one matrix against n_cols columns. Else entry j of expert e's run reads column order[j] / top_k, or j where top_k is 0.
+hipError_t mx4_gemm(const Launch &L, const uint8_t *w, const uint8_t *ws, int n_experts, int rows, int k, const uint8_t *q, const uint8_t *qs, int n_cols,
+                    const uint32_t *order, const uint32_t *start, int n_slots, int top_k, void *y, int et, int64_t ld);
+hipError_t mx4_gemm_x(const Launch &L, const uint8_t *w, const uint8_t *ws, int rows, int k, const void *x, int x_et, int64_t ld_x, int m, uint8_t *codes,
+                      uint8_t *scales, void *y, int et, int64_t ld);
+// The experts' step of a few tokens; work: mx4_moe_work bytes.
+constexpr int kMx4MoeTokens = 64;
+struct Mx4Stack {
+    const uint8_t *w, *scales;
+};
+size_t mx4_moe_work(int n_tokens, int top_k, int hidden, int ff);
+hipError_t mx4_moe(const Launch &L, const Mx4Stack &g, const Mx4Stack &u, const Mx4Stack &d, int n_experts, int hidden, int ff, const void *x, int et,
+                   int64_t ld_x, int n_tokens, const uint32_t *sel, const float *w, int top_k, const void *resid, int64_t ld_resid, void *y, int64_t ld_y,
+                   void *work);
+
 } // namespace bmk
 
 #endif // BM_KERNELS_H

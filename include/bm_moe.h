@@ -544,6 +544,57 @@ int bm_i8_gemm_experts(bm_ctx *ctx, const int8_t *w_dev, const float *w_scales_d
                        const int8_t *codes_dev, const float *scales_dev, int n_cols, const uint32_t *order_dev, const uint32_t *start_dev,
                        int n_slots, int top_k, void *y_dev, int y_type, int64_t ld_y);
 
+/* -------------------------------------------------------------- microscaled 4-bit floating point */
+
+/* Rows in blocks of 32 values: a code of four bits each - one sign, two exponent and one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6 - and a
+ * power of two for the block, 2^(b - 127), b a byte (255: NaN). A row of k values (1 .. 131072) is bm_mx4_row_bytes(k) = 16 ceil(k / 32) bytes
+ * of codes, the even value's in a byte's low half, zeros behind the k-th value, and bm_mx4_row_scales(k) = ceil(k / 32) rounded up
+ * to 16 bytes of scales, whose bytes behind the last block the quantizer zeroes and nothing looks at; rows back to back, both pointers
+ * 16-byte aligned. Rows of floating values as in the section of the experts' rows.
+ * The quantizer's block: 2^e with e the exponent of the block's largest magnitude less 2, held to -127 at least; a code the nearest
+ * of the values above to x / 2^e, halves to the even code, held to 6. The division is exact, so no code depends on how it is computed.
+ * A block holding a value that is not finite raises BM_SITE_QUANT_COLUMN and gets the NaN scale and zero codes. */
+int64_t bm_mx4_row_bytes(int k);
+int64_t bm_mx4_row_scales(int k);
+/* m rows (1 .. 2^22) of k elements. live_dev (optional): a device word; rows at or past its value keep what they held (of sorted rows:
+ * start_dev + n_experts). */
+int bm_mx4_quantize(bm_ctx *ctx, const void *x_dev, int elem_type, int64_t ld_x, int m, int k, const uint32_t *live_dev, uint8_t *codes_dev,
+                    uint8_t *scales_dev);
+/* The same of the gate rule's values of two inputs (bm_i8_swiglu_quantize in this form; rule NULL: the context's), g_dev and u_dev rows both ld
+ * apart; the values are f32 on the way. */
+int bm_mx4_swiglu_quantize(bm_ctx *ctx, const void *g_dev, const void *u_dev, int elem_type, int64_t ld, int m, int k, const bm_gate_act *rule,
+                           const uint32_t *live_dev, uint8_t *codes_dev, uint8_t *scales_dev);
+/* And back: the values that m rows' codes stand for, rounded once where the element does not hold them. */
+int bm_mx4_dequantize(bm_ctx *ctx, const uint8_t *codes_dev, const uint8_t *scales_dev, int m, int k, void *y_dev, int elem_type, int64_t ld_y);
+/* y[t * ld_y + r] = the sum over blocks of 2^(scales[t] + w_scales[r] - 254) times the sum of the 32 products of codes[t] and w[r], for
+ * t < m, r < rows (1 .. 2^22 each), formed in f32 (products and sums of 32 are exact; the order in which blocks are added
+ * depends on the sizes alone) and rounded once. A sum past f32's range is infinite, a NaN scale makes every value it takes part in NaN. w_dev:
+ * rows of bm_mx4_row_bytes(k) bytes. */
+int bm_mx4_gemm(bm_ctx *ctx, const uint8_t *w_dev, const uint8_t *w_scales_dev, int rows, int k, const uint8_t *codes_dev, const uint8_t *scales_dev,
+                int m, void *y_dev, int y_type, int64_t ld_y);
+/* bm_mx4_quantize of x_dev's m rows and bm_mx4_gemm in one call, with the same codes and scales (caller-held, m rows); the sums may be added in another
+ * order than the two calls'. */
+int bm_mx4_gemm_x(bm_ctx *ctx, const uint8_t *w_dev, const uint8_t *w_scales_dev, int rows, int k, const void *x_dev, int x_type, int64_t ld_x, int m,
+                  uint8_t *codes_dev, uint8_t *scales_dev, void *y_dev, int y_type, int64_t ld_y);
+/* The product over experts' runs, with bm_i8_gemm_experts' tables, columns, refusals and faults: entry j of start[e] .. start[e + 1] writes
+ * y[j * ld_y + r] = expert e's row r against column order[j] / top_k, or j itself where top_k is 0. */
+int bm_mx4_gemm_experts(bm_ctx *ctx, const uint8_t *w_dev, const uint8_t *w_scales_dev, int n_experts, int rows_per_expert, int k,
+                        const uint8_t *codes_dev, const uint8_t *scales_dev, int n_cols, const uint32_t *order_dev, const uint32_t *start_dev,
+                        int n_slots, int top_k, void *y_dev, int y_type, int64_t ld_y);
+/* The experts' whole step for a few tokens (bm_moe_decode in this form; n_tokens 1 .. 64, top_k 1 .. 64, 1 .. 1024 experts), whose values stay
+ * in floating point: for token t, slot s of its top_k, expert e = sel_dev[t * top_k + s]: g = wg[e] x[t], u = wu[e] x[t] (ff rows of hidden values each),
+ * h = the rule's value of (g, u), and y[t] = resid[t] + the sum over s ascending of w_dev[t * top_k + s] * (wd[e] h) (hidden rows of ff values). Products and
+ * sums are f32, h is kept to 16 bits of mantissa at least, and y is rounded once to elem_type, which x_dev, resid_dev (NULL: none) and y_dev share;
+ * y_dev may be resid_dev. An id of BM_HOST_SLOT is skipped; any other at or past n_experts raises BM_SITE_EXPERT_ID and adds nothing,
+ * whatever its weight; an expert may stand at several slots of a token. rule NULL: the context's.
+ * work_dev: bm_mx4_moe_work(..) bytes of scratch, 16-byte aligned, that holds nothing between calls: at most n_tokens * top_k * (8 * ff + 8 * hidden + 1024) + 65536.
+ * Calls that may run at the same time need one each. */
+int64_t bm_mx4_moe_work(int n_tokens, int top_k, int hidden, int ff);
+int bm_mx4_moe(bm_ctx *ctx, const uint8_t *wg_dev, const uint8_t *wg_scales_dev, const uint8_t *wu_dev, const uint8_t *wu_scales_dev,
+               const uint8_t *wd_dev, const uint8_t *wd_scales_dev, int n_experts, int hidden, int ff, const void *x_dev, int elem_type, int64_t ld_x,
+               int n_tokens, const uint32_t *sel_dev, const float *w_dev, int top_k, const void *resid_dev, int64_t ld_resid, const bm_gate_act *rule,
+               void *y_dev, int64_t ld_y, void *work_dev);
+
 /* ------------------------------------------------------------------------------------------- model files */
 
 /* A GGUF file's header and a read-only mapping of it: the part of the reference's reader (crates/gguf/src/lib.rs:
