@@ -548,12 +548,6 @@ struct I8Src {
     const int8_t *q, *w; // this step's
     u32 col[G::RT], row[G::RR], back[2];
 };
-// The eight rows of a wave's r-th load: where there are not as many for every wave, the last ones are asked for again.
-template <class G>
-__device__ __forceinline__ u32 i8_row_group(u32 wave, int r) {
-    const u32 group = wave * G::RR + r;
-    return G::kRows % (8 * G::kWaves) == 0 ? group : min(group, (u32)G::kRows / 8 - 1);
-}
 template <class G>
 __device__ __forceinline__ void i8_ask(I8Src<G> &s, uint8_t *buf, u32 wave, bool last) {
 #pragma unroll
@@ -563,7 +557,7 @@ __device__ __forceinline__ void i8_ask(I8Src<G> &s, uint8_t *buf, u32 wave, bool
     }
 #pragma unroll
     for (int r = 0; r < G::RR; r++) {
-        const u32 group = i8_row_group<G>(wave, r);
+        const u32 group = tile_row_group<G>(wave, r);
         __builtin_amdgcn_global_load_lds((lds_from *)(s.w + (s.row[r] - (last ? (group & 1 ? s.back[1] : s.back[0]) : 0u))),
                                          (lds_to *)(buf + G::kColumns * 128 + group * 1024), 16, 0, 0);
     }
@@ -578,18 +572,6 @@ __device__ __forceinline__ void i8_zero_past(uint8_t *buf, u32 have) {
     __syncthreads();
 }
 
-// Where a lane's reads begin, for each 64 bytes of a step: of rows and of columns. The upper buffers' carry the first one's place with them
-// (and are read that far in front), so that a read's address is one register and a constant that its instruction can hold.
-struct I8At {
-    u32 a[2], b[2];
-};
-// What the matrix instructions take of 64 bytes of k of N tiles, from the FIRST on.
-template <class G, int B, int N>
-__device__ __forceinline__ void i8_read(v4i (&f)[N], const uint8_t *__restrict__ buf, u32 at, int first) {
-    constexpr u32 up = B >= G::kUp ? (u32)G::kUp * G::kStage : 0u;
-#pragma unroll
-    for (int i = 0; i < N; i++) f[i] = *reinterpret_cast<const v4i *>(buf + (int)(at - up + (first + i) * 2048));
-}
 template <int N, int TT>
 __device__ __forceinline__ void i8_multiply(const v4i (&a)[N], const v4i (&b)[TT], v4i (*acc)[TT]) {
 #pragma unroll
@@ -597,16 +579,6 @@ __device__ __forceinline__ void i8_multiply(const v4i (&a)[N], const v4i (&b)[TT
 #pragma unroll
         for (int j = 0; j < TT; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i], b[j], acc[i][j], 0, 0, 0);
 }
-// READS of what comes next between MFMAS products of what is there.
-template <int READS, int MFMAS>
-__device__ __forceinline__ void i8_weave() {
-#pragma unroll
-    for (int i = 0; i < READS; i++) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);              // an LDS read
-        __builtin_amdgcn_sched_group_barrier(0x008, MFMAS / READS ? MFMAS / READS : 1, 0); // products
-    }
-}
-
 // A step: its 128 bytes of k from buf in four parts - 64 bytes against half of the wave's rows each -, whose first part's pieces are in a0 and b0
 // already; leaves the next step's there. A part's pieces are read under the products of the part before. That the two buffers are apart is
 // said by restrict: else the compiler waits for the loads into one in front of every read of the other. The turn comes before the last
@@ -614,19 +586,19 @@ __device__ __forceinline__ void i8_weave() {
 // FULL: more steps are left behind this one than the ring holds, so that nothing is asked of where the rows end. B: buf's number.
 template <class G, int B, bool FULL>
 __device__ __forceinline__ void i8_step(I8Src<G> &src, uint8_t *__restrict__ buf, uint8_t *__restrict__ next, u32 wave, u32 left, u32 tail,
-                                        const I8At (&at)[2], v4i (&a0)[G::H0], v4i (&b0)[G::TT], v4i (&acc)[G::TR][G::TT]) {
+                                        const TileAt (&at)[2], v4i (&a0)[G::H0], v4i (&b0)[G::TT], v4i (&acc)[G::TR][G::TT]) {
     constexpr int kUp = B >= G::kUp, kNext = (B + 1) % G::kRing, kNextUp = kNext >= G::kUp;
     v4i a1[G::H1], b1[G::TT];
-    i8_read<G, B>(a1, buf, at[kUp].a[0], G::H0);
+    tile_read<G, B>(a1, buf, at[kUp].a[0], G::H0);
     i8_multiply(a0, b0, acc);
-    i8_weave<G::H1, G::H0 * G::TT>();
-    i8_read<G, B>(a0, buf, at[kUp].a[1], 0);
-    i8_read<G, B>(b1, buf, at[kUp].b[1], 0);
+    tile_weave<G::H1, G::H0 * G::TT>();
+    tile_read<G, B>(a0, buf, at[kUp].a[1], 0);
+    tile_read<G, B>(b1, buf, at[kUp].b[1], 0);
     i8_multiply(a1, b0, acc + G::H0);
-    i8_weave<G::H0 + G::TT, G::H1 * G::TT>();
-    i8_read<G, B>(a1, buf, at[kUp].a[1], G::H0);
+    tile_weave<G::H0 + G::TT, G::H1 * G::TT>();
+    tile_read<G, B>(a1, buf, at[kUp].a[1], G::H0);
     i8_multiply(a0, b1, acc);
-    i8_weave<G::H1, G::H0 * G::TT>();
+    tile_weave<G::H1, G::H0 * G::TT>();
     if constexpr (FULL) {
         i8_turn<G, G::kRing - 2>();
         i8_ask<G>(src, buf, wave, false);
@@ -638,11 +610,11 @@ __device__ __forceinline__ void i8_step(I8Src<G> &src, uint8_t *__restrict__ buf
         else if (left == 1 && tail < 8) i8_zero_past<G>(next, tail);
     }
     if (FULL || left > 0) {
-        i8_read<G, kNext>(a0, next, at[kNextUp].a[0], 0);
-        i8_read<G, kNext>(b0, next, at[kNextUp].b[0], 0);
+        tile_read<G, kNext>(a0, next, at[kNextUp].a[0], 0);
+        tile_read<G, kNext>(b0, next, at[kNextUp].b[0], 0);
     }
     i8_multiply(a1, b1, acc + G::H0);
-    if constexpr (FULL) i8_weave<G::H0 + G::TT, G::H1 * G::TT>();
+    if constexpr (FULL) tile_weave<G::H0 + G::TT, G::H1 * G::TT>();
 }
 
 // The same with a whole step's pieces in registers, f for the present step and g for the next: where a part has few products, a step would be four
@@ -652,16 +624,16 @@ struct I8Whole {
     v4i a[2][G::TR], b[2][G::TT];
 };
 template <class G, int B>
-__device__ __forceinline__ void i8_read_whole(I8Whole<G> &f, const uint8_t *__restrict__ buf, const I8At (&at)[2]) {
+__device__ __forceinline__ void i8_read_whole(I8Whole<G> &f, const uint8_t *__restrict__ buf, const TileAt (&at)[2]) {
 #pragma unroll
     for (int c = 0; c < 2; c++) {
-        i8_read<G, B>(f.a[c], buf, at[B >= G::kUp].a[c], 0);
-        i8_read<G, B>(f.b[c], buf, at[B >= G::kUp].b[c], 0);
+        tile_read<G, B>(f.a[c], buf, at[B >= G::kUp].a[c], 0);
+        tile_read<G, B>(f.b[c], buf, at[B >= G::kUp].b[c], 0);
     }
 }
 template <class G, int B, bool FULL>
 __device__ __forceinline__ void i8_step_whole(I8Src<G> &src, uint8_t *__restrict__ buf, uint8_t *__restrict__ next, u32 wave, u32 left, u32 tail,
-                                              const I8At (&at)[2], const I8Whole<G> &f, I8Whole<G> &g, v4i (&acc)[G::TR][G::TT]) {
+                                              const TileAt (&at)[2], const I8Whole<G> &f, I8Whole<G> &g, v4i (&acc)[G::TR][G::TT]) {
     if constexpr (FULL) {
         i8_turn<G, G::kRing - 2>();
         i8_ask<G>(src, buf, wave, false);
@@ -675,13 +647,6 @@ __device__ __forceinline__ void i8_step_whole(I8Src<G> &src, uint8_t *__restrict
     if (FULL || left > 0) i8_read_whole<G, (B + 1) % G::kRing>(g, next, at);
 #pragma unroll
     for (int c = 0; c < 2; c++) i8_multiply(f.a[c], f.b[c], acc);
-}
-
-// Where piece p of column c lies in a line of LINE pieces: turned by the column within the pieces' largest power of two.
-template <int LINE>
-__device__ __forceinline__ u32 i8_turned(u32 p, u32 c) {
-    constexpr u32 kPow = LINE & -LINE;
-    return p ^ (c & (kPow - 1));
 }
 
 // A wave's sums as values. The matrix instruction leaves column l % 16, rows 4 (l / 16) .. + 3 of a 16 x 16 tile in lane l; the sums go through LDS
@@ -713,7 +678,7 @@ __device__ __forceinline__ void i8_tile_out(const I8Args &a, const I8Run &run, u
             const u32 t = 16 * jj + (lane & 15);
 #pragma unroll
             for (int i = 0; i < G::TR; i++)
-                *reinterpret_cast<v4i *>(lds + 16 * (t * kLine + i8_turned<kLine>(4 * i + (lane >> 4), t))) = acc[i][j + jj];
+                *reinterpret_cast<v4i *>(lds + 16 * (t * kLine + tile_turned<kLine>(4 * i + (lane >> 4), t))) = acc[i][j + jj];
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
@@ -724,7 +689,7 @@ __device__ __forceinline__ void i8_tile_out(const I8Args &a, const I8Run &run, u
             float v[kValues];
 #pragma unroll
             for (int p = 0; p < kPiecesOut; p++) {
-                const v4i sum = *reinterpret_cast<const v4i *>(lds + 16 * (c * kLine + i8_turned<kLine>(first + p, c)));
+                const v4i sum = *reinterpret_cast<const v4i *>(lds + 16 * (c * kLine + tile_turned<kLine>(first + p, c)));
 #pragma unroll
                 for (int x = 0; x < 4; x++) v[4 * p + x] = __fmul_rn(__fmul_rn((float)sum[x], s), r[4 * p + x]);
             }
@@ -778,7 +743,7 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     for (int r = 0; r < G::RT; r++) src.col[r] = (a.order ? col[r] : col[r] - t0) * a.kp + 16 * ((lane & 7) ^ line_swizzle((wave * G::RT + r) * 8 + (lane >> 3)));
 #pragma unroll
     for (int r = 0; r < G::RR; r++) {
-        const u32 line = i8_row_group<G>(wave, r) * 8 + (lane >> 3);
+        const u32 line = tile_row_group<G>(wave, r) * 8 + (lane >> 3);
         src.row[r] = (min(r0 + line, a.rows - 1) - r0) * a.kp + 16 * ((lane & 7) ^ line_swizzle(line));
     }
 #pragma unroll
@@ -793,7 +758,7 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
 #pragma unroll
         for (int j = 0; j < G::TT; j++) acc[i][j] = v4i{0, 0, 0, 0};
     const u32 wt = (wave % WT) * (BT / WT), wr = BT + (wave / WT) * (BR / WR); // this wave's first lines
-    I8At at[2];
+    TileAt at[2];
 #pragma unroll
     for (u32 c = 0; c < 2; c++) {
         const u32 piece = (lane & 15) * 128 + 16 * ((4 * c + (lane >> 4)) ^ line_swizzle(lane & 15));
@@ -848,8 +813,8 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     } else {
         static_assert(WHOLE || S == 2, "parts of a step in a ring of two");
         v4i a0[G::H0], b0[G::TT];
-        i8_read<G, 0>(a0, ring0, at[0].a[0], 0);
-        i8_read<G, 0>(b0, ring0, at[0].b[0], 0);
+        tile_read<G, 0>(a0, ring0, at[0].a[0], 0);
+        tile_read<G, 0>(b0, ring0, at[0].b[0], 0);
         for (; left >= 4; left -= 2) {
             i8_step<G, 0, true>(src, ring0, ring1, wave, 0, 0, at, a0, b0, acc);
             i8_step<G, 1, true>(src, ring1, ring0, wave, 0, 0, at, a0, b0, acc);

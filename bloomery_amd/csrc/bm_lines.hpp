@@ -152,6 +152,45 @@ __device__ __forceinline__ bool run_tile(const A &a, u32 tile, bool check, u32 &
     return found;
 }
 
+// ---- tiles of columns and rows. G: a tile's kColumns, kRows, kWaves, kStage, RR (a wave's loads of rows a step) and kUp.
+
+// The eight rows of a wave's r-th load: where there are not as many for every wave, the last ones are asked for again.
+template <class G>
+__device__ __forceinline__ u32 tile_row_group(u32 wave, int r) {
+    const u32 group = wave * G::RR + r;
+    return G::kRows % (8 * G::kWaves) == 0 ? group : min(group, (u32)G::kRows / 8 - 1);
+}
+
+// Where a lane's reads begin, for each 64 bytes of a step: of rows and of columns. The upper buffers' carry the first one's place with them
+// (and are read that far in front), so that a read's address is one register and a constant that its instruction can hold.
+struct TileAt {
+    u32 a[2], b[2];
+};
+// What the matrix instructions take of 64 bytes of k of N tiles, from the FIRST on.
+template <class G, int B, int N>
+__device__ __forceinline__ void tile_read(v4i (&f)[N], const uint8_t *__restrict__ buf, u32 at, int first) {
+    constexpr u32 up = B >= G::kUp ? (u32)G::kUp * G::kStage : 0u;
+#pragma unroll
+    for (int i = 0; i < N; i++) f[i] = *reinterpret_cast<const v4i *>(buf + (int)(at - up + (first + i) * 2048));
+}
+
+// READS of what comes next between MFMAS products of what is there.
+template <int READS, int MFMAS>
+__device__ __forceinline__ void tile_weave() {
+#pragma unroll
+    for (int i = 0; i < READS; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);              // an LDS read
+        __builtin_amdgcn_sched_group_barrier(0x008, MFMAS / READS ? MFMAS / READS : 1, 0); // products
+    }
+}
+
+// Where piece p of column c lies in a line of LINE pieces: turned by the column within the pieces' largest power of two.
+template <int LINE>
+__device__ __forceinline__ u32 tile_turned(u32 p, u32 c) {
+    constexpr u32 kPow = LINE & -LINE;
+    return p ^ (c & (kPow - 1));
+}
+
 } // namespace bmk
 
 #endif // BM_LINES_HPP
