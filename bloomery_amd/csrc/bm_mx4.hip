@@ -11,6 +11,8 @@
 // A row of codes is 16 bytes a block, a row of scales one, rounded up to 16.
 #include "bm_lines.hpp"
 
+#include <algorithm>
+
 namespace bmk {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
@@ -39,6 +41,24 @@ __device__ __forceinline__ u32 quad_max(u32 v) {
     return max(v, quad_swap<0x4e>(v));
 }
 
+// Eight values of a block that four neighbouring lanes hold: their codes, and the block's scale. The largest magnitude's biased exponent less 2 is the scale's
+// byte; the conversion takes that byte as an exponent's bits, 0 for 2^-127, divides exactly, rounds to the nearest code, halves to even, and holds to 6.
+__device__ __forceinline__ u32 mx4_block(const float (&v)[8], u32 &scale) {
+    u32 most = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) most = max(most, bm_f32_bits(v[j]) & 0x7fffffffu);
+    most = quad_max(most) >> 23;
+    const bool bad = most == 255;
+    scale = bad ? 255 : most > 2 ? most - 2 : 0;
+    const float s = bm_bits_f32(scale << 23);
+    u32 word = 0;
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[0], v[1], s, 0);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[2], v[3], s, 1);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[4], v[5], s, 2);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[6], v[7], s, 3);
+    return bad ? 0u : word;
+}
+
 // A wave takes sixteen blocks of a row, sixteen bytes of its scales: a lane eight values, four lanes a block.
 template <int ET, bool GLU>
 __global__ __launch_bounds__(256) void k_mx4_quantize(Mx4Rows a) {
@@ -64,24 +84,13 @@ __global__ __launch_bounds__(256) void k_mx4_quantize(Mx4Rows a) {
         }
     }
     if (GLU && odd) bm_raise(a.fault, a.layer, kSiteF32Product);
-    u32 most = 0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) most = max(most, bm_f32_bits(v[j]) & 0x7fffffffu);
-    most = quad_max(most) >> 23; // biased exponent
-    const bool bad = most == 255;
-    const u32 scale = bad ? 255 : most > 2 ? most - 2 : 0;
+    u32 scale;
+    const u32 word = mx4_block(v, scale);
     if ((lane & 3) == 0) {
         a.scales[(size_t)row * a.ks + block] = (uint8_t)scale;
-        if (bad) bm_raise(a.fault, a.layer, kSiteQuantColumn);
+        if (scale == 255) bm_raise(a.fault, a.layer, kSiteQuantColumn);
     }
-    if (16 * block >= a.kp) return;
-    u32 word = 0;
-    const float s = bm_bits_f32(scale << 23); // the conversion takes the exponent's bits, 0 for 2^-127
-    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[0], v[1], s, 0);
-    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[2], v[3], s, 1);
-    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[4], v[5], s, 2);
-    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[6], v[7], s, 3);
-    *reinterpret_cast<u32 *>(a.codes + (size_t)row * a.kp + c / 2) = bad ? 0u : word;
+    if (16 * block < a.kp) *reinterpret_cast<u32 *>(a.codes + (size_t)row * a.kp + c / 2) = word;
 }
 
 // Eight codes as values.
@@ -162,57 +171,776 @@ __device__ __forceinline__ bool mx4_run(const Mx4Args &a, u32 e, Mx4Run &r) {
     return j1 > j0;
 }
 
-// Sixteen rows by sixteen columns, 128 values of k: lane l holds a block of row (column) l % 16, four blocks in turn, and its scale in the
-// lowest byte; it gets column l % 16, rows 4 (l / 16) .. + 3.
+// Sixteen rows by sixteen columns, 128 values of k: lane l holds a block of row (column) l % 16, four blocks in turn, and its scale in byte H of
+// a word; it gets column l % 16, rows 4 (l / 16) .. + 3. Of a 128-byte line, eight blocks, lane l takes blocks 2 (l / 16) and the next, one for each of two
+// instructions: their scales are two neighbouring bytes.
+template <int H>
 __device__ __forceinline__ v4f mx4_mfma(v4i w, v4i q, v4f acc, u32 ws, u32 qs) {
     const v8i a = {w[0], w[1], w[2], w[3], 0, 0, 0, 0}, b = {q[0], q[1], q[2], q[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, 0, (int)ws, 0, (int)qs);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, H, (int)ws, H, (int)qs);
+}
+// Two scales, 1 in the place of those from block `blocks` on, whose codes are zeros.
+__device__ __forceinline__ u32 mx4_scales(u32 two, u32 block, u32 blocks) {
+    return block + 1 < blocks ? two : block < blocks ? (two & 0xffu) | 0x7f00u : 0x7f7fu;
+}
+__device__ __forceinline__ u32 mx4_two(const uint8_t *p) { return *reinterpret_cast<const uint16_t *>(p); }
+// What the matrix instructions take of line group t (sixteen lines) of a stage: piece 2 (l / 16) + h of the lines.
+__device__ __forceinline__ v4i mx4_of_line(const uint8_t *stage, u32 lane, int t, int h) {
+    return *reinterpret_cast<const v4i *>(stage + t * 2048 + (lane & 15) * 128 + 16 * ((2 * (lane >> 4) + h) ^ line_swizzle(lane & 15)));
 }
 
-// A wave sixteen rows and sixteen columns, straight from memory.
-__global__ __launch_bounds__(256) void k_mx4_gemm(Mx4Args a) {
-    const u32 lane = threadIdx.x & 63, r0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 16, blocks = a.kp / 16;
-    Mx4Run run;
-    if (!mx4_run(a, blockIdx.y, run) || r0 >= a.rows) return;
-    const size_t row = min(r0 + (lane & 15), a.rows - 1);
-    for (u32 t0 = run.j0 + blockIdx.z * 16; t0 < run.j1; t0 += gridDim.z * 16) {
-        bool bad;
-        const size_t col = run_column(a, min(t0 + (lane & 15), run.j1 - 1), bad);
-        v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (u32 b0 = 0; b0 < blocks; b0 += 4) {
-            const u32 b = b0 + (lane >> 4);
-            v4i w = {0, 0, 0, 0}, q = {0, 0, 0, 0};
-            u32 ws = 127, qs = 127;
-            if (b < blocks) {
-                w = *reinterpret_cast<const v4i *>(run.w + row * a.kp + 16 * b);
-                q = *reinterpret_cast<const v4i *>(a.q + col * a.kp + 16 * b);
-                ws = run.ws[row * a.ks + b], qs = a.qs[col * a.ks + b];
-            }
-            acc = mx4_mfma(w, q, acc, ws, qs);
-        }
-        const u32 j = t0 + (lane & 15), r = r0 + 4 * (lane >> 4);
-        if (j >= run.j1 || r >= a.rows) continue;
-        if (bad) bm_raise(a.fault, a.layer, kSiteExpertId);
-        float v[4];
+// The sums of a tile's waves, in the waves' order, are a thread's outputs: four rows (4 (l / 16) ..) of one column.
+template <int NW, class L>
+__device__ __forceinline__ v4f mx4_join(const uint8_t *ring, u32 tile, u32 lane) {
+    v4f sum = *reinterpret_cast<const v4f *>(ring + tile * 1024 + 16 * lane);
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = bad ? bm_bits_f32(0x7fc00000u) : acc[i];
-        run_store4(a, j, r, v);
+    for (int w = 1; w < NW; w++) sum += *reinterpret_cast<const v4f *>(ring + w * L::kStage + tile * 1024 + 16 * lane);
+    return sum;
+}
+
+// Few columns a matrix: 16 R rows a workgroup against 16 C columns, its NW waves dealing the row's lines among them, each through a ring of four
+// stages of its own, two on their way while one is multiplied and the fourth is asked for; a line's scales come straight to registers, asked for with it. The
+// waves' sums meet in LDS.
+template <int R, int C, int NW>
+__global__ __launch_bounds__(64 * NW) void k_mx4_few(Mx4Args a) {
+    typedef Lines<2 * (R + C)> L;
+    constexpr int kLoads = 3 * (R + C); // of a stage: 2 (R + C) of lines, R + C of scales
+    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[NW * L::kStage], ring3[NW * L::kStage];
+    static_assert(R * C * 1024 <= L::kStage && R * C <= NW, "a wave's sums lie in its stage, one piece a thread");
+    const u32 lane = threadIdx.x & 63, wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Mx4Run run;
+    if (!mx4_run(a, blockIdx.y, run)) return;
+    const u32 r0 = blockIdx.x * (16 * R), lines = (a.kp + 127) / 128, mine = wave * L::kStage, blocks = a.kp / 16, at = 2 * (lane >> 4);
+    L src;
+    src.begin(lane);
+    const uint8_t *scales[R + C];
+#pragma unroll
+    for (u32 g = 0; g < 2 * R; g++) src.from[g] = (const int8_t *)run.w + (size_t)min(r0 + 8 * g + (lane >> 3), a.rows - 1) * a.kp; // rows past the last are not stored
+#pragma unroll
+    for (u32 r = 0; r < R; r++) scales[r] = run.ws + (size_t)min(r0 + 16 * r + (lane & 15), a.rows - 1) * a.ks + at;
+    for (u32 t0 = run.j0 + blockIdx.z * (16 * C); t0 < run.j1; t0 += gridDim.z * (16 * C)) {
+        u32 col[3 * C];
+#pragma unroll
+        for (u32 g = 0; g < 2 * C; g++) col[g] = min(t0 + 8 * g + (lane >> 3), run.j1 - 1);
+#pragma unroll
+        for (u32 c = 0; c < C; c++) col[2 * C + c] = min(t0 + 16 * c + (lane & 15), run.j1 - 1);
+        if (a.order) run_columns(a, col);
+#pragma unroll
+        for (u32 g = 0; g < 2 * C; g++) src.from[2 * R + g] = (const int8_t *)a.q + (size_t)col[g] * a.kp;
+#pragma unroll
+        for (u32 c = 0; c < C; c++) scales[R + c] = a.qs + (size_t)col[2 * C + c] * a.ks + at;
+        u32 s0[R + C], s1[R + C], s2[R + C], s3[R + C];
+        const auto ask = [&](uint8_t *stage, u32 (&s)[R + C], u32 l) {
+#pragma unroll
+            for (int i = 0; i < R + C; i++) s[i] = mx4_two(scales[i] + 8 * l);
+            __builtin_amdgcn_sched_barrier(0);
+            src.ask(stage + mine, l, a.kp);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if (wave < lines) ask(ring0, s0, wave);
+        if (wave + NW < lines) ask(ring1, s1, wave + NW);
+        if (wave + 2 * NW < lines) ask(ring2, s2, wave + 2 * NW);
+        v4f acc[R][C];
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int c = 0; c < C; c++) acc[r][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        const auto step = [&](const uint8_t *stage, u32 (&s)[R + C], uint8_t *free, u32 (&next)[R + C], u32 l) {
+            if (l + 2 * NW < lines) loads_landed<2 * kLoads>();
+            else if (l + NW < lines) loads_landed<kLoads>();
+            else loads_landed<0>();
+            v4i A[2][R], B[2][C];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int r = 0; r < R; r++) A[h][r] = mx4_of_line(stage + mine, lane, r, h);
+#pragma unroll
+                for (int c = 0; c < C; c++) B[h][c] = mx4_of_line(stage + mine, lane, R + c, h);
+            }
+            u32 two[R + C];
+#pragma unroll
+            for (int i = 0; i < R + C; i++) two[i] = mx4_scales(s[i], 8 * l + at, blocks);
+            if (l + 3 * NW < lines) ask(free, next, l + 3 * NW);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const bool in = 8 * l + at + h < blocks;
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    const v4i b = in ? B[h][c] : v4i{0, 0, 0, 0};
+#pragma unroll
+                    for (int r = 0; r < R; r++) acc[r][c] = h ? mx4_mfma<1>(A[h][r], b, acc[r][c], two[r], two[R + c]) : mx4_mfma<0>(A[h][r], b, acc[r][c], two[r], two[R + c]);
+                }
+            }
+        };
+        for (u32 l = wave; l < lines;) {
+            step(ring0, s0, ring3, s3, l);
+            if ((l += NW) >= lines) break;
+            step(ring1, s1, ring0, s0, l);
+            if ((l += NW) >= lines) break;
+            step(ring2, s2, ring1, s1, l);
+            if ((l += NW) >= lines) break;
+            step(ring3, s3, ring2, s2, l);
+            l += NW;
+        }
+        const u32 tile = wave, j = t0 + 16 * (tile % C) + (lane & 15), row = r0 + 16 * (tile / C) + 4 * (lane >> 4);
+        const bool out = tile < R * C && j < run.j1 && row < a.rows;
+        bool bad = false;
+        if (out) {
+            run_column(a, j, bad);
+            if (bad) bm_raise(a.fault, a.layer, kSiteExpertId);
+        }
+        loads_landed<0>();
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int c = 0; c < C; c++) *reinterpret_cast<v4f *>(ring0 + mine + (r * C + c) * 1024 + 16 * lane) = acc[r][c];
+        __syncthreads();
+        if (out) {
+            const v4f sum = mx4_join<NW, L>(ring0, tile, lane);
+            float v[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) v[x] = bad ? bm_bits_f32(0x7fc00000u) : sum[x];
+            run_store4(a, j, row, v);
+        }
+        __syncthreads();
     }
+}
+
+// A few rows from their floating values: k_mx4_few's product with the quantizer in front of it in every workgroup, while the first weights are on
+// their way. M (a power of two, at least the rows): the waves are dealt to the rows, 4 pieces of eight values a thread at most, four threads a
+// block. Codes and scales go to LDS; the first workgroup leaves them in memory too.
+constexpr int kMx4FewX = 8, kMx4FewXWaves = 8; // rows at most
+constexpr u32 mx4_few_x_values(u32 M) { return 64 * kMx4FewXWaves * 8 * 4 / M; } // values a row may have
+template <int ET, int M, int R>
+__global__ __launch_bounds__(64 * kMx4FewXWaves) void k_mx4_few_x(Mx4Args a, Mx4Rows qa) {
+    constexpr int NW = kMx4FewXWaves, T = 64 * NW / M, kPieces = 4, V = kElemPiece<ET>, P = 8 / V; // threads a row, pieces a thread, loads a piece
+    constexpr u32 kRow = mx4_few_x_values(M) / 2 + 16, kRowScales = mx4_few_x_values(M) / 32;      // a row's bytes in LDS, sixteen more for the banks
+    typedef Lines<2 * R> L;
+    constexpr int kLoads = 3 * R;
+    __shared__ __align__(16) uint8_t codes[M * kRow], marks[M * kRowScales];
+    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[NW * L::kStage], ring3[NW * L::kStage];
+    static_assert(R * 1024 <= L::kStage && R <= NW, "a wave's sums lie in its stage, one piece a thread");
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = (u32)__builtin_amdgcn_readfirstlane(tid >> 6);
+    const u32 lines = (a.kp + 127) / 128, r0 = blockIdx.x * (16 * R), mine = wave * L::kStage, blocks = a.kp / 16, at = 2 * (lane >> 4);
+    // the rows' values, then the first weights
+    const u32 row = tid / T, first = tid % T, pieces = a.kp / 4, whole = qa.k / 8;
+    const size_t from = (size_t)min(row, qa.m - 1) * qa.ld; // rows past the last are the last once more, and not multiplied
+    uint4 x[kPieces][P];
+#pragma unroll
+    for (int i = 0; i < kPieces; i++)
+#pragma unroll
+        for (int p = 0; p < P; p++) x[i][p] = elem_piece<ET>(qa.x, from + 8 * min(first + i * T, whole - 1) + p * V);
+    L src;
+    src.begin(lane);
+    const uint8_t *scales[R];
+#pragma unroll
+    for (u32 g = 0; g < 2 * R; g++) src.from[g] = (const int8_t *)a.w + (size_t)min(r0 + 8 * g + (lane >> 3), a.rows - 1) * a.kp; // rows past the last are not stored
+#pragma unroll
+    for (u32 r = 0; r < R; r++) scales[r] = a.ws + (size_t)min(r0 + 16 * r + (lane & 15), a.rows - 1) * a.ks + at;
+    u32 s0[R], s1[R], s2[R], s3[R];
+    const auto ask = [&](uint8_t *stage, u32 (&s)[R], u32 l) {
+#pragma unroll
+        for (int i = 0; i < R; i++) s[i] = mx4_two(scales[i] + 8 * l);
+        __builtin_amdgcn_sched_barrier(0);
+        src.ask(stage + mine, l, a.kp);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // three lines whether or not there are as many (then the last once more): the wait for the values leaves a known number of loads on their way
+    ask(ring0, s0, min(wave, lines - 1));
+    ask(ring1, s1, min(wave + NW, lines - 1));
+    ask(ring2, s2, min(wave + 2 * NW, lines - 1));
+    loads_landed<3 * kLoads>();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kPieces; i++) {
+        const u32 c = first + i * T;
+        if (c >= pieces) break; // (a block's four threads together)
+        float v[8];
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            float e[V];
+            elem_unpack<ET>(x[i][p], e);
+#pragma unroll
+            for (int j = 0; j < V; j++) v[p * V + j] = c < whole ? e[j] : 0.0f;
+        }
+        if (c == whole && (qa.k & 7)) elem_load_some<ET, 8>(qa.x, from + 8 * c, qa.k - 8 * c, v);
+        u32 scale;
+        const u32 word = mx4_block(v, scale);
+        const bool mark = (c & 3) == 0, leave = blockIdx.x == 0 && row < qa.m;
+        *reinterpret_cast<u32 *>(codes + row * kRow + 4 * c) = word;
+        if (mark) marks[row * kRowScales + c / 4] = (uint8_t)scale;
+        if (leave) *reinterpret_cast<u32 *>(qa.codes + (size_t)row * a.kp + 4 * c) = word;
+        if (leave && mark) {
+            qa.scales[(size_t)row * a.ks + c / 4] = (uint8_t)scale;
+            if (scale == 255) bm_raise(qa.fault, qa.layer, kSiteQuantColumn);
+        }
+    }
+    if (blockIdx.x == 0 && row < qa.m)
+        for (u32 b = blocks + first; b < a.ks; b += T) qa.scales[(size_t)row * a.ks + b] = 0;
+    lds_meet();
+
+    v4f acc[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) acc[r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    const u32 col = lane & 15;
+    const auto step = [&](const uint8_t *stage, u32 (&s)[R], uint8_t *free, u32 (&next)[R], u32 l) {
+        if (l + 2 * NW < lines) loads_landed<2 * kLoads>();
+        else if (l + NW < lines) loads_landed<kLoads>();
+        else loads_landed<0>();
+        v4i A[2][R], B[2];
+        u32 two[R], q = 0x7f7fu;
+        const u32 block = 8 * l + at;
+        if (col < (u32)M && block < blocks) q = mx4_scales(mx4_two(marks + col * kRowScales + block), block, blocks);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const bool in = col < (u32)M && block + h < blocks;
+            const v4i b = *reinterpret_cast<const v4i *>(codes + (in ? col * kRow + 16 * (block + h) : 0u));
+            B[h] = in ? b : v4i{0, 0, 0, 0};
+#pragma unroll
+            for (int r = 0; r < R; r++) A[h][r] = mx4_of_line(stage + mine, lane, r, h);
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++) two[r] = mx4_scales(s[r], block, blocks);
+        if (l + 3 * NW < lines) ask(free, next, l + 3 * NW);
+#pragma unroll
+        for (int r = 0; r < R; r++) acc[r] = mx4_mfma<0>(A[0][r], B[0], acc[r], two[r], q);
+#pragma unroll
+        for (int r = 0; r < R; r++) acc[r] = mx4_mfma<1>(A[1][r], B[1], acc[r], two[r], q);
+    };
+    for (u32 l = wave; l < lines;) {
+        step(ring0, s0, ring3, s3, l);
+        if ((l += NW) >= lines) break;
+        step(ring1, s1, ring0, s0, l);
+        if ((l += NW) >= lines) break;
+        step(ring2, s2, ring1, s1, l);
+        if ((l += NW) >= lines) break;
+        step(ring3, s3, ring2, s2, l);
+        l += NW;
+    }
+    const u32 out = r0 + 16 * wave + 4 * (lane >> 4);
+    loads_landed<0>();
+#pragma unroll
+    for (int r = 0; r < R; r++) *reinterpret_cast<v4f *>(ring0 + mine + r * 1024 + 16 * lane) = acc[r];
+    __syncthreads();
+    if (wave >= R || col >= a.m || out >= a.rows) return;
+    const v4f sum = mx4_join<NW, L>(ring0, wave, lane);
+    const float y[4] = {sum[0], sum[1], sum[2], sum[3]};
+    run_store4(a, col, out, y);
+}
+
+// Many columns a matrix: BT columns x BR rows a workgroup, 128 bytes of k a step and eight bytes of scales a column and a row through a ring of S LDS
+// buffers, where the loads put them themselves (16 and 4 bytes a lane, no register in between): while the waves multiply one step the next S - 1 are
+// on their way, one barrier a step. A wave holds (BT / WT) x (BR / WR) sums in v_mfma_scale_f32_16x16x128_f8f6f4's form.
+template <int BT, int BR, int WT, int WR, int S, bool WHOLE>
+struct Mx4Tile {
+    static constexpr bool kWhole = WHOLE;
+    static constexpr int kColumns = BT, kRows = BR, kLines = BT + BR, kRing = S, kWaves = WT * WR, kThreads = 64 * kWaves;
+    // a stage: the lines, then eight bytes of scales for each, which loads of 32 lines bring
+    static constexpr int kCodes = kLines * 128, kMarks = kLines / 32, kStage = kCodes + kMarks * 256;
+    // a wave's loads a step: eight lines each, of columns and of rows, and 32 lines' scales (the last waves may repeat some)
+    static constexpr int RT = BT / 8 / kWaves, RR = (BR / 8 + kWaves - 1) / kWaves, RS = (kMarks + kWaves - 1) / kWaves, kLoads = RT + RR + RS;
+    static constexpr int TT = BT / WT / 16, TR = BR / WR / 16, H0 = (TR + 1) / 2, H1 = TR / 2; // a wave's tiles of 16, its rows in two halves
+    static_assert(BT % (8 * kWaves) == 0 && BT % (16 * WT) == 0 && BR % (16 * WR) == 0 && TR > 1 && BT % 32 == 0 && BR % 32 == 0, "whole waves");
+    static_assert(S == 2 || (S == 4 && BR % (8 * kWaves) == 0), "where steps overlap, their loads are counted: as many for every wave");
+    // buffers from this one on lie past what a read's constant reaches
+    static constexpr int kUp = S * kStage <= 65536 ? S : S / 2;
+};
+
+// All but the last AHEAD steps that a wave asked for have landed, and every wave is done with the buffer that is written next.
+template <class G, int AHEAD>
+__device__ __forceinline__ void mx4_turn() {
+    constexpr int n = AHEAD * G::kLoads;
+    static_assert(n < 64, "vmcnt");
+    __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (n & 15) | (n >> 4) << 14); // vmcnt(n) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __asm__ volatile("" ::: "memory");
+}
+
+// Where a lane's loads begin: offsets of its lines' pieces from the tile's first column and row, and how far each goes back in the last step
+// where the rows end before the piece does (to the line's first piece, which is there; the columns' are zeroed in LDS); and of its scales.
+template <class G>
+struct Mx4Src {
+    const uint8_t *q, *w, *qs, *ws; // this step's
+    u32 col[G::RT], row[G::RR], mark[G::RS], back[2];
+};
+template <class G>
+__device__ __forceinline__ u32 mx4_mark_group(u32 wave, int r) {
+    const u32 group = wave * G::RS + r;
+    return G::kMarks % G::kWaves == 0 ? group : min(group, (u32)G::kMarks - 1);
+}
+template <class G>
+__device__ __forceinline__ void mx4_ask(Mx4Src<G> &s, uint8_t *buf, u32 wave, bool last) {
+#pragma unroll
+    for (int r = 0; r < G::RS; r++) {
+        const u32 group = mx4_mark_group<G>(wave, r);
+        const uint8_t *from = group < G::kColumns / 32 ? s.qs : s.ws;
+        __builtin_amdgcn_global_load_lds((lds_from *)(from + s.mark[r]), (lds_to *)(buf + G::kCodes + group * 256), 4, 0, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < G::RT; r++) {
+        const u32 group = wave * G::RT + r;
+        __builtin_amdgcn_global_load_lds((lds_from *)(s.q + (s.col[r] - (last ? s.back[group & 1] : 0u))), (lds_to *)(buf + group * 1024), 16, 0, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < G::RR; r++) {
+        const u32 group = tile_row_group<G>(wave, r);
+        __builtin_amdgcn_global_load_lds((lds_from *)(s.w + (s.row[r] - (last ? (group & 1 ? s.back[1] : s.back[0]) : 0u))),
+                                         (lds_to *)(buf + G::kColumns * 128 + group * 1024), 16, 0, 0);
+    }
+    s.q += 128;
+    s.w += 128;
+    s.qs += 8;
+    s.ws += 8;
+}
+// In a step that has landed, the columns' blocks from `have` on become zeros, and the scales there 1, the rows' too.
+template <class G>
+__device__ __forceinline__ void mx4_zero_past(uint8_t *buf, u32 have) {
+    for (u32 i = threadIdx.x; i < G::kColumns * 8; i += G::kThreads)
+        if (((i & 7) ^ line_swizzle(i >> 3)) >= have) *reinterpret_cast<uint4 *>(buf + 16 * i) = make_uint4(0, 0, 0, 0);
+    for (u32 i = threadIdx.x; i < G::kLines; i += G::kThreads)
+        for (u32 b = have; b < 8; b++) buf[G::kCodes + 8 * i + b] = 127;
+    __syncthreads();
+}
+
+// Two blocks' scales of N tiles, from the FIRST on.
+template <class G, int B, int N>
+__device__ __forceinline__ void mx4_read_marks(u32 (&f)[N], const uint8_t *__restrict__ buf, u32 at, int first) {
+    constexpr u32 up = B >= G::kUp ? (u32)G::kUp * G::kStage : 0u;
+#pragma unroll
+    for (int i = 0; i < N; i++) f[i] = mx4_two(buf + (int)(at - up + (first + i) * 128));
+}
+template <int H, int N, int TT>
+__device__ __forceinline__ void mx4_multiply(const v4i (&a)[N], const v4i (&b)[TT], const u32 (&sa)[N], const u32 (&sb)[TT], v4f (*acc)[TT]) {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < TT; j++) acc[i][j] = mx4_mfma<H>(a[i], b[j], acc[i][j], sa[i], sb[j]);
+}
+
+// Where a lane's reads begin: the lines' (TileAt) and the scales'.
+struct Mx4At : TileAt {
+    u32 sa, sb;
+};
+// What of a step stands in registers in front of it: the first half of the rows' first pieces, the columns', and their scales.
+template <class G>
+struct Mx4Head {
+    v4i a[G::H0], b[G::TT];
+    u32 sa[G::H0], sb[G::TT];
+};
+template <class G, int B>
+__device__ __forceinline__ void mx4_head(Mx4Head<G> &f, const uint8_t *__restrict__ buf, const Mx4At (&at)[2]) {
+    constexpr int up = B >= G::kUp;
+    tile_read<G, B>(f.a, buf, at[up].a[0], 0);
+    tile_read<G, B>(f.b, buf, at[up].b[0], 0);
+    mx4_read_marks<G, B>(f.sa, buf, at[up].sa, 0);
+    mx4_read_marks<G, B>(f.sb, buf, at[up].sb, 0);
+}
+
+// The turn to the next step and what is asked for behind it, common to both forms of a step.
+template <class G, bool FULL>
+__device__ __forceinline__ void mx4_next(Mx4Src<G> &src, uint8_t *buf, uint8_t *next, u32 wave, u32 left, u32 tail) {
+    if constexpr (FULL) {
+        mx4_turn<G, G::kRing - 2>();
+        mx4_ask<G>(src, buf, wave, false);
+    } else if (left > 0) {
+        if (G::kRing == 2 || left == 1) mx4_turn<G, 0>();
+        else if (left == 2) mx4_turn<G, G::kRing == 2 ? 0 : 1>();
+        else mx4_turn<G, G::kRing - 2>();
+        if (left >= (u32)G::kRing) mx4_ask<G>(src, buf, wave, left == (u32)G::kRing);
+        else if (left == 1 && tail < 8) mx4_zero_past<G>(next, tail);
+    }
+}
+
+// A step: its 128 bytes of k from buf in four parts - 64 bytes against half of the wave's rows each -, whose first part's pieces are in f
+// already; leaves the next step's there. A part's pieces are read under the products of the part before. That the two buffers are apart is
+// said by restrict: else the compiler waits for the loads into one in front of every read of the other. The turn comes before the last
+// part, so that the next step's reads and the loads of the one behind it go out under its products.
+// FULL: more steps are left behind this one than the ring holds, so that nothing is asked of where the rows end. B: buf's number.
+template <class G, int B, bool FULL>
+__device__ __forceinline__ void mx4_step(Mx4Src<G> &src, uint8_t *__restrict__ buf, uint8_t *__restrict__ next, u32 wave, u32 left, u32 tail,
+                                         const Mx4At (&at)[2], Mx4Head<G> &f, v4f (&acc)[G::TR][G::TT]) {
+    constexpr int up = B >= G::kUp;
+    v4i a1[G::H1], b1[G::TT];
+    u32 sa1[G::H1], sa[G::H0], sb[G::TT];
+#pragma unroll
+    for (int i = 0; i < G::H0; i++) sa[i] = f.sa[i];
+#pragma unroll
+    for (int i = 0; i < G::TT; i++) sb[i] = f.sb[i];
+    tile_read<G, B>(a1, buf, at[up].a[0], G::H0);
+    mx4_read_marks<G, B>(sa1, buf, at[up].sa, G::H0);
+    mx4_multiply<0>(f.a, f.b, sa, sb, acc);
+    tile_weave<2 * G::H1, G::H0 * G::TT>();
+    tile_read<G, B>(f.a, buf, at[up].a[1], 0);
+    tile_read<G, B>(b1, buf, at[up].b[1], 0);
+    mx4_multiply<0>(a1, f.b, sa1, sb, acc + G::H0);
+    tile_weave<G::H0 + G::TT, G::H1 * G::TT>();
+    tile_read<G, B>(a1, buf, at[up].a[1], G::H0);
+    mx4_multiply<1>(f.a, b1, sa, sb, acc);
+    tile_weave<G::H1, G::H0 * G::TT>();
+    mx4_next<G, FULL>(src, buf, next, wave, left, tail);
+    if (FULL || left > 0) mx4_head<G, (B + 1) % G::kRing>(f, next, at);
+    mx4_multiply<1>(a1, b1, sa1, sb, acc + G::H0);
+    if constexpr (FULL) tile_weave<2 * (G::H0 + G::TT), G::H1 * G::TT>();
+}
+
+// The same with a whole step's pieces in registers, f for the present step and g for the next: where a part has few products, a step would be four
+// waits for LDS and is one so.
+template <class G>
+struct Mx4Whole {
+    v4i a[2][G::TR], b[2][G::TT];
+    u32 sa[G::TR], sb[G::TT];
+};
+template <class G, int B>
+__device__ __forceinline__ void mx4_read_whole(Mx4Whole<G> &f, const uint8_t *__restrict__ buf, const Mx4At (&at)[2]) {
+    constexpr int up = B >= G::kUp;
+    mx4_read_marks<G, B>(f.sa, buf, at[up].sa, 0);
+    mx4_read_marks<G, B>(f.sb, buf, at[up].sb, 0);
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        tile_read<G, B>(f.a[c], buf, at[up].a[c], 0);
+        tile_read<G, B>(f.b[c], buf, at[up].b[c], 0);
+    }
+}
+template <class G, int B, bool FULL>
+__device__ __forceinline__ void mx4_step_whole(Mx4Src<G> &src, uint8_t *__restrict__ buf, uint8_t *__restrict__ next, u32 wave, u32 left, u32 tail,
+                                               const Mx4At (&at)[2], const Mx4Whole<G> &f, Mx4Whole<G> &g, v4f (&acc)[G::TR][G::TT]) {
+    mx4_next<G, FULL>(src, buf, next, wave, left, tail);
+    if (FULL || left > 0) mx4_read_whole<G, (B + 1) % G::kRing>(g, next, at);
+    mx4_multiply<0>(f.a[0], f.b[0], f.sa, f.sb, acc);
+    mx4_multiply<1>(f.a[1], f.b[1], f.sa, f.sb, acc);
+}
+
+// A wave's sums as values. The matrix instruction leaves column l % 16, rows 4 (l / 16) .. + 3 of a 16 x 16 tile in lane l; the sums go through LDS
+// (32 columns at a time, a wave's own part of it, four rows a piece, pieces turned by the column for the banks), so that a lane stores
+// sixteen bytes of a row of y and a row's lanes are neighbours.
+template <int ET, class G>
+__device__ __forceinline__ void mx4_tile_out(const Mx4Args &a, const Mx4Run &run, uint8_t *lds, u32 e0, u32 row0, const v4f (&acc)[G::TR][G::TT]) {
+    constexpr int kLine = G::TR * 4, kPiecesOut = ET == kElemF32 ? 1 : 2, kValues = 4 * kPiecesOut; // a column's pieces; a lane's pieces and values a store
+    constexpr int kBusy = kLine / kPiecesOut, kLanes = kBusy <= 8 ? 8 : kBusy <= 16 ? 16 : 32;        // a column's lanes: a power of two, the last ones idle
+    static_assert(kLine % kPiecesOut == 0 && kBusy <= kLanes, "whole lanes");
+    static_assert(G::TT % 2 == 0 && G::TT <= 4, "a lane a column, 32 at a time");
+    const u32 lane = threadIdx.x & 63;
+    bool bad = false;
+    if (a.order && lane < G::TT * 16 && e0 + lane < run.j1) {
+        run_column(a, e0 + lane, bad);
+        if (bad) bm_raise(a.fault, a.layer, kSiteExpertId);
+    }
+    const unsigned long long none = __ballot(bad);
+    const u32 first = lane % kLanes * kPiecesOut, row = row0 + 4 * first; // this lane's pieces of every column, and its rows
+    const bool mine = lane % kLanes < (u32)kBusy && row < a.rows;
+#pragma unroll
+    for (int j = 0; j < G::TT; j += 2) {
+#pragma unroll
+        for (int jj = 0; jj < 2; jj++) {
+            const u32 t = 16 * jj + (lane & 15);
+#pragma unroll
+            for (int i = 0; i < G::TR; i++)
+                *reinterpret_cast<v4f *>(lds + 16 * (t * kLine + tile_turned<kLine>(4 * i + (lane >> 4), t))) = acc[i][j + jj];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int n = 0; n < 32 * kLanes / 64; n++) {
+            const u32 c = n * (64 / kLanes) + lane / kLanes, e = e0 + 16 * j + c;
+            if (!mine || e >= run.j1) continue;
+            float v[kValues];
+#pragma unroll
+            for (int p = 0; p < kPiecesOut; p++) {
+                const v4f sum = *reinterpret_cast<const v4f *>(lds + 16 * (c * kLine + tile_turned<kLine>(first + p, c)));
+#pragma unroll
+                for (int x = 0; x < 4; x++) v[4 * p + x] = none >> (16 * j + c) & 1 ? bm_bits_f32(0x7fc00000u) : sum[x];
+            }
+            elem_store_some<ET, kValues>(a.y, (size_t)e * a.ld + row, a.rows - row, v);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
+template <int BT, int BR, int WT, int WR, int S, bool WHOLE, int EU>
+__global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU))) void k_mx4_tile(Mx4Args a, u32 n_row_tiles, u32 group) {
+    using G = Mx4Tile<BT, BR, WT, WR, S, WHOLE>;
+    // in this order: the larger alignment comes first
+    __shared__ __align__(4096) uint8_t ring0[G::kStage];
+    __shared__ __align__(2048) uint8_t ring1[G::kStage];
+    __shared__ __align__(1024) uint8_t ring2[S > 2 ? G::kStage : 16];
+    __shared__ __align__(512) uint8_t ring3[S > 2 ? G::kStage : 16];
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = (u32)__builtin_amdgcn_readfirstlane(tid >> 6);
+    // Workgroups go to the chip's eight dies in turn (b to die b % 8, each with its own L2). Neighbouring workgroups share a tile's columns across
+    // the dies, and a die's workgroups four of the rows' tiles and eight of the columns'. An expert with fewer tiles of rows than dies
+    // would so have its rows on every die: there (`group`) a group of its tiles of columns stays on one die, all rows of it.
+    const u32 block = group_index();
+    u32 expert = 0, t0, row_tile, tile;
+    if (group) {
+        const u32 i = block >> 3, per = group * n_row_tiles;
+        row_tile = i % per / group;
+        tile = (i / per * 8 + (block & 7)) * group + i % group;
+    } else {
+        row_tile = block % n_row_tiles;
+        tile = block / n_row_tiles;
+    }
+    if (!a.start) {
+        t0 = tile * BT;
+        if (t0 >= a.m) return;
+    } else if (!run_tile<BT>(a, tile, tile == 0 && row_tile == 0, expert, t0)) return;
+    const u32 r0 = row_tile * BR;
+    Mx4Run run;
+    if (!mx4_run(a, expert, run)) return;
+    t0 = (u32)__builtin_amdgcn_readfirstlane((int)(t0 + run.j0));
+    const u32 steps = (a.kp + 127) / 128, tail = (a.kp - (steps - 1) * 128) / 16; // blocks of the last step
+
+    // columns and rows past the last are the last ones again, and not stored
+    Mx4Src<G> src;
+    src.q = a.order ? a.q : a.q + (size_t)t0 * a.kp;
+    src.qs = a.order ? a.qs : a.qs + (size_t)t0 * a.ks;
+    src.w = run.w + (size_t)r0 * a.kp;
+    src.ws = run.ws + (size_t)r0 * a.ks;
+    u32 col[G::RT + G::RS];
+#pragma unroll
+    for (int r = 0; r < G::RT; r++) col[r] = min(t0 + (wave * G::RT + r) * 8 + (lane >> 3), run.j1 - 1);
+#pragma unroll
+    for (int r = 0; r < G::RS; r++) col[G::RT + r] = min(t0 + mx4_mark_group<G>(wave, r) * 32 + (lane >> 1), run.j1 - 1); // (of a group of rows: not used)
+    if (a.order) run_columns(a, col);
+    else
+#pragma unroll
+        for (int r = 0; r < G::RT + G::RS; r++) col[r] -= t0;
+#pragma unroll
+    for (int r = 0; r < G::RT; r++) src.col[r] = col[r] * a.kp + 16 * ((lane & 7) ^ line_swizzle((wave * G::RT + r) * 8 + (lane >> 3)));
+#pragma unroll
+    for (int r = 0; r < G::RR; r++) {
+        const u32 line = tile_row_group<G>(wave, r) * 8 + (lane >> 3);
+        src.row[r] = (min(r0 + line, a.rows - 1) - r0) * a.kp + 16 * ((lane & 7) ^ line_swizzle(line));
+    }
+#pragma unroll
+    for (int r = 0; r < G::RS; r++) {
+        const u32 line = mx4_mark_group<G>(wave, r) * 32 + (lane >> 1);
+        const u32 row = min(r0 + line - (u32)BT, a.rows - 1) - r0;
+        src.mark[r] = (line < (u32)BT ? col[G::RT + r] : row) * a.ks + 4 * (lane & 1);
+    }
+#pragma unroll
+    for (int r = 0; r < 2; r++) { // (a lane's piece differs between even and odd groups of eight lines only)
+        const u32 piece = (lane & 7) ^ line_swizzle(8 * r + (lane >> 3));
+        src.back[r] = piece >= tail ? 16 * piece : 0;
+    }
+
+    v4f acc[G::TR][G::TT];
+#pragma unroll
+    for (int i = 0; i < G::TR; i++)
+#pragma unroll
+        for (int j = 0; j < G::TT; j++) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    const u32 wt = (wave % WT) * (BT / WT), wr = BT + (wave / WT) * (BR / WR); // this wave's first lines
+    Mx4At at[2];
+#pragma unroll
+    for (u32 up = 0; up < 2; up++) {
+        const u32 more = up * G::kUp * G::kStage, mark = G::kCodes + (lane & 15) * 8 + 2 * (lane >> 4) + more;
+        at[up].sa = mark + wr * 8;
+        at[up].sb = mark + wt * 8;
+        __asm__("" : "+v"(at[up].sa), "+v"(at[up].sb)); // one register each from here on, whatever constants meet them
+#pragma unroll
+        for (u32 c = 0; c < 2; c++) {
+            const u32 piece = (lane & 15) * 128 + 16 * ((2 * (lane >> 4) + c) ^ line_swizzle(lane & 15)) + more;
+            at[up].a[c] = piece + wr * 128;
+            at[up].b[c] = piece + wt * 128;
+            __asm__("" : "+v"(at[up].a[c]), "+v"(at[up].b[c]));
+        }
+    }
+    mx4_ask<G>(src, ring0, wave, steps == 1);
+    if (steps > 1) mx4_ask<G>(src, ring1, wave, steps == 2);
+    if (S > 2 && steps > 2) mx4_ask<G>(src, ring2, wave, steps == 3);
+    if (S > 2 && steps > 3) mx4_ask<G>(src, ring3, wave, steps == 4);
+    if (steps >= (u32)S) mx4_turn<G, S - 1>();
+    else mx4_turn<G, 0>();
+    if (steps == 1 && tail < 8) mx4_zero_past<G>(ring0, tail);
+    u32 left = steps - 1;
+    if constexpr (WHOLE) {
+        // (rings of an even number of buffers: the two sets of registers change places with every step)
+        Mx4Whole<G> f, g;
+        mx4_read_whole<G, 0>(f, ring0, at);
+        if constexpr (S == 2) {
+            for (; left >= 4; left -= 2) {
+                mx4_step_whole<G, 0, true>(src, ring0, ring1, wave, 0, 0, at, f, g, acc);
+                mx4_step_whole<G, 1, true>(src, ring1, ring0, wave, 0, 0, at, g, f, acc);
+            }
+            for (;;) {
+                mx4_step_whole<G, 0, false>(src, ring0, ring1, wave, left, tail, at, f, g, acc);
+                if (left-- == 0) break;
+                mx4_step_whole<G, 1, false>(src, ring1, ring0, wave, left, tail, at, g, f, acc);
+                if (left-- == 0) break;
+            }
+        } else {
+            for (; left >= 8; left -= 4) {
+                mx4_step_whole<G, 0, true>(src, ring0, ring1, wave, 0, 0, at, f, g, acc);
+                mx4_step_whole<G, 1, true>(src, ring1, ring2, wave, 0, 0, at, g, f, acc);
+                mx4_step_whole<G, 2, true>(src, ring2, ring3, wave, 0, 0, at, f, g, acc);
+                mx4_step_whole<G, 3, true>(src, ring3, ring0, wave, 0, 0, at, g, f, acc);
+            }
+            for (;;) {
+                mx4_step_whole<G, 0, false>(src, ring0, ring1, wave, left, tail, at, f, g, acc);
+                if (left-- == 0) break;
+                mx4_step_whole<G, 1, false>(src, ring1, ring2, wave, left, tail, at, g, f, acc);
+                if (left-- == 0) break;
+                mx4_step_whole<G, 2, false>(src, ring2, ring3, wave, left, tail, at, f, g, acc);
+                if (left-- == 0) break;
+                mx4_step_whole<G, 3, false>(src, ring3, ring0, wave, left, tail, at, g, f, acc);
+                if (left-- == 0) break;
+            }
+        }
+    } else {
+        static_assert(WHOLE || S == 2, "parts of a step in a ring of two");
+        Mx4Head<G> f;
+        mx4_head<G, 0>(f, ring0, at);
+        for (; left >= 4; left -= 2) {
+            mx4_step<G, 0, true>(src, ring0, ring1, wave, 0, 0, at, f, acc);
+            mx4_step<G, 1, true>(src, ring1, ring0, wave, 0, 0, at, f, acc);
+        }
+        for (;;) {
+            mx4_step<G, 0, false>(src, ring0, ring1, wave, left, tail, at, f, acc);
+            if (left-- == 0) break;
+            mx4_step<G, 1, false>(src, ring1, ring0, wave, left, tail, at, f, acc);
+            if (left-- == 0) break;
+        }
+    }
+    __syncthreads(); // the buffers are the sums' from here
+    constexpr u32 kPart = G::TR * 2048, kEven = G::kStage / kPart; // a wave's part, and how many lie in the first buffer
+    static_assert(G::kWaves <= 2 * kEven, "every part lies in one buffer");
+    uint8_t *part = wave < kEven ? ring0 + wave * kPart : ring1 + (wave - kEven) * kPart;
+    if (a.et == kElemF32) mx4_tile_out<kElemF32, G>(a, run, part, t0 + wt, r0 + (wr - BT), acc);
+    else if (a.et == kElemF16) mx4_tile_out<kElemF16, G>(a, run, part, t0 + wt, r0 + (wr - BT), acc);
+    else mx4_tile_out<kElemBF16, G>(a, run, part, t0 + wt, r0 + (wr - BT), acc);
+}
+
+template <int BT, int BR, int WT, int WR, int S, bool WHOLE, int EU>
+static hipError_t mx4_tile_launch(const Launch &L, const Mx4Args &a, u32 entries) {
+    const u32 row_tiles = (a.rows + BR - 1) / BR;
+    u32 tiles = (entries + BT - 1) / BT;
+    if (a.start) tiles = entries / BT + (a.n_experts < entries ? a.n_experts : entries); // at most a ragged tile an expert
+    const u32 group = a.start && row_tiles < 8 ? 2 : 0;
+    if (group) tiles = (tiles + 8 * group - 1) / (8 * group) * (8 * group);
+    hipLaunchKernelGGL((k_mx4_tile<BT, BR, WT, WR, S, WHOLE, EU>), group_grid((uint64_t)tiles * row_tiles, 64 * WT * WR), dim3(64 * WT * WR), 0, L.stream, a, row_tiles, group);
+    return hipGetLastError();
+}
+
+template <int R, int C, int NW>
+static hipError_t mx4_few_launch(const Launch &L, const Mx4Args &a, u32 entries) {
+    const u32 z = a.start ? 1u : (entries + 16 * C - 1) / (16 * C);
+    hipLaunchKernelGGL((k_mx4_few<R, C, NW>), dim3((a.rows + 16 * R - 1) / (16 * R), a.start ? a.n_experts : 1u, z < 65535u ? z : 65535u), dim3(64 * NW), 0,
+                       L.stream, a);
+    return hipGetLastError();
+}
+
+template <int ET, int M, int R>
+static void mx4_few_x_launch(const Launch &L, const Mx4Args &a, const Mx4Rows &q) {
+    hipLaunchKernelGGL((k_mx4_few_x<ET, M, R>), dim3((a.rows + 16 * R - 1) / (16 * R)), dim3(64 * kMx4FewXWaves), 0, L.stream, a, q);
+}
+template <int ET, int M>
+static void mx4_few_x_by_rows(const Launch &L, const Mx4Args &a, const Mx4Rows &q) {
+    if ((a.rows + 15) / 16 > 256) mx4_few_x_launch<ET, M, 2>(L, a, q);
+    else mx4_few_x_launch<ET, M, 1>(L, a, q);
+}
+template <int ET>
+static void mx4_few_x_by_columns(const Launch &L, const Mx4Args &a, const Mx4Rows &q) {
+    if (a.m == 1) mx4_few_x_by_rows<ET, 1>(L, a, q);
+    else if (a.m == 2) mx4_few_x_by_rows<ET, 2>(L, a, q);
+    else if (a.m <= 4) mx4_few_x_by_rows<ET, 4>(L, a, q);
+    else mx4_few_x_by_rows<ET, 8>(L, a, q);
+}
+
+hipError_t mx4_gemm_x(const Launch &L, const uint8_t *w, const uint8_t *ws, int rows, int k, const void *x, int x_et, int64_t ld_x, int m, uint8_t *codes,
+                      uint8_t *scales, void *y, int et, int64_t ld) {
+    const u32 kp = (u32)mx4_row_bytes(k), ks = (u32)mx4_row_scales(k), M = m <= 1 ? 1 : m <= 2 ? 2 : m <= 4 ? 4 : 8;
+    if (m <= kMx4FewX && k >= 8 && 2 * kp <= mx4_few_x_values(M)) {
+        const Mx4Args a = {w, ws, (u32)rows, kp, ks, codes, scales, (u32)m, nullptr, nullptr, 0, 0, (u32)m, 1, y, (size_t)ld, et, L.fault, L.layer};
+        const Mx4Rows q = {x, nullptr, (size_t)ld_x, (u32)m, (u32)k, kp, ks, nullptr, codes, scales, L.rule, L.fault, L.layer};
+        if (x_et == kElemF32) mx4_few_x_by_columns<kElemF32>(L, a, q);
+        else if (x_et == kElemF16) mx4_few_x_by_columns<kElemF16>(L, a, q);
+        else mx4_few_x_by_columns<kElemBF16>(L, a, q);
+        return hipGetLastError();
+    }
+    const hipError_t e = mx4_quantize(L, x, nullptr, x_et, ld_x, m, k, nullptr, codes, scales);
+    return e != hipSuccess ? e : mx4_gemm(L, w, ws, 1, rows, k, codes, scales, m, nullptr, nullptr, 0, 0, y, et, ld);
+}
+
+// The forms, by what a workgroup has: columns x rows, its waves and its LDS buffers.
+enum Mx4Form : u32 {
+    kMx4Few16x16, // k_mx4_few: 16 x 16, waves sharing k
+    kMx4Few16x32,
+    kMx4Few16x32Three,
+    kMx4Few32x32,
+    kMx4Tile32x64Ring4, // k_mx4_tile, steps in a ring of four or two
+    kMx4Tile32x64,
+    kMx4Tile64x64Ring4,
+    kMx4Tile64x64,
+    kMx4Tile64x128,
+    kMx4Tile64x256,
+    kMx4Tile128x128,
+    kMx4Tile256x224,
+    kMx4Tile256x256,
+};
+
+// n_experts 0: one matrix, n its columns; else n slots. reach: the tiles' offsets of gathered columns, 32 bits, hold the columns.
+static Mx4Form mx4_form(u32 n_experts, u32 rows, u32 kp, u32 n, bool reach) {
+    const auto up = [](u32 x, u32 y) { return (x + y - 1) / y; };
+    const auto tiles = [&](u32 bt, u32 br) { return (uint64_t)up(n, bt) * up(rows, br); };
+    if (n_experts) {
+        if (n <= 32 || !reach) return kMx4Few16x32Three;
+        const u32 each = n / n_experts, runs = n < n_experts ? n : n_experts;
+        // 64 x 64 tiles: every run has one, and half a one more than its slots fill
+        const uint64_t small = (uint64_t)std::max(runs, n / 64 + runs / 2) * up(rows, 64);
+        if (each <= 16 && small <= 64) return kMx4Few32x32;
+        if (each < 24 && small <= 600) return kMx4Tile32x64Ring4;
+        if (each >= 24 && small <= 256) return kMx4Tile64x64Ring4;
+        if (each >= 24 && small <= 1024) return kMx4Tile64x64;
+        if (each >= 352) return kMx4Tile256x256;
+        if (each >= 144) return kMx4Tile128x128;
+        if (each >= 96 || (each >= 12 && (uint64_t)(n / 64 + n_experts / 2) * up(rows, 256) <= 512)) return kMx4Tile64x256;
+        return each >= 12 ? kMx4Tile64x128 : kMx4Tile32x64;
+    }
+    if (tiles(16, 16) <= 256) return kMx4Few16x16;
+    if (tiles(16, 32) <= 256) return kMx4Few16x32;
+    if (n <= 16) return kMx4Few16x32Three;
+    if (n <= 32 || tiles(32, 32) <= 256) return kMx4Few32x32;
+    if (tiles(32, 64) <= 256) return kMx4Tile32x64Ring4;
+    if (tiles(64, 64) <= 512 && kp > 1024) return kMx4Tile64x64Ring4;
+    if (tiles(64, 64) <= 768) return kMx4Tile64x64;
+    if (tiles(256, 256) >= 96) {
+        const uint64_t by256 = 64 * ((tiles(256, 256) + 255) / 256), by224 = 57 * ((tiles(256, 224) + 255) / 256), by128 = 39 * ((tiles(128, 128) + 511) / 512);
+        if (by256 <= by224 && by256 <= by128) return kMx4Tile256x256;
+        return by224 <= by128 ? kMx4Tile256x224 : kMx4Tile128x128;
+    }
+    return tiles(64, 128) <= 640 ? kMx4Tile64x128 : kMx4Tile128x128;
+}
+static bool mx4_reach(bool gathered, int n_cols, u32 kp) { return !gathered || (uint64_t)n_cols * kp <= 0xffffffffu; }
+
+int mx4_gemm_form(int n_experts, int rows, int k, int n_cols, int n_slots, int top_k) {
+    static const struct {
+        u32 columns, rows, waves, buffers;
+    } of[] = {{16, 16, 8, 4}, {16, 32, 4, 4}, {16, 32, 3, 4}, {32, 32, 4, 4}, {32, 64, 2, 4}, {32, 64, 2, 2}, {64, 64, 4, 4},
+              {64, 64, 4, 2}, {64, 128, 4, 2}, {64, 256, 4, 2}, {128, 128, 4, 2}, {256, 224, 8, 2}, {256, 256, 8, 2}};
+    const u32 kp = (u32)mx4_row_bytes(k);
+    const auto &f = of[mx4_form((u32)n_experts, (u32)rows, kp, (u32)(n_experts ? n_slots : n_cols), mx4_reach(n_experts && top_k > 0, n_cols, kp))];
+    return (int)(f.columns | f.rows << 10 | f.waves << 20 | f.buffers << 24);
 }
 
 hipError_t mx4_gemm(const Launch &L, const uint8_t *w, const uint8_t *ws, int n_experts, int rows, int k, const uint8_t *q, const uint8_t *qs, int n_cols,
                     const uint32_t *order, const uint32_t *start, int n_slots, int top_k, void *y, int et, int64_t ld) {
     const Mx4Args a = {w, ws, (u32)rows, (u32)mx4_row_bytes(k), (u32)mx4_row_scales(k), q, qs, (u32)n_cols, order, start, (u32)n_slots, (u32)top_k,
                        (u32)n_cols, (u32)n_experts, y, (size_t)ld, et, L.fault, L.layer};
-    const u32 z = start ? 1u : (a.m + 15) / 16;
-    hipLaunchKernelGGL(k_mx4_gemm, dim3((a.rows + 63) / 64, start ? a.n_experts : 1u, z < 65535u ? z : 65535u), dim3(256), 0, L.stream, a);
-    return hipGetLastError();
-}
-
-hipError_t mx4_gemm_x(const Launch &L, const uint8_t *w, const uint8_t *ws, int rows, int k, const void *x, int x_et, int64_t ld_x, int m, uint8_t *codes,
-                      uint8_t *scales, void *y, int et, int64_t ld) {
-    const hipError_t e = mx4_quantize(L, x, nullptr, x_et, ld_x, m, k, nullptr, codes, scales);
-    return e != hipSuccess ? e : mx4_gemm(L, w, ws, 1, rows, k, codes, scales, m, nullptr, nullptr, 0, 0, y, et, ld);
+    const u32 n = start ? (u32)n_slots : (u32)n_cols;
+    switch (mx4_form(start ? a.n_experts : 0, a.rows, a.kp, n, mx4_reach(order != nullptr, n_cols, a.kp))) {
+    case kMx4Few16x16: return mx4_few_launch<1, 1, 8>(L, a, n);
+    case kMx4Few16x32: return mx4_few_launch<2, 1, 4>(L, a, n);
+    case kMx4Few16x32Three: return mx4_few_launch<2, 1, 3>(L, a, n);
+    case kMx4Few32x32: return mx4_few_launch<2, 2, 4>(L, a, n);
+    case kMx4Tile32x64Ring4: return mx4_tile_launch<32, 64, 1, 2, 4, true, 2>(L, a, n);
+    case kMx4Tile32x64: return mx4_tile_launch<32, 64, 1, 2, 2, true, 2>(L, a, n);
+    case kMx4Tile64x64Ring4: return mx4_tile_launch<64, 64, 2, 2, 4, true, 2>(L, a, n);
+    case kMx4Tile64x64: return mx4_tile_launch<64, 64, 2, 2, 2, true, 2>(L, a, n);
+    case kMx4Tile64x128: return mx4_tile_launch<64, 128, 1, 4, 2, true, 2>(L, a, n);
+    case kMx4Tile64x256: return mx4_tile_launch<64, 256, 1, 4, 2, true, 2>(L, a, n);
+    case kMx4Tile128x128: return mx4_tile_launch<128, 128, 2, 2, 2, true, 2>(L, a, n);
+    case kMx4Tile256x224: return mx4_tile_launch<256, 224, 4, 2, 2, false, 2>(L, a, n);
+    case kMx4Tile256x256: return mx4_tile_launch<256, 256, 4, 2, 2, false, 2>(L, a, n);
+    }
+    return hipErrorInvalidValue;
 }
 
 // ------------------------------------------------------------------------------------ a few tokens' experts
