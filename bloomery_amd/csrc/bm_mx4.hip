@@ -945,6 +945,10 @@ hipError_t mx4_gemm(const Launch &L, const uint8_t *w, const uint8_t *ws, int n_
 
 // ------------------------------------------------------------------------------------ a few tokens' experts
 
+// Two launches. The first forms h: a workgroup an expert that is hit and 16 of its rows of gate and of up, for the tokens that picked it. The second forms y: a workgroup
+// 16 rows of down, for all tokens, over the experts that are hit. Weights are read once by each, as lines through rings in LDS, and bound both; codes
+// become bf16 values exactly, a few instructions for eight, and the products run on the bf16 matrix instructions, the tokens' values in parts that
+// add up to them: one of bf16, two of f16, three of f32, and of h two (f32: three).
 struct Mx4Moe {
     const uint8_t *wg, *wgs, *wu, *wus, *wd, *wds;
     u32 n_experts, hidden, ff, n_tokens, top_k;
@@ -952,79 +956,407 @@ struct Mx4Moe {
     size_t ld_x, ld_resid, ld_y;
     const u32 *sel;
     const float *w;
-    float *h; // a row of ff values a slot
+    __bf16 *h; // a slot's parts, rows of ff rounded up to 32 values
     void *y;
     GateRule rule;
     u32 *fault, layer;
 };
+constexpr u32 kMoeExperts = 1024, kMoeSlots = kMx4MoeTokens * 64;
+typedef __bf16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v2h __attribute__((ext_vector_type(2)));
 
-// A row's share of lane `lane` of a dot with the values that `load` gives for eight of k at a time.
-template <class F>
-__device__ __forceinline__ float mx4_dot(const uint8_t *row, const uint8_t *scales, u32 k, u32 lane, F load) {
-    float sum = 0.0f;
-    for (u32 c = 8 * lane; c < k; c += 512) {
-        float w[8], v[8];
-        mx4_values(*reinterpret_cast<const u32 *>(row + c / 2), scales[c / 32], w);
-        load(c, v);
+// The experts that the picks hit, as bits, and the picks; every thread of the workgroup takes part. An id that names no expert is 0xffff, and raised by
+// `raise`'s workgroup.
+struct MoePicks {
+    u32 bits[kMoeExperts / 32], before[kMoeExperts / 32]; // before: experts hit in the words in front
+    uint16_t sel[kMoeSlots];
+};
+template <int T>
+__device__ __forceinline__ void moe_picks(const Mx4Moe &a, MoePicks &p, bool raise) {
+    if (threadIdx.x < kMoeExperts / 32) p.bits[threadIdx.x] = 0;
+    __syncthreads();
+    for (u32 i = threadIdx.x; i < a.n_tokens * a.top_k; i += T) {
+        const u32 e = a.sel[i];
+        const bool in = e < a.n_experts;
+        p.sel[i] = in ? (uint16_t)e : (uint16_t)0xffff;
+        if (in) atomicOr(&p.bits[e >> 5], 1u << (e & 31));
+        else if (raise && e != 0xffffffffu) bm_raise(a.fault, a.layer, kSiteExpertId);
+    }
+    __syncthreads();
+}
+// Inclusive sums of the words' counts, lane i's word i (lanes past the words: all).
+__device__ __forceinline__ u32 moe_upto(const MoePicks &p, u32 lane, u32 &mine) {
+    mine = lane < kMoeExperts / 32 ? (u32)__builtin_popcount(p.bits[lane]) : 0u;
+    u32 upto = mine;
 #pragma unroll
-        for (int j = 0; j < 8; j++) sum = fmaf(w[j], v[j], sum);
+    for (int d = 1; d < 64; d <<= 1) {
+        const u32 o = (u32)__shfl_up((int)upto, d, 64);
+        if (lane >= (u32)d) upto += o;
     }
-    return wave_sum(sum);
+    return upto;
+}
+// The n-th expert that is hit; false: there are not as many.
+__device__ __forceinline__ bool moe_nth(const MoePicks &p, u32 n, u32 &expert) {
+    const u32 lane = threadIdx.x & 63;
+    u32 mine;
+    const u32 upto = moe_upto(p, lane, mine);
+    const unsigned long long here = __ballot(mine != 0 && upto - mine <= n && n < upto);
+    if (!here) return false;
+    const int word = __builtin_ctzll(here);
+    u32 skip = n - (u32)__shfl((int)(upto - mine), word, 64), w = p.bits[word];
+    for (; skip; skip--) w &= w - 1;
+    expert = (u32)__builtin_amdgcn_readfirstlane(32 * word + __builtin_ctz(w));
+    return true;
 }
 
-// A wave a slot's value of h.
-template <int ET>
-__global__ __launch_bounds__(256) void k_mx4_moe_up(Mx4Moe a) {
-    const u32 lane = threadIdx.x & 63, slot = blockIdx.y, f = blockIdx.x * 4 + (threadIdx.x >> 6), e = a.sel[slot];
-    if (e >= a.n_experts) {
-        if (e != 0xffffffffu && threadIdx.x == 0) bm_raise(a.fault, a.layer, kSiteExpertId);
-        return;
+// Eight codes as bf16 values under their scale.
+__device__ __forceinline__ v8h moe_codes(u32 word, float s) {
+    const v2h p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 1),
+              p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 3);
+    return v8h{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+}
+// The two halves of a lane's scales of a line as factors.
+__device__ __forceinline__ float moe_scale(u32 two, int h) { return bm_bits_f32((h ? two >> 8 : two & 0xffu) << 23); }
+
+__device__ __forceinline__ v8h moe_as_parts(uint4 p) {
+    v8h r;
+    __builtin_memcpy(&r, &p, 16);
+    return r;
+}
+// Eight values in P parts: what a part leaves is the next one's, the last rounded where something is left.
+template <int P>
+__device__ __forceinline__ void moe_split(const float (&x)[8], v8h (&part)[P]) {
+    float rest[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) rest[j] = x[j];
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+        if (p == P - 1) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) part[p][j] = (__bf16)rest[j];
+            break;
+        }
+        u32 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = __builtin_amdgcn_perm(bm_f32_bits(rest[2 * j + 1]), bm_f32_bits(rest[2 * j]), 0x07060302u);
+        part[p] = moe_as_parts(make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+        for (int j = 0; j < 8; j++) rest[j] = __fsub_rn(rest[j], bm_bits_f32(bm_f32_bits(rest[j]) & 0xffff0000u));
     }
-    if (f >= a.ff) return;
-    const u32 kp = (a.hidden + 31) / 32 * 16, ks = (a.hidden + 511) / 512 * 16;
-    const size_t row = (size_t)e * a.ff + f, x = (size_t)(slot / a.top_k) * a.ld_x;
-    const auto load = [&](u32 c, float (&v)[8]) { elem_load_some<ET, 8>(a.x, x + c, a.hidden - c, v); };
-    const float g = mx4_dot(a.wg + row * kp, a.wgs + row * ks, a.hidden, lane, load), u = mx4_dot(a.wu + row * kp, a.wus + row * ks, a.hidden, lane, load);
-    if (lane) return;
-    bool odd;
-    a.h[(size_t)slot * a.ff + f] = bm_gate_rule(a.rule.act, a.rule.limit, g, u, odd);
-    if (odd) bm_raise(a.fault, a.layer, kSiteF32Product);
+}
+template <int ET>
+constexpr int kMoeParts = ET == kElemBF16 ? 1 : ET == kElemF16 ? 2 : 3; // of an x
+template <int ET>
+constexpr int kMoeKept = ET == kElemF32 ? 3 : 2; // of an h
+
+// A lane's 64 values of a line of x, two blocks, eight at a time.
+template <int ET>
+struct MoeX {
+    static constexpr int V = kElemPiece<ET>, N = 8 / V;
+    uint4 raw[8][N];
+    __device__ __forceinline__ void ask(const void *x, size_t row, u32 first, u32 k) {
+        if (first + 64 <= k) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int n = 0; n < N; n++) raw[i][n] = elem_piece<ET>(x, row + first + 8 * i + n * V);
+        } else {
+            for (int i = 0; i < 8; i++) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = 0.0f;
+                if (first + 8 * i < k) elem_load_some<ET, 8>(x, row + first + 8 * i, k - first - 8 * i, v);
+#pragma unroll
+                for (int n = 0; n < N; n++) {
+                    float e[V];
+#pragma unroll
+                    for (int j = 0; j < V; j++) e[j] = v[n * V + j];
+                    const uint4 p = elem_pack<ET>(e);
+#pragma unroll
+                    for (int ii = 0; ii < 8; ii++)
+                        if (ii == i) raw[ii][n] = p;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void parts(int i, v8h (&part)[kMoeParts<ET>]) const {
+        if constexpr (ET == kElemBF16) {
+            part[0] = moe_as_parts(raw[i][0]);
+        } else {
+            float v[8];
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                float e[V];
+                elem_unpack<ET>(raw[i][n], e);
+#pragma unroll
+                for (int j = 0; j < V; j++) v[n * V + j] = e[j];
+            }
+            moe_split<kMoeParts<ET>>(v, part);
+        }
+    }
+};
+
+constexpr int kMoeUpWaves = 4;
+template <int ET>
+__global__ __launch_bounds__(64 * kMoeUpWaves) void k_mx4_moe_up(Mx4Moe a) {
+    constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, PH = kMoeKept<ET>, kLoads = 6; // of a stage: four of lines, two of scales
+    typedef Lines<4> L; // sixteen rows of gate, sixteen of up
+    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[NW * L::kStage], ring3[NW * L::kStage];
+    __shared__ MoePicks picks;
+    __shared__ u32 col_slot[16];
+    __shared__ float col_weight[16];
+    const u32 lane = threadIdx.x & 63, wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    moe_picks<64 * NW>(a, picks, blockIdx.x == 0 && blockIdx.y == 0);
+    u32 expert;
+    if (!moe_nth(picks, blockIdx.y, expert)) return;
+    // lane t: token t's first slot of this expert, and its weight, over all its slots of it
+    u32 slot = 0;
+    float weight = 0.0f;
+    bool user = false;
+    if (lane < a.n_tokens)
+        for (u32 s = a.top_k; s-- > 0;)
+            if (picks.sel[lane * a.top_k + s] == expert) {
+                slot = lane * a.top_k + s;
+                weight += a.w[slot];
+                user = true;
+            }
+    const unsigned long long users = __ballot(user);
+    const u32 n_users = (u32)__builtin_popcountll(users), place = (u32)__builtin_popcountll(users & ((1ull << lane) - 1));
+
+    const u32 kp = (a.hidden + 31) / 32 * 16, ks = (a.hidden + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage, at = 2 * (lane >> 4);
+    const u32 r0 = blockIdx.x * 16, ffp = (a.ff + 31) / 32 * 32;
+    L src;
+    src.begin(lane);
+    const size_t stack = (size_t)expert * a.ff;
+#pragma unroll
+    for (u32 g = 0; g < 4; g++) src.from[g] = (const int8_t *)(g < 2 ? a.wg : a.wu) + (stack + min(r0 + 8 * (g & 1) + (lane >> 3), a.ff - 1)) * kp;
+    const size_t mark = (stack + min(r0 + (lane & 15), a.ff - 1)) * ks + at;
+    const uint8_t *scales[2] = {a.wgs + mark, a.wus + mark};
+    for (u32 z = 0; z < n_users; z += 16) {
+        if (user && place - z < 16) {
+            col_slot[place - z] = slot;
+            col_weight[place - z] = weight;
+        }
+        __syncthreads();
+        const u32 my_slot = col_slot[min(lane & 15, min(n_users - z, 16u) - 1)]; // columns past the last are the last once more, and not stored
+        const size_t row = (size_t)(my_slot / a.top_k) * a.ld_x;
+        u32 s0[2], s1[2], s2[2], s3[2];
+        const auto ask = [&](uint8_t *stage, u32 (&s)[2], u32 l) {
+            s[0] = mx4_two(scales[0] + 8 * l);
+            s[1] = mx4_two(scales[1] + 8 * l);
+            __builtin_amdgcn_sched_barrier(0);
+            src.ask(stage + mine, l, kp);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if (wave < lines) ask(ring0, s0, wave);
+        if (wave + NW < lines) ask(ring1, s1, wave + NW);
+        if (wave + 2 * NW < lines) ask(ring2, s2, wave + 2 * NW);
+        v4f acc[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+        const auto step = [&](const uint8_t *stage, u32 (&s)[2], uint8_t *free, u32 (&next)[2], u32 l) {
+            MoeX<ET> x;
+            x.ask(a.x, row, 256 * l + 32 * at, a.hidden);
+            __builtin_amdgcn_sched_barrier(0);
+            if (l + 3 * NW < lines) ask(free, next, l + 3 * NW);
+            if (l + 3 * NW < lines) loads_landed<kLoads>();
+            else loads_landed<0>();
+            v4i w[2][2];
+            u32 two[2];
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                two[g] = mx4_scales(s[g], 8 * l + at, blocks);
+#pragma unroll
+                for (int h = 0; h < 2; h++) w[g][h] = mx4_of_line(stage + mine, lane, g, h);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                v8h part[P];
+                x.parts(i, part);
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    const v8h c = moe_codes((u32)w[g][i / 4][i % 4], moe_scale(two[g], i / 4));
+#pragma unroll
+                    for (int p = 0; p < P; p++) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(c, part[p], acc[g], 0, 0, 0);
+                }
+            }
+        };
+        for (u32 l = wave; l < lines;) {
+            step(ring0, s0, ring3, s3, l);
+            if ((l += NW) >= lines) break;
+            step(ring1, s1, ring0, s0, l);
+            if ((l += NW) >= lines) break;
+            step(ring2, s2, ring1, s1, l);
+            if ((l += NW) >= lines) break;
+            step(ring3, s3, ring2, s2, l);
+            l += NW;
+        }
+        loads_landed<0>();
+#pragma unroll
+        for (int g = 0; g < 2; g++) *reinterpret_cast<v4f *>(ring0 + mine + g * 1024 + 16 * lane) = acc[g];
+        __syncthreads();
+        const u32 c = lane & 15, f = r0 + 4 * (lane >> 4);
+        if (wave == 0 && z + c < n_users) {
+            const v4f g = mx4_join<NW, L>(ring0, 0, lane), u = mx4_join<NW, L>(ring0, 1, lane);
+            const float by = col_weight[c];
+            float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            bool odd = false;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                bool o = false;
+                if (f + j < a.ff) v[j] = __fmul_rn(bm_gate_rule(a.rule.act, a.rule.limit, g[j], u[j], o), by);
+                odd |= o;
+            }
+            if (odd) bm_raise(a.fault, a.layer, kSiteF32Product);
+            v8h part[PH];
+            moe_split<PH>(v, part);
+            __bf16 *to = a.h + (size_t)my_slot * PH * ffp + f;
+#pragma unroll
+            for (int p = 0; p < PH; p++) {
+                *reinterpret_cast<uint2 *>(to + (size_t)p * ffp) = *reinterpret_cast<const uint2 *>(&part[p]);
+                if (r0 + 16 >= a.ff && r0 + 16 < ffp) *reinterpret_cast<uint2 *>(to + (size_t)p * ffp + 16) = make_uint2(0, 0); // the last block's other half
+            }
+        }
+        __syncthreads();
+    }
 }
 
-// A wave a token's value of y.
-template <int ET>
-__global__ __launch_bounds__(256) void k_mx4_moe_down(Mx4Moe a) {
-    const u32 lane = threadIdx.x & 63, token = blockIdx.y, r = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= a.hidden) return;
-    const u32 kp = (a.ff + 31) / 32 * 16, ks = (a.ff + 511) / 512 * 16;
-    float sum = 0.0f;
-    for (u32 s = token * a.top_k; s < (token + 1) * a.top_k; s++) {
-        const u32 e = a.sel[s];
-        if (e >= a.n_experts) continue;
-        const size_t row = (size_t)e * a.hidden + r, h = (size_t)s * a.ff;
-        sum = fmaf(a.w[s], mx4_dot(a.wd + row * kp, a.wds + row * ks, a.ff, lane, [&](u32 c, float (&v)[8]) { elem_load_some<kElemF32, 8>(a.h, h + c, a.ff - c, v); }), sum);
+constexpr int kMoeDownWaves = 8;
+// NT tiles of sixteen tokens.
+template <int ET, int NT>
+__global__ __launch_bounds__(64 * kMoeDownWaves) void k_mx4_moe_down(Mx4Moe a) {
+    constexpr int NW = kMoeDownWaves, PH = kMoeKept<ET>, kLoads = 3; // of a stage: two of lines, one of scales
+    typedef Lines<2> L;
+    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[NW * L::kStage], ring3[NW * L::kStage];
+    __shared__ MoePicks picks;
+    __shared__ uint16_t list[kMoeExperts];
+    extern __shared__ __align__(16) uint8_t map[]; // by expert that is hit, a byte a token: which of its slots, 0xff for none
+    const u32 lane = threadIdx.x & 63, wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    moe_picks<64 * NW>(a, picks, false);
+    u32 mine_count;
+    const u32 upto = moe_upto(picks, lane, mine_count), n_hit = (u32)__builtin_amdgcn_readfirstlane(__shfl((int)upto, 63, 64));
+    if (wave == 0 && lane < kMoeExperts / 32) picks.before[lane] = upto - mine_count;
+    for (u32 i = threadIdx.x; i < n_hit * (4 * NT); i += 64 * NW) reinterpret_cast<u32 *>(map)[i] = 0xffffffffu;
+    __syncthreads();
+    const auto rank = [&](u32 e) { return picks.before[e >> 5] + (u32)__builtin_popcount(picks.bits[e >> 5] & ((1u << (e & 31)) - 1)); };
+    for (u32 e = threadIdx.x; e < a.n_experts; e += 64 * NW)
+        if (picks.bits[e >> 5] >> (e & 31) & 1) list[rank(e)] = (uint16_t)e;
+    if (threadIdx.x < a.n_tokens)
+        for (u32 s = a.top_k; s-- > 0;) {
+            const u32 e = picks.sel[threadIdx.x * a.top_k + s];
+            if (e != 0xffff) map[rank(e) * (16 * NT) + threadIdx.x] = (uint8_t)s;
+        }
+    __syncthreads();
+
+    const u32 kp = (a.ff + 31) / 32 * 16, ks = (a.ff + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage, at = 2 * (lane >> 4);
+    const u32 r0 = blockIdx.x * 16, ffp = (a.ff + 31) / 32 * 32, items = n_hit * lines;
+    L src;
+    src.begin(lane);
+    const size_t from[2] = {(size_t)min(r0 + (lane >> 3), a.hidden - 1) * kp, (size_t)min(r0 + 8 + (lane >> 3), a.hidden - 1) * kp};
+    const size_t mark = (size_t)min(r0 + (lane & 15), a.hidden - 1) * ks + at;
+    u32 s0, s1, s2, s3;
+    const auto ask = [&](uint8_t *stage, u32 &s, u32 q) {
+        const u32 n = q / lines, l = q - n * lines, e = (u32)__builtin_amdgcn_readfirstlane(list[n]);
+        s = mx4_two(a.wds + (size_t)e * a.hidden * ks + mark + 8 * l);
+#pragma unroll
+        for (int g = 0; g < 2; g++) src.from[g] = (const int8_t *)a.wd + (size_t)e * a.hidden * kp + from[g];
+        __builtin_amdgcn_sched_barrier(0);
+        src.ask(stage + mine, l, kp);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (wave < items) ask(ring0, s0, wave);
+    if (wave + NW < items) ask(ring1, s1, wave + NW);
+    if (wave + 2 * NW < items) ask(ring2, s2, wave + 2 * NW);
+    v4f acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    const auto step = [&](const uint8_t *stage, u32 &s, uint8_t *free, u32 &next, u32 q) {
+        const u32 n = q / lines, l = q - n * lines;
+        const auto values = [&](int t, v8h (&part)[8][PH]) { // a lane's 64 values of h, or zeros; whether the tile has any
+            const u32 token = 16 * t + (lane & 15), which = map[n * (16 * NT) + token], block = 8 * l + at;
+            const bool user = which != 0xff;
+            if (!__ballot(user)) return false;
+            const __bf16 *h = a.h + (size_t)(token * a.top_k + which) * PH * ffp + 32 * block;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int p = 0; p < PH; p++) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (user && block + i / 4 < blocks) v = *reinterpret_cast<const uint4 *>(h + (size_t)p * ffp + 8 * i);
+                    part[i][p] = moe_as_parts(v);
+                }
+            return true;
+        };
+        v8h part[8][PH];
+        bool any = values(0, part);
+        __builtin_amdgcn_sched_barrier(0);
+        if (q + 3 * NW < items) ask(free, next, q + 3 * NW);
+        if (q + 3 * NW < items) loads_landed<kLoads>();
+        else loads_landed<0>();
+        const u32 two = mx4_scales(s, 8 * l + at, blocks);
+        v4i w[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) w[h] = mx4_of_line(stage + mine, lane, 0, h);
+        v8h codes[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) codes[i] = moe_codes((u32)w[i / 4][i % 4], moe_scale(two, i / 4));
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if (t) any = values(t, part);
+            if (any)
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int p = 0; p < PH; p++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes[i], part[i][p], acc[t], 0, 0, 0);
+        }
+    };
+    for (u32 q = wave; q < items;) {
+        step(ring0, s0, ring3, s3, q);
+        if ((q += NW) >= items) break;
+        step(ring1, s1, ring0, s0, q);
+        if ((q += NW) >= items) break;
+        step(ring2, s2, ring1, s1, q);
+        if ((q += NW) >= items) break;
+        step(ring3, s3, ring2, s2, q);
+        q += NW;
     }
-    if (lane) return;
-    if (a.resid) sum = __fadd_rn(sum, elem_load1<ET>(a.resid, token * a.ld_resid + r));
-    elem_store1<ET>(a.y, token * a.ld_y + r, sum);
+    loads_landed<0>();
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        *reinterpret_cast<v4f *>(ring0 + mine + 16 * lane) = acc[t];
+        __syncthreads();
+        const u32 token = 16 * t + (lane & 15), r = r0 + 4 * (lane >> 4);
+        if (wave == 0 && token < a.n_tokens && r < a.hidden) {
+            const v4f sum = mx4_join<NW, L>(ring0, 0, lane);
+            float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+            const u32 have = a.hidden - r;
+            if (a.resid)
+#pragma unroll
+                for (u32 j = 0; j < 4; j++)
+                    if (j < have) v[j] = __fadd_rn(v[j], elem_load1<ET>(a.resid, token * a.ld_resid + r + j));
+            elem_store_some<ET, 4>(a.y, token * a.ld_y + r, have, v);
+        }
+        __syncthreads();
+    }
 }
 
 template <int ET>
 static hipError_t moe_launch(const Launch &L, const Mx4Moe &a) {
-    hipLaunchKernelGGL((k_mx4_moe_up<ET>), dim3((a.ff + 3) / 4, a.n_tokens * a.top_k), dim3(256), 0, L.stream, a);
+    const u32 slots = a.n_tokens * a.top_k, hits = slots < a.n_experts ? slots : a.n_experts;
+    hipLaunchKernelGGL((k_mx4_moe_up<ET>), dim3((a.ff + 15) / 16, hits), dim3(64 * kMoeUpWaves), 0, L.stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((k_mx4_moe_down<ET>), dim3((a.hidden + 3) / 4, a.n_tokens), dim3(256), 0, L.stream, a);
+    const dim3 grid((a.hidden + 15) / 16), threads(64 * kMoeDownWaves);
+    if (a.n_tokens <= 16) hipLaunchKernelGGL((k_mx4_moe_down<ET, 1>), grid, threads, hits * 16, L.stream, a);
+    else hipLaunchKernelGGL((k_mx4_moe_down<ET, 4>), grid, threads, hits * 64, L.stream, a);
     return hipGetLastError();
 }
 
-size_t mx4_moe_work(int n_tokens, int top_k, int, int ff) { return (size_t)n_tokens * top_k * ff * sizeof(float); }
+size_t mx4_moe_work(int n_tokens, int top_k, int, int ff) { return (size_t)n_tokens * top_k * 3 * ((ff + 31) / 32 * 32) * 2; }
 
 hipError_t mx4_moe(const Launch &L, const Mx4Stack &g, const Mx4Stack &u, const Mx4Stack &d, int n_experts, int hidden, int ff, const void *x, int et,
                    int64_t ld_x, int n_tokens, const uint32_t *sel, const float *w, int top_k, const void *resid, int64_t ld_resid, void *y, int64_t ld_y,
                    void *work) {
     const Mx4Moe a = {g.w, g.scales, u.w, u.scales, d.w, d.scales, (u32)n_experts, (u32)hidden, (u32)ff, (u32)n_tokens, (u32)top_k, x, resid, (size_t)ld_x,
-                      (size_t)ld_resid, (size_t)ld_y, sel, w, (float *)work, y, L.rule, L.fault, L.layer};
+                      (size_t)ld_resid, (size_t)ld_y, sel, w, (__bf16 *)work, y, L.rule, L.fault, L.layer};
     if (et == kElemF32) return moe_launch<kElemF32>(L, a);
     if (et == kElemF16) return moe_launch<kElemF16>(L, a);
     return moe_launch<kElemBF16>(L, a);
