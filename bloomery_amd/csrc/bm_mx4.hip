@@ -12,6 +12,7 @@
 #include "bm_lines.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace bmk {
 
@@ -428,188 +429,192 @@ __global__ __launch_bounds__(64 * kMx4FewXWaves) void k_mx4_few_x(Mx4Args a, Mx4
     run_store4(a, col, out, y);
 }
 
-// Many columns a matrix: BT columns x BR rows a workgroup, 128 bytes of k a step and eight bytes of scales a column and a row through a ring of S LDS
-// buffers, where the loads put them themselves (16 and 4 bytes a lane, no register in between): while the waves multiply one step the next S - 1 are
-// on their way, one barrier a step. A wave holds (BT / WT) x (BR / WR) sums in v_mfma_scale_f32_16x16x128_f8f6f4's form.
-template <int BT, int BR, int WT, int WR, int S, bool WHOLE>
+// Many columns a matrix: BT columns x BR rows a workgroup, 128 bytes of k a step through two LDS buffers, where the loads put them themselves (16 bytes a
+// lane, no register in between), and 32 bytes of scales a column and a row, four steps' worth, through two more: while the waves multiply one step
+// the next is on its way, one barrier a step. A wave holds (BT / WT) x (BR / WR) sums in v_mfma_scale_f32_16x16x128_f8f6f4's form; Q of its tiles of rows are a part
+// of a step (0: all).
+template <int BT, int BR, int WT, int WR, int Q>
 struct Mx4Tile {
-    static constexpr bool kWhole = WHOLE;
-    static constexpr int kColumns = BT, kRows = BR, kLines = BT + BR, kRing = S, kWaves = WT * WR, kThreads = 64 * kWaves;
-    // a stage: the lines, then eight bytes of scales for each, which loads of 32 lines bring
-    static constexpr int kCodes = kLines * 128, kMarks = kLines / 32, kStage = kCodes + kMarks * 256;
-    // a wave's loads a step: eight lines each, of columns and of rows, and 32 lines' scales (the last waves may repeat some)
-    static constexpr int RT = BT / 8 / kWaves, RR = (BR / 8 + kWaves - 1) / kWaves, RS = (kMarks + kWaves - 1) / kWaves, kLoads = RT + RR + RS;
-    static constexpr int TT = BT / WT / 16, TR = BR / WR / 16, H0 = (TR + 1) / 2, H1 = TR / 2; // a wave's tiles of 16, its rows in two halves
-    static_assert(BT % (8 * kWaves) == 0 && BT % (16 * WT) == 0 && BR % (16 * WR) == 0 && TR > 1 && BT % 32 == 0 && BR % 32 == 0, "whole waves");
-    static_assert(S == 2 || (S == 4 && BR % (8 * kWaves) == 0), "where steps overlap, their loads are counted: as many for every wave");
+    static constexpr int kColumns = BT, kRows = BR, kLines = BT + BR, kWaves = WT * WR, kThreads = 64 * kWaves, kStage = kLines * 128, kMarks = kLines * 32;
+    // a wave's loads: eight lines each, of columns and of rows, and 32 lines' scales every four steps (the last waves may repeat some)
+    static constexpr int RT = BT / 8 / kWaves, RR = (BR / 8 + kWaves - 1) / kWaves, RG = (kLines / 32 + kWaves - 1) / kWaves;
+    static constexpr int TT = BT / WT / 16, TR = BR / WR / 16, kPart = Q ? Q : TR; // a wave's tiles of 16
+    static_assert(BT % (8 * kWaves) == 0 && BT % (16 * WT) == 0 && BR % (16 * WR) == 0 && BT % 32 == 0 && BR % 32 == 0 && TR % kPart == 0, "whole waves and parts");
     // buffers from this one on lie past what a read's constant reaches
-    static constexpr int kUp = S * kStage <= 65536 ? S : S / 2;
+    static constexpr int kUp = 2 * kStage <= 65536 ? 2 : 1;
 };
 
-// All but the last AHEAD steps that a wave asked for have landed, and every wave is done with the buffer that is written next.
-template <class G, int AHEAD>
+// What a wave asked for has landed, and every wave is done with the buffer that is written next.
 __device__ __forceinline__ void mx4_turn() {
-    constexpr int n = AHEAD * G::kLoads;
-    static_assert(n < 64, "vmcnt");
     __asm__ volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070 | (n & 15) | (n >> 4) << 14); // vmcnt(n) lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt(0x0070); // vmcnt(0) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     __asm__ volatile("" ::: "memory");
 }
 
-// Where a lane's loads begin: offsets of its lines' pieces from the tile's first column and row, and how far each goes back in the last step
-// where the rows end before the piece does (to the line's first piece, which is there; the columns' are zeroed in LDS); and of its scales.
+// Where a tile's loads begin: its columns and rows and their scales as buffers that end where the matrices do - what lies past their ends comes as zeros,
+// so that a line may run on behind its row's end -, and a lane's offsets in them.
 template <class G>
 struct Mx4Src {
-    const uint8_t *q, *w, *qs, *ws; // this step's
-    u32 col[G::RT], row[G::RR], mark[G::RS], back[2];
+    const uint8_t *q, *w, *qs, *ws;
+    u32 q_end, w_end, qs_end, ws_end; // bytes
+    u32 at, mark_at;                  // this step's place in the lines, this group's in the scales
+    u32 col[G::RT], row[G::RR], mark[G::RG];
 };
-template <class G>
-__device__ __forceinline__ u32 mx4_mark_group(u32 wave, int r) {
-    const u32 group = wave * G::RS + r;
-    return G::kMarks % G::kWaves == 0 ? group : min(group, (u32)G::kMarks - 1);
+__device__ __forceinline__ u32 mx4_end(size_t bytes) { return bytes < 0xffffffffu ? (u32)bytes : 0xffffffffu; }
+__device__ __forceinline__ void mx4_load(const uint8_t *from, u32 end, uint8_t *to, u32 lane_at, u32 at) {
+    const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(from), 0, (int)end, 0x00027000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (lds_to *)to, 16, (int)lane_at, (int)at, 0, 0);
 }
 template <class G>
-__device__ __forceinline__ void mx4_ask(Mx4Src<G> &s, uint8_t *buf, u32 wave, bool last) {
+__device__ __forceinline__ u32 mx4_mark_group(u32 wave, int r) {
+    const u32 group = wave * G::RG + r;
+    return (G::kLines / 32) % G::kWaves == 0 ? group : min(group, (u32)G::kLines / 32 - 1);
+}
+template <class G>
+__device__ __forceinline__ void mx4_ask(Mx4Src<G> &s, uint8_t *buf, u32 wave) {
 #pragma unroll
-    for (int r = 0; r < G::RS; r++) {
+    for (int r = 0; r < G::RT; r++) mx4_load(s.q, s.q_end, buf + (wave * G::RT + r) * 1024, s.col[r], s.at);
+#pragma unroll
+    for (int r = 0; r < G::RR; r++) mx4_load(s.w, s.w_end, buf + G::kColumns * 128 + tile_row_group<G>(wave, r) * 1024, s.row[r], s.at);
+    s.at += 128;
+}
+// Four steps' scales.
+template <class G>
+__device__ __forceinline__ void mx4_ask_marks(Mx4Src<G> &s, uint8_t *marks, u32 wave) {
+#pragma unroll
+    for (int r = 0; r < G::RG; r++) {
         const u32 group = mx4_mark_group<G>(wave, r);
-        const uint8_t *from = group < G::kColumns / 32 ? s.qs : s.ws;
-        __builtin_amdgcn_global_load_lds((lds_from *)(from + s.mark[r]), (lds_to *)(buf + G::kCodes + group * 256), 4, 0, 0);
+        const bool columns = group < G::kColumns / 32;
+        mx4_load(columns ? s.qs : s.ws, columns ? s.qs_end : s.ws_end, marks + group * 1024, s.mark[r], s.mark_at);
     }
-#pragma unroll
-    for (int r = 0; r < G::RT; r++) {
-        const u32 group = wave * G::RT + r;
-        __builtin_amdgcn_global_load_lds((lds_from *)(s.q + (s.col[r] - (last ? s.back[group & 1] : 0u))), (lds_to *)(buf + group * 1024), 16, 0, 0);
-    }
-#pragma unroll
-    for (int r = 0; r < G::RR; r++) {
-        const u32 group = tile_row_group<G>(wave, r);
-        __builtin_amdgcn_global_load_lds((lds_from *)(s.w + (s.row[r] - (last ? (group & 1 ? s.back[1] : s.back[0]) : 0u))),
-                                         (lds_to *)(buf + G::kColumns * 128 + group * 1024), 16, 0, 0);
-    }
-    s.q += 128;
-    s.w += 128;
-    s.qs += 8;
-    s.ws += 8;
+    s.mark_at += 32;
 }
 // In a step that has landed, the columns' blocks from `have` on become zeros, and the scales there 1, the rows' too.
 template <class G>
-__device__ __forceinline__ void mx4_zero_past(uint8_t *buf, u32 have) {
+__device__ __forceinline__ void mx4_zero_past(uint8_t *buf, uint8_t *marks, u32 have) {
     for (u32 i = threadIdx.x; i < G::kColumns * 8; i += G::kThreads)
         if (((i & 7) ^ line_swizzle(i >> 3)) >= have) *reinterpret_cast<uint4 *>(buf + 16 * i) = make_uint4(0, 0, 0, 0);
     for (u32 i = threadIdx.x; i < G::kLines; i += G::kThreads)
-        for (u32 b = have; b < 8; b++) buf[G::kCodes + 8 * i + b] = 127;
+        for (u32 b = have; b < 8; b++) marks[32 * i + b] = 127;
     __syncthreads();
 }
 
-// Two blocks' scales of N tiles, from the FIRST on.
-template <class G, int B, int N>
-__device__ __forceinline__ void mx4_read_marks(u32 (&f)[N], const uint8_t *__restrict__ buf, u32 at, int first) {
-    constexpr u32 up = B >= G::kUp ? (u32)G::kUp * G::kStage : 0u;
+// Where a lane's reads begin: the lines' (TileAt, by buffer) and the scales'.
+struct Mx4At {
+    TileAt line[2];
+    u32 sa, sb;
+};
+// A step's scales: two blocks' of each of a wave's tiles.
+template <class G>
+struct Mx4Marks {
+    u32 a[G::TR], b[G::TT];
+    __device__ __forceinline__ void read(const uint8_t *__restrict__ marks, const Mx4At &at) {
 #pragma unroll
-    for (int i = 0; i < N; i++) f[i] = mx4_two(buf + (int)(at - up + (first + i) * 128));
-}
+        for (int j = 0; j < G::TT; j++) b[j] = mx4_two(marks + at.sb + j * 512);
+#pragma unroll
+        for (int i = 0; i < G::TR; i++) a[i] = mx4_two(marks + at.sa + i * 512);
+    }
+};
+// Where a step's scales lie: four steps' in one half, the next four's in the other.
+template <class G>
+__device__ __forceinline__ u32 mx4_mark_at(u32 step) { return (step >> 2 & 1) * G::kMarks + (step & 3) * 8; }
 template <int H, int N, int TT>
-__device__ __forceinline__ void mx4_multiply(const v4i (&a)[N], const v4i (&b)[TT], const u32 (&sa)[N], const u32 (&sb)[TT], v4f (*acc)[TT]) {
+__device__ __forceinline__ void mx4_multiply(const v4i (&a)[N], const v4i (&b)[TT], const u32 *sa, const u32 (&sb)[TT], v4f (*acc)[TT]) {
 #pragma unroll
     for (int i = 0; i < N; i++)
 #pragma unroll
         for (int j = 0; j < TT; j++) acc[i][j] = mx4_mfma<H>(a[i], b[j], acc[i][j], sa[i], sb[j]);
 }
 
-// Where a lane's reads begin: the lines' (TileAt) and the scales'.
-struct Mx4At : TileAt {
-    u32 sa, sb;
+// What a step does beside its products: between kFull, where the one behind the next is asked for, kNext, where there is none behind the next, which
+// is the last, and kLast, with none behind it. No branch stands in a step but in kNext: the compiler would carry the products past it.
+enum Mx4Steps { kFull, kNext, kLast };
+struct Mx4Way {
+    u32 step, tail, wave; // this step's number, and the blocks of the last one
 };
-// What of a step stands in registers in front of it: the first half of the rows' first pieces, the columns', and their scales.
+template <class G, Mx4Steps STEP, class F>
+__device__ __forceinline__ void mx4_next(Mx4Src<G> &src, uint8_t *buf, uint8_t *next, uint8_t *marks, const Mx4Way &way, F read) {
+    if constexpr (STEP == kLast) return;
+    mx4_turn();
+    if (STEP == kNext && way.tail < 8) mx4_zero_past<G>(next, marks + mx4_mark_at<G>(way.step + 1), way.tail);
+    read(marks + mx4_mark_at<G>(way.step + 1));
+    if (STEP == kNext) return;
+    mx4_ask<G>(src, buf, way.wave);
+}
+
+// A step in parts: Q of a wave's tiles of rows against 64 bytes of k each. The first part's pieces and the scales are in registers already, and
+// the next step's are left there. A part's pieces are read under the products of the part before. That the two buffers are apart is said by
+// restrict: else the compiler waits for the loads into one in front of every read of the other. The turn comes before the last part, so
+// that the next step's reads and the loads of the one behind it go out under its products. B: the buffer's number.
 template <class G>
-struct Mx4Head {
-    v4i a[G::H0], b[G::TT];
-    u32 sa[G::H0], sb[G::TT];
-};
-template <class G, int B>
-__device__ __forceinline__ void mx4_head(Mx4Head<G> &f, const uint8_t *__restrict__ buf, const Mx4At (&at)[2]) {
-    constexpr int up = B >= G::kUp;
-    tile_read<G, B>(f.a, buf, at[up].a[0], 0);
-    tile_read<G, B>(f.b, buf, at[up].b[0], 0);
-    mx4_read_marks<G, B>(f.sa, buf, at[up].sa, 0);
-    mx4_read_marks<G, B>(f.sb, buf, at[up].sb, 0);
-}
-
-// The turn to the next step and what is asked for behind it, common to both forms of a step.
-template <class G, bool FULL>
-__device__ __forceinline__ void mx4_next(Mx4Src<G> &src, uint8_t *buf, uint8_t *next, u32 wave, u32 left, u32 tail) {
-    if constexpr (FULL) {
-        mx4_turn<G, G::kRing - 2>();
-        mx4_ask<G>(src, buf, wave, false);
-    } else if (left > 0) {
-        if (G::kRing == 2 || left == 1) mx4_turn<G, 0>();
-        else if (left == 2) mx4_turn<G, G::kRing == 2 ? 0 : 1>();
-        else mx4_turn<G, G::kRing - 2>();
-        if (left >= (u32)G::kRing) mx4_ask<G>(src, buf, wave, left == (u32)G::kRing);
-        else if (left == 1 && tail < 8) mx4_zero_past<G>(next, tail);
+struct Mx4Parts {
+    v4i a[G::kPart], b[G::TT];
+    Mx4Marks<G> s;
+    template <int B>
+    __device__ __forceinline__ void begin(const uint8_t *buf, const uint8_t *marks, const Mx4At &at) {
+        constexpr int up = B >= G::kUp;
+        s.read(marks, at);
+        tile_read<G, B>(a, buf, at.line[up].a[0], 0);
+        tile_read<G, B>(b, buf, at.line[up].b[0], 0);
     }
-}
-
-// A step: its 128 bytes of k from buf in four parts - 64 bytes against half of the wave's rows each -, whose first part's pieces are in f
-// already; leaves the next step's there. A part's pieces are read under the products of the part before. That the two buffers are apart is
-// said by restrict: else the compiler waits for the loads into one in front of every read of the other. The turn comes before the last
-// part, so that the next step's reads and the loads of the one behind it go out under its products.
-// FULL: more steps are left behind this one than the ring holds, so that nothing is asked of where the rows end. B: buf's number.
-template <class G, int B, bool FULL>
-__device__ __forceinline__ void mx4_step(Mx4Src<G> &src, uint8_t *__restrict__ buf, uint8_t *__restrict__ next, u32 wave, u32 left, u32 tail,
-                                         const Mx4At (&at)[2], Mx4Head<G> &f, v4f (&acc)[G::TR][G::TT]) {
-    constexpr int up = B >= G::kUp;
-    v4i a1[G::H1], b1[G::TT];
-    u32 sa1[G::H1], sa[G::H0], sb[G::TT];
+    template <int B, Mx4Steps STEP>
+    __device__ __forceinline__ void step(Mx4Src<G> &src, uint8_t *__restrict__ buf, uint8_t *__restrict__ next, uint8_t *__restrict__ marks, Mx4Way &way,
+                                         const Mx4At &at, v4f (&acc)[G::TR][G::TT]) {
+        constexpr int Q = G::kPart, N = G::TR / Q, up = B >= G::kUp, nextUp = 1 - B >= G::kUp;
+        v4i part[2][Q], b1[G::TT];
 #pragma unroll
-    for (int i = 0; i < G::H0; i++) sa[i] = f.sa[i];
+        for (int i = 0; i < Q; i++) part[0][i] = a[i];
 #pragma unroll
-    for (int i = 0; i < G::TT; i++) sb[i] = f.sb[i];
-    tile_read<G, B>(a1, buf, at[up].a[0], G::H0);
-    mx4_read_marks<G, B>(sa1, buf, at[up].sa, G::H0);
-    mx4_multiply<0>(f.a, f.b, sa, sb, acc);
-    tile_weave<2 * G::H1, G::H0 * G::TT>();
-    tile_read<G, B>(f.a, buf, at[up].a[1], 0);
-    tile_read<G, B>(b1, buf, at[up].b[1], 0);
-    mx4_multiply<0>(a1, f.b, sa1, sb, acc + G::H0);
-    tile_weave<G::H0 + G::TT, G::H1 * G::TT>();
-    tile_read<G, B>(a1, buf, at[up].a[1], G::H0);
-    mx4_multiply<1>(f.a, b1, sa, sb, acc);
-    tile_weave<G::H1, G::H0 * G::TT>();
-    mx4_next<G, FULL>(src, buf, next, wave, left, tail);
-    if (FULL || left > 0) mx4_head<G, (B + 1) % G::kRing>(f, next, at);
-    mx4_multiply<1>(a1, b1, sa1, sb, acc + G::H0);
-    if constexpr (FULL) tile_weave<2 * (G::H0 + G::TT), G::H1 * G::TT>();
-}
+        for (int p = 0; p < 2 * N - 1; p++) {
+            tile_read<G, B>(part[(p + 1) & 1], buf, at.line[up].a[(p + 1) / N], (p + 1) % N * Q); // the next part's
+            if (p == N - 1) tile_read<G, B>(b1, buf, at.line[up].b[1], 0);
+            if (p < N) mx4_multiply<0>(part[p & 1], b, s.a + p % N * Q, s.b, acc + p % N * Q);
+            else mx4_multiply<1>(part[p & 1], b1, s.a + p % N * Q, s.b, acc + p % N * Q);
+            if (p == N - 1) tile_weave<Q + G::TT, Q * G::TT>();
+            else tile_weave<Q, Q * G::TT>();
+        }
+        const Mx4Marks<G> mine = s;
+        mx4_next<G, STEP>(src, buf, next, marks, way, [&](const uint8_t *m) {
+            s.read(m, at);
+            tile_read<G, 1 - B>(a, next, at.line[nextUp].a[0], 0);
+            tile_read<G, 1 - B>(b, next, at.line[nextUp].b[0], 0);
+        });
+        mx4_multiply<1>(part[1], b1, mine.a + (N - 1) * Q, mine.b, acc + (N - 1) * Q);
+        if constexpr (STEP == kFull) tile_weave<Q + 2 * G::TT + G::TR, Q * G::TT>();
+        way.step++;
+    }
+};
 
-// The same with a whole step's pieces in registers, f for the present step and g for the next: where a part has few products, a step would be four
+// The same with a whole step's pieces in registers, two sets that change places with every step: where a part has few products, a step would be many
 // waits for LDS and is one so.
 template <class G>
 struct Mx4Whole {
-    v4i a[2][G::TR], b[2][G::TT];
-    u32 sa[G::TR], sb[G::TT];
-};
-template <class G, int B>
-__device__ __forceinline__ void mx4_read_whole(Mx4Whole<G> &f, const uint8_t *__restrict__ buf, const Mx4At (&at)[2]) {
-    constexpr int up = B >= G::kUp;
-    mx4_read_marks<G, B>(f.sa, buf, at[up].sa, 0);
-    mx4_read_marks<G, B>(f.sb, buf, at[up].sb, 0);
+    struct Set {
+        v4i a[2][G::TR], b[2][G::TT];
+        Mx4Marks<G> s;
+    } set[2];
+    template <int B>
+    __device__ __forceinline__ void read(const uint8_t *__restrict__ buf, const uint8_t *__restrict__ marks, const Mx4At &at) {
+        constexpr int up = B >= G::kUp;
+        set[B].s.read(marks, at);
 #pragma unroll
-    for (int c = 0; c < 2; c++) {
-        tile_read<G, B>(f.a[c], buf, at[up].a[c], 0);
-        tile_read<G, B>(f.b[c], buf, at[up].b[c], 0);
+        for (int c = 0; c < 2; c++) {
+            tile_read<G, B>(set[B].a[c], buf, at.line[up].a[c], 0);
+            tile_read<G, B>(set[B].b[c], buf, at.line[up].b[c], 0);
+        }
     }
-}
-template <class G, int B, bool FULL>
-__device__ __forceinline__ void mx4_step_whole(Mx4Src<G> &src, uint8_t *__restrict__ buf, uint8_t *__restrict__ next, u32 wave, u32 left, u32 tail,
-                                               const Mx4At (&at)[2], const Mx4Whole<G> &f, Mx4Whole<G> &g, v4f (&acc)[G::TR][G::TT]) {
-    mx4_next<G, FULL>(src, buf, next, wave, left, tail);
-    if (FULL || left > 0) mx4_read_whole<G, (B + 1) % G::kRing>(g, next, at);
-    mx4_multiply<0>(f.a[0], f.b[0], f.sa, f.sb, acc);
-    mx4_multiply<1>(f.a[1], f.b[1], f.sa, f.sb, acc);
-}
+    template <int B>
+    __device__ __forceinline__ void begin(const uint8_t *buf, const uint8_t *marks, const Mx4At &at) { read<B>(buf, marks, at); }
+    template <int B, Mx4Steps STEP>
+    __device__ __forceinline__ void step(Mx4Src<G> &src, uint8_t *__restrict__ buf, uint8_t *__restrict__ next, uint8_t *__restrict__ marks, Mx4Way &way,
+                                         const Mx4At &at, v4f (&acc)[G::TR][G::TT]) {
+        mx4_next<G, STEP>(src, buf, next, marks, way, [&](const uint8_t *m) { read<1 - B>(next, m, at); });
+        mx4_multiply<0>(set[B].a[0], set[B].b[0], set[B].s.a, set[B].s.b, acc);
+        mx4_multiply<1>(set[B].a[1], set[B].b[1], set[B].s.a, set[B].s.b, acc);
+        way.step++;
+    }
+};
 
 // A wave's sums as values. The matrix instruction leaves column l % 16, rows 4 (l / 16) .. + 3 of a 16 x 16 tile in lane l; the sums go through LDS
 // (32 columns at a time, a wave's own part of it, four rows a piece, pieces turned by the column for the banks), so that a lane stores
@@ -656,14 +661,13 @@ __device__ __forceinline__ void mx4_tile_out(const Mx4Args &a, const Mx4Run &run
     }
 }
 
-template <int BT, int BR, int WT, int WR, int S, bool WHOLE, int EU>
+template <int BT, int BR, int WT, int WR, int Q, int EU>
 __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU))) void k_mx4_tile(Mx4Args a, u32 n_row_tiles, u32 group) {
-    using G = Mx4Tile<BT, BR, WT, WR, S, WHOLE>;
+    using G = Mx4Tile<BT, BR, WT, WR, Q>;
     // in this order: the larger alignment comes first
     __shared__ __align__(4096) uint8_t ring0[G::kStage];
     __shared__ __align__(2048) uint8_t ring1[G::kStage];
-    __shared__ __align__(1024) uint8_t ring2[S > 2 ? G::kStage : 16];
-    __shared__ __align__(512) uint8_t ring3[S > 2 ? G::kStage : 16];
+    __shared__ __align__(1024) uint8_t marks[2 * G::kMarks];
     const u32 tid = threadIdx.x, lane = tid & 63, wave = (u32)__builtin_amdgcn_readfirstlane(tid >> 6);
     // Workgroups go to the chip's eight dies in turn (b to die b % 8, each with its own L2). Neighbouring workgroups share a tile's columns across
     // the dies, and a die's workgroups four of the rows' tiles and eight of the columns'. An expert with fewer tiles of rows than dies
@@ -686,23 +690,27 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     Mx4Run run;
     if (!mx4_run(a, expert, run)) return;
     t0 = (u32)__builtin_amdgcn_readfirstlane((int)(t0 + run.j0));
-    const u32 steps = (a.kp + 127) / 128, tail = (a.kp - (steps - 1) * 128) / 16; // blocks of the last step
+    const u32 steps = (a.kp + 127) / 128, last = steps - 1;
 
     // columns and rows past the last are the last ones again, and not stored
     Mx4Src<G> src;
-    src.q = a.order ? a.q : a.q + (size_t)t0 * a.kp;
-    src.qs = a.order ? a.qs : a.qs + (size_t)t0 * a.ks;
-    src.w = run.w + (size_t)r0 * a.kp;
-    src.ws = run.ws + (size_t)r0 * a.ks;
-    u32 col[G::RT + G::RS];
+    {
+        const size_t c0 = a.order ? 0 : t0, columns = (a.start ? a.n_cols : a.m) - c0, rows = a.rows - r0;
+        src.q = a.q + c0 * a.kp, src.q_end = mx4_end(columns * a.kp);
+        src.qs = a.qs + c0 * a.ks, src.qs_end = mx4_end(columns * a.ks);
+        src.w = run.w + (size_t)r0 * a.kp, src.w_end = mx4_end(rows * a.kp);
+        src.ws = run.ws + (size_t)r0 * a.ks, src.ws_end = mx4_end(rows * a.ks);
+    }
+    src.at = src.mark_at = 0;
+    u32 col[G::RT + G::RG];
 #pragma unroll
     for (int r = 0; r < G::RT; r++) col[r] = min(t0 + (wave * G::RT + r) * 8 + (lane >> 3), run.j1 - 1);
 #pragma unroll
-    for (int r = 0; r < G::RS; r++) col[G::RT + r] = min(t0 + mx4_mark_group<G>(wave, r) * 32 + (lane >> 1), run.j1 - 1); // (of a group of rows: not used)
+    for (int r = 0; r < G::RG; r++) col[G::RT + r] = min(t0 + mx4_mark_group<G>(wave, r) * 32 + (lane >> 1), run.j1 - 1); // (of a group of rows: not used)
     if (a.order) run_columns(a, col);
     else
 #pragma unroll
-        for (int r = 0; r < G::RT + G::RS; r++) col[r] -= t0;
+        for (int r = 0; r < G::RT + G::RG; r++) col[r] -= t0;
 #pragma unroll
     for (int r = 0; r < G::RT; r++) src.col[r] = col[r] * a.kp + 16 * ((lane & 7) ^ line_swizzle((wave * G::RT + r) * 8 + (lane >> 3)));
 #pragma unroll
@@ -711,15 +719,10 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
         src.row[r] = (min(r0 + line, a.rows - 1) - r0) * a.kp + 16 * ((lane & 7) ^ line_swizzle(line));
     }
 #pragma unroll
-    for (int r = 0; r < G::RS; r++) {
+    for (int r = 0; r < G::RG; r++) {
         const u32 line = mx4_mark_group<G>(wave, r) * 32 + (lane >> 1);
         const u32 row = min(r0 + line - (u32)BT, a.rows - 1) - r0;
-        src.mark[r] = (line < (u32)BT ? col[G::RT + r] : row) * a.ks + 4 * (lane & 1);
-    }
-#pragma unroll
-    for (int r = 0; r < 2; r++) { // (a lane's piece differs between even and odd groups of eight lines only)
-        const u32 piece = (lane & 7) ^ line_swizzle(8 * r + (lane >> 3));
-        src.back[r] = piece >= tail ? 16 * piece : 0;
+        src.mark[r] = (line < (u32)BT ? col[G::RT + r] : row) * a.ks + 16 * (lane & 1);
     }
 
     v4f acc[G::TR][G::TT];
@@ -728,77 +731,48 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
 #pragma unroll
         for (int j = 0; j < G::TT; j++) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     const u32 wt = (wave % WT) * (BT / WT), wr = BT + (wave / WT) * (BR / WR); // this wave's first lines
-    Mx4At at[2];
+    Mx4At at;
+    at.sa = (wr + (lane & 15)) * 32 + 2 * (lane >> 4);
+    at.sb = (wt + (lane & 15)) * 32 + 2 * (lane >> 4);
 #pragma unroll
-    for (u32 up = 0; up < 2; up++) {
-        const u32 more = up * G::kUp * G::kStage, mark = G::kCodes + (lane & 15) * 8 + 2 * (lane >> 4) + more;
-        at[up].sa = mark + wr * 8;
-        at[up].sb = mark + wt * 8;
-        __asm__("" : "+v"(at[up].sa), "+v"(at[up].sb)); // one register each from here on, whatever constants meet them
+    for (u32 c = 0; c < 2; c++) {
+        const u32 piece = (lane & 15) * 128 + 16 * ((2 * (lane >> 4) + c) ^ line_swizzle(lane & 15));
 #pragma unroll
-        for (u32 c = 0; c < 2; c++) {
-            const u32 piece = (lane & 15) * 128 + 16 * ((2 * (lane >> 4) + c) ^ line_swizzle(lane & 15)) + more;
-            at[up].a[c] = piece + wr * 128;
-            at[up].b[c] = piece + wt * 128;
-            __asm__("" : "+v"(at[up].a[c]), "+v"(at[up].b[c]));
+        for (u32 up = 0; up < 2; up++) {
+            at.line[up].a[c] = piece + wr * 128 + up * G::kUp * G::kStage;
+            at.line[up].b[c] = piece + wt * 128 + up * G::kUp * G::kStage;
+            __asm__("" : "+v"(at.line[up].a[c]), "+v"(at.line[up].b[c])); // one register each from here on, whatever constants meet them
         }
     }
-    mx4_ask<G>(src, ring0, wave, steps == 1);
-    if (steps > 1) mx4_ask<G>(src, ring1, wave, steps == 2);
-    if (S > 2 && steps > 2) mx4_ask<G>(src, ring2, wave, steps == 3);
-    if (S > 2 && steps > 3) mx4_ask<G>(src, ring3, wave, steps == 4);
-    if (steps >= (u32)S) mx4_turn<G, S - 1>();
-    else mx4_turn<G, 0>();
-    if (steps == 1 && tail < 8) mx4_zero_past<G>(ring0, tail);
-    u32 left = steps - 1;
-    if constexpr (WHOLE) {
-        // (rings of an even number of buffers: the two sets of registers change places with every step)
-        Mx4Whole<G> f, g;
-        mx4_read_whole<G, 0>(f, ring0, at);
-        if constexpr (S == 2) {
-            for (; left >= 4; left -= 2) {
-                mx4_step_whole<G, 0, true>(src, ring0, ring1, wave, 0, 0, at, f, g, acc);
-                mx4_step_whole<G, 1, true>(src, ring1, ring0, wave, 0, 0, at, g, f, acc);
-            }
-            for (;;) {
-                mx4_step_whole<G, 0, false>(src, ring0, ring1, wave, left, tail, at, f, g, acc);
-                if (left-- == 0) break;
-                mx4_step_whole<G, 1, false>(src, ring1, ring0, wave, left, tail, at, g, f, acc);
-                if (left-- == 0) break;
-            }
-        } else {
-            for (; left >= 8; left -= 4) {
-                mx4_step_whole<G, 0, true>(src, ring0, ring1, wave, 0, 0, at, f, g, acc);
-                mx4_step_whole<G, 1, true>(src, ring1, ring2, wave, 0, 0, at, g, f, acc);
-                mx4_step_whole<G, 2, true>(src, ring2, ring3, wave, 0, 0, at, f, g, acc);
-                mx4_step_whole<G, 3, true>(src, ring3, ring0, wave, 0, 0, at, g, f, acc);
-            }
-            for (;;) {
-                mx4_step_whole<G, 0, false>(src, ring0, ring1, wave, left, tail, at, f, g, acc);
-                if (left-- == 0) break;
-                mx4_step_whole<G, 1, false>(src, ring1, ring2, wave, left, tail, at, g, f, acc);
-                if (left-- == 0) break;
-                mx4_step_whole<G, 2, false>(src, ring2, ring3, wave, left, tail, at, f, g, acc);
-                if (left-- == 0) break;
-                mx4_step_whole<G, 3, false>(src, ring3, ring0, wave, left, tail, at, g, f, acc);
-                if (left-- == 0) break;
-            }
-        }
+    Mx4Way way = {0, a.kp / 16 - 8 * last, wave};
+    typename std::conditional<Q == 0, Mx4Whole<G>, Mx4Parts<G>>::type f;
+    mx4_ask_marks<G>(src, marks, wave);
+    if (last & 1) { // an even number of steps: the first and the last two by themselves, pairs between them
+        mx4_ask<G>(src, ring0, wave);
+        mx4_turn();
+        mx4_ask<G>(src, ring1, wave);
+        f.template begin<0>(ring0, marks, at);
     } else {
-        static_assert(WHOLE || S == 2, "parts of a step in a ring of two");
-        Mx4Head<G> f;
-        mx4_head<G, 0>(f, ring0, at);
-        for (; left >= 4; left -= 2) {
-            mx4_step<G, 0, true>(src, ring0, ring1, wave, 0, 0, at, f, acc);
-            mx4_step<G, 1, true>(src, ring1, ring0, wave, 0, 0, at, f, acc);
-        }
-        for (;;) {
-            mx4_step<G, 0, false>(src, ring0, ring1, wave, left, tail, at, f, acc);
-            if (left-- == 0) break;
-            mx4_step<G, 1, false>(src, ring1, ring0, wave, left, tail, at, f, acc);
-            if (left-- == 0) break;
+        mx4_ask<G>(src, ring1, wave);
+        mx4_turn();
+        if (last == 0 && way.tail < 8) mx4_zero_past<G>(ring1, marks, way.tail);
+        if (last) mx4_ask<G>(src, ring0, wave);
+        f.template begin<1>(ring1, marks, at);
+        if (last) {
+            mx4_ask_marks<G>(src, marks + G::kMarks, wave);
+            f.template step<1, kFull>(src, ring1, ring0, marks, way, at, acc);
         }
     }
+    if (last) {
+        while (way.step + 1 < last) {
+            // in the first pair of four steps, or the second and third of them, the next four's scales; those of steps 4 to 7 may be on their way
+            if ((way.step & 3) < 2 && way.step != 1) mx4_ask_marks<G>(src, marks + (~way.step >> 2 & 1) * G::kMarks, wave);
+            f.template step<0, kFull>(src, ring0, ring1, marks, way, at, acc);
+            f.template step<1, kFull>(src, ring1, ring0, marks, way, at, acc);
+        }
+        f.template step<0, kNext>(src, ring0, ring1, marks, way, at, acc);
+    }
+    f.template step<1, kLast>(src, ring1, ring0, marks, way, at, acc);
     __syncthreads(); // the buffers are the sums' from here
     constexpr u32 kPart = G::TR * 2048, kEven = G::kStage / kPart; // a wave's part, and how many lie in the first buffer
     static_assert(G::kWaves <= 2 * kEven, "every part lies in one buffer");
@@ -808,14 +782,14 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     else mx4_tile_out<kElemBF16, G>(a, run, part, t0 + wt, r0 + (wr - BT), acc);
 }
 
-template <int BT, int BR, int WT, int WR, int S, bool WHOLE, int EU>
+template <int BT, int BR, int WT, int WR, int Q, int EU>
 static hipError_t mx4_tile_launch(const Launch &L, const Mx4Args &a, u32 entries) {
     const u32 row_tiles = (a.rows + BR - 1) / BR;
     u32 tiles = (entries + BT - 1) / BT;
     if (a.start) tiles = entries / BT + (a.n_experts < entries ? a.n_experts : entries); // at most a ragged tile an expert
     const u32 group = a.start && row_tiles < 8 ? 2 : 0;
     if (group) tiles = (tiles + 8 * group - 1) / (8 * group) * (8 * group);
-    hipLaunchKernelGGL((k_mx4_tile<BT, BR, WT, WR, S, WHOLE, EU>), group_grid((uint64_t)tiles * row_tiles, 64 * WT * WR), dim3(64 * WT * WR), 0, L.stream, a, row_tiles, group);
+    hipLaunchKernelGGL((k_mx4_tile<BT, BR, WT, WR, Q, EU>), group_grid((uint64_t)tiles * row_tiles, 64 * WT * WR), dim3(64 * WT * WR), 0, L.stream, a, row_tiles, group);
     return hipGetLastError();
 }
 
@@ -865,14 +839,11 @@ enum Mx4Form : u32 {
     kMx4Few16x32,
     kMx4Few16x32Three,
     kMx4Few32x32,
-    kMx4Tile32x64Ring4, // k_mx4_tile, steps in a ring of four or two
-    kMx4Tile32x64,
-    kMx4Tile64x64Ring4,
+    kMx4Tile32x64, // k_mx4_tile
     kMx4Tile64x64,
     kMx4Tile64x128,
-    kMx4Tile64x256,
     kMx4Tile128x128,
-    kMx4Tile256x224,
+    kMx4Tile256x128,
     kMx4Tile256x256,
 };
 
@@ -883,38 +854,26 @@ static Mx4Form mx4_form(u32 n_experts, u32 rows, u32 kp, u32 n, bool reach) {
     if (n_experts) {
         if (n <= 32 || !reach) return kMx4Few16x32Three;
         const u32 each = n / n_experts, runs = n < n_experts ? n : n_experts;
-        // 64 x 64 tiles: every run has one, and half a one more than its slots fill
         const uint64_t small = (uint64_t)std::max(runs, n / 64 + runs / 2) * up(rows, 64);
         if (each <= 16 && small <= 64) return kMx4Few32x32;
-        if (each < 24 && small <= 600) return kMx4Tile32x64Ring4;
-        if (each >= 24 && small <= 256) return kMx4Tile64x64Ring4;
         if (each >= 24 && small <= 1024) return kMx4Tile64x64;
-        if (each >= 352) return kMx4Tile256x256;
-        if (each >= 144) return kMx4Tile128x128;
-        if (each >= 96 || (each >= 12 && (uint64_t)(n / 64 + n_experts / 2) * up(rows, 256) <= 512)) return kMx4Tile64x256;
+        if (each >= 96) return kMx4Tile128x128;
         return each >= 12 ? kMx4Tile64x128 : kMx4Tile32x64;
     }
     if (tiles(16, 16) <= 256) return kMx4Few16x16;
     if (tiles(16, 32) <= 256) return kMx4Few16x32;
     if (n <= 16) return kMx4Few16x32Three;
     if (n <= 32 || tiles(32, 32) <= 256) return kMx4Few32x32;
-    if (tiles(32, 64) <= 256) return kMx4Tile32x64Ring4;
-    if (tiles(64, 64) <= 512 && kp > 1024) return kMx4Tile64x64Ring4;
     if (tiles(64, 64) <= 768) return kMx4Tile64x64;
-    if (tiles(256, 256) >= 96) {
-        const uint64_t by256 = 64 * ((tiles(256, 256) + 255) / 256), by224 = 57 * ((tiles(256, 224) + 255) / 256), by128 = 39 * ((tiles(128, 128) + 511) / 512);
-        if (by256 <= by224 && by256 <= by128) return kMx4Tile256x256;
-        return by224 <= by128 ? kMx4Tile256x224 : kMx4Tile128x128;
-    }
-    return tiles(64, 128) <= 640 ? kMx4Tile64x128 : kMx4Tile128x128;
+    return kMx4Tile128x128;
 }
 static bool mx4_reach(bool gathered, int n_cols, u32 kp) { return !gathered || (uint64_t)n_cols * kp <= 0xffffffffu; }
 
 int mx4_gemm_form(int n_experts, int rows, int k, int n_cols, int n_slots, int top_k) {
     static const struct {
         u32 columns, rows, waves, buffers;
-    } of[] = {{16, 16, 8, 4}, {16, 32, 4, 4}, {16, 32, 3, 4}, {32, 32, 4, 4}, {32, 64, 2, 4}, {32, 64, 2, 2}, {64, 64, 4, 4},
-              {64, 64, 4, 2}, {64, 128, 4, 2}, {64, 256, 4, 2}, {128, 128, 4, 2}, {256, 224, 8, 2}, {256, 256, 8, 2}};
+    } of[] = {{16, 16, 8, 4}, {16, 32, 4, 4}, {16, 32, 3, 4}, {32, 32, 4, 4}, {32, 64, 2, 2}, {64, 64, 4, 2}, {64, 128, 4, 2}, {128, 128, 4, 2},
+              {256, 128, 8, 2}, {256, 256, 8, 2}};
     const u32 kp = (u32)mx4_row_bytes(k);
     const auto &f = of[mx4_form((u32)n_experts, (u32)rows, kp, (u32)(n_experts ? n_slots : n_cols), mx4_reach(n_experts && top_k > 0, n_cols, kp))];
     return (int)(f.columns | f.rows << 10 | f.waves << 20 | f.buffers << 24);
@@ -930,15 +889,12 @@ hipError_t mx4_gemm(const Launch &L, const uint8_t *w, const uint8_t *ws, int n_
     case kMx4Few16x32: return mx4_few_launch<2, 1, 4>(L, a, n);
     case kMx4Few16x32Three: return mx4_few_launch<2, 1, 3>(L, a, n);
     case kMx4Few32x32: return mx4_few_launch<2, 2, 4>(L, a, n);
-    case kMx4Tile32x64Ring4: return mx4_tile_launch<32, 64, 1, 2, 4, true, 2>(L, a, n);
-    case kMx4Tile32x64: return mx4_tile_launch<32, 64, 1, 2, 2, true, 2>(L, a, n);
-    case kMx4Tile64x64Ring4: return mx4_tile_launch<64, 64, 2, 2, 4, true, 2>(L, a, n);
-    case kMx4Tile64x64: return mx4_tile_launch<64, 64, 2, 2, 2, true, 2>(L, a, n);
-    case kMx4Tile64x128: return mx4_tile_launch<64, 128, 1, 4, 2, true, 2>(L, a, n);
-    case kMx4Tile64x256: return mx4_tile_launch<64, 256, 1, 4, 2, true, 2>(L, a, n);
-    case kMx4Tile128x128: return mx4_tile_launch<128, 128, 2, 2, 2, true, 2>(L, a, n);
-    case kMx4Tile256x224: return mx4_tile_launch<256, 224, 4, 2, 2, false, 2>(L, a, n);
-    case kMx4Tile256x256: return mx4_tile_launch<256, 256, 4, 2, 2, false, 2>(L, a, n);
+    case kMx4Tile32x64: return mx4_tile_launch<32, 64, 1, 2, 0, 2>(L, a, n);
+    case kMx4Tile64x64: return mx4_tile_launch<64, 64, 2, 2, 0, 2>(L, a, n);
+    case kMx4Tile64x128: return mx4_tile_launch<64, 128, 1, 4, 0, 2>(L, a, n);
+    case kMx4Tile128x128: return mx4_tile_launch<128, 128, 2, 2, 0, 2>(L, a, n);
+    case kMx4Tile256x128: return mx4_tile_launch<256, 128, 4, 2, 2, 2>(L, a, n);
+    case kMx4Tile256x256: return mx4_tile_launch<256, 256, 4, 2, 2, 2>(L, a, n);
     }
     return hipErrorInvalidValue;
 }
