@@ -901,10 +901,18 @@ hipError_t mx4_gemm(const Launch &L, const uint8_t *w, const uint8_t *ws, int n_
 
 // ------------------------------------------------------------------------------------ a few tokens' experts
 
-// Two launches. The first forms h: a workgroup an expert that is hit and 16 of its rows of gate and of up, for the tokens that picked it. The second forms y: a workgroup
-// 16 rows of down, for all tokens, over the experts that are hit. Weights are read once by each, as lines through rings in LDS, and bound both; codes
+// Two launches. The first forms h: a workgroup an expert that is hit and some of its rows of gate and of up, for the tokens that picked it. The second forms y: a
+// workgroup sixteen rows of down, for all tokens, over the experts that are hit. Weights are read once by each, as lines through rings in LDS, and bound both; codes
 // become bf16 values exactly, a few instructions for eight, and the products run on the bf16 matrix instructions, the tokens' values in parts that
 // add up to them: one of bf16, two of f16, three of f32, and of h two (f32: three).
+
+// What the first launch leaves for the second: the experts that are hit, ascending, and their tokens' slots, of a token that picked an expert twice the
+// first.
+constexpr u32 kMoeExperts = 1024;
+struct MoeTable {
+    u32 n_hit, unused[15];
+    uint16_t expert[kMoeExperts], count[kMoeExperts], slot[kMoeExperts][kMx4MoeTokens];
+};
 struct Mx4Moe {
     const uint8_t *wg, *wgs, *wu, *wus, *wd, *wds;
     u32 n_experts, hidden, ff, n_tokens, top_k;
@@ -912,56 +920,52 @@ struct Mx4Moe {
     size_t ld_x, ld_resid, ld_y;
     const u32 *sel;
     const float *w;
-    __bf16 *h; // a slot's parts, rows of ff rounded up to 32 values
+    MoeTable *table; // (as many of the slots' rows as there can be hits)
+    __bf16 *h;       // a slot's parts, rows of ff rounded up to 32 values
     void *y;
     GateRule rule;
     u32 *fault, layer;
 };
-constexpr u32 kMoeExperts = 1024, kMoeSlots = kMx4MoeTokens * 64;
 typedef __bf16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v2h __attribute__((ext_vector_type(2)));
 
+// A wave's inclusive sums.
+__device__ __forceinline__ u32 moe_upto(u32 v) {
+    v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);  // one lane up within sixteen
+    v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
+    v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
+    v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
+    v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false); // a row's last onto the next
+    v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+    return v;
+}
 // The experts that the picks hit, as bits, and the picks; every thread of the workgroup takes part. An id that names no expert is 0xffff, and raised by
 // `raise`'s workgroup.
-struct MoePicks {
-    u32 bits[kMoeExperts / 32], before[kMoeExperts / 32]; // before: experts hit in the words in front
-    uint16_t sel[kMoeSlots];
-};
 template <int T>
-__device__ __forceinline__ void moe_picks(const Mx4Moe &a, MoePicks &p, bool raise) {
-    if (threadIdx.x < kMoeExperts / 32) p.bits[threadIdx.x] = 0;
+__device__ __forceinline__ void moe_picks(const Mx4Moe &a, u32 *bits, uint16_t *sel, bool raise) {
+    const u32 n = a.n_tokens * a.top_k;
+    u32 e = threadIdx.x < n ? a.sel[threadIdx.x] : 0u;
+    if (threadIdx.x < kMoeExperts / 32) bits[threadIdx.x] = 0;
     __syncthreads();
-    for (u32 i = threadIdx.x; i < a.n_tokens * a.top_k; i += T) {
-        const u32 e = a.sel[i];
+    for (u32 i = threadIdx.x; i < n;) {
         const bool in = e < a.n_experts;
-        p.sel[i] = in ? (uint16_t)e : (uint16_t)0xffff;
-        if (in) atomicOr(&p.bits[e >> 5], 1u << (e & 31));
+        sel[i] = in ? (uint16_t)e : (uint16_t)0xffff;
+        if (in) atomicOr(&bits[e >> 5], 1u << (e & 31));
         else if (raise && e != 0xffffffffu) bm_raise(a.fault, a.layer, kSiteExpertId);
+        if ((i += T) < n) e = a.sel[i];
     }
     __syncthreads();
 }
-// Inclusive sums of the words' counts, lane i's word i (lanes past the words: all).
-__device__ __forceinline__ u32 moe_upto(const MoePicks &p, u32 lane, u32 &mine) {
-    mine = lane < kMoeExperts / 32 ? (u32)__builtin_popcount(p.bits[lane]) : 0u;
-    u32 upto = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const u32 o = (u32)__shfl_up((int)upto, d, 64);
-        if (lane >= (u32)d) upto += o;
-    }
-    return upto;
-}
-// The n-th expert that is hit; false: there are not as many.
-__device__ __forceinline__ bool moe_nth(const MoePicks &p, u32 n, u32 &expert) {
-    const u32 lane = threadIdx.x & 63;
-    u32 mine;
-    const u32 upto = moe_upto(p, lane, mine);
-    const unsigned long long here = __ballot(mine != 0 && upto - mine <= n && n < upto);
+// The n-th expert that is hit, and how many are; false: there are not as many.
+__device__ __forceinline__ bool moe_nth(const u32 *bits, u32 n, u32 &expert, u32 &n_hit) {
+    const u32 lane = threadIdx.x & 63, word = lane < kMoeExperts / 32 ? bits[lane] : 0u, mine = (u32)__builtin_popcount(word), upto = moe_upto(mine);
+    n_hit = (u32)__builtin_amdgcn_readlane((int)upto, 63);
+    const unsigned long long here = __ballot(upto - mine <= n && n < upto);
     if (!here) return false;
-    const int word = __builtin_ctzll(here);
-    u32 skip = n - (u32)__shfl((int)(upto - mine), word, 64), w = p.bits[word];
+    const int at = __builtin_ctzll(here);
+    u32 w = (u32)__builtin_amdgcn_readlane((int)word, at), skip = n - (u32)__builtin_amdgcn_readlane((int)(upto - mine), at);
     for (; skip; skip--) w &= w - 1;
-    expert = (u32)__builtin_amdgcn_readfirstlane(32 * word + __builtin_ctz(w));
+    expert = 32 * (u32)at + (u32)__builtin_ctz(w);
     return true;
 }
 
@@ -1052,73 +1056,93 @@ struct MoeX {
     }
 };
 
+// h. T times sixteen rows of gate and as many of up; SHORT: a row's lines are two a wave at most, asked for at once.
 constexpr int kMoeUpWaves = 4;
-template <int ET>
+template <int ET, int T, bool SHORT>
 __global__ __launch_bounds__(64 * kMoeUpWaves) void k_mx4_moe_up(Mx4Moe a) {
-    constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, PH = kMoeKept<ET>, kLoads = 6; // of a stage: four of lines, two of scales
-    typedef Lines<4> L; // sixteen rows of gate, sixteen of up
-    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[NW * L::kStage], ring3[NW * L::kStage];
-    __shared__ MoePicks picks;
-    __shared__ u32 col_slot[16];
+    constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, PH = kMoeKept<ET>, R = 2 * T, kLoads = 3 * R; // of a stage: 2 R of lines, R of scales
+    typedef Lines<2 * R> L;
+    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[SHORT ? 16 : NW * L::kStage], ring3[SHORT ? 16 : NW * L::kStage];
+    __shared__ u32 bits[kMoeExperts / 32], col_slot[16];
     __shared__ float col_weight[16];
-    const u32 lane = threadIdx.x & 63, wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    moe_picks<64 * NW>(a, picks, blockIdx.x == 0 && blockIdx.y == 0);
-    u32 expert;
-    if (!moe_nth(picks, blockIdx.y, expert)) return;
+    extern __shared__ __align__(16) uint16_t sel[];
+    const u32 lane = threadIdx.x & 63, wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = blockIdx.y;
+    moe_picks<64 * NW>(a, bits, sel, blockIdx.x == 0 && n == 0);
+    u32 expert, n_hit;
+    const bool there = moe_nth(bits, n, expert, n_hit);
+    if (blockIdx.x == 0 && n == 0 && threadIdx.x == 0) a.table->n_hit = n_hit;
+    if (!there) return;
+
+    const u32 kp = (a.hidden + 31) / 32 * 16, ks = (a.hidden + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage, at = 2 * (lane >> 4);
+    const u32 r0 = blockIdx.x * (16 * T), ffp = (a.ff + 31) / 32 * 32;
+    L src;
+    src.begin(lane);
+    const size_t stack = (size_t)expert * a.ff;
+    const uint8_t *scales[R];
+#pragma unroll
+    for (u32 g = 0; g < 2 * R; g++) // rows past the last are the last once more, and their values zeros
+        src.from[g] = (const int8_t *)(g < R ? a.wg : a.wu) + (stack + min(r0 + 8 * (g % R) + (lane >> 3), a.ff - 1)) * kp;
+#pragma unroll
+    for (u32 g = 0; g < R; g++) scales[g] = (g < T ? a.wgs : a.wus) + (stack + min(r0 + 16 * (g % T) + (lane & 15), a.ff - 1)) * ks + at;
+    u32 s0[R], s1[R], s2[R], s3[R];
+    const auto ask = [&](uint8_t *stage, u32 (&s)[R], u32 l) {
+#pragma unroll
+        for (int g = 0; g < R; g++) s[g] = mx4_two(scales[g] + 8 * l);
+        __builtin_amdgcn_sched_barrier(0);
+        src.ask(stage + mine, l, kp);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto begin = [&] {
+        if (wave < lines) ask(ring0, s0, wave);
+        if (wave + NW < lines) ask(ring1, s1, wave + NW);
+        if (!SHORT && wave + 2 * NW < lines) ask(ring2, s2, wave + 2 * NW);
+    };
+    begin();
+
     // lane t: token t's first slot of this expert, and its weight, over all its slots of it
     u32 slot = 0;
     float weight = 0.0f;
     bool user = false;
     if (lane < a.n_tokens)
         for (u32 s = a.top_k; s-- > 0;)
-            if (picks.sel[lane * a.top_k + s] == expert) {
+            if (sel[lane * a.top_k + s] == expert) {
                 slot = lane * a.top_k + s;
-                weight += a.w[slot];
+                weight = __fadd_rn(a.w[slot], weight);
                 user = true;
             }
     const unsigned long long users = __ballot(user);
     const u32 n_users = (u32)__builtin_popcountll(users), place = (u32)__builtin_popcountll(users & ((1ull << lane) - 1));
-
-    const u32 kp = (a.hidden + 31) / 32 * 16, ks = (a.hidden + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage, at = 2 * (lane >> 4);
-    const u32 r0 = blockIdx.x * 16, ffp = (a.ff + 31) / 32 * 32;
-    L src;
-    src.begin(lane);
-    const size_t stack = (size_t)expert * a.ff;
-#pragma unroll
-    for (u32 g = 0; g < 4; g++) src.from[g] = (const int8_t *)(g < 2 ? a.wg : a.wu) + (stack + min(r0 + 8 * (g & 1) + (lane >> 3), a.ff - 1)) * kp;
-    const size_t mark = (stack + min(r0 + (lane & 15), a.ff - 1)) * ks + at;
-    const uint8_t *scales[2] = {a.wgs + mark, a.wus + mark};
+    if (blockIdx.x == 0 && wave == 0) {
+        if (lane == 0) {
+            a.table->expert[n] = (uint16_t)expert;
+            a.table->count[n] = (uint16_t)n_users;
+        }
+        if (user) a.table->slot[n][place] = (uint16_t)slot;
+    }
     for (u32 z = 0; z < n_users; z += 16) {
         if (user && place - z < 16) {
             col_slot[place - z] = slot;
             col_weight[place - z] = weight;
         }
         __syncthreads();
+        if (z) begin();
         const u32 my_slot = col_slot[min(lane & 15, min(n_users - z, 16u) - 1)]; // columns past the last are the last once more, and not stored
         const size_t row = (size_t)(my_slot / a.top_k) * a.ld_x;
-        u32 s0[2], s1[2], s2[2], s3[2];
-        const auto ask = [&](uint8_t *stage, u32 (&s)[2], u32 l) {
-            s[0] = mx4_two(scales[0] + 8 * l);
-            s[1] = mx4_two(scales[1] + 8 * l);
-            __builtin_amdgcn_sched_barrier(0);
-            src.ask(stage + mine, l, kp);
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        if (wave < lines) ask(ring0, s0, wave);
-        if (wave + NW < lines) ask(ring1, s1, wave + NW);
-        if (wave + 2 * NW < lines) ask(ring2, s2, wave + 2 * NW);
-        v4f acc[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
-        const auto step = [&](const uint8_t *stage, u32 (&s)[2], uint8_t *free, u32 (&next)[2], u32 l) {
+        v4f acc[R];
+#pragma unroll
+        for (int g = 0; g < R; g++) acc[g] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        const auto step = [&](const uint8_t *stage, u32 (&s)[R], uint8_t *free, u32 (&next)[R], u32 l) {
             MoeX<ET> x;
             x.ask(a.x, row, 256 * l + 32 * at, a.hidden);
             __builtin_amdgcn_sched_barrier(0);
-            if (l + 3 * NW < lines) ask(free, next, l + 3 * NW);
-            if (l + 3 * NW < lines) loads_landed<kLoads>();
+            const bool more = !SHORT && l + 3 * NW < lines;
+            if (more) ask(free, next, l + 3 * NW);
+            if (more) loads_landed<kLoads>();
             else loads_landed<0>();
-            v4i w[2][2];
-            u32 two[2];
+            v4i w[R][2];
+            u32 two[R];
 #pragma unroll
-            for (int g = 0; g < 2; g++) {
+            for (int g = 0; g < R; g++) {
                 two[g] = mx4_scales(s[g], 8 * l + at, blocks);
 #pragma unroll
                 for (int h = 0; h < 2; h++) w[g][h] = mx4_of_line(stage + mine, lane, g, h);
@@ -1128,30 +1152,35 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) void k_mx4_moe_up(Mx4Moe a) {
                 v8h part[P];
                 x.parts(i, part);
 #pragma unroll
-                for (int g = 0; g < 2; g++) {
+                for (int g = 0; g < R; g++) {
                     const v8h c = moe_codes((u32)w[g][i / 4][i % 4], moe_scale(two[g], i / 4));
 #pragma unroll
                     for (int p = 0; p < P; p++) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(c, part[p], acc[g], 0, 0, 0);
                 }
             }
         };
-        for (u32 l = wave; l < lines;) {
-            step(ring0, s0, ring3, s3, l);
-            if ((l += NW) >= lines) break;
-            step(ring1, s1, ring0, s0, l);
-            if ((l += NW) >= lines) break;
-            step(ring2, s2, ring1, s1, l);
-            if ((l += NW) >= lines) break;
-            step(ring3, s3, ring2, s2, l);
-            l += NW;
+        if constexpr (SHORT) {
+            if (wave < lines) step(ring0, s0, nullptr, s3, wave);
+            if (wave + NW < lines) step(ring1, s1, nullptr, s3, wave + NW);
+        } else {
+            for (u32 l = wave; l < lines;) {
+                step(ring0, s0, ring3, s3, l);
+                if ((l += NW) >= lines) break;
+                step(ring1, s1, ring0, s0, l);
+                if ((l += NW) >= lines) break;
+                step(ring2, s2, ring1, s1, l);
+                if ((l += NW) >= lines) break;
+                step(ring3, s3, ring2, s2, l);
+                l += NW;
+            }
         }
         loads_landed<0>();
 #pragma unroll
-        for (int g = 0; g < 2; g++) *reinterpret_cast<v4f *>(ring0 + mine + g * 1024 + 16 * lane) = acc[g];
+        for (int g = 0; g < R; g++) *reinterpret_cast<v4f *>(ring0 + mine + g * 1024 + 16 * lane) = acc[g];
         __syncthreads();
-        const u32 c = lane & 15, f = r0 + 4 * (lane >> 4);
-        if (wave == 0 && z + c < n_users) {
-            const v4f g = mx4_join<NW, L>(ring0, 0, lane), u = mx4_join<NW, L>(ring0, 1, lane);
+        const u32 c = lane & 15, f = r0 + 16 * wave + 4 * (lane >> 4);
+        if (wave < T && f < ffp && z + c < n_users) {
+            const v4f g = mx4_join<NW, L>(ring0, wave, lane), u = mx4_join<NW, L>(ring0, T + wave, lane);
             const float by = col_weight[c];
             float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
             bool odd = false;
@@ -1168,151 +1197,199 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) void k_mx4_moe_up(Mx4Moe a) {
 #pragma unroll
             for (int p = 0; p < PH; p++) {
                 *reinterpret_cast<uint2 *>(to + (size_t)p * ffp) = *reinterpret_cast<const uint2 *>(&part[p]);
-                if (r0 + 16 >= a.ff && r0 + 16 < ffp) *reinterpret_cast<uint2 *>(to + (size_t)p * ffp + 16) = make_uint2(0, 0); // the last block's other half
+                if (T == 1 && r0 + 16 >= a.ff && r0 + 16 < ffp) *reinterpret_cast<uint2 *>(to + (size_t)p * ffp + 16) = make_uint2(0, 0); // the last block's other half
             }
         }
         __syncthreads();
     }
 }
 
-constexpr int kMoeDownWaves = 8;
-// NT tiles of sixteen tokens.
-template <int ET, int NT>
-__global__ __launch_bounds__(64 * kMoeDownWaves) void k_mx4_moe_down(Mx4Moe a) {
-    constexpr int NW = kMoeDownWaves, PH = kMoeKept<ET>, kLoads = 3; // of a stage: two of lines, one of scales
+// y. The lines of the experts that are hit, one expert's after another's, are dealt to the waves in stretches; a wave adds an expert's sums of its tokens, sixteen
+// at a time, onto its own of all tokens, in LDS, when it has done with the expert. NZ: sixteens of tokens there may be.
+template <int ET, int NW, int NZ>
+__global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
+    constexpr int PH = kMoeKept<ET>, kLoads = 3; // of a stage: two of lines, one of scales
     typedef Lines<2> L;
     __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[NW * L::kStage], ring3[NW * L::kStage];
-    __shared__ MoePicks picks;
-    __shared__ uint16_t list[kMoeExperts];
-    extern __shared__ __align__(16) uint8_t map[]; // by expert that is hit, a byte a token: which of its slots, 0xff for none
-    const u32 lane = threadIdx.x & 63, wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    moe_picks<64 * NW>(a, picks, false);
-    u32 mine_count;
-    const u32 upto = moe_upto(picks, lane, mine_count), n_hit = (u32)__builtin_amdgcn_readfirstlane(__shfl((int)upto, 63, 64));
-    if (wave == 0 && lane < kMoeExperts / 32) picks.before[lane] = upto - mine_count;
-    for (u32 i = threadIdx.x; i < n_hit * (4 * NT); i += 64 * NW) reinterpret_cast<u32 *>(map)[i] = 0xffffffffu;
-    __syncthreads();
-    const auto rank = [&](u32 e) { return picks.before[e >> 5] + (u32)__builtin_popcount(picks.bits[e >> 5] & ((1u << (e & 31)) - 1)); };
-    for (u32 e = threadIdx.x; e < a.n_experts; e += 64 * NW)
-        if (picks.bits[e >> 5] >> (e & 31) & 1) list[rank(e)] = (uint16_t)e;
-    if (threadIdx.x < a.n_tokens)
-        for (u32 s = a.top_k; s-- > 0;) {
-            const u32 e = picks.sel[threadIdx.x * a.top_k + s];
-            if (e != 0xffff) map[rank(e) * (16 * NT) + threadIdx.x] = (uint8_t)s;
-        }
+    __shared__ __align__(16) uint16_t list[kMoeExperts];
+    extern __shared__ __align__(16) float sums[]; // waves x tokens x 16
+    const u32 lane = threadIdx.x & 63, wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), at = 2 * (lane >> 4), c = lane & 15;
+    const u32 n_hit = a.table->n_hit;
+    for (u32 i = threadIdx.x; 2 * i < a.n_experts; i += 64 * NW) reinterpret_cast<u32 *>(list)[i] = reinterpret_cast<const u32 *>(a.table->expert)[i];
+    float *const my_sums = sums + wave * a.n_tokens * 16;
+    for (u32 i = lane; i < a.n_tokens * 4; i += 64) *reinterpret_cast<v4f *>(my_sums + 4 * i) = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     __syncthreads();
 
-    const u32 kp = (a.ff + 31) / 32 * 16, ks = (a.ff + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage, at = 2 * (lane >> 4);
-    const u32 r0 = blockIdx.x * 16, ffp = (a.ff + 31) / 32 * 32, items = n_hit * lines;
+    const u32 kp = (a.ff + 31) / 32 * 16, ks = (a.ff + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage;
+    const u32 r0 = blockIdx.x * 16, ffp = (a.ff + 31) / 32 * 32, items = n_hit * lines, q0 = items * wave / NW, q1 = items * (wave + 1) / NW;
     L src;
     src.begin(lane);
-    const size_t from[2] = {(size_t)min(r0 + (lane >> 3), a.hidden - 1) * kp, (size_t)min(r0 + 8 + (lane >> 3), a.hidden - 1) * kp};
-    const size_t mark = (size_t)min(r0 + (lane & 15), a.hidden - 1) * ks + at;
-    u32 s0, s1, s2, s3;
-    const auto ask = [&](uint8_t *stage, u32 &s, u32 q) {
-        const u32 n = q / lines, l = q - n * lines, e = (u32)__builtin_amdgcn_readfirstlane(list[n]);
-        s = mx4_two(a.wds + (size_t)e * a.hidden * ks + mark + 8 * l);
+    const size_t from[2] = {(size_t)min(r0 + (lane >> 3), a.hidden - 1) * kp, (size_t)min(r0 + 8 + (lane >> 3), a.hidden - 1) * kp}; // rows past the last are not stored
+    const size_t mark = (size_t)min(r0 + c, a.hidden - 1) * ks + at;
+    u32 ask_n = q0 / lines, ask_l = q0 - ask_n * lines, ask_q = q0, n = ask_n, l = ask_l;
+    u32 s0 = 0, s1 = 0, s2 = 0, s3 = 0;
+    const auto ask = [&](uint8_t *stage, u32 &s) {
+        const u32 e = (u32)__builtin_amdgcn_readfirstlane(list[ask_n]);
+        s = mx4_two(a.wds + (size_t)e * a.hidden * ks + mark + 8 * ask_l);
 #pragma unroll
         for (int g = 0; g < 2; g++) src.from[g] = (const int8_t *)a.wd + (size_t)e * a.hidden * kp + from[g];
         __builtin_amdgcn_sched_barrier(0);
-        src.ask(stage + mine, l, kp);
+        src.ask(stage + mine, ask_l, kp);
         __builtin_amdgcn_sched_barrier(0);
+        ask_q++;
+        if (++ask_l == lines) ask_l = 0, ask_n++;
     };
-    if (wave < items) ask(ring0, s0, wave);
-    if (wave + NW < items) ask(ring1, s1, wave + NW);
-    if (wave + 2 * NW < items) ask(ring2, s2, wave + 2 * NW);
-    v4f acc[NT];
+    if (ask_q < q1) ask(ring0, s0);
+    if (ask_q < q1) ask(ring1, s1);
+    if (ask_q < q1) ask(ring2, s2);
+
+    v4f acc[NZ], odd_acc;
+    u32 users, slots[NZ], next_users = 0, next_slots[NZ];
+    const auto look = [&](u32 e) { // the e-th expert's users
+        if (e < n_hit) {
+            next_users = a.table->count[e];
 #pragma unroll
-    for (int t = 0; t < NT; t++) acc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    const auto step = [&](const uint8_t *stage, u32 &s, uint8_t *free, u32 &next, u32 q) {
-        const u32 n = q / lines, l = q - n * lines;
-        const auto values = [&](int t, v8h (&part)[8][PH]) { // a lane's 64 values of h, or zeros; whether the tile has any
-            const u32 token = 16 * t + (lane & 15), which = map[n * (16 * NT) + token], block = 8 * l + at;
-            const bool user = which != 0xff;
-            if (!__ballot(user)) return false;
-            const __bf16 *h = a.h + (size_t)(token * a.top_k + which) * PH * ffp + 32 * block;
+            for (int z = 0; z < NZ; z++)
+                if ((u32)z * 16 < a.n_tokens) next_slots[z] = a.table->slot[e][16 * z + c];
+        }
+    };
+    const auto turn = [&] { // to the expert that was looked at
+        users = (u32)__builtin_amdgcn_readfirstlane((int)next_users);
+#pragma unroll
+        for (int z = 0; z < NZ; z++) {
+            slots[z] = next_slots[z];
+            acc[z] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        odd_acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        look(n + 1);
+    };
+    const auto leave = [&] {
+        acc[0] += odd_acc;
+#pragma unroll
+        for (int z = 0; z < NZ; z++)
+            if (16 * z + c < users) *reinterpret_cast<v4f *>(my_sums + slots[z] / a.top_k * 16 + 4 * (lane >> 4)) += acc[z];
+    };
+    const auto values = [&](int z, v8h (&part)[8][PH]) { // a lane's 64 values of h
+        if (16 * z + c >= users) return; // (a column that is not looked at)
+        const u32 block = 8 * l + at;
+        const __bf16 *h = a.h + (size_t)slots[z] * PH * ffp + 32 * block;
+        if (8 * l + 8 <= blocks) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int p = 0; p < PH; p++) part[i][p] = moe_as_parts(*reinterpret_cast<const uint4 *>(h + (size_t)p * ffp + 8 * i));
+        } else {
 #pragma unroll
             for (int i = 0; i < 8; i++)
 #pragma unroll
                 for (int p = 0; p < PH; p++) {
                     uint4 v = make_uint4(0, 0, 0, 0);
-                    if (user && block + i / 4 < blocks) v = *reinterpret_cast<const uint4 *>(h + (size_t)p * ffp + 8 * i);
+                    if (block + i / 4 < blocks) v = *reinterpret_cast<const uint4 *>(h + (size_t)p * ffp + 8 * i);
                     part[i][p] = moe_as_parts(v);
                 }
-            return true;
-        };
+        }
+    };
+    const auto step = [&](const uint8_t *stage, u32 &s, uint8_t *free, u32 &next) {
         v8h part[8][PH];
-        bool any = values(0, part);
+        values(0, part);
         __builtin_amdgcn_sched_barrier(0);
-        if (q + 3 * NW < items) ask(free, next, q + 3 * NW);
-        if (q + 3 * NW < items) loads_landed<kLoads>();
-        else loads_landed<0>();
+        if (ask_q < q1) {
+            ask(free, next);
+            loads_landed<kLoads>();
+        } else {
+            loads_landed<0>();
+        }
         const u32 two = mx4_scales(s, 8 * l + at, blocks);
         v4i w[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) w[h] = mx4_of_line(stage + mine, lane, 0, h);
-        v8h codes[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) codes[i] = moe_codes((u32)w[i / 4][i % 4], moe_scale(two, i / 4));
+        for (int i = 0; i < 8; i++) {
+            const v8h code = moe_codes((u32)w[i / 4][i % 4], moe_scale(two, i / 4));
+            v4f &to = i & 1 ? odd_acc : acc[0];
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            if (t) any = values(t, part);
-            if (any)
+            for (int p = 0; p < PH; p++) to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code, part[i][p], to, 0, 0, 0);
+        }
 #pragma unroll
-                for (int i = 0; i < 8; i++)
+        for (int z = 1; z < NZ; z++)
+            if (16 * (u32)z < users) {
+                values(z, part);
 #pragma unroll
-                    for (int p = 0; p < PH; p++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes[i], part[i][p], acc[t], 0, 0, 0);
+                for (int i = 0; i < 8; i++) {
+                    const v8h code = moe_codes((u32)w[i / 4][i % 4], moe_scale(two, i / 4));
+#pragma unroll
+                    for (int p = 0; p < PH; p++) acc[z] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code, part[i][p], acc[z], 0, 0, 0);
+                }
+            }
+        if (++l == lines) {
+            leave();
+            l = 0, n++;
+            turn();
         }
     };
-    for (u32 q = wave; q < items;) {
-        step(ring0, s0, ring3, s3, q);
-        if ((q += NW) >= items) break;
-        step(ring1, s1, ring0, s0, q);
-        if ((q += NW) >= items) break;
-        step(ring2, s2, ring1, s1, q);
-        if ((q += NW) >= items) break;
-        step(ring3, s3, ring2, s2, q);
-        q += NW;
-    }
-    loads_landed<0>();
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-        *reinterpret_cast<v4f *>(ring0 + mine + 16 * lane) = acc[t];
-        __syncthreads();
-        const u32 token = 16 * t + (lane & 15), r = r0 + 4 * (lane >> 4);
-        if (wave == 0 && token < a.n_tokens && r < a.hidden) {
-            const v4f sum = mx4_join<NW, L>(ring0, 0, lane);
-            float v[4] = {sum[0], sum[1], sum[2], sum[3]};
-            const u32 have = a.hidden - r;
-            if (a.resid)
-#pragma unroll
-                for (u32 j = 0; j < 4; j++)
-                    if (j < have) v[j] = __fadd_rn(v[j], elem_load1<ET>(a.resid, token * a.ld_resid + r + j));
-            elem_store_some<ET, 4>(a.y, token * a.ld_y + r, have, v);
+    if (q0 < q1) {
+        look(n);
+        turn();
+        for (u32 q = q0;;) {
+            step(ring0, s0, ring3, s3);
+            if (++q == q1) break;
+            step(ring1, s1, ring0, s0);
+            if (++q == q1) break;
+            step(ring2, s2, ring1, s1);
+            if (++q == q1) break;
+            step(ring3, s3, ring2, s2);
+            if (++q == q1) break;
         }
-        __syncthreads();
+        if (l) leave();
+    }
+    __syncthreads();
+    for (u32 i = threadIdx.x; i < a.n_tokens * 4; i += 64 * NW) {
+        const u32 token = i / 4, r = r0 + 4 * (i & 3);
+        if (r >= a.hidden) continue;
+        v4f sum = *reinterpret_cast<const v4f *>(sums + 4 * i);
+        for (u32 w = 1; w < NW; w++) sum += *reinterpret_cast<const v4f *>(sums + (w * a.n_tokens * 4 + i) * 4);
+        float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+        const u32 have = a.hidden - r;
+        if (a.resid)
+#pragma unroll
+            for (u32 j = 0; j < 4; j++)
+                if (j < have) v[j] = __fadd_rn(v[j], elem_load1<ET>(a.resid, token * a.ld_resid + r + j));
+        elem_store_some<ET, 4>(a.y, token * a.ld_y + r, have, v);
     }
 }
 
+static u32 moe_hits(int n_tokens, int top_k, int n_experts) { return (u32)std::min(n_tokens * top_k, n_experts); }
+template <int ET, int T, bool SHORT>
+static void moe_up(const Launch &L, const Mx4Moe &a) {
+    hipLaunchKernelGGL((k_mx4_moe_up<ET, T, SHORT>), dim3((a.ff + 16 * T - 1) / (16 * T), moe_hits(a.n_tokens, a.top_k, a.n_experts)), dim3(64 * kMoeUpWaves),
+                       (a.n_tokens * a.top_k * 2 + 15) & ~15u, L.stream, a);
+}
+template <int ET, int NW, int NZ>
+static void moe_down(const Launch &L, const Mx4Moe &a) {
+    hipLaunchKernelGGL((k_mx4_moe_down<ET, NW, NZ>), dim3((a.hidden + 15) / 16), dim3(64 * NW), NW * a.n_tokens * 64, L.stream, a);
+}
 template <int ET>
 static hipError_t moe_launch(const Launch &L, const Mx4Moe &a) {
-    const u32 slots = a.n_tokens * a.top_k, hits = slots < a.n_experts ? slots : a.n_experts;
-    hipLaunchKernelGGL((k_mx4_moe_up<ET>), dim3((a.ff + 15) / 16, hits), dim3(64 * kMoeUpWaves), 0, L.stream, a);
+    const u32 tiles = (a.ff + 31) / 32 * moe_hits(a.n_tokens, a.top_k, a.n_experts);
+    if (a.hidden <= 256 * 2 * kMoeUpWaves && tiles >= 512) moe_up<ET, 2, true>(L, a);
+    else moe_up<ET, 1, false>(L, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const dim3 grid((a.hidden + 15) / 16), threads(64 * kMoeDownWaves);
-    if (a.n_tokens <= 16) hipLaunchKernelGGL((k_mx4_moe_down<ET, 1>), grid, threads, hits * 16, L.stream, a);
-    else hipLaunchKernelGGL((k_mx4_moe_down<ET, 4>), grid, threads, hits * 64, L.stream, a);
+    if (a.n_tokens > 16) moe_down<ET, 8, 4>(L, a);
+    else if (a.hidden < 4096 && ET != kElemF32) moe_down<ET, 16, 1>(L, a);
+    else moe_down<ET, 8, 1>(L, a);
     return hipGetLastError();
 }
 
-size_t mx4_moe_work(int n_tokens, int top_k, int, int ff) { return (size_t)n_tokens * top_k * 3 * ((ff + 31) / 32 * 32) * 2; }
+static size_t moe_table(int n_tokens, int top_k) { return offsetof(MoeTable, slot) + (size_t)moe_hits(n_tokens, top_k, kMoeExperts) * sizeof(MoeTable::slot[0]); }
+size_t mx4_moe_work(int n_tokens, int top_k, int, int ff) { return moe_table(n_tokens, top_k) + (size_t)n_tokens * top_k * 3 * ((ff + 31) / 32 * 32) * 2; }
 
 hipError_t mx4_moe(const Launch &L, const Mx4Stack &g, const Mx4Stack &u, const Mx4Stack &d, int n_experts, int hidden, int ff, const void *x, int et,
                    int64_t ld_x, int n_tokens, const uint32_t *sel, const float *w, int top_k, const void *resid, int64_t ld_resid, void *y, int64_t ld_y,
                    void *work) {
     const Mx4Moe a = {g.w, g.scales, u.w, u.scales, d.w, d.scales, (u32)n_experts, (u32)hidden, (u32)ff, (u32)n_tokens, (u32)top_k, x, resid, (size_t)ld_x,
-                      (size_t)ld_resid, (size_t)ld_y, sel, w, (__bf16 *)work, y, L.rule, L.fault, L.layer};
+                      (size_t)ld_resid, (size_t)ld_y, sel, w, (MoeTable *)work, (__bf16 *)((uint8_t *)work + moe_table(n_tokens, top_k)), y, L.rule, L.fault,
+                      L.layer};
     if (et == kElemF32) return moe_launch<kElemF32>(L, a);
     if (et == kElemF16) return moe_launch<kElemF16>(L, a);
     return moe_launch<kElemBF16>(L, a);
