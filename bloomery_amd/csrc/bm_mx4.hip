@@ -906,12 +906,12 @@ hipError_t mx4_gemm(const Launch &L, const uint8_t *w, const uint8_t *ws, int n_
 // become bf16 values exactly, a few instructions for eight, and the products run on the bf16 matrix instructions, the tokens' values in parts that
 // add up to them: one of bf16, two of f16, three of f32, and of h two (f32: three).
 
-// What the first launch leaves for the second: the experts that are hit, ascending, and their tokens' slots, of a token that picked an expert twice the
-// first.
-constexpr u32 kMoeExperts = 1024;
+// What the first launch leaves for the second: the experts that are hit, ascending, and for each the slot by which a token picked it, the first if
+// there are several, kMoeNone for none.
+constexpr u32 kMoeExperts = 1024, kMoeNone = 0xffff;
 struct MoeTable {
     u32 n_hit, unused[15];
-    uint16_t expert[kMoeExperts], count[kMoeExperts], slot[kMoeExperts][kMx4MoeTokens];
+    uint16_t expert[kMoeExperts], slot[kMoeExperts][kMx4MoeTokens];
 };
 struct Mx4Moe {
     const uint8_t *wg, *wgs, *wu, *wus, *wd, *wds;
@@ -969,6 +969,8 @@ __device__ __forceinline__ bool moe_nth(const u32 *bits, u32 n, u32 &expert, u32
     return true;
 }
 
+// Has the compiler take w anew: what is made of it in a loop stays there, and does not wait in registers (eight times as many) for all of them.
+__device__ __forceinline__ void moe_anew(v4i &w) { __asm__ volatile("" : "+v"(w)); }
 // Eight codes as bf16 values under their scale.
 __device__ __forceinline__ v8h moe_codes(u32 word, float s) {
     const v2h p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 1),
@@ -983,6 +985,13 @@ __device__ __forceinline__ v8h moe_as_parts(uint4 p) {
     __builtin_memcpy(&r, &p, 16);
     return r;
 }
+// A value's first eight bits of mantissa.
+__device__ __forceinline__ __bf16 moe_cut(float v) {
+    const uint16_t high = (uint16_t)(bm_f32_bits(v) >> 16);
+    __bf16 r;
+    __builtin_memcpy(&r, &high, 2);
+    return r;
+}
 // Eight values in P parts: what a part leaves is the next one's, the last rounded where something is left.
 template <int P>
 __device__ __forceinline__ void moe_split(const float (&x)[8], v8h (&part)[P]) {
@@ -991,7 +1000,7 @@ __device__ __forceinline__ void moe_split(const float (&x)[8], v8h (&part)[P]) {
     for (int j = 0; j < 8; j++) rest[j] = x[j];
 #pragma unroll
     for (int p = 0; p < P; p++) {
-        if (p == P - 1) {
+        if (p == P - 1) { // bf16's own rounding, and f16's second part, to nearest even
 #pragma unroll
             for (int j = 0; j < 8; j++) part[p][j] = (__bf16)rest[j];
             break;
@@ -1007,47 +1016,38 @@ __device__ __forceinline__ void moe_split(const float (&x)[8], v8h (&part)[P]) {
 template <int ET>
 constexpr int kMoeParts = ET == kElemBF16 ? 1 : ET == kElemF16 ? 2 : 3; // of an x
 template <int ET>
-constexpr int kMoeKept = ET == kElemF32 ? 3 : 2; // of an h
+constexpr int kMoeKept = kMoeParts<ET>; // of an h: as the type's own rows would hold it, at least
 
-// A lane's 64 values of a line of x, two blocks, eight at a time.
+// Eight neighbouring values of a row on their way, those behind its end zeros.
 template <int ET>
-struct MoeX {
+struct MoePiece {
     static constexpr int V = kElemPiece<ET>, N = 8 / V;
-    uint4 raw[8][N];
+    uint4 raw[N];
     __device__ __forceinline__ void ask(const void *x, size_t row, u32 first, u32 k) {
-        if (first + 64 <= k) {
+        if (first + 8 <= k) {
 #pragma unroll
-            for (int i = 0; i < 8; i++)
+            for (int n = 0; n < N; n++) raw[n] = elem_piece<ET>(x, row + first + n * V);
+            return;
+        }
+        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (first < k) elem_load_some<ET, 8>(x, row + first, k - first, v);
 #pragma unroll
-                for (int n = 0; n < N; n++) raw[i][n] = elem_piece<ET>(x, row + first + 8 * i + n * V);
-        } else {
-            for (int i = 0; i < 8; i++) {
-                float v[8];
+        for (int n = 0; n < N; n++) {
+            float e[V];
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = 0.0f;
-                if (first + 8 * i < k) elem_load_some<ET, 8>(x, row + first + 8 * i, k - first - 8 * i, v);
-#pragma unroll
-                for (int n = 0; n < N; n++) {
-                    float e[V];
-#pragma unroll
-                    for (int j = 0; j < V; j++) e[j] = v[n * V + j];
-                    const uint4 p = elem_pack<ET>(e);
-#pragma unroll
-                    for (int ii = 0; ii < 8; ii++)
-                        if (ii == i) raw[ii][n] = p;
-                }
-            }
+            for (int j = 0; j < V; j++) e[j] = v[n * V + j];
+            raw[n] = elem_pack<ET>(e);
         }
     }
-    __device__ __forceinline__ void parts(int i, v8h (&part)[kMoeParts<ET>]) const {
+    __device__ __forceinline__ void parts(v8h (&part)[kMoeParts<ET>]) const {
         if constexpr (ET == kElemBF16) {
-            part[0] = moe_as_parts(raw[i][0]);
+            part[0] = moe_as_parts(raw[0]);
         } else {
             float v[8];
 #pragma unroll
             for (int n = 0; n < N; n++) {
                 float e[V];
-                elem_unpack<ET>(raw[i][n], e);
+                elem_unpack<ET>(raw[n], e);
 #pragma unroll
                 for (int j = 0; j < V; j++) v[n * V + j] = e[j];
             }
@@ -1055,18 +1055,39 @@ struct MoeX {
         }
     }
 };
+// A line's values of a token in LDS: a part of 256, sixteen bytes behind every 256 for the banks; what the matrix instructions take begins at moe_at.
+constexpr int kMoePart = 544;
+__device__ __forceinline__ u32 moe_put(u32 piece) { return 16 * piece + (piece & 16); }
+__device__ __forceinline__ u32 moe_at(u32 lane) { return 128 * (lane >> 4) + 16 * (lane >> 5); }
+// A wave's reads of LDS are done.
+__device__ __forceinline__ void lds_read() {
+    __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f); // lgkmcnt(0)
+    __asm__ volatile("" ::: "memory");
+}
+// The lowest N bits of m.
+template <int N>
+__device__ __forceinline__ unsigned long long moe_first(unsigned long long m) {
+    unsigned long long rest = m;
+#pragma unroll
+    for (int j = 0; j < N; j++) rest &= rest - 1;
+    return m ^ rest;
+}
 
-// h. T times sixteen rows of gate and as many of up; SHORT: a row's lines are two a wave at most, asked for at once.
+// h. T times sixteen rows of gate and as many of up, their lines dealt to the waves, each through S stages, of which all but one, or of two one, are on
+// their way while one is multiplied. A line's values of x come through LDS, UC tokens' at a time in parts, the next line's asked for in front of the weights: asked for in the matrix
+// instructions' form, each of sixteen requests a line would take the vector cache as long as a line of weights does.
 constexpr int kMoeUpWaves = 4;
-template <int ET, int T, bool SHORT>
-__global__ __launch_bounds__(64 * kMoeUpWaves) void k_mx4_moe_up(Mx4Moe a) {
-    constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, PH = kMoeKept<ET>, R = 2 * T, kLoads = 3 * R; // of a stage: 2 R of lines, R of scales
+template <int ET, int T, int S, int UC, int EU>
+__global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(EU))) void k_mx4_moe_up(Mx4Moe a) {
+    constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, PH = kMoeKept<ET>, R = 2 * T, kLoads = 3 * R, kRow = P * kMoePart; // loads of a stage: 2 R of lines, R of scales
     typedef Lines<2 * R> L;
-    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[SHORT ? 16 : NW * L::kStage], ring3[SHORT ? 16 : NW * L::kStage];
-    __shared__ u32 bits[kMoeExperts / 32], col_slot[16];
-    __shared__ float col_weight[16];
+    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[S > 2 ? NW * L::kStage : 16];
+    __shared__ __align__(16) uint8_t rows[(NW * UC + 1) * kRow]; // the last: zeros
+    __shared__ u32 bits[kMoeExperts / 32], col_slot[16], col_token[16];
     extern __shared__ __align__(16) uint16_t sel[];
-    const u32 lane = threadIdx.x & 63, wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = blockIdx.y;
+    const u32 lane = threadIdx.x & 63, wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = blockIdx.y, c = lane & 15;
+    for (u32 i = threadIdx.x; i < kRow / 16; i += 64 * NW) reinterpret_cast<uint4 *>(rows + NW * UC * kRow)[i] = make_uint4(0, 0, 0, 0);
     moe_picks<64 * NW>(a, bits, sel, blockIdx.x == 0 && n == 0);
     u32 expert, n_hit;
     const bool there = moe_nth(bits, n, expert, n_hit);
@@ -1083,8 +1104,8 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) void k_mx4_moe_up(Mx4Moe a) {
     for (u32 g = 0; g < 2 * R; g++) // rows past the last are the last once more, and their values zeros
         src.from[g] = (const int8_t *)(g < R ? a.wg : a.wu) + (stack + min(r0 + 8 * (g % R) + (lane >> 3), a.ff - 1)) * kp;
 #pragma unroll
-    for (u32 g = 0; g < R; g++) scales[g] = (g < T ? a.wgs : a.wus) + (stack + min(r0 + 16 * (g % T) + (lane & 15), a.ff - 1)) * ks + at;
-    u32 s0[R], s1[R], s2[R], s3[R];
+    for (u32 g = 0; g < R; g++) scales[g] = (g < T ? a.wgs : a.wus) + (stack + min(r0 + 16 * (g % T) + c, a.ff - 1)) * ks + at;
+    u32 s0[R], s1[R], s2[R];
     const auto ask = [&](uint8_t *stage, u32 (&s)[R], u32 l) {
 #pragma unroll
         for (int g = 0; g < R; g++) s[g] = mx4_two(scales[g] + 8 * l);
@@ -1092,85 +1113,107 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) void k_mx4_moe_up(Mx4Moe a) {
         src.ask(stage + mine, l, kp);
         __builtin_amdgcn_sched_barrier(0);
     };
-    const auto begin = [&] {
-        if (wave < lines) ask(ring0, s0, wave);
-        if (wave + NW < lines) ask(ring1, s1, wave + NW);
-        if (!SHORT && wave + 2 * NW < lines) ask(ring2, s2, wave + 2 * NW);
-    };
-    begin();
 
-    // lane t: token t's first slot of this expert, and its weight, over all its slots of it
-    u32 slot = 0;
-    float weight = 0.0f;
-    bool user = false;
+    // lane t: token t's first slot of this expert
+    u32 slot = kMoeNone;
     if (lane < a.n_tokens)
         for (u32 s = a.top_k; s-- > 0;)
-            if (sel[lane * a.top_k + s] == expert) {
-                slot = lane * a.top_k + s;
-                weight = __fadd_rn(a.w[slot], weight);
-                user = true;
-            }
-    const unsigned long long users = __ballot(user);
+            if (sel[lane * a.top_k + s] == expert) slot = lane * a.top_k + s;
+    const unsigned long long users = __ballot(slot != kMoeNone);
     const u32 n_users = (u32)__builtin_popcountll(users), place = (u32)__builtin_popcountll(users & ((1ull << lane) - 1));
     if (blockIdx.x == 0 && wave == 0) {
-        if (lane == 0) {
-            a.table->expert[n] = (uint16_t)expert;
-            a.table->count[n] = (uint16_t)n_users;
-        }
-        if (user) a.table->slot[n][place] = (uint16_t)slot;
+        if (lane == 0) a.table->expert[n] = (uint16_t)expert;
+        a.table->slot[n][lane] = (uint16_t)slot;
     }
     for (u32 z = 0; z < n_users; z += 16) {
-        if (user && place - z < 16) {
+        const u32 columns = min(n_users - z, 16u);
+        if (slot != kMoeNone && place - z < 16) {
             col_slot[place - z] = slot;
-            col_weight[place - z] = weight;
+            col_token[place - z] = lane;
         }
         __syncthreads();
-        if (z) begin();
-        const u32 my_slot = col_slot[min(lane & 15, min(n_users - z, 16u) - 1)]; // columns past the last are the last once more, and not stored
-        const size_t row = (size_t)(my_slot / a.top_k) * a.ld_x;
+        // lanes 0 to 31 take one token's values of a line, eight each, lanes 32 to 63 the next one's
+        MoePiece<ET> held[UC / 2];
+        size_t row_of[UC / 2]; // of the first UC columns
+#pragma unroll
+        for (int j = 0; j < UC / 2; j++) row_of[j] = (size_t)col_token[min(2 * j + (lane >> 5), columns - 1)] * a.ld_x;
+        const auto fetch = [&](u32 l) {
+#pragma unroll
+            for (int j = 0; j < UC / 2; j++)
+                if (2 * j + (lane >> 5) < columns) held[j].ask(a.x, row_of[j], 256 * l + 8 * (lane & 31), a.hidden);
+        };
+        const auto put = [&](const MoePiece<ET> (&from)[UC / 2], u32 first) {
+#pragma unroll
+            for (int j = 0; j < UC / 2; j++) {
+                if (first + 2 * j + (lane >> 5) >= columns) continue;
+                v8h part[P];
+                from[j].parts(part);
+                uint8_t *to = rows + (wave * UC + 2 * j + (lane >> 5)) * kRow + moe_put(lane & 31);
+#pragma unroll
+                for (int p = 0; p < P; p++) *reinterpret_cast<v8h *>(to + p * kMoePart) = part[p];
+            }
+        };
+        if (wave < lines) fetch(wave);
+        __builtin_amdgcn_sched_barrier(0);
+        if (wave < lines) ask(ring0, s0, wave);
+        if (wave + NW < lines) ask(ring1, s1, wave + NW);
         v4f acc[R];
 #pragma unroll
         for (int g = 0; g < R; g++) acc[g] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        const auto step = [&](const uint8_t *stage, u32 (&s)[R], uint8_t *free, u32 (&next)[R], u32 l) {
-            MoeX<ET> x;
-            x.ask(a.x, row, 256 * l + 32 * at, a.hidden);
-            __builtin_amdgcn_sched_barrier(0);
-            const bool more = !SHORT && l + 3 * NW < lines;
-            if (more) ask(free, next, l + 3 * NW);
-            if (more) loads_landed<kLoads>();
+        const auto step = [&](uint8_t *stage, u32 (&s)[R], uint8_t *free, u32 (&next)[R], u32 l) {
+            if (l + NW < lines) loads_landed<kLoads>(); // the next stage may be on its way; this line's values of x are older than it
             else loads_landed<0>();
+            put(held, 0);
+            if (l + NW < lines) fetch(l + NW);
+            __builtin_amdgcn_sched_barrier(0);
+            if (S > 2 && l + 2 * NW < lines) ask(free, next, l + 2 * NW);
             v4i w[R][2];
-            u32 two[R];
+            float by[R][2];
 #pragma unroll
             for (int g = 0; g < R; g++) {
-                two[g] = mx4_scales(s[g], 8 * l + at, blocks);
+                const u32 two = mx4_scales(s[g], 8 * l + at, blocks);
 #pragma unroll
-                for (int h = 0; h < 2; h++) w[g][h] = mx4_of_line(stage + mine, lane, g, h);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                v8h part[P];
-                x.parts(i, part);
-#pragma unroll
-                for (int g = 0; g < R; g++) {
-                    const v8h c = moe_codes((u32)w[g][i / 4][i % 4], moe_scale(two[g], i / 4));
-#pragma unroll
-                    for (int p = 0; p < P; p++) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(c, part[p], acc[g], 0, 0, 0);
+                for (int h = 0; h < 2; h++) {
+                    w[g][h] = mx4_of_line(stage + mine, lane, g, h);
+                    by[g][h] = moe_scale(two, h);
                 }
             }
+            if (S == 2 && l + 2 * NW < lines) {
+                lds_read(); // the stage is in registers
+                ask(stage, s, l + 2 * NW);
+            }
+            for (u32 first = 0;;) {
+#pragma unroll
+                for (int g = 0; g < R; g++) moe_anew(w[g][0]), moe_anew(w[g][1]);
+                const uint8_t *row = rows + (c - first < (u32)UC && c < columns ? wave * UC + c - first : (u32)(NW * UC)) * kRow + moe_at(lane);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    v8h value[P];
+#pragma unroll
+                    for (int p = 0; p < P; p++) value[p] = *reinterpret_cast<const v8h *>(row + p * kMoePart + 16 * i);
+#pragma unroll
+                    for (int g = 0; g < R; g++) {
+                        const v8h code = moe_codes((u32)w[g][i / 4][i % 4], by[g][i / 4]);
+#pragma unroll
+                        for (int p = 0; p < P; p++) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code, value[p], acc[g], 0, 0, 0);
+                    }
+                }
+                if ((first += UC) >= columns) break;
+                MoePiece<ET> more[UC / 2];
+#pragma unroll
+                for (int j = 0; j < UC / 2; j++)
+                    if (const u32 column = first + 2 * j + (lane >> 5); column < columns)
+                        more[j].ask(a.x, (size_t)col_token[column] * a.ld_x, 256 * l + 8 * (lane & 31), a.hidden);
+                put(more, first);
+            }
         };
-        if constexpr (SHORT) {
-            if (wave < lines) step(ring0, s0, nullptr, s3, wave);
-            if (wave + NW < lines) step(ring1, s1, nullptr, s3, wave + NW);
-        } else {
-            for (u32 l = wave; l < lines;) {
-                step(ring0, s0, ring3, s3, l);
-                if ((l += NW) >= lines) break;
-                step(ring1, s1, ring0, s0, l);
-                if ((l += NW) >= lines) break;
+        for (u32 l = wave; l < lines;) {
+            step(ring0, s0, ring2, s2, l);
+            if ((l += NW) >= lines) break;
+            step(ring1, s1, ring0, s0, l);
+            if ((l += NW) >= lines) break;
+            if (S > 2) {
                 step(ring2, s2, ring1, s1, l);
-                if ((l += NW) >= lines) break;
-                step(ring3, s3, ring2, s2, l);
                 l += NW;
             }
         }
@@ -1178,206 +1221,250 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) void k_mx4_moe_up(Mx4Moe a) {
 #pragma unroll
         for (int g = 0; g < R; g++) *reinterpret_cast<v4f *>(ring0 + mine + g * 1024 + 16 * lane) = acc[g];
         __syncthreads();
-        const u32 c = lane & 15, f = r0 + 16 * wave + 4 * (lane >> 4);
-        if (wave < T && f < ffp && z + c < n_users) {
-            const v4f g = mx4_join<NW, L>(ring0, wave, lane), u = mx4_join<NW, L>(ring0, T + wave, lane);
-            const float by = col_weight[c];
-            float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-            bool odd = false;
+        // a thread a value: row threadIdx.x % 16 of each sixteen, column threadIdx.x / 16
+        static_assert(64 * NW == 256, "sixteen rows by sixteen columns");
+        const u32 column = threadIdx.x >> 4;
+        if (column < columns) {
+            const u32 of = col_slot[column], first_slot = col_token[column] * a.top_k;
+            float by = 0.0f; // the token's weights of all its slots of this expert
+            for (u32 s = of; s < first_slot + a.top_k; s++)
+                if (sel[s] == expert) by = __fadd_rn(by, a.w[s]);
+#pragma unroll 1
+            for (int t = 0; t < T; t++) {
+                const u32 f = r0 + 16 * t + (threadIdx.x & 15);
+                if (f >= ffp) break;
+                const uint8_t *from = ring0 + 256 * (threadIdx.x >> 2 & 3) + 16 * column + 4 * (threadIdx.x & 3) + t * 1024;
+                float g = 0.0f, u = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                bool o = false;
-                if (f + j < a.ff) v[j] = __fmul_rn(bm_gate_rule(a.rule.act, a.rule.limit, g[j], u[j], o), by);
-                odd |= o;
-            }
-            if (odd) bm_raise(a.fault, a.layer, kSiteF32Product);
-            v8h part[PH];
-            moe_split<PH>(v, part);
-            __bf16 *to = a.h + (size_t)my_slot * PH * ffp + f;
+                for (int w = 0; w < NW; w++) {
+                    g = __fadd_rn(g, *reinterpret_cast<const float *>(from + w * L::kStage));
+                    u = __fadd_rn(u, *reinterpret_cast<const float *>(from + w * L::kStage + T * 1024));
+                }
+                bool odd = false;
+                float v = 0.0f;
+                if (f < a.ff) v = __fmul_rn(bm_gate_rule(a.rule.act, a.rule.limit, g, u, odd), by);
+                if (odd) bm_raise(a.fault, a.layer, kSiteF32Product);
+                __bf16 *to = a.h + (size_t)of * PH * ffp + f;
 #pragma unroll
-            for (int p = 0; p < PH; p++) {
-                *reinterpret_cast<uint2 *>(to + (size_t)p * ffp) = *reinterpret_cast<const uint2 *>(&part[p]);
-                if (T == 1 && r0 + 16 >= a.ff && r0 + 16 < ffp) *reinterpret_cast<uint2 *>(to + (size_t)p * ffp + 16) = make_uint2(0, 0); // the last block's other half
+                for (int p = 0; p < PH; p++) {
+                    const __bf16 part = p == PH - 1 ? (__bf16)v : moe_cut(v);
+                    v = __fsub_rn(v, (float)part);
+                    to[(size_t)p * ffp] = part;
+                    if (T == 1 && r0 + 16 >= a.ff && r0 + 16 < ffp) to[(size_t)p * ffp + 16] = (__bf16)0.0f; // the last block's other half
+                }
             }
         }
         __syncthreads();
     }
 }
 
-// y. The lines of the experts that are hit, one expert's after another's, are dealt to the waves in stretches; a wave adds an expert's sums of its tokens, sixteen
-// at a time, onto its own of all tokens, in LDS, when it has done with the expert. NZ: sixteens of tokens there may be.
-template <int ET, int NW, int NZ>
+// y. The lines of the experts that are hit, one expert's after another's, are dealt to the waves in stretches, each through two stages of 16 R rows; the
+// waves' sums, NT tiles of sixteen tokens, meet in LDS. A line's values of h come through LDS too, UC tokens' at a time and the next line's asked for in front of the
+// weights.
+template <int ET, int NW, int R, int UC, int NT>
 __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
-    constexpr int PH = kMoeKept<ET>, kLoads = 3; // of a stage: two of lines, one of scales
-    typedef Lines<2> L;
-    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[NW * L::kStage], ring3[NW * L::kStage];
+    constexpr int PH = kMoeKept<ET>, NL = (PH + 1) / 2, CH = NT * R == 1 ? 2 : 1; // requests of a token's values; chains of products
+    constexpr int kLoads = 3 * R, kRow = PH * kMoePart;                          // loads of a stage
+    typedef Lines<2 * R> L;
+    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage];
+    __shared__ __align__(16) uint8_t rows[(NW * UC + 1) * kRow]; // the last: zeros
     __shared__ __align__(16) uint16_t list[kMoeExperts];
-    extern __shared__ __align__(16) float sums[]; // waves x tokens x 16
     const u32 lane = threadIdx.x & 63, wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), at = 2 * (lane >> 4), c = lane & 15;
     const u32 n_hit = a.table->n_hit;
     for (u32 i = threadIdx.x; 2 * i < a.n_experts; i += 64 * NW) reinterpret_cast<u32 *>(list)[i] = reinterpret_cast<const u32 *>(a.table->expert)[i];
-    float *const my_sums = sums + wave * a.n_tokens * 16;
-    for (u32 i = lane; i < a.n_tokens * 4; i += 64) *reinterpret_cast<v4f *>(my_sums + 4 * i) = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (u32 i = threadIdx.x; i < kRow / 16; i += 64 * NW) reinterpret_cast<uint4 *>(rows + NW * UC * kRow)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
 
     const u32 kp = (a.ff + 31) / 32 * 16, ks = (a.ff + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage;
-    const u32 r0 = blockIdx.x * 16, ffp = (a.ff + 31) / 32 * 32, items = n_hit * lines, q0 = items * wave / NW, q1 = items * (wave + 1) / NW;
+    const u32 r0 = blockIdx.x * (16 * R), ffp = (a.ff + 31) / 32 * 32, items = n_hit * lines, q0 = items * wave / NW, q1 = items * (wave + 1) / NW;
     L src;
     src.begin(lane);
-    const size_t from[2] = {(size_t)min(r0 + (lane >> 3), a.hidden - 1) * kp, (size_t)min(r0 + 8 + (lane >> 3), a.hidden - 1) * kp}; // rows past the last are not stored
-    const size_t mark = (size_t)min(r0 + c, a.hidden - 1) * ks + at;
-    u32 ask_n = q0 / lines, ask_l = q0 - ask_n * lines, ask_q = q0, n = ask_n, l = ask_l;
-    u32 s0 = 0, s1 = 0, s2 = 0, s3 = 0;
-    const auto ask = [&](uint8_t *stage, u32 &s) {
-        const u32 e = (u32)__builtin_amdgcn_readfirstlane(list[ask_n]);
-        s = mx4_two(a.wds + (size_t)e * a.hidden * ks + mark + 8 * ask_l);
+    size_t from[2 * R], mark[R]; // rows past the last are the last once more, and not stored
 #pragma unroll
-        for (int g = 0; g < 2; g++) src.from[g] = (const int8_t *)a.wd + (size_t)e * a.hidden * kp + from[g];
+    for (u32 g = 0; g < 2 * R; g++) from[g] = (size_t)min(r0 + 8 * g + (lane >> 3), a.hidden - 1) * kp;
+#pragma unroll
+    for (u32 g = 0; g < R; g++) mark[g] = (size_t)min(r0 + 16 * g + c, a.hidden - 1) * ks + at;
+    u32 n = q0 / lines, l = q0 - n * lines, ask_n = n, ask_l = l, ask_q = q0;
+    u32 s0[R], s1[R];
+    const auto ask = [&](uint8_t *stage, u32 (&s)[R]) {
+        const u32 e = (u32)__builtin_amdgcn_readfirstlane(list[ask_n]);
+#pragma unroll
+        for (int g = 0; g < R; g++) s[g] = mx4_two(a.wds + (size_t)e * a.hidden * ks + mark[g] + 8 * ask_l);
+#pragma unroll
+        for (int g = 0; g < 2 * R; g++) src.from[g] = (const int8_t *)a.wd + (size_t)e * a.hidden * kp + from[g];
         __builtin_amdgcn_sched_barrier(0);
         src.ask(stage + mine, ask_l, kp);
         __builtin_amdgcn_sched_barrier(0);
         ask_q++;
         if (++ask_l == lines) ask_l = 0, ask_n++;
     };
-    if (ask_q < q1) ask(ring0, s0);
-    if (ask_q < q1) ask(ring1, s1);
-    if (ask_q < q1) ask(ring2, s2);
 
-    v4f acc[NZ], odd_acc;
-    u32 users, slots[NZ], next_users = 0, next_slots[NZ];
-    const auto look = [&](u32 e) { // the e-th expert's users
-        if (e < n_hit) {
-            next_users = a.table->count[e];
+    // The tokens of an expert: lane t's slot, and those that have one, as bits.
+    u32 slot = kMoeNone, next_slot = kMoeNone;
+    unsigned long long users = 0;
+    const u32 part_at = (lane >> 5) * ffp + 8 * (lane & 31), put_at = (lane >> 5) * kMoePart + moe_put(lane & 31);
+    uint4 held[UC * NL];
+    // Line `line` of the tokens that `some` holds, the first UC of them.
+    const auto fetch = [&](unsigned long long some, u32 slots, u32 line) {
 #pragma unroll
-            for (int z = 0; z < NZ; z++)
-                if ((u32)z * 16 < a.n_tokens) next_slots[z] = a.table->slot[e][16 * z + c];
-        }
-    };
-    const auto turn = [&] { // to the expert that was looked at
-        users = (u32)__builtin_amdgcn_readfirstlane((int)next_users);
+        for (int j = 0; j < UC; j++) {
+            if (some) {
+                const u32 of = (u32)__builtin_amdgcn_readlane((int)slots, __builtin_ctzll(some));
+                const __bf16 *h = a.h + (size_t)of * PH * ffp + 256 * line + part_at;
+                const bool there = 8 * line + (lane & 31) / 4 < blocks;
 #pragma unroll
-        for (int z = 0; z < NZ; z++) {
-            slots[z] = next_slots[z];
-            acc[z] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-        odd_acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        look(n + 1);
-    };
-    const auto leave = [&] {
-        acc[0] += odd_acc;
-#pragma unroll
-        for (int z = 0; z < NZ; z++)
-            if (16 * z + c < users) *reinterpret_cast<v4f *>(my_sums + slots[z] / a.top_k * 16 + 4 * (lane >> 4)) += acc[z];
-    };
-    const auto values = [&](int z, v8h (&part)[8][PH]) { // a lane's 64 values of h
-        if (16 * z + c >= users) return; // (a column that is not looked at)
-        const u32 block = 8 * l + at;
-        const __bf16 *h = a.h + (size_t)slots[z] * PH * ffp + 32 * block;
-        if (8 * l + 8 <= blocks) {
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-#pragma unroll
-                for (int p = 0; p < PH; p++) part[i][p] = moe_as_parts(*reinterpret_cast<const uint4 *>(h + (size_t)p * ffp + 8 * i));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-#pragma unroll
-                for (int p = 0; p < PH; p++) {
+                for (int i = 0; i < NL; i++) {
                     uint4 v = make_uint4(0, 0, 0, 0);
-                    if (block + i / 4 < blocks) v = *reinterpret_cast<const uint4 *>(h + (size_t)p * ffp + 8 * i);
-                    part[i][p] = moe_as_parts(v);
-                }
-        }
-    };
-    const auto step = [&](const uint8_t *stage, u32 &s, uint8_t *free, u32 &next) {
-        v8h part[8][PH];
-        values(0, part);
-        __builtin_amdgcn_sched_barrier(0);
-        if (ask_q < q1) {
-            ask(free, next);
-            loads_landed<kLoads>();
-        } else {
-            loads_landed<0>();
-        }
-        const u32 two = mx4_scales(s, 8 * l + at, blocks);
-        v4i w[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++) w[h] = mx4_of_line(stage + mine, lane, 0, h);
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const v8h code = moe_codes((u32)w[i / 4][i % 4], moe_scale(two, i / 4));
-            v4f &to = i & 1 ? odd_acc : acc[0];
-#pragma unroll
-            for (int p = 0; p < PH; p++) to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code, part[i][p], to, 0, 0, 0);
-        }
-#pragma unroll
-        for (int z = 1; z < NZ; z++)
-            if (16 * (u32)z < users) {
-                values(z, part);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const v8h code = moe_codes((u32)w[i / 4][i % 4], moe_scale(two, i / 4));
-#pragma unroll
-                    for (int p = 0; p < PH; p++) acc[z] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code, part[i][p], acc[z], 0, 0, 0);
+                    if (there && (2 * i + 1 < PH || lane < 32)) v = *reinterpret_cast<const uint4 *>(h + (size_t)(2 * i) * ffp);
+                    held[j * NL + i] = v;
                 }
             }
-        if (++l == lines) {
-            leave();
+            some &= some - 1;
+        }
+    };
+    const auto put = [&](unsigned long long some) {
+#pragma unroll
+        for (int j = 0; j < UC; j++) {
+            if (some)
+#pragma unroll
+                for (int i = 0; i < NL; i++)
+                    if (2 * i + 1 < PH || lane < 32) *reinterpret_cast<uint4 *>(rows + (wave * UC + j) * kRow + 2 * i * kMoePart + put_at) = held[j * NL + i];
+            some &= some - 1;
+        }
+    };
+    v4f acc[NT][R][CH];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int i = 0; i < CH; i++) acc[t][r][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    const auto step = [&](uint8_t *stage, u32 (&s)[R], u32 q) {
+        if (q + 1 < q1) loads_landed<kLoads>(); // the next stage may be on its way; this line's values of h are older than it
+        else loads_landed<0>();
+        unsigned long long some = moe_first<UC>(users), left = users ^ some;
+        put(some);
+        const bool turn = l + 1 == lines;
+        const unsigned long long next_users = turn ? __ballot(next_slot != kMoeNone) : users;
+        if (q + 1 < q1) fetch(moe_first<UC>(next_users), turn ? next_slot : slot, turn ? 0 : l + 1);
+        const u32 after = turn && n + 2 < n_hit ? a.table->slot[n + 2][lane] : kMoeNone;
+        __builtin_amdgcn_sched_barrier(0);
+        v4i w[R][2];
+        float by[R][2];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const u32 two = mx4_scales(s[r], 8 * l + at, blocks);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                w[r][h] = mx4_of_line(stage + mine, lane, r, h);
+                by[r][h] = moe_scale(two, h);
+            }
+        }
+        if (ask_q < q1) {
+            lds_read(); // the stage is in registers
+            ask(stage, s);
+        }
+        for (;;) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const u32 here = (u32)(some >> (16 * t)) & 0xffffu;
+                if (NT > 1 && here == 0) continue;
+#pragma unroll
+                for (int r = 0; r < R; r++) moe_anew(w[r][0]), moe_anew(w[r][1]);
+                const u32 before = (u32)__builtin_popcountll(some & ((1ull << (16 * t)) - 1)) + (u32)__builtin_popcount(here & ((1u << c) - 1));
+                const uint8_t *row = rows + (here >> c & 1 ? wave * UC + before : (u32)(NW * UC)) * kRow + moe_at(lane);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    v8h code[R];
+#pragma unroll
+                    for (int r = 0; r < R; r++) code[r] = moe_codes((u32)w[r][i / 4][i % 4], by[r][i / 4]);
+#pragma unroll
+                    for (int p = 0; p < PH; p++) {
+                        const v8h value = moe_as_parts(*reinterpret_cast<const uint4 *>(row + p * kMoePart + 16 * i));
+#pragma unroll
+                        for (int r = 0; r < R; r++) acc[t][r][i % CH] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code[r], value, acc[t][r][i % CH], 0, 0, 0);
+                    }
+                }
+            }
+            if (!left) break;
+            some = moe_first<UC>(left);
+            // (the values of the next line that are held are in LDS only after these)
+            uint4 keep[UC * NL];
+#pragma unroll
+            for (int i = 0; i < UC * NL; i++) keep[i] = held[i];
+            fetch(some, slot, l);
+            put(some);
+#pragma unroll
+            for (int i = 0; i < UC * NL; i++) held[i] = keep[i];
+            left ^= some;
+        }
+        if (turn) {
             l = 0, n++;
-            turn();
+            slot = next_slot, users = next_users, next_slot = after;
+        } else {
+            l++;
         }
     };
     if (q0 < q1) {
-        look(n);
-        turn();
+        slot = a.table->slot[n][lane];
+        if (n + 1 < n_hit) next_slot = a.table->slot[n + 1][lane];
+        users = __ballot(slot != kMoeNone);
+        fetch(moe_first<UC>(users), slot, l);
+        __builtin_amdgcn_sched_barrier(0);
+        ask(ring0, s0);
+        if (ask_q < q1) ask(ring1, s1);
         for (u32 q = q0;;) {
-            step(ring0, s0, ring3, s3);
+            step(ring0, s0, q);
             if (++q == q1) break;
-            step(ring1, s1, ring0, s0);
-            if (++q == q1) break;
-            step(ring2, s2, ring1, s1);
-            if (++q == q1) break;
-            step(ring3, s3, ring2, s2);
+            step(ring1, s1, q);
             if (++q == q1) break;
         }
-        if (l) leave();
     }
-    __syncthreads();
-    for (u32 i = threadIdx.x; i < a.n_tokens * 4; i += 64 * NW) {
-        const u32 token = i / 4, r = r0 + 4 * (i & 3);
-        if (r >= a.hidden) continue;
-        v4f sum = *reinterpret_cast<const v4f *>(sums + 4 * i);
-        for (u32 w = 1; w < NW; w++) sum += *reinterpret_cast<const v4f *>(sums + (w * a.n_tokens * 4 + i) * 4);
-        float v[4] = {sum[0], sum[1], sum[2], sum[3]};
-        const u32 have = a.hidden - r;
-        if (a.resid)
+    loads_landed<0>();
 #pragma unroll
-            for (u32 j = 0; j < 4; j++)
-                if (j < have) v[j] = __fadd_rn(v[j], elem_load1<ET>(a.resid, token * a.ld_resid + r + j));
-        elem_store_some<ET, 4>(a.y, token * a.ld_y + r, have, v);
+    for (int t = 0; t < NT; t++) {
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            v4f sum = acc[t][r][0];
+            if (CH > 1) sum += acc[t][r][CH - 1];
+            *reinterpret_cast<v4f *>(ring0 + mine + r * 1024 + 16 * lane) = sum;
+        }
+        __syncthreads();
+        const u32 token = 16 * t + c, row = r0 + 16 * wave + 4 * (lane >> 4);
+        if (wave < R && token < a.n_tokens && row < a.hidden) {
+            const v4f sum = mx4_join<NW, L>(ring0, wave, lane);
+            float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+            const u32 have = a.hidden - row;
+            if (a.resid)
+#pragma unroll
+                for (u32 j = 0; j < 4; j++)
+                    if (j < have) v[j] = __fadd_rn(v[j], elem_load1<ET>(a.resid, token * a.ld_resid + row + j));
+            elem_store_some<ET, 4>(a.y, token * a.ld_y + row, have, v);
+        }
+        __syncthreads();
     }
 }
 
 static u32 moe_hits(int n_tokens, int top_k, int n_experts) { return (u32)std::min(n_tokens * top_k, n_experts); }
-template <int ET, int T, bool SHORT>
+template <int ET, int T, int S, int UC, int EU>
 static void moe_up(const Launch &L, const Mx4Moe &a) {
-    hipLaunchKernelGGL((k_mx4_moe_up<ET, T, SHORT>), dim3((a.ff + 16 * T - 1) / (16 * T), moe_hits(a.n_tokens, a.top_k, a.n_experts)), dim3(64 * kMoeUpWaves),
+    hipLaunchKernelGGL((k_mx4_moe_up<ET, T, S, UC, EU>), dim3((a.ff + 16 * T - 1) / (16 * T), moe_hits(a.n_tokens, a.top_k, a.n_experts)), dim3(64 * kMoeUpWaves),
                        (a.n_tokens * a.top_k * 2 + 15) & ~15u, L.stream, a);
 }
-template <int ET, int NW, int NZ>
+template <int ET, int NW, int R, int UC, int NT>
 static void moe_down(const Launch &L, const Mx4Moe &a) {
-    hipLaunchKernelGGL((k_mx4_moe_down<ET, NW, NZ>), dim3((a.hidden + 15) / 16), dim3(64 * NW), NW * a.n_tokens * 64, L.stream, a);
+    hipLaunchKernelGGL((k_mx4_moe_down<ET, NW, R, UC, NT>), dim3((a.hidden + 16 * R - 1) / (16 * R)), dim3(64 * NW), 0, L.stream, a);
 }
 template <int ET>
 static hipError_t moe_launch(const Launch &L, const Mx4Moe &a) {
     const u32 tiles = (a.ff + 31) / 32 * moe_hits(a.n_tokens, a.top_k, a.n_experts);
-    if (a.hidden <= 256 * 2 * kMoeUpWaves && tiles >= 512) moe_up<ET, 2, true>(L, a);
-    else moe_up<ET, 1, false>(L, a);
+    if (a.hidden <= 256 * 2 * kMoeUpWaves && tiles >= 512) moe_up<ET, 2, 2, 2, 2>(L, a);
+    else moe_up<ET, 1, 3, kMoeParts<ET> == 1 ? 8 : 4, 2>(L, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.n_tokens > 16) moe_down<ET, 8, 4>(L, a);
-    else if (a.hidden < 4096 && ET != kElemF32) moe_down<ET, 16, 1>(L, a);
-    else moe_down<ET, 8, 1>(L, a);
+    if (a.hidden < 4096) a.n_tokens > 16 ? moe_down<ET, 16, 1, kMoeParts<ET> == 3 ? 3 : 4, 4>(L, a) : moe_down<ET, 16, 1, kMoeParts<ET> == 3 ? 3 : 4, 1>(L, a);
+    else a.n_tokens > 16 ? moe_down<ET, kMoeParts<ET> == 1 ? 16 : 8, 2, kMoeParts<ET> == 1 ? 3 : 4, 4>(L, a)
+                       : moe_down<ET, kMoeParts<ET> == 1 ? 16 : 8, 2, kMoeParts<ET> == 1 ? 3 : 4, 1>(L, a);
     return hipGetLastError();
 }
 

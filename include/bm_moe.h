@@ -584,7 +584,7 @@ int bm_mx4_gemm_experts(bm_ctx *ctx, const uint8_t *w_dev, const uint8_t *w_scal
 /* The experts' whole step for a few tokens (bm_moe_decode in this form; n_tokens 1 .. 64, top_k 1 .. 64, 1 .. 1024 experts), whose values stay
  * in floating point: for token t, slot s of its top_k, expert e = sel_dev[t * top_k + s]: g = wg[e] x[t], u = wu[e] x[t] (ff rows of hidden values each),
  * h = the rule's value of (g, u), and y[t] = resid[t] + the sum over s ascending of w_dev[t * top_k + s] * (wd[e] h) (hidden rows of ff values). Products and
- * sums are f32, h is kept to 16 bits of mantissa at least, and y is rounded once to elem_type, which x_dev, resid_dev (NULL: none) and y_dev share;
+ * sums are f32, h is kept as precisely as elem_type at least (f32: in f32), and y is rounded once to elem_type, which x_dev, resid_dev (NULL: none) and y_dev share;
  * y_dev may be resid_dev. An id of BM_HOST_SLOT is skipped; any other at or past n_experts raises BM_SITE_EXPERT_ID and adds nothing,
  * whatever its weight; an expert may stand at several slots of a token. rule NULL: the context's.
  * work_dev: bm_mx4_moe_work(..) bytes of scratch, 16-byte aligned, that holds nothing between calls: at most n_tokens * top_k * (8 * ff + 8 * hidden + 1024) + 65536.

@@ -366,8 +366,9 @@ def test_tables_that_are_none_are_skipped(gpu, held, rows):
 
 # ------------------------------------------------------------------------------------ a few tokens' experts
 
-# h and its rule: 16 bits of mantissa and the rule's f32 operations; in f32 the operations alone
-KEPT = {bm.F32: 2.0 ** -20, bm.F16: 2.0 ** -15, bm.BF16: 2.0 ** -15}
+# h and its rule: the rule's f32 operations, and what h is held in: f32's 24 bits, f16 rows' two parts of 8 and 8 (the first cut, the second rounded: off by
+# 2^-9 of what is below 2^-7), bf16 rows' one rounding, half a step
+KEPT = {bm.F32: 2.0 ** -20, bm.F16: 2.0 ** -15, bm.BF16: 2.0 ** -20 + HALF_STEP[bm.BF16]}
 
 
 class Stack:
