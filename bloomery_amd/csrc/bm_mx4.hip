@@ -1074,28 +1074,237 @@ __device__ __forceinline__ unsigned long long moe_first(unsigned long long m) {
     return m ^ rest;
 }
 
+// A workgroup's expert, the n-th that is hit: lane t of every wave has token t's first slot of it (kMoeNone: none) and its place among the expert's tokens. The
+// first workgroup of an expert leaves them for the second launch. False: there are not as many experts.
+struct MoeEntry {
+    u32 expert, slot, place, n_users;
+};
+template <int THREADS>
+__device__ __forceinline__ bool moe_entry(const Mx4Moe &a, u32 *bits, uint16_t *sel, u32 n, MoeEntry &e) {
+    const u32 lane = threadIdx.x & 63;
+    moe_picks<THREADS>(a, bits, sel, blockIdx.x == 0 && n == 0);
+    u32 n_hit;
+    const bool there = moe_nth(bits, n, e.expert, n_hit);
+    if (blockIdx.x == 0 && n == 0 && threadIdx.x == 0) a.table->n_hit = n_hit;
+    if (!there) return false;
+    e.slot = kMoeNone;
+    if (lane < a.n_tokens)
+        for (u32 s = a.top_k; s-- > 0;)
+            if (sel[lane * a.top_k + s] == e.expert) e.slot = lane * a.top_k + s;
+    const unsigned long long users = __ballot(e.slot != kMoeNone);
+    e.n_users = (u32)__builtin_popcountll(users);
+    e.place = (u32)__builtin_popcountll(users & ((1ull << lane) - 1));
+    if (blockIdx.x == 0 && threadIdx.x < 64) {
+        if (lane == 0) a.table->expert[n] = (uint16_t)e.expert;
+        a.table->slot[n][lane] = (uint16_t)e.slot;
+    }
+    return true;
+}
+// Up to sixteen of an expert's tokens, a column each.
+struct MoeColumns {
+    u32 slot[16], token[16];
+    float weight[16];
+};
+// The tokens from place z on.
+__device__ __forceinline__ void moe_columns(const MoeEntry &e, u32 z, u32 n, MoeColumns &col) {
+    if (e.slot == kMoeNone || e.place - z >= n) return;
+    col.slot[e.place - z] = e.slot;
+    col.token[e.place - z] = threadIdx.x & 63;
+}
+// And their weights, each over all of a token's slots of the expert. (Asked for behind the first lines, which are waited for anyway.)
+__device__ __forceinline__ void moe_weights(const Mx4Moe &a, const uint16_t *sel, const MoeEntry &e, u32 z, u32 n, MoeColumns &col) {
+    const u32 token = threadIdx.x & 63;
+    if (threadIdx.x >= 64 || e.slot == kMoeNone || e.place - z >= n) return;
+    float by = a.w[e.slot];
+    for (u32 s = e.slot + 1; s < (token + 1) * a.top_k; s++)
+        if (sel[s] == e.expert) by = __fadd_rn(by, a.w[s]);
+    col.weight[e.place - z] = by;
+}
+// Sixteen rows of h from r0 on, of as many columns as 256 threads have: a thread a value, row threadIdx.x % 16, column threadIdx.x / 16. gate, up: the first of
+// the waves' sums, `stride` bytes apart. ONE: the rows may end in the first half of a block, whose other half becomes zeros.
+template <int ET, int NW, bool ONE>
+__device__ __forceinline__ void moe_leave(const Mx4Moe &a, const MoeColumns &col, u32 columns, u32 r0, const uint8_t *gate, const uint8_t *up, u32 stride) {
+    constexpr int PH = kMoeKept<ET>;
+    static_assert(64 * NW == 256, "sixteen rows by sixteen columns");
+    const u32 column = threadIdx.x >> 4, f = r0 + (threadIdx.x & 15), ffp = (a.ff + 31) / 32 * 32;
+    if (column >= columns || f >= ffp) return;
+    const u32 of = col.slot[column], at = 256 * (threadIdx.x >> 2 & 3) + 16 * column + 4 * (threadIdx.x & 3);
+    float g = 0.0f, u = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+        g = __fadd_rn(g, *reinterpret_cast<const float *>(gate + w * stride + at));
+        u = __fadd_rn(u, *reinterpret_cast<const float *>(up + w * stride + at));
+    }
+    bool odd = false;
+    float v = 0.0f;
+    if (f < a.ff) v = __fmul_rn(bm_gate_rule(a.rule.act, a.rule.limit, g, u, odd), col.weight[column]);
+    if (odd) bm_raise(a.fault, a.layer, kSiteF32Product);
+    __bf16 *to = a.h + (size_t)of * PH * ffp + f;
+#pragma unroll
+    for (int p = 0; p < PH; p++) {
+        const __bf16 part = p == PH - 1 ? (__bf16)v : moe_cut(v);
+        v = __fsub_rn(v, (float)part);
+        to[(size_t)p * ffp] = part;
+        if (ONE && r0 + 16 >= a.ff && r0 + 16 < ffp) to[(size_t)p * ffp + 16] = (__bf16)0.0f;
+    }
+}
+constexpr int kMoeUpWaves = 4;
+
+// h of rows of up to 2048 values, two lines a wave at most: a workgroup goes over several tiles of sixteen rows of gate and as many of up, whose lines come through
+// a ring of S stages without a stop between the tiles; the tokens' values of a wave's lines stay in LDS, UC tokens' at a time.
+template <int ET, int S, int UC>
+__global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(2))) void k_mx4_moe_up_short(Mx4Moe a, u32 per) {
+    constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, kRow = P * kMoePart, kLoads = 6; // loads of a stage: four of lines, two of scales
+    typedef Lines<4> L;
+    static_assert(S == 2 || S == 3, "two or three stages");
+    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[S > 2 ? NW * L::kStage : 16];
+    __shared__ __align__(16) uint8_t sums[NW * 2048], rows[(NW * 2 * UC + 1) * kRow]; // the last row: zeros
+    __shared__ u32 bits[kMoeExperts / 32];
+    __shared__ MoeColumns col;
+    extern __shared__ __align__(16) uint16_t sel[];
+    const u32 lane = threadIdx.x & 63, wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = blockIdx.y, c = lane & 15;
+    for (u32 i = threadIdx.x; i < kRow / 16; i += 64 * NW) reinterpret_cast<uint4 *>(rows + NW * 2 * UC * kRow)[i] = make_uint4(0, 0, 0, 0);
+    MoeEntry entry;
+    if (!moe_entry<64 * NW>(a, bits, sel, n, entry)) return;
+
+    const u32 kp = (a.hidden + 31) / 32 * 16, ks = (a.hidden + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage, at = 2 * (lane >> 4);
+    const u32 tile0 = blockIdx.x * per, tiles = min(per, (a.ff + 15) / 16 - tile0), each = wave + NW < lines ? 2 : wave < lines ? 1 : 0, items = tiles * each; // this wave's
+    const size_t stack = (size_t)entry.expert * a.ff;
+    const uint8_t *const gate = a.wg + stack * kp, *const up = a.wu + stack * kp, *const gate_scales = a.wgs + stack * ks, *const up_scales = a.wus + stack * ks;
+    L src;
+    src.begin(lane);
+    u32 s0[2], s1[2], s2[2], asked = 0;
+    const auto ask = [&](uint8_t *stage, u32 (&s)[2]) {
+        const u32 tile = each == 2 ? asked >> 1 : asked, l = each == 2 && (asked & 1) ? wave + NW : wave, r0 = 16 * (tile0 + tile);
+        const u32 mark = min(r0 + c, a.ff - 1) * ks + at + 8 * l; // rows past the last are the last once more, and their values zeros
+        s[0] = mx4_two(gate_scales + mark);
+        s[1] = mx4_two(up_scales + mark);
+#pragma unroll
+        for (u32 g = 0; g < 4; g++) src.from[g] = (const int8_t *)(g < 2 ? gate : up) + (size_t)min(r0 + 8 * (g & 1) + (lane >> 3), a.ff - 1) * kp;
+        __builtin_amdgcn_sched_barrier(0);
+        src.ask(stage + mine, l, kp);
+        __builtin_amdgcn_sched_barrier(0);
+        asked++;
+    };
+    for (u32 z = 0; z < entry.n_users; z += UC) {
+        const u32 columns = min(entry.n_users - z, (u32)UC);
+        moe_columns(entry, z, UC, col);
+        __syncthreads();
+        // lanes 0 to 31 take one token's values of a line, eight each, lanes 32 to 63 the next one's
+        MoePiece<ET> held[2][UC / 2];
+#pragma unroll
+        for (u32 i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < UC / 2; j++)
+                if (const u32 column = 2 * j + (lane >> 5); i < each && column < columns)
+                    held[i][j].ask(a.x, (size_t)col.token[column] * a.ld_x, 256 * (wave + i * NW) + 8 * (lane & 31), a.hidden);
+        __builtin_amdgcn_sched_barrier(0);
+        asked = 0;
+        if (asked < items) ask(ring0, s0);
+        if (asked < items) ask(ring1, s1);
+#pragma unroll
+        for (u32 i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < UC / 2; j++)
+                if (const u32 column = 2 * j + (lane >> 5); i < each && column < columns) {
+                    v8h part[P];
+                    held[i][j].parts(part);
+                    uint8_t *to = rows + ((wave * 2 + i) * UC + column) * kRow + moe_put(lane & 31);
+#pragma unroll
+                    for (int p = 0; p < P; p++) *reinterpret_cast<v8h *>(to + p * kMoePart) = part[p];
+                }
+        moe_weights(a, sel, entry, z, UC, col);
+        v4f acc[2];
+        u32 done = 0, tile = 0;
+        const auto step = [&](uint8_t *stage, u32 (&s)[2], uint8_t *free, u32 (&next)[2]) {
+            const u32 i = each == 2 ? done & 1 : 0, l = wave + i * NW;
+            if (done + 1 < items) loads_landed<kLoads>(); // the next stage may be on its way
+            else loads_landed<0>();
+            if (S > 2 && asked < items) ask(free, next);
+            v4i w[2][2];
+            float by[2][2];
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                const u32 two = mx4_scales(s[g], 8 * l + at, blocks);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    w[g][h] = mx4_of_line(stage + mine, lane, g, h);
+                    by[g][h] = moe_scale(two, h);
+                }
+            }
+            if (S == 2 && asked < items) {
+                lds_read(); // the stage is in registers
+                ask(stage, s);
+            }
+            if (i == 0) acc[0] = acc[1] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            const uint8_t *row = rows + (c < columns ? (wave * 2 + i) * UC + c : (u32)(NW * 2 * UC)) * kRow + moe_at(lane);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                v8h value[P];
+#pragma unroll
+                for (int p = 0; p < P; p++) value[p] = *reinterpret_cast<const v8h *>(row + p * kMoePart + 16 * j);
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    const v8h code = moe_codes((u32)w[g][j / 4][j % 4], by[g][j / 4]);
+#pragma unroll
+                    for (int p = 0; p < P; p++) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code, value[p], acc[g], 0, 0, 0);
+                }
+            }
+            done++;
+        };
+        // A tile's sums meet: one barrier in front of the sums' reading and one behind it, neither of which waits for lines on their way.
+        const auto leave = [&] {
+#pragma unroll
+            for (int g = 0; g < 2; g++) *reinterpret_cast<v4f *>(sums + wave * 2048 + g * 1024 + 16 * lane) = each ? acc[g] : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            lds_meet();
+            moe_leave<ET, NW, true>(a, col, columns, 16 * (tile0 + tile), sums, sums + 1024, 2048);
+            lds_meet();
+            tile++;
+        };
+        const auto turn = [&] { // behind a step: whether its tile is done
+            if (each == 1 || !(done & 1)) leave();
+        };
+        if (each == 0) {
+            while (tile < tiles) leave();
+        } else {
+            for (;;) {
+                step(ring0, s0, ring2, s2);
+                turn();
+                if (done == items) break;
+                step(ring1, s1, ring0, s0);
+                turn();
+                if (done == items) break;
+                if (S > 2) {
+                    step(ring2, s2, ring1, s1);
+                    turn();
+                    if (done == items) break;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
 // h. T times sixteen rows of gate and as many of up, their lines dealt to the waves, each through S stages, of which all but one, or of two one, are on
 // their way while one is multiplied. A line's values of x come through LDS, UC tokens' at a time in parts, the next line's asked for in front of the weights: asked for in the matrix
 // instructions' form, each of sixteen requests a line would take the vector cache as long as a line of weights does.
-constexpr int kMoeUpWaves = 4;
 template <int ET, int T, int S, int UC, int EU>
 __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(EU))) void k_mx4_moe_up(Mx4Moe a) {
-    constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, PH = kMoeKept<ET>, R = 2 * T, kLoads = 3 * R, kRow = P * kMoePart; // loads of a stage: 2 R of lines, R of scales
+    constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, R = 2 * T, kLoads = 3 * R, kRow = P * kMoePart; // loads of a stage: 2 R of lines, R of scales
     typedef Lines<2 * R> L;
     __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[S > 2 ? NW * L::kStage : 16];
     __shared__ __align__(16) uint8_t rows[(NW * UC + 1) * kRow]; // the last: zeros
-    __shared__ u32 bits[kMoeExperts / 32], col_slot[16], col_token[16];
+    __shared__ u32 bits[kMoeExperts / 32];
+    __shared__ MoeColumns col;
     extern __shared__ __align__(16) uint16_t sel[];
     const u32 lane = threadIdx.x & 63, wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = blockIdx.y, c = lane & 15;
     for (u32 i = threadIdx.x; i < kRow / 16; i += 64 * NW) reinterpret_cast<uint4 *>(rows + NW * UC * kRow)[i] = make_uint4(0, 0, 0, 0);
-    moe_picks<64 * NW>(a, bits, sel, blockIdx.x == 0 && n == 0);
-    u32 expert, n_hit;
-    const bool there = moe_nth(bits, n, expert, n_hit);
-    if (blockIdx.x == 0 && n == 0 && threadIdx.x == 0) a.table->n_hit = n_hit;
-    if (!there) return;
+    MoeEntry entry;
+    if (!moe_entry<64 * NW>(a, bits, sel, n, entry)) return;
+    const u32 expert = entry.expert, n_users = entry.n_users;
 
     const u32 kp = (a.hidden + 31) / 32 * 16, ks = (a.hidden + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage, at = 2 * (lane >> 4);
-    const u32 r0 = blockIdx.x * (16 * T), ffp = (a.ff + 31) / 32 * 32;
+    const u32 r0 = blockIdx.x * (16 * T);
     L src;
     src.begin(lane);
     const size_t stack = (size_t)expert * a.ff;
@@ -1114,29 +1323,15 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
         __builtin_amdgcn_sched_barrier(0);
     };
 
-    // lane t: token t's first slot of this expert
-    u32 slot = kMoeNone;
-    if (lane < a.n_tokens)
-        for (u32 s = a.top_k; s-- > 0;)
-            if (sel[lane * a.top_k + s] == expert) slot = lane * a.top_k + s;
-    const unsigned long long users = __ballot(slot != kMoeNone);
-    const u32 n_users = (u32)__builtin_popcountll(users), place = (u32)__builtin_popcountll(users & ((1ull << lane) - 1));
-    if (blockIdx.x == 0 && wave == 0) {
-        if (lane == 0) a.table->expert[n] = (uint16_t)expert;
-        a.table->slot[n][lane] = (uint16_t)slot;
-    }
     for (u32 z = 0; z < n_users; z += 16) {
         const u32 columns = min(n_users - z, 16u);
-        if (slot != kMoeNone && place - z < 16) {
-            col_slot[place - z] = slot;
-            col_token[place - z] = lane;
-        }
+        moe_columns(entry, z, 16, col);
         __syncthreads();
         // lanes 0 to 31 take one token's values of a line, eight each, lanes 32 to 63 the next one's
         MoePiece<ET> held[UC / 2];
         size_t row_of[UC / 2]; // of the first UC columns
 #pragma unroll
-        for (int j = 0; j < UC / 2; j++) row_of[j] = (size_t)col_token[min(2 * j + (lane >> 5), columns - 1)] * a.ld_x;
+        for (int j = 0; j < UC / 2; j++) row_of[j] = (size_t)col.token[min(2 * j + (lane >> 5), columns - 1)] * a.ld_x;
         const auto fetch = [&](u32 l) {
 #pragma unroll
             for (int j = 0; j < UC / 2; j++)
@@ -1157,6 +1352,7 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
         __builtin_amdgcn_sched_barrier(0);
         if (wave < lines) ask(ring0, s0, wave);
         if (wave + NW < lines) ask(ring1, s1, wave + NW);
+        moe_weights(a, sel, entry, z, 16, col);
         v4f acc[R];
 #pragma unroll
         for (int g = 0; g < R; g++) acc[g] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -1203,7 +1399,7 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
                 for (int j = 0; j < UC / 2; j++)
                     if (const u32 column = first + 2 * j + (lane >> 5); column < columns)
-                        more[j].ask(a.x, (size_t)col_token[column] * a.ld_x, 256 * l + 8 * (lane & 31), a.hidden);
+                        more[j].ask(a.x, (size_t)col.token[column] * a.ld_x, 256 * l + 8 * (lane & 31), a.hidden);
                 put(more, first);
             }
         };
@@ -1221,39 +1417,9 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
         for (int g = 0; g < R; g++) *reinterpret_cast<v4f *>(ring0 + mine + g * 1024 + 16 * lane) = acc[g];
         __syncthreads();
-        // a thread a value: row threadIdx.x % 16 of each sixteen, column threadIdx.x / 16
-        static_assert(64 * NW == 256, "sixteen rows by sixteen columns");
-        const u32 column = threadIdx.x >> 4;
-        if (column < columns) {
-            const u32 of = col_slot[column], first_slot = col_token[column] * a.top_k;
-            float by = 0.0f; // the token's weights of all its slots of this expert
-            for (u32 s = of; s < first_slot + a.top_k; s++)
-                if (sel[s] == expert) by = __fadd_rn(by, a.w[s]);
 #pragma unroll 1
-            for (int t = 0; t < T; t++) {
-                const u32 f = r0 + 16 * t + (threadIdx.x & 15);
-                if (f >= ffp) break;
-                const uint8_t *from = ring0 + 256 * (threadIdx.x >> 2 & 3) + 16 * column + 4 * (threadIdx.x & 3) + t * 1024;
-                float g = 0.0f, u = 0.0f;
-#pragma unroll
-                for (int w = 0; w < NW; w++) {
-                    g = __fadd_rn(g, *reinterpret_cast<const float *>(from + w * L::kStage));
-                    u = __fadd_rn(u, *reinterpret_cast<const float *>(from + w * L::kStage + T * 1024));
-                }
-                bool odd = false;
-                float v = 0.0f;
-                if (f < a.ff) v = __fmul_rn(bm_gate_rule(a.rule.act, a.rule.limit, g, u, odd), by);
-                if (odd) bm_raise(a.fault, a.layer, kSiteF32Product);
-                __bf16 *to = a.h + (size_t)of * PH * ffp + f;
-#pragma unroll
-                for (int p = 0; p < PH; p++) {
-                    const __bf16 part = p == PH - 1 ? (__bf16)v : moe_cut(v);
-                    v = __fsub_rn(v, (float)part);
-                    to[(size_t)p * ffp] = part;
-                    if (T == 1 && r0 + 16 >= a.ff && r0 + 16 < ffp) to[(size_t)p * ffp + 16] = (__bf16)0.0f; // the last block's other half
-                }
-            }
-        }
+        for (int t = 0; t < T; t++)
+            moe_leave<ET, NW, T == 1>(a, col, columns, r0 + 16 * t, ring0 + t * 1024, ring0 + (T + t) * 1024, L::kStage);
         __syncthreads();
     }
 }
@@ -1451,14 +1617,18 @@ static void moe_up(const Launch &L, const Mx4Moe &a) {
     hipLaunchKernelGGL((k_mx4_moe_up<ET, T, S, UC, EU>), dim3((a.ff + 16 * T - 1) / (16 * T), moe_hits(a.n_tokens, a.top_k, a.n_experts)), dim3(64 * kMoeUpWaves),
                        (a.n_tokens * a.top_k * 2 + 15) & ~15u, L.stream, a);
 }
+template <int ET, int S, int UC>
+static void moe_up_short(const Launch &L, const Mx4Moe &a) {
+    const u32 tiles = (a.ff + 15) / 16, hits = moe_hits(a.n_tokens, a.top_k, a.n_experts), per = std::max(1u, tiles * hits / 1536);
+    hipLaunchKernelGGL((k_mx4_moe_up_short<ET, S, UC>), dim3((tiles + per - 1) / per, hits), dim3(64 * kMoeUpWaves), (a.n_tokens * a.top_k * 2 + 15) & ~15u, L.stream, a, per);
+}
 template <int ET, int NW, int R, int UC, int NT>
 static void moe_down(const Launch &L, const Mx4Moe &a) {
     hipLaunchKernelGGL((k_mx4_moe_down<ET, NW, R, UC, NT>), dim3((a.hidden + 16 * R - 1) / (16 * R)), dim3(64 * NW), 0, L.stream, a);
 }
 template <int ET>
 static hipError_t moe_launch(const Launch &L, const Mx4Moe &a) {
-    const u32 tiles = (a.ff + 31) / 32 * moe_hits(a.n_tokens, a.top_k, a.n_experts);
-    if (a.hidden <= 256 * 2 * kMoeUpWaves && tiles >= 512) moe_up<ET, 2, 2, 2, 2>(L, a);
+    if (a.hidden <= 256 * 2 * kMoeUpWaves) moe_up_short<ET, kMoeParts<ET> == 1 ? 3 : 2, kMoeParts<ET> == 3 ? 2 : 4>(L, a);
     else moe_up<ET, 1, 3, kMoeParts<ET> == 1 ? 8 : 4, 2>(L, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
