@@ -939,34 +939,61 @@ __device__ __forceinline__ u32 moe_upto(u32 v) {
     v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
     return v;
 }
-// The experts that the picks hit, as bits, and the picks; every thread of the workgroup takes part. An id that names no expert is 0xffff, and raised by
+// How often the picks name each expert, and the picks; every thread of the workgroup takes part. An id that names no expert is 0xffff, and raised by
 // `raise`'s workgroup.
+struct MoePicks {
+    u32 count[kMoeExperts / 2]; // two to a word
+};
 template <int T>
-__device__ __forceinline__ void moe_picks(const Mx4Moe &a, u32 *bits, uint16_t *sel, bool raise) {
+__device__ __forceinline__ void moe_picks(const Mx4Moe &a, MoePicks &p, uint16_t *sel, bool raise) {
     const u32 n = a.n_tokens * a.top_k;
     u32 e = threadIdx.x < n ? a.sel[threadIdx.x] : 0u;
-    if (threadIdx.x < kMoeExperts / 32) bits[threadIdx.x] = 0;
+    for (u32 i = threadIdx.x; i < kMoeExperts / 2; i += T) p.count[i] = 0;
     __syncthreads();
     for (u32 i = threadIdx.x; i < n;) {
         const bool in = e < a.n_experts;
-        sel[i] = in ? (uint16_t)e : (uint16_t)0xffff;
-        if (in) atomicOr(&bits[e >> 5], 1u << (e & 31));
+        sel[i] = in ? (uint16_t)e : (uint16_t)kMoeNone;
+        if (in) atomicAdd(&p.count[e >> 1], 1u << (16 * (e & 1)));
         else if (raise && e != 0xffffffffu) bm_raise(a.fault, a.layer, kSiteExpertId);
         if ((i += T) < n) e = a.sel[i];
     }
     __syncthreads();
 }
-// The n-th expert that is hit, and how many are; false: there are not as many.
-__device__ __forceinline__ bool moe_nth(const u32 *bits, u32 n, u32 &expert, u32 &n_hit) {
-    const u32 lane = threadIdx.x & 63, word = lane < kMoeExperts / 32 ? bits[lane] : 0u, mine = (u32)__builtin_popcount(word), upto = moe_upto(mine);
-    n_hit = (u32)__builtin_amdgcn_readlane((int)upto, 63);
-    const unsigned long long here = __ballot(upto - mine <= n && n < upto);
-    if (!here) return false;
-    const int at = __builtin_ctzll(here);
-    u32 w = (u32)__builtin_amdgcn_readlane((int)word, at), skip = n - (u32)__builtin_amdgcn_readlane((int)(upto - mine), at);
-    for (; skip; skip--) w &= w - 1;
-    expert = 32 * (u32)at + (u32)__builtin_ctz(w);
-    return true;
+// The experts that are hit, ascending, taken UC picks at a time: the n-th of those shares. False: there are not as many.
+struct MoeShare {
+    u32 expert, rank, share, n_hit, n_shares; // the expert's number among those that are hit, the share's number among the expert's; of all experts
+};
+template <int UC>
+__device__ __forceinline__ bool moe_nth(const MoePicks &p, u32 n_experts, u32 n, MoeShare &s) {
+    const u32 lane = threadIdx.x & 63, words = (n_experts + 127) / 128; // a lane's, two experts each
+    u32 word[8], mine = 0;                                              // shares in the upper half, experts in the lower
+#pragma unroll
+    for (u32 i = 0; i < 8; i++) {
+        if (i >= words) break;
+        word[i] = p.count[words * lane + i];
+        const u32 c0 = word[i] & 0xffffu, c1 = word[i] >> 16;
+        mine += ((c0 + UC - 1) / UC + (c1 + UC - 1) / UC << 16) + (c0 ? 1u : 0u) + (c1 ? 1u : 0u);
+    }
+    const u32 upto = moe_upto(mine), before = upto - mine, all = (u32)__builtin_amdgcn_readlane((int)upto, 63);
+    s.n_hit = all & 0xffffu;
+    s.n_shares = all >> 16;
+    if (n >= s.n_shares) return false;
+    const int at = __builtin_ctzll(__ballot(before >> 16 <= n && n < upto >> 16));
+    const u32 start = (u32)__builtin_amdgcn_readlane((int)before, at);
+    u32 left = n - (start >> 16);
+    s.rank = start & 0xffffu;
+#pragma unroll
+    for (u32 i = 0; i < 16; i++) {
+        const u32 w = (u32)__builtin_amdgcn_readlane((int)word[i / 2], at), c = i & 1 ? w >> 16 : w & 0xffffu, shares = (c + UC - 1) / UC;
+        if (left < shares) {
+            s.expert = 2 * words * (u32)at + i;
+            s.share = left;
+            return true;
+        }
+        left -= shares;
+        s.rank += c ? 1u : 0u;
+    }
+    return false;
 }
 
 // Has the compiler take w anew: what is made of it in a loop stays there, and does not wait in registers (eight times as many) for all of them.
@@ -1074,51 +1101,54 @@ __device__ __forceinline__ unsigned long long moe_first(unsigned long long m) {
     return m ^ rest;
 }
 
-// A workgroup's expert, the n-th that is hit: lane t of every wave has token t's first slot of it (kMoeNone: none) and its place among the expert's tokens. The
-// first workgroup of an expert leaves them for the second launch. False: there are not as many experts.
+// A workgroup's share, the n-th: up to UC tokens of an expert. Lane t of every wave has token t's first slot of the expert (kMoeNone: none) and its place among
+// the expert's tokens, less those of the shares in front. The first workgroup of an expert leaves its slots for the second launch. 0: there are not as many
+// shares; 1: tokens that picked the expert twice have left none for this one; 2: there it is.
 struct MoeEntry {
-    u32 expert, slot, place, n_users;
+    u32 expert, slot, place, columns, n_shares;
 };
-template <int THREADS>
-__device__ __forceinline__ bool moe_entry(const Mx4Moe &a, u32 *bits, uint16_t *sel, u32 n, MoeEntry &e) {
+template <int UC>
+__device__ __forceinline__ int moe_entry(const Mx4Moe &a, const MoePicks &p, const uint16_t *sel, u32 n, MoeEntry &e) {
     const u32 lane = threadIdx.x & 63;
-    moe_picks<THREADS>(a, bits, sel, blockIdx.x == 0 && n == 0);
-    u32 n_hit;
-    const bool there = moe_nth(bits, n, e.expert, n_hit);
-    if (blockIdx.x == 0 && n == 0 && threadIdx.x == 0) a.table->n_hit = n_hit;
-    if (!there) return false;
+    MoeShare s;
+    const bool there = moe_nth<UC>(p, a.n_experts, n, s);
+    if (blockIdx.x == 0 && n == 0 && threadIdx.x == 0) a.table->n_hit = s.n_hit;
+    if (!there) return 0;
+    e.n_shares = s.n_shares;
+    e.expert = s.expert;
     e.slot = kMoeNone;
     if (lane < a.n_tokens)
-        for (u32 s = a.top_k; s-- > 0;)
-            if (sel[lane * a.top_k + s] == e.expert) e.slot = lane * a.top_k + s;
+        for (u32 i = a.top_k; i-- > 0;)
+            if (sel[lane * a.top_k + i] == e.expert) e.slot = lane * a.top_k + i;
     const unsigned long long users = __ballot(e.slot != kMoeNone);
-    e.n_users = (u32)__builtin_popcountll(users);
-    e.place = (u32)__builtin_popcountll(users & ((1ull << lane) - 1));
-    if (blockIdx.x == 0 && threadIdx.x < 64) {
-        if (lane == 0) a.table->expert[n] = (uint16_t)e.expert;
-        a.table->slot[n][lane] = (uint16_t)e.slot;
+    const u32 n_users = (u32)__builtin_popcountll(users);
+    e.place = (u32)__builtin_popcountll(users & ((1ull << lane) - 1)) - s.share * UC;
+    if (blockIdx.x == 0 && s.share == 0 && threadIdx.x < 64) {
+        if (lane == 0) a.table->expert[s.rank] = (uint16_t)e.expert;
+        a.table->slot[s.rank][lane] = (uint16_t)e.slot;
     }
-    return true;
+    if (s.share * UC >= n_users) return 1;
+    e.columns = min(n_users - s.share * UC, (u32)UC);
+    return 2;
 }
 // Up to sixteen of an expert's tokens, a column each.
 struct MoeColumns {
     u32 slot[16], token[16];
     float weight[16];
 };
-// The tokens from place z on.
-__device__ __forceinline__ void moe_columns(const MoeEntry &e, u32 z, u32 n, MoeColumns &col) {
-    if (e.slot == kMoeNone || e.place - z >= n) return;
-    col.slot[e.place - z] = e.slot;
-    col.token[e.place - z] = threadIdx.x & 63;
+__device__ __forceinline__ void moe_columns(const MoeEntry &e, MoeColumns &col) {
+    if (e.slot == kMoeNone || e.place >= e.columns) return;
+    col.slot[e.place] = e.slot;
+    col.token[e.place] = threadIdx.x & 63;
 }
 // And their weights, each over all of a token's slots of the expert. (Asked for behind the first lines, which are waited for anyway.)
-__device__ __forceinline__ void moe_weights(const Mx4Moe &a, const uint16_t *sel, const MoeEntry &e, u32 z, u32 n, MoeColumns &col) {
+__device__ __forceinline__ void moe_weights(const Mx4Moe &a, const uint16_t *sel, const MoeEntry &e, MoeColumns &col) {
     const u32 token = threadIdx.x & 63;
-    if (threadIdx.x >= 64 || e.slot == kMoeNone || e.place - z >= n) return;
+    if (threadIdx.x >= 64 || e.slot == kMoeNone || e.place >= e.columns) return;
     float by = a.w[e.slot];
     for (u32 s = e.slot + 1; s < (token + 1) * a.top_k; s++)
         if (sel[s] == e.expert) by = __fadd_rn(by, a.w[s]);
-    col.weight[e.place - z] = by;
+    col.weight[e.place] = by;
 }
 // Sixteen rows of h from r0 on, of as many columns as 256 threads have: a thread a value, row threadIdx.x % 16, column threadIdx.x / 16. gate, up: the first of
 // the waves' sums, `stride` bytes apart. ONE: the rows may end in the first half of a block, whose other half becomes zeros.
@@ -1151,7 +1181,7 @@ __device__ __forceinline__ void moe_leave(const Mx4Moe &a, const MoeColumns &col
 constexpr int kMoeUpWaves = 4;
 
 // h of rows of up to 2048 values, two lines a wave at most: a workgroup goes over several tiles of sixteen rows of gate and as many of up, whose lines come through
-// a ring of S stages without a stop between the tiles; the tokens' values of a wave's lines stay in LDS, UC tokens' at a time.
+// a ring of S stages without a stop between the tiles; the tokens' values of a wave's lines stay in LDS.
 template <int ET, int S, int UC>
 __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(2))) void k_mx4_moe_up_short(Mx4Moe a, u32 per) {
     constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, kRow = P * kMoePart, kLoads = 6; // loads of a stage: four of lines, two of scales
@@ -1159,36 +1189,42 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
     static_assert(S == 2 || S == 3, "two or three stages");
     __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[S > 2 ? NW * L::kStage : 16];
     __shared__ __align__(16) uint8_t sums[NW * 2048], rows[(NW * 2 * UC + 1) * kRow]; // the last row: zeros
-    __shared__ u32 bits[kMoeExperts / 32];
+    __shared__ MoePicks picks;
     __shared__ MoeColumns col;
     extern __shared__ __align__(16) uint16_t sel[];
-    const u32 lane = threadIdx.x & 63, wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = blockIdx.y, c = lane & 15;
+    const u32 wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (u32 i = threadIdx.x; i < kRow / 16; i += 64 * NW) reinterpret_cast<uint4 *>(rows + NW * 2 * UC * kRow)[i] = make_uint4(0, 0, 0, 0);
-    MoeEntry entry;
-    if (!moe_entry<64 * NW>(a, bits, sel, n, entry)) return;
+    moe_picks<64 * NW>(a, picks, sel, blockIdx.x == 0 && blockIdx.y == 0);
+    for (u32 n = blockIdx.y;; n += gridDim.y) { // (once, where no expert has more than one share)
+        u32 lane = threadIdx.x & 63;
+        __asm__ volatile("" : "+v"(lane)); // anew for each share: what follows from it does not wait in registers from one to the next
+        const u32 c = lane & 15;
+        MoeEntry entry;
+        const int kind = moe_entry<UC>(a, picks, sel, n, entry);
+        if (kind == 0) return;
+        if (kind == 1) continue;
+        const u32 columns = entry.columns;
 
-    const u32 kp = (a.hidden + 31) / 32 * 16, ks = (a.hidden + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage, at = 2 * (lane >> 4);
-    const u32 tile0 = blockIdx.x * per, tiles = min(per, (a.ff + 15) / 16 - tile0), each = wave + NW < lines ? 2 : wave < lines ? 1 : 0, items = tiles * each; // this wave's
-    const size_t stack = (size_t)entry.expert * a.ff;
-    const uint8_t *const gate = a.wg + stack * kp, *const up = a.wu + stack * kp, *const gate_scales = a.wgs + stack * ks, *const up_scales = a.wus + stack * ks;
-    L src;
-    src.begin(lane);
-    u32 s0[2], s1[2], s2[2], asked = 0;
-    const auto ask = [&](uint8_t *stage, u32 (&s)[2]) {
-        const u32 tile = each == 2 ? asked >> 1 : asked, l = each == 2 && (asked & 1) ? wave + NW : wave, r0 = 16 * (tile0 + tile);
-        const u32 mark = min(r0 + c, a.ff - 1) * ks + at + 8 * l; // rows past the last are the last once more, and their values zeros
-        s[0] = mx4_two(gate_scales + mark);
-        s[1] = mx4_two(up_scales + mark);
+        const u32 kp = (a.hidden + 31) / 32 * 16, ks = (a.hidden + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage, at = 2 * (lane >> 4);
+        const u32 tile0 = blockIdx.x * per, tiles = min(per, (a.ff + 15) / 16 - tile0), each = wave + NW < lines ? 2 : wave < lines ? 1 : 0, items = tiles * each; // this wave's
+        const size_t stack = (size_t)entry.expert * a.ff;
+        const uint8_t *const gate = a.wg + stack * kp, *const up = a.wu + stack * kp, *const gate_scales = a.wgs + stack * ks, *const up_scales = a.wus + stack * ks;
+        L src;
+        src.begin(lane);
+        u32 s0[2], s1[2], s2[2], asked = 0;
+        const auto ask = [&](uint8_t *stage, u32 (&s)[2]) {
+            const u32 tile = each == 2 ? asked >> 1 : asked, l = each == 2 && (asked & 1) ? wave + NW : wave, r0 = 16 * (tile0 + tile);
+            const u32 mark = min(r0 + c, a.ff - 1) * ks + at + 8 * l; // rows past the last are the last once more, and their values zeros
+            s[0] = mx4_two(gate_scales + mark);
+            s[1] = mx4_two(up_scales + mark);
 #pragma unroll
-        for (u32 g = 0; g < 4; g++) src.from[g] = (const int8_t *)(g < 2 ? gate : up) + (size_t)min(r0 + 8 * (g & 1) + (lane >> 3), a.ff - 1) * kp;
-        __builtin_amdgcn_sched_barrier(0);
-        src.ask(stage + mine, l, kp);
-        __builtin_amdgcn_sched_barrier(0);
-        asked++;
-    };
-    for (u32 z = 0; z < entry.n_users; z += UC) {
-        const u32 columns = min(entry.n_users - z, (u32)UC);
-        moe_columns(entry, z, UC, col);
+            for (u32 g = 0; g < 4; g++) src.from[g] = (const int8_t *)(g < 2 ? gate : up) + (size_t)min(r0 + 8 * (g & 1) + (lane >> 3), a.ff - 1) * kp;
+            __builtin_amdgcn_sched_barrier(0);
+            src.ask(stage + mine, l, kp);
+            __builtin_amdgcn_sched_barrier(0);
+            asked++;
+        };
+        moe_columns(entry, col);
         __syncthreads();
         // lanes 0 to 31 take one token's values of a line, eight each, lanes 32 to 63 the next one's
         MoePiece<ET> held[2][UC / 2];
@@ -1199,7 +1235,6 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
                 if (const u32 column = 2 * j + (lane >> 5); i < each && column < columns)
                     held[i][j].ask(a.x, (size_t)col.token[column] * a.ld_x, 256 * (wave + i * NW) + 8 * (lane & 31), a.hidden);
         __builtin_amdgcn_sched_barrier(0);
-        asked = 0;
         if (asked < items) ask(ring0, s0);
         if (asked < items) ask(ring1, s1);
 #pragma unroll
@@ -1213,7 +1248,7 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
                     for (int p = 0; p < P; p++) *reinterpret_cast<v8h *>(to + p * kMoePart) = part[p];
                 }
-        moe_weights(a, sel, entry, z, UC, col);
+        moe_weights(a, sel, entry, col);
         v4f acc[2];
         u32 done = 0, tile = 0;
         const auto step = [&](uint8_t *stage, u32 (&s)[2], uint8_t *free, u32 (&next)[2]) {
@@ -1281,12 +1316,13 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
                 }
             }
         }
+        if (n + gridDim.y >= entry.n_shares) return;
         __syncthreads();
     }
 }
 
 // h. T times sixteen rows of gate and as many of up, their lines dealt to the waves, each through S stages, of which all but one, or of two one, are on
-// their way while one is multiplied. A line's values of x come through LDS, UC tokens' at a time in parts, the next line's asked for in front of the weights: asked for in the matrix
+// their way while one is multiplied. A line's values of x come through LDS in parts, the next line's asked for in front of the weights: asked for in the matrix
 // instructions' form, each of sixteen requests a line would take the vector cache as long as a line of weights does.
 template <int ET, int T, int S, int UC, int EU>
 __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(EU))) void k_mx4_moe_up(Mx4Moe a) {
@@ -1294,42 +1330,47 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
     typedef Lines<2 * R> L;
     __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[S > 2 ? NW * L::kStage : 16];
     __shared__ __align__(16) uint8_t rows[(NW * UC + 1) * kRow]; // the last: zeros
-    __shared__ u32 bits[kMoeExperts / 32];
+    __shared__ MoePicks picks;
     __shared__ MoeColumns col;
     extern __shared__ __align__(16) uint16_t sel[];
-    const u32 lane = threadIdx.x & 63, wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = blockIdx.y, c = lane & 15;
+    const u32 wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (u32 i = threadIdx.x; i < kRow / 16; i += 64 * NW) reinterpret_cast<uint4 *>(rows + NW * UC * kRow)[i] = make_uint4(0, 0, 0, 0);
-    MoeEntry entry;
-    if (!moe_entry<64 * NW>(a, bits, sel, n, entry)) return;
-    const u32 expert = entry.expert, n_users = entry.n_users;
+    moe_picks<64 * NW>(a, picks, sel, blockIdx.x == 0 && blockIdx.y == 0);
+    for (u32 n = blockIdx.y;; n += gridDim.y) { // (once, where no expert has more than one share)
+        u32 lane = threadIdx.x & 63;
+        __asm__ volatile("" : "+v"(lane)); // anew for each share: what follows from it does not wait in registers from one to the next
+        const u32 c = lane & 15;
+        MoeEntry entry;
+        const int kind = moe_entry<UC>(a, picks, sel, n, entry);
+        if (kind == 0) return;
+        if (kind == 1) continue;
+        const u32 expert = entry.expert, columns = entry.columns;
 
-    const u32 kp = (a.hidden + 31) / 32 * 16, ks = (a.hidden + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage, at = 2 * (lane >> 4);
-    const u32 r0 = blockIdx.x * (16 * T);
-    L src;
-    src.begin(lane);
-    const size_t stack = (size_t)expert * a.ff;
-    const uint8_t *scales[R];
+        const u32 kp = (a.hidden + 31) / 32 * 16, ks = (a.hidden + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage, at = 2 * (lane >> 4);
+        const u32 r0 = blockIdx.x * (16 * T);
+        L src;
+        src.begin(lane);
+        const size_t stack = (size_t)expert * a.ff;
+        const uint8_t *scales[R];
 #pragma unroll
-    for (u32 g = 0; g < 2 * R; g++) // rows past the last are the last once more, and their values zeros
-        src.from[g] = (const int8_t *)(g < R ? a.wg : a.wu) + (stack + min(r0 + 8 * (g % R) + (lane >> 3), a.ff - 1)) * kp;
+        for (u32 g = 0; g < 2 * R; g++) // rows past the last are the last once more, and their values zeros
+            src.from[g] = (const int8_t *)(g < R ? a.wg : a.wu) + (stack + min(r0 + 8 * (g % R) + (lane >> 3), a.ff - 1)) * kp;
 #pragma unroll
-    for (u32 g = 0; g < R; g++) scales[g] = (g < T ? a.wgs : a.wus) + (stack + min(r0 + 16 * (g % T) + c, a.ff - 1)) * ks + at;
-    u32 s0[R], s1[R], s2[R];
-    const auto ask = [&](uint8_t *stage, u32 (&s)[R], u32 l) {
+        for (u32 g = 0; g < R; g++) scales[g] = (g < T ? a.wgs : a.wus) + (stack + min(r0 + 16 * (g % T) + c, a.ff - 1)) * ks + at;
+        u32 s0[R], s1[R], s2[R];
+        const auto ask = [&](uint8_t *stage, u32 (&s)[R], u32 l) {
 #pragma unroll
-        for (int g = 0; g < R; g++) s[g] = mx4_two(scales[g] + 8 * l);
-        __builtin_amdgcn_sched_barrier(0);
-        src.ask(stage + mine, l, kp);
-        __builtin_amdgcn_sched_barrier(0);
-    };
+            for (int g = 0; g < R; g++) s[g] = mx4_two(scales[g] + 8 * l);
+            __builtin_amdgcn_sched_barrier(0);
+            src.ask(stage + mine, l, kp);
+            __builtin_amdgcn_sched_barrier(0);
+        };
 
-    for (u32 z = 0; z < n_users; z += 16) {
-        const u32 columns = min(n_users - z, 16u);
-        moe_columns(entry, z, 16, col);
+        moe_columns(entry, col);
         __syncthreads();
         // lanes 0 to 31 take one token's values of a line, eight each, lanes 32 to 63 the next one's
         MoePiece<ET> held[UC / 2];
-        size_t row_of[UC / 2]; // of the first UC columns
+        size_t row_of[UC / 2];
 #pragma unroll
         for (int j = 0; j < UC / 2; j++) row_of[j] = (size_t)col.token[min(2 * j + (lane >> 5), columns - 1)] * a.ld_x;
         const auto fetch = [&](u32 l) {
@@ -1337,12 +1378,12 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
             for (int j = 0; j < UC / 2; j++)
                 if (2 * j + (lane >> 5) < columns) held[j].ask(a.x, row_of[j], 256 * l + 8 * (lane & 31), a.hidden);
         };
-        const auto put = [&](const MoePiece<ET> (&from)[UC / 2], u32 first) {
+        const auto put = [&] {
 #pragma unroll
             for (int j = 0; j < UC / 2; j++) {
-                if (first + 2 * j + (lane >> 5) >= columns) continue;
+                if (2 * j + (lane >> 5) >= columns) continue;
                 v8h part[P];
-                from[j].parts(part);
+                held[j].parts(part);
                 uint8_t *to = rows + (wave * UC + 2 * j + (lane >> 5)) * kRow + moe_put(lane & 31);
 #pragma unroll
                 for (int p = 0; p < P; p++) *reinterpret_cast<v8h *>(to + p * kMoePart) = part[p];
@@ -1352,14 +1393,14 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
         __builtin_amdgcn_sched_barrier(0);
         if (wave < lines) ask(ring0, s0, wave);
         if (wave + NW < lines) ask(ring1, s1, wave + NW);
-        moe_weights(a, sel, entry, z, 16, col);
+        moe_weights(a, sel, entry, col);
         v4f acc[R];
 #pragma unroll
         for (int g = 0; g < R; g++) acc[g] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         const auto step = [&](uint8_t *stage, u32 (&s)[R], uint8_t *free, u32 (&next)[R], u32 l) {
             if (l + NW < lines) loads_landed<kLoads>(); // the next stage may be on its way; this line's values of x are older than it
             else loads_landed<0>();
-            put(held, 0);
+            put();
             if (l + NW < lines) fetch(l + NW);
             __builtin_amdgcn_sched_barrier(0);
             if (S > 2 && l + 2 * NW < lines) ask(free, next, l + 2 * NW);
@@ -1378,29 +1419,18 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
                 lds_read(); // the stage is in registers
                 ask(stage, s, l + 2 * NW);
             }
-            for (u32 first = 0;;) {
+            const uint8_t *row = rows + (c < columns ? wave * UC + c : (u32)(NW * UC)) * kRow + moe_at(lane);
 #pragma unroll
-                for (int g = 0; g < R; g++) moe_anew(w[g][0]), moe_anew(w[g][1]);
-                const uint8_t *row = rows + (c - first < (u32)UC && c < columns ? wave * UC + c - first : (u32)(NW * UC)) * kRow + moe_at(lane);
+            for (int i = 0; i < 8; i++) {
+                v8h value[P];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    v8h value[P];
+                for (int p = 0; p < P; p++) value[p] = *reinterpret_cast<const v8h *>(row + p * kMoePart + 16 * i);
 #pragma unroll
-                    for (int p = 0; p < P; p++) value[p] = *reinterpret_cast<const v8h *>(row + p * kMoePart + 16 * i);
+                for (int g = 0; g < R; g++) {
+                    const v8h code = moe_codes((u32)w[g][i / 4][i % 4], by[g][i / 4]);
 #pragma unroll
-                    for (int g = 0; g < R; g++) {
-                        const v8h code = moe_codes((u32)w[g][i / 4][i % 4], by[g][i / 4]);
-#pragma unroll
-                        for (int p = 0; p < P; p++) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code, value[p], acc[g], 0, 0, 0);
-                    }
+                    for (int p = 0; p < P; p++) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code, value[p], acc[g], 0, 0, 0);
                 }
-                if ((first += UC) >= columns) break;
-                MoePiece<ET> more[UC / 2];
-#pragma unroll
-                for (int j = 0; j < UC / 2; j++)
-                    if (const u32 column = first + 2 * j + (lane >> 5); column < columns)
-                        more[j].ask(a.x, (size_t)col.token[column] * a.ld_x, 256 * l + 8 * (lane & 31), a.hidden);
-                put(more, first);
             }
         };
         for (u32 l = wave; l < lines;) {
@@ -1420,6 +1450,7 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll 1
         for (int t = 0; t < T; t++)
             moe_leave<ET, NW, T == 1>(a, col, columns, r0 + 16 * t, ring0 + t * 1024, ring0 + (T + t) * 1024, L::kStage);
+        if (n + gridDim.y >= entry.n_shares) return;
         __syncthreads();
     }
 }
