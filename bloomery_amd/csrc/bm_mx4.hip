@@ -922,6 +922,7 @@ struct Mx4Moe {
     const float *w;
     MoeTable *table; // (as many of the slots' rows as there can be hits)
     __bf16 *h;       // a slot's parts, rows of ff rounded up to 32 values
+    float *partial;  // the second launch's sums where several workgroups share the experts: by workgroup, tokens x hidden rounded up to 4
     void *y;
     GateRule rule;
     u32 *fault, layer;
@@ -972,7 +973,7 @@ __device__ __forceinline__ bool moe_nth(const MoePicks &p, u32 n_experts, u32 n,
         if (i >= words) break;
         word[i] = p.count[words * lane + i];
         const u32 c0 = word[i] & 0xffffu, c1 = word[i] >> 16;
-        mine += ((c0 + UC - 1) / UC + (c1 + UC - 1) / UC << 16) + (c0 ? 1u : 0u) + (c1 ? 1u : 0u);
+        mine += ((c0 + UC - 1) / UC + (c1 + UC - 1) / UC) * 0x10000u + (c0 ? 1u : 0u) + (c1 ? 1u : 0u);
     }
     const u32 upto = moe_upto(mine), before = upto - mine, all = (u32)__builtin_amdgcn_readlane((int)upto, 63);
     s.n_hit = all & 0xffffu;
@@ -1455,9 +1456,19 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
     }
 }
 
+// Four rows' sums of a token onto the residual.
+template <int ET>
+__device__ __forceinline__ void moe_onto(const Mx4Moe &a, u32 token, u32 row, float (&v)[4]) {
+    const u32 have = a.hidden - row;
+    if (a.resid)
+#pragma unroll
+        for (u32 j = 0; j < 4; j++)
+            if (j < have) v[j] = __fadd_rn(v[j], elem_load1<ET>(a.resid, token * a.ld_resid + row + j));
+    elem_store_some<ET, 4>(a.y, token * a.ld_y + row, have, v);
+}
 // y. The lines of the experts that are hit, one expert's after another's, are dealt to the waves in stretches, each through two stages of 16 R rows; the
 // waves' sums, NT tiles of sixteen tokens, meet in LDS. A line's values of h come through LDS too, UC tokens' at a time and the next line's asked for in front of the
-// weights.
+// weights. gridDim.y workgroups share the lines: where they are several, a third launch adds their sums.
 template <int ET, int NW, int R, int UC, int NT>
 __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
     constexpr int PH = kMoeKept<ET>, NL = (PH + 1) / 2, CH = NT * R == 1 ? 2 : 1; // requests of a token's values; chains of products
@@ -1473,7 +1484,8 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
     __syncthreads();
 
     const u32 kp = (a.ff + 31) / 32 * 16, ks = (a.ff + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage;
-    const u32 r0 = blockIdx.x * (16 * R), ffp = (a.ff + 31) / 32 * 32, items = n_hit * lines, q0 = items * wave / NW, q1 = items * (wave + 1) / NW;
+    const u32 r0 = blockIdx.x * (16 * R), ffp = (a.ff + 31) / 32 * 32, shares = NW * gridDim.y, share = NW * blockIdx.y + wave, items = n_hit * lines;
+    const u32 q0 = items * share / shares, q1 = items * (share + 1) / shares;
     L src;
     src.begin(lane);
     size_t from[2 * R], mark[R]; // rows past the last are the last once more, and not stored
@@ -1631,15 +1643,21 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
         if (wave < R && token < a.n_tokens && row < a.hidden) {
             const v4f sum = mx4_join<NW, L>(ring0, wave, lane);
             float v[4] = {sum[0], sum[1], sum[2], sum[3]};
-            const u32 have = a.hidden - row;
-            if (a.resid)
-#pragma unroll
-                for (u32 j = 0; j < 4; j++)
-                    if (j < have) v[j] = __fadd_rn(v[j], elem_load1<ET>(a.resid, token * a.ld_resid + row + j));
-            elem_store_some<ET, 4>(a.y, token * a.ld_y + row, have, v);
+            if (gridDim.y > 1) *reinterpret_cast<v4f *>(a.partial + ((size_t)blockIdx.y * a.n_tokens + token) * ((a.hidden + 3) / 4 * 4) + row) = sum;
+            else moe_onto<ET>(a, token, row, v);
         }
         __syncthreads();
     }
+}
+// The workgroups' sums, in their order.
+template <int ET>
+__global__ __launch_bounds__(256) void k_mx4_moe_join(Mx4Moe a, u32 n) {
+    const u32 quads = (a.hidden + 3) / 4, i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= quads * a.n_tokens) return;
+    v4f sum = *reinterpret_cast<const v4f *>(a.partial + (size_t)i * 4);
+    for (u32 z = 1; z < n; z++) sum += *reinterpret_cast<const v4f *>(a.partial + ((size_t)z * quads * a.n_tokens + i) * 4);
+    float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+    moe_onto<ET>(a, i / quads, 4 * (i % quads), v);
 }
 
 static u32 moe_hits(int n_tokens, int top_k, int n_experts) { return (u32)std::min(n_tokens * top_k, n_experts); }
@@ -1653,34 +1671,49 @@ static void moe_up_short(const Launch &L, const Mx4Moe &a) {
     const u32 tiles = (a.ff + 15) / 16, hits = moe_hits(a.n_tokens, a.top_k, a.n_experts), per = std::max(1u, tiles * hits / 1536);
     hipLaunchKernelGGL((k_mx4_moe_up_short<ET, S, UC>), dim3((tiles + per - 1) / per, hits), dim3(64 * kMoeUpWaves), (a.n_tokens * a.top_k * 2 + 15) & ~15u, L.stream, a, per);
 }
+// Workgroups that share the lines of down's experts: where its rows are few, as many as fill the card (two a slot of a token at most: what the scratch holds).
+static u32 moe_sharers(int top_k, int hidden) { return (u32)std::max(1, std::min({8, 2 * top_k, 256 * 32 / hidden})); }
 template <int ET, int NW, int R, int UC, int NT>
-static void moe_down(const Launch &L, const Mx4Moe &a) {
-    hipLaunchKernelGGL((k_mx4_moe_down<ET, NW, R, UC, NT>), dim3((a.hidden + 16 * R - 1) / (16 * R)), dim3(64 * NW), 0, L.stream, a);
+static hipError_t moe_down(const Launch &L, const Mx4Moe &a, u32 sharers) {
+    hipLaunchKernelGGL((k_mx4_moe_down<ET, NW, R, UC, NT>), dim3((a.hidden + 16 * R - 1) / (16 * R), sharers), dim3(64 * NW), 0, L.stream, a);
+    const hipError_t e = hipGetLastError();
+    if (sharers == 1 || e != hipSuccess) return e;
+    hipLaunchKernelGGL((k_mx4_moe_join<ET>), dim3(((a.hidden + 3) / 4 * a.n_tokens + 255) / 256), dim3(256), 0, L.stream, a, sharers);
+    return hipGetLastError();
 }
-template <int ET>
+template <int ET, int NT>
 static hipError_t moe_launch(const Launch &L, const Mx4Moe &a) {
-    if (a.hidden <= 256 * 2 * kMoeUpWaves) moe_up_short<ET, kMoeParts<ET> == 1 ? 3 : 2, kMoeParts<ET> == 3 ? 2 : 4>(L, a);
-    else moe_up<ET, 1, 3, kMoeParts<ET> == 1 ? 8 : 4, 2>(L, a);
+    constexpr int P = kMoeParts<ET>;
+    if (a.hidden <= 256 * 2 * kMoeUpWaves) moe_up_short<ET, P == 1 ? 3 : 2, P == 3 ? 2 : 4>(L, a);
+    else moe_up<ET, 1, 3, P == 1 ? 8 : 4, 2>(L, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.hidden < 4096) a.n_tokens > 16 ? moe_down<ET, 16, 1, kMoeParts<ET> == 3 ? 3 : 4, 4>(L, a) : moe_down<ET, 16, 1, kMoeParts<ET> == 3 ? 3 : 4, 1>(L, a);
-    else a.n_tokens > 16 ? moe_down<ET, kMoeParts<ET> == 1 ? 16 : 8, 2, kMoeParts<ET> == 1 ? 3 : 4, 4>(L, a)
-                       : moe_down<ET, kMoeParts<ET> == 1 ? 16 : 8, 2, kMoeParts<ET> == 1 ? 3 : 4, 1>(L, a);
-    return hipGetLastError();
+    constexpr int NW = P == 1 ? 16 : 8, UC = P == 1 ? 3 : 4;
+    const u32 items = moe_hits(a.n_tokens, a.top_k, a.n_experts) * ((a.ff + 255) / 256);
+    const u32 sharers = std::min(moe_sharers(a.top_k, a.hidden), items / (4 * NW));
+    if (sharers > 1) return moe_down<ET, NW, 2, UC, NT>(L, a, sharers);
+    if (a.hidden < 4096) return moe_down<ET, 16, 1, P == 3 ? 3 : 4, NT>(L, a, 1);
+    return moe_down<ET, NW, 2, UC, NT>(L, a, 1);
 }
 
 static size_t moe_table(int n_tokens, int top_k) { return offsetof(MoeTable, slot) + (size_t)moe_hits(n_tokens, top_k, kMoeExperts) * sizeof(MoeTable::slot[0]); }
-size_t mx4_moe_work(int n_tokens, int top_k, int, int ff) { return moe_table(n_tokens, top_k) + (size_t)n_tokens * top_k * 3 * ((ff + 31) / 32 * 32) * 2; }
+static size_t moe_h(int n_tokens, int top_k, int ff) { return (size_t)n_tokens * top_k * 3 * ((ff + 31) / 32 * 32) * 2; }
+size_t mx4_moe_work(int n_tokens, int top_k, int hidden, int ff) {
+    const u32 sharers = moe_sharers(top_k, hidden);
+    return moe_table(n_tokens, top_k) + moe_h(n_tokens, top_k, ff) + (sharers > 1 ? (size_t)sharers * n_tokens * ((hidden + 3) / 4 * 4) * sizeof(float) : 0);
+}
 
 hipError_t mx4_moe(const Launch &L, const Mx4Stack &g, const Mx4Stack &u, const Mx4Stack &d, int n_experts, int hidden, int ff, const void *x, int et,
                    int64_t ld_x, int n_tokens, const uint32_t *sel, const float *w, int top_k, const void *resid, int64_t ld_resid, void *y, int64_t ld_y,
                    void *work) {
     const Mx4Moe a = {g.w, g.scales, u.w, u.scales, d.w, d.scales, (u32)n_experts, (u32)hidden, (u32)ff, (u32)n_tokens, (u32)top_k, x, resid, (size_t)ld_x,
-                      (size_t)ld_resid, (size_t)ld_y, sel, w, (MoeTable *)work, (__bf16 *)((uint8_t *)work + moe_table(n_tokens, top_k)), y, L.rule, L.fault,
+                      (size_t)ld_resid, (size_t)ld_y, sel, w, (MoeTable *)work, (__bf16 *)((uint8_t *)work + moe_table(n_tokens, top_k)),
+                      (float *)((uint8_t *)work + moe_table(n_tokens, top_k) + moe_h(n_tokens, top_k, ff)), y, L.rule, L.fault,
                       L.layer};
-    if (et == kElemF32) return moe_launch<kElemF32>(L, a);
-    if (et == kElemF16) return moe_launch<kElemF16>(L, a);
-    return moe_launch<kElemBF16>(L, a);
+    const bool few = n_tokens <= 16;
+    if (et == kElemF32) return few ? moe_launch<kElemF32, 1>(L, a) : moe_launch<kElemF32, 4>(L, a);
+    if (et == kElemF16) return few ? moe_launch<kElemF16, 1>(L, a) : moe_launch<kElemF16, 4>(L, a);
+    return few ? moe_launch<kElemBF16, 1>(L, a) : moe_launch<kElemBF16, 4>(L, a);
 }
 
 } // namespace bmk
