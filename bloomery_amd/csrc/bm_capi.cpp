@@ -1755,6 +1755,14 @@ int bm_mx4_gemm_experts(bm_ctx *ctx, const uint8_t *w_dev, const uint8_t *w_scal
                                            top_k > 0 ? order_dev : nullptr, start_dev, n_slots, top_k, y_dev, y_type, ld_y));
 }
 
+int bm_mx4_gemm_form(int n_experts, int rows, int k, int n_cols, int n_slots, int top_k) {
+    const char *what = "bm_mx4_gemm_form";
+    BM_TRY(check_mx4_size(nullptr, what, "rows", rows, k));
+    if (n_experts == 0) BM_TRY(check_mx4_size(nullptr, what, "n_cols", n_cols, k));
+    else BM_TRY(check_i8_runs(nullptr, what, n_experts, n_cols, n_slots, top_k));
+    return bmk::mx4_gemm_form(n_experts, rows, k, n_cols, n_slots, top_k);
+}
+
 static int check_mx4_moe(bm_ctx *ctx, const char *what, int n_tokens, int top_k, int hidden, int ff) {
     if (n_tokens < 1 || n_tokens > bmk::kMx4MoeTokens || top_k < 1 || top_k > bmk::kMaxCombineSlots)
         return fail(ctx, BM_ESHAPE, "%s: %d tokens of %d slots (1 .. %d tokens, 1 .. %d slots a token)", what, n_tokens, top_k, bmk::kMx4MoeTokens,

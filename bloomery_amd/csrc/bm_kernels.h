@@ -244,6 +244,8 @@ hipError_t mx4_gemm(const Launch &L, const uint8_t *w, const uint8_t *ws, int n_
                     const uint32_t *order, const uint32_t *start, int n_slots, int top_k, void *y, int et, int64_t ld);
 hipError_t mx4_gemm_x(const Launch &L, const uint8_t *w, const uint8_t *ws, int rows, int k, const void *x, int x_et, int64_t ld_x, int m, uint8_t *codes,
                       uint8_t *scales, void *y, int et, int64_t ld);
+// The form that mx4_gemm takes (bm_mx4_gemm_form's word). n_experts 0: one matrix against n_cols columns.
+int mx4_gemm_form(int n_experts, int rows, int k, int n_cols, int n_slots, int top_k);
 // The experts' step of a few tokens; work: mx4_moe_work bytes.
 constexpr int kMx4MoeTokens = 64;
 struct Mx4Stack {

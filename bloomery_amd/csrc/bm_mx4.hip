@@ -835,47 +835,58 @@ hipError_t mx4_gemm_x(const Launch &L, const uint8_t *w, const uint8_t *ws, int 
 
 // The forms, by what a workgroup has: columns x rows, its waves and its LDS buffers.
 enum Mx4Form : u32 {
-    kMx4Few16x16, // k_mx4_few: 16 x 16, waves sharing k
+    kMx4Few16x16, // k_mx4_few: waves sharing k
     kMx4Few16x32,
-    kMx4Few16x32Three,
     kMx4Few32x32,
     kMx4Tile32x64, // k_mx4_tile
     kMx4Tile64x64,
-    kMx4Tile64x128,
     kMx4Tile128x128,
     kMx4Tile256x128,
     kMx4Tile256x256,
 };
 
+// Which form, us on MI355X, bf16 out, weights of three sets in turn (two for experts), the chosen form's first.
+//   One matrix. While tiles of at most 32 x 32 are no more than the compute units a workgroup's waves share a row's k, in the smallest tile that is one round: 16 x 2048 x
+//   7168 in 16 x 16 5.3 (16 x 32: 6.9, 32 x 64: 9.4), 64 x 2048 x 7168 in 16 x 32 7.0 (32 x 32: 8.3; 16 x 16, two rounds: 9.3), 128 x 2048 x 7168 in 32 x 32 8.5 (32 x 64: 13.5), one
+//   row of 7168 x 7168 7.6 (16 x 16: 8.8, 32 x 64: 14.8). Then whole rows of k in tiles that leave few units idle: 32 x 64 up to two a unit, 128 x 7168 x 7168 16.1 (64 x 64: 17.0), 512 x
+//   2048 x 7168 16.0 (16.7), but 1024 x 2048 x 7168 19.5 (18.6); 64 x 64 up to four, 4096 x 768 x 2048 10.3 (128 x 128: 11.9), 512 x 7168 x 7168 28.4 (29.1). Behind that whole rounds of
+//   256 units count: one of 256 x 256 tiles takes 55 units of time, of 256 x 128 34, of two 128 x 128 a unit 38. 4096 x 7168 x 7168: 107.6 in 448 tiles of 256 x 256 (256 x 128: 133, 128 x
+//   128: 138), 1024 x 7168 x 7168 34.1 in 224 of 256 x 128 (38.7; 256 x 256: 47.9), 2048 x 7168 x 2048 22.3 (25.6, 27.9), 4096 x 2048 x 2048 15.5 in 256 x 128 (16.6, 21.5).
+//   Experts, by slots an expert. Up to 12, while the rows' tiles are two a unit, by waves sharing k: 16 tokens, top 4 of 8, 2048 x 2048 5.6 (32 x 64: 7.5); 64 experts of 7168 rows: 70, 32 x 64
+//   50.6. 32 x 64 below 24 slots, or while its tiles are few: 333 tokens, top 2 of 64, 7168 x 2048 90 (64 x 64: 95), 16 slots, 128 experts, 2048 x 768 26.5 (28.7), 128 slots, 8 experts,
+//   2048 x 2048 10.6 (11.2). 64 x 64 below 56, or while few: 32 slots, 64 experts, 7168 x 2048 118.5 (128 x 128: 127.5). 128 x 128: 64 slots, 128 experts, 768 x 2048 33.4 (64 x 64: 37.9), 128
+//   slots 44.9 (256 x 256: 46.6, 64 x 64: 52.6), 256 slots 65.5 (71). 256 x 256 from 352 on: 512 slots 102.6 (128 x 128: 121.9), 64 experts, 7168 x 2048 442 (488).
 // n_experts 0: one matrix, n its columns; else n slots. reach: the tiles' offsets of gathered columns, 32 bits, hold the columns.
-static Mx4Form mx4_form(u32 n_experts, u32 rows, u32 kp, u32 n, bool reach) {
+static Mx4Form mx4_form(u32 n_experts, u32 rows, u32 n, bool reach) {
     const auto up = [](u32 x, u32 y) { return (x + y - 1) / y; };
     const auto tiles = [&](u32 bt, u32 br) { return (uint64_t)up(n, bt) * up(rows, br); };
     if (n_experts) {
-        if (n <= 32 || !reach) return kMx4Few16x32Three;
         const u32 each = n / n_experts, runs = n < n_experts ? n : n_experts;
-        const uint64_t small = (uint64_t)std::max(runs, n / 64 + runs / 2) * up(rows, 64);
-        if (each <= 16 && small <= 64) return kMx4Few32x32;
-        if (each >= 24 && small <= 1024) return kMx4Tile64x64;
-        if (each >= 96) return kMx4Tile128x128;
-        return each >= 12 ? kMx4Tile64x128 : kMx4Tile32x64;
+        if (n <= 32 || !reach || (each <= 12 && (uint64_t)up(rows, 32) * n_experts <= 512)) return kMx4Few16x32;
+        // tiles that runs fill, and half a one more for each
+        const auto filled = [&](u32 bt) { return (uint64_t)(n / bt + runs / 2) * up(rows, 64); };
+        if (each < 24 || filled(32) <= 1200) return kMx4Tile32x64;
+        if (each < 56 || filled(64) <= 800) return kMx4Tile64x64;
+        return each < 352 ? kMx4Tile128x128 : kMx4Tile256x256;
     }
     if (tiles(16, 16) <= 256) return kMx4Few16x16;
-    if (tiles(16, 32) <= 256) return kMx4Few16x32;
-    if (n <= 16) return kMx4Few16x32Three;
+    if (n <= 16 || tiles(16, 32) <= 256) return kMx4Few16x32;
     if (n <= 32 || tiles(32, 32) <= 256) return kMx4Few32x32;
-    if (tiles(64, 64) <= 768) return kMx4Tile64x64;
-    return kMx4Tile128x128;
+    if (tiles(32, 64) <= 512) return kMx4Tile32x64;
+    if (tiles(64, 64) <= 1024) return kMx4Tile64x64;
+    const auto rounds = [&](u32 bt, u32 br, u32 at_once) { return (tiles(bt, br) + at_once - 1) / at_once; };
+    const uint64_t by256 = 55 * rounds(256, 256, 256), by128 = 34 * rounds(256, 128, 256), by_two = 38 * rounds(128, 128, 512);
+    if (by256 <= by128 && by256 <= by_two) return kMx4Tile256x256;
+    return by128 <= by_two ? kMx4Tile256x128 : kMx4Tile128x128;
 }
 static bool mx4_reach(bool gathered, int n_cols, u32 kp) { return !gathered || (uint64_t)n_cols * kp <= 0xffffffffu; }
 
 int mx4_gemm_form(int n_experts, int rows, int k, int n_cols, int n_slots, int top_k) {
     static const struct {
         u32 columns, rows, waves, buffers;
-    } of[] = {{16, 16, 8, 4}, {16, 32, 4, 4}, {16, 32, 3, 4}, {32, 32, 4, 4}, {32, 64, 2, 2}, {64, 64, 4, 2}, {64, 128, 4, 2}, {128, 128, 4, 2},
-              {256, 128, 8, 2}, {256, 256, 8, 2}};
+    } of[] = {{16, 16, 8, 4}, {16, 32, 3, 4}, {32, 32, 4, 4}, {32, 64, 2, 2}, {64, 64, 4, 2}, {128, 128, 4, 2}, {256, 128, 8, 2}, {256, 256, 8, 2}};
     const u32 kp = (u32)mx4_row_bytes(k);
-    const auto &f = of[mx4_form((u32)n_experts, (u32)rows, kp, (u32)(n_experts ? n_slots : n_cols), mx4_reach(n_experts && top_k > 0, n_cols, kp))];
+    const auto &f = of[mx4_form((u32)n_experts, (u32)rows, (u32)(n_experts ? n_slots : n_cols), mx4_reach(n_experts && top_k > 0, n_cols, kp))];
     return (int)(f.columns | f.rows << 10 | f.waves << 20 | f.buffers << 24);
 }
 
@@ -884,14 +895,12 @@ hipError_t mx4_gemm(const Launch &L, const uint8_t *w, const uint8_t *ws, int n_
     const Mx4Args a = {w, ws, (u32)rows, (u32)mx4_row_bytes(k), (u32)mx4_row_scales(k), q, qs, (u32)n_cols, order, start, (u32)n_slots, (u32)top_k,
                        (u32)n_cols, (u32)n_experts, y, (size_t)ld, et, L.fault, L.layer};
     const u32 n = start ? (u32)n_slots : (u32)n_cols;
-    switch (mx4_form(start ? a.n_experts : 0, a.rows, a.kp, n, mx4_reach(order != nullptr, n_cols, a.kp))) {
+    switch (mx4_form(start ? a.n_experts : 0, a.rows, n, mx4_reach(order != nullptr, n_cols, a.kp))) {
     case kMx4Few16x16: return mx4_few_launch<1, 1, 8>(L, a, n);
-    case kMx4Few16x32: return mx4_few_launch<2, 1, 4>(L, a, n);
-    case kMx4Few16x32Three: return mx4_few_launch<2, 1, 3>(L, a, n);
+    case kMx4Few16x32: return mx4_few_launch<2, 1, 3>(L, a, n);
     case kMx4Few32x32: return mx4_few_launch<2, 2, 4>(L, a, n);
     case kMx4Tile32x64: return mx4_tile_launch<32, 64, 1, 2, 0, 2>(L, a, n);
     case kMx4Tile64x64: return mx4_tile_launch<64, 64, 2, 2, 0, 2>(L, a, n);
-    case kMx4Tile64x128: return mx4_tile_launch<64, 128, 1, 4, 0, 2>(L, a, n);
     case kMx4Tile128x128: return mx4_tile_launch<128, 128, 2, 2, 0, 2>(L, a, n);
     case kMx4Tile256x128: return mx4_tile_launch<256, 128, 4, 2, 2, 2>(L, a, n);
     case kMx4Tile256x256: return mx4_tile_launch<256, 256, 4, 2, 2, 2>(L, a, n);

@@ -569,7 +569,7 @@ int bm_mx4_dequantize(bm_ctx *ctx, const uint8_t *codes_dev, const uint8_t *scal
 /* y[t * ld_y + r] = the sum over blocks of 2^(scales[t] + w_scales[r] - 254) times the sum of the 32 products of codes[t] and w[r], for
  * t < m, r < rows (1 .. 2^22 each), formed in f32 (products and sums of 32 are exact; the order in which blocks are added
  * depends on the sizes alone) and rounded once. A sum past f32's range is infinite, a NaN scale makes every value it takes part in NaN. w_dev:
- * rows of bm_mx4_row_bytes(k) bytes. */
+ * rows of bm_mx4_row_bytes(k) bytes; what their codes hold behind the k-th is not looked at (the columns' zeros meet it). */
 int bm_mx4_gemm(bm_ctx *ctx, const uint8_t *w_dev, const uint8_t *w_scales_dev, int rows, int k, const uint8_t *codes_dev, const uint8_t *scales_dev,
                 int m, void *y_dev, int y_type, int64_t ld_y);
 /* bm_mx4_quantize of x_dev's m rows and bm_mx4_gemm in one call, with the same codes and scales (caller-held, m rows); the sums may be added in another
@@ -659,6 +659,8 @@ int bm_block_sums(bm_ctx *ctx, const bm_weights *w, int64_t row, const bm_act *a
  * bm_i8_gemm_experts takes for these sizes, so that a test knows which kernel a size runs: the columns and rows of a workgroup in bits 0..9
  * and 10..19, its waves in 20..23, its LDS buffers in 24..27. All forms give the same bits. BM_ESHAPE for numbers that the entry refuses. */
 int bm_i8_gemm_form(int n_experts, int rows, int k, int n_cols, int n_slots, int top_k);
+/* The same of bm_mx4_gemm and bm_mx4_gemm_experts. (The forms add a row's blocks in orders of their own.) */
+int bm_mx4_gemm_form(int n_experts, int rows, int k, int n_cols, int n_slots, int top_k);
 
 /* ------------------------------------------------------------------------------------ graphs and events */
 
