@@ -915,12 +915,16 @@ hipError_t mx4_gemm(const Launch &L, const uint8_t *w, const uint8_t *ws, int n_
 // become bf16 values exactly, a few instructions for eight, and the products run on the bf16 matrix instructions, the tokens' values in parts that
 // add up to them: one of bf16, two of f16, three of f32, and of h two (f32: three).
 
-// What the first launch leaves for the second: the experts that are hit, ascending, and for each the slot by which a token picked it, the first if
-// there are several, kMoeNone for none.
+// What the first launch leaves for the second: the experts that are hit, ascending, and for each and each token the slot that picked it, the first if
+// there are several, kMoeNone for none, and its weight, the sum over all of the token's slots of it.
 constexpr u32 kMoeExperts = 1024, kMoeNone = 0xffff;
 struct MoeTable {
     u32 n_hit, unused[15];
-    uint16_t expert[kMoeExperts], slot[kMoeExperts][kMx4MoeTokens];
+    uint16_t expert[kMoeExperts];
+    struct Hit {
+        float weight[kMx4MoeTokens];
+        uint16_t slot[kMx4MoeTokens];
+    } hit[kMoeExperts];
 };
 struct Mx4Moe {
     const uint8_t *wg, *wgs, *wu, *wus, *wd, *wds;
@@ -929,7 +933,7 @@ struct Mx4Moe {
     size_t ld_x, ld_resid, ld_y;
     const u32 *sel;
     const float *w;
-    MoeTable *table; // (as many of the slots' rows as there can be hits)
+    MoeTable *table; // (as many hits as there can be)
     __bf16 *h;       // a slot's parts, rows of ff rounded up to 32 values
     float *partial;  // the second launch's sums where several workgroups share the experts: by workgroup, tokens x hidden rounded up to 4
     void *y;
@@ -1008,6 +1012,10 @@ __device__ __forceinline__ bool moe_nth(const MoePicks &p, u32 n_experts, u32 n,
 
 // Has the compiler take w anew: what is made of it in a loop stays there, and does not wait in registers (eight times as many) for all of them.
 __device__ __forceinline__ void moe_anew(v4i &w) { __asm__ volatile("" : "+v"(w)); }
+__device__ __forceinline__ u32 moe_anew(u32 v) {
+    __asm__ volatile("" : "+v"(v));
+    return v;
+}
 // Eight codes as bf16 values under their scale.
 __device__ __forceinline__ v8h moe_codes(u32 word, float s) {
     const v2h p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 1),
@@ -1115,7 +1123,7 @@ __device__ __forceinline__ unsigned long long moe_first(unsigned long long m) {
 // the expert's tokens, less those of the shares in front. The first workgroup of an expert leaves its slots for the second launch. 0: there are not as many
 // shares; 1: tokens that picked the expert twice have left none for this one; 2: there it is.
 struct MoeEntry {
-    u32 expert, slot, place, columns, n_shares;
+    u32 expert, slot, place, columns, n_shares, rank; // rank: of an expert's first workgroup's first wave
 };
 template <int UC>
 __device__ __forceinline__ int moe_entry(const Mx4Moe &a, const MoePicks &p, const uint16_t *sel, u32 n, MoeEntry &e) {
@@ -1126,7 +1134,7 @@ __device__ __forceinline__ int moe_entry(const Mx4Moe &a, const MoePicks &p, con
     if (!there) return 0;
     e.n_shares = s.n_shares;
     e.expert = s.expert;
-    e.slot = kMoeNone;
+    e.slot = e.rank = kMoeNone;
     if (lane < a.n_tokens)
         for (u32 i = a.top_k; i-- > 0;)
             if (sel[lane * a.top_k + i] == e.expert) e.slot = lane * a.top_k + i;
@@ -1135,7 +1143,8 @@ __device__ __forceinline__ int moe_entry(const Mx4Moe &a, const MoePicks &p, con
     e.place = (u32)__builtin_popcountll(users & ((1ull << lane) - 1)) - s.share * UC;
     if (blockIdx.x == 0 && s.share == 0 && threadIdx.x < 64) {
         if (lane == 0) a.table->expert[s.rank] = (uint16_t)e.expert;
-        a.table->slot[s.rank][lane] = (uint16_t)e.slot;
+        a.table->hit[s.rank].slot[lane] = (uint16_t)e.slot;
+        e.rank = s.rank;
     }
     if (s.share * UC >= n_users) return 1;
     e.columns = min(n_users - s.share * UC, (u32)UC);
@@ -1144,21 +1153,20 @@ __device__ __forceinline__ int moe_entry(const Mx4Moe &a, const MoePicks &p, con
 // Up to sixteen of an expert's tokens, a column each.
 struct MoeColumns {
     u32 slot[16], token[16];
-    float weight[16];
 };
 __device__ __forceinline__ void moe_columns(const MoeEntry &e, MoeColumns &col) {
     if (e.slot == kMoeNone || e.place >= e.columns) return;
     col.slot[e.place] = e.slot;
     col.token[e.place] = threadIdx.x & 63;
 }
-// And their weights, each over all of a token's slots of the expert. (Asked for behind the first lines, which are waited for anyway.)
-__device__ __forceinline__ void moe_weights(const Mx4Moe &a, const uint16_t *sel, const MoeEntry &e, MoeColumns &col) {
+// And the weights for the second launch. (Asked for behind the first lines, which are waited for anyway.)
+__device__ __forceinline__ void moe_weights(const Mx4Moe &a, const uint16_t *sel, const MoeEntry &e) {
     const u32 token = threadIdx.x & 63;
-    if (threadIdx.x >= 64 || e.slot == kMoeNone || e.place >= e.columns) return;
+    if (e.rank == kMoeNone || e.slot == kMoeNone) return;
     float by = a.w[e.slot];
     for (u32 s = e.slot + 1; s < (token + 1) * a.top_k; s++)
         if (sel[s] == e.expert) by = __fadd_rn(by, a.w[s]);
-    col.weight[e.place] = by;
+    a.table->hit[e.rank].weight[token] = by;
 }
 // Sixteen rows of h from r0 on, of as many columns as 256 threads have: a thread a value, row threadIdx.x % 16, column threadIdx.x / 16. gate, up: the first of
 // the waves' sums, `stride` bytes apart. ONE: the rows may end in the first half of a block, whose other half becomes zeros.
@@ -1177,7 +1185,7 @@ __device__ __forceinline__ void moe_leave(const Mx4Moe &a, const MoeColumns &col
     }
     bool odd = false;
     float v = 0.0f;
-    if (f < a.ff) v = __fmul_rn(bm_gate_rule(a.rule.act, a.rule.limit, g, u, odd), col.weight[column]);
+    if (f < a.ff) v = bm_gate_rule(a.rule.act, a.rule.limit, g, u, odd);
     if (odd) bm_raise(a.fault, a.layer, kSiteF32Product);
     __bf16 *to = a.h + (size_t)of * PH * ffp + f;
 #pragma unroll
@@ -1258,7 +1266,7 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
                     for (int p = 0; p < P; p++) *reinterpret_cast<v8h *>(to + p * kMoePart) = part[p];
                 }
-        moe_weights(a, sel, entry, col);
+        moe_weights(a, sel, entry);
         v4f acc[2];
         u32 done = 0, tile = 0;
         const auto step = [&](uint8_t *stage, u32 (&s)[2], uint8_t *free, u32 (&next)[2]) {
@@ -1403,7 +1411,7 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
         __builtin_amdgcn_sched_barrier(0);
         if (wave < lines) ask(ring0, s0, wave);
         if (wave + NW < lines) ask(ring1, s1, wave + NW);
-        moe_weights(a, sel, entry, col);
+        moe_weights(a, sel, entry);
         v4f acc[R];
 #pragma unroll
         for (int g = 0; g < R; g++) acc[g] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -1497,19 +1505,16 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
     const u32 q0 = items * share / shares, q1 = items * (share + 1) / shares;
     L src;
     src.begin(lane);
-    size_t from[2 * R], mark[R]; // rows past the last are the last once more, and not stored
-#pragma unroll
-    for (u32 g = 0; g < 2 * R; g++) from[g] = (size_t)min(r0 + 8 * g + (lane >> 3), a.hidden - 1) * kp;
-#pragma unroll
-    for (u32 g = 0; g < R; g++) mark[g] = (size_t)min(r0 + 16 * g + c, a.hidden - 1) * ks + at;
     u32 n = q0 / lines, l = q0 - n * lines, ask_n = n, ask_l = l, ask_q = q0;
     u32 s0[R], s1[R];
     const auto ask = [&](uint8_t *stage, u32 (&s)[R]) {
-        const u32 e = (u32)__builtin_amdgcn_readfirstlane(list[ask_n]);
+        const size_t row = (size_t)(u32)__builtin_amdgcn_readfirstlane(list[ask_n]) * a.hidden + r0;
+        const uint8_t *const codes = a.wd + row * kp, *const scales = a.wds + row * ks + 8 * ask_l;
+        const u32 of = moe_anew(lane), last = a.hidden - 1 - r0; // rows past the last are the last once more, and not stored
 #pragma unroll
-        for (int g = 0; g < R; g++) s[g] = mx4_two(a.wds + (size_t)e * a.hidden * ks + mark[g] + 8 * ask_l);
+        for (u32 g = 0; g < R; g++) s[g] = mx4_two(scales + (min(16 * g + (of & 15), last) * ks + 2 * (of >> 4)));
 #pragma unroll
-        for (int g = 0; g < 2 * R; g++) src.from[g] = (const int8_t *)a.wd + (size_t)e * a.hidden * kp + from[g];
+        for (u32 g = 0; g < 2 * R; g++) src.from[g] = (const int8_t *)codes + min(8 * g + (of >> 3), last) * kp;
         __builtin_amdgcn_sched_barrier(0);
         src.ask(stage + mine, ask_l, kp);
         __builtin_amdgcn_sched_barrier(0);
@@ -1517,8 +1522,9 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
         if (++ask_l == lines) ask_l = 0, ask_n++;
     };
 
-    // The tokens of an expert: lane t's slot, and those that have one, as bits.
+    // The tokens of an expert: lane t's slot and weight, and those that have one, as bits.
     u32 slot = kMoeNone, next_slot = kMoeNone;
+    float weight = 0.0f, next_weight = 0.0f;
     unsigned long long users = 0;
     const u32 part_at = (lane >> 5) * ffp + 8 * (lane & 31), put_at = (lane >> 5) * kMoePart + moe_put(lane & 31);
     uint4 held[UC * NL];
@@ -1528,7 +1534,7 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
         for (int j = 0; j < UC; j++) {
             if (some) {
                 const u32 of = (u32)__builtin_amdgcn_readlane((int)slots, __builtin_ctzll(some));
-                const __bf16 *h = a.h + (size_t)of * PH * ffp + 256 * line + part_at;
+                const __bf16 *h = a.h + (size_t)of * PH * ffp + 256 * line + moe_anew(part_at);
                 const bool there = 8 * line + (lane & 31) / 4 < blocks;
 #pragma unroll
                 for (int i = 0; i < NL; i++) {
@@ -1550,13 +1556,11 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
             some &= some - 1;
         }
     };
-    v4f acc[NT][R][CH];
+    v4f acc[NT][R];
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int i = 0; i < CH; i++) acc[t][r][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int r = 0; r < R; r++) acc[t][r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     const auto step = [&](uint8_t *stage, u32 (&s)[R], u32 q) {
         if (q + 1 < q1) loads_landed<kLoads>(); // the next stage may be on its way; this line's values of h are older than it
         else loads_landed<0>();
@@ -1565,7 +1569,9 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
         const bool turn = l + 1 == lines;
         const unsigned long long next_users = turn ? __ballot(next_slot != kMoeNone) : users;
         if (q + 1 < q1) fetch(moe_first<UC>(next_users), turn ? next_slot : slot, turn ? 0 : l + 1);
-        const u32 after = turn && n + 2 < n_hit ? a.table->slot[n + 2][lane] : kMoeNone;
+        const bool more = turn && n + 2 < n_hit;
+        const u32 of = moe_anew(lane), after = more ? a.table->hit[n + 2].slot[of] : kMoeNone;
+        const float after_weight = more ? a.table->hit[n + 2].weight[of] : 0.0f;
         __builtin_amdgcn_sched_barrier(0);
         v4i w[R][2];
         float by[R][2];
@@ -1590,7 +1596,9 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
 #pragma unroll
                 for (int r = 0; r < R; r++) moe_anew(w[r][0]), moe_anew(w[r][1]);
                 const u32 before = (u32)__builtin_popcountll(some & ((1ull << (16 * t)) - 1)) + (u32)__builtin_popcount(here & ((1u << c) - 1));
-                const uint8_t *row = rows + (here >> c & 1 ? wave * UC + before : (u32)(NW * UC)) * kRow + moe_at(lane);
+                const bool user = here >> c & 1;
+                const uint8_t *row = rows + (user ? wave * UC + before : (u32)(NW * UC)) * kRow + moe_at(lane);
+                v4f sum[R][CH];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     v8h code[R];
@@ -1600,8 +1608,17 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
                     for (int p = 0; p < PH; p++) {
                         const v8h value = moe_as_parts(*reinterpret_cast<const uint4 *>(row + p * kMoePart + 16 * i));
 #pragma unroll
-                        for (int r = 0; r < R; r++) acc[t][r][i % CH] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code[r], value, acc[t][r][i % CH], 0, 0, 0);
+                        for (int r = 0; r < R; r++)
+                            sum[r][i % CH] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code[r], value, i < CH && p == 0 ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : sum[r][i % CH], 0, 0, 0);
                     }
+                }
+                // What a token has that did not pick the expert stays: its zeros times a NaN scale or an infinity would be NaN.
+                const float by_weight = __shfl(weight, 16 * t + c);
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    if (CH > 1) sum[r][0] += sum[r][CH - 1];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[t][r][i] = user ? __fmaf_rn(by_weight, sum[r][0][i], acc[t][r][i]) : acc[t][r][i];
                 }
             }
             if (!left) break;
@@ -1619,13 +1636,14 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
         if (turn) {
             l = 0, n++;
             slot = next_slot, users = next_users, next_slot = after;
+            weight = next_weight, next_weight = after_weight;
         } else {
             l++;
         }
     };
     if (q0 < q1) {
-        slot = a.table->slot[n][lane];
-        if (n + 1 < n_hit) next_slot = a.table->slot[n + 1][lane];
+        slot = a.table->hit[n].slot[lane], weight = a.table->hit[n].weight[lane];
+        if (n + 1 < n_hit) next_slot = a.table->hit[n + 1].slot[lane], next_weight = a.table->hit[n + 1].weight[lane];
         users = __ballot(slot != kMoeNone);
         fetch(moe_first<UC>(users), slot, l);
         __builtin_amdgcn_sched_barrier(0);
@@ -1642,11 +1660,7 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
 #pragma unroll
     for (int t = 0; t < NT; t++) {
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-            v4f sum = acc[t][r][0];
-            if (CH > 1) sum += acc[t][r][CH - 1];
-            *reinterpret_cast<v4f *>(ring0 + mine + r * 1024 + 16 * lane) = sum;
-        }
+        for (int r = 0; r < R; r++) *reinterpret_cast<v4f *>(ring0 + mine + r * 1024 + 16 * lane) = acc[t][r];
         __syncthreads();
         const u32 token = 16 * t + c, row = r0 + 16 * wave + 4 * (lane >> 4);
         if (wave < R && token < a.n_tokens && row < a.hidden) {
@@ -1658,13 +1672,19 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
         __syncthreads();
     }
 }
+constexpr u32 kMoeSharers = 8;
 // The workgroups' sums, in their order.
 template <int ET>
 __global__ __launch_bounds__(256) void k_mx4_moe_join(Mx4Moe a, u32 n) {
     const u32 quads = (a.hidden + 3) / 4, i = blockIdx.x * 256 + threadIdx.x;
     if (i >= quads * a.n_tokens) return;
-    v4f sum = *reinterpret_cast<const v4f *>(a.partial + (size_t)i * 4);
-    for (u32 z = 1; z < n; z++) sum += *reinterpret_cast<const v4f *>(a.partial + ((size_t)z * quads * a.n_tokens + i) * 4);
+    v4f part[kMoeSharers], sum; // all asked for at once, the last as often as there are fewer
+#pragma unroll
+    for (u32 z = 0; z < kMoeSharers; z++) part[z] = *reinterpret_cast<const v4f *>(a.partial + ((size_t)min(z, n - 1) * quads * a.n_tokens + i) * 4);
+    sum = part[0];
+#pragma unroll
+    for (u32 z = 1; z < kMoeSharers; z++)
+        if (z < n) sum += part[z];
     float v[4] = {sum[0], sum[1], sum[2], sum[3]};
     moe_onto<ET>(a, i / quads, 4 * (i % quads), v);
 }
@@ -1681,7 +1701,7 @@ static void moe_up_short(const Launch &L, const Mx4Moe &a) {
     hipLaunchKernelGGL((k_mx4_moe_up_short<ET, S, UC>), dim3((tiles + per - 1) / per, hits), dim3(64 * kMoeUpWaves), (a.n_tokens * a.top_k * 2 + 15) & ~15u, L.stream, a, per);
 }
 // Workgroups that share the lines of down's experts: where its rows are few, as many as fill the card (two a slot of a token at most: what the scratch holds).
-static u32 moe_sharers(int top_k, int hidden) { return (u32)std::max(1, std::min({8, 2 * top_k, 256 * 32 / hidden})); }
+static u32 moe_sharers(int top_k, int hidden) { return (u32)std::max(1, std::min({(int)kMoeSharers, 2 * top_k, 256 * 32 / hidden})); }
 template <int ET, int NW, int R, int UC, int NT>
 static hipError_t moe_down(const Launch &L, const Mx4Moe &a, u32 sharers) {
     hipLaunchKernelGGL((k_mx4_moe_down<ET, NW, R, UC, NT>), dim3((a.hidden + 16 * R - 1) / (16 * R), sharers), dim3(64 * NW), 0, L.stream, a);
@@ -1705,7 +1725,7 @@ static hipError_t moe_launch(const Launch &L, const Mx4Moe &a) {
     return moe_down<ET, NW, 2, UC, NT>(L, a, 1);
 }
 
-static size_t moe_table(int n_tokens, int top_k) { return offsetof(MoeTable, slot) + (size_t)moe_hits(n_tokens, top_k, kMoeExperts) * sizeof(MoeTable::slot[0]); }
+static size_t moe_table(int n_tokens, int top_k) { return offsetof(MoeTable, hit) + (size_t)moe_hits(n_tokens, top_k, kMoeExperts) * sizeof(MoeTable::Hit); }
 static size_t moe_h(int n_tokens, int top_k, int ff) { return (size_t)n_tokens * top_k * 3 * ((ff + 31) / 32 * 32) * 2; }
 size_t mx4_moe_work(int n_tokens, int top_k, int hidden, int ff) {
     const u32 sharers = moe_sharers(top_k, hidden);
