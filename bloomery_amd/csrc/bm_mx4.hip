@@ -479,7 +479,8 @@ __device__ __forceinline__ void mx4_ask(Mx4Src<G> &s, uint8_t *buf, u32 wave) {
     for (int r = 0; r < G::RR; r++) mx4_load(s.w, s.w_end, buf + G::kColumns * 128 + tile_row_group<G>(wave, r) * 1024, s.row[r], s.at);
     s.at += 128;
 }
-// Four steps' scales.
+// Four steps' scales, 32 bytes a line, two pieces, which change places in every second eight lines: a step's of sixteen lines come from all the banks.
+__device__ __forceinline__ u32 mx4_mark_turn(u32 line) { return 2 * (line & 8); }
 template <class G>
 __device__ __forceinline__ void mx4_ask_marks(Mx4Src<G> &s, uint8_t *marks, u32 wave) {
 #pragma unroll
@@ -492,33 +493,35 @@ __device__ __forceinline__ void mx4_ask_marks(Mx4Src<G> &s, uint8_t *marks, u32 
 }
 // In a step that has landed, the columns' blocks from `have` on become zeros, and the scales there 1, the rows' too.
 template <class G>
-__device__ __forceinline__ void mx4_zero_past(uint8_t *buf, uint8_t *marks, u32 have) {
+__device__ __forceinline__ void mx4_zero_past(uint8_t *buf, uint8_t *marks, u32 place, u32 have) {
     for (u32 i = threadIdx.x; i < G::kColumns * 8; i += G::kThreads)
         if (((i & 7) ^ line_swizzle(i >> 3)) >= have) *reinterpret_cast<uint4 *>(buf + 16 * i) = make_uint4(0, 0, 0, 0);
     for (u32 i = threadIdx.x; i < G::kLines; i += G::kThreads)
-        for (u32 b = have; b < 8; b++) marks[32 * i + b] = 127;
+        for (u32 b = have; b < 8; b++) marks[32 * i + (place ^ mx4_mark_turn(i)) + b] = 127;
     __syncthreads();
 }
 
 // Where a lane's reads begin: the lines' (TileAt, by buffer) and the scales'.
 struct Mx4At {
     TileAt line[2];
-    u32 sa, sb;
+    u32 sa, sb, turn;
 };
 // A step's scales: two blocks' of each of a wave's tiles.
 template <class G>
 struct Mx4Marks {
     u32 a[G::TR], b[G::TT];
-    __device__ __forceinline__ void read(const uint8_t *__restrict__ marks, const Mx4At &at) {
+    __device__ __forceinline__ void read(const uint8_t *__restrict__ marks, u32 place, const Mx4At &at) {
+        const uint8_t *mine = marks + (place ^ at.turn);
 #pragma unroll
-        for (int j = 0; j < G::TT; j++) b[j] = mx4_two(marks + at.sb + j * 512);
+        for (int j = 0; j < G::TT; j++) b[j] = mx4_two(mine + at.sb + j * 512);
 #pragma unroll
-        for (int i = 0; i < G::TR; i++) a[i] = mx4_two(marks + at.sa + i * 512);
+        for (int i = 0; i < G::TR; i++) a[i] = mx4_two(mine + at.sa + i * 512);
     }
 };
-// Where a step's scales lie: four steps' in one half, the next four's in the other.
+// Where a step's scales lie: four steps' in one half, the next four's in the other; and their place in a line's.
 template <class G>
-__device__ __forceinline__ u32 mx4_mark_at(u32 step) { return (step >> 2 & 1) * G::kMarks + (step & 3) * 8; }
+__device__ __forceinline__ u32 mx4_mark_half(u32 step) { return (step >> 2 & 1) * G::kMarks; }
+__device__ __forceinline__ u32 mx4_mark_place(u32 step) { return (step & 3) * 8; }
 template <int H, int N, int TT>
 __device__ __forceinline__ void mx4_multiply(const v4i (&a)[N], const v4i (&b)[TT], const u32 *sa, const u32 (&sb)[TT], v4f (*acc)[TT]) {
 #pragma unroll
@@ -537,8 +540,10 @@ template <class G, Mx4Steps STEP, class F>
 __device__ __forceinline__ void mx4_next(Mx4Src<G> &src, uint8_t *buf, uint8_t *next, uint8_t *marks, const Mx4Way &way, F read) {
     if constexpr (STEP == kLast) return;
     mx4_turn();
-    if (STEP == kNext && way.tail < 8) mx4_zero_past<G>(next, marks + mx4_mark_at<G>(way.step + 1), way.tail);
-    read(marks + mx4_mark_at<G>(way.step + 1));
+    uint8_t *half = marks + mx4_mark_half<G>(way.step + 1);
+    const u32 place = mx4_mark_place(way.step + 1);
+    if (STEP == kNext && way.tail < 8) mx4_zero_past<G>(next, half, place, way.tail);
+    read(half, place);
     if (STEP == kNext) return;
     mx4_ask<G>(src, buf, way.wave);
 }
@@ -554,7 +559,7 @@ struct Mx4Parts {
     template <int B>
     __device__ __forceinline__ void begin(const uint8_t *buf, const uint8_t *marks, const Mx4At &at) {
         constexpr int up = B >= G::kUp;
-        s.read(marks, at);
+        s.read(marks, 0, at);
         tile_read<G, B>(a, buf, at.line[up].a[0], 0);
         tile_read<G, B>(b, buf, at.line[up].b[0], 0);
     }
@@ -575,8 +580,8 @@ struct Mx4Parts {
             else tile_weave<Q, Q * G::TT>();
         }
         const Mx4Marks<G> mine = s;
-        mx4_next<G, STEP>(src, buf, next, marks, way, [&](const uint8_t *m) {
-            s.read(m, at);
+        mx4_next<G, STEP>(src, buf, next, marks, way, [&](const uint8_t *m, u32 place) {
+            s.read(m, place, at);
             tile_read<G, 1 - B>(a, next, at.line[nextUp].a[0], 0);
             tile_read<G, 1 - B>(b, next, at.line[nextUp].b[0], 0);
         });
@@ -595,9 +600,9 @@ struct Mx4Whole {
         Mx4Marks<G> s;
     } set[2];
     template <int B>
-    __device__ __forceinline__ void read(const uint8_t *__restrict__ buf, const uint8_t *__restrict__ marks, const Mx4At &at) {
+    __device__ __forceinline__ void read(const uint8_t *__restrict__ buf, const uint8_t *__restrict__ marks, u32 place, const Mx4At &at) {
         constexpr int up = B >= G::kUp;
-        set[B].s.read(marks, at);
+        set[B].s.read(marks, place, at);
 #pragma unroll
         for (int c = 0; c < 2; c++) {
             tile_read<G, B>(set[B].a[c], buf, at.line[up].a[c], 0);
@@ -605,11 +610,11 @@ struct Mx4Whole {
         }
     }
     template <int B>
-    __device__ __forceinline__ void begin(const uint8_t *buf, const uint8_t *marks, const Mx4At &at) { read<B>(buf, marks, at); }
+    __device__ __forceinline__ void begin(const uint8_t *buf, const uint8_t *marks, const Mx4At &at) { read<B>(buf, marks, 0, at); }
     template <int B, Mx4Steps STEP>
     __device__ __forceinline__ void step(Mx4Src<G> &src, uint8_t *__restrict__ buf, uint8_t *__restrict__ next, uint8_t *__restrict__ marks, Mx4Way &way,
                                          const Mx4At &at, v4f (&acc)[G::TR][G::TT]) {
-        mx4_next<G, STEP>(src, buf, next, marks, way, [&](const uint8_t *m) { read<1 - B>(next, m, at); });
+        mx4_next<G, STEP>(src, buf, next, marks, way, [&](const uint8_t *m, u32 place) { read<1 - B>(next, m, place, at); });
         mx4_multiply<0>(set[B].a[0], set[B].b[0], set[B].s.a, set[B].s.b, acc);
         mx4_multiply<1>(set[B].a[1], set[B].b[1], set[B].s.a, set[B].s.b, acc);
         way.step++;
@@ -722,7 +727,7 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     for (int r = 0; r < G::RG; r++) {
         const u32 line = mx4_mark_group<G>(wave, r) * 32 + (lane >> 1);
         const u32 row = min(r0 + line - (u32)BT, a.rows - 1) - r0;
-        src.mark[r] = (line < (u32)BT ? col[G::RT + r] : row) * a.ks + 16 * (lane & 1);
+        src.mark[r] = (line < (u32)BT ? col[G::RT + r] : row) * a.ks + (16 * (lane & 1) ^ mx4_mark_turn(line));
     }
 
     v4f acc[G::TR][G::TT];
@@ -734,6 +739,7 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     Mx4At at;
     at.sa = (wr + (lane & 15)) * 32 + 2 * (lane >> 4);
     at.sb = (wt + (lane & 15)) * 32 + 2 * (lane >> 4);
+    at.turn = mx4_mark_turn(lane);
 #pragma unroll
     for (u32 c = 0; c < 2; c++) {
         const u32 piece = (lane & 15) * 128 + 16 * ((2 * (lane >> 4) + c) ^ line_swizzle(lane & 15));
@@ -755,7 +761,7 @@ __global__ __launch_bounds__(64 * WT * WR) __attribute__((amdgpu_waves_per_eu(EU
     } else {
         mx4_ask<G>(src, ring1, wave);
         mx4_turn();
-        if (last == 0 && way.tail < 8) mx4_zero_past<G>(ring1, marks, way.tail);
+        if (last == 0 && way.tail < 8) mx4_zero_past<G>(ring1, marks, 0, way.tail);
         if (last) mx4_ask<G>(src, ring0, wave);
         f.template begin<1>(ring1, marks, at);
         if (last) {
