@@ -60,7 +60,9 @@ __device__ __forceinline__ u32 mx4_block(const float (&v)[8], u32 &scale) {
     return bad ? 0u : word;
 }
 
-// A wave takes sixteen blocks of a row, sixteen bytes of its scales: a lane eight values, four lanes a block.
+// A wave takes sixteen blocks of a row, sixteen bytes of its scales: a lane eight values, four lanes a block, whose maximum is two exchanges between
+// neighbours, so that nothing goes through LDS and a value is read once. Memory bounds it: 4096 x 7168 bf16 17 us, 4.3 TB/s of 74 MB; behind the gate rule 2664 x 2048
+// f16 5 us; 16 x 2048 f32 2.4 us, a launch.
 template <int ET, bool GLU>
 __global__ __launch_bounds__(256) void k_mx4_quantize(Mx4Rows a) {
     const u32 lane = threadIdx.x & 63, units = a.ks / 16, unit = group_index() * 4 + (threadIdx.x >> 6), row = unit / units;
@@ -102,6 +104,7 @@ __device__ __forceinline__ void mx4_values(u32 word, u32 scale, float (&v)[8]) {
     v[0] = p0[0], v[1] = p0[1], v[2] = p1[0], v[3] = p1[1], v[4] = p2[0], v[5] = p2[1], v[6] = p3[0], v[7] = p3[1];
 }
 
+// And back, the same shares: 4096 x 7168 to bf16 12.3 us, 6.0 TB/s (the codes come from the last-level cache).
 template <int ET>
 __global__ __launch_bounds__(256) void k_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, u32 m, u32 k, u32 kp, u32 ks, void *y, size_t ld) {
     const u32 lane = threadIdx.x & 63, units = ks / 16, unit = group_index() * 4 + (threadIdx.x >> 6), row = unit / units;
@@ -201,7 +204,8 @@ __device__ __forceinline__ v4f mx4_join(const uint8_t *ring, u32 tile, u32 lane)
 
 // Few columns a matrix: 16 R rows a workgroup against 16 C columns, its NW waves dealing the row's lines among them, each through a ring of four
 // stages of its own, two on their way while one is multiplied and the fourth is asked for; a line's scales come straight to registers, asked for with it. The
-// waves' sums meet in LDS.
+// waves' sums meet in LDS. Few workgroups have a row's whole k to get through, so the way from memory bounds it, and with k over the waves a workgroup has as
+// many lines on their way as it has waves and stages: 24 x 7168 x 2048 4.9 us (with whole rows of k in tiles of 32 x 64 5.8), one row of 7168 x 7168 7.7, 3.5 TB/s.
 template <int R, int C, int NW>
 __global__ __launch_bounds__(64 * NW) void k_mx4_few(Mx4Args a) {
     typedef Lines<2 * (R + C)> L;
@@ -309,7 +313,8 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_few(Mx4Args a) {
 
 // A few rows from their floating values: k_mx4_few's product with the quantizer in front of it in every workgroup, while the first weights are on
 // their way. M (a power of two, at least the rows): the waves are dealt to the rows, 4 pieces of eight values a thread at most, four threads a
-// block. Codes and scales go to LDS; the first workgroup leaves them in memory too.
+// block. Codes and scales go to LDS; the first workgroup leaves them in memory too. One launch for two, whose cost it is: 1 x 768 x 2048 f32 3.9 us,
+// as much as k_mx4_few alone; for more than eight rows the values would cost each workgroup more than a launch.
 constexpr int kMx4FewX = 8, kMx4FewXWaves = 8; // rows at most
 constexpr u32 mx4_few_x_values(u32 M) { return 64 * kMx4FewXWaves * 8 * 4 / M; } // values a row may have
 template <int ET, int M, int R>
@@ -433,6 +438,10 @@ __global__ __launch_bounds__(64 * kMx4FewXWaves) void k_mx4_few_x(Mx4Args a, Mx4
 // lane, no register in between), and 32 bytes of scales a column and a row, four steps' worth, through two more: while the waves multiply one step
 // the next is on its way, one barrier a step. A wave holds (BT / WT) x (BR / WR) sums in v_mfma_scale_f32_16x16x128_f8f6f4's form; Q of its tiles of rows are a part
 // of a step (0: all).
+// What bounds it: in large products the way into LDS, some 32 bytes a cycle and unit, so that an instruction of 16 cycles wants tiles of 256 x 256 (8192 cubed 247 us,
+// 4.5 PFLOP/s, of 6.5 that the instructions alone reach on random codes; 256 x 128 302, 128 x 128 328), whose 128 sums a lane leave no registers for a
+// third set: scales come four steps at once, offsets go into the buffers' descriptors, and no step has a branch (without these 203 registers
+// and more went to scratch). In small ones the way from memory: 777 x 2000 x 1996 8 us at 1.6 tiles a unit.
 template <int BT, int BR, int WT, int WR, int Q>
 struct Mx4Tile {
     static constexpr int kColumns = BT, kRows = BR, kLines = BT + BR, kWaves = WT * WR, kThreads = 64 * kWaves, kStage = kLines * 128, kMarks = kLines * 32;
@@ -853,15 +862,15 @@ enum Mx4Form : u32 {
 
 // Which form, us on MI355X, bf16 out, weights of three sets in turn (two for experts), the chosen form's first.
 //   One matrix. While tiles of at most 32 x 32 are no more than the compute units a workgroup's waves share a row's k, in the smallest tile that is one round: 16 x 2048 x
-//   7168 in 16 x 16 5.3 (16 x 32: 6.9, 32 x 64: 9.4), 64 x 2048 x 7168 in 16 x 32 7.0 (32 x 32: 8.3; 16 x 16, two rounds: 9.3), 128 x 2048 x 7168 in 32 x 32 8.5 (32 x 64: 13.5), one
-//   row of 7168 x 7168 7.6 (16 x 16: 8.8, 32 x 64: 14.8). Then whole rows of k in tiles that leave few units idle: 32 x 64 up to two a unit, 128 x 7168 x 7168 16.1 (64 x 64: 17.0), 512 x
-//   2048 x 7168 16.0 (16.7), but 1024 x 2048 x 7168 19.5 (18.6); 64 x 64 up to four, 4096 x 768 x 2048 10.3 (128 x 128: 11.9), 512 x 7168 x 7168 28.4 (29.1). Behind that whole rounds of
-//   256 units count: one of 256 x 256 tiles takes 55 units of time, of 256 x 128 34, of two 128 x 128 a unit 38. 4096 x 7168 x 7168: 107.6 in 448 tiles of 256 x 256 (256 x 128: 133, 128 x
-//   128: 138), 1024 x 7168 x 7168 34.1 in 224 of 256 x 128 (38.7; 256 x 256: 47.9), 2048 x 7168 x 2048 22.3 (25.6, 27.9), 4096 x 2048 x 2048 15.5 in 256 x 128 (16.6, 21.5).
-//   Experts, by slots an expert. Up to 12, while the rows' tiles are two a unit, by waves sharing k: 16 tokens, top 4 of 8, 2048 x 2048 5.6 (32 x 64: 7.5); 64 experts of 7168 rows: 70, 32 x 64
-//   50.6. 32 x 64 below 24 slots, or while its tiles are few: 333 tokens, top 2 of 64, 7168 x 2048 90 (64 x 64: 95), 16 slots, 128 experts, 2048 x 768 26.5 (28.7), 128 slots, 8 experts,
-//   2048 x 2048 10.6 (11.2). 64 x 64 below 56, or while few: 32 slots, 64 experts, 7168 x 2048 118.5 (128 x 128: 127.5). 128 x 128: 64 slots, 128 experts, 768 x 2048 33.4 (64 x 64: 37.9), 128
-//   slots 44.9 (256 x 256: 46.6, 64 x 64: 52.6), 256 slots 65.5 (71). 256 x 256 from 352 on: 512 slots 102.6 (128 x 128: 121.9), 64 experts, 7168 x 2048 442 (488).
+//   7168 in 16 x 16 5.3 (16 x 32: 6.9, 32 x 64: 9.5), 64 x 2048 x 7168 in 16 x 32 7.0 (32 x 32: 8.4; 16 x 16, two rounds: 9.3), 128 x 2048 x 7168 in 32 x 32 8.5 (32 x 64: 12.0), one
+//   row of 7168 x 7168 7.7 (16 x 16: 8.8, 32 x 64: 14.8). Then whole rows of k in tiles that leave few units idle: 32 x 64 up to two a unit, 128 x 7168 x 7168 16.1 (64 x 64: 16.6), 512 x
+//   2048 x 7168 16.2 (16.4), but 1024 x 2048 x 7168 19.3 (17.7); 64 x 64 up to four, 4096 x 768 x 2048 9.8 (128 x 128: 11.5), 512 x 7168 x 7168 26.6 (27.9). Behind that whole rounds of
+//   256 units count: one of 256 x 256 tiles takes 55 parts of time, of 256 x 128 34, of two 128 x 128 a unit 38. 4096 x 7168 x 7168: 104 in 448 tiles of 256 x 256 (256 x 128: 128, 128 x
+//   128: 130), 1024 x 7168 x 7168 32.5 in 224 of 256 x 128 (35.7; 256 x 256: 44.6), 2048 x 7168 x 2048 22.3 (25.4, 26.2), 4096 x 2048 x 2048 15.5 in 256 x 128 (16.2, 20.3).
+//   Experts, by slots an expert. Up to 12, while the rows' tiles are two a unit, by waves sharing k: 16 tokens, top 4 of 8, 2048 x 2048 5.9 (32 x 64: 7.5); 64 experts of 7168 rows: 70, 32 x 64
+//   50.5. 32 x 64 below 24 slots, or while its tiles are few: 333 tokens, top 2 of 64, 7168 x 2048 90 (64 x 64: 94), 16 slots, 128 experts, 2048 x 768 24.3 (25.9), 128 slots, 8 experts,
+//   2048 x 2048 10.6 (10.5). 64 x 64 below 56, or while few: 32 slots, 64 experts, 7168 x 2048 112 (32 x 64: 115, 128 x 128: 121). 128 x 128: 64 slots, 128 experts, 768 x 2048 32.0 (64 x 64:
+//   34.9), 128 slots 42.8 (256 x 256: 45.7, 64 x 64: 47.5), 256 slots 62.3 (68.6). 256 x 256 from 352 on: 512 slots 100 (128 x 128: 117), 64 experts, 7168 x 2048 419 (460).
 // n_experts 0: one matrix, n its columns; else n slots. reach: the tiles' offsets of gathered columns, 32 bits, hold the columns.
 static Mx4Form mx4_form(u32 n_experts, u32 rows, u32 n, bool reach) {
     const auto up = [](u32 x, u32 y) { return (x + y - 1) / y; };
@@ -916,10 +925,13 @@ hipError_t mx4_gemm(const Launch &L, const uint8_t *w, const uint8_t *ws, int n_
 
 // ------------------------------------------------------------------------------------ a few tokens' experts
 
-// Two launches. The first forms h: a workgroup an expert that is hit and some of its rows of gate and of up, for the tokens that picked it. The second forms y: a
-// workgroup sixteen rows of down, for all tokens, over the experts that are hit. Weights are read once by each, as lines through rings in LDS, and bound both; codes
-// become bf16 values exactly, a few instructions for eight, and the products run on the bf16 matrix instructions, the tokens' values in parts that
-// add up to them: one of bf16, two of f16, three of f32, and of h two (f32: three).
+// Two launches, three where workgroups share down's lines. The first forms h: a workgroup some rows of gate and of up of an expert that is hit, for up to UC of the tokens that
+// picked it. The second forms y: a workgroup 16 R rows of down, for all tokens, over the experts that are hit. Weights are read once by each (once for UC tokens by the first), as lines
+// through rings in LDS, and bound both; codes become bf16 values exactly, a few instructions for eight, and the products run on the bf16 matrix instructions, the tokens' values in parts
+// that add up to them, x and h alike: one of bf16, two of f16, three of f32. (The instructions that take 4-bit codes would want x and h as codes too, or as 8-bit values, whose errors
+// a decode step would not have otherwise.)
+// On MI355X, us of each launch: 1 token, top 8 of 128, 2048 x 768 bf16 8.4 + 7.1; 16 tokens in f32 44 + 29 + 4.7, 205 MB of hit experts' weights; 64 tokens, 64 of 256 experts of 7168 x 2048 here,
+// bf16, 174 (5.7 TB/s) + 113 (4.4 TB/s).
 
 // What the first launch leaves for the second: the experts that are hit, ascending, and for each and each token the slot that picked it, the first if
 // there are several, kMoeNone for none, and its weight, the sum over all of the token's slots of it.
@@ -1110,6 +1122,14 @@ struct MoePiece {
 constexpr int kMoePart = 544;
 __device__ __forceinline__ u32 moe_put(u32 piece) { return 16 * piece + (piece & 16); }
 __device__ __forceinline__ u32 moe_at(u32 lane) { return 128 * (lane >> 4) + 16 * (lane >> 5); }
+// The sixteen columns of a matrix instruction are P parts of UC tokens each, from column `first` on: where lane column c finds its part of its token in LDS, of rows from
+// `row` on; `none`: the row of zeros, for columns that are no token's.
+template <int P, int UC>
+__device__ __forceinline__ u32 moe_column(u32 c, u32 tokens, u32 row, u32 none, u32 first = 0) {
+    static_assert(P * UC <= 16, "a token's parts are columns of one instruction");
+    const u32 of = c - first, part = of / UC, token = of - part * UC;
+    return part < (u32)P && token < tokens ? (row + token) * (P * kMoePart) + part * kMoePart : none * (P * kMoePart);
+}
 // A wave's reads of LDS are done.
 __device__ __forceinline__ void lds_read() {
     __asm__ volatile("" ::: "memory");
@@ -1176,7 +1196,7 @@ __device__ __forceinline__ void moe_weights(const Mx4Moe &a, const uint16_t *sel
 }
 // Sixteen rows of h from r0 on, of as many columns as 256 threads have: a thread a value, row threadIdx.x % 16, column threadIdx.x / 16. gate, up: the first of
 // the waves' sums, `stride` bytes apart. ONE: the rows may end in the first half of a block, whose other half becomes zeros.
-template <int ET, int NW, bool ONE>
+template <int ET, int NW, int UC, bool ONE>
 __device__ __forceinline__ void moe_leave(const Mx4Moe &a, const MoeColumns &col, u32 columns, u32 r0, const uint8_t *gate, const uint8_t *up, u32 stride) {
     constexpr int PH = kMoeKept<ET>;
     static_assert(64 * NW == 256, "sixteen rows by sixteen columns");
@@ -1185,10 +1205,12 @@ __device__ __forceinline__ void moe_leave(const Mx4Moe &a, const MoeColumns &col
     const u32 of = col.slot[column], at = 256 * (threadIdx.x >> 2 & 3) + 16 * column + 4 * (threadIdx.x & 3);
     float g = 0.0f, u = 0.0f;
 #pragma unroll
-    for (int w = 0; w < NW; w++) {
-        g = __fadd_rn(g, *reinterpret_cast<const float *>(gate + w * stride + at));
-        u = __fadd_rn(u, *reinterpret_cast<const float *>(up + w * stride + at));
-    }
+    for (int w = 0; w < NW; w++)
+#pragma unroll
+        for (int p = 0; p < kMoeParts<ET>; p++) {
+            g = __fadd_rn(g, *reinterpret_cast<const float *>(gate + w * stride + at + 16 * p * UC));
+            u = __fadd_rn(u, *reinterpret_cast<const float *>(up + w * stride + at + 16 * p * UC));
+        }
     bool odd = false;
     float v = 0.0f;
     if (f < a.ff) v = bm_gate_rule(a.rule.act, a.rule.limit, g, u, odd);
@@ -1205,7 +1227,8 @@ __device__ __forceinline__ void moe_leave(const Mx4Moe &a, const MoeColumns &col
 constexpr int kMoeUpWaves = 4;
 
 // h of rows of up to 2048 values, two lines a wave at most: a workgroup goes over several tiles of sixteen rows of gate and as many of up, whose lines come through
-// a ring of S stages without a stop between the tiles; the tokens' values of a wave's lines stay in LDS.
+// a ring of S stages without a stop between the tiles; the tokens' values of a wave's lines stay in LDS. UC tokens a workgroup (an expert with more has several): LDS holds two
+// workgroups a unit with 4 of bf16 and f16, 2 of f32, and experts of a decode batch have fewer (16 tokens, top 8 of 128: one mostly, in f32 44 us; UC 4: 49).
 template <int ET, int S, int UC>
 __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(2))) void k_mx4_moe_up_short(Mx4Moe a, u32 per) {
     constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, kRow = P * kMoePart, kLoads = 6; // loads of a stage: four of lines, two of scales
@@ -1296,18 +1319,12 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
                 ask(stage, s);
             }
             if (i == 0) acc[0] = acc[1] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            const uint8_t *row = rows + (c < columns ? (wave * 2 + i) * UC + c : (u32)(NW * 2 * UC)) * kRow + moe_at(lane);
+            const uint8_t *row = rows + moe_column<P, UC>(c, columns, (wave * 2 + i) * UC, NW * 2 * UC) + moe_at(lane);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                v8h value[P];
+                const v8h value = *reinterpret_cast<const v8h *>(row + 16 * j);
 #pragma unroll
-                for (int p = 0; p < P; p++) value[p] = *reinterpret_cast<const v8h *>(row + p * kMoePart + 16 * j);
-#pragma unroll
-                for (int g = 0; g < 2; g++) {
-                    const v8h code = moe_codes((u32)w[g][j / 4][j % 4], by[g][j / 4]);
-#pragma unroll
-                    for (int p = 0; p < P; p++) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code, value[p], acc[g], 0, 0, 0);
-                }
+                for (int g = 0; g < 2; g++) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(moe_codes((u32)w[g][j / 4][j % 4], by[g][j / 4]), value, acc[g], 0, 0, 0);
             }
             done++;
         };
@@ -1316,7 +1333,7 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
             for (int g = 0; g < 2; g++) *reinterpret_cast<v4f *>(sums + wave * 2048 + g * 1024 + 16 * lane) = each ? acc[g] : v4f{0.0f, 0.0f, 0.0f, 0.0f};
             lds_meet();
-            moe_leave<ET, NW, true>(a, col, columns, 16 * (tile0 + tile), sums, sums + 1024, 2048);
+            moe_leave<ET, NW, UC, true>(a, col, columns, 16 * (tile0 + tile), sums, sums + 1024, 2048);
             lds_meet();
             tile++;
         };
@@ -1443,18 +1460,12 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
                 lds_read(); // the stage is in registers
                 ask(stage, s, l + 2 * NW);
             }
-            const uint8_t *row = rows + (c < columns ? wave * UC + c : (u32)(NW * UC)) * kRow + moe_at(lane);
+            const uint8_t *row = rows + moe_column<P, UC>(c, columns, wave * UC, NW * UC) + moe_at(lane);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                v8h value[P];
+                const v8h value = *reinterpret_cast<const v8h *>(row + 16 * i);
 #pragma unroll
-                for (int p = 0; p < P; p++) value[p] = *reinterpret_cast<const v8h *>(row + p * kMoePart + 16 * i);
-#pragma unroll
-                for (int g = 0; g < R; g++) {
-                    const v8h code = moe_codes((u32)w[g][i / 4][i % 4], by[g][i / 4]);
-#pragma unroll
-                    for (int p = 0; p < P; p++) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code, value[p], acc[g], 0, 0, 0);
-                }
+                for (int g = 0; g < R; g++) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(moe_codes((u32)w[g][i / 4][i % 4], by[g][i / 4]), value, acc[g], 0, 0, 0);
             }
         };
         for (u32 l = wave; l < lines;) {
@@ -1473,7 +1484,7 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
         __syncthreads();
 #pragma unroll 1
         for (int t = 0; t < T; t++)
-            moe_leave<ET, NW, T == 1>(a, col, columns, r0 + 16 * t, ring0 + t * 1024, ring0 + (T + t) * 1024, L::kStage);
+            moe_leave<ET, NW, UC, T == 1>(a, col, columns, r0 + 16 * t, ring0 + t * 1024, ring0 + (T + t) * 1024, L::kStage);
         if (n + gridDim.y >= entry.n_shares) return;
         __syncthreads();
     }
@@ -1494,7 +1505,8 @@ __device__ __forceinline__ void moe_onto(const Mx4Moe &a, u32 token, u32 row, fl
 // weights. gridDim.y workgroups share the lines: where they are several, a third launch adds their sums.
 template <int ET, int NW, int R, int UC, int NT>
 __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
-    constexpr int PH = kMoeKept<ET>, NL = (PH + 1) / 2, CH = NT * R == 1 ? 2 : 1; // requests of a token's values; chains of products
+    constexpr int PH = kMoeKept<ET>, NL = (PH + 1) / 2, CH = R == 1 ? 2 : 1; // requests of a token's values; chains of products
+    constexpr int kGroups = 16 / (PH * UC), kTokens = kGroups * UC;          // of UC tokens in an instruction's columns
     constexpr int kLoads = 3 * R, kRow = PH * kMoePart;                          // loads of a stage
     typedef Lines<2 * R> L;
     __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage];
@@ -1567,11 +1579,42 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
     for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int r = 0; r < R; r++) acc[t][r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    v4f sum[R][CH];
+    const auto clear = [&] {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int i = 0; i < CH; i++) sum[r][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    };
+    clear();
+    // The sums of the tokens `here`, which have columns by their order, under their weights onto what these tokens have. What the others have stays: zeros times a NaN
+    // scale or an infinity are no zeros.
+    const auto count = [&](unsigned long long here) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const u32 some = (u32)(here >> (16 * t)) & 0xffffu;
+            if (NT > 1 && some == 0) continue;
+            const bool user = some >> c & 1;
+            const u32 rank = (u32)__builtin_popcountll(here & ((1ull << (16 * t)) - 1)) + (u32)__builtin_popcount(some & ((1u << c) - 1)), group = rank / UC;
+            const int from = (int)((lane & 48) + group * (PH * UC) + (rank - group * UC));
+            const float by = __shfl(weight, 16 * t + c);
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float mine = CH > 1 ? __fadd_rn(sum[r][0][i], sum[r][CH - 1][i]) : sum[r][0][i];
+                    float v = __shfl(mine, from);
+#pragma unroll
+                    for (int p = 1; p < PH; p++) v = __fadd_rn(v, __shfl(mine, from + p * UC));
+                    acc[t][r][i] = user ? __fmaf_rn(by, v, acc[t][r][i]) : acc[t][r][i];
+                }
+        }
+        clear();
+    };
     const auto step = [&](uint8_t *stage, u32 (&s)[R], u32 q) {
         if (q + 1 < q1) loads_landed<kLoads>(); // the next stage may be on its way; this line's values of h are older than it
         else loads_landed<0>();
-        unsigned long long some = moe_first<UC>(users), left = users ^ some;
-        put(some);
+        put(moe_first<UC>(users));
         const bool turn = l + 1 == lines;
         const unsigned long long next_users = turn ? __ballot(next_slot != kMoeNone) : users;
         if (q + 1 < q1) fetch(moe_first<UC>(next_users), turn ? next_slot : slot, turn ? 0 : l + 1);
@@ -1594,50 +1637,36 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
             lds_read(); // the stage is in registers
             ask(stage, s);
         }
-        for (;;) {
+        // The expert's tokens, as many as have columns of their own at a time: where that is all of them, their sums stay over the expert's lines.
+        for (unsigned long long rest = users, first = moe_first<UC>(users);;) {
+            const unsigned long long here = moe_first<kTokens>(rest);
+            unsigned long long some = moe_first<UC>(here), left = here ^ some;
+            for (u32 column = 0;; column += PH * UC) {
+                if (some != first) { // (the values of the next line that are held are in LDS only after these)
+                    uint4 keep[UC * NL];
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const u32 here = (u32)(some >> (16 * t)) & 0xffffu;
-                if (NT > 1 && here == 0) continue;
+                    for (int i = 0; i < UC * NL; i++) keep[i] = held[i];
+                    fetch(some, slot, l);
+                    put(some);
+#pragma unroll
+                    for (int i = 0; i < UC * NL; i++) held[i] = keep[i];
+                }
 #pragma unroll
                 for (int r = 0; r < R; r++) moe_anew(w[r][0]), moe_anew(w[r][1]);
-                const u32 before = (u32)__builtin_popcountll(some & ((1ull << (16 * t)) - 1)) + (u32)__builtin_popcount(here & ((1u << c) - 1));
-                const bool user = here >> c & 1;
-                const uint8_t *row = rows + (user ? wave * UC + before : (u32)(NW * UC)) * kRow + moe_at(lane);
-                v4f sum[R][CH];
+                const uint8_t *row = rows + moe_column<PH, UC>(c, (u32)__builtin_popcountll(some), wave * UC, NW * UC, column) + moe_at(lane);
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    v8h code[R];
+                    const v8h value = *reinterpret_cast<const v8h *>(row + 16 * i);
 #pragma unroll
-                    for (int r = 0; r < R; r++) code[r] = moe_codes((u32)w[r][i / 4][i % 4], by[r][i / 4]);
-#pragma unroll
-                    for (int p = 0; p < PH; p++) {
-                        const v8h value = moe_as_parts(*reinterpret_cast<const uint4 *>(row + p * kMoePart + 16 * i));
-#pragma unroll
-                        for (int r = 0; r < R; r++)
-                            sum[r][i % CH] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code[r], value, i < CH && p == 0 ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : sum[r][i % CH], 0, 0, 0);
-                    }
+                    for (int r = 0; r < R; r++) sum[r][i % CH] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(moe_codes((u32)w[r][i / 4][i % 4], by[r][i / 4]), value, sum[r][i % CH], 0, 0, 0);
                 }
-                // What a token has that did not pick the expert stays: its zeros times a NaN scale or an infinity would be NaN.
-                const float by_weight = __shfl(weight, 16 * t + c);
-#pragma unroll
-                for (int r = 0; r < R; r++) {
-                    if (CH > 1) sum[r][0] += sum[r][CH - 1];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[t][r][i] = user ? __fmaf_rn(by_weight, sum[r][0][i], acc[t][r][i]) : acc[t][r][i];
-                }
+                if (!left) break;
+                some = moe_first<UC>(left);
+                left ^= some;
             }
-            if (!left) break;
-            some = moe_first<UC>(left);
-            // (the values of the next line that are held are in LDS only after these)
-            uint4 keep[UC * NL];
-#pragma unroll
-            for (int i = 0; i < UC * NL; i++) keep[i] = held[i];
-            fetch(some, slot, l);
-            put(some);
-#pragma unroll
-            for (int i = 0; i < UC * NL; i++) held[i] = keep[i];
-            left ^= some;
+            rest ^= here;
+            if (turn || q + 1 == q1 || here != users) count(here);
+            if (!rest) break;
         }
         if (turn) {
             l = 0, n++;
