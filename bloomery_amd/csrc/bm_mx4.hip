@@ -1130,6 +1130,11 @@ __device__ __forceinline__ u32 moe_column(u32 c, u32 tokens, u32 row, u32 none, 
     const u32 of = c - first, part = of / UC, token = of - part * UC;
     return part < (u32)P && token < tokens ? (row + token) * (P * kMoePart) + part * kMoePart : none * (P * kMoePart);
 }
+// What the lane N behind has, of the same sixteen.
+template <int N>
+__device__ __forceinline__ float moe_behind(float v) {
+    return bm_bits_f32((u32)__builtin_amdgcn_update_dpp(0, (int)bm_f32_bits(v), 0x100 | N, 0xf, 0xf, true));
+}
 // A wave's reads of LDS are done.
 __device__ __forceinline__ void lds_read() {
     __asm__ volatile("" ::: "memory");
@@ -1506,7 +1511,8 @@ __device__ __forceinline__ void moe_onto(const Mx4Moe &a, u32 token, u32 row, fl
 template <int ET, int NW, int R, int UC, int NT>
 __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
     constexpr int PH = kMoeKept<ET>, NL = (PH + 1) / 2, CH = R == 1 ? 2 : 1; // requests of a token's values; chains of products
-    constexpr int kGroups = 16 / (PH * UC), kTokens = kGroups * UC;          // of UC tokens in an instruction's columns
+    constexpr bool kOwn = NT == 1 && PH == 1;                                // a token's column is its number
+    constexpr int kGroups = 16 / (PH * UC), kTokens = kOwn ? 16 : kGroups * UC; // of UC tokens in an instruction's columns
     constexpr int kLoads = 3 * R, kRow = PH * kMoePart;                          // loads of a stage
     typedef Lines<2 * R> L;
     __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage];
@@ -1540,7 +1546,7 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
         if (++ask_l == lines) ask_l = 0, ask_n++;
     };
 
-    // The tokens of an expert: lane t's slot and weight, and those that have one, as bits.
+    // The tokens of an expert: lane t's slot and weight (of up to 16 tokens: lane t % 16's), and those that have one, as bits.
     u32 slot = kMoeNone, next_slot = kMoeNone;
     float weight = 0.0f, next_weight = 0.0f;
     unsigned long long users = 0;
@@ -1597,15 +1603,16 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
             const bool user = some >> c & 1;
             const u32 rank = (u32)__builtin_popcountll(here & ((1ull << (16 * t)) - 1)) + (u32)__builtin_popcount(some & ((1u << c) - 1)), group = rank / UC;
             const int from = (int)((lane & 48) + group * (PH * UC) + (rank - group * UC));
-            const float by = __shfl(weight, 16 * t + c);
+            const float by = NT == 1 ? weight : __shfl(weight, 16 * t + c);
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float mine = CH > 1 ? __fadd_rn(sum[r][0][i], sum[r][CH - 1][i]) : sum[r][0][i];
-                    float v = __shfl(mine, from);
-#pragma unroll
-                    for (int p = 1; p < PH; p++) v = __fadd_rn(v, __shfl(mine, from + p * UC));
+                    float v = mine;
+                    if (PH > 1) v = __fadd_rn(v, moe_behind<UC>(mine));
+                    if (PH > 2) v = __fadd_rn(v, moe_behind<2 * UC>(mine));
+                    if (!kOwn) v = __shfl(v, from);
                     acc[t][r][i] = user ? __fmaf_rn(by, v, acc[t][r][i]) : acc[t][r][i];
                 }
         }
@@ -1620,7 +1627,7 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
         if (q + 1 < q1) fetch(moe_first<UC>(next_users), turn ? next_slot : slot, turn ? 0 : l + 1);
         const bool more = turn && n + 2 < n_hit;
         const u32 of = moe_anew(lane), after = more ? a.table->hit[n + 2].slot[of] : kMoeNone;
-        const float after_weight = more ? a.table->hit[n + 2].weight[of] : 0.0f;
+        const float after_weight = more ? a.table->hit[n + 2].weight[NT == 1 ? of & 15 : of] : 0.0f;
         __builtin_amdgcn_sched_barrier(0);
         v4i w[R][2];
         float by[R][2];
@@ -1639,7 +1646,8 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
         }
         // The expert's tokens, as many as have columns of their own at a time: where that is all of them, their sums stay over the expert's lines.
         for (unsigned long long rest = users, first = moe_first<UC>(users);;) {
-            const unsigned long long here = moe_first<kTokens>(rest);
+            unsigned long long here = rest;
+            if (__builtin_popcountll(rest) > kTokens) here = moe_first<kTokens>(rest);
             unsigned long long some = moe_first<UC>(here), left = here ^ some;
             for (u32 column = 0;; column += PH * UC) {
                 if (some != first) { // (the values of the next line that are held are in LDS only after these)
@@ -1653,7 +1661,9 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
                 }
 #pragma unroll
                 for (int r = 0; r < R; r++) moe_anew(w[r][0]), moe_anew(w[r][1]);
-                const uint8_t *row = rows + moe_column<PH, UC>(c, (u32)__builtin_popcountll(some), wave * UC, NW * UC, column) + moe_at(lane);
+                u32 own = moe_column<PH, UC>(c, (u32)__builtin_popcountll(some), wave * UC, NW * UC, column);
+                if (kOwn) own = ((u32)some >> c & 1 ? wave * UC + (u32)__builtin_popcount((u32)some & ((1u << c) - 1)) : NW * UC) * kRow;
+                const uint8_t *row = rows + own + moe_at(lane);
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const v8h value = *reinterpret_cast<const v8h *>(row + 16 * i);
@@ -1677,8 +1687,8 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
         }
     };
     if (q0 < q1) {
-        slot = a.table->hit[n].slot[lane], weight = a.table->hit[n].weight[lane];
-        if (n + 1 < n_hit) next_slot = a.table->hit[n + 1].slot[lane], next_weight = a.table->hit[n + 1].weight[lane];
+        slot = a.table->hit[n].slot[lane], weight = a.table->hit[n].weight[NT == 1 ? c : lane];
+        if (n + 1 < n_hit) next_slot = a.table->hit[n + 1].slot[lane], next_weight = a.table->hit[n + 1].weight[NT == 1 ? c : lane];
         users = __ballot(slot != kMoeNone);
         fetch(moe_first<UC>(users), slot, l);
         __builtin_amdgcn_sched_barrier(0);
