@@ -930,8 +930,8 @@ hipError_t mx4_gemm(const Launch &L, const uint8_t *w, const uint8_t *ws, int n_
 // through rings in LDS, and bound both; codes become bf16 values exactly, a few instructions for eight, and the products run on the bf16 matrix instructions, the tokens' values in parts
 // that add up to them, x and h alike: one of bf16, two of f16, three of f32. (The instructions that take 4-bit codes would want x and h as codes too, or as 8-bit values, whose errors
 // a decode step would not have otherwise.)
-// On MI355X, us of each launch: 1 token, top 8 of 128, 2048 x 768 bf16 8.4 + 7.1; 16 tokens in f32 44 + 29 + 4.7, 205 MB of hit experts' weights; 64 tokens, 64 of 256 experts of 7168 x 2048 here,
-// bf16, 174 (5.7 TB/s) + 113 (4.4 TB/s).
+// On MI355X, us of each launch: 1 token, top 8 of 128, 2048 x 768 bf16 8.2 + 7.5; 16 tokens in f32 39 + 27 + 4.7 for 168 MB of some 66 hit experts' weights (a copy's rate: 32); 64 tokens, 41
+// of the 64 experts of 7168 x 2048 here hit, bf16, 174 (3.7 TB/s) + 97 (3.3 TB/s).
 
 // What the first launch leaves for the second: the experts that are hit, ascending, and for each and each token the slot that picked it, the first if
 // there are several, kMoeNone for none, and its weight, the sum over all of the token's slots of it.
@@ -1233,7 +1233,7 @@ constexpr int kMoeUpWaves = 4;
 
 // h of rows of up to 2048 values, two lines a wave at most: a workgroup goes over several tiles of sixteen rows of gate and as many of up, whose lines come through
 // a ring of S stages without a stop between the tiles; the tokens' values of a wave's lines stay in LDS. UC tokens a workgroup (an expert with more has several): LDS holds two
-// workgroups a unit with 4 of bf16 and f16, 2 of f32, and experts of a decode batch have fewer (16 tokens, top 8 of 128: one mostly, in f32 44 us; UC 4: 49).
+// workgroups a unit with 4 of bf16 and f16, 2 of f32, and experts of a decode batch mostly have fewer (16 tokens, top 8 of 128, f32: 39 us; without the products 31).
 template <int ET, int S, int UC>
 __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(2))) void k_mx4_moe_up_short(Mx4Moe a, u32 per) {
     constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, kRow = P * kMoePart, kLoads = 6; // loads of a stage: four of lines, two of scales
@@ -1369,7 +1369,8 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
 
 // h. T times sixteen rows of gate and as many of up, their lines dealt to the waves, each through S stages, of which all but one, or of two one, are on
 // their way while one is multiplied. A line's values of x come through LDS in parts, the next line's asked for in front of the weights: asked for in the matrix
-// instructions' form, each of sixteen requests a line would take the vector cache as long as a line of weights does.
+// instructions' form, each of sixteen requests a line would take the vector cache as long as a line of weights does. (64 tokens, 41 experts of 7168 x 2048 hit, bf16: 174 us, without
+// x 145; several tiles a workgroup instead of one 172.)
 template <int ET, int T, int S, int UC, int EU>
 __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(EU))) void k_mx4_moe_up(Mx4Moe a) {
     constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, R = 2 * T, kLoads = 3 * R, kRow = P * kMoePart; // loads of a stage: 2 R of lines, R of scales
@@ -1507,7 +1508,9 @@ __device__ __forceinline__ void moe_onto(const Mx4Moe &a, u32 token, u32 row, fl
 }
 // y. The lines of the experts that are hit, one expert's after another's, are dealt to the waves in stretches, each through two stages of 16 R rows; the
 // waves' sums, NT tiles of sixteen tokens, meet in LDS. A line's values of h come through LDS too, UC tokens' at a time and the next line's asked for in front of the
-// weights. gridDim.y workgroups share the lines: where they are several, a third launch adds their sums.
+// weights. The tokens of an expert stand side by side in a matrix instruction's columns, and their sums change to the tokens' own places when the expert's lines end: by
+// the tokens' places from the start a line would be multiplied for every tile of sixteen that has one of them (64 tokens, bf16: 113 us for 97). gridDim.y workgroups share the
+// lines: where they are several, a third launch adds their sums.
 template <int ET, int NW, int R, int UC, int NT>
 __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
     constexpr int PH = kMoeKept<ET>, NL = (PH + 1) / 2, CH = R == 1 ? 2 : 1; // requests of a token's values; chains of products
@@ -1755,6 +1758,8 @@ static hipError_t moe_down(const Launch &L, const Mx4Moe &a, u32 sharers) {
     hipLaunchKernelGGL((k_mx4_moe_join<ET>), dim3(((a.hidden + 3) / 4 * a.n_tokens + 255) / 256), dim3(256), 0, L.stream, a, sharers);
     return hipGetLastError();
 }
+// Up's lines stay with their values where a wave has two at most: 16 tokens in f32, rows of 2048, 46 us (a line at a time: 50), one token in bf16 8.2 (8.8). Down in 32 rows a workgroup where these fill the
+// card, alone or shared (64 tokens, 7168 rows, bf16: 16 waves 106, 8 waves 163; 16 tokens, 2048 rows, f32: four sharers 29 and 4.7 for their sums, of 16 rows a workgroup 33, unshared 42), else 16.
 template <int ET, int NT>
 static hipError_t moe_launch(const Launch &L, const Mx4Moe &a) {
     constexpr int P = kMoeParts<ET>;
