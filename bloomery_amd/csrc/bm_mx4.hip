@@ -312,28 +312,30 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_few(Mx4Args a) {
 }
 
 // A few rows from their floating values: k_mx4_few's product with the quantizer in front of it in every workgroup, while the first weights are on
-// their way. M (a power of two, at least the rows): the waves are dealt to the rows, 4 pieces of eight values a thread at most, four threads a
+// their way. M (a power of two, at least the rows): the waves are dealt to the rows, PC pieces of eight values a thread at most, four threads a
 // block. Codes and scales go to LDS; the first workgroup leaves them in memory too. One launch for two, whose cost it is: 1 x 768 x 2048 f32 3.9 us,
-// as much as k_mx4_few alone; for more than eight rows the values would cost each workgroup more than a launch.
-constexpr int kMx4FewX = 8, kMx4FewXWaves = 8; // rows at most
-constexpr u32 mx4_few_x_values(u32 M) { return 64 * kMx4FewXWaves * 8 * 4 / M; } // values a row may have
-template <int ET, int M, int R>
+// as much as k_mx4_few alone. What it costs more is every workgroup's reading of all rows: bf16, us,
+// 16 x 1024 against 4096 and 8192 rows of weights 4.3, 5.2 (two launches 7.2, 7.5), 16 x 2048 6.0, 6.8 (8.4), 32 x 1024 6.0, 6.8 (8.5), 1 x 32768 18.9, 33.5 (19.8, 38.3), f32 16 x 2048 6.5, 7.7 (8.4);
+// but twice the values in two turns 8.9, 9.7 (24 x 2048, two launches 8.0), and more than 8192 rows of weights, several rounds of workgroups, 8 x 2048 against 16000 9.7 (8.2).
+constexpr int kMx4FewX = 32, kMx4FewXWaves = 8; // rows at most
+constexpr u32 mx4_few_x_values(u32 M, u32 PC) { return 64 * kMx4FewXWaves * 8 * PC / M; } // values a row may have
+template <int ET, int M, int R, int PC>
 __global__ __launch_bounds__(64 * kMx4FewXWaves) void k_mx4_few_x(Mx4Args a, Mx4Rows qa) {
-    constexpr int NW = kMx4FewXWaves, T = 64 * NW / M, kPieces = 4, V = kElemPiece<ET>, P = 8 / V; // threads a row, pieces a thread, loads a piece
-    constexpr u32 kRow = mx4_few_x_values(M) / 2 + 16, kRowScales = mx4_few_x_values(M) / 32;      // a row's bytes in LDS, sixteen more for the banks
+    constexpr int NW = kMx4FewXWaves, T = 64 * NW / M, V = kElemPiece<ET>, P = 8 / V, C = M <= 16 ? 1 : 2;    // threads a row, loads a piece, columns' tiles
+    constexpr u32 kRow = mx4_few_x_values(M, PC) / 2 + 16, kRowScales = mx4_few_x_values(M, PC) / 32; // a row's bytes in LDS, sixteen more for the banks
     typedef Lines<2 * R> L;
     constexpr int kLoads = 3 * R;
     __shared__ __align__(16) uint8_t codes[M * kRow], marks[M * kRowScales];
     __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[NW * L::kStage], ring3[NW * L::kStage];
-    static_assert(R * 1024 <= L::kStage && R <= NW, "a wave's sums lie in its stage, one piece a thread");
+    static_assert(R * C * 1024 <= L::kStage && R * C <= NW, "a wave's sums lie in its stage, one piece a thread");
     const u32 tid = threadIdx.x, lane = tid & 63, wave = (u32)__builtin_amdgcn_readfirstlane(tid >> 6);
     const u32 lines = (a.kp + 127) / 128, r0 = blockIdx.x * (16 * R), mine = wave * L::kStage, blocks = a.kp / 16, at = 2 * (lane >> 4);
     // the rows' values, then the first weights
     const u32 row = tid / T, first = tid % T, pieces = a.kp / 4, whole = qa.k / 8;
     const size_t from = (size_t)min(row, qa.m - 1) * qa.ld; // rows past the last are the last once more, and not multiplied
-    uint4 x[kPieces][P];
+    uint4 x[PC][P];
 #pragma unroll
-    for (int i = 0; i < kPieces; i++)
+    for (int i = 0; i < PC; i++)
 #pragma unroll
         for (int p = 0; p < P; p++) x[i][p] = elem_piece<ET>(qa.x, from + 8 * min(first + i * T, whole - 1) + p * V);
     L src;
@@ -358,7 +360,7 @@ __global__ __launch_bounds__(64 * kMx4FewXWaves) void k_mx4_few_x(Mx4Args a, Mx4
     loads_landed<3 * kLoads>();
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < kPieces; i++) {
+    for (int i = 0; i < PC; i++) {
         const u32 c = first + i * T;
         if (c >= pieces) break; // (a block's four threads together)
         float v[8];
@@ -385,23 +387,33 @@ __global__ __launch_bounds__(64 * kMx4FewXWaves) void k_mx4_few_x(Mx4Args a, Mx4
         for (u32 b = blocks + first; b < a.ks; b += T) qa.scales[(size_t)row * a.ks + b] = 0;
     lds_meet();
 
-    v4f acc[R];
+    v4f acc[R][C];
 #pragma unroll
-    for (int r = 0; r < R; r++) acc[r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int c = 0; c < C; c++) acc[r][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     const u32 col = lane & 15;
     const auto step = [&](const uint8_t *stage, u32 (&s)[R], uint8_t *free, u32 (&next)[R], u32 l) {
         if (l + 2 * NW < lines) loads_landed<2 * kLoads>();
         else if (l + NW < lines) loads_landed<kLoads>();
         else loads_landed<0>();
-        v4i A[2][R], B[2];
-        u32 two[R], q = 0x7f7fu;
+        v4i A[2][R], B[2][C];
+        u32 two[R], q[C];
         const u32 block = 8 * l + at;
-        if (col < (u32)M && block < blocks) q = mx4_scales(mx4_two(marks + col * kRowScales + block), block, blocks);
+        const bool here = M >= 16 || col < (u32)M;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            q[c] = 0x7f7fu;
+            if (here && block < blocks) q[c] = mx4_scales(mx4_two(marks + (16 * c + col) * kRowScales + block), block, blocks);
+        }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const bool in = col < (u32)M && block + h < blocks;
-            const v4i b = *reinterpret_cast<const v4i *>(codes + (in ? col * kRow + 16 * (block + h) : 0u));
-            B[h] = in ? b : v4i{0, 0, 0, 0};
+            const bool in = here && block + h < blocks;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                const v4i b = *reinterpret_cast<const v4i *>(codes + (in ? (16 * c + col) * kRow + 16 * (block + h) : 0u));
+                B[h][c] = in ? b : v4i{0, 0, 0, 0};
+            }
 #pragma unroll
             for (int r = 0; r < R; r++) A[h][r] = mx4_of_line(stage + mine, lane, r, h);
         }
@@ -409,9 +421,13 @@ __global__ __launch_bounds__(64 * kMx4FewXWaves) void k_mx4_few_x(Mx4Args a, Mx4
         for (int r = 0; r < R; r++) two[r] = mx4_scales(s[r], block, blocks);
         if (l + 3 * NW < lines) ask(free, next, l + 3 * NW);
 #pragma unroll
-        for (int r = 0; r < R; r++) acc[r] = mx4_mfma<0>(A[0][r], B[0], acc[r], two[r], q);
+        for (int r = 0; r < R; r++)
 #pragma unroll
-        for (int r = 0; r < R; r++) acc[r] = mx4_mfma<1>(A[1][r], B[1], acc[r], two[r], q);
+            for (int c = 0; c < C; c++) acc[r][c] = mx4_mfma<0>(A[0][r], B[0][c], acc[r][c], two[r], q[c]);
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int c = 0; c < C; c++) acc[r][c] = mx4_mfma<1>(A[1][r], B[1][c], acc[r][c], two[r], q[c]);
     };
     for (u32 l = wave; l < lines;) {
         step(ring0, s0, ring3, s3, l);
@@ -423,15 +439,17 @@ __global__ __launch_bounds__(64 * kMx4FewXWaves) void k_mx4_few_x(Mx4Args a, Mx4
         step(ring3, s3, ring2, s2, l);
         l += NW;
     }
-    const u32 out = r0 + 16 * wave + 4 * (lane >> 4);
+    const u32 out = r0 + 16 * (wave / C) + 4 * (lane >> 4), j = 16 * (wave % C) + col;
     loads_landed<0>();
 #pragma unroll
-    for (int r = 0; r < R; r++) *reinterpret_cast<v4f *>(ring0 + mine + r * 1024 + 16 * lane) = acc[r];
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int c = 0; c < C; c++) *reinterpret_cast<v4f *>(ring0 + mine + (r * C + c) * 1024 + 16 * lane) = acc[r][c];
     __syncthreads();
-    if (wave >= R || col >= a.m || out >= a.rows) return;
+    if (wave >= R * C || j >= a.m || out >= a.rows) return;
     const v4f sum = mx4_join<NW, L>(ring0, wave, lane);
     const float y[4] = {sum[0], sum[1], sum[2], sum[3]};
-    run_store4(a, col, out, y);
+    run_store4(a, j, out, y);
 }
 
 // Many columns a matrix: BT columns x BR rows a workgroup, 128 bytes of k a step through two LDS buffers, where the loads put them themselves (16 bytes a
@@ -816,27 +834,33 @@ static hipError_t mx4_few_launch(const Launch &L, const Mx4Args &a, u32 entries)
     return hipGetLastError();
 }
 
-template <int ET, int M, int R>
+template <int ET, int M, int R, int PC>
 static void mx4_few_x_launch(const Launch &L, const Mx4Args &a, const Mx4Rows &q) {
-    hipLaunchKernelGGL((k_mx4_few_x<ET, M, R>), dim3((a.rows + 16 * R - 1) / (16 * R)), dim3(64 * kMx4FewXWaves), 0, L.stream, a, q);
+    hipLaunchKernelGGL((k_mx4_few_x<ET, M, R, PC>), dim3((a.rows + 16 * R - 1) / (16 * R)), dim3(64 * kMx4FewXWaves), 0, L.stream, a, q);
 }
 template <int ET, int M>
 static void mx4_few_x_by_rows(const Launch &L, const Mx4Args &a, const Mx4Rows &q) {
-    if ((a.rows + 15) / 16 > 256) mx4_few_x_launch<ET, M, 2>(L, a, q);
-    else mx4_few_x_launch<ET, M, 1>(L, a, q);
+    const bool two = (a.rows + 15) / 16 > 256;
+    if (2 * a.kp <= mx4_few_x_values(M, 4)) {
+        if (two) mx4_few_x_launch<ET, M, 2, 4>(L, a, q);
+        else mx4_few_x_launch<ET, M, 1, 4>(L, a, q);
+    } else if (two) mx4_few_x_launch<ET, M, 2, 8>(L, a, q);
+    else mx4_few_x_launch<ET, M, 1, 8>(L, a, q);
 }
 template <int ET>
 static void mx4_few_x_by_columns(const Launch &L, const Mx4Args &a, const Mx4Rows &q) {
     if (a.m == 1) mx4_few_x_by_rows<ET, 1>(L, a, q);
     else if (a.m == 2) mx4_few_x_by_rows<ET, 2>(L, a, q);
     else if (a.m <= 4) mx4_few_x_by_rows<ET, 4>(L, a, q);
-    else mx4_few_x_by_rows<ET, 8>(L, a, q);
+    else if (a.m <= 8) mx4_few_x_by_rows<ET, 8>(L, a, q);
+    else if (a.m <= 16) mx4_few_x_by_rows<ET, 16>(L, a, q);
+    else mx4_few_x_by_rows<ET, 32>(L, a, q);
 }
 
 hipError_t mx4_gemm_x(const Launch &L, const uint8_t *w, const uint8_t *ws, int rows, int k, const void *x, int x_et, int64_t ld_x, int m, uint8_t *codes,
                       uint8_t *scales, void *y, int et, int64_t ld) {
-    const u32 kp = (u32)mx4_row_bytes(k), ks = (u32)mx4_row_scales(k), M = m <= 1 ? 1 : m <= 2 ? 2 : m <= 4 ? 4 : 8;
-    if (m <= kMx4FewX && k >= 8 && 2 * kp <= mx4_few_x_values(M)) {
+    const u32 kp = (u32)mx4_row_bytes(k), ks = (u32)mx4_row_scales(k), M = m <= 1 ? 1 : m <= 2 ? 2 : m <= 4 ? 4 : m <= 8 ? 8 : m <= 16 ? 16 : 32;
+    if (m <= kMx4FewX && k >= 8 && 2 * kp <= mx4_few_x_values(M, 8) && rows <= 256 * 32) {
         const Mx4Args a = {w, ws, (u32)rows, kp, ks, codes, scales, (u32)m, nullptr, nullptr, 0, 0, (u32)m, 1, y, (size_t)ld, et, L.fault, L.layer};
         const Mx4Rows q = {x, nullptr, (size_t)ld_x, (u32)m, (u32)k, kp, ks, nullptr, codes, scales, L.rule, L.fault, L.layer};
         if (x_et == kElemF32) mx4_few_x_by_columns<kElemF32>(L, a, q);

@@ -204,7 +204,9 @@ def test_captured_and_replayed_while_another_context_works(gpu, m, rows, k):
 
 
 @pytest.mark.parametrize("dtype", (bm.F32, bm.F16, bm.BF16), ids=NAMES.get)
-@pytest.mark.parametrize("m,rows,k", ((1, 5000, 2048), (2, 5000, 8192), (3, 700, 4096), (4, 300, 4090), (8, 4500, 2048), (8, 64, 2049), (5, 64, 2049), (1, 40, 16384), (1, 40, 16390), (1, 7, 7)))
+@pytest.mark.parametrize("m,rows,k", ((1, 5000, 2048), (2, 5000, 8192), (3, 700, 4096), (4, 300, 4090), (8, 4500, 2048), (8, 64, 2049), (5, 64, 2049), (1, 40, 16384), (1, 40, 16390), (1, 7, 7),
+                                      (9, 300, 1024), (16, 8192, 2048), (16, 4500, 2041), (16, 100, 2049), (12, 64, 40), (17, 300, 1024), (32, 8192, 1019), (32, 64, 1025), (31, 5000, 520), (24, 33, 8),
+                                      (33, 64, 512), (8, 100, 4096), (8, 100, 4100), (4, 64, 8190), (3, 4200, 4097), (2, 40, 16384), (1, 40, 32768), (1, 40, 32770), (1, 8193, 100), (32, 8193, 512)))
 def test_few_rows_at_either_end_of_one_launch(gpu, dtype, m, rows, k):
     gen = torch.Generator(device="cuda")
     gen.manual_seed(m + k)
