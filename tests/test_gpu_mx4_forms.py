@@ -240,3 +240,76 @@ def test_a_value_that_is_not_finite_among_few_rows(gpu):
     assert torch.isnan(y[1]).all() and torch.isfinite(y[[0, 2]]).all()
     assert gpu.fault()[0] & 0xFF == bm.SITE_QUANT_COLUMN
     gpu.fault_clear()
+
+
+def needs_memory(gigabytes):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < gigabytes << 30:
+        pytest.skip(f"{gigabytes} GiB of the card's memory are not free")
+
+
+def test_the_most_rows_there_and_back(gpu):
+    """2^22 rows of 8192 values, a wave every 512 of them: 2^32 threads. Rows of zeros, some others spread among them; and back into the same rows."""
+    needs_memory(100)
+    m, k = 1 << 22, 8192
+    at = torch.tensor([0, 1, (1 << 20) - 1, 1 << 20, (1 << 21) + 7, 3 << 20, m - 2, m - 1])
+    torch.manual_seed(5)
+    some = torch.randn(at.numel(), k).bfloat16()
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    x[at.cuda()] = some.cuda()
+    codes, scales = torch.full((m, k // 2), 0x55, dtype=torch.uint8, device="cuda"), torch.full((m, k // 32), 0x55, dtype=torch.uint8, device="cuda")
+    q, b = mx.encode(some.double().numpy())
+    words, padded = mx.pack(q, b, k)
+    live = torch.tensor([m - 1], dtype=torch.int32, device="cuda")
+    try:
+        for n, word in ((m - 1, PTR(live)), (m, None)):
+            torch.cuda.synchronize()
+            gpu.enqueue_mx4_quantize(PTR(x), bm.BF16, m, k, PTR(codes), PTR(scales), live=word)
+            gpu.sync()
+            if n < m:
+                assert (codes[n:] == 0x55).all() and (scales[n:] == 0x55).all()
+            there = at[at < n]
+            assert np.array_equal(codes[there.cuda()].cpu().numpy(), words[:there.numel()]) and np.array_equal(scales[there.cuda()].cpu().numpy(), padded[:there.numel()])
+        gpu.enqueue_mx4_dequantize(PTR(codes), PTR(scales), m, k, PTR(x), bm.BF16)
+        gpu.sync()
+        assert np.array_equal(x[at.cuda()].double().cpu().numpy(), mx.decode(q, b, k))
+        for held in (codes, scales, x):
+            held[at.cuda()] = 0
+            for part in held.view(torch.int64).split(1 << 19):
+                assert not part.any().item()
+        clean(gpu)
+    finally:
+        del x, codes, scales, held
+        torch.cuda.empty_cache()
+
+
+def test_the_most_rows_an_expert(gpu):
+    """Experts of 2^22 rows each: more than 2^32 threads of tiles, counted by the most that the runs may make."""
+    needs_memory(110)
+    n, rows, k = 600, 1 << 22, 16
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(6)
+    w, ws = torch.empty(n * rows, 16, dtype=torch.uint8, device="cuda"), torch.full((n * rows, 16), 255, dtype=torch.uint8, device="cuda")
+    for part in w.split(1 << 28):
+        part.random_(0, 256, generator=gen)
+    for part in ws.split(1 << 28):
+        part[:, 0].random_(117, 126, generator=gen)
+    q = rows_of(gen, n, k, True)
+    # a slot an expert, but for one with none and its neighbour with two
+    start = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    start[8] = 7
+    y = torch.empty(n, rows, dtype=torch.bfloat16, device="cuda").fill_(float("nan"))
+    try:
+        torch.cuda.synchronize()
+        gpu.enqueue_mx4_gemm_experts(PTR(w), PTR(ws), n, rows, k, PTR(q[0]), PTR(q[1]), None, PTR(start), n, 0, PTR(y), bm.BF16)
+        gpu.sync()
+        x = values_of(*q, k)
+        for e in (0, 1, 6, 7, 8, 9, 300, n - 2, n - 1):
+            a, b = int(start[e]), int(start[e + 1])
+            for r in (slice(0, 5000), slice(rows - 5000, rows)):
+                assert_near(y[a:b, r], bm.BF16, x[a:b], values_of(w[e * rows:(e + 1) * rows][r], ws[e * rows:(e + 1) * rows][r], k), e)
+        assert torch.isfinite(y).all()
+        clean(gpu)
+    finally:
+        del w, ws, y, part
+        torch.cuda.empty_cache()

@@ -99,11 +99,11 @@ def assert_step(y, dtype, stack, x, sel, wts, resid):
 
 
 # (tokens, experts, top_k, hidden, ff). With top_k and hidden the number of workgroups that share down's lines goes from 1 to 8, by its lines and waves; hidden
-# decides the forms at 2048 and 4096; few experts have many tokens each, more than one workgroup takes of them (2 to 8) and more than a tile of 16.
+# decides the forms at 2048 and 4096; few experts have many tokens each, more than one workgroup takes of them (2 to 8) and more than a tile of 16; stacks past 4 GiB.
 SIZES = ((1, 128, 8, 2048, 768), (16, 128, 8, 2048, 768), (4, 64, 8, 1023, 1500), (16, 8, 1, 2048, 4096), (12, 40, 3, 2049, 2300), (5, 20, 8, 2600, 2048), (16, 64, 8, 4096, 1536),
          (16, 2, 2, 4096, 500), (2, 32, 4, 7168, 2048), (16, 24, 8, 8200, 300), (1, 300, 64, 512, 700), (16, 1024, 64, 64, 96), (64, 128, 8, 2048, 768), (64, 4, 4, 2048, 768),
          (64, 4, 2, 2100, 1100), (64, 1, 1, 2048, 4096), (64, 1, 1, 33, 20000), (40, 16, 8, 4500, 1100), (64, 2, 2, 4100, 1000), (64, 1024, 64, 96, 40), (64, 64, 64, 2080, 64),
-         (17, 1000, 64, 40, 33), (33, 8, 8, 256, 16384))
+         (17, 1000, 64, 40, 33), (33, 8, 8, 256, 16384), (2, 700, 8, 7168, 2048), (17, 2, 2, 33000, 300), (3, 2, 2, 300, 33000))
 
 
 @DTYPES
