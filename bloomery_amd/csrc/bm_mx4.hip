@@ -955,7 +955,7 @@ hipError_t mx4_gemm(const Launch &L, const uint8_t *w, const uint8_t *ws, int n_
 // that add up to them, x and h alike: one of bf16, two of f16, three of f32. (The instructions that take 4-bit codes would want x and h as codes too, or as 8-bit values, whose errors
 // a decode step would not have otherwise.)
 // On MI355X, us of each launch: 1 token, top 8 of 128, 2048 x 768 bf16 8.2 + 7.5; 16 tokens in f32 39 + 27 + 4.7 for 168 MB of some 66 hit experts' weights (a copy's rate: 32); 64 tokens, 41
-// of the 64 experts of 7168 x 2048 here hit, bf16, 174 (3.7 TB/s) + 97 (3.3 TB/s).
+// of the 64 experts of 7168 x 2048 here hit, bf16, 153 (4.2 TB/s) + 97 (3.3 TB/s).
 
 // What the first launch leaves for the second: the experts that are hit, ascending, and for each and each token the slot that picked it, the first if
 // there are several, kMoeNone for none, and its weight, the sum over all of the token's slots of it.
@@ -1520,6 +1520,128 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
     }
 }
 
+// The same of bf16 rows that lie on 16 bytes and end with a block: their lines and all scales go into LDS as the weights do, two stages of each, and are multiplied as they are. A stage is
+// read to registers as a whole and asked for again before it is multiplied, so that values as well as weights are two lines on their way; no load hangs on a condition, since the compiler waits
+// by the loads that it can count (of a line's values ASKS loads, two tokens each). Piece p of token c lies at place p ^ c of its line, for the banks. 64 tokens, 41 experts of 7168 x 2048 hit:
+// 153 us, 4.2 TB/s (through registers, a line ahead: 174).
+template <int UC>
+__global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(2))) void k_mx4_moe_up_direct(Mx4Moe a) {
+    constexpr int NW = kMoeUpWaves, kLoads = 6, kValues = UC * 512; // loads of a stage's weights; bytes of its values
+    typedef Lines<4> L;
+    static_assert(UC == 8, "a token's number turns the pieces of eight");
+    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], rows0[NW * kValues + 512], rows1[NW * kValues + 512]; // the last lines: zeros
+    __shared__ __align__(1024) uint8_t marks0[NW * 512], marks1[NW * 512];
+    __shared__ MoePicks picks;
+    __shared__ MoeColumns col;
+    extern __shared__ __align__(16) uint16_t sel[];
+    const u32 wave = (u32)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (threadIdx.x < 64) reinterpret_cast<uint4 *>((threadIdx.x < 32 ? rows0 : rows1) + NW * kValues)[threadIdx.x & 31] = make_uint4(0, 0, 0, 0);
+    moe_picks<64 * NW>(a, picks, sel, blockIdx.x == 0 && blockIdx.y == 0);
+    for (u32 n = blockIdx.y;; n += gridDim.y) { // (once, where no expert has more than one share)
+        u32 lane = threadIdx.x & 63;
+        __asm__ volatile("" : "+v"(lane)); // anew for each share: what follows from it does not wait in registers from one to the next
+        const u32 c = lane & 15;
+        MoeEntry entry;
+        const int kind = moe_entry<UC>(a, picks, sel, n, entry);
+        if (kind == 0) return;
+        if (kind == 1) continue;
+        const u32 columns = entry.columns, asks = (columns + 1) / 2; // of a line's values, two tokens each
+
+        const u32 kp = (a.hidden + 31) / 32 * 16, ks = (a.hidden + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage, at = 2 * (lane >> 4);
+        const u32 r0 = blockIdx.x * 16;
+        const size_t stack = (size_t)entry.expert * a.ff;
+        L src;
+        src.begin(lane);
+        const uint8_t *scales[2];
+#pragma unroll
+        for (u32 g = 0; g < 4; g++) // rows past the last are the last once more, and their values zeros
+            src.from[g] = (const int8_t *)(g < 2 ? a.wg : a.wu) + (stack + min(r0 + 8 * (g & 1) + (lane >> 3), a.ff - 1)) * kp;
+#pragma unroll
+        for (u32 g = 0; g < 2; g++) scales[g] = (g < 1 ? a.wgs : a.wus) + (stack + min(r0 + c, a.ff - 1)) * ks + (at & 4); // four blocks' at once, of which two are this lane's
+        moe_columns(entry, col);
+        __syncthreads();
+        const uint8_t *of[UC / 2]; // this lane's token of each ask
+#pragma unroll
+        for (int j = 0; j < UC / 2; j++) of[j] = (const uint8_t *)a.x + (size_t)col.token[min(2 * j + (lane >> 5), columns - 1)] * a.ld_x * 2;
+        const auto ask = [&](auto each, uint8_t *stage, uint8_t *rows, uint8_t *marks, u32 l) {
+            constexpr int ASKS = decltype(each)::value;
+#pragma unroll
+            for (int g = 0; g < 2; g++) __builtin_amdgcn_global_load_lds((lds_from *)(scales[g] + 8 * l), (lds_to *)(marks + wave * 512 + 256 * g), 4, 0, 0);
+            src.ask(stage + mine, l, kp);
+#pragma unroll
+            for (int j = 0; j < ASKS; j++) {
+                const u32 piece = (lane & 31) ^ (2 * j + (lane >> 5)); // behind the row's end its line's first: there, and met by zeros
+                __builtin_amdgcn_global_load_lds((lds_from *)(of[j] + 512 * l + (8 * l + piece / 4 < blocks ? 16 * piece : 0u)), (lds_to *)(rows + wave * kValues + 1024 * j), 16, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        v4f acc[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+        // kFull: two lines behind this one, the second to be asked for; kNext: one; kLast: none. (No load hangs on a condition: the compiler waits by what it can count.)
+        const auto step = [&](auto each, auto place, uint8_t *stage, uint8_t *rows, uint8_t *marks, u32 l) {
+            constexpr int ASKS = decltype(each)::value;
+            constexpr Mx4Steps STEP = decltype(place)::value;
+            loads_landed<STEP == kLast ? 0 : kLoads + ASKS>();
+            v4i w[2][2];
+            float by[2][2];
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                const u32 two = mx4_scales(*reinterpret_cast<const u32 *>(marks + wave * 512 + 256 * g + 4 * lane) >> 8 * (at & 2) & 0xffff, 8 * l + at, blocks);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const v4i codes = mx4_of_line(stage + mine, lane, g, h);
+                    w[g][h] = 8 * l + at + h < blocks ? codes : v4i{0, 0, 0, 0};
+                    by[g][h] = moe_scale(two, h);
+                }
+            }
+            const uint8_t *row = rows + (c < columns ? wave * kValues + 512 * c : (u32)(NW * kValues)) + 128 * (lane >> 4);
+            v8h value[8];
+#pragma unroll
+            for (u32 i = 0; i < 8; i++) value[i] = *reinterpret_cast<const v8h *>(row + 16 * (i ^ (c & 7)));
+            if (STEP == kFull) {
+                lds_read(); // the stage is in registers
+                ask(each, stage, rows, marks, l + 2 * NW);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int g = 0; g < 2; g++) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(moe_codes((u32)w[g][i / 4][i % 4], by[g][i / 4]), value[i], acc[g], 0, 0, 0);
+        };
+        const std::integral_constant<Mx4Steps, kFull> full;
+        const std::integral_constant<Mx4Steps, kNext> next;
+        const std::integral_constant<Mx4Steps, kLast> end;
+        const auto run = [&](auto each) {
+            ask(each, ring0, rows0, marks0, wave);
+            ask(each, ring1, rows1, marks1, wave + NW);
+            moe_weights(a, sel, entry);
+            u32 l = wave;
+            for (; l + 3 * NW < lines; l += 2 * NW) {
+                step(each, full, ring0, rows0, marks0, l);
+                step(each, full, ring1, rows1, marks1, l + NW);
+            }
+            if (l + 2 * NW < lines) {
+                step(each, full, ring0, rows0, marks0, l);
+                step(each, next, ring1, rows1, marks1, l + NW);
+                step(each, end, ring0, rows0, marks0, l + 2 * NW);
+            } else {
+                step(each, next, ring0, rows0, marks0, l);
+                step(each, end, ring1, rows1, marks1, l + NW);
+            }
+        };
+        static_assert(UC / 2 == 4, "as many asks");
+        if (asks == 1) run(std::integral_constant<int, 1>());
+        else if (asks == 2) run(std::integral_constant<int, 2>());
+        else if (asks == 3) run(std::integral_constant<int, 3>());
+        else run(std::integral_constant<int, 4>());
+        loads_landed<0>();
+#pragma unroll
+        for (int g = 0; g < 2; g++) *reinterpret_cast<v4f *>(ring0 + mine + g * 1024 + 16 * lane) = acc[g];
+        __syncthreads();
+        moe_leave<kElemBF16, NW, UC, true>(a, col, columns, r0, ring0, ring0 + 1024, L::kStage);
+        if (n + gridDim.y >= entry.n_shares) return;
+        __syncthreads();
+    }
+}
+
 // Four rows' sums of a token onto the residual.
 template <int ET>
 __device__ __forceinline__ void moe_onto(const Mx4Moe &a, u32 token, u32 row, float (&v)[4]) {
@@ -1788,6 +1910,9 @@ template <int ET, int NT>
 static hipError_t moe_launch(const Launch &L, const Mx4Moe &a) {
     constexpr int P = kMoeParts<ET>;
     if (a.hidden <= 256 * 2 * kMoeUpWaves) moe_up_short<ET, P == 1 ? 3 : 2, P == 3 ? 2 : 4>(L, a);
+    else if (P == 1 && a.hidden % 32 == 0 && a.ld_x % 8 == 0 && ((uintptr_t)a.x & 15) == 0)
+        hipLaunchKernelGGL((k_mx4_moe_up_direct<8>), dim3((a.ff + 15) / 16, moe_hits(a.n_tokens, a.top_k, a.n_experts)), dim3(64 * kMoeUpWaves),
+                           (a.n_tokens * a.top_k * 2 + 15) & ~15u, L.stream, a);
     else moe_up<ET, 1, 3, P == 1 ? 8 : 4, 2>(L, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;

@@ -103,7 +103,8 @@ def assert_step(y, dtype, stack, x, sel, wts, resid):
 SIZES = ((1, 128, 8, 2048, 768), (16, 128, 8, 2048, 768), (4, 64, 8, 1023, 1500), (16, 8, 1, 2048, 4096), (12, 40, 3, 2049, 2300), (5, 20, 8, 2600, 2048), (16, 64, 8, 4096, 1536),
          (16, 2, 2, 4096, 500), (2, 32, 4, 7168, 2048), (16, 24, 8, 8200, 300), (1, 300, 64, 512, 700), (16, 1024, 64, 64, 96), (64, 128, 8, 2048, 768), (64, 4, 4, 2048, 768),
          (64, 4, 2, 2100, 1100), (64, 1, 1, 2048, 4096), (64, 1, 1, 33, 20000), (40, 16, 8, 4500, 1100), (64, 2, 2, 4100, 1000), (64, 1024, 64, 96, 40), (64, 64, 64, 2080, 64),
-         (17, 1000, 64, 40, 33), (33, 8, 8, 256, 16384), (2, 700, 8, 7168, 2048), (17, 2, 2, 33000, 300), (3, 2, 2, 300, 33000))
+         (17, 1000, 64, 40, 33), (33, 8, 8, 256, 16384), (2, 700, 8, 7168, 2048), (17, 2, 2, 33000, 300), (3, 2, 2, 300, 33000),
+         (64, 4, 2, 4096, 300), (64, 2, 2, 2336, 100), (30, 8, 2, 3328, 40), (7, 5, 3, 2560, 33))
 
 
 @DTYPES
@@ -127,6 +128,23 @@ def test_the_step_where_its_work_is_divided(gpu, dtype, m, n, top_k, hidden, ff)
     step(gpu, stack, x, dtype, sel, wts, held, y=held)
     gpu.sync()
     assert torch.equal(y, held)
+    clean(gpu)
+
+
+@DTYPES
+@pytest.mark.parametrize("apart,shift", ((0, 0), (8, 0), (8, 8), (1, 0), (8, 1), (4, 2)))
+@pytest.mark.parametrize("hidden", (1024, 2080, 4096))
+def test_rows_on_every_kind_of_address(gpu, dtype, hidden, apart, shift):
+    m, n, top_k, ff = 20, 9, 3, 100
+    stack = Stack(3, n, hidden, ff)
+    held = torch.full((m * (hidden + apart) + shift,), float("nan"), dtype=TORCH[dtype], device="cuda")
+    x = held[shift:].view(m, hidden + apart)[:, :hidden]
+    x.copy_(stack.rows(m, dtype))
+    sel, wts = ids(picks(np.random.default_rng(4), m, n, top_k)), some_weights(stack.gen, m, top_k)
+    torch.cuda.synchronize()
+    y, _ = step(gpu, stack, x, dtype, sel, wts, None)
+    gpu.sync()
+    assert_step(y, dtype, stack, x, sel, wts, None)
     clean(gpu)
 
 
