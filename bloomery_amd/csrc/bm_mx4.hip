@@ -952,7 +952,8 @@ hipError_t mx4_gemm(const Launch &L, const uint8_t *w, const uint8_t *ws, int n_
 // Two launches, three where workgroups share down's lines. The first forms h: a workgroup some rows of gate and of up of an expert that is hit, for up to UC of the tokens that
 // picked it. The second forms y: a workgroup 16 R rows of down, for all tokens, over the experts that are hit. Weights are read once by each (once for UC tokens by the first), as lines
 // through rings in LDS, and bound both; codes become bf16 values exactly, a few instructions for eight, and the products run on the bf16 matrix instructions, the tokens' values in parts
-// that add up to them, x and h alike: one of bf16, two of f16, three of f32. (The instructions that take 4-bit codes would want x and h as codes too, or as 8-bit values, whose errors
+// that add up to them: x in one of bf16, two of f16, three of f32; h, which is f32 by then, in two parts, 16 bits of mantissa, where y has 8 or 11 (one part of bf16 would leave h the largest
+// error of the step: 64 tokens of 7168 x 2048 0.0020 from 64 bits, in two 0.0016, which is y's own rounding; the step 245.6 and 250.5 us), in three where y is f32. (The instructions that take 4-bit codes would want x and h as codes too, or as 8-bit values, whose errors
 // a decode step would not have otherwise.)
 // On MI355X, us of each launch: 1 token, top 8 of 128, 2048 x 768 bf16 8.2 + 7.5; 16 tokens in f32 39 + 27 + 4.7 for 168 MB of some 66 hit experts' weights (a copy's rate: 32); 64 tokens, 41
 // of the 64 experts of 7168 x 2048 here hit, bf16, 153 (4.2 TB/s) + 97 (3.3 TB/s).
@@ -1072,9 +1073,10 @@ __device__ __forceinline__ v8h moe_as_parts(uint4 p) {
     __builtin_memcpy(&r, &p, 16);
     return r;
 }
-// A value's first eight bits of mantissa.
+// A value's first eight bits of mantissa, of the next value towards zero: so that what they leave of v has v's sign and is not zero (an infinity leaves an infinity, and
+// a code that is one meets no zero but a zero's), and still has as few bits.
 __device__ __forceinline__ __bf16 moe_cut(float v) {
-    const uint16_t high = (uint16_t)(bm_f32_bits(v) >> 16);
+    const uint16_t high = (uint16_t)((bm_f32_bits(v) - (v != 0.0f ? 1u : 0u)) >> 16);
     __bf16 r;
     __builtin_memcpy(&r, &high, 2);
     return r;
@@ -1103,7 +1105,7 @@ __device__ __forceinline__ void moe_split(const float (&x)[8], v8h (&part)[P]) {
 template <int ET>
 constexpr int kMoeParts = ET == kElemBF16 ? 1 : ET == kElemF16 ? 2 : 3; // of an x
 template <int ET>
-constexpr int kMoeKept = kMoeParts<ET>; // of an h: as the type's own rows would hold it, at least
+constexpr int kMoeKept = ET == kElemF32 ? 3 : 2; // of an h: 16 bits of mantissa where y has fewer, f32's where it is f32
 
 // Eight neighbouring values of a row on their way, those behind its end zeros.
 template <int ET>
@@ -1660,9 +1662,8 @@ __device__ __forceinline__ void moe_onto(const Mx4Moe &a, u32 token, u32 row, fl
 template <int ET, int NW, int R, int UC, int NT>
 __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
     constexpr int PH = kMoeKept<ET>, NL = (PH + 1) / 2, CH = R == 1 ? 2 : 1; // requests of a token's values; chains of products
-    constexpr bool kOwn = NT == 1 && PH == 1;                                // a token's column is its number
-    constexpr int kGroups = 16 / (PH * UC), kTokens = kOwn ? 16 : kGroups * UC; // of UC tokens in an instruction's columns
-    constexpr int kLoads = 3 * R, kRow = PH * kMoePart;                          // loads of a stage
+    constexpr int kGroups = 16 / (PH * UC), kTokens = kGroups * UC;          // of UC tokens in an instruction's columns
+    constexpr int kLoads = 3 * R, kRow = PH * kMoePart;                      // loads of a stage
     typedef Lines<2 * R> L;
     __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage];
     __shared__ __align__(16) uint8_t rows[(NW * UC + 1) * kRow]; // the last: zeros
@@ -1759,9 +1760,9 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
                 for (int i = 0; i < 4; i++) {
                     const float mine = CH > 1 ? __fadd_rn(sum[r][0][i], sum[r][CH - 1][i]) : sum[r][0][i];
                     float v = mine;
-                    if (PH > 1) v = __fadd_rn(v, moe_behind<UC>(mine));
+                    v = __fadd_rn(v, moe_behind<UC>(mine));
                     if (PH > 2) v = __fadd_rn(v, moe_behind<2 * UC>(mine));
-                    if (!kOwn) v = __shfl(v, from);
+                    v = __shfl(v, from);
                     acc[t][r][i] = user ? __fmaf_rn(by, v, acc[t][r][i]) : acc[t][r][i];
                 }
         }
@@ -1810,9 +1811,7 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
                 }
 #pragma unroll
                 for (int r = 0; r < R; r++) moe_anew(w[r][0]), moe_anew(w[r][1]);
-                u32 own = moe_column<PH, UC>(c, (u32)__builtin_popcountll(some), wave * UC, NW * UC, column);
-                if (kOwn) own = ((u32)some >> c & 1 ? wave * UC + (u32)__builtin_popcount((u32)some & ((1u << c) - 1)) : NW * UC) * kRow;
-                const uint8_t *row = rows + own + moe_at(lane);
+                const uint8_t *row = rows + moe_column<PH, UC>(c, (u32)__builtin_popcountll(some), wave * UC, NW * UC, column) + moe_at(lane);
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const v8h value = *reinterpret_cast<const v8h *>(row + 16 * i);
@@ -1905,7 +1904,8 @@ static hipError_t moe_down(const Launch &L, const Mx4Moe &a, u32 sharers) {
     return hipGetLastError();
 }
 // Up's lines stay with their values where a wave has two at most: 16 tokens in f32, rows of 2048, 46 us (a line at a time: 50), one token in bf16 8.2 (8.8). Down in 32 rows a workgroup where these fill the
-// card, alone or shared (64 tokens, 7168 rows, bf16: 16 waves 106, 8 waves 163; 16 tokens, 2048 rows, f32: four sharers 29 and 4.7 for their sums, of 16 rows a workgroup 33, unshared 42), else 16.
+// card, alone or shared (16 tokens, 2048 rows, f32: four sharers 29 and 4.7 for their sums, of 16 rows a workgroup 33, unshared 42), else 16. The whole step of 64 tokens, 7168 rows, bf16: 250.5 with 12
+// waves, 272 with 14 that have the values of three tokens, 284 with 8; f16 302, 324, 336.
 template <int ET, int NT>
 static hipError_t moe_launch(const Launch &L, const Mx4Moe &a) {
     constexpr int P = kMoeParts<ET>;
@@ -1916,7 +1916,7 @@ static hipError_t moe_launch(const Launch &L, const Mx4Moe &a) {
     else moe_up<ET, 1, 3, P == 1 ? 8 : 4, 2>(L, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    constexpr int NW = P == 1 ? 16 : 8, UC = P == 1 ? 3 : 4;
+    constexpr int NW = kMoeKept<ET> == 3 ? 8 : 12, UC = 4; // what LDS holds: their lines, and the values of UC tokens each
     const u32 items = moe_hits(a.n_tokens, a.top_k, a.n_experts) * ((a.ff + 255) / 256);
     const u32 sharers = std::min(moe_sharers(a.top_k, a.hidden), items / (4 * NW));
     if (sharers > 1) return moe_down<ET, NW, 2, UC, NT>(L, a, sharers);

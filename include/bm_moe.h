@@ -584,7 +584,7 @@ int bm_mx4_gemm_experts(bm_ctx *ctx, const uint8_t *w_dev, const uint8_t *w_scal
 /* The experts' whole step for a few tokens (bm_moe_decode in this form; n_tokens 1 .. 64, top_k 1 .. 64, 1 .. 1024 experts), whose values stay
  * in floating point: for token t, slot s of its top_k, expert e = sel_dev[t * top_k + s]: g = wg[e] x[t], u = wu[e] x[t] (ff rows of hidden values each),
  * h = the rule's value of (g, u), and y[t] = resid[t] + the sum over s of w_dev[t * top_k + s] * (wd[e] h) (hidden rows of ff values). Products and
- * sums are f32, in an order that follows from sizes and picks alone, h is kept as precisely as elem_type at least (f32: in f32), and y is rounded once to
+ * sums are f32, in an order that follows from sizes and picks alone, h is kept in 16 bits of mantissa (f32: in f32), and y is rounded once to
  * elem_type, which x_dev, resid_dev (NULL: none) and y_dev share; y_dev may be resid_dev. An id of BM_HOST_SLOT is skipped; any other at or past n_experts raises
  * BM_SITE_EXPERT_ID and adds nothing, whatever its weight; an expert may stand at several slots of a token, whose weights are added first. Codes count as f32 values:
  * one past f32's range (a scale byte of 253 or 254) as an infinity, behind the k-th value too. What is not finite in an expert or a token stays with the tokens that
