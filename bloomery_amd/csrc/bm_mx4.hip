@@ -1073,10 +1073,12 @@ __device__ __forceinline__ v8h moe_as_parts(uint4 p) {
     __builtin_memcpy(&r, &p, 16);
     return r;
 }
-// A value's first eight bits of mantissa, of the next value towards zero: so that what they leave of v has v's sign and is not zero (an infinity leaves an infinity, and
-// a code that is one meets no zero but a zero's), and still has as few bits.
+// The bits of a value's first part, its first eight bits of mantissa, in their upper half: of the next value towards zero, so that what the part leaves of v has v's sign and is not
+// zero. An infinity so leaves an infinity, and a code that is one meets no zero but a zero's (and that of a part below bf16's smallest number, of values below 2^-109). What is
+// left has no more bits than behind v's own: where v ends with them, the whole of its last one.
+__device__ __forceinline__ u32 moe_first_part(float v) { return bm_f32_bits(v) - (v != 0.0f ? 1u : 0u); }
 __device__ __forceinline__ __bf16 moe_cut(float v) {
-    const uint16_t high = (uint16_t)((bm_f32_bits(v) - (v != 0.0f ? 1u : 0u)) >> 16);
+    const uint16_t high = (uint16_t)(moe_first_part(v) >> 16);
     __bf16 r;
     __builtin_memcpy(&r, &high, 2);
     return r;
@@ -1094,12 +1096,14 @@ __device__ __forceinline__ void moe_split(const float (&x)[8], v8h (&part)[P]) {
             for (int j = 0; j < 8; j++) part[p][j] = (__bf16)rest[j];
             break;
         }
-        u32 w[4];
+        u32 first[8], w[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = __builtin_amdgcn_perm(bm_f32_bits(rest[2 * j + 1]), bm_f32_bits(rest[2 * j]), 0x07060302u);
+        for (int j = 0; j < 8; j++) first[j] = moe_first_part(rest[j]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = __builtin_amdgcn_perm(first[2 * j + 1], first[2 * j], 0x07060302u);
         part[p] = moe_as_parts(make_uint4(w[0], w[1], w[2], w[3]));
 #pragma unroll
-        for (int j = 0; j < 8; j++) rest[j] = __fsub_rn(rest[j], bm_bits_f32(bm_f32_bits(rest[j]) & 0xffff0000u));
+        for (int j = 0; j < 8; j++) rest[j] = __fsub_rn(rest[j], bm_bits_f32(first[j] & 0xffff0000u));
     }
 }
 template <int ET>

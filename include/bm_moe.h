@@ -587,7 +587,7 @@ int bm_mx4_gemm_experts(bm_ctx *ctx, const uint8_t *w_dev, const uint8_t *w_scal
  * sums are f32, in an order that follows from sizes and picks alone, h is kept in 16 bits of mantissa (f32: in f32), and y is rounded once to
  * elem_type, which x_dev, resid_dev (NULL: none) and y_dev share; y_dev may be resid_dev. An id of BM_HOST_SLOT is skipped; any other at or past n_experts raises
  * BM_SITE_EXPERT_ID and adds nothing, whatever its weight; an expert may stand at several slots of a token, whose weights are added first. Codes count as f32 values:
- * one past f32's range (a scale byte of 253 or 254) as an infinity, behind the k-th value too. What is not finite in an expert or a token stays with the tokens that
+ * one past f32's range (a scale byte of 253 or 254) as an infinity, behind the k-th value too (against a value of x or h below 2^-109 it may give NaN). What is not finite in an expert or a token stays with the tokens that
  * picked that expert, and with that token. rule NULL: the context's.
  * work_dev: bm_mx4_moe_work(..) bytes of scratch, 16-byte aligned, that holds nothing between calls: at most n_tokens * top_k * (8 * ff + 8 * hidden + 1024) + 65536.
  * Calls that may run at the same time need one each. */

@@ -103,3 +103,46 @@ def test_an_infinite_h_stays_infinite(gpu, dtype, m, hidden):
     y = run(gpu, stack, rows(x, dtype), dtype, np.zeros(m)).double().cpu().numpy()
     assert (y[::2] == np.inf * sign).all() and (y[1::2] == 0).all()
     clean(gpu)
+
+
+@DTYPES
+@pytest.mark.parametrize("m,hidden", SIZES)
+def test_an_infinite_value_of_a_token(gpu, dtype, m, hidden):
+    """At the row's ends and between them, alone and under either sign: the token's sums are infinite, the others' what they are without it."""
+    rng, ff = np.random.default_rng(hidden), 40
+    gate, up, down, sign = signed(rng, hidden, ff)
+    for minus in (False, True):
+        if minus:
+            gate[:], up[:] = MINUS_ONE, MINUS_ONE
+        stack = Given(gate, up, down)
+        x = np.where(minus, -1.0, 1.0) * rng.integers(1, 9, (m, hidden)) / 2.0 ** 14
+        before = run(gpu, stack, rows(x, dtype), dtype, np.zeros(m))
+        assert torch.isfinite(before).all()
+        for at in (0, 5, hidden // 2, hidden - 1):
+            z = x.copy()
+            z[1, at] *= np.inf
+            after = run(gpu, stack, rows(z, dtype), dtype, np.zeros(m))
+            assert (after[1].double().cpu().numpy() == np.inf * sign).all(), at
+            rest = torch.arange(m) != 1
+            assert torch.equal(before[rest], after[rest]), at
+    clean(gpu)
+
+
+@DTYPES
+@pytest.mark.parametrize("byte", (253, 254))
+@pytest.mark.parametrize("name", ("gate", "up"))
+@pytest.mark.parametrize("m,hidden", SIZES)
+def test_a_code_past_f32s_range_is_an_infinity(gpu, dtype, name, byte, m, hidden):
+    """Against values that a first part holds whole as well as others."""
+    rng, ff = np.random.default_rng(hidden), 72
+    gate, up, down, sign = signed(rng, hidden, ff)
+    row = {"gate": gate, "up": up}[name][0, 3]
+    row[32:64] = 0
+    row[40] = 7
+    x = rng.choice([1.0, 1.5, 1.0 + 2.0 ** -7, 1.0 + 2.0 ** -10, 1.0 + 2.0 ** -23], (m, hidden)) / 2.0 ** 13  # (f16: ordinary numbers)
+    stack = Given(gate, up, down)
+    assert torch.isfinite(run(gpu, stack, rows(x, dtype), dtype, np.zeros(m))).all()
+    stack.dev[name][1][3, 1] = byte
+    y = run(gpu, stack, rows(x, dtype), dtype, np.zeros(m)).double().cpu().numpy()
+    assert (y == np.inf * sign).all()
+    clean(gpu)
