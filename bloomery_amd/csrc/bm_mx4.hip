@@ -1530,6 +1530,7 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
 // read to registers as a whole and asked for again before it is multiplied, so that values as well as weights are two lines on their way; no load hangs on a condition, since the compiler waits
 // by the loads that it can count (of a line's values ASKS loads, two tokens each). Piece p of token c lies at place p ^ c of its line, for the banks. 64 tokens, 41 experts of 7168 x 2048 hit:
 // 153 us, 4.2 TB/s (through registers, a line ahead: 174).
+__device__ const uint4 moe_zeros[1] = {};
 template <int UC>
 __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(2))) void k_mx4_moe_up_direct(Mx4Moe a) {
     constexpr int NW = kMoeUpWaves, kLoads = 6, kValues = UC * 512; // loads of a stage's weights; bytes of its values
@@ -1576,8 +1577,9 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
             src.ask(stage + mine, l, kp);
 #pragma unroll
             for (int j = 0; j < ASKS; j++) {
-                const u32 piece = (lane & 31) ^ (2 * j + (lane >> 5)); // behind the row's end its line's first: there, and met by zeros
-                __builtin_amdgcn_global_load_lds((lds_from *)(of[j] + 512 * l + (8 * l + piece / 4 < blocks ? 16 * piece : 0u)), (lds_to *)(rows + wave * kValues + 1024 * j), 16, 0, 0);
+                const u32 piece = (lane & 31) ^ (2 * j + (lane >> 5)); // behind the row's end zeros: the codes there are the line's first once more, under the scale 1
+                const uint8_t *const from = 8 * l + piece / 4 < blocks ? of[j] + (512 * l + 16 * piece) : (const uint8_t *)moe_zeros;
+                __builtin_amdgcn_global_load_lds((lds_from *)from, (lds_to *)(rows + wave * kValues + 1024 * j), 16, 0, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
         };
@@ -1594,8 +1596,7 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
                 const u32 two = mx4_scales(*reinterpret_cast<const u32 *>(marks + wave * 512 + 256 * g + 4 * lane) >> 8 * (at & 2) & 0xffff, 8 * l + at, blocks);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const v4i codes = mx4_of_line(stage + mine, lane, g, h);
-                    w[g][h] = 8 * l + at + h < blocks ? codes : v4i{0, 0, 0, 0};
+                    w[g][h] = mx4_of_line(stage + mine, lane, g, h);
                     by[g][h] = moe_scale(two, h);
                 }
             }

@@ -129,6 +129,22 @@ def test_an_infinite_value_of_a_token(gpu, dtype, m, hidden):
 
 
 @DTYPES
+@pytest.mark.parametrize("m,hidden", [s for s in SIZES if s[1] > 2048])
+def test_an_infinite_value_where_the_last_line_begins(gpu, dtype, m, hidden):
+    """Whatever a kernel reads in the place of what is behind a row's end, it counts for nothing."""
+    rng, ff = np.random.default_rng(hidden), 40
+    gate, up, down, sign = signed(rng, hidden, ff)
+    stack = Given(gate, up, down)
+    x = rng.integers(1, 9, (m, hidden)) / 2.0 ** 14
+    for at in range(256 * ((hidden - 1) // 256), hidden, 7):
+        z = x.copy()
+        z[1, at] = np.inf
+        y = run(gpu, stack, rows(z, dtype), dtype, np.zeros(m)).double().cpu().numpy()
+        assert (y[1] == np.inf * sign).all() and np.isfinite(np.delete(y, 1, 0)).all(), at
+    clean(gpu)
+
+
+@DTYPES
 @pytest.mark.parametrize("byte", (253, 254))
 @pytest.mark.parametrize("name", ("gate", "up"))
 @pytest.mark.parametrize("m,hidden", SIZES)
