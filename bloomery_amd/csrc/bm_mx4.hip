@@ -1804,6 +1804,7 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
             unsigned long long here = rest;
             if (__builtin_popcountll(rest) > kTokens) here = moe_first<kTokens>(rest);
             unsigned long long some = moe_first<UC>(here), left = here ^ some;
+            const bool groups = left != 0;
             for (u32 column = 0;; column += PH * UC) {
                 if (some != first) { // (the values of the next line that are held are in LDS only after these)
                     uint4 keep[UC * NL];
@@ -1817,11 +1818,25 @@ __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
 #pragma unroll
                 for (int r = 0; r < R; r++) moe_anew(w[r][0]), moe_anew(w[r][1]);
                 const uint8_t *row = rows + moe_column<PH, UC>(c, (u32)__builtin_popcountll(some), wave * UC, NW * UC, column) + moe_at(lane);
+                v4f others[R][CH]; // what the other groups' columns have: an infinite code would make NaN of the zeros that stand there now
+                if constexpr (kGroups > 1) {
+#pragma unroll
+                    for (int r = 0; r < R; r++)
+#pragma unroll
+                        for (int i = 0; i < CH; i++) others[r][i] = sum[r][i];
+                }
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const v8h value = *reinterpret_cast<const v8h *>(row + 16 * i);
 #pragma unroll
                     for (int r = 0; r < R; r++) sum[r][i % CH] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(moe_codes((u32)w[r][i / 4][i % 4], by[r][i / 4]), value, sum[r][i % CH], 0, 0, 0);
+                }
+                if constexpr (kGroups > 1) {
+                    if (groups)
+#pragma unroll
+                        for (int r = 0; r < R; r++)
+#pragma unroll
+                            for (int i = 0; i < CH; i++) sum[r][i] = c - column < (u32)(PH * UC) ? sum[r][i] : others[r][i];
                 }
                 if (!left) break;
                 some = moe_first<UC>(left);

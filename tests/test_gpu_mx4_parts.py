@@ -162,3 +162,27 @@ def test_a_code_past_f32s_range_is_an_infinity(gpu, dtype, name, byte, m, hidden
     y = run(gpu, stack, rows(x, dtype), dtype, np.zeros(m)).double().cpu().numpy()
     assert (y == np.inf * sign).all()
     clean(gpu)
+
+
+# experts with up to four tokens, up to eight (two groups side by side in a matrix instruction's columns), and more; several lines of down
+@DTYPES
+@pytest.mark.parametrize("byte", (253, 254))
+@pytest.mark.parametrize("m,hidden,ff", ((3, 64, 72), (7, 64, 72), (8, 4096, 300), (16, 300, 600), (20, 2056, 72), (40, 4096, 600), (64, 512, 2048)))
+def test_a_code_of_down_past_f32s_range_is_an_infinity(gpu, dtype, byte, m, hidden, ff):
+    """Its row alone is infinite, for every token, by the code's sign."""
+    rng = np.random.default_rng(hidden)
+    gate, up, down, _ = signed(rng, hidden, ff)
+    for row, code in ((5, 7), (6, 15)):
+        down[0, row, 32:64] = 0
+        down[0, row, 40] = code
+    x = rng.choice([1.0, 1.5, 1.0 + 2.0 ** -7, 1.0 + 2.0 ** -10, 1.0 + 2.0 ** -23], (m, hidden)) / 2.0 ** 13  # (f16: ordinary numbers)
+    stack = Given(gate, up, down)
+    before = run(gpu, stack, rows(x, dtype), dtype, np.zeros(m))
+    assert torch.isfinite(before).all()
+    stack.dev["down"][1][5:7, 1] = byte
+    after = run(gpu, stack, rows(x, dtype), dtype, np.zeros(m))
+    assert (after[:, 5] == np.inf).all() and (after[:, 6] == -np.inf).all()
+    rest = torch.ones(hidden, dtype=torch.bool, device="cuda")
+    rest[5:7] = False
+    assert torch.equal(before[:, rest], after[:, rest])
+    clean(gpu)
