@@ -1230,8 +1230,8 @@ __device__ __forceinline__ void moe_weights(const Mx4Moe &a, const uint16_t *sel
     a.table->hit[e.rank].weight[token] = by;
 }
 // Sixteen rows of h from r0 on, of as many columns as 256 threads have: a thread a value, row threadIdx.x % 16, column threadIdx.x / 16. gate, up: the first of
-// the waves' sums, `stride` bytes apart. ONE: the rows may end in the first half of a block, whose other half becomes zeros.
-template <int ET, int NW, int UC, bool ONE>
+// the waves' sums, `stride` bytes apart. Where the rows end in the first half of a block its other half becomes zeros.
+template <int ET, int NW, int UC>
 __device__ __forceinline__ void moe_leave(const Mx4Moe &a, const MoeColumns &col, u32 columns, u32 r0, const uint8_t *gate, const uint8_t *up, u32 stride) {
     constexpr int PH = kMoeKept<ET>;
     static_assert(64 * NW == 256, "sixteen rows by sixteen columns");
@@ -1256,7 +1256,7 @@ __device__ __forceinline__ void moe_leave(const Mx4Moe &a, const MoeColumns &col
         const __bf16 part = p == PH - 1 ? (__bf16)v : moe_cut(v);
         v = __fsub_rn(v, (float)part);
         to[(size_t)p * ffp] = part;
-        if (ONE && r0 + 16 >= a.ff && r0 + 16 < ffp) to[(size_t)p * ffp + 16] = (__bf16)0.0f;
+        if (r0 + 16 >= a.ff && r0 + 16 < ffp) to[(size_t)p * ffp + 16] = (__bf16)0.0f;
     }
 }
 constexpr int kMoeUpWaves = 4;
@@ -1368,7 +1368,7 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
             for (int g = 0; g < 2; g++) *reinterpret_cast<v4f *>(sums + wave * 2048 + g * 1024 + 16 * lane) = each ? acc[g] : v4f{0.0f, 0.0f, 0.0f, 0.0f};
             lds_meet();
-            moe_leave<ET, NW, UC, true>(a, col, columns, 16 * (tile0 + tile), sums, sums + 1024, 2048);
+            moe_leave<ET, NW, UC>(a, col, columns, 16 * (tile0 + tile), sums, sums + 1024, 2048);
             lds_meet();
             tile++;
         };
@@ -1397,15 +1397,15 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
     }
 }
 
-// h. T times sixteen rows of gate and as many of up, their lines dealt to the waves, each through S stages, of which all but one, or of two one, are on
+// h. Sixteen rows of gate and as many of up, their lines dealt to the waves, each through three stages, of which two are on
 // their way while one is multiplied. A line's values of x come through LDS in parts, the next line's asked for in front of the weights: asked for in the matrix
 // instructions' form, each of sixteen requests a line would take the vector cache as long as a line of weights does. (64 tokens, 41 experts of 7168 x 2048 hit, bf16: 174 us, without
 // x 145; several tiles a workgroup instead of one 172.)
-template <int ET, int T, int S, int UC, int EU>
-__global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(EU))) void k_mx4_moe_up(Mx4Moe a) {
-    constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, R = 2 * T, kLoads = 3 * R, kRow = P * kMoePart; // loads of a stage: 2 R of lines, R of scales
-    typedef Lines<2 * R> L;
-    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[S > 2 ? NW * L::kStage : 16];
+template <int ET, int UC>
+__global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(2))) void k_mx4_moe_up(Mx4Moe a) {
+    constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, kLoads = 6, kRow = P * kMoePart; // loads of a stage: four of lines, two of scales
+    typedef Lines<4> L;
+    __shared__ __align__(1024) uint8_t ring0[NW * L::kStage], ring1[NW * L::kStage], ring2[NW * L::kStage];
     __shared__ __align__(16) uint8_t rows[(NW * UC + 1) * kRow]; // the last: zeros
     __shared__ MoePicks picks;
     __shared__ MoeColumns col;
@@ -1424,20 +1424,20 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
         const u32 expert = entry.expert, columns = entry.columns;
 
         const u32 kp = (a.hidden + 31) / 32 * 16, ks = (a.hidden + 511) / 512 * 16, lines = (kp + 127) / 128, blocks = kp / 16, mine = wave * L::kStage, at = 2 * (lane >> 4);
-        const u32 r0 = blockIdx.x * (16 * T);
+        const u32 r0 = blockIdx.x * 16;
         L src;
         src.begin(lane);
         const size_t stack = (size_t)expert * a.ff;
-        const uint8_t *scales[R];
+        const uint8_t *scales[2];
 #pragma unroll
-        for (u32 g = 0; g < 2 * R; g++) // rows past the last are the last once more, and their values zeros
-            src.from[g] = (const int8_t *)(g < R ? a.wg : a.wu) + (stack + min(r0 + 8 * (g % R) + (lane >> 3), a.ff - 1)) * kp;
+        for (u32 g = 0; g < 4; g++) // rows past the last are the last once more, and their values zeros
+            src.from[g] = (const int8_t *)(g < 2 ? a.wg : a.wu) + (stack + min(r0 + 8 * (g & 1) + (lane >> 3), a.ff - 1)) * kp;
 #pragma unroll
-        for (u32 g = 0; g < R; g++) scales[g] = (g < T ? a.wgs : a.wus) + (stack + min(r0 + 16 * (g % T) + c, a.ff - 1)) * ks + at;
-        u32 s0[R], s1[R], s2[R];
-        const auto ask = [&](uint8_t *stage, u32 (&s)[R], u32 l) {
+        for (u32 g = 0; g < 2; g++) scales[g] = (g < 1 ? a.wgs : a.wus) + (stack + min(r0 + c, a.ff - 1)) * ks + at;
+        u32 s0[2], s1[2], s2[2];
+        const auto ask = [&](uint8_t *stage, u32 (&s)[2], u32 l) {
 #pragma unroll
-            for (int g = 0; g < R; g++) s[g] = mx4_two(scales[g] + 8 * l);
+            for (int g = 0; g < 2; g++) s[g] = mx4_two(scales[g] + 8 * l);
             __builtin_amdgcn_sched_barrier(0);
             src.ask(stage + mine, l, kp);
             __builtin_amdgcn_sched_barrier(0);
@@ -1471,20 +1471,18 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
         if (wave < lines) ask(ring0, s0, wave);
         if (wave + NW < lines) ask(ring1, s1, wave + NW);
         moe_weights(a, sel, entry);
-        v4f acc[R];
-#pragma unroll
-        for (int g = 0; g < R; g++) acc[g] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        const auto step = [&](uint8_t *stage, u32 (&s)[R], uint8_t *free, u32 (&next)[R], u32 l) {
+        v4f acc[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+        const auto step = [&](const uint8_t *stage, u32 (&s)[2], uint8_t *free, u32 (&next)[2], u32 l) {
             if (l + NW < lines) loads_landed<kLoads>(); // the next stage may be on its way; this line's values of x are older than it
             else loads_landed<0>();
             put();
             if (l + NW < lines) fetch(l + NW);
             __builtin_amdgcn_sched_barrier(0);
-            if (S > 2 && l + 2 * NW < lines) ask(free, next, l + 2 * NW);
-            v4i w[R][2];
-            float by[R][2];
+            if (l + 2 * NW < lines) ask(free, next, l + 2 * NW);
+            v4i w[2][2];
+            float by[2][2];
 #pragma unroll
-            for (int g = 0; g < R; g++) {
+            for (int g = 0; g < 2; g++) {
                 const u32 two = mx4_scales(s[g], 8 * l + at, blocks);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
@@ -1492,16 +1490,12 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
                     by[g][h] = moe_scale(two, h);
                 }
             }
-            if (S == 2 && l + 2 * NW < lines) {
-                lds_read(); // the stage is in registers
-                ask(stage, s, l + 2 * NW);
-            }
             const uint8_t *row = rows + moe_column<P, UC>(c, columns, wave * UC, NW * UC) + moe_at(lane);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const v8h value = *reinterpret_cast<const v8h *>(row + 16 * i);
 #pragma unroll
-                for (int g = 0; g < R; g++) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(moe_codes((u32)w[g][i / 4][i % 4], by[g][i / 4]), value, acc[g], 0, 0, 0);
+                for (int g = 0; g < 2; g++) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(moe_codes((u32)w[g][i / 4][i % 4], by[g][i / 4]), value, acc[g], 0, 0, 0);
             }
         };
         for (u32 l = wave; l < lines;) {
@@ -1509,18 +1503,14 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
             if ((l += NW) >= lines) break;
             step(ring1, s1, ring0, s0, l);
             if ((l += NW) >= lines) break;
-            if (S > 2) {
-                step(ring2, s2, ring1, s1, l);
-                l += NW;
-            }
+            step(ring2, s2, ring1, s1, l);
+            l += NW;
         }
         loads_landed<0>();
 #pragma unroll
-        for (int g = 0; g < R; g++) *reinterpret_cast<v4f *>(ring0 + mine + g * 1024 + 16 * lane) = acc[g];
+        for (int g = 0; g < 2; g++) *reinterpret_cast<v4f *>(ring0 + mine + g * 1024 + 16 * lane) = acc[g];
         __syncthreads();
-#pragma unroll 1
-        for (int t = 0; t < T; t++)
-            moe_leave<ET, NW, UC, T == 1>(a, col, columns, r0 + 16 * t, ring0 + t * 1024, ring0 + (T + t) * 1024, L::kStage);
+        moe_leave<ET, NW, UC>(a, col, columns, r0, ring0, ring0 + 1024, L::kStage);
         if (n + gridDim.y >= entry.n_shares) return;
         __syncthreads();
     }
@@ -1643,7 +1633,7 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
         for (int g = 0; g < 2; g++) *reinterpret_cast<v4f *>(ring0 + mine + g * 1024 + 16 * lane) = acc[g];
         __syncthreads();
-        moe_leave<kElemBF16, NW, UC, true>(a, col, columns, r0, ring0, ring0 + 1024, L::kStage);
+        moe_leave<kElemBF16, NW, UC>(a, col, columns, r0, ring0, ring0 + 1024, L::kStage);
         if (n + gridDim.y >= entry.n_shares) return;
         __syncthreads();
     }
@@ -1903,9 +1893,9 @@ __global__ __launch_bounds__(256) void k_mx4_moe_join(Mx4Moe a, u32 n) {
 }
 
 static u32 moe_hits(int n_tokens, int top_k, int n_experts) { return (u32)std::min(n_tokens * top_k, n_experts); }
-template <int ET, int T, int S, int UC, int EU>
+template <int ET, int UC>
 static void moe_up(const Launch &L, const Mx4Moe &a) {
-    hipLaunchKernelGGL((k_mx4_moe_up<ET, T, S, UC, EU>), dim3((a.ff + 16 * T - 1) / (16 * T), moe_hits(a.n_tokens, a.top_k, a.n_experts)), dim3(64 * kMoeUpWaves),
+    hipLaunchKernelGGL((k_mx4_moe_up<ET, UC>), dim3((a.ff + 15) / 16, moe_hits(a.n_tokens, a.top_k, a.n_experts)), dim3(64 * kMoeUpWaves),
                        (a.n_tokens * a.top_k * 2 + 15) & ~15u, L.stream, a);
 }
 template <int ET, int S, int UC>
@@ -1933,7 +1923,7 @@ static hipError_t moe_launch(const Launch &L, const Mx4Moe &a) {
     else if (P == 1 && a.hidden % 32 == 0 && a.ld_x % 8 == 0 && ((uintptr_t)a.x & 15) == 0)
         hipLaunchKernelGGL((k_mx4_moe_up_direct<8>), dim3((a.ff + 15) / 16, moe_hits(a.n_tokens, a.top_k, a.n_experts)), dim3(64 * kMoeUpWaves),
                            (a.n_tokens * a.top_k * 2 + 15) & ~15u, L.stream, a);
-    else moe_up<ET, 1, 3, P == 1 ? 8 : 4, 2>(L, a);
+    else moe_up<ET, P == 1 ? 8 : 4>(L, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     constexpr int NW = kMoeKept<ET> == 3 ? 8 : 12, UC = 4; // what LDS holds: their lines, and the values of UC tokens each
