@@ -61,8 +61,8 @@ __device__ __forceinline__ u32 mx4_block(const float (&v)[8], u32 &scale) {
 }
 
 // A wave takes sixteen blocks of a row, sixteen bytes of its scales: a lane eight values, four lanes a block, whose maximum is two exchanges between
-// neighbours, so that nothing goes through LDS and a value is read once. Memory bounds it: 4096 x 7168 bf16 17 us, 4.3 TB/s of 74 MB; behind the gate rule 2664 x 2048
-// f16 5 us; 16 x 2048 f32 2.4 us, a launch.
+// neighbours, so that nothing goes through LDS and a value is read once. Memory bounds it: 4096 x 7168 bf16 17 us, 4.3 TB/s of 74 MB; 16 x 2048 f32 2.4 us, a launch. Behind the gate rule
+// the vector units do, by the rule's exponential and its exact division: 4096 x 7168 bf16 38 us, 3.5 TB/s (f32 47 us, 5.3 TB/s), 2664 x 2048 f16 10.3, 666 x 2048 5.1.
 template <int ET, bool GLU>
 __global__ __launch_bounds__(256) void k_mx4_quantize(Mx4Rows a) {
     const u32 lane = threadIdx.x & 63, units = a.ks / 16, unit = group_index() * 4 + (threadIdx.x >> 6), row = unit / units;
@@ -955,8 +955,8 @@ hipError_t mx4_gemm(const Launch &L, const uint8_t *w, const uint8_t *ws, int n_
 // that add up to them: x in one of bf16, two of f16, three of f32; h, which is f32 by then, in two parts, 16 bits of mantissa, where y has 8 or 11 (one part of bf16 would leave h the largest
 // error of the step: 64 tokens of 7168 x 2048 0.0020 from 64 bits, in two 0.0016, which is y's own rounding; the step 245.6 and 250.5 us), in three where y is f32. (The instructions that take 4-bit codes would want x and h as codes too, or as 8-bit values, whose errors
 // a decode step would not have otherwise.)
-// On MI355X, us of each launch: 1 token, top 8 of 128, 2048 x 768 bf16 8.2 + 7.5; 16 tokens in f32 39 + 27 + 4.7 for 168 MB of some 66 hit experts' weights (a copy's rate: 32); 64 tokens, 41
-// of the 64 experts of 7168 x 2048 here hit, bf16, 153 (4.2 TB/s) + 97 (3.3 TB/s).
+// On MI355X, us of each launch: 1 token, top 8 of 128, 2048 x 768 bf16 8.4 + 7.6; 16 tokens in f32 40 + 28 + 4.9 for 168 MB of some 66 hit experts' weights (a copy's rate: 32); 64 tokens, 41
+// of the 64 experts of 7168 x 2048 here hit, bf16, 149 (4.3 TB/s) + 107 (3.0 TB/s), 44 of them hit, f16 210 + 111, f32 225 + 168.
 
 // What the first launch leaves for the second: the experts that are hit, ascending, and for each and each token the slot that picked it, the first if
 // there are several, kMoeNone for none, and its weight, the sum over all of the token's slots of it.
@@ -1263,7 +1263,7 @@ constexpr int kMoeUpWaves = 4;
 
 // h of rows of up to 2048 values, two lines a wave at most: a workgroup goes over several tiles of sixteen rows of gate and as many of up, whose lines come through
 // a ring of S stages without a stop between the tiles; the tokens' values of a wave's lines stay in LDS. UC tokens a workgroup (an expert with more has several): LDS holds two
-// workgroups a unit with 4 of bf16 and f16, 2 of f32, and experts of a decode batch mostly have fewer (16 tokens, top 8 of 128, f32: 39 us; without the products 31).
+// workgroups a unit with 4 of bf16 and f16, 2 of f32, and experts of a decode batch mostly have fewer (16 tokens, top 8 of 128, f32: 40 us; without the products 31).
 template <int ET, int S, int UC>
 __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(2))) void k_mx4_moe_up_short(Mx4Moe a, u32 per) {
     constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, kRow = P * kMoePart, kLoads = 6; // loads of a stage: four of lines, two of scales
@@ -1399,8 +1399,8 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
 
 // h. Sixteen rows of gate and as many of up, their lines dealt to the waves, each through three stages, of which two are on
 // their way while one is multiplied. A line's values of x come through LDS in parts, the next line's asked for in front of the weights: asked for in the matrix
-// instructions' form, each of sixteen requests a line would take the vector cache as long as a line of weights does. (64 tokens, 41 experts of 7168 x 2048 hit, bf16: 174 us, without
-// x 145; several tiles a workgroup instead of one 172.)
+// instructions' form, each of sixteen requests a line would take the vector cache as long as a line of weights does. (64 tokens, experts of 7168 x 2048: f32 225 us, f16 210 for 44 that are hit; bf16
+// 174 for 41, without x 145, several tiles a workgroup instead of one 172.)
 template <int ET, int UC>
 __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(2))) void k_mx4_moe_up(Mx4Moe a) {
     constexpr int NW = kMoeUpWaves, P = kMoeParts<ET>, kLoads = 6, kRow = P * kMoePart; // loads of a stage: four of lines, two of scales
@@ -1519,7 +1519,7 @@ __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_e
 // The same of bf16 rows that lie on 16 bytes and end with a block: their lines and all scales go into LDS as the weights do, two stages of each, and are multiplied as they are. A stage is
 // read to registers as a whole and asked for again before it is multiplied, so that values as well as weights are two lines on their way; no load hangs on a condition, since the compiler waits
 // by the loads that it can count (of a line's values ASKS loads, two tokens each). Piece p of token c lies at place p ^ c of its line, for the banks. 64 tokens, 41 experts of 7168 x 2048 hit:
-// 153 us, 4.2 TB/s (through registers, a line ahead: 174).
+// 149 to 153 us, 4.2 TB/s (through registers, a line ahead: 174).
 __device__ const uint4 moe_zeros[1] = {};
 template <int UC>
 __global__ __launch_bounds__(64 * kMoeUpWaves) __attribute__((amdgpu_waves_per_eu(2))) void k_mx4_moe_up_direct(Mx4Moe a) {
@@ -1652,7 +1652,7 @@ __device__ __forceinline__ void moe_onto(const Mx4Moe &a, u32 token, u32 row, fl
 // y. The lines of the experts that are hit, one expert's after another's, are dealt to the waves in stretches, each through two stages of 16 R rows; the
 // waves' sums, NT tiles of sixteen tokens, meet in LDS. A line's values of h come through LDS too, UC tokens' at a time and the next line's asked for in front of the
 // weights. The tokens of an expert stand side by side in a matrix instruction's columns, and their sums change to the tokens' own places when the expert's lines end: by
-// the tokens' places from the start a line would be multiplied for every tile of sixteen that has one of them (64 tokens, bf16: 113 us for 97). gridDim.y workgroups share the
+// the tokens' places from the start a line would be multiplied for every tile of sixteen that has one of them (64 tokens, bf16, h in one part: 113 us for 97; in two, 107). gridDim.y workgroups share the
 // lines: where they are several, a third launch adds their sums.
 template <int ET, int NW, int R, int UC, int NT>
 __global__ __launch_bounds__(64 * NW) void k_mx4_moe_down(Mx4Moe a) {
@@ -1913,8 +1913,8 @@ static hipError_t moe_down(const Launch &L, const Mx4Moe &a, u32 sharers) {
     hipLaunchKernelGGL((k_mx4_moe_join<ET>), dim3(((a.hidden + 3) / 4 * a.n_tokens + 255) / 256), dim3(256), 0, L.stream, a, sharers);
     return hipGetLastError();
 }
-// Up's lines stay with their values where a wave has two at most: 16 tokens in f32, rows of 2048, 46 us (a line at a time: 50), one token in bf16 8.2 (8.8). Down in 32 rows a workgroup where these fill the
-// card, alone or shared (16 tokens, 2048 rows, f32: four sharers 29 and 4.7 for their sums, of 16 rows a workgroup 33, unshared 42), else 16. The whole step of 64 tokens, 7168 rows, bf16: 250.5 with 12
+// Up's lines stay with their values where a wave has two at most: 16 tokens in f32, rows of 2048, 40 us (46 against 50 a line at a time before a token's parts were columns of one instruction), one token in
+// bf16 8.2 (8.8). Down in 32 rows a workgroup where these fill the card, alone or shared (16 tokens, 2048 rows, f32: four sharers 28 and 4.9 for their sums; when these took 29, of 16 rows a workgroup 33, unshared 42), else 16. The whole step of 64 tokens, 7168 rows, bf16: 250.5 with 12
 // waves, 272 with 14 that have the values of three tokens, 284 with 8; f16 302, 324, 336.
 template <int ET, int NT>
 static hipError_t moe_launch(const Launch &L, const Mx4Moe &a) {
